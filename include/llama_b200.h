@@ -567,6 +567,92 @@ B200_API int b200_op_attention_cached(const float* q, const float* k_cache, cons
 B200_API int b200_op_attention(const float* q, const float* k, const float* v, float* out, int n_heads, int n_kv_heads,
                       int seq_len, int head_dim, float scale);
 
+/* ---- operators on device tensors -----------------------------------------
+ * The per-op surface again for data that is on the device already: the pointers are device memory of GPU `device`, the work is queued
+ * on `stream` (a cudaStream_t of that GPU; NULL: its default stream) and the call returns without waiting for it, so that the calls can be
+ * captured into a CUDA graph.  The caller's current device stays as it is.  Nothing is allocated or kept; where a call needs a workspace the caller brings it, for itself alone
+ * until the work is done.  Arguments are checked on the host first (also without a GPU); indices that lie in device memory are checked by the kernels: a bad
+ * one is never followed, and sets a bit of *status (int32 on the device, added to with atomicOr, NULL: not wanted).
+ * Activations are f32, f16 or bf16 (B200_TYPE_*); distances between rows, tokens and heads are in elements, the last dimension is contiguous. */
+enum { B200_STATUS_BAD_SLOT = 1, B200_STATUS_BAD_POSITION = 2, B200_STATUS_BAD_PAGE = 4, B200_STATUS_BAD_LENGTH = 8 };
+/* RMS norm of a residual sum, with the result in 8 bits and one scale per row:
+ *   r = x + residual, rounded to the type, to `sum` (residual NULL: r = x, `sum` unused); y = r / sqrt(mean(r^2) + eps) * weight (f32);
+ *   scales[row] = max |y| / 127, q = round(y * (127 / max |y|)), halves to even.
+ * The squares are added in 64 bits; mean, root and reciprocal are taken there and rounded to f32 once.  Rows with max |y| < 2^-119 give zeros with scale 0, rows with
+ * max |y| = infinity or NaN give zeros with scale NaN.  `sum` may be `residual` or `x` with the same row distance; other overlaps are not
+ * allowed.  1 <= hidden <= 65536. */
+B200_API int b200_dev_add_rms_norm_q8(int device, void* stream, uint32_t type, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                                      void* sum, int64_t lds, const float* weight, float eps, int8_t* q, int64_t ldq, float* scales,
+                                      int64_t rows, int64_t hidden);
+/* Product of 8-bit integers: out[t][n] = a_scales[t] * w_scales[n] * sum_k a[t][k] w[n][k] (+ bias[n]); sums in s32 (exact: k <= 131071),
+ * then f32: ((float)sum * a_scale) * w_scale + bias, rounded to out_type.  a and w start on 16 bytes and their rows are a multiple of 16 bytes apart; what lies
+ * between k and the next row is not used. */
+B200_API int b200_dev_mat_mat_i8(int device, void* stream, uint32_t out_type, const int8_t* a, int64_t lda, const float* a_scales,
+                                 const int8_t* w, int64_t ldw, const float* w_scales, const float* bias /* may be NULL */, void* out, int64_t ldo,
+                                 int64_t t_rows, int64_t k, int64_t n);
+/* Paged cache in 4 bits.  A page holds page_size positions; per kv head one block of page_size * (head_dim + 8) bytes: page_size rows of
+ * head_dim / 2 bytes of keys, as many of values, page_size f32 key scales, page_size f32 value scales.  Byte i of a row has channel 2i in
+ * its low four bits and channel 2i + 1 in its high four; a value is scale * (n - 8).  Blocks follow one another: [page][kv head].
+ * Quantisation of a row: top = its value of the largest magnitude (the positive one of two), scale = top / -8, n = round(x * (1 / scale)) + 8,
+ * halves to even, cut at 15.  Rows with |top| < 2^-119 get scale 0, rows with an infinity or NaN scale NaN (what attends to them becomes NaN).
+ * head_dim 64 or 128; page_size a multiple of 16 up to 1024; data on 16 bytes. */
+typedef struct b200_q4_pages {
+    void* data;
+    int64_t n_pages;
+    int32_t page_size, n_kv_heads, head_dim;
+} b200_q4_pages;
+/* Rotation of queries and keys, and keys and values into the cache.  Token t's position selects row positions[t] of cos_sin ([table_rows][rot_dims]: rot_dims / 2
+ * cosines, then as many sines); the pairs are (i, i + rot_dims / 2) with use_neox, (2i, 2i + 1) without, the channels from rot_dims on stay:
+ * (a cos - b sin, b cos + a sin), every product and sum rounded to f32.  q_out receives the queries in the activations' type (it may be q itself; q NULL: no queries); keys and
+ * values are quantised from f32 and written to slot slots[t] (page * page_size + offset).  slots[t] < 0: the token is not cached (its query is
+ * rotated all the same).  A slot behind the last page: not cached, BAD_SLOT; a position outside the table: query rows of NaN, not cached, BAD_POSITION.
+ * With the same slot twice in one call the slot holds either token's parts. */
+typedef struct b200_q4_append {
+    int32_t device;
+    uint32_t type;
+    void* stream;
+    const void *q, *k, *v;
+    void* q_out;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, q_out_token, q_out_head;
+    const float* cos_sin;
+    int64_t table_rows;
+    const int32_t* positions;
+    const int64_t* slots;
+    int64_t tokens;
+    int32_t n_heads, rot_dims, use_neox;
+    b200_q4_pages cache;
+    int32_t* status;
+} b200_q4_append;
+B200_API int b200_dev_rope_append_q4(const b200_q4_append* a);
+/* Rows of the cache as the values they stand for: k_out, v_out [tokens][n_kv_heads][head_dim] contiguous, of `type`; slots < 0 (and, with BAD_SLOT, slots
+ * behind the last page) give zeros.  Either output may be NULL. */
+B200_API int b200_dev_read_q4(int device, void* stream, uint32_t type, const b200_q4_pages* cache, const int64_t* slots, int64_t tokens, void* k_out,
+                              void* v_out, int32_t* status);
+/* Attention over the paged cache: o = softmax(scale * q K^T) V, query head h reads kv head floor(h * n_kv_heads / n_heads).  Sequence s has kv_lens[s] cached positions,
+ * position p in page page_table[s * table_stride + p / page_size], and the query tokens q_starts[s] .. q_starts[s + 1] - 1 (NULL: token s), which are its last
+ * positions: token i of m sits at kv_lens[s] - m + i and sees the positions up to its own (window > 0: the last `window` of them).  A token that sees nothing gets zeros;
+ * tokens before q_starts[0] or from q_starts[seqs] on are left as they were.  Pages outside the cache count as not seen, BAD_PAGE; lengths beyond table_pages * page_size
+ * are cut there, and negative ones taken as zero, BAD_LENGTH; q_starts that do not ascend within 0 .. tokens: BAD_LENGTH, the sequence is left out.  max_q: the most query tokens
+ * of a sequence, as far as the host knows (0: not known); it only chooses between kernels.  workspace: b200_dev_attention_paged_q4_workspace bytes on 256 bytes. */
+typedef struct b200_q4_attention {
+    int32_t device;
+    uint32_t type;
+    void* stream;
+    const void* q;
+    void* out;
+    int64_t q_token, q_head, out_token, out_head;
+    const int32_t *q_starts, *kv_lens, *page_table;
+    int64_t table_stride, tokens;
+    int32_t table_pages, seqs, max_q, n_heads, window;
+    float scale;
+    b200_q4_pages cache;
+    int32_t* status;
+    void* workspace;
+    size_t workspace_bytes;
+} b200_q4_attention;
+B200_API int b200_dev_attention_paged_q4_workspace(const b200_q4_attention* a, size_t* bytes);
+B200_API int b200_dev_attention_paged_q4(const b200_q4_attention* a);
+
 #ifdef __cplusplus
 }
 #endif

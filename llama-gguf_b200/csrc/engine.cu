@@ -50,6 +50,7 @@
 #include "stream.cuh"
 #include "stream2.cuh"
 #include "layerprog.h"
+#include "device_ops.h"
 
 using namespace b200;
 
@@ -71,6 +72,8 @@ static int fail(int code, const std::string& msg) {
         if (e_ != cudaSuccess)                                                                         \
             return fail(B200_ERR_ALLOCATION_FAILED, std::string(#expr) + ": " + cudaGetErrorString(e_)); \
     } while (0)
+
+int dev_fail(int code, const char* msg) { return fail(code, msg); }
 
 extern "C" const char* b200_backend_name(void) { return "cuda-b200"; }
 extern "C" const char* b200_last_error(void) { return g_err.c_str(); }
