@@ -575,6 +575,8 @@ B200_API int b200_op_attention(const float* q, const float* k, const float* v, f
  * one is never followed, and sets a bit of *status (int32 on the device, added to with atomicOr, NULL: not wanted).
  * Activations are f32, f16 or bf16 (B200_TYPE_*); distances between rows, tokens and heads are in elements, the last dimension is contiguous. */
 enum { B200_STATUS_BAD_SLOT = 1, B200_STATUS_BAD_POSITION = 2, B200_STATUS_BAD_PAGE = 4, B200_STATUS_BAD_LENGTH = 8 };
+/* 0, or the code of the bounded wait inside one of these operators that gave up last (its results are then not valid); clears it.  Waits for the device's default stream. */
+B200_API int b200_dev_watchdog(int device, int* out);
 /* RMS norm of a residual sum, with the result in 8 bits and one scale per row:
  *   r = x + residual, rounded to the type, to `sum` (residual NULL: r = x, `sum` unused); y = r / sqrt(mean(r^2) + eps) * weight (f32);
  *   scales[row] = max |y| / 127, q = round(y * (127 / max |y|)), halves to even.

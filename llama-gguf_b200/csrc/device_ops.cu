@@ -2,6 +2,7 @@
 // the call, and the choice among types.  Nothing is allocated here and nothing waits for the device.
 #include "device_ops.h"
 
+#include <algorithm>
 #include <exception>
 #include <string>
 
@@ -65,6 +66,19 @@ int check_pages(const char* op, const b200_q4_pages& c) {
 
 }  // namespace
 
+extern "C" int b200_dev_watchdog(int device, int* out) {
+    const char* op = "watchdog";
+    return entry(op, [&]() -> int {
+        if (!out) return bad(op, "null pointer");
+        return on_device(op, device, [&] {
+            const int zero = 0;
+            cudaError_t e = cudaMemcpyFromSymbol(out, dev_watchdog, sizeof(int));
+            if (e == cudaSuccess && *out) e = cudaMemcpyToSymbol(dev_watchdog, &zero, sizeof(int));
+            return e;
+        });
+    });
+}
+
 extern "C" int b200_dev_add_rms_norm_q8(int device, void* stream, uint32_t type, const void* x, int64_t ldx, const void* residual, int64_t ldr, void* sum, int64_t lds,
                                         const float* weight, float eps, int8_t* q, int64_t ldq, float* scales, int64_t rows, int64_t hidden) {
     const char* op = "add_rms_norm_q8";
@@ -92,8 +106,8 @@ extern "C" int b200_dev_mat_mat_i8(int device, void* stream, uint32_t out_type, 
         if (t_rows == 0) return B200_OK;
         if (!a || !a_scales || !w || !w_scales || !out) return bad(op, "null pointer");
         if (off16(a) || off16(w) || lda % 16 || ldw % 16) return bad(op, "a and w must start on 16 bytes, with rows a multiple of 16 bytes apart");
-        GemmI8Args g{a, w, a_scales, w_scales, bias, out, lda, ldw, ldo, (int)t_rows, (int)k, (int)n};
-        return on_device(op, device, [&] { return by_type(out_type, [&](auto t) { return gemm_i8<decltype(t)>(g, (cudaStream_t)stream); }); });
+        const GemmI8Args g{a_scales, w_scales, bias, out, ldo, (int)t_rows, (int)k, (int)n, 1};
+        return on_device(op, device, [&] { return by_type(out_type, [&](auto t) { return gemm_i8<decltype(t)>(a, lda, w, ldw, g, (cudaStream_t)stream); }); });
     });
 }
 

@@ -53,6 +53,7 @@ def _lib():
     if _library is None:
         L = lib()
         i64, vp, sp = C.c_int64, C.c_void_p, C.POINTER(C.c_size_t)
+        L.b200_dev_watchdog.argtypes = [C.c_int, C.POINTER(C.c_int)]
         L.b200_dev_add_rms_norm_q8.argtypes = [C.c_int, vp, C.c_uint32, vp, i64, vp, i64, vp, i64, vp, C.c_float, vp, i64, vp, i64, i64]
         L.b200_dev_mat_mat_i8.argtypes = [C.c_int, vp, C.c_uint32, vp, i64, vp, vp, i64, vp, vp, vp, i64, i64, i64, i64]
         L.b200_dev_rope_append_q4.argtypes = [C.POINTER(Q4Append)]
@@ -128,6 +129,13 @@ def _ld(t):
 
 def _stream(device):
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def watchdog(device=0):
+    """0, or the code of the bounded wait inside one of these operators that gave up last on this device (its results are then not valid); clears it."""
+    v = C.c_int(0)
+    _check(_lib().b200_dev_watchdog(int(device), C.byref(v)))
+    return v.value
 
 
 def padded_rows(rows, cols, device, dtype=torch.int8):

@@ -14,7 +14,9 @@ TYPES = [torch.float32, torch.float16, torch.bfloat16]
 def D(b200):
     from llama_gguf_b200 import device_ops
 
-    return device_ops
+    yield device_ops
+    torch.cuda.synchronize()
+    assert device_ops.watchdog() == 0      # (no bounded wait gave up)
 
 
 def normal(seed, *shape):
