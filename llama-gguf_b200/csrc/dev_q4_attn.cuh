@@ -1,65 +1,530 @@
 // dev_q4_attn.cuh — attention over the paged 4-bit cache (b200_dev_attention_paged_q4).
+//
+// One pass over the keys with a running maximum: o = sum_j p_j d_j (n_j - 8) / sum_j p_j, p_j = 2^(z_j - m), z_j = log2(e) scale k_j q . (n_j - 8), k_j and d_j the scales of key and value j.
+//
+// Work.  An item is eight query rows of one sequence and kv head (row = token * G + head, G query heads per kv head) with the keys they see, in tiles of 16 W positions (W warps).  All items'
+// tiles lie on one line, sequence after sequence, and every block takes an equal stretch of it, so that a long sequence among short ones, or alone, keeps every SM busy; lengths are read on
+// the device only.  A stretch that ends inside an item leaves its sums in the workspace, and the second kernel joins them.
+//
+// A warp takes 16 positions at a time (never more than one page) through a ring in shared memory (cp.async, 16 bytes per lane) and multiplies with mma.m16n8k16 (fp16, f32 sums):
+//   scores  a nibble in the low bits of an fp16 is the number n 2^-24 exactly (four bits further up: 16 n 2^-24, and that channel's query element is divided by 16): one shift
+//           and four ands turn eight nibbles into operands.  - 8 sum q is taken off afterwards in f32.
+//   values  1024 + n is n in the low bits of the fp16 1024; minus 1032 it is n - 8.  (Sums of n alone would grow with the keys while the result does not: the f32 sums lost 1e-4 of it.)
+// The sixteen rows of the instruction are eight query rows twice: rows 0-7 multiply with the fp16 of a query element (or weight), rows 8-15 with what that left over, so that f32 results keep
+// 22 bits.  The 16-bit types get it for nothing.
+// The weight of a value is p_j d_j.  Its reference is not m but the largest z_j + floor(log2 |d_j|) so far: p_j d_j stays in fp16's range whatever the values' scales are.  Both references move only when
+// something passes them by 2^8, so the usual step has no exchange between lanes.
+// What bounds it: the bytes of the cache, 2 (hd / 2 + 4) per position and kv head.
 #pragma once
-#include "dev_common.cuh"
+#include "dev_umma.cuh"
 
 namespace dev {
 
-template <typename T, int HD> __global__ void __launch_bounds__(128) attention_q4_plain_kernel(const b200_q4_attention a) {
-    constexpr int E = HD / 32;
-    const int64_t item = (int64_t)blockIdx.x * 4 + threadIdx.x / 32, s = item / a.n_heads;
-    const int h = (int)(item - s * a.n_heads), lane = threadIdx.x & 31, kv = h / (a.n_heads / a.cache.n_kv_heads), page_size = a.cache.page_size;
-    if (s >= a.seqs) return;
-    const int64_t first = a.q_starts ? a.q_starts[s] : s, end = a.q_starts ? a.q_starts[s + 1] : s + 1, count = end - first;
-    const int64_t cap = (int64_t)a.table_pages * page_size;
-    int64_t len = a.kv_lens[s];
-    if (len < 0 || len > cap || first < 0 || count < 0 || end > a.tokens) {
-        if (a.status && lane == 0) atomicOr(a.status, (int)B200_STATUS_BAD_LENGTH);
-        len = len < 0 ? 0 : len > cap ? cap : len;
-        if (first < 0 || count < 0 || end > a.tokens) return;
-    }
-    for (int64_t t = first + blockIdx.y; t < end; t += gridDim.y) {
-    const int64_t pos = len - count + (t - first), begin = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
-    float q[E], o[E], m = -INFINITY, l = 0.0f;
+enum { QA_ROWS = 8, QA_STAGES = 4 };
+
+struct Q4Seq {
+    int first, count;      // query tokens
+    int64_t len;           // cached positions
+};
+__device__ __forceinline__ Q4Seq q4_seq(const b200_q4_attention& a, int s, bool report) {
+    Q4Seq q;
+    const int64_t b = a.q_starts ? a.q_starts[s] : s, e = a.q_starts ? a.q_starts[s + 1] : s + 1, cap = (int64_t)a.table_pages * a.cache.page_size;
+    q.len = a.kv_lens[s];
+    const bool wrong = b < 0 || e < b || e > a.tokens;
+    if (report && a.status && (wrong || q.len < 0 || q.len > cap)) atomicOr(a.status, (int)B200_STATUS_BAD_LENGTH);
+    q.len = q.len < 0 ? 0 : q.len > cap ? cap : q.len;
+    q.first = wrong ? 0 : (int)b;
+    q.count = wrong ? 0 : (int)(e - b);
+    return q;
+}
+// positions [base, hi) that the rows of block rb see, in `tiles` tiles; rows that see nothing have one tile all the same (it writes their zeros)
+struct Q4Span {
+    int base, hi, tiles;
+};
+template <int TILE> __device__ __forceinline__ Q4Span q4_span(const b200_q4_attention& a, const Q4Seq& q, int G, int rb) {
+    const int last = (min(rb * QA_ROWS + QA_ROWS, q.count * G) - 1) / G, first = rb * QA_ROWS / G;
+    const int64_t at = q.len - q.count;
+    Q4Span s;
+    s.hi = (int)max((int64_t)0, at + last + 1);
+    s.base = a.window > 0 ? (int)max((int64_t)0, at + first + 1 - a.window) / TILE * TILE : 0;
+    s.tiles = max(1, (s.hi - s.base + TILE - 1) / TILE);
+    return s;
+}
+
+// the workspace: per block, two parts of [8][HD] sums, [8][4] (m, reference of the sums, l, -); then per block what its first stretch ends
+struct Q4End {
+    int first_cta, first_slot, seq, rb, head, ends;
+};
+template <int HD> __host__ __device__ constexpr int q4_part_floats() { return QA_ROWS * (HD + 4); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_h2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+__device__ __forceinline__ uint32_t sub_h2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+template <int N> __device__ __forceinline__ void lds(uint32_t (&v)[N], uint32_t at) {
+    if constexpr (N == 4) asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+    else if constexpr (N == 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(at) : "memory");
+    else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(at) : "memory");
+}
+
+// a stage of a warp's ring: 16 key rows as they are, 16 value rows in 16-byte pieces, 16 + 16 scales.  Piece q of value row r is at q4_piece(r, q): the words that a step reads together (rows of one
+// parity and half, neighbouring words) are in different banks.
+template <int HD> struct Q4Stage {
+    static constexpr int ROW = HD / 2, V = 16 * ROW, KS = 32 * ROW, VS = KS + 64, BYTES = KS + 128;
+};
+__device__ __forceinline__ int q4_piece(int row, int q) { return (((row & 1) | ((row >> 3) & 1) << 1 | (q >> 1) << 2) << 3) | (q & 1) | ((row >> 1) & 3) << 1; }
+
+template <typename T, int HD, int W> struct Q4Smem {
+    static constexpr int TILE = 16 * W, RING = W * QA_STAGES * Q4Stage<HD>::BYTES, MERGE = W * QA_ROWS * (HD + 4) * 4 + W * QA_ROWS * 16, BYTES = RING + MERGE;
+};
+
+template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 16 / W) attention_q4_kernel(const b200_q4_attention a, uint64_t page16) {
+    using St = Q4Stage<HD>;
+    using Sm = Q4Smem<T, HD, W>;
+    constexpr int TILE = Sm::TILE, WORDS = HD / 32, NT = HD / 8;      // words of a key row per lane; column tiles of the values
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ long long s_sum[W];
+    __shared__ int s_item[4];      // sequence, row block, head, tile
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    const int nkv = a.cache.n_kv_heads, G = a.n_heads / nkv, page_size = a.cache.page_size;
+
+    // ---- the line of all tiles, and where this block's stretch begins
+    const int chunk = (a.seqs + 32 * W - 1) / (32 * W), s_beg = min(a.seqs, tid * chunk), s_end = min(a.seqs, s_beg + chunk);
+    auto tiles_of = [&](const Q4Seq& q) {
+        long long n = 0;
+        for (int rb = 0; rb * QA_ROWS < q.count * G; rb++) n += q4_span<TILE>(a, q, G, rb).tiles;
+        return n * nkv;
+    };
+    long long mine = 0;
+    for (int s = s_beg; s < s_end; s++) mine += tiles_of(q4_seq(a, s, blockIdx.x == 0));
+    long long before = mine;
 #pragma unroll
-    for (int i = 0; i < E; i++) {
-        q[i] = to_f(reinterpret_cast<const T*>(a.q)[t * a.q_token + h * a.q_head + lane * E + i]) * a.scale * 1.44269504f;
-        o[i] = 0.0f;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
     }
-    for (int64_t j = begin; j <= pos; j++) {
-        const int64_t page = a.page_table[s * a.table_stride + j / page_size];
-        if (page < 0 || page >= a.cache.n_pages) {
-            if (a.status && lane == 0) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
-            continue;
+    if (lane == 31) s_sum[warp] = before;
+    __syncthreads();
+    long long total = 0;
+    before -= mine;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        if (w < warp) before += s_sum[w];
+        total += s_sum[w];
+    }
+    const long long grid = min((long long)gridDim.x, total);      // (every block up to `grid` has a tile)
+    Q4End* ends = reinterpret_cast<Q4End*>(reinterpret_cast<float*>(a.workspace) + (size_t)gridDim.x * 2 * q4_part_floats<HD>()) + blockIdx.x;
+    if (blockIdx.x >= grid) {      // (the whole block)
+        if (tid == 0) ends->ends = 0;
+        return;
+    }
+    const long long c0 = total * blockIdx.x / grid, c1 = total * (blockIdx.x + 1) / grid;
+    if (before <= c0 && c0 < before + mine) {
+        long long at = c0 - before;
+        for (int s = s_beg; s < s_end; s++) {
+            const Q4Seq q = q4_seq(a, s, false);
+            const long long n = tiles_of(q);
+            if (at >= n) { at -= n; continue; }
+            for (int rb = 0;; rb++) {
+                const int per = q4_span<TILE>(a, q, G, rb).tiles;
+                if (at >= (long long)per * nkv) { at -= (long long)per * nkv; continue; }
+                s_item[0] = s;
+                s_item[1] = rb;
+                s_item[2] = (int)(at / per);
+                s_item[3] = (int)(at % per);
+                break;
+            }
+            break;
         }
-        const Q4Block b = q4_block(a.cache, page, kv);
-        const int at = (int)(j % page_size);
-        float z = 0.0f;
-        float vv[E];
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-            const int c = lane * E + i;
-            z += q[i] * (float)(((b.k[at * (HD / 2) + c / 2] >> (4 * (c & 1))) & 15) - 8);
-            vv[i] = (float)(((b.v[at * (HD / 2) + c / 2] >> (4 * (c & 1))) & 15) - 8) * b.vs[at];
-        }
-#pragma unroll
-        for (int d = 16; d; d >>= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
-        z *= b.ks[at];
-        const float top = fmaxf(m, z), f = m == top ? 1.0f : exp2f(m - top), p = z == top ? 1.0f : exp2f(z - top);
-        l = l * f + p;
-#pragma unroll
-        for (int i = 0; i < E; i++) o[i] = o[i] * f + p * vv[i];
-        m = top;
     }
+    __syncthreads();
+    int s = s_item[0], rb = s_item[1], h = s_item[2], tile = s_item[3];
+
+    const uint32_t ring = sm_u32(smem) + warp * QA_STAGES * St::BYTES;
+    float* merge = reinterpret_cast<float*>(smem + Sm::RING);             // [W][8][HD + 4]
+    float* stat = merge + W * QA_ROWS * (HD + 4);                         // [W][8][4]
+    Q4Seq q = q4_seq(a, s, false);
+    for (long long cur = c0; cur < c1;) {
+        const Q4Span sp = q4_span<TILE>(a, q, G, rb);
+        const int stop = (int)min((long long)sp.tiles, tile + (c1 - cur));
+
+        // ---- this lane's row: its query, its keys
+        const int r = rb * QA_ROWS + g, token = r / G;
+        const bool live = r < q.count * G;
+        const int64_t pos = q.len - q.count + token;
+        // (rows behind the last one compute along with the first: nothing of theirs is written)
+        const int row_hi = live ? (int)max((int64_t)0, pos + 1) : INT32_MAX, row_lo = live && a.window > 0 ? (int)max((int64_t)0, pos + 1 - a.window) : 0;
+        uint32_t qa[WORDS][2][4];
+        float alpha, q8;
+        {
+            float x[HD / 4];
+            const T* p = reinterpret_cast<const T*>(a.q) + (q.first + (live ? token : 0)) * a.q_token + (h * G + (live ? r - token * G : 0)) * a.q_head + c * (HD / 4);
+            if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) load_n<T, HD / 4, true>(p, x);
+            else load_n<T, HD / 4, false>(p, x);
+            float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < E; i++) reinterpret_cast<T*>(a.out)[t * a.out_token + h * a.out_head + lane * E + i] = from_f<T>(l == 0.0f ? 0.0f : o[i] / l);
+            for (int i = 0; i < HD / 4; i++) top = fmaxf(top, fabsf(x[i]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // elements times 2^e are below 2^14: fp16 holds the fp16 of them and what that leaves over
+            const int e = top > 0.0f && top < INFINITY ? 13 - ilogbf(top) : 0;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HD / 4; i++) x[i] = ldexpf(x[i], e);
+            auto part = [&](float u, float v, float f, uint32_t& hi, uint32_t& lo) {
+                hi = pack_h2(u * f, v * f);
+                const float2 b = unpack_h2(hi);
+                lo = pack_h2(u * f - b.x, v * f - b.y);
+                const float2 d = unpack_h2(lo);
+                sum += ((b.x + d.x) + (b.y + d.y)) / f;
+            };
+#pragma unroll
+            for (int j = 0; j < WORDS; j++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    part(x[8 * j + 2 * u], x[8 * j + 2 * u + 4], 1.0f, qa[j][u][0], qa[j][u][1]);
+                    part(x[8 * j + 2 * u + 1], x[8 * j + 2 * u + 5], 0.0625f, qa[j][u][2], qa[j][u][3]);
+                }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            q8 = sum * (8.0f / 16384.0f);                                  // in units of 2^-10: (sums of n 2^-24) * 2^10
+            alpha = ldexpf(a.scale * 1.4426950408889634f, 14 - e);
+        }
+        float m = -INFINITY, mv = -INFINITY, l = 0.0f, acc[NT][4];
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) acc[i][k] = 0.0f;
+
+        // ---- the ring: stage i holds step tile + i
+        const int64_t table = (int64_t)s * a.table_stride;
+        auto fetch = [&](int step, int stage) {
+            const int p0 = sp.base + step * TILE + warp * 16;
+            if (step < stop && p0 < sp.hi) {
+                const int p16 = p0 >> 4, index = (int)(((uint64_t)p16 * page16) >> 36);
+                int64_t page = a.page_table[table + index];
+                page = page >= 0 && page < a.cache.n_pages ? page : 0;      // (masked below)
+                const int row = p0 - index * page_size;
+                const Q4Block b = q4_block(a.cache, page, h);
+                const uint32_t at = ring + stage * St::BYTES;
+                constexpr int P = St::ROW / 16;                             // pieces of a row
+#pragma unroll
+                for (int i = 0; i < 16 * P; i += 32) {
+                    const int n = i + lane;
+                    if (16 * P >= 32 || n < 16 * P) {
+                        cp16(at + n * 16, b.k + row * St::ROW + n * 16);
+                        cp16(at + St::V + q4_piece(n / P, n % P) * 16, b.v + row * St::ROW + n * 16);
+                    }
+                }
+                if (lane < 4) cp16(at + St::KS + lane * 16, b.ks + row + lane * 4);
+                else if (lane < 8) cp16(at + St::VS + (lane - 4) * 16, b.vs + row + (lane - 4) * 4);
+            }
+            cp_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < QA_STAGES - 1; i++) fetch(tile + i, i);
+        int stage = 0;
+        for (int step = tile; step < stop; step++) {
+            cp_wait<QA_STAGES - 2>();
+            __syncwarp();
+            fetch(step + QA_STAGES - 1, stage == 0 ? QA_STAGES - 1 : stage - 1);
+            const uint32_t at = ring + stage * St::BYTES;
+            stage = stage == QA_STAGES - 1 ? 0 : stage + 1;
+            const int p0 = sp.base + step * TILE + warp * 16;
+            if (p0 >= sp.hi) continue;
+            // scores of positions p0 + 8 u + 2 c, + 1
+            float z[2][2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                uint32_t w[WORDS];
+                lds<WORDS>(w, at + (8 * u + g) * St::ROW + c * (WORDS * 4));
+                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < WORDS; j++) {
+                    mma16(d, qa[j][0][0], qa[j][0][1], qa[j][0][2], qa[j][0][3], w[j] & 0x000f000fu, w[j] & 0x00f000f0u);
+                    const uint32_t x = w[j] >> 8;
+                    mma16(d, qa[j][1][0], qa[j][1][1], qa[j][1][2], qa[j][1][3], x & 0x000f000fu, x & 0x00f000f0u);
+                }
+                uint32_t ks[2];
+                lds<2>(ks, at + St::KS + (8 * u + 2 * c) * 4);
+#pragma unroll
+                for (int k = 0; k < 2; k++) z[u][k] = (fmaf(d[k] + d[k + 2], 1024.0f, -q8) * alpha) * __uint_as_float(ks[k]);
+            }
+            uint32_t ok = 0xfu;
+            const int index = (int)(((uint64_t)(p0 >> 4) * page16) >> 36);
+            const int64_t page = a.page_table[table + index];
+            const bool there = page >= 0 && page < a.cache.n_pages;
+            if (!there && a.status && lane == 0) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
+            if (!there || !__all_sync(0xffffffffu, p0 >= row_lo && p0 + 16 <= row_hi)) {
+                ok = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int j = p0 + 8 * (i >> 1) + 2 * c + (i & 1);
+                    if (there && j >= row_lo && j < row_hi) ok |= 1u << i;
+                    else z[i >> 1][i & 1] = -INFINITY;
+                }
+            }
+            // the values' scales as 2^E * mant
+            float y[2][2], mant[2][2];
+            bool past = false;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                uint32_t vs[2];
+                lds<2>(vs, at + St::VS + (8 * u + 2 * c) * 4);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const uint32_t ex = (vs[k] >> 23) & 255u;
+                    y[u][k] = z[u][k] + (__uint_as_float(0x4b000000u + ex) - 8388735.0f);      // + (ex - 127)
+                    mant[u][k] = ex == 0 ? 0.0f : ex == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float((vs[k] & 0x807fffffu) | 0x3f800000u);
+                    past |= z[u][k] > m + 8.0f || y[u][k] > mv + 8.0f;
+                }
+            }
+            if (__any_sync(0xffffffffu, past)) {
+                float top = fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[1][0], z[1][1])), topv = fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[1][0], y[1][1]));
+#pragma unroll
+                for (int o = 1; o <= 2; o <<= 1) {
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, o));
+                }
+                top = fmaxf(top, m);
+                topv = fmaxf(topv, mv);
+                l *= top == m ? 1.0f : ex2(m - top);
+                const float f = topv == mv ? 1.0f : ex2(mv - topv);
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) acc[i][k] *= f;
+                m = top;
+                mv = topv;
+            }
+            uint32_t pa[2][2];      // [positions' half][fp16, what it leaves over]
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                float w[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const bool in = (ok >> (2 * u + k)) & 1u;
+                    l += in ? ex2(z[u][k] - m) : 0.0f;
+                    w[k] = in ? ex2(y[u][k] - mv) * mant[u][k] : 0.0f;
+                }
+                pa[u][0] = pack_h2(w[0], w[1]);
+                const float2 b = unpack_h2(pa[u][0]);
+                pa[u][1] = pack_h2(w[0] - b.x, w[1] - b.y);
+            }
+            // values: column n of tile i is channel 8 n + i (and 64 more from tile 8 on)
+#pragma unroll
+            for (int half = 0; half < NT / 8; half++) {
+                uint32_t t[2][2];      // [positions' half][channels 0-3, 4-7 of the word]
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    uint32_t w0[1], w1[1];
+                    const int piece = 2 * half + (g >> 2);
+                    lds<1>(w0, at + St::V + q4_piece(8 * u + 2 * c, piece) * 16 + (g & 3) * 4);
+                    lds<1>(w1, at + St::V + q4_piece(8 * u + 2 * c + 1, piece) * 16 + (g & 3) * 4);
+                    t[u][0] = __byte_perm(w0[0], w1[0], 0x5410);
+                    t[u][1] = __byte_perm(w0[0], w1[0], 0x7632);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const bool odd = i & 1;      // 16 (n - 8): the result is divided by 16 at the end
+                    uint32_t b[2];
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const uint32_t v = (i & 2) ? t[u][i >> 2] >> 8 : t[u][i >> 2];
+                        b[u] = sub_h2((v & (odd ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u, odd ? 0x64806480u : 0x64086408u);
+                    }
+                    mma16(acc[8 * half + i], pa[0][0], pa[0][1], pa[1][0], pa[1][1], b[0], b[1]);
+                }
+            }
+        }
+        cp_wait<0>();
+
+        // ---- the warps' sums into one
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (c == 0) *reinterpret_cast<float4*>(stat + (warp * QA_ROWS + g) * 4) = make_float4(m, mv, l, 0.0f);
+        float* mine_out = merge + (warp * QA_ROWS + g) * (HD + 4);
+#pragma unroll
+        for (int half = 0; half < NT / 8; half++)
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) mine_out[64 * half + 8 * (2 * c + k) + i] = (acc[8 * half + i][k] + acc[8 * half + i][k + 2]) * ((i & 1) ? 0.0625f : 1.0f);
+        __syncthreads();
+        const bool whole = tile == 0 && stop == sp.tiles, first = cur == c0;
+        float* part = reinterpret_cast<float*>(a.workspace) + ((size_t)blockIdx.x * 2 + (first ? 0 : 1)) * q4_part_floats<HD>();
+        for (int i = tid; i < QA_ROWS * (HD / 4); i += 32 * W) {
+            const int row = i / (HD / 4), ch = (i % (HD / 4)) * 4;
+            float top = -INFINITY, topv = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                top = fmaxf(top, stat[(w * QA_ROWS + row) * 4]);
+                topv = fmaxf(topv, stat[(w * QA_ROWS + row) * 4 + 1]);
+            }
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                const float4 st = *reinterpret_cast<const float4*>(stat + (w * QA_ROWS + row) * 4), v = *reinterpret_cast<const float4*>(merge + (w * QA_ROWS + row) * (HD + 4) + ch);
+                sum += st.z * (st.x == top ? 1.0f : ex2(st.x - top));
+                const float f = st.y == topv ? 1.0f : ex2(st.y - topv);
+                o.x += v.x * f;
+                o.y += v.y * f;
+                o.z += v.z * f;
+                o.w += v.w * f;
+            }
+            if (whole) {
+                const int rr = rb * QA_ROWS + row;
+                if (rr < q.count * G) {
+                    // (l = 0: the row saw nothing, and the sums are zeros)
+                    const float f = sum == 0.0f ? 0.0f : 1.0f / sum, e = topv == -INFINITY ? 0.0f : topv - top;
+                    const float v[4] = {o.x, o.y, o.z, o.w};
+                    T* p = reinterpret_cast<T*>(a.out) + (q.first + rr / G) * a.out_token + (h * G + rr % G) * a.out_head + ch;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) p[k] = from_f<T>(sum == 0.0f ? 0.0f : ldexpf(v[k] * f, (int)floorf(e)) * ex2(e - floorf(e)));
+                }
+            } else {
+                *reinterpret_cast<float4*>(part + row * HD + ch) = o;
+                if (ch == 0) *reinterpret_cast<float4*>(part + QA_ROWS * HD + row * 4) = make_float4(top, topv, sum, 0.0f);
+            }
+        }
+        if (first && tid == 0) {
+            const long long start = cur - tile;
+            Q4End e{};
+            if (tile > 0 && stop == sp.tiles) {
+                e.first_cta = (int)(((start + 1) * grid - 1) / total);
+                e.first_slot = total * e.first_cta / grid < start;
+                e.seq = s;
+                e.rb = rb;
+                e.head = h;
+                e.ends = 1;
+            }
+            *ends = e;
+        }
+        __syncthreads();
+        // ---- on to the next item
+        cur += stop - tile;
+        tile = 0;
+        if (cur < c1 && ++h == nkv) {
+            h = 0;
+            rb++;
+            while (rb * QA_ROWS >= q.count * G) {      // (there is one: cur < total)
+                rb = 0;
+                q = q4_seq(a, ++s, false);
+            }
+        }
     }
 }
 
-template <typename T, int HD> cudaError_t attention_q4(const b200_q4_attention& a, cudaStream_t st) {
-    const int64_t items = (int64_t)a.seqs * a.n_heads;
-    attention_q4_plain_kernel<T, HD><<<dim3((unsigned)((items + 3) / 4), (unsigned)(a.tokens > a.seqs ? 256 : 1)), 128, 0, st>>>(a);
-    return cudaGetLastError();
+// Joins the parts of the items that ended in a block's first stretch: block (x, y) = that block, a row.
+template <typename T, int HD> __global__ void __launch_bounds__(128) attention_q4_join_kernel(const b200_q4_attention a, int grid) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr int LANES = HD / 4, GROUPS = 128 / LANES, PART = q4_part_floats<HD>();
+    __shared__ float s_red[3][4];
+    __shared__ __align__(16) float s_o[GROUPS][HD];
+    const float* ws = reinterpret_cast<const float*>(a.workspace);
+    const Q4End e = reinterpret_cast<const Q4End*>(ws + (size_t)grid * 2 * PART)[blockIdx.x];
+    if (!e.ends) return;
+    const int row = blockIdx.y, tid = threadIdx.x, n = (int)blockIdx.x - e.first_cta + 1, G = a.n_heads / a.cache.n_kv_heads, rr = e.rb * QA_ROWS + row;
+    const Q4Seq q = q4_seq(a, e.seq, false);
+    if (rr >= q.count * G) return;
+    auto part = [&](int i) { return ws + ((size_t)(e.first_cta + i) * 2 + (i == 0 ? e.first_slot : 0)) * PART; };
+    float top = -INFINITY, topv = -INFINITY, sum = 0.0f;
+    for (int i = tid; i < n; i += 128) {
+        const float* st = part(i) + QA_ROWS * HD + row * 4;
+        top = fmaxf(top, st[0]);
+        topv = fmaxf(topv, st[1]);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, o));
+    }
+    if ((tid & 31) == 0) {
+        s_red[0][tid >> 5] = top;
+        s_red[1][tid >> 5] = topv;
+    }
+    __syncthreads();
+    top = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+    topv = fmaxf(fmaxf(s_red[1][0], s_red[1][1]), fmaxf(s_red[1][2], s_red[1][3]));
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = tid / LANES; i < n; i += GROUPS) {
+        const float4 st = *reinterpret_cast<const float4*>(part(i) + QA_ROWS * HD + row * 4), v = *reinterpret_cast<const float4*>(part(i) + row * HD + (tid % LANES) * 4);
+        sum += st.z * (st.x == top ? 1.0f : ex2(st.x - top));
+        const float f = st.y == topv ? 1.0f : ex2(st.y - topv);
+        o.x += v.x * f;
+        o.y += v.y * f;
+        o.z += v.z * f;
+        o.w += v.w * f;
+    }
+    *reinterpret_cast<float4*>(&s_o[tid / LANES][(tid % LANES) * 4]) = o;
+    __shared__ float s_l[GROUPS];
+    if (tid % LANES == 0) s_l[tid / LANES] = sum;
+    __syncthreads();
+    if (tid < HD) {
+        float v = 0.0f, l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < GROUPS; k++) {
+            v += s_o[k][tid];
+            l += s_l[k];
+        }
+        const float x = topv == -INFINITY ? 0.0f : topv - top;
+        reinterpret_cast<T*>(a.out)[(q.first + rr / G) * a.out_token + (e.head * G + rr % G) * a.out_head + tid] =
+            from_f<T>(l == 0.0f ? 0.0f : ldexpf(v * (1.0f / l), (int)floorf(x)) * ex2(x - floorf(x)));
+    }
 }
-inline size_t attention_q4_workspace(const b200_q4_attention&) { return 0; }
+
+// ------------------------------------------------------------------------------------------------------------------- host
+constexpr int QA_W = 4;      // warps of a block
+// blocks of the first kernel: as many as run at once on 148 SMs, fewer where even one tile each could not be found
+inline int attention_q4_grid(const b200_q4_attention& a) {
+    const int64_t G = a.n_heads / a.cache.n_kv_heads, blocks = (a.tokens * G + QA_ROWS - 1) / QA_ROWS + a.seqs;
+    const int64_t tiles = blocks * a.cache.n_kv_heads * (((int64_t)a.table_pages * a.cache.page_size + 16 * QA_W - 1) / (16 * QA_W) + 1);
+    return (int)std::min<int64_t>(148 * (16 / QA_W), tiles);
+}
+inline size_t attention_q4_workspace(const b200_q4_attention& a) {
+    const size_t grid = (size_t)attention_q4_grid(a), part = QA_ROWS * (a.cache.head_dim + 4) * 4;
+    return grid * (2 * part + sizeof(Q4End));
+}
+template <typename T, int HD> cudaError_t attention_q4(const b200_q4_attention& a, cudaStream_t st) {
+    using Sm = Q4Smem<T, HD, QA_W>;
+    static SmemAllowed allowed;
+    const auto kernel = attention_q4_kernel<T, HD, QA_W>;
+    cudaError_t e = allowed((const void*)kernel, Sm::BYTES);
+    if (e != cudaSuccess) return e;
+    const uint64_t d = (uint64_t)a.cache.page_size / 16, page16 = (((uint64_t)1 << 36) + d - 1) / d;      // n / d = n * page16 >> 36 for n < 2^27
+    const int grid = attention_q4_grid(a);
+    e = launch(kernel, dim3(grid), dim3(32 * QA_W), Sm::BYTES, 1, st, a, page16);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid, QA_ROWS);
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attention_q4_join_kernel<T, HD>, a, grid);
+}
 
 }  // namespace dev
