@@ -6,16 +6,19 @@
 // tiles lie on one line, sequence after sequence, and every block takes an equal stretch of it, so that a long sequence among short ones, or alone, keeps every SM busy; lengths are read on
 // the device only.  A stretch that ends inside an item leaves its sums in the workspace, and the second kernel joins them.
 //
-// A warp takes 16 positions at a time (never more than one page) through a ring in shared memory (cp.async, 16 bytes per lane) and multiplies with mma.m16n8k16 (fp16, f32 sums):
+// A warp takes 16 positions at a time (never more than one page) through a ring in shared memory (cp.async, 16 bytes per lane) and multiplies with mma.m16n8k16 (fp16, f32 sums), the
+// positions (scores) or channels (values) as its 16 rows and the eight query rows as its columns:
 //   scores  a nibble in the low bits of an fp16 is the number n 2^-24 exactly (four bits further up: 16 n 2^-24, and that channel's query element is divided by 16): one shift
 //           and four ands turn eight nibbles into operands.  - 8 sum q is taken off afterwards in f32.
-//   values  1024 + n is n in the low bits of the fp16 1024; minus 1032 it is n - 8.  (Sums of n alone would grow with the keys while the result does not: the f32 sums lost 1e-4 of it.)
-// The sixteen rows of the instruction are eight query rows twice: rows 0-7 multiply with the fp16 of a query element (or weight), rows 8-15 with what that left over, so that f32 results keep
-// 22 bits.  The 16-bit types get it for nothing.
-// The weight of a value is p_j d_j.  Its reference is not m but the largest z_j + floor(log2 |d_j|) so far: p_j d_j stays in fp16's range whatever the values' scales are.  Both references move only when
-// something passes them by 2^8, so the usual step has no exchange between lanes.
+//   values  1024 + n is n in the low bits of the fp16 1024; minus 1032 it is n - 8.  (Sums of n alone would grow with the keys while the result does not: f32 sums would lose 1e-4 of it.)
+// Queries are scaled by a power of two into fp16's range.  f32 queries are two fp16 numbers (what the first leaves over is the second), and so are the weights of f32 and f16 results: the
+// second ones go through another mma into the same sums.  bf16 has its queries exactly in one, and its weights are rounded to one (2^-11, an eighth of the result's own step).
+// The weight of a value is p_j d_j.  Its reference is not m but m + r, the largest z_j + log2 |d_j| so far: p_j d_j stays in fp16's range whatever the values' scales are (r is kept by itself: large
+// scores leave no bits of log2 |d_j| in a sum).  Both references move only when something passes them by 2^8, so the usual step has no exchange between lanes but the 8 x 8 transposition that makes operands of the weights.
 // What bounds it: the bytes of the cache, 2 (hd / 2 + 4) per position and kv head.
 #pragma once
+#include <type_traits>
+
 #include "dev_umma.cuh"
 
 namespace dev {
@@ -51,7 +54,7 @@ template <int TILE> __device__ __forceinline__ Q4Span q4_span(const b200_q4_atte
     return s;
 }
 
-// the workspace: per block, two parts of [8][HD] sums, [8][4] (m, reference of the sums, l, -); then per block what its first stretch ends
+// the workspace: per block, two parts of [8][HD] sums, [8][4] (m, r, l, -); then per block what its first stretch ends
 struct Q4End {
     int first_cta, first_slot, seq, rb, head, ends;
 };
@@ -62,6 +65,8 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// a reference's distance to one that is at least as high (0 where both are -infinity)
+__device__ __forceinline__ float below(float x, float top) { return x == top ? 0.0f : x - top; }
 __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -75,6 +80,12 @@ __device__ __forceinline__ float2 unpack_h2(uint32_t v) { return __half22float2(
 __device__ __forceinline__ uint32_t sub_h2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// an 8 x 8 matrix of 16-bit numbers, two neighbours of row lane / 4 per lane
+__device__ __forceinline__ uint32_t transposed8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
@@ -100,7 +111,8 @@ template <typename T, int HD, int W> struct Q4Smem {
 template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 16 / W) attention_q4_kernel(const b200_q4_attention a, uint64_t page16) {
     using St = Q4Stage<HD>;
     using Sm = Q4Smem<T, HD, W>;
-    constexpr int TILE = Sm::TILE, WORDS = HD / 32, NT = HD / 8;      // words of a key row per lane; column tiles of the values
+    constexpr int TILE = Sm::TILE, WORDS = HD / 32, NT = HD / 16;      // words of a key row per lane; row tiles of the values
+    constexpr bool Q2 = sizeof(T) == 4, P2 = !std::is_same<T, __nv_bfloat16>::value;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ long long s_sum[W];
@@ -163,20 +175,24 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
     const uint32_t ring = sm_u32(smem) + warp * QA_STAGES * St::BYTES;
     float* merge = reinterpret_cast<float*>(smem + Sm::RING);             // [W][8][HD + 4]
     float* stat = merge + W * QA_ROWS * (HD + 4);                         // [W][8][4]
+    // where this lane's words of a stage are: keys of positions g and g + 8; values of positions 2 c + (0, 1, 8, 9), words g and g + 8
+    const uint32_t k_at = g * St::ROW + c * (WORDS * 4), v_at = St::V + q4_piece(2 * c, g >> 2) * 16 + (g & 3) * 4;
+    constexpr int P = St::ROW / 16;                                       // pieces of a row
     Q4Seq q = q4_seq(a, s, false);
     for (long long cur = c0; cur < c1;) {
         const Q4Span sp = q4_span<TILE>(a, q, G, rb);
         const int stop = (int)min((long long)sp.tiles, tile + (c1 - cur));
 
-        // ---- this lane's row: its query, its keys
-        const int r = rb * QA_ROWS + g, token = r / G;
-        const bool live = r < q.count * G;
-        const int64_t pos = q.len - q.count + token;
-        // (rows behind the last one compute along with the first: nothing of theirs is written)
-        const int row_hi = live ? (int)max((int64_t)0, pos + 1) : INT32_MAX, row_lo = live && a.window > 0 ? (int)max((int64_t)0, pos + 1 - a.window) : 0;
-        uint32_t qa[WORDS][2][4];
-        float alpha, q8;
+        // ---- query row g as operand; what scores of rows 2 c and 2 c + 1 need
+        uint32_t qb[WORDS][2][2], ql[Q2 ? WORDS : 1][2][2];
+        float alpha[2], q8[2], m[2], mr[2], l[2], acc[NT][4];
+        int hi[2], lo[2], hi_min, lo_max;
         {
+            const int r = rb * QA_ROWS + g, token = r / G;
+            const bool live = r < q.count * G;
+            const int64_t pos = q.len - q.count + token;
+            // (rows behind the last one compute along with the first: nothing of theirs is written)
+            const int row_hi = live ? (int)max((int64_t)0, pos + 1) : INT32_MAX, row_lo = live && a.window > 0 ? (int)max((int64_t)0, pos + 1 - a.window) : 0;
             float x[HD / 4];
             const T* p = reinterpret_cast<const T*>(a.q) + (q.first + (live ? token : 0)) * a.q_token + (h * G + (live ? r - token * G : 0)) * a.q_head + c * (HD / 4);
             if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) load_n<T, HD / 4, true>(p, x);
@@ -191,185 +207,241 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < HD / 4; i++) x[i] = ldexpf(x[i], e);
-            auto part = [&](float u, float v, float f, uint32_t& hi, uint32_t& lo) {
-                hi = pack_h2(u * f, v * f);
-                const float2 b = unpack_h2(hi);
-                lo = pack_h2(u * f - b.x, v * f - b.y);
-                const float2 d = unpack_h2(lo);
-                sum += ((b.x + d.x) + (b.y + d.y)) / f;
+            auto part = [&](float u, float v, float f, uint32_t& first, uint32_t& second) {
+                first = pack_h2(u * f, v * f);
+                const float2 b = unpack_h2(first);
+                sum += (b.x + b.y) / f;
+                if (Q2) {
+                    second = pack_h2(u * f - b.x, v * f - b.y);
+                    const float2 d = unpack_h2(second);
+                    sum += (d.x + d.y) / f;
+                }
             };
 #pragma unroll
             for (int j = 0; j < WORDS; j++)
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    part(x[8 * j + 2 * u], x[8 * j + 2 * u + 4], 1.0f, qa[j][u][0], qa[j][u][1]);
-                    part(x[8 * j + 2 * u + 1], x[8 * j + 2 * u + 5], 0.0625f, qa[j][u][2], qa[j][u][3]);
+                    part(x[8 * j + 2 * u], x[8 * j + 2 * u + 4], 1.0f, qb[j][u][0], ql[Q2 ? j : 0][u][0]);
+                    part(x[8 * j + 2 * u + 1], x[8 * j + 2 * u + 5], 0.0625f, qb[j][u][1], ql[Q2 ? j : 0][u][1]);
                 }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            q8 = sum * (8.0f / 16384.0f);                                  // in units of 2^-10: (sums of n 2^-24) * 2^10
-            alpha = ldexpf(a.scale * 1.4426950408889634f, 14 - e);
+            const float row_q8 = sum * (8.0f / 16384.0f);                  // in units of 2^-10: (sums of n 2^-24) * 2^10
+            const float row_alpha = ldexpf(a.scale * 1.4426950408889634f, 14 - e);
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                q8[k] = __shfl_sync(0xffffffffu, row_q8, 4 * (2 * c + k));
+                alpha[k] = __shfl_sync(0xffffffffu, row_alpha, 4 * (2 * c + k));
+                hi[k] = __shfl_sync(0xffffffffu, row_hi, 4 * (2 * c + k));
+                lo[k] = __shfl_sync(0xffffffffu, row_lo, 4 * (2 * c + k));
+                m[k] = mr[k] = -INFINITY;
+                l[k] = 0.0f;
+            }
+            hi_min = __reduce_min_sync(0xffffffffu, row_hi);
+            lo_max = __reduce_max_sync(0xffffffffu, row_lo);
         }
-        float m = -INFINITY, mv = -INFINITY, l = 0.0f, acc[NT][4];
 #pragma unroll
         for (int i = 0; i < NT; i++)
 #pragma unroll
             for (int k = 0; k < 4; k++) acc[i][k] = 0.0f;
 
-        // ---- the ring: stage i holds step tile + i
-        const int64_t table = (int64_t)s * a.table_stride;
-        auto fetch = [&](int step, int stage) {
+        // ---- the ring.  The page of a step is looked up one step before its rows are asked for.
+        const int32_t* table = a.page_table + (int64_t)s * a.table_stride;
+        int page = -1, row = 0;
+        uint32_t good = 0;      // by stage: the page is one of the cache's
+        auto look = [&](int step) {
             const int p0 = sp.base + step * TILE + warp * 16;
             if (step < stop && p0 < sp.hi) {
-                const int p16 = p0 >> 4, index = (int)(((uint64_t)p16 * page16) >> 36);
-                int64_t page = a.page_table[table + index];
-                page = page >= 0 && page < a.cache.n_pages ? page : 0;      // (masked below)
-                const int row = p0 - index * page_size;
-                const Q4Block b = q4_block(a.cache, page, h);
+                const int index = (int)(((uint64_t)(p0 >> 4) * page16) >> 36);
+                row = p0 - index * page_size;
+                page = table[index];
+            }
+        };
+        auto fetch = [&](int step) {
+            const int p0 = sp.base + step * TILE + warp * 16, stage = step & (QA_STAGES - 1);
+            if (step < stop && p0 < sp.hi) {
+                const bool there = (unsigned)page < (unsigned long long)a.cache.n_pages;
+                good = there ? good | 1u << stage : good & ~(1u << stage);
+                if (!there && a.status && lane == 0) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
+                const Q4Block b = q4_block(a.cache, there ? page : 0, h);      // (masked below)
                 const uint32_t at = ring + stage * St::BYTES;
-                constexpr int P = St::ROW / 16;                             // pieces of a row
+                const uint8_t *k = b.k + row * St::ROW + lane * 16, *v = b.v + row * St::ROW + lane * 16;
 #pragma unroll
                 for (int i = 0; i < 16 * P; i += 32) {
-                    const int n = i + lane;
-                    if (16 * P >= 32 || n < 16 * P) {
-                        cp16(at + n * 16, b.k + row * St::ROW + n * 16);
-                        cp16(at + St::V + q4_piece(n / P, n % P) * 16, b.v + row * St::ROW + n * 16);
-                    }
+                    cp16(at + (i + lane) * 16, k + i * 16);
+                    cp16(at + St::V + q4_piece((i + lane) / P, (i + lane) % P) * 16, v + i * 16);
                 }
-                if (lane < 4) cp16(at + St::KS + lane * 16, b.ks + row + lane * 4);
-                else if (lane < 8) cp16(at + St::VS + (lane - 4) * 16, b.vs + row + (lane - 4) * 4);
+                if (lane < 8) cp16(at + St::KS + lane * 16, (lane < 4 ? b.ks : b.vs - 16) + row + lane * 4);
             }
             cp_commit();
         };
+        look(tile);
 #pragma unroll
-        for (int i = 0; i < QA_STAGES - 1; i++) fetch(tile + i, i);
-        int stage = 0;
+        for (int i = 0; i < QA_STAGES - 1; i++) {
+            fetch(tile + i);
+            look(tile + i + 1);
+        }
         for (int step = tile; step < stop; step++) {
             cp_wait<QA_STAGES - 2>();
             __syncwarp();
-            fetch(step + QA_STAGES - 1, stage == 0 ? QA_STAGES - 1 : stage - 1);
-            const uint32_t at = ring + stage * St::BYTES;
-            stage = stage == QA_STAGES - 1 ? 0 : stage + 1;
+            fetch(step + QA_STAGES - 1);
+            look(step + QA_STAGES);
+            const uint32_t at = ring + (step & (QA_STAGES - 1)) * St::BYTES;
             const int p0 = sp.base + step * TILE + warp * 16;
             if (p0 >= sp.hi) continue;
-            // scores of positions p0 + 8 u + 2 c, + 1
+            // scores: [position g, g + 8][row 2 c, 2 c + 1]
             float z[2][2];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                uint32_t w[WORDS];
-                lds<WORDS>(w, at + (8 * u + g) * St::ROW + c * (WORDS * 4));
+            uint32_t vs[2];
+            {
+                uint32_t w[2][WORDS], ks[2][1];
                 float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int j = 0; j < WORDS; j++) {
-                    mma16(d, qa[j][0][0], qa[j][0][1], qa[j][0][2], qa[j][0][3], w[j] & 0x000f000fu, w[j] & 0x00f000f0u);
-                    const uint32_t x = w[j] >> 8;
-                    mma16(d, qa[j][1][0], qa[j][1][1], qa[j][1][2], qa[j][1][3], x & 0x000f000fu, x & 0x00f000f0u);
-                }
-                uint32_t ks[2];
-                lds<2>(ks, at + St::KS + (8 * u + 2 * c) * 4);
+                for (int u = 0; u < 2; u++) lds<WORDS>(w[u], at + k_at + u * 8 * St::ROW);
 #pragma unroll
-                for (int k = 0; k < 2; k++) z[u][k] = (fmaf(d[k] + d[k + 2], 1024.0f, -q8) * alpha) * __uint_as_float(ks[k]);
-            }
-            uint32_t ok = 0xfu;
-            const int index = (int)(((uint64_t)(p0 >> 4) * page16) >> 36);
-            const int64_t page = a.page_table[table + index];
-            const bool there = page >= 0 && page < a.cache.n_pages;
-            if (!there && a.status && lane == 0) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
-            if (!there || !__all_sync(0xffffffffu, p0 >= row_lo && p0 + 16 <= row_hi)) {
-                ok = 0;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int j = p0 + 8 * (i >> 1) + 2 * c + (i & 1);
-                    if (there && j >= row_lo && j < row_hi) ok |= 1u << i;
-                    else z[i >> 1][i & 1] = -INFINITY;
+                for (int u = 0; u < 2; u++) {
+                    uint32_t v[1];
+                    lds<1>(ks[u], at + St::KS + (8 * u + g) * 4);
+                    lds<1>(v, at + St::VS + (8 * u + g) * 4);
+                    vs[u] = v[0];
                 }
+#pragma unroll
+                for (int j = 0; j < WORDS; j++)
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        const uint32_t x = t ? w[0][j] >> 8 : w[0][j], y = t ? w[1][j] >> 8 : w[1][j];
+                        mma16(d, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qb[j][t][0], qb[j][t][1]);
+                        if (Q2) mma16(d, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, ql[Q2 ? j : 0][t][0], ql[Q2 ? j : 0][t][1]);
+                    }
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) z[u][k] = (fmaf(d[2 * u + k], 1024.0f, -q8[k]) * alpha[k]) * __uint_as_float(ks[u][0]);
             }
-            // the values' scales as 2^E * mant
-            float y[2][2], mant[2][2];
+            const float zs[2][2] = {{z[0][0], z[0][1]}, {z[1][0], z[1][1]}};
+            const bool there = (good >> (step & (QA_STAGES - 1))) & 1u, all = there && p0 >= lo_max && p0 + 16 <= hi_min;
+            uint32_t in = 0xfu;
+            if (!all) {
+                in = 0;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const int j = p0 + 8 * u + g;
+                        if (there && j >= lo[k] && j < hi[k]) in |= 1u << (2 * u + k);
+                        else z[u][k] = -INFINITY;
+                    }
+            }
+            auto score = [&](int u, int k) { return (in >> (2 * u + k)) & 1u ? zs[u][k] : -INFINITY; };
+            float y[2][2], ex[2];      // z becomes log2 p, y is log2 of the weight's magnitude
             bool past = false;
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                uint32_t vs[2];
-                lds<2>(vs, at + St::VS + (8 * u + 2 * c) * 4);
+                // (a scale of zero: as 2^-1000, which leaves nothing of it; NaN stays)
+                asm("{\n\t.reg .f32 t;\n\tlg2.approx.f32 t, %1;\n\tmax.NaN.f32 %0, t, 0fC47A0000;\n\t}" : "=f"(ex[u]) : "f"(fabsf(__uint_as_float(vs[u]))));
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    const uint32_t ex = (vs[k] >> 23) & 255u;
-                    y[u][k] = z[u][k] + (__uint_as_float(0x4b000000u + ex) - 8388735.0f);      // + (ex - 127)
-                    mant[u][k] = ex == 0 ? 0.0f : ex == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float((vs[k] & 0x807fffffu) | 0x3f800000u);
-                    past |= z[u][k] > m + 8.0f || y[u][k] > mv + 8.0f;
+                    z[u][k] -= m[k];
+                    y[u][k] = z[u][k] + ex[u] - mr[k];
+                    past |= z[u][k] > 8.0f || y[u][k] > 8.0f;
                 }
             }
             if (__any_sync(0xffffffffu, past)) {
-                float top = fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[1][0], z[1][1])), topv = fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[1][0], y[1][1]));
 #pragma unroll
-                for (int o = 1; o <= 2; o <<= 1) {
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, o));
+                for (int k = 0; k < 2; k++) {
+                    // (the differences are taken again from the scores: a first step has no finite reference)
+                    const float z0 = score(0, k), z1 = score(1, k);
+                    float top = fmaxf(z0, z1);
+#pragma unroll
+                    for (int o = 4; o <= 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    top = fmaxf(top, m[k]);
+                    z[0][k] = z0 - top;
+                    z[1][k] = z1 - top;
+                    const float up = top == m[k] ? 0.0f : m[k] - top, was = mr[k] + up;
+                    float topv = fmaxf(z[0][k] + ex[0], z[1][k] + ex[1]);
+#pragma unroll
+                    for (int o = 4; o <= 16; o <<= 1) topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, o));
+                    topv = fmaxf(topv, was);
+                    y[0][k] = z[0][k] + ex[0] - topv;
+                    y[1][k] = z[1][k] + ex[1] - topv;
+                    l[k] *= ex2(up);
+                    const float f = topv == was ? 1.0f : ex2(was - topv);
+#pragma unroll
+                    for (int i = 0; i < NT; i++) {
+                        acc[i][k] *= f;
+                        acc[i][k + 2] *= f;
+                    }
+                    m[k] = top;
+                    mr[k] = topv;
                 }
-                top = fmaxf(top, m);
-                topv = fmaxf(topv, mv);
-                l *= top == m ? 1.0f : ex2(m - top);
-                const float f = topv == mv ? 1.0f : ex2(mv - topv);
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) acc[i][k] *= f;
-                m = top;
-                mv = topv;
             }
-            uint32_t pa[2][2];      // [positions' half][fp16, what it leaves over]
+            uint32_t pb[2], pl[2];      // the weights of positions 2 c, 2 c + 1 (+ 8) for row g, and what their fp16 leave over
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 float w[2];
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    const bool in = (ok >> (2 * u + k)) & 1u;
-                    l += in ? ex2(z[u][k] - m) : 0.0f;
-                    w[k] = in ? ex2(y[u][k] - mv) * mant[u][k] : 0.0f;
+                    const float p = ex2(z[u][k]);
+                    w[k] = __uint_as_float(__float_as_uint(ex2(y[u][k])) ^ (vs[u] & 0x80000000u));
+                    if (all) {
+                        l[k] += p;
+                    } else {
+                        const bool seen = (in >> (2 * u + k)) & 1u;
+                        l[k] += seen ? p : 0.0f;
+                        w[k] = seen ? w[k] : 0.0f;
+                    }
                 }
-                pa[u][0] = pack_h2(w[0], w[1]);
-                const float2 b = unpack_h2(pa[u][0]);
-                pa[u][1] = pack_h2(w[0] - b.x, w[1] - b.y);
+                pb[u] = pack_h2(w[0], w[1]);
+                if (P2) {
+                    const float2 b = unpack_h2(pb[u]);
+                    pl[u] = transposed8x8(pack_h2(w[0] - b.x, w[1] - b.y));
+                }
+                pb[u] = transposed8x8(pb[u]);
             }
-            // values: column n of tile i is channel 8 n + i (and 64 more from tile 8 on)
+            // values: [positions 2 c, 2 c + 1; + 8][word g, word g + 8], channels 0-3 and 4-7 of the word
+            uint32_t t[HD / 64][2][2];
 #pragma unroll
-            for (int half = 0; half < NT / 8; half++) {
-                uint32_t t[2][2];      // [positions' half][channels 0-3, 4-7 of the word]
+            for (int half = 0; half < HD / 64; half++)
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     uint32_t w0[1], w1[1];
-                    const int piece = 2 * half + (g >> 2);
-                    lds<1>(w0, at + St::V + q4_piece(8 * u + 2 * c, piece) * 16 + (g & 3) * 4);
-                    lds<1>(w1, at + St::V + q4_piece(8 * u + 2 * c + 1, piece) * 16 + (g & 3) * 4);
-                    t[u][0] = __byte_perm(w0[0], w1[0], 0x5410);
-                    t[u][1] = __byte_perm(w0[0], w1[0], 0x7632);
+                    lds<1>(w0, at + v_at + q4_piece(8 * u, 2 * half) * 16);
+                    lds<1>(w1, at + v_at + q4_piece(8 * u + 1, 2 * half) * 16);
+                    t[half][u][0] = __byte_perm(w0[0], w1[0], 0x5410);
+                    t[half][u][1] = __byte_perm(w0[0], w1[0], 0x7632);
                 }
+            // nibble i of its word; odd ones 16 times too large, which is put right at the end
+            auto nibble = [&](int half, int u, int i) {
+                const uint32_t v = (i & 2) ? t[half][u][i >> 2] >> 8 : t[half][u][i >> 2];
+                return sub_h2((v & ((i & 1) ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u, (i & 1) ? 0x64806480u : 0x64086408u);
+            };
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const bool odd = i & 1;      // 16 (n - 8): the result is divided by 16 at the end
-                    uint32_t b[2];
+            for (int i = 0; i < NT; i++) {
+                uint32_t v[4];      // rows g of the tile: word g, nibble i; rows g + 8: word g + 8 (hd 64: nibble i + 4)
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const uint32_t v = (i & 2) ? t[u][i >> 2] >> 8 : t[u][i >> 2];
-                        b[u] = sub_h2((v & (odd ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u, odd ? 0x64806480u : 0x64086408u);
-                    }
-                    mma16(acc[8 * half + i], pa[0][0], pa[0][1], pa[1][0], pa[1][1], b[0], b[1]);
+                for (int u = 0; u < 2; u++) {
+                    v[2 * u] = nibble(0, u, i);
+                    v[2 * u + 1] = HD == 128 ? nibble(HD / 64 - 1, u, i) : nibble(0, u, i + 4);
                 }
+                mma16(acc[i], v[0], v[1], v[2], v[3], pb[0], pb[1]);
+                if (P2) mma16(acc[i], v[0], v[1], v[2], v[3], pl[0], pl[1]);
             }
         }
         cp_wait<0>();
 
         // ---- the warps' sums into one
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (c == 0) *reinterpret_cast<float4*>(stat + (warp * QA_ROWS + g) * 4) = make_float4(m, mv, l, 0.0f);
-        float* mine_out = merge + (warp * QA_ROWS + g) * (HD + 4);
 #pragma unroll
-        for (int half = 0; half < NT / 8; half++)
+        for (int k = 0; k < 2; k++) {
 #pragma unroll
-            for (int k = 0; k < 2; k++)
+            for (int o = 4; o <= 16; o <<= 1) l[k] += __shfl_xor_sync(0xffffffffu, l[k], o);
+            if (g == 0) *reinterpret_cast<float4*>(stat + (warp * QA_ROWS + 2 * c + k) * 4) = make_float4(m[k], mr[k], l[k], 0.0f);
+            float* to = merge + (warp * QA_ROWS + 2 * c + k) * (HD + 4) + 8 * g;
 #pragma unroll
-                for (int i = 0; i < 8; i++) mine_out[64 * half + 8 * (2 * c + k) + i] = (acc[8 * half + i][k] + acc[8 * half + i][k + 2]) * ((i & 1) ? 0.0625f : 1.0f);
+            for (int i = 0; i < NT; i++) {
+                const float f = (i & 1) ? 0.0625f : 1.0f;
+                to[i] = acc[i][k] * f;
+                to[HD == 128 ? 64 + i : 4 + i] = acc[i][k + 2] * f;
+            }
+        }
         __syncthreads();
         const bool whole = tile == 0 && stop == sp.tiles, first = cur == c0;
         float* part = reinterpret_cast<float*>(a.workspace) + ((size_t)blockIdx.x * 2 + (first ? 0 : 1)) * q4_part_floats<HD>();
@@ -377,16 +449,15 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
             const int row = i / (HD / 4), ch = (i % (HD / 4)) * 4;
             float top = -INFINITY, topv = -INFINITY, sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < W; w++) {
-                top = fmaxf(top, stat[(w * QA_ROWS + row) * 4]);
-                topv = fmaxf(topv, stat[(w * QA_ROWS + row) * 4 + 1]);
-            }
+            for (int w = 0; w < W; w++) top = fmaxf(top, stat[(w * QA_ROWS + row) * 4]);
+#pragma unroll
+            for (int w = 0; w < W; w++) topv = fmaxf(topv, stat[(w * QA_ROWS + row) * 4 + 1] + below(stat[(w * QA_ROWS + row) * 4], top));
             float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < W; w++) {
                 const float4 st = *reinterpret_cast<const float4*>(stat + (w * QA_ROWS + row) * 4), v = *reinterpret_cast<const float4*>(merge + (w * QA_ROWS + row) * (HD + 4) + ch);
-                sum += st.z * (st.x == top ? 1.0f : ex2(st.x - top));
-                const float f = st.y == topv ? 1.0f : ex2(st.y - topv);
+                const float d = below(st.x, top), f = ex2(below(st.y + d, topv));
+                sum += st.z * ex2(d);
                 o.x += v.x * f;
                 o.y += v.y * f;
                 o.z += v.z * f;
@@ -396,7 +467,7 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
                 const int rr = rb * QA_ROWS + row;
                 if (rr < q.count * G) {
                     // (l = 0: the row saw nothing, and the sums are zeros)
-                    const float f = sum == 0.0f ? 0.0f : 1.0f / sum, e = topv == -INFINITY ? 0.0f : topv - top;
+                    const float f = sum == 0.0f ? 0.0f : 1.0f / sum, e = topv == -INFINITY ? 0.0f : topv;
                     const float v[4] = {o.x, o.y, o.z, o.w};
                     T* p = reinterpret_cast<T*>(a.out) + (q.first + rr / G) * a.out_token + (h * G + rr % G) * a.out_head + ch;
 #pragma unroll
@@ -439,38 +510,33 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
 template <typename T, int HD> __global__ void __launch_bounds__(128) attention_q4_join_kernel(const b200_q4_attention a, int grid) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int LANES = HD / 4, GROUPS = 128 / LANES, PART = q4_part_floats<HD>();
-    __shared__ float s_red[3][4];
     __shared__ __align__(16) float s_o[GROUPS][HD];
     const float* ws = reinterpret_cast<const float*>(a.workspace);
     const Q4End e = reinterpret_cast<const Q4End*>(ws + (size_t)grid * 2 * PART)[blockIdx.x];
     if (!e.ends) return;
-    const int row = blockIdx.y, tid = threadIdx.x, n = (int)blockIdx.x - e.first_cta + 1, G = a.n_heads / a.cache.n_kv_heads, rr = e.rb * QA_ROWS + row;
+    const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31, n = (int)blockIdx.x - e.first_cta + 1, G = a.n_heads / a.cache.n_kv_heads, rr = e.rb * QA_ROWS + row;
     const Q4Seq q = q4_seq(a, e.seq, false);
     if (rr >= q.count * G) return;
     auto part = [&](int i) { return ws + ((size_t)(e.first_cta + i) * 2 + (i == 0 ? e.first_slot : 0)) * PART; };
     float top = -INFINITY, topv = -INFINITY, sum = 0.0f;
-    for (int i = tid; i < n; i += 128) {
-        const float* st = part(i) + QA_ROWS * HD + row * 4;
-        top = fmaxf(top, st[0]);
-        topv = fmaxf(topv, st[1]);
+    // (a warp has both maxima by itself: no exchange between warps)
+    for (int i = lane; i < n; i += 32) {
+        const float2 st = *reinterpret_cast<const float2*>(part(i) + QA_ROWS * HD + row * 4);
+        const float was = top;
+        top = fmaxf(top, st.x);
+        topv = fmaxf(topv + below(was, top), st.y + below(st.x, top));
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, o));
+        const float x = __shfl_xor_sync(0xffffffffu, top, o), y = __shfl_xor_sync(0xffffffffu, topv, o), was = top;
+        top = fmaxf(top, x);
+        topv = fmaxf(topv + below(was, top), y + below(x, top));
     }
-    if ((tid & 31) == 0) {
-        s_red[0][tid >> 5] = top;
-        s_red[1][tid >> 5] = topv;
-    }
-    __syncthreads();
-    top = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
-    topv = fmaxf(fmaxf(s_red[1][0], s_red[1][1]), fmaxf(s_red[1][2], s_red[1][3]));
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int i = tid / LANES; i < n; i += GROUPS) {
         const float4 st = *reinterpret_cast<const float4*>(part(i) + QA_ROWS * HD + row * 4), v = *reinterpret_cast<const float4*>(part(i) + row * HD + (tid % LANES) * 4);
-        sum += st.z * (st.x == top ? 1.0f : ex2(st.x - top));
-        const float f = st.y == topv ? 1.0f : ex2(st.y - topv);
+        const float d = below(st.x, top), f = ex2(below(st.y + d, topv));
+        sum += st.z * ex2(d);
         o.x += v.x * f;
         o.y += v.y * f;
         o.z += v.z * f;
@@ -487,7 +553,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(128) attention_q
             v += s_o[k][tid];
             l += s_l[k];
         }
-        const float x = topv == -INFINITY ? 0.0f : topv - top;
+        const float x = topv == -INFINITY ? 0.0f : topv;
         reinterpret_cast<T*>(a.out)[(q.first + rr / G) * a.out_token + (e.head * G + rr % G) * a.out_head + tid] =
             from_f<T>(l == 0.0f ? 0.0f : ldexpf(v * (1.0f / l), (int)floorf(x)) * ex2(x - floorf(x)));
     }

@@ -250,7 +250,7 @@ def check_attention(D, dtype, nh, nkv, hd, page, lens, q_lens, window=0, seed=1,
     status = torch.zeros(1, dtype=torch.int32).cuda()
     args = dict(q_starts=None if all(m == 1 for m in q_lens) and not kw.pop("ragged", False) else torch.tensor(starts, dtype=torch.int32).cuda(), window=window, status=status, scale=scale)
     o = D.attention_paged_q4(q.cuda(), pages.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), **args, **kw)
-    want, off = R.attention(q.double(), R.values(pages, page, hd), table.tolist(), lens, starts, page, hd**-0.5 if scale is None else scale, window, pages.shape[0])
+    want, off = R.attention(q.double(), R.values(pages, page, hd), table.tolist(), lens, starts, page, hd**-0.5 if scale is None else scale, window, pages.shape[0], dtype)
     tol = off + 1.001 * R.HALF_STEP[dtype] * (want.abs() + off) + R.LEAST[dtype]
     got = o.cpu().double()
     assert torch.isfinite(got).all()
@@ -407,7 +407,7 @@ def test_a_layer(D, dtype, q_lens, cached):
     R.put_rows(first["pages"], 16, 64, first["slots"], R.rotate(qkv[:, 8:10], cs[..., :32], cs[..., 32:], False), qkv[:, 10:])
     assert torch.equal(first["pages"], s["pages"].cpu())
     q = R.rotate(qkv[:, :8], cs[..., :32], cs[..., 32:], False).to(dtype).double()
-    o, off = R.attention(q, R.values(first["pages"], 16, 64), first["page_table"].tolist(), first["lens"].tolist(), first["starts"].tolist(), 16, 0.125, 0, first["pages"].shape[0])
+    o, off = R.attention(q, R.values(first["pages"], 16, 64), first["page_table"].tolist(), first["lens"].tolist(), first["starts"].tolist(), 16, 0.125, 0, first["pages"].shape[0], dtype)
     o, off = o.flatten(1), (off + R.HALF_STEP[dtype] * 1.001 * (o.abs() + off) + R.LEAST[dtype]).flatten(1)
     rms = (o.square().mean(1, keepdim=True) + 1e-5).sqrt()
     n = o / rms * first["w2"].double()
