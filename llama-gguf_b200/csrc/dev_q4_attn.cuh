@@ -178,6 +178,11 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
     // where this lane's words of a stage are: keys of positions g and g + 8; values of positions 2 c + (0, 1, 8, 9), words g and g + 8
     const uint32_t k_at = g * St::ROW + c * (WORDS * 4), v_at = St::V + q4_piece(2 * c, g >> 2) * 16 + (g & 3) * 4;
     constexpr int P = St::ROW / 16;                                       // pieces of a row
+    // where it puts what it fetches, and from which offsets of a kv head's block (lane * 16 into the rows of a position)
+    const uint32_t v_to = St::V + q4_piece(lane / P, lane % P) * 16;
+    const int block = page_size * (HD + 8), page_bytes = nkv * block, v_off = page_size * St::ROW, s_off = 2 * v_off + (lane < 4 ? 0 : page_size * 4 - 64);
+    const unsigned n_pages = (unsigned)a.cache.n_pages;
+    const int tile_pages = TILE / page_size, tile_rows = TILE - tile_pages * page_size;
     Q4Seq q = q4_seq(a, s, false);
     for (long long cur = c0; cur < c1;) {
         const Q4Span sp = q4_span<TILE>(a, q, G, rb);
@@ -203,10 +208,12 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // elements times 2^e are below 2^14: fp16 holds the fp16 of them and what that leaves over
-            const int e = top > 0.0f && top < INFINITY ? 13 - ilogbf(top) : 0;
+            // (e is at most 140: two factors, each a number)
+            const int e = top < INFINITY ? 140 - (int)(__float_as_uint(top) >> 23) : 0;
+            const float e1 = __int_as_float((127 + e / 2) << 23), e2 = __int_as_float((127 + e - e / 2) << 23);
             float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < HD / 4; i++) x[i] = ldexpf(x[i], e);
+            for (int i = 0; i < HD / 4; i++) x[i] = x[i] * e1 * e2;
             auto part = [&](float u, float v, float f, uint32_t& first, uint32_t& second) {
                 first = pack_h2(u * f, v * f);
                 const float2 b = unpack_h2(first);
@@ -247,48 +254,56 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
 
         // ---- the ring.  The page of a step is looked up one step before its rows are asked for.
         const int32_t* table = a.page_table + (int64_t)s * a.table_stride;
-        int page = -1, row = 0;
-        uint32_t good = 0;      // by stage: the page is one of the cache's
-        auto look = [&](int step) {
-            const int p0 = sp.base + step * TILE + warp * 16;
-            if (step < stop && p0 < sp.hi) {
-                const int index = (int)(((uint64_t)(p0 >> 4) * page16) >> 36);
-                row = p0 - index * page_size;
-                page = table[index];
+        const uint8_t* mine_k = reinterpret_cast<const uint8_t*>(a.cache.data) + (int64_t)h * block + lane * 16;
+        int p_look = sp.base + tile * TILE + warp * 16, index = (int)(((uint64_t)(p_look >> 4) * page16) >> 36), row_look = p_look - index * page_size;
+        int p_fetch = p_look, page = 0, row = 0;
+        const int p_stop = min(sp.hi, sp.base + stop * TILE);
+        bool odd_page = false;      // a page that is none of the cache's came by in this item
+        auto look = [&]() {
+            if (p_look < p_stop) page = table[index];
+            row = row_look;
+            p_look += TILE;
+            index += tile_pages;
+            row_look += tile_rows;
+            if (row_look >= page_size) {
+                row_look -= page_size;
+                index++;
             }
         };
-        auto fetch = [&](int step) {
-            const int p0 = sp.base + step * TILE + warp * 16, stage = step & (QA_STAGES - 1);
-            if (step < stop && p0 < sp.hi) {
-                const bool there = (unsigned)page < (unsigned long long)a.cache.n_pages;
-                good = there ? good | 1u << stage : good & ~(1u << stage);
-                if (!there && a.status && lane == 0) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
-                const Q4Block b = q4_block(a.cache, there ? page : 0, h);      // (masked below)
+        auto fetch = [&](int stage) {
+            if (p_fetch < p_stop) {
+                if ((unsigned)page >= n_pages) {      // (masked below)
+                    odd_page = true;
+                    page = 0;
+                    if (a.status && lane == 0) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
+                }
+                const uint8_t* k = mine_k + (int64_t)page * page_bytes + row * St::ROW;
                 const uint32_t at = ring + stage * St::BYTES;
-                const uint8_t *k = b.k + row * St::ROW + lane * 16, *v = b.v + row * St::ROW + lane * 16;
 #pragma unroll
                 for (int i = 0; i < 16 * P; i += 32) {
-                    cp16(at + (i + lane) * 16, k + i * 16);
-                    cp16(at + St::V + q4_piece((i + lane) / P, (i + lane) % P) * 16, v + i * 16);
+                    cp16(at + lane * 16 + i * 16, k + i * 16);
+                    cp16(at + v_to + q4_piece(i / P, 0) * 16, k + v_off + i * 16);
                 }
-                if (lane < 8) cp16(at + St::KS + lane * 16, (lane < 4 ? b.ks : b.vs - 16) + row + lane * 4);
+                // (lanes 0-3 key scales, 4-7 value scales, which follow page_size floats later: lane * 16 is in k, 64 of it too much for those)
+                if (lane < 8) cp16(at + St::KS + lane * 16, k - row * (St::ROW - 4) + s_off);
             }
             cp_commit();
+            p_fetch += TILE;
         };
-        look(tile);
+        look();
 #pragma unroll
         for (int i = 0; i < QA_STAGES - 1; i++) {
-            fetch(tile + i);
-            look(tile + i + 1);
+            fetch(i);
+            look();
         }
-        for (int step = tile; step < stop; step++) {
+        int stage = 0;
+        for (int p0 = sp.base + tile * TILE + warp * 16; p0 < p_stop; p0 += TILE) {
             cp_wait<QA_STAGES - 2>();
             __syncwarp();
-            fetch(step + QA_STAGES - 1);
-            look(step + QA_STAGES);
-            const uint32_t at = ring + (step & (QA_STAGES - 1)) * St::BYTES;
-            const int p0 = sp.base + step * TILE + warp * 16;
-            if (p0 >= sp.hi) continue;
+            fetch((stage + QA_STAGES - 1) & (QA_STAGES - 1));
+            look();
+            const uint32_t at = ring + stage * St::BYTES;
+            stage = (stage + 1) & (QA_STAGES - 1);
             // scores: [position g, g + 8][row 2 c, 2 c + 1]
             float z[2][2];
             uint32_t vs[2];
@@ -318,10 +333,11 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
                     for (int k = 0; k < 2; k++) z[u][k] = (fmaf(d[2 * u + k], 1024.0f, -q8[k]) * alpha[k]) * __uint_as_float(ks[u][0]);
             }
             const float zs[2][2] = {{z[0][0], z[0][1]}, {z[1][0], z[1][1]}};
-            const bool there = (good >> (step & (QA_STAGES - 1))) & 1u, all = there && p0 >= lo_max && p0 + 16 <= hi_min;
+            const bool all = !odd_page && p0 >= lo_max && p0 + 16 <= hi_min;
             uint32_t in = 0xfu;
             if (!all) {
                 in = 0;
+                const bool there = (unsigned)table[(int)(((uint64_t)(p0 >> 4) * page16) >> 36)] < n_pages;
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
