@@ -72,6 +72,18 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// ... with sums that begin here
+__device__ __forceinline__ void mma16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// (v & mask) | set in one instruction
+__device__ __forceinline__ uint32_t masked_or(uint32_t v, uint32_t mask, uint32_t set) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(set));
+    return r;
+}
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -297,6 +309,8 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
             look();
         }
         int stage = 0;
+        uint32_t magic = 0x64006400u;
+        asm("" : "+r"(magic));      // (kept in a register: an instruction has room for one constant)
         for (int p0 = sp.base + tile * TILE + warp * 16; p0 < p_stop; p0 += TILE) {
             cp_wait<QA_STAGES - 2>();
             __syncwarp();
@@ -309,7 +323,7 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
             uint32_t vs[2];
             {
                 uint32_t w[2][WORDS], ks[2][1];
-                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float d[4];
 #pragma unroll
                 for (int u = 0; u < 2; u++) lds<WORDS>(w[u], at + k_at + u * 8 * St::ROW);
 #pragma unroll
@@ -324,7 +338,8 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
 #pragma unroll
                     for (int t = 0; t < 2; t++) {
                         const uint32_t x = t ? w[0][j] >> 8 : w[0][j], y = t ? w[1][j] >> 8 : w[1][j];
-                        mma16(d, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qb[j][t][0], qb[j][t][1]);
+                        if (j + t == 0) mma16_first(d, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qb[j][t][0], qb[j][t][1]);
+                        else mma16(d, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qb[j][t][0], qb[j][t][1]);
                         if (Q2) mma16(d, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, ql[Q2 ? j : 0][t][0], ql[Q2 ? j : 0][t][1]);
                     }
 #pragma unroll
@@ -390,6 +405,15 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
                     mr[k] = topv;
                 }
             }
+            if (!all) {      // (a row that has seen nothing yet has no reference, and a scale may be NaN)
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+                        if (!((in >> (2 * u + k)) & 1u)) {
+                            z[u][k] = y[u][k] = -INFINITY;
+                        }
+            }
             uint32_t pb[2], pl[2];      // the weights of positions 2 c, 2 c + 1 (+ 8) for row g, and what their fp16 leave over
 #pragma unroll
             for (int u = 0; u < 2; u++) {
@@ -398,13 +422,7 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
                 for (int k = 0; k < 2; k++) {
                     const float p = ex2(z[u][k]);
                     w[k] = __uint_as_float(__float_as_uint(ex2(y[u][k])) ^ (vs[u] & 0x80000000u));
-                    if (all) {
-                        l[k] += p;
-                    } else {
-                        const bool seen = (in >> (2 * u + k)) & 1u;
-                        l[k] += seen ? p : 0.0f;
-                        w[k] = seen ? w[k] : 0.0f;
-                    }
+                    l[k] += p;
                 }
                 pb[u] = pack_h2(w[0], w[1]);
                 if (P2) {
@@ -428,7 +446,7 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
             // nibble i of its word; odd ones 16 times too large, which is put right at the end
             auto nibble = [&](int half, int u, int i) {
                 const uint32_t v = (i & 2) ? t[half][u][i >> 2] >> 8 : t[half][u][i >> 2];
-                return sub_h2((v & ((i & 1) ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u, (i & 1) ? 0x64806480u : 0x64086408u);
+                return sub_h2(masked_or(v, (i & 1) ? 0x00f000f0u : 0x000f000fu, magic), (i & 1) ? 0x64806480u : 0x64086408u);
             };
 #pragma unroll
             for (int i = 0; i < NT; i++) {
