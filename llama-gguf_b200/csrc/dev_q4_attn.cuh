@@ -2,9 +2,10 @@
 //
 // One pass over the keys with a running maximum: o = sum_j p_j d_j (n_j - 8) / sum_j p_j, p_j = 2^(z_j - m), z_j = log2(e) scale k_j q . (n_j - 8), k_j and d_j the scales of key and value j.
 //
-// Work.  An item is eight query rows of one sequence and kv head (row = token * G + head, G query heads per kv head) with the keys they see, in tiles of 16 W positions (W warps).  All items'
-// tiles lie on one line, sequence after sequence, and every block takes an equal stretch of it, so that a long sequence among short ones, or alone, keeps every SM busy; lengths are read on
-// the device only.  A stretch that ends inside an item leaves its sums in the workspace, and the second kernel joins them.
+// Work.  An item is eight query rows of one sequence and kv head (row = token * G + head, G query heads per kv head) with the keys they see, in tiles of 16 W positions (W warps).  All items
+// lie on one line, sequence after sequence, QA_START units for what an item takes by itself and one for each of its tiles, and every block takes an equal stretch of it, so that a long sequence among
+// short ones, or alone, keeps every SM busy; lengths are read on the device only.  A stretch that ends inside an item leaves its sums in the workspace, and the second kernel joins them.
+// (Without the units for the start 32 sequences of up to 8000 took 60 us for 46 of longer ones: the block with the shortest sequences took twice the others' time.)
 //
 // A warp takes 16 positions at a time (never more than one page) through a ring in shared memory (cp.async, 16 bytes per lane) and multiplies with mma.m16n8k16 (fp16, f32 sums), the
 // positions (scores) or channels (values) as its 16 rows and the eight query rows as its columns:
@@ -23,7 +24,7 @@
 
 namespace dev {
 
-enum { QA_ROWS = 8, QA_STAGES = 4 };
+enum { QA_ROWS = 8, QA_STAGES = 4, QA_START = 4 };
 
 struct Q4Seq {
     int first, count;      // query tokens
@@ -128,7 +129,7 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ long long s_sum[W];
-    __shared__ int s_item[4];      // sequence, row block, head, tile
+    __shared__ int s_item[4];      // sequence, row block, head, unit of the item
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int nkv = a.cache.n_kv_heads, G = a.n_heads / nkv, page_size = a.cache.page_size;
 
@@ -136,7 +137,7 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
     const int chunk = (a.seqs + 32 * W - 1) / (32 * W), s_beg = min(a.seqs, tid * chunk), s_end = min(a.seqs, s_beg + chunk);
     auto tiles_of = [&](const Q4Seq& q) {
         long long n = 0;
-        for (int rb = 0; rb * QA_ROWS < q.count * G; rb++) n += q4_span<TILE>(a, q, G, rb).tiles;
+        for (int rb = 0; rb * QA_ROWS < q.count * G; rb++) n += QA_START + q4_span<TILE>(a, q, G, rb).tiles;
         return n * nkv;
     };
     long long mine = 0;
@@ -156,7 +157,7 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
         if (w < warp) before += s_sum[w];
         total += s_sum[w];
     }
-    const long long grid = min((long long)gridDim.x, total);      // (every block up to `grid` has a tile)
+    const long long grid = min((long long)gridDim.x, total);
     Q4End* ends = reinterpret_cast<Q4End*>(reinterpret_cast<float*>(a.workspace) + (size_t)gridDim.x * 2 * q4_part_floats<HD>()) + blockIdx.x;
     if (blockIdx.x >= grid) {      // (the whole block)
         if (tid == 0) ends->ends = 0;
@@ -170,7 +171,7 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
             const long long n = tiles_of(q);
             if (at >= n) { at -= n; continue; }
             for (int rb = 0;; rb++) {
-                const int per = q4_span<TILE>(a, q, G, rb).tiles;
+                const int per = QA_START + q4_span<TILE>(a, q, G, rb).tiles;
                 if (at >= (long long)per * nkv) { at -= (long long)per * nkv; continue; }
                 s_item[0] = s;
                 s_item[1] = rb;
@@ -182,7 +183,7 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
         }
     }
     __syncthreads();
-    int s = s_item[0], rb = s_item[1], h = s_item[2], tile = s_item[3];
+    int s = s_item[0], rb = s_item[1], h = s_item[2], unit = s_item[3];
 
     const uint32_t ring = sm_u32(smem) + warp * QA_STAGES * St::BYTES;
     float* merge = reinterpret_cast<float*>(smem + Sm::RING);             // [W][8][HD + 4]
@@ -196,9 +197,28 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
     const unsigned n_pages = (unsigned)a.cache.n_pages;
     const int tile_pages = TILE / page_size, tile_rows = TILE - tile_pages * page_size;
     Q4Seq q = q4_seq(a, s, false);
+    bool first = true;      // no part of this block's yet
+    Q4End end{};
+    auto next_item = [&]() {
+        unit = 0;
+        if (++h == nkv) {
+            h = 0;
+            rb++;
+            while (rb * QA_ROWS >= q.count * G) {      // (there is one: the line goes on)
+                rb = 0;
+                q = q4_seq(a, ++s, false);
+            }
+        }
+    };
     for (long long cur = c0; cur < c1;) {
         const Q4Span sp = q4_span<TILE>(a, q, G, rb);
-        const int stop = (int)min((long long)sp.tiles, tile + (c1 - cur));
+        const int unit_end = (int)min((long long)sp.tiles + QA_START, unit + (c1 - cur)), tile = max(0, unit - QA_START), stop = max(0, unit_end - QA_START);
+        const long long start = cur - unit;      // the item's first unit
+        cur += unit_end - unit;
+        if (stop == tile) {                      // (nothing but units of the start)
+            if (cur < c1) next_item();
+            continue;
+        }
 
         // ---- query row g as operand; what scores of rows 2 c and 2 c + 1 need
         uint32_t qb[WORDS][2][2], ql[Q2 ? WORDS : 1][2][2];
@@ -388,21 +408,21 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
                     z[0][k] = z0 - top;
                     z[1][k] = z1 - top;
                     const float up = top == m[k] ? 0.0f : m[k] - top, was = mr[k] + up;
-                    float topv = fmaxf(z[0][k] + ex[0], z[1][k] + ex[1]);
+                    float topr = fmaxf(z[0][k] + ex[0], z[1][k] + ex[1]);
 #pragma unroll
-                    for (int o = 4; o <= 16; o <<= 1) topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, o));
-                    topv = fmaxf(topv, was);
-                    y[0][k] = z[0][k] + ex[0] - topv;
-                    y[1][k] = z[1][k] + ex[1] - topv;
+                    for (int o = 4; o <= 16; o <<= 1) topr = fmaxf(topr, __shfl_xor_sync(0xffffffffu, topr, o));
+                    topr = fmaxf(topr, was);
+                    y[0][k] = z[0][k] + ex[0] - topr;
+                    y[1][k] = z[1][k] + ex[1] - topr;
                     l[k] *= ex2(up);
-                    const float f = topv == was ? 1.0f : ex2(was - topv);
+                    const float f = topr == was ? 1.0f : ex2(was - topr);
 #pragma unroll
                     for (int i = 0; i < NT; i++) {
                         acc[i][k] *= f;
                         acc[i][k + 2] *= f;
                     }
                     m[k] = top;
-                    mr[k] = topv;
+                    mr[k] = topr;
                 }
             }
             if (!all) {      // (a row that has seen nothing yet has no reference, and a scale may be NaN)
@@ -477,20 +497,20 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
             }
         }
         __syncthreads();
-        const bool whole = tile == 0 && stop == sp.tiles, first = cur == c0;
+        const bool whole = tile == 0 && stop == sp.tiles;
         float* part = reinterpret_cast<float*>(a.workspace) + ((size_t)blockIdx.x * 2 + (first ? 0 : 1)) * q4_part_floats<HD>();
         for (int i = tid; i < QA_ROWS * (HD / 4); i += 32 * W) {
             const int row = i / (HD / 4), ch = (i % (HD / 4)) * 4;
-            float top = -INFINITY, topv = -INFINITY, sum = 0.0f;
+            float top = -INFINITY, topr = -INFINITY, sum = 0.0f;
 #pragma unroll
             for (int w = 0; w < W; w++) top = fmaxf(top, stat[(w * QA_ROWS + row) * 4]);
 #pragma unroll
-            for (int w = 0; w < W; w++) topv = fmaxf(topv, stat[(w * QA_ROWS + row) * 4 + 1] + below(stat[(w * QA_ROWS + row) * 4], top));
+            for (int w = 0; w < W; w++) topr = fmaxf(topr, stat[(w * QA_ROWS + row) * 4 + 1] + below(stat[(w * QA_ROWS + row) * 4], top));
             float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < W; w++) {
                 const float4 st = *reinterpret_cast<const float4*>(stat + (w * QA_ROWS + row) * 4), v = *reinterpret_cast<const float4*>(merge + (w * QA_ROWS + row) * (HD + 4) + ch);
-                const float d = below(st.x, top), f = ex2(below(st.y + d, topv));
+                const float d = below(st.x, top), f = ex2(below(st.y + d, topr));
                 sum += st.z * ex2(d);
                 o.x += v.x * f;
                 o.y += v.y * f;
@@ -501,7 +521,7 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
                 const int rr = rb * QA_ROWS + row;
                 if (rr < q.count * G) {
                     // (l = 0: the row saw nothing, and the sums are zeros)
-                    const float f = sum == 0.0f ? 0.0f : 1.0f / sum, e = topv == -INFINITY ? 0.0f : topv;
+                    const float f = sum == 0.0f ? 0.0f : 1.0f / sum, e = topr == -INFINITY ? 0.0f : topr;
                     const float v[4] = {o.x, o.y, o.z, o.w};
                     T* p = reinterpret_cast<T*>(a.out) + (q.first + rr / G) * a.out_token + (h * G + rr % G) * a.out_head + ch;
 #pragma unroll
@@ -509,42 +529,31 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
                 }
             } else {
                 *reinterpret_cast<float4*>(part + row * HD + ch) = o;
-                if (ch == 0) *reinterpret_cast<float4*>(part + QA_ROWS * HD + row * 4) = make_float4(top, topv, sum, 0.0f);
+                if (ch == 0) *reinterpret_cast<float4*>(part + QA_ROWS * HD + row * 4) = make_float4(top, topr, sum, 0.0f);
             }
         }
-        if (first && tid == 0) {
-            const long long start = cur - tile;
-            Q4End e{};
-            if (tile > 0 && stop == sp.tiles) {
-                e.first_cta = (int)(((start + 1) * grid - 1) / total);
-                e.first_slot = total * e.first_cta / grid < start;
-                e.seq = s;
-                e.rb = rb;
-                e.head = h;
-                e.ends = 1;
-            }
-            *ends = e;
+        if (first && tile > 0 && stop == sp.tiles) {      // (a part, and the last one)
+            // the block that has the first tile; this item is its first one unless its stretch begins ahead of the item
+            end.first_cta = (int)(((start + QA_START + 1) * grid - 1) / total);
+            end.first_slot = total * end.first_cta / grid < start;
+            end.seq = s;
+            end.rb = rb;
+            end.head = h;
+            end.ends = 1;
         }
+        first = false;
         __syncthreads();
-        // ---- on to the next item
-        cur += stop - tile;
-        tile = 0;
-        if (cur < c1 && ++h == nkv) {
-            h = 0;
-            rb++;
-            while (rb * QA_ROWS >= q.count * G) {      // (there is one: cur < total)
-                rb = 0;
-                q = q4_seq(a, ++s, false);
-            }
-        }
+        if (cur < c1) next_item();
     }
+    if (tid == 0) *ends = end;
 }
 
 // Joins the parts of the items that ended in a block's first stretch: block (x, y) = that block, a row.
-template <typename T, int HD> __global__ void __launch_bounds__(128) attention_q4_join_kernel(const b200_q4_attention a, int grid) {
+template <typename T, int HD> __global__ void __launch_bounds__(256) attention_q4_join_kernel(const b200_q4_attention a, int grid) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    constexpr int LANES = HD / 4, GROUPS = 128 / LANES, PART = q4_part_floats<HD>();
+    constexpr int LANES = HD / 4, GROUPS = 256 / LANES, PART = q4_part_floats<HD>(), AHEAD = 5;
     __shared__ __align__(16) float s_o[GROUPS][HD];
+    __shared__ float s_l[GROUPS];
     const float* ws = reinterpret_cast<const float*>(a.workspace);
     const Q4End e = reinterpret_cast<const Q4End*>(ws + (size_t)grid * 2 * PART)[blockIdx.x];
     if (!e.ends) return;
@@ -552,44 +561,61 @@ template <typename T, int HD> __global__ void __launch_bounds__(128) attention_q
     const Q4Seq q = q4_seq(a, e.seq, false);
     if (rr >= q.count * G) return;
     auto part = [&](int i) { return ws + ((size_t)(e.first_cta + i) * 2 + (i == 0 ? e.first_slot : 0)) * PART; };
-    float top = -INFINITY, topv = -INFINITY, sum = 0.0f;
+    // every group's first parts are asked for before anything waits
+    float4 st[AHEAD], v[AHEAD];
+    auto ask = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            const int i = i0 + u * GROUPS;
+            if (i < n) {
+                st[u] = *reinterpret_cast<const float4*>(part(i) + QA_ROWS * HD + row * 4);
+                v[u] = *reinterpret_cast<const float4*>(part(i) + row * HD + (tid % LANES) * 4);
+            }
+        }
+    };
+    ask(tid / LANES);
+    float top = -INFINITY, topr = -INFINITY, sum = 0.0f;
     // (a warp has both maxima by itself: no exchange between warps)
+#pragma unroll 4
     for (int i = lane; i < n; i += 32) {
-        const float2 st = *reinterpret_cast<const float2*>(part(i) + QA_ROWS * HD + row * 4);
+        const float2 x = *reinterpret_cast<const float2*>(part(i) + QA_ROWS * HD + row * 4);
         const float was = top;
-        top = fmaxf(top, st.x);
-        topv = fmaxf(topv + below(was, top), st.y + below(st.x, top));
+        top = fmaxf(top, x.x);
+        topr = fmaxf(topr + below(was, top), x.y + below(x.x, top));
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
-        const float x = __shfl_xor_sync(0xffffffffu, top, o), y = __shfl_xor_sync(0xffffffffu, topv, o), was = top;
+        const float x = __shfl_xor_sync(0xffffffffu, top, o), y = __shfl_xor_sync(0xffffffffu, topr, o), was = top;
         top = fmaxf(top, x);
-        topv = fmaxf(topv + below(was, top), y + below(x, top));
+        topr = fmaxf(topr + below(was, top), y + below(x, top));
     }
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int i = tid / LANES; i < n; i += GROUPS) {
-        const float4 st = *reinterpret_cast<const float4*>(part(i) + QA_ROWS * HD + row * 4), v = *reinterpret_cast<const float4*>(part(i) + row * HD + (tid % LANES) * 4);
-        const float d = below(st.x, top), f = ex2(below(st.y + d, topv));
-        sum += st.z * ex2(d);
-        o.x += v.x * f;
-        o.y += v.y * f;
-        o.z += v.z * f;
-        o.w += v.w * f;
+    for (int i0 = tid / LANES; i0 < n; i0 += AHEAD * GROUPS) {
+        if (i0 >= AHEAD * GROUPS) ask(i0);
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++)
+            if (i0 + u * GROUPS < n) {
+                const float d = below(st[u].x, top), f = ex2(below(st[u].y + d, topr));
+                sum += st[u].z * ex2(d);
+                o.x += v[u].x * f;
+                o.y += v[u].y * f;
+                o.z += v[u].z * f;
+                o.w += v[u].w * f;
+            }
     }
     *reinterpret_cast<float4*>(&s_o[tid / LANES][(tid % LANES) * 4]) = o;
-    __shared__ float s_l[GROUPS];
     if (tid % LANES == 0) s_l[tid / LANES] = sum;
     __syncthreads();
     if (tid < HD) {
-        float v = 0.0f, l = 0.0f;
+        float x = 0.0f, l = 0.0f;
 #pragma unroll
         for (int k = 0; k < GROUPS; k++) {
-            v += s_o[k][tid];
+            x += s_o[k][tid];
             l += s_l[k];
         }
-        const float x = topv == -INFINITY ? 0.0f : topv;
+        const float r = topr == -INFINITY ? 0.0f : topr;
         reinterpret_cast<T*>(a.out)[(q.first + rr / G) * a.out_token + (e.head * G + rr % G) * a.out_head + tid] =
-            from_f<T>(l == 0.0f ? 0.0f : ldexpf(v * (1.0f / l), (int)floorf(x)) * ex2(x - floorf(x)));
+            from_f<T>(l == 0.0f ? 0.0f : ldexpf(x * (1.0f / l), (int)floorf(r)) * ex2(r - floorf(r)));
     }
 }
 
@@ -598,7 +624,7 @@ constexpr int QA_W = 4;      // warps of a block
 // blocks of the first kernel: as many as run at once on 148 SMs, fewer where even one tile each could not be found
 inline int attention_q4_grid(const b200_q4_attention& a) {
     const int64_t G = a.n_heads / a.cache.n_kv_heads, blocks = (a.tokens * G + QA_ROWS - 1) / QA_ROWS + a.seqs;
-    const int64_t tiles = blocks * a.cache.n_kv_heads * (((int64_t)a.table_pages * a.cache.page_size + 16 * QA_W - 1) / (16 * QA_W) + 1);
+    const int64_t tiles = blocks * a.cache.n_kv_heads * (((int64_t)a.table_pages * a.cache.page_size + 16 * QA_W - 1) / (16 * QA_W) + 1 + QA_START);
     return (int)std::min<int64_t>(148 * (16 / QA_W), tiles);
 }
 inline size_t attention_q4_workspace(const b200_q4_attention& a) {
@@ -617,7 +643,7 @@ template <typename T, int HD> cudaError_t attention_q4(const b200_q4_attention& 
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid, QA_ROWS);
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
