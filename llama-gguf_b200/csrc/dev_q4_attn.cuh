@@ -24,7 +24,7 @@
 
 namespace dev {
 
-enum { QA_ROWS = 8, QA_STAGES = 4, QA_START = 4 };
+enum { QA_ROWS = 8, QA_START = 4 };
 
 struct Q4Seq {
     int first, count;      // query tokens
@@ -117,14 +117,14 @@ template <int HD> struct Q4Stage {
 };
 __device__ __forceinline__ int q4_piece(int row, int q) { return (((row & 1) | ((row >> 3) & 1) << 1 | (q >> 1) << 2) << 3) | (q & 1) | ((row >> 1) & 3) << 1; }
 
-template <typename T, int HD, int W> struct Q4Smem {
-    static constexpr int TILE = 16 * W, RING = W * QA_STAGES * Q4Stage<HD>::BYTES, MERGE = W * QA_ROWS * (HD + 4) * 4 + W * QA_ROWS * 16, BYTES = RING + MERGE;
+template <int HD, int W, int U> struct Q4Smem {
+    static constexpr int TILE = 16 * W * U, STAGES = U == 1 ? 4 : 3, RING = W * STAGES * U * Q4Stage<HD>::BYTES, MERGE = W * QA_ROWS * (HD + 4) * 4 + W * QA_ROWS * 16, BYTES = RING + MERGE;
 };
 
-template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 16 / W) attention_q4_kernel(const b200_q4_attention a, uint64_t page16) {
+template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32 * W, U == 1 ? 16 / W : 12 / W) attention_q4_kernel(const b200_q4_attention a, uint64_t page16) {
     using St = Q4Stage<HD>;
-    using Sm = Q4Smem<T, HD, W>;
-    constexpr int TILE = Sm::TILE, WORDS = HD / 32, NT = HD / 16;      // words of a key row per lane; row tiles of the values
+    using Sm = Q4Smem<HD, W, U>;
+    constexpr int STAGES = Sm::STAGES, TILE = Sm::TILE, WORDS = HD / 32, NT = HD / 16;      // words of a key row per lane; row tiles of the values
     constexpr bool Q2 = sizeof(T) == 4, P2 = !std::is_same<T, __nv_bfloat16>::value;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -185,7 +185,7 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
     __syncthreads();
     int s = s_item[0], rb = s_item[1], h = s_item[2], unit = s_item[3];
 
-    const uint32_t ring = sm_u32(smem) + warp * QA_STAGES * St::BYTES;
+    const uint32_t ring = sm_u32(smem) + warp * STAGES * U * St::BYTES;
     float* merge = reinterpret_cast<float*>(smem + Sm::RING);             // [W][8][HD + 4]
     float* stat = merge + W * QA_ROWS * (HD + 4);                         // [W][8][4]
     // where this lane's words of a stage are: keys of positions g and g + 8; values of positions 2 c + (0, 1, 8, 9), words g and g + 8
@@ -287,13 +287,19 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
         // ---- the ring.  The page of a step is looked up one step before its rows are asked for.
         const int32_t* table = a.page_table + (int64_t)s * a.table_stride;
         const uint8_t* mine_k = reinterpret_cast<const uint8_t*>(a.cache.data) + (int64_t)h * block + lane * 16;
-        int p_look = sp.base + tile * TILE + warp * 16, index = (int)(((uint64_t)(p_look >> 4) * page16) >> 36), row_look = p_look - index * page_size;
-        int p_fetch = p_look, page = 0, row = 0;
+        int p_look = sp.base + tile * TILE + warp * 16 * U, index = (int)(((uint64_t)(p_look >> 4) * page16) >> 36), row_look = p_look - index * page_size;
+        int p_fetch = p_look, page[U], row[U];
         const int p_stop = min(sp.hi, sp.base + stop * TILE);
         bool odd_page = false;      // a page that is none of the cache's came by in this item
+#pragma unroll
+        for (int b = 0; b < U; b++) page[b] = row[b] = 0;
         auto look = [&]() {
-            if (p_look < p_stop) page = table[index];
-            row = row_look;
+#pragma unroll
+            for (int b = 0; b < U; b++) {
+                const bool over = row_look + 16 * b >= page_size;
+                row[b] = row_look + 16 * b - (over ? page_size : 0);
+                if (p_look + 16 * b < p_stop) page[b] = table[index + over];
+            }
             p_look += TILE;
             index += tile_pages;
             row_look += tile_rows;
@@ -303,45 +309,50 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
             }
         };
         auto fetch = [&](int stage) {
-            if (p_fetch < p_stop) {
-                if ((unsigned)page >= n_pages) {      // (masked below)
-                    odd_page = true;
-                    page = 0;
-                    if (a.status && lane == 0) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
-                }
-                const uint8_t* k = mine_k + (int64_t)page * page_bytes + row * St::ROW;
-                const uint32_t at = ring + stage * St::BYTES;
 #pragma unroll
-                for (int i = 0; i < 16 * P; i += 32) {
-                    cp16(at + lane * 16 + i * 16, k + i * 16);
-                    cp16(at + v_to + q4_piece(i / P, 0) * 16, k + v_off + i * 16);
+            for (int b = 0; b < U; b++)
+                if (p_fetch + 16 * b < p_stop) {
+                    if ((unsigned)page[b] >= n_pages) {      // (masked below)
+                        odd_page = true;
+                        page[b] = 0;
+                        if (a.status && lane == 0) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
+                    }
+                    const uint8_t* k = mine_k + (int64_t)page[b] * page_bytes + row[b] * St::ROW;
+                    const uint32_t at = ring + (stage * U + b) * St::BYTES;
+#pragma unroll
+                    for (int i = 0; i < 16 * P; i += 32) {
+                        cp16(at + lane * 16 + i * 16, k + i * 16);
+                        cp16(at + v_to + q4_piece(i / P, 0) * 16, k + v_off + i * 16);
+                    }
+                    // (lanes 0-3 key scales, 4-7 value scales, which follow page_size floats later: lane * 16 is in k, 64 of it too much for those)
+                    if (lane < 8) cp16(at + St::KS + lane * 16, k - row[b] * (St::ROW - 4) + s_off);
                 }
-                // (lanes 0-3 key scales, 4-7 value scales, which follow page_size floats later: lane * 16 is in k, 64 of it too much for those)
-                if (lane < 8) cp16(at + St::KS + lane * 16, k - row * (St::ROW - 4) + s_off);
-            }
             cp_commit();
             p_fetch += TILE;
         };
         look();
 #pragma unroll
-        for (int i = 0; i < QA_STAGES - 1; i++) {
+        for (int i = 0; i < STAGES - 1; i++) {
             fetch(i);
             look();
         }
-        int stage = 0;
+        int stage = 0, stage_to = STAGES - 1;
         uint32_t magic = 0x64006400u;
         asm("" : "+r"(magic));      // (kept in a register: an instruction has room for one constant)
-        for (int p0 = sp.base + tile * TILE + warp * 16; p0 < p_stop; p0 += TILE) {
-            cp_wait<QA_STAGES - 2>();
+        for (int p0 = sp.base + tile * TILE + warp * 16 * U; p0 < p_stop; p0 += TILE) {
+            cp_wait<STAGES - 2>();
             __syncwarp();
-            fetch((stage + QA_STAGES - 1) & (QA_STAGES - 1));
+            fetch(stage_to);
             look();
-            const uint32_t at = ring + stage * St::BYTES;
-            stage = (stage + 1) & (QA_STAGES - 1);
-            // scores: [position g, g + 8][row 2 c, 2 c + 1]
-            float z[2][2];
-            uint32_t vs[2];
-            {
+            const uint32_t at0 = ring + stage * U * St::BYTES;
+            stage_to = stage;
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
+            // scores: [16 positions][position g, g + 8][row 2 c, 2 c + 1]
+            float z[U][2][2];
+            uint32_t vs[U][2];
+#pragma unroll
+            for (int b = 0; b < U; b++) {
+                const uint32_t at = at0 + b * St::BYTES;
                 uint32_t w[2][WORDS], ks[2][1];
                 float d[4];
 #pragma unroll
@@ -351,7 +362,7 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
                     uint32_t v[1];
                     lds<1>(ks[u], at + St::KS + (8 * u + g) * 4);
                     lds<1>(v, at + St::VS + (8 * u + g) * 4);
-                    vs[u] = v[0];
+                    vs[b][u] = v[0];
                 }
 #pragma unroll
                 for (int j = 0; j < WORDS; j++)
@@ -365,57 +376,62 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int k = 0; k < 2; k++) z[u][k] = (fmaf(d[2 * u + k], 1024.0f, -q8[k]) * alpha[k]) * __uint_as_float(ks[u][0]);
+                    for (int k = 0; k < 2; k++) z[b][u][k] = (fmaf(d[2 * u + k], 1024.0f, -q8[k]) * alpha[k]) * __uint_as_float(ks[u][0]);
             }
-            const float zs[2][2] = {{z[0][0], z[0][1]}, {z[1][0], z[1][1]}};
-            const bool all = !odd_page && p0 >= lo_max && p0 + 16 <= hi_min;
-            uint32_t in = 0xfu;
-            if (!all) {
-                in = 0;
-                const bool there = (unsigned)table[(int)(((uint64_t)(p0 >> 4) * page16) >> 36)] < n_pages;
+            const bool all = !odd_page && p0 >= lo_max && p0 + 16 * U <= hi_min;
+            uint32_t hidden = 0;      // bit 4 b + 2 u + k
+            if (!all) {               // (uniform)
 #pragma unroll
-                for (int u = 0; u < 2; u++)
+                for (int b = 0; b < U; b++) {
+                    // (a block of 16 behind the stop was not fetched)
+                    const bool there = p0 + 16 * b < p_stop && (unsigned)table[(int)(((uint64_t)((p0 + 16 * b) >> 4) * page16) >> 36)] < n_pages;
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const int j = p0 + 8 * u + g;
-                        if (there && j >= lo[k] && j < hi[k]) in |= 1u << (2 * u + k);
-                        else z[u][k] = -INFINITY;
+                    for (int u = 0; u < 2; u++) {
+                        const int j = p0 + 16 * b + 8 * u + g;
+                        // (a scale of a position that nobody sees may be NaN)
+                        if (!there || !((j >= lo[0] && j < hi[0]) || (j >= lo[1] && j < hi[1]))) vs[b][u] = 0;
+#pragma unroll
+                        for (int k = 0; k < 2; k++)
+                            if (!there || j < lo[k] || j >= hi[k]) {
+                                z[b][u][k] = -INFINITY;
+                                hidden |= 1u << (4 * b + 2 * u + k);
+                            }
                     }
-            }
-            auto score = [&](int u, int k) { return (in >> (2 * u + k)) & 1u ? zs[u][k] : -INFINITY; };
-            float y[2][2], ex[2];      // z becomes log2 p, y is log2 of the weight's magnitude
-            bool past = false;
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                // (a scale of zero: as 2^-1000, which leaves nothing of it; NaN stays)
-                asm("{\n\t.reg .f32 t;\n\tlg2.approx.f32 t, %1;\n\tmax.NaN.f32 %0, t, 0fC47A0000;\n\t}" : "=f"(ex[u]) : "f"(fabsf(__uint_as_float(vs[u]))));
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    z[u][k] -= m[k];
-                    y[u][k] = z[u][k] + ex[u] - mr[k];
-                    past |= z[u][k] > 8.0f || y[u][k] > 8.0f;
                 }
             }
+            float x[U][2][2], y[U][2][2], ex[U][2];      // log2 p, log2 of the weight's magnitude, log2 of the value's scale
+            bool past = false;
+#pragma unroll
+            for (int b = 0; b < U; b++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    // (a scale of zero: as 2^-1000, which leaves nothing of it; NaN stays)
+                    asm("{\n\t.reg .f32 t;\n\tlg2.approx.f32 t, %1;\n\tmax.NaN.f32 %0, t, 0fC47A0000;\n\t}" : "=f"(ex[b][u]) : "f"(fabsf(__uint_as_float(vs[b][u]))));
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        x[b][u][k] = z[b][u][k] - m[k];
+                        y[b][u][k] = x[b][u][k] + (ex[b][u] - mr[k]);
+                        past |= x[b][u][k] > 8.0f || y[b][u][k] > 8.0f;
+                    }
+                }
             if (__any_sync(0xffffffffu, past)) {
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    // (the differences are taken again from the scores: a first step has no finite reference)
-                    const float z0 = score(0, k), z1 = score(1, k);
-                    float top = fmaxf(z0, z1);
+                    float top = z[0][0][k];
+#pragma unroll
+                    for (int b = 0; b < U; b++) top = fmaxf(top, fmaxf(z[b][0][k], z[b][1][k]));
 #pragma unroll
                     for (int o = 4; o <= 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                     top = fmaxf(top, m[k]);
-                    z[0][k] = z0 - top;
-                    z[1][k] = z1 - top;
-                    const float up = top == m[k] ? 0.0f : m[k] - top, was = mr[k] + up;
-                    float topr = fmaxf(z[0][k] + ex[0], z[1][k] + ex[1]);
+                    const float up = below(m[k], top), was = mr[k] + up;
+                    float topr = -INFINITY;
+#pragma unroll
+                    for (int b = 0; b < U; b++) topr = fmaxf(topr, fmaxf(z[b][0][k] - top + ex[b][0], z[b][1][k] - top + ex[b][1]));
 #pragma unroll
                     for (int o = 4; o <= 16; o <<= 1) topr = fmaxf(topr, __shfl_xor_sync(0xffffffffu, topr, o));
                     topr = fmaxf(topr, was);
-                    y[0][k] = z[0][k] + ex[0] - topr;
-                    y[1][k] = z[1][k] + ex[1] - topr;
                     l[k] *= ex2(up);
-                    const float f = topr == was ? 1.0f : ex2(was - topr);
+                    const float f = ex2(below(was, topr));
 #pragma unroll
                     for (int i = 0; i < NT; i++) {
                         acc[i][k] *= f;
@@ -423,61 +439,71 @@ template <typename T, int HD, int W> __global__ void __launch_bounds__(32 * W, 1
                     }
                     m[k] = top;
                     mr[k] = topr;
-                }
-            }
-            if (!all) {      // (a row that has seen nothing yet has no reference, and a scale may be NaN)
 #pragma unroll
-                for (int u = 0; u < 2; u++)
+                    for (int b = 0; b < U; b++)
 #pragma unroll
-                    for (int k = 0; k < 2; k++)
-                        if (!((in >> (2 * u + k)) & 1u)) {
-                            z[u][k] = y[u][k] = -INFINITY;
+                        for (int u = 0; u < 2; u++) {
+                            x[b][u][k] = z[b][u][k] - top;
+                            y[b][u][k] = x[b][u][k] + (ex[b][u] - topr);
                         }
-            }
-            uint32_t pb[2], pl[2];      // the weights of positions 2 c, 2 c + 1 (+ 8) for row g, and what their fp16 leave over
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                float w[2];
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const float p = ex2(z[u][k]);
-                    w[k] = __uint_as_float(__float_as_uint(ex2(y[u][k])) ^ (vs[u] & 0x80000000u));
-                    l[k] += p;
                 }
-                pb[u] = pack_h2(w[0], w[1]);
-                if (P2) {
-                    const float2 b = unpack_h2(pb[u]);
-                    pl[u] = transposed8x8(pack_h2(w[0] - b.x, w[1] - b.y));
-                }
-                pb[u] = transposed8x8(pb[u]);
             }
-            // values: [positions 2 c, 2 c + 1; + 8][word g, word g + 8], channels 0-3 and 4-7 of the word
-            uint32_t t[HD / 64][2][2];
+            if (!all) {      // (a row that has seen nothing yet has no reference, and a scale that another row sees may be NaN)
 #pragma unroll
-            for (int half = 0; half < HD / 64; half++)
+                for (int b = 0; b < U; b++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int k = 0; k < 2; k++)
+                            if ((hidden >> (4 * b + 2 * u + k)) & 1u) x[b][u][k] = y[b][u][k] = -INFINITY;
+            }
+#pragma unroll
+            for (int b = 0; b < U; b++) {
+                const uint32_t at = at0 + b * St::BYTES;
+                uint32_t pb[2], pl[2];      // the weights of positions 2 c, 2 c + 1 (+ 8) for row g, and what their fp16 leave over
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    uint32_t w0[1], w1[1];
-                    lds<1>(w0, at + v_at + q4_piece(8 * u, 2 * half) * 16);
-                    lds<1>(w1, at + v_at + q4_piece(8 * u + 1, 2 * half) * 16);
-                    t[half][u][0] = __byte_perm(w0[0], w1[0], 0x5410);
-                    t[half][u][1] = __byte_perm(w0[0], w1[0], 0x7632);
-                }
-            // nibble i of its word; odd ones 16 times too large, which is put right at the end
-            auto nibble = [&](int half, int u, int i) {
-                const uint32_t v = (i & 2) ? t[half][u][i >> 2] >> 8 : t[half][u][i >> 2];
-                return sub_h2(masked_or(v, (i & 1) ? 0x00f000f0u : 0x000f000fu, magic), (i & 1) ? 0x64806480u : 0x64086408u);
-            };
+                    float w[2];
 #pragma unroll
-            for (int i = 0; i < NT; i++) {
-                uint32_t v[4];      // rows g of the tile: word g, nibble i; rows g + 8: word g + 8 (hd 64: nibble i + 4)
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    v[2 * u] = nibble(0, u, i);
-                    v[2 * u + 1] = HD == 128 ? nibble(HD / 64 - 1, u, i) : nibble(0, u, i + 4);
+                    for (int k = 0; k < 2; k++) {
+                        l[k] += ex2(x[b][u][k]);
+                        w[k] = __uint_as_float(__float_as_uint(ex2(y[b][u][k])) ^ (vs[b][u] & 0x80000000u));
+                    }
+                    pb[u] = pack_h2(w[0], w[1]);
+                    if (P2) {
+                        const float2 f = unpack_h2(pb[u]);
+                        pl[u] = transposed8x8(pack_h2(w[0] - f.x, w[1] - f.y));
+                    }
+                    pb[u] = transposed8x8(pb[u]);
                 }
-                mma16(acc[i], v[0], v[1], v[2], v[3], pb[0], pb[1]);
-                if (P2) mma16(acc[i], v[0], v[1], v[2], v[3], pl[0], pl[1]);
+                // values: [positions 2 c, 2 c + 1; + 8][word g, word g + 8], channels 0-3 and 4-7 of the word
+                uint32_t t[HD / 64][2][2];
+#pragma unroll
+                for (int half = 0; half < HD / 64; half++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        uint32_t w0[1], w1[1];
+                        lds<1>(w0, at + v_at + q4_piece(8 * u, 2 * half) * 16);
+                        lds<1>(w1, at + v_at + q4_piece(8 * u + 1, 2 * half) * 16);
+                        t[half][u][0] = __byte_perm(w0[0], w1[0], 0x5410);
+                        t[half][u][1] = __byte_perm(w0[0], w1[0], 0x7632);
+                    }
+                // nibble i of its word; odd ones 16 times too large, which is put right at the end
+                auto nibble = [&](int half, int u, int i) {
+                    const uint32_t v = (i & 2) ? t[half][u][i >> 2] >> 8 : t[half][u][i >> 2];
+                    return sub_h2(masked_or(v, (i & 1) ? 0x00f000f0u : 0x000f000fu, magic), (i & 1) ? 0x64806480u : 0x64086408u);
+                };
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    uint32_t v[4];      // rows g of the tile: word g, nibble i; rows g + 8: word g + 8 (hd 64: nibble i + 4)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        v[2 * u] = nibble(0, u, i);
+                        v[2 * u + 1] = HD == 128 ? nibble(HD / 64 - 1, u, i) : nibble(0, u, i + 4);
+                    }
+                    mma16(acc[i], v[0], v[1], v[2], v[3], pb[0], pb[1]);
+                    if (P2) mma16(acc[i], v[0], v[1], v[2], v[3], pl[0], pl[1]);
+                }
             }
         }
         cp_wait<0>();
@@ -620,21 +646,21 @@ template <typename T, int HD> __global__ void __launch_bounds__(256) attention_q
 }
 
 // ------------------------------------------------------------------------------------------------------------------- host
-constexpr int QA_W = 4;      // warps of a block
+constexpr int QA_W = 4, QA_U = 2;      // warps of a block, 16 positions a warp takes at a time
 // blocks of the first kernel: as many as run at once on 148 SMs, fewer where even one tile each could not be found
 inline int attention_q4_grid(const b200_q4_attention& a) {
     const int64_t G = a.n_heads / a.cache.n_kv_heads, blocks = (a.tokens * G + QA_ROWS - 1) / QA_ROWS + a.seqs;
-    const int64_t tiles = blocks * a.cache.n_kv_heads * (((int64_t)a.table_pages * a.cache.page_size + 16 * QA_W - 1) / (16 * QA_W) + 1 + QA_START);
-    return (int)std::min<int64_t>(148 * (16 / QA_W), tiles);
+    const int64_t tiles = blocks * a.cache.n_kv_heads * (((int64_t)a.table_pages * a.cache.page_size + 16 * QA_W * QA_U - 1) / (16 * QA_W * QA_U) + 1 + QA_START);
+    return (int)std::min<int64_t>(148 * (QA_U == 1 ? 16 / QA_W : 12 / QA_W), tiles);
 }
 inline size_t attention_q4_workspace(const b200_q4_attention& a) {
     const size_t grid = (size_t)attention_q4_grid(a), part = QA_ROWS * (a.cache.head_dim + 4) * 4;
     return grid * (2 * part + sizeof(Q4End));
 }
 template <typename T, int HD> cudaError_t attention_q4(const b200_q4_attention& a, cudaStream_t st) {
-    using Sm = Q4Smem<T, HD, QA_W>;
+    using Sm = Q4Smem<HD, QA_W, QA_U>;
     static SmemAllowed allowed;
-    const auto kernel = attention_q4_kernel<T, HD, QA_W>;
+    const auto kernel = attention_q4_kernel<T, HD, QA_W, QA_U>;
     cudaError_t e = allowed((const void*)kernel, Sm::BYTES);
     if (e != cudaSuccess) return e;
     const uint64_t d = (uint64_t)a.cache.page_size / 16, page16 = (((uint64_t)1 << 36) + d - 1) / d;      // n / d = n * page16 >> 36 for n < 2^27
