@@ -586,6 +586,9 @@ B200_API int b200_dev_watchdog(int device, int* out);
 B200_API int b200_dev_add_rms_norm_q8(int device, void* stream, uint32_t type, const void* x, int64_t ldx, const void* residual, int64_t ldr,
                                       void* sum, int64_t lds, const float* weight, float eps, int8_t* q, int64_t ldq, float* scales,
                                       int64_t rows, int64_t hidden);
+/* The values that rows in 8 bits stand for: out[row][i] = scales[row] * q[row][i], rounded to the type. */
+B200_API int b200_dev_read_q8(int device, void* stream, uint32_t type, const int8_t* q, int64_t ldq, const float* scales, void* out, int64_t ldo, int64_t rows,
+                              int64_t n);
 /* Product of 8-bit integers: out[t][n] = a_scales[t] * w_scales[n] * sum_k a[t][k] w[n][k] (+ bias[n]); sums in s32 (exact: k <= 131071),
  * then f32: ((float)sum * a_scale) * w_scale + bias, rounded to out_type.  a and w start on 16 bytes and their rows are a multiple of 16 bytes apart; what lies
  * between k and the next row is not used. */

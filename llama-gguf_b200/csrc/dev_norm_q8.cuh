@@ -1,5 +1,7 @@
 // dev_norm_q8.cuh — RMS norm of a residual sum with the result in 8 bits and a scale per row (b200_dev_add_rms_norm_q8).
 #pragma once
+#include <algorithm>
+
 #include "dev_common.cuh"
 
 namespace dev {
@@ -164,6 +166,35 @@ template <typename T> cudaError_t add_rms_norm_q8(const NormQ8Args& a, cudaStrea
     const int n = a.hidden / E, few = a.rows <= 296;
     const int v = n > 2048 || (!few && n >= 256) ? 4 : n > 1024 || (!few && n >= 128) ? 2 : 1, threads = ((n + v - 1) / v + 31) / 32 * 32;
     return v == 4 ? add_rms_norm_q8_words<T, 4>(a, threads, st) : v == 2 ? add_rms_norm_q8_words<T, 2>(a, threads, st) : add_rms_norm_q8_words<T, 1>(a, threads, st);
+}
+
+// Rows in 8 bits as values: sixteen neighbours per thread and step, or one where rows are not on 16 bytes.  Blocks (x) along a row, (y) over rows.
+struct ReadQ8Args {
+    const int8_t* q;
+    const float* scales;
+    void* out;
+    int64_t ldq, ldo, rows, n;
+};
+template <typename T, int E> __global__ void __launch_bounds__(256) read_q8_kernel(const ReadQ8Args a) {
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        const float s = a.scales[row];
+        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * E; i < a.n; i += (int64_t)gridDim.x * 256 * E) {
+            struct __align__(E) W { int8_t v[E]; };
+            const W w = *reinterpret_cast<const W*>(a.q + row * a.ldq + i);
+            float f[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) f[e] = (float)w.v[e] * s;
+            store_n<T, E, (E > 1)>(reinterpret_cast<T*>(a.out) + row * a.ldo + i, f);
+        }
+    }
+}
+template <typename T> cudaError_t read_q8(const ReadQ8Args& a, cudaStream_t st) {
+    const bool words = a.n % 16 == 0 && !((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) & 15) && a.ldq % 16 == 0 && a.ldo * sizeof(T) % 16 == 0;
+    const int64_t per = words ? 4096 : 256;
+    const dim3 grid((unsigned)std::min<int64_t>((a.n + per - 1) / per, 1024), (unsigned)std::min<int64_t>(a.rows, 16384));
+    if (words) read_q8_kernel<T, 16><<<grid, 256, 0, st>>>(a);
+    else read_q8_kernel<T, 1><<<grid, 256, 0, st>>>(a);
+    return cudaGetLastError();
 }
 
 }  // namespace dev

@@ -95,6 +95,19 @@ extern "C" int b200_dev_add_rms_norm_q8(int device, void* stream, uint32_t type,
     });
 }
 
+extern "C" int b200_dev_read_q8(int device, void* stream, uint32_t type, const int8_t* q, int64_t ldq, const float* scales, void* out, int64_t ldo, int64_t rows, int64_t n) {
+    const char* op = "read_q8";
+    return entry(op, [&]() -> int {
+        if (!type_bytes(type)) return bad_type(op, type);
+        if (rows < 0 || rows >= kMost || n < 1 || n >= kMost) return shape(op, "0 <= rows < 2^31 and 1 <= n < 2^31 expected");
+        if (ldq < 0 || ldo < n) return shape(op, "negative distance, or rows of an output overlap");
+        if (rows == 0) return B200_OK;
+        if (!q || !scales || !out) return bad(op, "null pointer");
+        const ReadQ8Args a{q, scales, out, ldq, ldo, rows, n};
+        return on_device(op, device, [&] { return by_type(type, [&](auto t) { return read_q8<decltype(t)>(a, (cudaStream_t)stream); }); });
+    });
+}
+
 extern "C" int b200_dev_mat_mat_i8(int device, void* stream, uint32_t out_type, const int8_t* a, int64_t lda, const float* a_scales, const int8_t* w, int64_t ldw,
                                    const float* w_scales, const float* bias, void* out, int64_t ldo, int64_t t_rows, int64_t k, int64_t n) {
     const char* op = "mat_mat_i8";

@@ -32,6 +32,19 @@ def test_norm_refusals(b200, D):
     assert D._lib().b200_dev_add_rms_norm_q8(*{**good, "rows": 0, "x": None}.values()) == 0
 
 
+def test_values_refusals(b200, D):
+    good = dict(device=0, stream=None, type=0, q=AT, ldq=64, s=AT, out=AT, ldo=64, rows=2, n=64)
+    for change, exc, words in [(dict(type=9), b200.UnsupportedDType, "type 9"), (dict(rows=-1), b200.ShapeMismatch, "rows"), (dict(n=0), b200.ShapeMismatch, "n"),
+                               (dict(ldo=63), b200.ShapeMismatch, "overlap"), (dict(ldq=-1), b200.ShapeMismatch, "negative"), (dict(s=None), b200.InvalidArgument, "null")]:
+        refused(b200, D._lib().b200_dev_read_q8(*{**good, **change}.values()), exc, words)
+    with pytest.raises(b200.DTypeMismatch):
+        D.read_q8(torch.zeros(2, 3), torch.ones(2))
+    with pytest.raises(b200.ShapeMismatch):
+        D.read_q8(torch.zeros(2, 3, dtype=torch.int8), torch.ones(3))
+    with pytest.raises(TypeError):
+        D.read_q8([1, 2], torch.ones(2))
+
+
 def test_product_refusals(b200, D):
     good = dict(device=0, stream=None, type=0, a=AT, lda=64, s=AT, w=AT, ldw=64, ws=AT, bias=None, out=AT, ldo=8, t=2, k=64, n=8)
     for change, exc, words in [

@@ -84,6 +84,21 @@ def test_norm_of_rows_that_are_zero_tiny_or_not_finite(D):
     assert D.add_rms_norm_q8(x[:0].cuda(), torch.ones(260).cuda(), 1e-6)[0].shape == (0, 260)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n", [(1, 1), (3, 31), (5, 4096), (700, 48), (2, 70000)])
+def test_values_of_rows_in_8_bits(D, dtype, rows, n):
+    q, s = torch.randint(-128, 128, (rows, n), dtype=torch.int8).cuda(), (0.01 * normal(3, rows)).cuda()
+    s[rows // 2] = math.nan
+    want = q.double() * s.double()[:, None]
+    got = D.read_q8(q, s, dtype)
+    assert got.dtype == dtype and torch.equal(torch.isnan(got), torch.isnan(want))
+    # the product to f32, that to the type
+    tol = (1.001 * 2.0**-24 + (1.001 * R.HALF_STEP[dtype] if dtype != torch.float32 else 0)) * want.abs() + R.LEAST[dtype]
+    assert (torch.nan_to_num((got.double() - want).abs()) <= torch.nan_to_num(tol)).all()
+    wide = torch.randint(-128, 128, (rows, n + 21), dtype=torch.int8).cuda()[:, 5 : 5 + n]
+    assert torch.equal(torch.nan_to_num(D.read_q8(wide, s, dtype)), torch.nan_to_num(D.read_q8(wide.contiguous(), s, dtype)))
+
+
 # ---------------------------------------------------------------------------------------------------------------- product
 def bytes_of(seed, rows, k, extra=0):
     g = torch.Generator().manual_seed(seed)
