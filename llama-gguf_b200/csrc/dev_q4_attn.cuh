@@ -30,7 +30,8 @@ struct Q4Seq {
     int first, count;      // query tokens
     int64_t len;           // cached positions
 };
-__device__ __forceinline__ Q4Seq q4_seq(const b200_q4_attention& a, int s, bool report) {
+// a sequence's query tokens (none where the tokens do not lie within the call's, or there are more than `limit` rows)
+__device__ __forceinline__ Q4Seq q4_seq(const b200_q4_attention& a, int s, bool report, int64_t limit = INT64_MAX) {
     Q4Seq q;
     const int64_t b = a.q_starts ? a.q_starts[s] : s, e = a.q_starts ? a.q_starts[s + 1] : s + 1, cap = (int64_t)a.table_pages * a.cache.page_size;
     q.len = a.kv_lens[s];
@@ -38,7 +39,7 @@ __device__ __forceinline__ Q4Seq q4_seq(const b200_q4_attention& a, int s, bool 
     if (report && a.status && (wrong || q.len < 0 || q.len > cap)) atomicOr(a.status, (int)B200_STATUS_BAD_LENGTH);
     q.len = q.len < 0 ? 0 : q.len > cap ? cap : q.len;
     q.first = wrong ? 0 : (int)b;
-    q.count = wrong ? 0 : (int)(e - b);
+    q.count = wrong || (e - b) * (a.n_heads / a.cache.n_kv_heads) > limit ? 0 : (int)(e - b);
     return q;
 }
 // positions [base, hi) that the rows of block rb see, in `tiles` tiles; rows that see nothing have one tile all the same (it writes their zeros)
@@ -121,7 +122,7 @@ template <int HD, int W, int U> struct Q4Smem {
     static constexpr int TILE = 16 * W * U, STAGES = U == 1 ? 4 : 3, RING = W * STAGES * U * Q4Stage<HD>::BYTES, MERGE = W * QA_ROWS * (HD + 4) * 4 + W * QA_ROWS * 16, BYTES = RING + MERGE;
 };
 
-template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32 * W, U == 1 ? 16 / W : 12 / W) attention_q4_kernel(const b200_q4_attention a, uint64_t page16) {
+template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32 * W, U == 1 ? 16 / W : 12 / W) attention_q4_kernel(const b200_q4_attention a, uint64_t page16, int64_t limit) {
     using St = Q4Stage<HD>;
     using Sm = Q4Smem<HD, W, U>;
     constexpr int STAGES = Sm::STAGES, TILE = Sm::TILE, WORDS = HD / 32, NT = HD / 16;      // words of a key row per lane; row tiles of the values
@@ -141,7 +142,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
         return n * nkv;
     };
     long long mine = 0;
-    for (int s = s_beg; s < s_end; s++) mine += tiles_of(q4_seq(a, s, blockIdx.x == 0));
+    for (int s = s_beg; s < s_end; s++) mine += tiles_of(q4_seq(a, s, blockIdx.x == 0, limit));
     long long before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -167,7 +168,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
     if (before <= c0 && c0 < before + mine) {
         long long at = c0 - before;
         for (int s = s_beg; s < s_end; s++) {
-            const Q4Seq q = q4_seq(a, s, false);
+            const Q4Seq q = q4_seq(a, s, false, limit);
             const long long n = tiles_of(q);
             if (at >= n) { at -= n; continue; }
             for (int rb = 0;; rb++) {
@@ -196,7 +197,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
     const int block = page_size * (HD + 8), page_bytes = nkv * block, v_off = page_size * St::ROW, s_off = 2 * v_off + (lane < 4 ? 0 : page_size * 4 - 64);
     const unsigned n_pages = (unsigned)a.cache.n_pages;
     const int tile_pages = TILE / page_size, tile_rows = TILE - tile_pages * page_size;
-    Q4Seq q = q4_seq(a, s, false);
+    Q4Seq q = q4_seq(a, s, false, limit);
     bool first = true;      // no part of this block's yet
     Q4End end{};
     auto next_item = [&]() {
@@ -206,7 +207,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
             rb++;
             while (rb * QA_ROWS >= q.count * G) {      // (there is one: the line goes on)
                 rb = 0;
-                q = q4_seq(a, ++s, false);
+                q = q4_seq(a, ++s, false, limit);
             }
         }
     };
@@ -657,7 +658,8 @@ inline size_t attention_q4_workspace(const b200_q4_attention& a) {
     const size_t grid = (size_t)attention_q4_grid(a), part = QA_ROWS * (a.cache.head_dim + 4) * 4;
     return grid * (2 * part + sizeof(Q4End));
 }
-template <typename T, int HD> cudaError_t attention_q4(const b200_q4_attention& a, cudaStream_t st) {
+// limit: sequences with more rows are left out
+template <typename T, int HD> cudaError_t attention_q4_rows(const b200_q4_attention& a, int64_t limit, cudaStream_t st) {
     using Sm = Q4Smem<HD, QA_W, QA_U>;
     static SmemAllowed allowed;
     const auto kernel = attention_q4_kernel<T, HD, QA_W, QA_U>;
@@ -665,7 +667,7 @@ template <typename T, int HD> cudaError_t attention_q4(const b200_q4_attention& 
     if (e != cudaSuccess) return e;
     const uint64_t d = (uint64_t)a.cache.page_size / 16, page16 = (((uint64_t)1 << 36) + d - 1) / d;      // n / d = n * page16 >> 36 for n < 2^27
     const int grid = attention_q4_grid(a);
-    e = launch(kernel, dim3(grid), dim3(32 * QA_W), Sm::BYTES, 1, st, a, page16);
+    e = launch(kernel, dim3(grid), dim3(32 * QA_W), Sm::BYTES, 1, st, a, page16, limit);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid, QA_ROWS);

@@ -1,0 +1,494 @@
+// dev_q4_prompt.cuh — attention of many query tokens over the paged 4-bit cache, on tcgen05 (the sequences of b200_dev_attention_paged_q4 with many rows).
+//
+// The same function as dev_q4_attn.cuh.  A block has 128 query rows (row = token * G + head) of one sequence and kv head and walks the keys they see in tiles of 128:
+//   warps 8-11  read a tile's nibbles (a page's row is one to four 16-byte words) and write them to shared memory as operands: 128 + n is n in the low bits of the bf16 128, 1024 + n those of the
+//               fp16 1024; minus 136 or 1032 it is n - 8.  Keys as they lie, their channels in groups of eight in the order 0 4 1 5 2 6 3 7 (one shift and one and give two of them), which the
+//               queries have too; values transposed, two positions per 32-bit word.
+//   warp 12     issues S = Q K^T (128 x 128, K = hd) and O += P V (N = hd, K = 128).
+//   warps 0-7   one thread per row, two groups of four warps that take every second tile with sums, maximum and statistics of their own, so that one group's exponentials run under the other's
+//               products; the two are joined at the end.  P goes back to tensor memory in place of S.
+// Keys' scales multiply the scores, values' scales the weights.  The weights are bf16 pairs (what the first leaves over is the second: 2^-17), since a weight p_j d_j needs f32's range; f32 queries are
+// pairs of fp16 numbers scaled by a power of two.  The reference of a row's exponentials moves only when a score passes it by 2^8.
+// What bounds it: per tile and row 128 x (2 + 2) products of 128 (the values twice for the pairs), and 128 exponentials and their 10 instructions; a tile's MMAs alone are 1536 clocks at hd 128.
+#pragma once
+#include <type_traits>
+
+#include "dev_q4_attn.cuh"
+
+namespace dev {
+
+enum { QP_ROWS = 128, QP_KEYS = 128, QP_SOFT = 8, QP_MAKE = 8, QP_MMA = 12, QP_THREADS = 416 };
+
+template <typename T, int HD> struct Q4PromptSmem {
+    static constexpr int NQ = sizeof(T) == 4 ? 2 : 1;
+    static constexpr int SLAB = 128 * 128, Q = NQ * (HD / 64) * SLAB, K = (HD / 64) * SLAB, V = 2 * HD * 128;      // rows of 128 bytes, SWIZZLE_128B
+    static constexpr int K_AT = Q, V_AT = K_AT + 2 * K, META_AT = V_AT + 2 * V, META = 128 * 4 * 2 + 16, STAT_AT = META_AT + 4 * META, BAR_AT = STAT_AT + 2 * 128 * 8, BYTES = BAR_AT + 16 * 8;
+};
+template <bool BF> __device__ __forceinline__ uint32_t sub_2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (BF) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// two nibbles (bits 0-3 and 16-19 of v) as n - 8
+template <bool BF> __device__ __forceinline__ uint32_t nibbles(uint32_t v) { return sub_2<BF>((v & 0x000f000fu) | (BF ? 0x43004300u : 0x64006400u), BF ? 0x43084308u : 0x64086408u); }
+__device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void sts32(uint32_t at, uint32_t a) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(a) : "memory"); }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+        "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+        "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// D = f32, A = B = bf16 (1) or fp16 (0), K-major
+__device__ __forceinline__ uint32_t f16_idesc(bool bf, int M, int N) { return (1u << 4) | (bf ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) attention_q4_prompt_kernel(const b200_q4_attention a, uint64_t page16, int64_t limit) {
+    using Sm = Q4PromptSmem<T, HD>;
+    constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+    constexpr int NQ = Sm::NQ, SLABS = HD / 64;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_item[2];
+    uint8_t* smem = smem_raw + ((1024u - (sm_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t base = sm_u32(smem);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nkv = a.cache.n_kv_heads, G = a.n_heads / nkv, page_size = a.cache.page_size;
+
+    // ---- this block's rows.  The last ones of a sequence see the most keys and come first.
+    const int id = (int)(gridDim.x - 1 - blockIdx.x), h = id % nkv, item = id / nkv;
+    if (warp == 0) {
+        int at = item, seq = -1, rb = 0;
+        for (int s0 = 0; s0 < a.seqs && seq < 0; s0 += 32) {
+            int blocks = 0;
+            if (s0 + lane < a.seqs) {
+                const int64_t rows = (int64_t)q4_seq(a, s0 + lane, false).count * G;
+                blocks = rows > limit ? (int)((rows + QP_ROWS - 1) / QP_ROWS) : 0;
+            }
+            int upto = blocks;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, at < upto);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                seq = s0 + l;
+                rb = at - __shfl_sync(0xffffffffu, upto - blocks, l);
+            } else {
+                at -= __shfl_sync(0xffffffffu, upto, 31);
+            }
+        }
+        if (lane == 0) {
+            s_item[0] = seq;
+            s_item[1] = rb;
+        }
+    }
+    const uint32_t bars = base + Sm::BAR_AT;
+    const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64, p_full = bars + 80, pv_done = bars + 96;
+    if (tid == 32) {
+        for (int i = 0; i < 2; i++) {
+            bar_init(k_full + 8 * i, 4);
+            bar_init(k_empty + 8 * i, 1);
+            bar_init(v_full + 8 * i, 4);
+            bar_init(v_empty + 8 * i, 1);
+            bar_init(s_full + 8 * i, 1);
+            bar_init(p_full + 8 * i, 4);
+            bar_init(pv_done + 8 * i, 1);
+        }
+        bar_init_done();
+    }
+    __syncthreads();
+    const int s = s_item[0], rb = s_item[1];
+    if (s < 0) return;      // (the whole block)
+    const Q4Seq q = q4_seq(a, s, false);
+    const int rows = min(QP_ROWS, q.count * G - rb * QP_ROWS), first = rb * QP_ROWS / G, last = (rb * QP_ROWS + rows - 1) / G;
+    const int64_t at0 = q.len - q.count;      // position of the sequence's first query token
+    const int hi = (int)max((int64_t)0, at0 + last + 1), hi_min = (int)max((int64_t)0, at0 + first + 1);
+    const int lo_min = a.window > 0 ? (int)max((int64_t)0, at0 + first + 1 - a.window) : 0, lo_max = a.window > 0 ? (int)max((int64_t)0, at0 + last + 1 - a.window) : 0;
+    const int begin = lo_min & ~15, n = (hi - begin + QP_KEYS - 1) / QP_KEYS;      // tiles (0: nothing is seen)
+    if (warp == QP_MMA) tmem_alloc<false>(&s_tmem, 512);
+
+    // ---- queries: thread = row, half the channels each of two; pairs of fp16 for f32, scaled so that the row's elements are below 2^14
+    float alpha = 0.0f;      // what a row's scores are multiplied with (its sign is in the queries)
+    if (warp < QP_SOFT) {
+        const int r = tid & 127, half = tid >> 7;
+        const bool live = r < rows;
+        const int rr = rb * QP_ROWS + (live ? r : 0), token = rr / G;
+        const T* p = reinterpret_cast<const T*>(a.q) + (q.first + token) * a.q_token + (h * G + rr - token * G) * a.q_head;
+        const bool vec = (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+        float f1 = 1.0f, f2 = 1.0f;
+        int e = 0;
+        if (!BF) {
+            float top = 0.0f;
+#pragma unroll 4
+            for (int i = 0; i < HD; i += 8) {
+                float x[8];
+                if (vec) load_n<T, 8, true>(p + i, x);
+                else load_n<T, 8, false>(p + i, x);
+#pragma unroll
+                for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(x[k]));
+            }
+            e = top < INFINITY ? 140 - (int)(__float_as_uint(top) >> 23) : 0;
+            f1 = __int_as_float((127 + e / 2) << 23);
+            f2 = __int_as_float((127 + e - e / 2) << 23);
+        }
+        alpha = ldexpf(fabsf(a.scale) * 1.4426950408889634f, -e);
+        if (a.scale < 0.0f) f1 = -f1;
+        if (!live) f1 = 0.0f;
+#pragma unroll 2
+        for (int i = half * (HD / 16); i < (half + 1) * (HD / 16); i++) {
+            float x[8];
+            if (vec) load_n<T, 8, true>(p + 8 * i, x);
+            else load_n<T, 8, false>(p + 8 * i, x);
+            uint32_t o[4], ol[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float u = live ? x[k] * f1 * f2 : 0.0f, v = live ? x[k + 4] * f1 * f2 : 0.0f;
+                if (BF) {
+                    o[k] = pack_bf2(u, v);
+                } else {
+                    o[k] = pack_h2(u, v);
+                    if (NQ == 2) {
+                        const float2 b = unpack_h2(o[k]);
+                        ol[k] = pack_h2(u - b.x, v - b.y);
+                    }
+                }
+            }
+            const uint32_t to = base + (i >> 3) * Sm::SLAB + r * 128 + (((i & 7) ^ (r & 7)) << 4);
+            sts128(to, o[0], o[1], o[2], o[3]);
+            if (NQ == 2) sts128(to + SLABS * Sm::SLAB, ol[0], ol[1], ol[2], ol[3]);
+        }
+        async_fence();
+    }
+    umma_before_sync();
+    __syncthreads();
+    umma_after_sync();
+    const uint32_t tmem = s_tmem;
+    bool alive = true;
+
+    if (warp >= QP_MAKE && warp < QP_MMA) {
+        // ---- operands of keys and values
+        const int pw = warp - QP_MAKE, key = pw * 32 + lane;
+        constexpr int CH = HD / 32, PER = 32 / CH;              // 16-byte words of a row; rows a warp reads at once
+        constexpr int KN = 32 / PER, VN = HD / 64;              // words of keys per thread; words of each of two values
+        const int block = page_size * (HD + 8), v_off = page_size * (HD / 2);
+        const uint8_t* head = reinterpret_cast<const uint8_t*>(a.cache.data) + (int64_t)h * block;
+        const int64_t page_bytes = (int64_t)nkv * block;
+        const int32_t* table = a.page_table + (int64_t)s * a.table_stride;
+        // the page block of position p and p's place in it; null where there is none
+        auto where = [&](int p, int& row) -> const uint8_t* {
+            if (p >= hi) return nullptr;
+            const int index = (int)(((uint64_t)(p >> 4) * page16) >> 36);
+            const int page = table[index];
+            row = p - index * page_size;
+            if ((unsigned)page >= (uint64_t)a.cache.n_pages) {
+                if (a.status) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
+                return nullptr;
+            }
+            return head + page * page_bytes;
+        };
+        uint4 kw[KN], vw[2][VN];
+        float ks = 0.0f, vs = 0.0f;
+        bool there = false;
+        const int v_key = 64 * (pw & 1) + 2 * lane, v_word = (pw >> 1) * VN;
+        auto ask = [&](int t) {
+            const int p0 = begin + t * QP_KEYS;
+            int row = 0;
+#pragma unroll
+            for (int i = 0; i < KN; i++) {
+                const uint8_t* b = where(p0 + pw * 32 + i * PER + lane / CH, row);
+                kw[i] = b ? *reinterpret_cast<const uint4*>(b + row * (HD / 2) + (lane % CH) * 16) : make_uint4(0, 0, 0, 0);
+            }
+            const uint8_t* b = where(p0 + v_key, row);          // (both of a pair: a page holds whole sixteens)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < VN; i++) vw[u][i] = b ? *reinterpret_cast<const uint4*>(b + v_off + (row + u) * (HD / 2) + (v_word + i) * 16) : make_uint4(0, 0, 0, 0);
+            b = where(p0 + key, row);
+            there = b != nullptr;
+            const float* sc = reinterpret_cast<const float*>(b + 2 * v_off) + row;
+            ks = there ? sc[0] : 0.0f;
+            vs = there ? sc[page_size] : 0.0f;
+        };
+        if (n > 0) ask(0);
+        for (int t = 0; t < n; t++) {
+            const int st = t & 1;
+            const uint32_t ph = ((t >> 1) & 1) ^ 1u;
+            bar_wait(k_empty + 8 * st, ph, alive, 11);
+            const uint32_t kt = base + Sm::K_AT + st * Sm::K;
+#pragma unroll
+            for (int i = 0; i < KN; i++) {
+                const int r = pw * 32 + i * PER + lane / CH;
+                const uint32_t w[4] = {kw[i].x, kw[i].y, kw[i].z, kw[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int g = (lane % CH) * 4 + j;          // eight channels
+                    sts128(kt + (g >> 3) * Sm::SLAB + r * 128 + (((g & 7) ^ (r & 7)) << 4), nibbles<BF>(w[j]), nibbles<BF>(w[j] >> 4), nibbles<BF>(w[j] >> 8), nibbles<BF>(w[j] >> 12));
+                }
+            }
+            uint8_t* meta = smem + Sm::META_AT + (t & 3) * Sm::META;
+            reinterpret_cast<float*>(meta)[key] = ks;
+            reinterpret_cast<float*>(meta)[128 + key] = vs;
+            const uint32_t gone = ~__ballot_sync(0xffffffffu, there);
+            if (lane == 0) reinterpret_cast<uint32_t*>(meta + 1024)[pw] = gone;
+            async_fence();
+            __syncwarp();
+            if (lane == 0) bar_arrive(k_full + 8 * st);
+            bar_wait(v_empty + 8 * st, ph, alive, 12);
+            const uint32_t vt = base + Sm::V_AT + st * Sm::V + (pw & 1) * (HD * 128) + (lane & 3) * 4;
+#pragma unroll
+            for (int i = 0; i < VN; i++) {
+                const uint32_t w0[4] = {vw[0][i].x, vw[0][i].y, vw[0][i].z, vw[0][i].w}, w1[4] = {vw[1][i].x, vw[1][i].y, vw[1][i].z, vw[1][i].w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t x[2] = {__byte_perm(w0[j], w1[j], 0x5410), __byte_perm(w0[j], w1[j], 0x7632)};
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const int ch = ((v_word + i) * 4 + j) * 8 + k;
+                        sts32(vt + ch * 128 + (((lane >> 2) ^ (k & 7)) << 4), nibbles<true>(x[k >> 2] >> (4 * (k & 3))));
+                    }
+                }
+            }
+            if (t + 1 < n) ask(t + 1);
+            async_fence();
+            __syncwarp();
+            if (lane == 0) bar_arrive(v_full + 8 * st);
+        }
+    } else if (warp == QP_MMA) {
+        const uint32_t iqk = f16_idesc(BF, 128, QP_KEYS), ipv = f16_idesc(true, 128, HD);
+        auto scores = [&](int t) {
+            const int st = t & 1;
+            bar_wait(k_full + 8 * st, (t >> 1) & 1, alive, 13);
+            alive = __all_sync(0xffffffffu, alive);
+            umma_after_sync();
+            if (elect()) {
+                if (alive) {
+                    const uint64_t dk = umma_desc(base + Sm::K_AT + st * Sm::K);
+#pragma unroll
+                    for (int u = 0; u < NQ; u++)
+#pragma unroll
+                        for (int sl = 0; sl < SLABS; sl++)
+#pragma unroll
+                            for (int kk = 0; kk < 4; kk++)
+                                mma_ss(tmem + st * 128, umma_desc(base + (u * SLABS + sl) * Sm::SLAB) + 2 * kk, dk + (uint64_t)(sl * (Sm::SLAB >> 4) + 2 * kk), iqk, u + sl + kk > 0);
+                }
+                umma_commit<false>(k_empty + 8 * st);
+                umma_commit<false>(s_full + 8 * st);
+            }
+            __syncwarp();
+        };
+        for (int t = 0; t < min(n, 2); t++) scores(t);
+        for (int t = 0; t < n; t++) {
+            const int st = t & 1;
+            const uint32_t ph = (t >> 1) & 1;
+            bar_wait(v_full + 8 * st, ph, alive, 14);
+            bar_wait(p_full + 8 * st, ph, alive, 15);
+            alive = __all_sync(0xffffffffu, alive);
+            umma_after_sync();
+            if (elect()) {
+                if (alive) {
+                    const uint64_t dv = umma_desc(base + Sm::V_AT + st * Sm::V);
+#pragma unroll
+                    for (int kk = 0; kk < 8; kk++)
+#pragma unroll
+                        for (int u = 0; u < 2; u++)
+                            mma_ts(tmem + 256 + st * HD, tmem + st * 128 + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * u, dv + (uint64_t)((kk >> 2) * (HD * 128 >> 4) + 2 * (kk & 3)), ipv,
+                                   t >= 2 || kk + u > 0);
+                }
+                umma_commit<false>(v_empty + 8 * st);
+                umma_commit<false>(pv_done + 8 * st);
+            }
+            __syncwarp();
+            if (t + 2 < n) {
+                // (the scores of t + 2 go where the weights of t are)
+                bar_wait(pv_done + 8 * st, ph, alive, 16);
+                scores(t + 2);
+            }
+        }
+    } else {
+        // ---- rows
+        const int r = tid & 127, grp = warp >> 2, rr = rb * QP_ROWS + r, token = rr / G;
+        const bool live = r < rows;
+        const int row_hi = live ? (int)max((int64_t)0, at0 + token + 1) : INT32_MAX, row_lo = live && a.window > 0 ? (int)max((int64_t)0, at0 + token + 1 - a.window) : 0;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), S = lanes + grp * 128, O = lanes + 256 + grp * HD;
+        float m = -INFINITY, l = 0.0f;
+        for (int t = grp; t < n; t += 2) {
+            const int p0 = begin + t * QP_KEYS;
+            const uint8_t* meta = smem + Sm::META_AT + (t & 3) * Sm::META;
+            bar_wait(s_full + 8 * grp, (t >> 1) & 1, alive, 17);
+            __syncwarp();
+            umma_after_sync();
+            const uint4 gone = *reinterpret_cast<const uint4*>(meta + 1024);
+            const uint32_t out[4] = {gone.x, gone.y, gone.z, gone.w};
+            const bool all = p0 >= lo_max && p0 + QP_KEYS <= hi_min && !(gone.x | gone.y | gone.z | gone.w);      // (uniform)
+            // a bit per key of a batch of 32 that this row does not see
+            auto hidden = [&](int j) {
+                const int p = p0 + 32 * j, above = row_hi - p, below_ = row_lo - p;
+                uint32_t b = out[j];
+                if (above < 32) b |= above <= 0 ? 0xffffffffu : 0xffffffffu << above;
+                if (below_ > 0) b |= below_ >= 32 ? 0xffffffffu : ~(0xffffffffu << below_);
+                return b;
+            };
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t v[32];
+                tmem_ld32(v, S + 32 * j);
+                const float4* k4 = reinterpret_cast<const float4*>(meta) + 8 * j;
+                const uint32_t hid = all ? 0u : hidden(j);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float4 k = k4[i];
+                    const float z[4] = {__uint_as_float(v[4 * i]) * k.x, __uint_as_float(v[4 * i + 1]) * k.y, __uint_as_float(v[4 * i + 2]) * k.z, __uint_as_float(v[4 * i + 3]) * k.w};
+                    if (all) {
+                        top = fmaxf(fmaxf(top, fmaxf(z[0], z[1])), fmaxf(z[2], z[3]));
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 4; x++)
+                            if (!((hid >> (4 * i + x)) & 1u)) top = fmaxf(top, z[x]);
+                    }
+                }
+            }
+            top *= alpha;      // (alpha = 0: 0, or NaN where nothing is seen, which moves nothing)
+            if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+                const float was = m;
+                m = fmaxf(m, top);
+                const float f = ex2(below(was, m));
+                l *= f;
+                if (t >= 2) {      // (the group's products so far are done: the scores came after them)
+#pragma unroll 1
+                    for (int j = 0; j < HD / 32; j++) {
+                        uint32_t v[32];
+                        tmem_ld32(v, O + 32 * j);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                        tmem_st32(O + 32 * j, v);
+                    }
+                    tmem_st_done();
+                }
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t v[32], o[32];
+                tmem_ld32(v, S + 32 * j);
+                const float4 *k4 = reinterpret_cast<const float4*>(meta) + 8 * j, *v4 = k4 + 32;
+                const uint32_t hid = all ? 0u : hidden(j);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float4 k = k4[i], d = v4[i];
+                    const float kk[4] = {k.x, k.y, k.z, k.w}, dd[4] = {d.x, d.y, d.z, d.w};
+                    float w[4];
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        float p = ex2(fmaf(__uint_as_float(v[4 * i + x]) * kk[x], alpha, -ref));
+                        w[x] = p * dd[x];
+                        if (!all && ((hid >> (4 * i + x)) & 1u)) p = w[x] = 0.0f;
+                        l += p;
+                    }
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const uint32_t b = pack_bf2(w[2 * x], w[2 * x + 1]);
+                        o[2 * i + x] = b;
+                        o[16 + 2 * i + x] = pack_bf2(w[2 * x] - __uint_as_float(b << 16), w[2 * x + 1] - __uint_as_float(b & 0xffff0000u));
+                    }
+                }
+                tmem_st32(S + 32 * j, o);      // columns 32 j ..: the first ones of 32 keys, then what they leave over
+            }
+            tmem_st_done();
+            umma_before_sync();
+            __syncwarp();
+            if (lane == 0) bar_arrive(p_full + 8 * grp);
+        }
+        // ---- the two groups into one: each thread has its row's half of the channels
+        float2* stat = reinterpret_cast<float2*>(smem + Sm::STAT_AT);
+        stat[grp * 128 + r] = make_float2(m, l);
+        const int tiles = grp ? n / 2 : (n + 1) / 2;
+        if (tiles > 0) bar_wait(pv_done + 8 * grp, (tiles - 1) & 1, alive, 18);
+        __syncwarp();
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        __syncwarp();
+        umma_after_sync();
+        const float2 s0 = stat[r], s1 = stat[128 + r];
+        const float t2 = fmaxf(s0.x, s1.x), f0 = ex2(below(s0.x, t2)), f1 = ex2(below(s1.x, t2)), sum = s0.y * f0 + s1.y * f1, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        T* to = reinterpret_cast<T*>(a.out) + (q.first + token) * a.out_token + (h * G + rr - token * G) * a.out_head + grp * (HD / 2);
+        const bool vec = (reinterpret_cast<uintptr_t>(to) & 15) == 0;
+#pragma unroll 1
+        for (int j = 0; j < HD / 64; j++) {
+            float y[32];
+#pragma unroll
+            for (int i = 0; i < 32; i++) y[i] = 0.0f;
+            if (n > 0) {
+                uint32_t v[32];
+                tmem_ld32(v, lanes + 256 + grp * (HD / 2) + 32 * j);
+#pragma unroll
+                for (int i = 0; i < 32; i++) y[i] = __uint_as_float(v[i]) * f0;
+            }
+            if (n > 1) {
+                uint32_t v[32];
+                tmem_ld32(v, lanes + 256 + HD + grp * (HD / 2) + 32 * j);
+#pragma unroll
+                for (int i = 0; i < 32; i++) y[i] = fmaf(__uint_as_float(v[i]), f1, y[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i++) y[i] = sum == 0.0f ? 0.0f : y[i] * inv;
+            if (live) {
+                if (vec) store_n<T, 32, true>(to + 32 * j, y);
+                else store_n<T, 32, false>(to + 32 * j, y);
+            }
+        }
+    }
+    __syncwarp();
+    umma_before_sync();
+    __syncthreads();
+    umma_after_sync();
+    if (warp == QP_MMA) tmem_free<false>(tmem, 512);
+}
+
+// ------------------------------------------------------------------------------------------------------------------- host
+// Sequences with more rows than this go to attention_q4_prompt_kernel.
+constexpr int64_t kPromptRows = 32;
+template <typename T, int HD> cudaError_t attention_q4_prompt(const b200_q4_attention& a, cudaStream_t st) {
+    using Sm = Q4PromptSmem<T, HD>;
+    static SmemAllowed allowed;
+    const auto kernel = attention_q4_prompt_kernel<T, HD>;
+    const cudaError_t e = allowed((const void*)kernel, Sm::BYTES + 1024);
+    if (e != cudaSuccess) return e;
+    const int64_t G = a.n_heads / a.cache.n_kv_heads, rows = a.tokens * G;
+    // blocks of 128 rows: whole ones, and a last one of each sequence that has more rows than kPromptRows
+    const int64_t blocks = rows / QP_ROWS + std::min<int64_t>(a.seqs, rows / (kPromptRows + 1));
+    const uint64_t d = (uint64_t)a.cache.page_size / 16, page16 = (((uint64_t)1 << 36) + d - 1) / d;
+    if (blocks == 0) return cudaSuccess;
+    return launch(kernel, dim3((unsigned)(blocks * a.cache.n_kv_heads)), dim3(QP_THREADS), Sm::BYTES + 1024, 1, st, a, page16, kPromptRows);
+}
+// Whether a call may have such sequences, as far as the host can tell.
+inline bool attention_q4_has_prompts(const b200_q4_attention& a) {
+    return a.q_starts && (a.max_q ? a.max_q : a.tokens) * (a.n_heads / a.cache.n_kv_heads) > kPromptRows;
+}
+template <typename T, int HD> cudaError_t attention_q4(const b200_q4_attention& a, cudaStream_t st) {
+    const bool prompts = attention_q4_has_prompts(a);
+    if (prompts) {
+        const cudaError_t e = attention_q4_prompt<T, HD>(a, st);
+        if (e != cudaSuccess) return e;
+    }
+    return attention_q4_rows<T, HD>(a, prompts ? kPromptRows : INT64_MAX, st);
+}
+
+}  // namespace dev

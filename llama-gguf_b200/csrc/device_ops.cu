@@ -10,6 +10,7 @@
 #include "dev_norm_q8.cuh"
 #include "dev_q4_attn.cuh"
 #include "dev_q4_cache.cuh"
+#include "dev_q4_prompt.cuh"
 
 namespace {
 

@@ -309,33 +309,69 @@ def test_attention_of_large_scores_and_other_scales(D):
 
 
 @pytest.mark.parametrize("magnitude", [2.0**-100, 1e-6, 1e6, 2.0**100])
-def test_attention_of_values_and_queries_of_any_magnitude(D, magnitude):
+@pytest.mark.parametrize("q_lens", [[1, 1], [20, 17]])
+def test_attention_of_values_and_queries_of_any_magnitude(D, magnitude, q_lens):
     """Scales pass through in 32 bits: nothing is rounded to a type of less range."""
     pages, table = cache(5, [70, 20], 2, 64, 16)
-    vs = R.sections(pages, 16, 64)[3]
+    ks, vs = R.sections(pages, 16, 64)[2:]
     vs.mul_(magnitude)
-    ks = R.sections(pages, 16, 64)[2]
-    q = normal(9, 2, 4, 64)
-    lens = torch.tensor([70, 20], dtype=torch.int32)
+    starts = [0, q_lens[0], sum(q_lens)]
+    q = normal(9, starts[-1], 4, 64)
+    lens = torch.tensor([70, 20], dtype=torch.int32).cuda()
     for f in (1.0, magnitude):
         ks.mul_(1 / f)
-        want, off = R.attention(q.double() * f, R.values(pages, 16, 64), table.tolist(), [70, 20], [0, 1, 2], 16, 0.125, 0, pages.shape[0])
-        got = D.attention_paged_q4((q * f).cuda(), pages.cuda(), table.cuda(), lens.cuda()).cpu().double()
+        want, off = R.attention(q.double() * f, R.values(pages, 16, 64), table.tolist(), [70, 20], starts, 16, 0.125, 0, pages.shape[0])
+        got = D.attention_paged_q4((q * f).cuda(), pages.cuda(), table.cuda(), lens, q_starts=torch.tensor(starts, dtype=torch.int32).cuda()).cpu().double()
         assert ((got - want).abs() <= off + 2.0**-24 * want.abs()).all()
         ks.mul_(f)
 
 
-def test_attention_what_is_masked_is_not_seen(D):
-    """NaN and infinite rows behind a sequence's end or ahead of its window change nothing; inside they make the result NaN."""
-    pages, table = cache(5, [70], 2, 64, 16)
-    lens, q = torch.tensor([70], dtype=torch.int32), normal(9, 1, 4, 64).cuda()
-    want = D.attention_paged_q4(q, pages.cuda(), table.cuda(), lens.cuda(), window=20)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("q_len", [1, 5, 60])
+def test_attention_what_is_masked_is_not_seen(D, dtype, q_len):
+    """NaN and infinite rows behind a sequence's end or ahead of its windows change nothing; inside they make NaN of the rows that see them, and of no others."""
+    pages, table = cache(5, [270], 2, 64, 16)
+    lens, q = torch.tensor([270], dtype=torch.int32).cuda(), normal(9, q_len, 4, 64).to(dtype).cuda()
+    starts, w = torch.tensor([0, q_len], dtype=torch.int32).cuda(), 20
+    run = lambda window: D.attention_paged_q4(q, pages.cuda(), table.cuda(), lens, q_starts=starts, window=window)  # noqa: E731
+    want = run(w)
     ks, vs = R.sections(pages, 16, 64)[2:]
-    for j in list(range(0, 50)) + list(range(70, 80)):
+
+    def spoil(j, i):
         page = int(table[0, j // 16])
-        ks[page, :, j % 16], vs[page, :, j % 16] = math.nan, (math.inf if j % 2 else math.nan)
-    assert torch.equal(D.attention_paged_q4(q, pages.cuda(), table.cuda(), lens.cuda(), window=20), want)
-    assert torch.isnan(D.attention_paged_q4(q, pages.cuda(), table.cuda(), lens.cuda(), window=21)).all()
+        ks[page, :, j % 16], vs[page, :, j % 16] = math.nan, (math.inf if i % 2 else math.nan)
+
+    for j in list(range(0, 270 - q_len - w + 1)) + list(range(270, 272)):
+        spoil(j, j)
+    assert torch.equal(run(w), want)
+    seen = torch.isnan(run(w + 1)).flatten(1)
+    assert seen[0].all() and not seen[1:].any()
+    # the last position: only the last token sees it
+    spoil(269, 0)
+    seen = torch.isnan(run(w)).flatten(1)
+    assert seen[-1].all() and not seen[:-1].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_of_prompts(D, dtype, hd):
+    """More rows than a block has, tiles that end anywhere, groups of heads that do not divide a block's rows."""
+    check_attention(D, dtype, 4, 2, hd, 16, [129, 700], [129, 70])
+    check_attention(D, dtype, 7, 1, hd, 48, [400, 33, 5], [45, 33, 5])
+    check_attention(D, dtype, 5, 5, hd, 32, [257, 1], [200, 1], window=64)
+    check_attention(D, dtype, 2, 2, hd, 64, [40, 70], [90, 70])      # (more tokens than positions: the first ones see nothing)
+
+
+@pytest.mark.parametrize("q_len", [9, 50])
+def test_attention_of_several_tokens_with_bad_pages(D, q_len):
+    lens = [300, 200]
+    pages, table = cache(5, lens, 2, 128, 16)
+    table[0, 2], table[0, 9], table[1, 12] = -3, pages.shape[0], 2**31 - 1
+    q, status = normal(9, 2 * q_len, 4, 128).to(torch.bfloat16), torch.zeros(1, dtype=torch.int32).cuda()
+    starts = [0, q_len, 2 * q_len]
+    got = D.attention_paged_q4(q.cuda(), pages.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), q_starts=torch.tensor(starts, dtype=torch.int32).cuda(), status=status)
+    want, off = R.attention(q.double(), R.values(pages, 16, 128), table.tolist(), lens, starts, 16, 128**-0.5, 0, pages.shape[0], torch.bfloat16)
+    assert ((got.cpu().double() - want).abs() <= off + 2.0**-8 * 1.001 * (want.abs() + off)).all() and status.item() == D.STATUS_BAD_PAGE
 
 
 def test_attention_bad_pages_lengths_and_starts(D):
