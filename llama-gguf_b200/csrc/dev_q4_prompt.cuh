@@ -48,6 +48,41 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
         "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                 "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr)
+                 : "memory");
+}
+// sixteen columns of this warp's lanes: asked for, and there (the registers are not to be touched in between)
+__device__ __forceinline__ void tmem_ask16(uint32_t (&v)[16], uint32_t taddr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+                   "=r"(v[14]), "=r"(v[15])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_got(uint32_t (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]),
+                   "+r"(v[14]), "+r"(v[15])::"memory");
+}
+// two f32 operations in one instruction
+__device__ __forceinline__ uint64_t two(float2 v) { return (uint64_t)__float_as_uint(v.x) | (uint64_t)__float_as_uint(v.y) << 32; }
+__device__ __forceinline__ float2 two(uint64_t v) { return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(a)), "l"(two(b)));
+    return two(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(a)), "l"(two(b)));
+    return two(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(two(a)), "l"(two(b)), "l"(two(c)));
+    return two(r);
+}
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // D = f32, A = B = bf16 (1) or fp16 (0), K-major
@@ -192,84 +227,105 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
         const uint8_t* head = reinterpret_cast<const uint8_t*>(a.cache.data) + (int64_t)h * block;
         const int64_t page_bytes = (int64_t)nkv * block;
         const int32_t* table = a.page_table + (int64_t)s * a.table_stride;
-        // the page block of position p and p's place in it; null where there is none
-        auto where = [&](int p, int& row) -> const uint8_t* {
+        // the rows of sixteen positions from p (a multiple of 16) on: their first key row; null where there is no page
+        auto rows_of = [&](int p) -> const uint8_t* {
             if (p >= hi) return nullptr;
             const int index = (int)(((uint64_t)(p >> 4) * page16) >> 36);
             const int page = table[index];
-            row = p - index * page_size;
             if ((unsigned)page >= (uint64_t)a.cache.n_pages) {
                 if (a.status) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
                 return nullptr;
             }
-            return head + page * page_bytes;
+            return head + page * page_bytes + (p - index * page_size) * (HD / 2);
         };
-        uint4 kw[KN], vw[2][VN];
-        float ks = 0.0f, vs = 0.0f;
-        bool there = false;
+        // what a tile needs of memory, asked for a tile ahead
+        struct Raw {
+            uint4 k[KN], v[2][VN];
+            float ks, vs;
+            bool there;
+        };
         const int v_key = 64 * (pw & 1) + 2 * lane, v_word = (pw >> 1) * VN;
-        auto ask = [&](int t) {
+        auto ask = [&](int t, Raw& w) {
             const int p0 = begin + t * QP_KEYS;
-            int row = 0;
+            const uint8_t* kb[2] = {rows_of(p0 + pw * 32), rows_of(p0 + pw * 32 + 16)};
+            const uint8_t* vb = rows_of(p0 + (v_key & ~15));
 #pragma unroll
             for (int i = 0; i < KN; i++) {
-                const uint8_t* b = where(p0 + pw * 32 + i * PER + lane / CH, row);
-                kw[i] = b ? *reinterpret_cast<const uint4*>(b + row * (HD / 2) + (lane % CH) * 16) : make_uint4(0, 0, 0, 0);
+                const int r = i * PER + lane / CH;
+                const uint8_t* b = kb[r >> 4];
+                w.k[i] = b ? *reinterpret_cast<const uint4*>(b + (r & 15) * (HD / 2) + (lane % CH) * 16) : make_uint4(0, 0, 0, 0);
             }
-            const uint8_t* b = where(p0 + v_key, row);          // (both of a pair: a page holds whole sixteens)
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int i = 0; i < VN; i++) vw[u][i] = b ? *reinterpret_cast<const uint4*>(b + v_off + (row + u) * (HD / 2) + (v_word + i) * 16) : make_uint4(0, 0, 0, 0);
-            b = where(p0 + key, row);
-            there = b != nullptr;
-            const float* sc = reinterpret_cast<const float*>(b + 2 * v_off) + row;
-            ks = there ? sc[0] : 0.0f;
-            vs = there ? sc[page_size] : 0.0f;
+                for (int i = 0; i < VN; i++)
+                    w.v[u][i] = vb ? *reinterpret_cast<const uint4*>(vb + v_off + ((v_key & 15) + u) * (HD / 2) + (v_word + i) * 16) : make_uint4(0, 0, 0, 0);
+            const uint8_t* sb = kb[lane >> 4];
+            w.there = sb != nullptr && p0 + key < hi;
+            // (the scales of those sixteen: from the block's start 2 v_off on, four bytes where a row has HD / 2)
+            if (sb) {
+                const int p = p0 + (key & ~15), row = p - (int)(((uint64_t)(p >> 4) * page16) >> 36) * page_size;
+                const float* sc = reinterpret_cast<const float*>(sb - row * (HD / 2) + 2 * v_off) + row + (key & 15);
+                w.ks = sc[0];
+                w.vs = sc[page_size];
+            }
         };
-        if (n > 0) ask(0);
-        for (int t = 0; t < n; t++) {
-            const int st = t & 1;
-            const uint32_t ph = ((t >> 1) & 1) ^ 1u;
-            bar_wait(k_empty + 8 * st, ph, alive, 11);
-            const uint32_t kt = base + Sm::K_AT + st * Sm::K;
+        auto make_keys = [&](int t, const Raw& w) {
+            const uint32_t kt = base + Sm::K_AT + (t & 1) * Sm::K;
 #pragma unroll
             for (int i = 0; i < KN; i++) {
                 const int r = pw * 32 + i * PER + lane / CH;
-                const uint32_t w[4] = {kw[i].x, kw[i].y, kw[i].z, kw[i].w};
+                const uint32_t x[4] = {w.k[i].x, w.k[i].y, w.k[i].z, w.k[i].w};
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int g = (lane % CH) * 4 + j;          // eight channels
-                    sts128(kt + (g >> 3) * Sm::SLAB + r * 128 + (((g & 7) ^ (r & 7)) << 4), nibbles<BF>(w[j]), nibbles<BF>(w[j] >> 4), nibbles<BF>(w[j] >> 8), nibbles<BF>(w[j] >> 12));
+                    sts128(kt + (g >> 3) * Sm::SLAB + r * 128 + (((g & 7) ^ (r & 7)) << 4), nibbles<BF>(x[j]), nibbles<BF>(x[j] >> 4), nibbles<BF>(x[j] >> 8), nibbles<BF>(x[j] >> 12));
                 }
             }
             uint8_t* meta = smem + Sm::META_AT + (t & 3) * Sm::META;
-            reinterpret_cast<float*>(meta)[key] = ks;
-            reinterpret_cast<float*>(meta)[128 + key] = vs;
-            const uint32_t gone = ~__ballot_sync(0xffffffffu, there);
+            reinterpret_cast<float*>(meta)[key] = w.there ? w.ks : 0.0f;
+            reinterpret_cast<float*>(meta)[128 + key] = w.there ? w.vs : 0.0f;
+            const uint32_t gone = ~__ballot_sync(0xffffffffu, w.there);
             if (lane == 0) reinterpret_cast<uint32_t*>(meta + 1024)[pw] = gone;
-            async_fence();
-            __syncwarp();
-            if (lane == 0) bar_arrive(k_full + 8 * st);
-            bar_wait(v_empty + 8 * st, ph, alive, 12);
-            const uint32_t vt = base + Sm::V_AT + st * Sm::V + (pw & 1) * (HD * 128) + (lane & 3) * 4;
+        };
+        auto make_values = [&](int t, const Raw& w) {
+            const uint32_t vt = base + Sm::V_AT + (t & 1) * Sm::V + (pw & 1) * (HD * 128) + (lane & 3) * 4;
+            const uint32_t c8 = lane >> 2;
 #pragma unroll
             for (int i = 0; i < VN; i++) {
-                const uint32_t w0[4] = {vw[0][i].x, vw[0][i].y, vw[0][i].z, vw[0][i].w}, w1[4] = {vw[1][i].x, vw[1][i].y, vw[1][i].z, vw[1][i].w};
+                const uint32_t w0[4] = {w.v[0][i].x, w.v[0][i].y, w.v[0][i].z, w.v[0][i].w}, w1[4] = {w.v[1][i].x, w.v[1][i].y, w.v[1][i].z, w.v[1][i].w};
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const uint32_t x[2] = {__byte_perm(w0[j], w1[j], 0x5410), __byte_perm(w0[j], w1[j], 0x7632)};
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
                         const int ch = ((v_word + i) * 4 + j) * 8 + k;
-                        sts32(vt + ch * 128 + (((lane >> 2) ^ (k & 7)) << 4), nibbles<true>(x[k >> 2] >> (4 * (k & 3))));
+                        sts32(vt + ch * 128 + ((c8 ^ k) << 4), nibbles<true>(x[k >> 2] >> (4 * (k & 3))));
                     }
                 }
             }
-            if (t + 1 < n) ask(t + 1);
+        };
+        auto tile = [&](int t, const Raw& now, Raw& next) {
+            if (t + 1 < n) ask(t + 1, next);
+            const int st = t & 1;
+            const uint32_t ph = ((t >> 1) & 1) ^ 1u;
+            bar_wait(k_empty + 8 * st, ph, alive, 11);
+            make_keys(t, now);
+            async_fence();
+            __syncwarp();
+            if (lane == 0) bar_arrive(k_full + 8 * st);
+            bar_wait(v_empty + 8 * st, ph, alive, 12);
+            make_values(t, now);
             async_fence();
             __syncwarp();
             if (lane == 0) bar_arrive(v_full + 8 * st);
+        };
+        Raw one, two;
+        if (n > 0) ask(0, one);
+#pragma unroll 1
+        for (int t = 0; t < n; t += 2) {
+            tile(t, one, two);
+            if (t + 1 < n) tile(t + 1, two, one);
         }
     } else if (warp == QP_MMA) {
         const uint32_t iqk = f16_idesc(BF, 128, QP_KEYS), ipv = f16_idesc(true, 128, HD);
@@ -309,7 +365,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                     for (int kk = 0; kk < 8; kk++)
 #pragma unroll
                         for (int u = 0; u < 2; u++)
-                            mma_ts(tmem + 256 + st * HD, tmem + st * 128 + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * u, dv + (uint64_t)((kk >> 2) * (HD * 128 >> 4) + 2 * (kk & 3)), ipv,
+                            mma_ts(tmem + 256 + st * HD, tmem + st * 128 + 16 * kk + 8 * u, dv + (uint64_t)((kk >> 2) * (HD * 128 >> 4) + 2 * (kk & 3)), ipv,
                                    t >= 2 || kk + u > 0);
                 }
                 umma_commit<false>(v_empty + 8 * st);
@@ -346,27 +402,38 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 if (below_ > 0) b |= below_ >= 32 ? 0xffffffffu : ~(0xffffffffu << below_);
                 return b;
             };
-            float top = -INFINITY;
+            const float4* k4 = reinterpret_cast<const float4*>(meta);
+            // the largest score; sixteen columns at a time, the next ones on their way
+            auto largest = [&](auto whole) {
+                constexpr bool ALL = decltype(whole)::value;
+                float top[2] = {-INFINITY, -INFINITY};
+                uint32_t v[2][16];
+                tmem_ask16(v[0], S);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint32_t v[32];
-                tmem_ld32(v, S + 32 * j);
-                const float4* k4 = reinterpret_cast<const float4*>(meta) + 8 * j;
-                const uint32_t hid = all ? 0u : hidden(j);
+                for (int j = 0; j < 8; j++) {
+                    tmem_got(v[j & 1]);
+                    if (j < 7) tmem_ask16(v[(j + 1) & 1], S + 16 * (j + 1));
+                    const uint32_t hid = ALL ? 0u : hidden(j >> 1) >> (16 * (j & 1));
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float4 k = k4[i];
-                    const float z[4] = {__uint_as_float(v[4 * i]) * k.x, __uint_as_float(v[4 * i + 1]) * k.y, __uint_as_float(v[4 * i + 2]) * k.z, __uint_as_float(v[4 * i + 3]) * k.w};
-                    if (all) {
-                        top = fmaxf(fmaxf(top, fmaxf(z[0], z[1])), fmaxf(z[2], z[3]));
-                    } else {
+                    for (int i = 0; i < 4; i++) {
+                        const float4 k = k4[4 * j + i];
+                        const float2 x = mul2(make_float2(__uint_as_float(v[j & 1][4 * i]), __uint_as_float(v[j & 1][4 * i + 1])), make_float2(k.x, k.y)),
+                                     y = mul2(make_float2(__uint_as_float(v[j & 1][4 * i + 2]), __uint_as_float(v[j & 1][4 * i + 3])), make_float2(k.z, k.w));
+                        if (ALL) {
+                            top[0] = fmaxf(fmaxf(x.x, x.y), top[0]);
+                            top[1] = fmaxf(fmaxf(y.x, y.y), top[1]);
+                        } else {
+                            const float z[4] = {x.x, x.y, y.x, y.y};
 #pragma unroll
-                        for (int x = 0; x < 4; x++)
-                            if (!((hid >> (4 * i + x)) & 1u)) top = fmaxf(top, z[x]);
+                            for (int u = 0; u < 4; u++)
+                                if (!((hid >> (4 * i + u)) & 1u)) top[0] = fmaxf(top[0], z[u]);
+                        }
                     }
                 }
-            }
-            top *= alpha;      // (alpha = 0: 0, or NaN where nothing is seen, which moves nothing)
+                return fmaxf(top[0], top[1]);
+            };
+            // (alpha = 0: 0, or NaN where nothing is seen, which moves nothing)
+            const float top = (all ? largest(std::true_type{}) : largest(std::false_type{})) * alpha;
             if (__any_sync(0xffffffffu, top > m + 8.0f)) {
                 const float was = m;
                 m = fmaxf(m, top);
@@ -385,33 +452,44 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 }
             }
             const float ref = m == -INFINITY ? 0.0f : m;
+            // the weights, in place of the scores: of sixteen columns the first eight words are theirs, the others what those leave over
+            auto weights = [&](auto whole) {
+                constexpr bool ALL = decltype(whole)::value;
+                const float2 al = make_float2(alpha, alpha), rf = make_float2(-ref, -ref);
+                float2 sum = make_float2(0.0f, 0.0f);
+                uint32_t v[2][16];
+                tmem_ask16(v[0], S);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint32_t v[32], o[32];
-                tmem_ld32(v, S + 32 * j);
-                const float4 *k4 = reinterpret_cast<const float4*>(meta) + 8 * j, *v4 = k4 + 32;
-                const uint32_t hid = all ? 0u : hidden(j);
+                for (int j = 0; j < 8; j++) {
+                    tmem_got(v[j & 1]);
+                    if (j < 7) tmem_ask16(v[(j + 1) & 1], S + 16 * (j + 1));
+                    const uint32_t hid = ALL ? 0u : hidden(j >> 1) >> (16 * (j & 1));
+                    uint32_t o[16];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float4 k = k4[i], d = v4[i];
-                    const float kk[4] = {k.x, k.y, k.z, k.w}, dd[4] = {d.x, d.y, d.z, d.w};
-                    float w[4];
+                    for (int i = 0; i < 4; i++) {
+                        const float4 k = k4[4 * j + i], d = k4[32 + 4 * j + i];
 #pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        float p = ex2(fmaf(__uint_as_float(v[4 * i + x]) * kk[x], alpha, -ref));
-                        w[x] = p * dd[x];
-                        if (!all && ((hid >> (4 * i + x)) & 1u)) p = w[x] = 0.0f;
-                        l += p;
+                        for (int u = 0; u < 2; u++) {
+                            const float2 z = mul2(make_float2(__uint_as_float(v[j & 1][4 * i + 2 * u]), __uint_as_float(v[j & 1][4 * i + 2 * u + 1])), u ? make_float2(k.z, k.w) : make_float2(k.x, k.y));
+                            const float2 x = fma2(z, al, rf);
+                            float2 p = make_float2(ex2(x.x), ex2(x.y)), w = mul2(p, u ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
+                            if (!ALL) {
+                                if ((hid >> (4 * i + 2 * u)) & 1u) p.x = w.x = 0.0f;
+                                if ((hid >> (4 * i + 2 * u + 1)) & 1u) p.y = w.y = 0.0f;
+                            }
+                            sum = add2(sum, p);
+                            const uint32_t b = pack_bf2(w.x, w.y);
+                            const float2 rest = add2(w, make_float2(-__uint_as_float(b << 16), -__uint_as_float(b & 0xffff0000u)));
+                            o[2 * i + u] = b;
+                            o[8 + 2 * i + u] = pack_bf2(rest.x, rest.y);
+                        }
                     }
-#pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        const uint32_t b = pack_bf2(w[2 * x], w[2 * x + 1]);
-                        o[2 * i + x] = b;
-                        o[16 + 2 * i + x] = pack_bf2(w[2 * x] - __uint_as_float(b << 16), w[2 * x + 1] - __uint_as_float(b & 0xffff0000u));
-                    }
+                    tmem_st16(S + 16 * j, o);
                 }
-                tmem_st32(S + 32 * j, o);      // columns 32 j ..: the first ones of 32 keys, then what they leave over
-            }
+                l += sum.x + sum.y;
+            };
+            if (all) weights(std::true_type{});
+            else weights(std::false_type{});
             tmem_st_done();
             umma_before_sync();
             __syncwarp();
