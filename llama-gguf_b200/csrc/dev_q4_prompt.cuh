@@ -31,7 +31,7 @@ template <bool BF> __device__ __forceinline__ uint32_t sub_2(uint32_t a, uint32_
     return r;
 }
 // two nibbles (bits 0-3 and 16-19 of v) as n - 8
-template <bool BF> __device__ __forceinline__ uint32_t nibbles(uint32_t v) { return sub_2<BF>((v & 0x000f000fu) | (BF ? 0x43004300u : 0x64006400u), BF ? 0x43084308u : 0x64086408u); }
+template <bool BF> __device__ __forceinline__ uint32_t nibbles(uint32_t v, uint32_t mask) { return sub_2<BF>(masked_or(v, mask, BF ? 0x43004300u : 0x64006400u), BF ? 0x43084308u : 0x64086408u); }
 __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -64,6 +64,20 @@ __device__ __forceinline__ void tmem_got(uint32_t (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]),
                    "+r"(v[14]), "+r"(v[15])::"memory");
+}
+// take(j, columns 16 j .. 16 j + 15) for a tile's 128, the next sixteen on their way (a loop: the code of a tile's columns at once does not stay in the instruction cache)
+template <typename F> __device__ __forceinline__ void by_sixteens(uint32_t taddr, uint32_t (&v)[2][16], F&& take) {
+    tmem_ask16(v[0], taddr);
+#pragma unroll 1
+    for (int j = 0; j < 8; j += 2) {
+        tmem_got(v[0]);
+        tmem_ask16(v[1], taddr + 16 * (j + 1));
+        take(j, v[0]);
+        tmem_got(v[1]);
+        tmem_ask16(v[0], taddr + 16 * (j < 6 ? j + 2 : j + 1));      // (after the last: anything)
+        take(j + 1, v[1]);
+    }
+    tmem_got(v[0]);
 }
 // two f32 operations in one instruction
 __device__ __forceinline__ uint64_t two(float2 v) { return (uint64_t)__float_as_uint(v.x) | (uint64_t)__float_as_uint(v.y) << 32; }
@@ -227,45 +241,54 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
         const uint8_t* head = reinterpret_cast<const uint8_t*>(a.cache.data) + (int64_t)h * block;
         const int64_t page_bytes = (int64_t)nkv * block;
         const int32_t* table = a.page_table + (int64_t)s * a.table_stride;
-        // the rows of sixteen positions from p (a multiple of 16) on: their first key row; null where there is no page
-        auto rows_of = [&](int p) -> const uint8_t* {
-            if (p >= hi) return nullptr;
-            const int index = (int)(((uint64_t)(p >> 4) * page16) >> 36);
-            const int page = table[index];
-            if ((unsigned)page >= (uint64_t)a.cache.n_pages) {
-                if (a.status) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
-                return nullptr;
+        uint32_t mask = 0x000f000fu;
+        asm("" : "+r"(mask));      // (kept in a register: an instruction has room for one constant)
+        // Lane l looks after the sixteen positions l & 7 of a tile: the page is looked up two tiles ahead, the rows are asked for one tile ahead.
+        int page = 0, row = 0;
+        bool wanted = false;
+        auto look = [&](int t) {
+            const int p = begin + t * QP_KEYS + 16 * (lane & 7);
+            wanted = t < n && p < hi;
+            if (wanted) {
+                const int index = (int)(((uint64_t)(p >> 4) * page16) >> 36);
+                row = p - index * page_size;
+                page = table[index];
             }
-            return head + page * page_bytes + (p - index * page_size) * (HD / 2);
         };
-        // what a tile needs of memory, asked for a tile ahead
         struct Raw {
             uint4 k[KN], v[2][VN];
             float ks, vs;
             bool there;
-        };
+        } raw, next;
         const int v_key = 64 * (pw & 1) + 2 * lane, v_word = (pw >> 1) * VN;
         auto ask = [&](int t, Raw& w) {
-            const int p0 = begin + t * QP_KEYS;
-            const uint8_t* kb[2] = {rows_of(p0 + pw * 32), rows_of(p0 + pw * 32 + 16)};
-            const uint8_t* vb = rows_of(p0 + (v_key & ~15));
+            const bool good = wanted && (unsigned)page < (uint64_t)a.cache.n_pages;
+            if (wanted && !good && a.status) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
+            const unsigned long long mine = good ? (unsigned long long)(head + page * page_bytes) : 0ull;
+            const int my_row = row;
+            look(t + 1);
+            auto of = [&](int g, int& r) {
+                r = __shfl_sync(0xffffffffu, my_row, g);
+                return reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, mine, g));
+            };
+            int r0, r1, rv;
+            const uint8_t *k0 = of(2 * pw, r0), *k1 = of(2 * pw + 1, r1), *vb = of(v_key >> 4, rv);
 #pragma unroll
             for (int i = 0; i < KN; i++) {
                 const int r = i * PER + lane / CH;
-                const uint8_t* b = kb[r >> 4];
-                w.k[i] = b ? *reinterpret_cast<const uint4*>(b + (r & 15) * (HD / 2) + (lane % CH) * 16) : make_uint4(0, 0, 0, 0);
+                const uint8_t* b = i < KN / 2 ? k0 : k1;
+                w.k[i] = b ? *reinterpret_cast<const uint4*>(b + ((i < KN / 2 ? r0 : r1) + (r & 15)) * (HD / 2) + (lane % CH) * 16) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int i = 0; i < VN; i++)
-                    w.v[u][i] = vb ? *reinterpret_cast<const uint4*>(vb + v_off + ((v_key & 15) + u) * (HD / 2) + (v_word + i) * 16) : make_uint4(0, 0, 0, 0);
-            const uint8_t* sb = kb[lane >> 4];
-            w.there = sb != nullptr && p0 + key < hi;
-            // (the scales of those sixteen: from the block's start 2 v_off on, four bytes where a row has HD / 2)
-            if (sb) {
-                const int p = p0 + (key & ~15), row = p - (int)(((uint64_t)(p >> 4) * page16) >> 36) * page_size;
-                const float* sc = reinterpret_cast<const float*>(sb - row * (HD / 2) + 2 * v_off) + row + (key & 15);
+                    w.v[u][i] = vb ? *reinterpret_cast<const uint4*>(vb + v_off + (rv + (v_key & 15) + u) * (HD / 2) + (v_word + i) * 16) : make_uint4(0, 0, 0, 0);
+            const uint8_t* sb = lane < 16 ? k0 : k1;
+            w.there = sb != nullptr && begin + t * QP_KEYS + key < hi;
+            w.ks = w.vs = 0.0f;
+            if (w.there) {
+                const float* sc = reinterpret_cast<const float*>(sb + 2 * v_off) + (lane < 16 ? r0 : r1) + (key & 15);
                 w.ks = sc[0];
                 w.vs = sc[page_size];
             }
@@ -279,12 +302,13 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int g = (lane % CH) * 4 + j;          // eight channels
-                    sts128(kt + (g >> 3) * Sm::SLAB + r * 128 + (((g & 7) ^ (r & 7)) << 4), nibbles<BF>(x[j]), nibbles<BF>(x[j] >> 4), nibbles<BF>(x[j] >> 8), nibbles<BF>(x[j] >> 12));
+                    sts128(kt + (g >> 3) * Sm::SLAB + r * 128 + (((g & 7) ^ (r & 7)) << 4), nibbles<BF>(x[j], mask), nibbles<BF>(x[j] >> 4, mask),
+                           nibbles<BF>(x[j] >> 8, mask), nibbles<BF>(x[j] >> 12, mask));
                 }
             }
             uint8_t* meta = smem + Sm::META_AT + (t & 3) * Sm::META;
-            reinterpret_cast<float*>(meta)[key] = w.there ? w.ks : 0.0f;
-            reinterpret_cast<float*>(meta)[128 + key] = w.there ? w.vs : 0.0f;
+            reinterpret_cast<float*>(meta)[key] = w.ks;
+            reinterpret_cast<float*>(meta)[128 + key] = w.vs;
             const uint32_t gone = ~__ballot_sync(0xffffffffu, w.there);
             if (lane == 0) reinterpret_cast<uint32_t*>(meta + 1024)[pw] = gone;
         };
@@ -300,32 +324,29 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
                         const int ch = ((v_word + i) * 4 + j) * 8 + k;
-                        sts32(vt + ch * 128 + ((c8 ^ k) << 4), nibbles<true>(x[k >> 2] >> (4 * (k & 3))));
+                        sts32(vt + ch * 128 + ((c8 ^ k) << 4), nibbles<true>(x[k >> 2] >> (4 * (k & 3)), mask));
                     }
                 }
             }
         };
-        auto tile = [&](int t, const Raw& now, Raw& next) {
+        look(0);
+        if (n > 0) ask(0, raw);
+#pragma unroll 1
+        for (int t = 0; t < n; t++) {
             if (t + 1 < n) ask(t + 1, next);
             const int st = t & 1;
             const uint32_t ph = ((t >> 1) & 1) ^ 1u;
             bar_wait(k_empty + 8 * st, ph, alive, 11);
-            make_keys(t, now);
+            make_keys(t, raw);
             async_fence();
             __syncwarp();
             if (lane == 0) bar_arrive(k_full + 8 * st);
             bar_wait(v_empty + 8 * st, ph, alive, 12);
-            make_values(t, now);
+            make_values(t, raw);
             async_fence();
             __syncwarp();
             if (lane == 0) bar_arrive(v_full + 8 * st);
-        };
-        Raw one, two;
-        if (n > 0) ask(0, one);
-#pragma unroll 1
-        for (int t = 0; t < n; t += 2) {
-            tile(t, one, two);
-            if (t + 1 < n) tile(t + 1, two, one);
+            raw = next;
         }
     } else if (warp == QP_MMA) {
         const uint32_t iqk = f16_idesc(BF, 128, QP_KEYS), ipv = f16_idesc(true, 128, HD);
@@ -392,12 +413,11 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
             __syncwarp();
             umma_after_sync();
             const uint4 gone = *reinterpret_cast<const uint4*>(meta + 1024);
-            const uint32_t out[4] = {gone.x, gone.y, gone.z, gone.w};
             const bool all = p0 >= lo_max && p0 + QP_KEYS <= hi_min && !(gone.x | gone.y | gone.z | gone.w);      // (uniform)
             // a bit per key of a batch of 32 that this row does not see
             auto hidden = [&](int j) {
                 const int p = p0 + 32 * j, above = row_hi - p, below_ = row_lo - p;
-                uint32_t b = out[j];
+                uint32_t b = reinterpret_cast<const uint32_t*>(meta + 1024)[j];
                 if (above < 32) b |= above <= 0 ? 0xffffffffu : 0xffffffffu << above;
                 if (below_ > 0) b |= below_ >= 32 ? 0xffffffffu : ~(0xffffffffu << below_);
                 return b;
@@ -408,17 +428,13 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 constexpr bool ALL = decltype(whole)::value;
                 float top[2] = {-INFINITY, -INFINITY};
                 uint32_t v[2][16];
-                tmem_ask16(v[0], S);
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    tmem_got(v[j & 1]);
-                    if (j < 7) tmem_ask16(v[(j + 1) & 1], S + 16 * (j + 1));
+                auto take = [&](int j, const uint32_t (&v)[16]) {
                     const uint32_t hid = ALL ? 0u : hidden(j >> 1) >> (16 * (j & 1));
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const float4 k = k4[4 * j + i];
-                        const float2 x = mul2(make_float2(__uint_as_float(v[j & 1][4 * i]), __uint_as_float(v[j & 1][4 * i + 1])), make_float2(k.x, k.y)),
-                                     y = mul2(make_float2(__uint_as_float(v[j & 1][4 * i + 2]), __uint_as_float(v[j & 1][4 * i + 3])), make_float2(k.z, k.w));
+                        const float2 x = mul2(make_float2(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1])), make_float2(k.x, k.y)),
+                                     y = mul2(make_float2(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])), make_float2(k.z, k.w));
                         if (ALL) {
                             top[0] = fmaxf(fmaxf(x.x, x.y), top[0]);
                             top[1] = fmaxf(fmaxf(y.x, y.y), top[1]);
@@ -429,7 +445,8 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                                 if (!((hid >> (4 * i + u)) & 1u)) top[0] = fmaxf(top[0], z[u]);
                         }
                     }
-                }
+                };
+                by_sixteens(S, v, take);
                 return fmaxf(top[0], top[1]);
             };
             // (alpha = 0: 0, or NaN where nothing is seen, which moves nothing)
@@ -458,11 +475,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 const float2 al = make_float2(alpha, alpha), rf = make_float2(-ref, -ref);
                 float2 sum = make_float2(0.0f, 0.0f);
                 uint32_t v[2][16];
-                tmem_ask16(v[0], S);
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    tmem_got(v[j & 1]);
-                    if (j < 7) tmem_ask16(v[(j + 1) & 1], S + 16 * (j + 1));
+                auto take = [&](int j, const uint32_t (&v)[16]) {
                     const uint32_t hid = ALL ? 0u : hidden(j >> 1) >> (16 * (j & 1));
                     uint32_t o[16];
 #pragma unroll
@@ -470,7 +483,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                         const float4 k = k4[4 * j + i], d = k4[32 + 4 * j + i];
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
-                            const float2 z = mul2(make_float2(__uint_as_float(v[j & 1][4 * i + 2 * u]), __uint_as_float(v[j & 1][4 * i + 2 * u + 1])), u ? make_float2(k.z, k.w) : make_float2(k.x, k.y));
+                            const float2 z = mul2(make_float2(__uint_as_float(v[4 * i + 2 * u]), __uint_as_float(v[4 * i + 2 * u + 1])), u ? make_float2(k.z, k.w) : make_float2(k.x, k.y));
                             const float2 x = fma2(z, al, rf);
                             float2 p = make_float2(ex2(x.x), ex2(x.y)), w = mul2(p, u ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
                             if (!ALL) {
@@ -479,13 +492,14 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                             }
                             sum = add2(sum, p);
                             const uint32_t b = pack_bf2(w.x, w.y);
-                            const float2 rest = add2(w, make_float2(-__uint_as_float(b << 16), -__uint_as_float(b & 0xffff0000u)));
+                            const float2 rest = fma2(make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)), make_float2(-1.0f, -1.0f), w);
                             o[2 * i + u] = b;
                             o[8 + 2 * i + u] = pack_bf2(rest.x, rest.y);
                         }
                     }
                     tmem_st16(S + 16 * j, o);
-                }
+                };
+                by_sixteens(S, v, take);
                 l += sum.x + sum.y;
             };
             if (all) weights(std::true_type{});
