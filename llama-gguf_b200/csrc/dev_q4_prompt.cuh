@@ -1,14 +1,15 @@
 // dev_q4_prompt.cuh — attention of many query tokens over the paged 4-bit cache, on tcgen05 (the sequences of b200_dev_attention_paged_q4 with many rows).
 //
 // The same function as dev_q4_attn.cuh.  A block has 128 query rows (row = token * G + head) of one sequence and kv head and walks the keys they see in tiles of 128:
-//   warps 8-11  read a tile's nibbles (a page's row is one to four 16-byte words) and write them to shared memory as operands: 128 + n is n in the low bits of the bf16 128, 1024 + n those of the
+//   warps 8-15  read a tile's nibbles (a page's row is one to four 16-byte words) and write them to shared memory as operands: 128 + n is n in the low bits of the bf16 128, 1024 + n those of the
 //               fp16 1024; minus 136 or 1032 it is n - 8.  Keys as they lie, their channels in groups of eight in the order 0 4 1 5 2 6 3 7 (one shift and one and give two of them), which the
 //               queries have too; values transposed, two positions per 32-bit word.
-//   warp 12     issues S = Q K^T (128 x 128, K = hd) and O += P V (N = hd, K = 128).
+//   warp 16     issues S = Q K^T (128 x 128, K = hd) and O += P V (N = hd, K = 128).
 //   warps 0-7   one thread per row, two groups of four warps that take every second tile with sums, maximum and statistics of their own, so that one group's exponentials run under the other's
 //               products; the two are joined at the end.  P goes back to tensor memory in place of S.
 // Keys' scales multiply the scores, values' scales the weights.  The weights are bf16 pairs (what the first leaves over is the second: 2^-17), since a weight p_j d_j needs f32's range; f32 queries are
-// pairs of fp16 numbers scaled by a power of two.  The reference of a row's exponentials moves only when a score passes it by 2^8.
+// pairs of fp16 numbers scaled by a power of two.  bf16 has f32's range, so that the reference of a row's exponentials need only be near: it is the largest score of the first tile
+// that the row sees, and moves (by a whole number, which no bf16 notices) when a score passes it by 2^16.  A tile's scores are so read once.
 // What bounds it: per tile and row 128 x (2 + 2) products of 128 (the values twice for the pairs), and 128 exponentials and their 10 instructions; a tile's MMAs alone are 1536 clocks at hd 128.
 #pragma once
 #include <type_traits>
@@ -17,7 +18,7 @@
 
 namespace dev {
 
-enum { QP_ROWS = 128, QP_KEYS = 128, QP_SOFT = 8, QP_MAKE = 8, QP_MMA = 12, QP_THREADS = 416 };
+enum { QP_ROWS = 128, QP_KEYS = 128, QP_SOFT = 8, QP_MAKE = 8, QP_MMA = 16, QP_THREADS = 544 };
 
 template <typename T, int HD> struct Q4PromptSmem {
     static constexpr int NQ = sizeof(T) == 4 ? 2 : 1;
@@ -65,19 +66,14 @@ __device__ __forceinline__ void tmem_got(uint32_t (&v)[16]) {
                  : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]),
                    "+r"(v[14]), "+r"(v[15])::"memory");
 }
-// take(j, columns 16 j .. 16 j + 15) for a tile's 128, the next sixteen on their way (a loop: the code of a tile's columns at once does not stay in the instruction cache)
-template <typename F> __device__ __forceinline__ void by_sixteens(uint32_t taddr, uint32_t (&v)[2][16], F&& take) {
-    tmem_ask16(v[0], taddr);
+// take(j, columns 32 j .. 32 j + 31) for a tile's 128 (a loop: the code of all of them at once does not stay in the instruction cache)
+template <typename F> __device__ __forceinline__ void by_32(uint32_t taddr, F&& take) {
 #pragma unroll 1
-    for (int j = 0; j < 8; j += 2) {
-        tmem_got(v[0]);
-        tmem_ask16(v[1], taddr + 16 * (j + 1));
-        take(j, v[0]);
-        tmem_got(v[1]);
-        tmem_ask16(v[0], taddr + 16 * (j < 6 ? j + 2 : j + 1));      // (after the last: anything)
-        take(j + 1, v[1]);
+    for (int j = 0; j < 4; j++) {
+        uint32_t v[32];
+        tmem_ld32(v, taddr + 32 * j);
+        take(j, v);
     }
-    tmem_got(v[0]);
 }
 // two f32 operations in one instruction
 __device__ __forceinline__ uint64_t two(float2 v) { return (uint64_t)__float_as_uint(v.x) | (uint64_t)__float_as_uint(v.y) << 32; }
@@ -153,9 +149,9 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
     const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64, p_full = bars + 80, pv_done = bars + 96;
     if (tid == 32) {
         for (int i = 0; i < 2; i++) {
-            bar_init(k_full + 8 * i, 4);
+            bar_init(k_full + 8 * i, QP_MMA - QP_MAKE);
             bar_init(k_empty + 8 * i, 1);
-            bar_init(v_full + 8 * i, 4);
+            bar_init(v_full + 8 * i, QP_MMA - QP_MAKE);
             bar_init(v_empty + 8 * i, 1);
             bar_init(s_full + 8 * i, 1);
             bar_init(p_full + 8 * i, 4);
@@ -234,9 +230,9 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
 
     if (warp >= QP_MAKE && warp < QP_MMA) {
         // ---- operands of keys and values
-        const int pw = warp - QP_MAKE, key = pw * 32 + lane;
+        const int pw = warp - QP_MAKE;
         constexpr int CH = HD / 32, PER = 32 / CH;              // 16-byte words of a row; rows a warp reads at once
-        constexpr int KN = 32 / PER, VN = HD / 64;              // words of keys per thread; words of each of two values
+        constexpr int KN = 16 / PER, VW = HD / 32;              // 16-byte words of keys per thread; 32-bit words of each of two values
         const int block = page_size * (HD + 8), v_off = page_size * (HD / 2);
         const uint8_t* head = reinterpret_cast<const uint8_t*>(a.cache.data) + (int64_t)h * block;
         const int64_t page_bytes = (int64_t)nkv * block;
@@ -256,11 +252,13 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
             }
         };
         struct Raw {
-            uint4 k[KN], v[2][VN];
-            float ks, vs;
+            uint4 k[KN];
+            uint32_t v[2][VW];
+            float scale;      // of key 16 pw + lane, or of the value there (lanes from 16 on)
             bool there;
         } raw, next;
-        const int v_key = 64 * (pw & 1) + 2 * lane, v_word = (pw >> 1) * VN;
+        // this warp's keys: the sixteen pw; its values: pairs of half the tile's positions, a quarter of the channels
+        const int v_key = 64 * (pw & 1) + 2 * lane, v_word = (pw >> 1) * VW;
         auto ask = [&](int t, Raw& w) {
             const bool good = wanted && (unsigned)page < (uint64_t)a.cache.n_pages;
             if (wanted && !good && a.status) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
@@ -271,33 +269,27 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 r = __shfl_sync(0xffffffffu, my_row, g);
                 return reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, mine, g));
             };
-            int r0, r1, rv;
-            const uint8_t *k0 = of(2 * pw, r0), *k1 = of(2 * pw + 1, r1), *vb = of(v_key >> 4, rv);
+            int rk, rv;
+            const uint8_t *kb = of(pw, rk), *vb = of(v_key >> 4, rv);
 #pragma unroll
-            for (int i = 0; i < KN; i++) {
-                const int r = i * PER + lane / CH;
-                const uint8_t* b = i < KN / 2 ? k0 : k1;
-                w.k[i] = b ? *reinterpret_cast<const uint4*>(b + ((i < KN / 2 ? r0 : r1) + (r & 15)) * (HD / 2) + (lane % CH) * 16) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < KN; i++)
+                w.k[i] = kb ? *reinterpret_cast<const uint4*>(kb + (rk + i * PER + lane / CH) * (HD / 2) + (lane % CH) * 16) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                struct __align__(4 * VW) W { uint32_t x[VW]; };
+                W x{};
+                if (vb) x = *reinterpret_cast<const W*>(vb + v_off + (rv + (v_key & 15) + u) * (HD / 2) + v_word * 4);
+#pragma unroll
+                for (int i = 0; i < VW; i++) w.v[u][i] = x.x[i];
             }
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int i = 0; i < VN; i++)
-                    w.v[u][i] = vb ? *reinterpret_cast<const uint4*>(vb + v_off + (rv + (v_key & 15) + u) * (HD / 2) + (v_word + i) * 16) : make_uint4(0, 0, 0, 0);
-            const uint8_t* sb = lane < 16 ? k0 : k1;
-            w.there = sb != nullptr && begin + t * QP_KEYS + key < hi;
-            w.ks = w.vs = 0.0f;
-            if (w.there) {
-                const float* sc = reinterpret_cast<const float*>(sb + 2 * v_off) + (lane < 16 ? r0 : r1) + (key & 15);
-                w.ks = sc[0];
-                w.vs = sc[page_size];
-            }
+            w.there = kb != nullptr && begin + t * QP_KEYS + 16 * pw + (lane & 15) < hi;
+            w.scale = w.there ? reinterpret_cast<const float*>(kb + 2 * v_off)[rk + (lane & 15) + (lane < 16 ? 0 : page_size)] : 0.0f;
         };
         auto make_keys = [&](int t, const Raw& w) {
             const uint32_t kt = base + Sm::K_AT + (t & 1) * Sm::K;
 #pragma unroll
             for (int i = 0; i < KN; i++) {
-                const int r = pw * 32 + i * PER + lane / CH;
+                const int r = pw * 16 + i * PER + lane / CH;
                 const uint32_t x[4] = {w.k[i].x, w.k[i].y, w.k[i].z, w.k[i].w};
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
@@ -307,26 +299,18 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 }
             }
             uint8_t* meta = smem + Sm::META_AT + (t & 3) * Sm::META;
-            reinterpret_cast<float*>(meta)[key] = w.ks;
-            reinterpret_cast<float*>(meta)[128 + key] = w.vs;
+            reinterpret_cast<float*>(meta)[(lane < 16 ? 0 : 128) + 16 * pw + (lane & 15)] = w.scale;
             const uint32_t gone = ~__ballot_sync(0xffffffffu, w.there);
-            if (lane == 0) reinterpret_cast<uint32_t*>(meta + 1024)[pw] = gone;
+            if (lane == 0) reinterpret_cast<uint16_t*>(meta + 1024)[pw] = (uint16_t)gone;
         };
         auto make_values = [&](int t, const Raw& w) {
             const uint32_t vt = base + Sm::V_AT + (t & 1) * Sm::V + (pw & 1) * (HD * 128) + (lane & 3) * 4;
             const uint32_t c8 = lane >> 2;
 #pragma unroll
-            for (int i = 0; i < VN; i++) {
-                const uint32_t w0[4] = {w.v[0][i].x, w.v[0][i].y, w.v[0][i].z, w.v[0][i].w}, w1[4] = {w.v[1][i].x, w.v[1][i].y, w.v[1][i].z, w.v[1][i].w};
+            for (int j = 0; j < VW; j++) {
+                const uint32_t x[2] = {__byte_perm(w.v[0][j], w.v[1][j], 0x5410), __byte_perm(w.v[0][j], w.v[1][j], 0x7632)};
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint32_t x[2] = {__byte_perm(w0[j], w1[j], 0x5410), __byte_perm(w0[j], w1[j], 0x7632)};
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const int ch = ((v_word + i) * 4 + j) * 8 + k;
-                        sts32(vt + ch * 128 + ((c8 ^ k) << 4), nibbles<true>(x[k >> 2] >> (4 * (k & 3)), mask));
-                    }
-                }
+                for (int k = 0; k < 8; k++) sts32(vt + ((v_word + j) * 8 + k) * 128 + ((c8 ^ k) << 4), nibbles<true>(x[k >> 2] >> (4 * (k & 3)), mask));
             }
         };
         look(0);
@@ -386,7 +370,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                     for (int kk = 0; kk < 8; kk++)
 #pragma unroll
                         for (int u = 0; u < 2; u++)
-                            mma_ts(tmem + 256 + st * HD, tmem + st * 128 + 16 * kk + 8 * u, dv + (uint64_t)((kk >> 2) * (HD * 128 >> 4) + 2 * (kk & 3)), ipv,
+                            mma_ts(tmem + 256 + st * HD, tmem + st * 128 + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * u, dv + (uint64_t)((kk >> 2) * (HD * 128 >> 4) + 2 * (kk & 3)), ipv,
                                    t >= 2 || kk + u > 0);
                 }
                 umma_commit<false>(v_empty + 8 * st);
@@ -423,16 +407,15 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 return b;
             };
             const float4* k4 = reinterpret_cast<const float4*>(meta);
-            // the largest score; sixteen columns at a time, the next ones on their way
+            // the largest score
             auto largest = [&](auto whole) {
                 constexpr bool ALL = decltype(whole)::value;
                 float top[2] = {-INFINITY, -INFINITY};
-                uint32_t v[2][16];
-                auto take = [&](int j, const uint32_t (&v)[16]) {
-                    const uint32_t hid = ALL ? 0u : hidden(j >> 1) >> (16 * (j & 1));
+                auto take = [&](int j, const uint32_t (&v)[32]) {
+                    const uint32_t hid = ALL ? 0u : hidden(j);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float4 k = k4[4 * j + i];
+                    for (int i = 0; i < 8; i++) {
+                        const float4 k = k4[8 * j + i];
                         const float2 x = mul2(make_float2(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1])), make_float2(k.x, k.y)),
                                      y = mul2(make_float2(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])), make_float2(k.z, k.w));
                         if (ALL) {
@@ -446,60 +429,95 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                         }
                     }
                 };
-                by_sixteens(S, v, take);
+                by_32(S, take);
                 return fmaxf(top[0], top[1]);
             };
-            // (alpha = 0: 0, or NaN where nothing is seen, which moves nothing)
-            const float top = (all ? largest(std::true_type{}) : largest(std::false_type{})) * alpha;
-            if (__any_sync(0xffffffffu, top > m + 8.0f)) {
-                const float was = m;
-                m = fmaxf(m, top);
-                const float f = ex2(below(was, m));
+            // the reference goes up by `up` (a whole number, or 0): the sums so far, and the weights of the tile's first `cols` columns, are 2^-up times what they were
+            auto raise = [&](float up, int cols, float2& sum) {
+                const float f = ex2(-up);
+                m += up;
                 l *= f;
-                if (t >= 2) {      // (the group's products so far are done: the scores came after them)
+                sum = mul2(sum, make_float2(f, f));
+                uint32_t v[16];
 #pragma unroll 1
-                    for (int j = 0; j < HD / 32; j++) {
-                        uint32_t v[32];
-                        tmem_ld32(v, O + 32 * j);
+                for (int j = 0; t >= 2 && j < HD; j += 16) {      // (the group's products so far are done: the scores came after them)
+                    tmem_ask16(v, O + j);
+                    tmem_got(v);
 #pragma unroll
-                        for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                        tmem_st32(O + 32 * j, v);
-                    }
-                    tmem_st_done();
+                    for (int i = 0; i < 16; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                    tmem_st16(O + j, v);
                 }
+                tmem_st_done();
+#pragma unroll 1
+                for (int j = 0; j < cols; j += 16) {
+                    tmem_ask16(v, S + j);
+                    tmem_got(v);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) v[i] = pack_bf2(__uint_as_float(v[i] << 16) * f, __uint_as_float(v[i] & 0xffff0000u) * f);
+                    tmem_st16(S + j, v);
+                }
+                tmem_st_done();
+            };
+            if (__any_sync(0xffffffffu, m == -INFINITY)) {
+                // (alpha = 0: 0, or NaN where nothing is seen, which sets nothing)
+                const float top = (all ? largest(std::true_type{}) : largest(std::false_type{})) * alpha;
+                if (m == -INFINITY) m = fmaxf(m, top);
             }
-            const float ref = m == -INFINITY ? 0.0f : m;
-            // the weights, in place of the scores: of sixteen columns the first eight words are theirs, the others what those leave over
+            // the weights, in place of the scores: of 32 columns the first sixteen words are theirs, the others what those leave over
             auto weights = [&](auto whole) {
                 constexpr bool ALL = decltype(whole)::value;
-                const float2 al = make_float2(alpha, alpha), rf = make_float2(-ref, -ref);
+                const float2 al = make_float2(alpha, alpha);
+                float ref = m == -INFINITY ? 0.0f : m;
                 float2 sum = make_float2(0.0f, 0.0f);
-                uint32_t v[2][16];
-                auto take = [&](int j, const uint32_t (&v)[16]) {
-                    const uint32_t hid = ALL ? 0u : hidden(j >> 1) >> (16 * (j & 1));
-                    uint32_t o[16];
+                auto take = [&](int j, const uint32_t (&v)[32]) {
+                    const uint32_t hid = ALL ? 0u : hidden(j);
+                    float2 x[16];
+                    float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float4 k = k4[4 * j + i], d = k4[32 + 4 * j + i];
+                    for (int i = 0; i < 8; i++) {
+                        const float4 k = k4[8 * j + i];
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
                             const float2 z = mul2(make_float2(__uint_as_float(v[4 * i + 2 * u]), __uint_as_float(v[4 * i + 2 * u + 1])), u ? make_float2(k.z, k.w) : make_float2(k.x, k.y));
-                            const float2 x = fma2(z, al, rf);
-                            float2 p = make_float2(ex2(x.x), ex2(x.y)), w = mul2(p, u ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
+                            float2 y = fma2(z, al, make_float2(-ref, -ref));
                             if (!ALL) {
-                                if ((hid >> (4 * i + 2 * u)) & 1u) p.x = w.x = 0.0f;
-                                if ((hid >> (4 * i + 2 * u + 1)) & 1u) p.y = w.y = 0.0f;
+                                if ((hid >> (4 * i + 2 * u)) & 1u) y.x = -INFINITY;
+                                if ((hid >> (4 * i + 2 * u + 1)) & 1u) y.y = -INFINITY;
+                            }
+                            x[2 * i + u] = y;
+                            top[u] = fmaxf(fmaxf(y.x, y.y), top[u]);
+                        }
+                    }
+                    const float most = fmaxf(top[0], top[1]);
+                    if (__any_sync(0xffffffffu, most > 16.0f)) {
+                        const float up = most > 16.0f ? ceilf(most) : 0.0f;
+                        raise(up, 32 * j, sum);
+                        ref += up;
+#pragma unroll
+                        for (int i = 0; i < 16; i++) x[i] = add2(x[i], make_float2(-up, -up));
+                    }
+                    uint32_t o[32];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float4 d = k4[32 + 8 * j + i];
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const float2 p = make_float2(ex2(x[2 * i + u].x), ex2(x[2 * i + u].y));
+                            float2 w = mul2(p, u ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
+                            if (!ALL) {      // (a scale that other rows see may be NaN)
+                                if ((hid >> (4 * i + 2 * u)) & 1u) w.x = 0.0f;
+                                if ((hid >> (4 * i + 2 * u + 1)) & 1u) w.y = 0.0f;
                             }
                             sum = add2(sum, p);
                             const uint32_t b = pack_bf2(w.x, w.y);
                             const float2 rest = fma2(make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)), make_float2(-1.0f, -1.0f), w);
                             o[2 * i + u] = b;
-                            o[8 + 2 * i + u] = pack_bf2(rest.x, rest.y);
+                            o[16 + 2 * i + u] = pack_bf2(rest.x, rest.y);
                         }
                     }
-                    tmem_st16(S + 16 * j, o);
+                    tmem_st32(S + 32 * j, o);
                 };
-                by_sixteens(S, v, take);
+                by_32(S, take);
                 l += sum.x + sum.y;
             };
             if (all) weights(std::true_type{});
