@@ -140,7 +140,7 @@ extern "C" int b200_dev_rope_append_q4(const b200_q4_append* a) {
         if (!a->k || !a->v || !a->cos_sin || !a->positions || !a->slots || (a->q && !a->q_out)) return bad(op, "null pointer");
         if (a->q && a->q == a->q_out && (a->q_token != a->q_out_token || a->q_head != a->q_out_head)) return bad(op, "q in place needs the same strides");
         const int e = 16 / type_bytes(a->type);
-        bool vec = !off16(a->k) && !off16(a->v) && a->k_token % e == 0 && a->k_head % e == 0 && a->v_token % e == 0 && a->v_head % e == 0 && a->rot_dims % 16 == 0;
+        bool vec = !off16(a->k) && !off16(a->v) && a->k_token % e == 0 && a->k_head % e == 0 && a->v_token % e == 0 && a->v_head % e == 0 && a->rot_dims % 16 == 0 && !off16(a->cos_sin);
         if (a->q) vec = vec && !off16(a->q) && !off16(a->q_out) && a->q_token % e == 0 && a->q_head % e == 0 && a->q_out_token % e == 0 && a->q_out_head % e == 0;
         return on_device(op, a->device, [&] {
             return by_type(a->type, [&](auto t) {
