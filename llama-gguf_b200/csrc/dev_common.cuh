@@ -65,4 +65,27 @@ __device__ __forceinline__ Q4Block q4_block(const b200_q4_pages& c, int64_t page
     return Q4Block{p, p + rows, reinterpret_cast<const float*>(p + 2 * rows), reinterpret_cast<const float*>(p + 2 * rows) + c.page_size};
 }
 
+// Programmatic launches: a kernel may be scheduled while the one before it on the stream ends.  Every block of every kernel here calls before() first thing, ahead of any access to global memory (it
+// returns when all that came before is done and visible), and so no kernel can end before its predecessors have.
+__device__ __forceinline__ void before() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... P, typename... A> cudaError_t launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, int cluster, cudaStream_t st, const A&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 }  // namespace dev

@@ -79,6 +79,7 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_wide_kernel(const __gri
     const uint32_t ring = (sm_u32(smem) + 1023u) & ~1023u;      // (the swizzle is on absolute address bits)
     const uint32_t full = sm_u32(s_bar), empty = full + 8u * NS, acc_full = full + 16u * NS, acc_empty = acc_full + 16u;
     i8_setup<PAIR>(full, NS, 2, &s_tmem, 2 * TN);
+    before();
     const uint32_t tmem = s_tmem, rank = PAIR ? cluster_rank() : 0u;
     const int steps = (g.k + GI_STEP - 1) / GI_STEP, mt = (g.n + GI_M - 1) / GI_M, per = PAIR ? (mt + 1) / 2 : mt, nt = (g.t + TN - 1) / TN, tiles = per * nt;
     const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, stride = PAIR ? gridDim.x >> 1 : gridDim.x;
@@ -176,6 +177,7 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_split_kernel(const __gr
     const uint32_t ring = (sm_u32(smem) + 1023u) & ~1023u;
     const uint32_t full = sm_u32(s_bar), empty = full + 8u * NS, acc_full = full + 16u * NS;
     i8_setup<false>(full, NS, 1, &s_tmem, COLS);
+    before();
     const uint32_t tmem = s_tmem;
     const int all = (g.k + GI_STEP - 1) / GI_STEP, k_beg = (int)((int64_t)rank * all / S), k_end = (int)((int64_t)(rank + 1) * all / S);      // (S <= all)
     bool alive = true;
@@ -301,14 +303,14 @@ template <typename T, int TN, bool PAIR> cudaError_t gemm_i8_wide(const GemmI8Ca
     if (e != cudaSuccess) return e;
     const int64_t mt = (c.g.n + GI_M - 1) / GI_M, nt = (c.g.t + TN - 1) / TN;
     const int64_t grid = PAIR ? 2 * std::min<int64_t>((mt + 1) / 2 * nt, 74) : std::min<int64_t>(mt * nt, 148);
-    return launch(kernel, dim3((unsigned)grid), dim3(GI_THREADS), GI_RING + 1024, PAIR ? 2 : 1, c.st, c.amap, c.wmap, c.g);
+    return launch(kernel, dim3((unsigned)grid), GI_THREADS, GI_RING + 1024, PAIR ? 2 : 1, c.st, c.amap, c.wmap, c.g);
 }
 template <typename T, int TN> cudaError_t gemm_i8_split(const GemmI8Call& c) {
     static SmemAllowed allowed;
     const auto kernel = gemm_i8_split_kernel<T, TN>;
     const cudaError_t e = allowed((const void*)kernel, SplitRing<TN>::SMEM);
     if (e != cudaSuccess) return e;
-    return launch(kernel, dim3((unsigned)((c.g.n + GI_M - 1) / GI_M * c.g.splits), (unsigned)((c.g.t + TN - 1) / TN)), dim3(GI_THREADS), SplitRing<TN>::SMEM, c.g.splits, c.st, c.amap, c.wmap, c.g);
+    return launch(kernel, dim3((unsigned)((c.g.n + GI_M - 1) / GI_M * c.g.splits), (unsigned)((c.g.t + TN - 1) / TN)), GI_THREADS, SplitRing<TN>::SMEM, c.g.splits, c.st, c.amap, c.wmap, c.g);
 }
 template <typename T> cudaError_t gemm_i8(const int8_t* a, int64_t lda, const int8_t* w, int64_t ldw, GemmI8Args g, cudaStream_t st) {
     GemmI8Call c{};

@@ -52,6 +52,7 @@ __device__ __forceinline__ Q8Row q8_row(uint32_t top) {
 // Rows of whole 16-byte words on 16 bytes: a block per row, which stays in registers (V words per thread, asked for together) from its only load on.
 // The squares of 16-bit types are exact in f32; each is added in 64 bits, so that the sum, and with it every 8-bit number, does not depend on the order.
 template <typename T, int V> __global__ void __launch_bounds__(1024) add_rms_norm_q8_kernel(const NormQ8Args a) {
+    before();
     constexpr int E = 16 / (int)sizeof(T);
     __shared__ double s_sum[32];
     __shared__ uint32_t s_max[32];
@@ -123,6 +124,7 @@ template <typename T, int V> __global__ void __launch_bounds__(1024) add_rms_nor
 // Rows of any length and alignment: a block per row, which is read once per step (sum of squares, maximum, result); the sum is read back where it was written, each element by the
 // thread that wrote it.
 template <typename T> __global__ void __launch_bounds__(256) add_rms_norm_q8_any_kernel(const NormQ8Args a) {
+    before();
     __shared__ double s_sum[32];
     __shared__ uint32_t s_max[32];
     const int64_t row = blockIdx.x;
@@ -149,8 +151,7 @@ template <typename T> __global__ void __launch_bounds__(256) add_rms_norm_q8_any
 }
 
 template <typename T, int V> cudaError_t add_rms_norm_q8_words(const NormQ8Args& a, int threads, cudaStream_t st) {
-    add_rms_norm_q8_kernel<T, V><<<(unsigned)a.rows, threads, 0, st>>>(a);
-    return cudaGetLastError();
+    return launch(add_rms_norm_q8_kernel<T, V>, dim3((unsigned)a.rows), threads, 0, 1, st, a);
 }
 // Few rows: as many threads as the row has words, up to 1024 (one token of 4096 in bf16: latency).  Many rows: four words per thread, so that a block has fewer warps to wait for and the loads of a
 // thread cover one another.  Rows of more than 4 x 1024 words do not fit the registers.
@@ -159,10 +160,7 @@ template <typename T> cudaError_t add_rms_norm_q8(const NormQ8Args& a, cudaStrea
     auto off = [](const void* p, int64_t ld, int bytes, int size) { return reinterpret_cast<uintptr_t>(p) % bytes || ld * size % bytes; };
     const bool words = a.hidden % E == 0 && a.hidden / E <= 4096 && !off(a.x, a.ldx, 16, sizeof(T)) && !off(a.weight, 0, 16, 4) && !off(a.q, a.ldq, E, 1) &&
                        (!a.residual || (!off(a.residual, a.ldr, 16, sizeof(T)) && !off(a.sum, a.lds, 16, sizeof(T))));
-    if (!words) {
-        add_rms_norm_q8_any_kernel<T><<<(unsigned)a.rows, 256, 0, st>>>(a);
-        return cudaGetLastError();
-    }
+    if (!words) return launch(add_rms_norm_q8_any_kernel<T>, dim3((unsigned)a.rows), 256, 0, 1, st, a);
     const int n = a.hidden / E, few = a.rows <= 296;
     const int v = n > 2048 || (!few && n >= 256) ? 4 : n > 1024 || (!few && n >= 128) ? 2 : 1, threads = ((n + v - 1) / v + 31) / 32 * 32;
     return v == 4 ? add_rms_norm_q8_words<T, 4>(a, threads, st) : v == 2 ? add_rms_norm_q8_words<T, 2>(a, threads, st) : add_rms_norm_q8_words<T, 1>(a, threads, st);
@@ -176,6 +174,7 @@ struct ReadQ8Args {
     int64_t ldq, ldo, rows, n;
 };
 template <typename T, int E> __global__ void __launch_bounds__(256) read_q8_kernel(const ReadQ8Args a) {
+    before();
     for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const float s = a.scales[row];
         for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * E; i < a.n; i += (int64_t)gridDim.x * 256 * E) {
@@ -192,9 +191,7 @@ template <typename T> cudaError_t read_q8(const ReadQ8Args& a, cudaStream_t st) 
     const bool words = a.n % 16 == 0 && !((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) & 15) && a.ldq % 16 == 0 && a.ldo * sizeof(T) % 16 == 0;
     const int64_t per = words ? 4096 : 256;
     const dim3 grid((unsigned)std::min<int64_t>((a.n + per - 1) / per, 1024), (unsigned)std::min<int64_t>(a.rows, 16384));
-    if (words) read_q8_kernel<T, 16><<<grid, 256, 0, st>>>(a);
-    else read_q8_kernel<T, 1><<<grid, 256, 0, st>>>(a);
-    return cudaGetLastError();
+    return words ? launch(read_q8_kernel<T, 16>, grid, 256, 0, 1, st, a) : launch(read_q8_kernel<T, 1>, grid, 256, 0, 1, st, a);
 }
 
 }  // namespace dev

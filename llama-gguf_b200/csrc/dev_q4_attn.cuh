@@ -127,7 +127,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
     using Sm = Q4Smem<HD, W, U>;
     constexpr int STAGES = Sm::STAGES, TILE = Sm::TILE, WORDS = HD / 32, NT = HD / 16;      // words of a key row per lane; row tiles of the values
     constexpr bool Q2 = sizeof(T) == 4, P2 = !std::is_same<T, __nv_bfloat16>::value;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    before();
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ long long s_sum[W];
     __shared__ int s_item[4];      // sequence, row block, head, unit of the item
@@ -577,7 +577,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
 
 // Joins the parts of the items that ended in a block's first stretch: block (x, y) = that block, a row.
 template <typename T, int HD> __global__ void __launch_bounds__(256) attention_q4_join_kernel(const b200_q4_attention a, int grid) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    before();
     constexpr int LANES = HD / 4, GROUPS = 256 / LANES, PART = q4_part_floats<HD>(), AHEAD = 5;
     __shared__ __align__(16) float s_o[GROUPS][HD];
     __shared__ float s_l[GROUPS];
@@ -667,18 +667,9 @@ template <typename T, int HD> cudaError_t attention_q4_rows(const b200_q4_attent
     if (e != cudaSuccess) return e;
     const uint64_t d = (uint64_t)a.cache.page_size / 16, page16 = (((uint64_t)1 << 36) + d - 1) / d;      // n / d = n * page16 >> 36 for n < 2^27
     const int grid = attention_q4_grid(a);
-    e = launch(kernel, dim3(grid), dim3(32 * QA_W), Sm::BYTES, 1, st, a, page16, limit);
+    e = launch(kernel, dim3(grid), 32 * QA_W, Sm::BYTES, 1, st, a, page16, limit);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid, QA_ROWS);
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_q4_join_kernel<T, HD>, a, grid);
+    return launch(attention_q4_join_kernel<T, HD>, dim3(grid, QA_ROWS), 256, 0, 1, st, a, grid);
 }
 
 }  // namespace dev

@@ -87,6 +87,7 @@ template <typename T, int HD, bool VEC> struct RopeLane {
 
 template <typename T, int HD, bool VEC, int QPER>
 __global__ void __launch_bounds__(256) rope_append_q4_kernel(const b200_q4_append a, const Divisor kv_rows, const Divisor q_groups, unsigned kv_blocks, const Divisor page16) {
+    before();
     constexpr int L = HD / 8, PB = 256 / L;
     RopeLane<T, HD, VEC> lane(a);
     const bool leader = threadIdx.x % L == 0;
@@ -195,6 +196,7 @@ struct ReadQ4Args {
     int32_t* status;
 };
 template <typename T, int HD> __global__ void __launch_bounds__(256) read_q4_kernel(const ReadQ4Args a, const Divisor rows) {
+    before();
     constexpr int L = HD / 8;
     const int nkv = a.cache.n_kv_heads;
     const uint32_t item = blockIdx.x * (256 / L) + threadIdx.x / L;
@@ -223,9 +225,8 @@ template <typename T, int HD> __global__ void __launch_bounds__(256) read_q4_ker
 template <typename T, int HD, bool VEC, int QPER> cudaError_t rope_append_q4_by(const b200_q4_append& a, cudaStream_t st) {
     const int64_t per = 256 / (HD / 8), kv = 2 * a.cache.n_kv_heads, kv_blocks = (a.tokens * kv + per - 1) / per, groups = a.q ? (a.n_heads + QPER - 1) / QPER : 1;
     const int64_t q_blocks = a.q ? (a.tokens * groups + per - 1) / per : 0;
-    rope_append_q4_kernel<T, HD, VEC, QPER><<<(unsigned)(kv_blocks + q_blocks), 256, 0, st>>>(a, Divisor((uint32_t)kv), Divisor((uint32_t)groups), (unsigned)kv_blocks,
-                                                                                             Divisor((uint32_t)a.cache.page_size / 16));
-    return cudaGetLastError();
+    return launch(rope_append_q4_kernel<T, HD, VEC, QPER>, dim3((unsigned)(kv_blocks + q_blocks)), 256, 0, 1, st, a, Divisor((uint32_t)kv), Divisor((uint32_t)groups), (unsigned)kv_blocks,
+                  Divisor((uint32_t)a.cache.page_size / 16));
 }
 // Four query rows per group of lanes where one each would be more than all SMs hold at once (2048 threads each): fewer instructions per row.  Below that one: more rows on their way.
 template <typename T, int HD> cudaError_t rope_append_q4(const b200_q4_append& a, bool vec, cudaStream_t st) {
@@ -234,8 +235,7 @@ template <typename T, int HD> cudaError_t rope_append_q4(const b200_q4_append& a
 template <typename T, int HD> cudaError_t read_q4(const ReadQ4Args& a, cudaStream_t st) {
     const uint32_t rows = 2 * a.cache.n_kv_heads;
     const int64_t per = 256 / (HD / 8);
-    read_q4_kernel<T, HD><<<(unsigned)((a.tokens * rows + per - 1) / per), 256, 0, st>>>(a, Divisor(rows));
-    return cudaGetLastError();
+    return launch(read_q4_kernel<T, HD>, dim3((unsigned)((a.tokens * rows + per - 1) / per)), 256, 0, 1, st, a, Divisor(rows));
 }
 
 }  // namespace dev

@@ -105,6 +105,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 }
 
 template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) attention_q4_prompt_kernel(const b200_q4_attention a, uint64_t page16, int64_t limit) {
+    before();
     using Sm = Q4PromptSmem<T, HD>;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
     constexpr int NQ = Sm::NQ, SLABS = HD / 64;
@@ -586,7 +587,7 @@ template <typename T, int HD> cudaError_t attention_q4_prompt(const b200_q4_atte
     const int64_t blocks = rows / QP_ROWS + std::min<int64_t>(a.seqs, rows / (kPromptRows + 1));
     const uint64_t d = (uint64_t)a.cache.page_size / 16, page16 = (((uint64_t)1 << 36) + d - 1) / d;
     if (blocks == 0) return cudaSuccess;
-    return launch(kernel, dim3((unsigned)(blocks * a.cache.n_kv_heads)), dim3(QP_THREADS), Sm::BYTES + 1024, 1, st, a, page16, kPromptRows);
+    return launch(kernel, dim3((unsigned)(blocks * a.cache.n_kv_heads)), QP_THREADS, Sm::BYTES + 1024, 1, st, a, page16, kPromptRows);
 }
 // Whether a call may have such sequences, as far as the host can tell.
 inline bool attention_q4_has_prompts(const b200_q4_attention& a) {
