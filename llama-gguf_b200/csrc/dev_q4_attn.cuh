@@ -24,7 +24,7 @@
 
 namespace dev {
 
-enum { QA_ROWS = 8, QA_START = 4 };
+enum { QA_ROWS = 8, QA_START = 4, QA_WARPS = 12 };      // rows of an item, units of its start, warps of an SM
 
 struct Q4Seq {
     int first, count;      // query tokens
@@ -58,7 +58,7 @@ template <int TILE> __device__ __forceinline__ Q4Span q4_span(const b200_q4_atte
 
 // the workspace: per block, two parts of [8][HD] sums, [8][4] (m, r, l, -); then per block what its first stretch ends
 struct Q4End {
-    int first_cta, first_slot, seq, rb, head, ends;
+    int first_cta, first_slot, token, rb, head, rows;      // the sequence's first query token; rows of the item (0: nothing ends)
 };
 template <int HD> __host__ __device__ constexpr int q4_part_floats() { return QA_ROWS * (HD + 4); }
 
@@ -118,11 +118,11 @@ template <int HD> struct Q4Stage {
 };
 __device__ __forceinline__ int q4_piece(int row, int q) { return (((row & 1) | ((row >> 3) & 1) << 1 | (q >> 1) << 2) << 3) | (q & 1) | ((row >> 1) & 3) << 1; }
 
-template <int HD, int W, int U> struct Q4Smem {
-    static constexpr int TILE = 16 * W * U, STAGES = U == 1 ? 4 : 3, RING = W * STAGES * U * Q4Stage<HD>::BYTES, MERGE = W * QA_ROWS * (HD + 4) * 4 + W * QA_ROWS * 16, BYTES = RING + MERGE;
+template <int HD, int W, int U> struct Q4Smem {      // (the warps' sums lie over the drained ring)
+    static constexpr int TILE = 16 * W * U, STAGES = U == 1 ? 4 : 3, RING = W * STAGES * U * Q4Stage<HD>::BYTES, MERGE = W * QA_ROWS * (HD + 4) * 4 + W * QA_ROWS * 16, BYTES = RING > MERGE ? RING : MERGE;
 };
 
-template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32 * W, U == 1 ? 16 / W : 12 / W) attention_q4_kernel(const b200_q4_attention a, uint64_t page16, int64_t limit) {
+template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32 * W, QA_WARPS / W) attention_q4_kernel(const b200_q4_attention a, uint64_t page16, int64_t limit) {
     using St = Q4Stage<HD>;
     using Sm = Q4Smem<HD, W, U>;
     constexpr int STAGES = Sm::STAGES, TILE = Sm::TILE, WORDS = HD / 32, NT = HD / 16;      // words of a key row per lane; row tiles of the values
@@ -161,7 +161,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
     const long long grid = min((long long)gridDim.x, total);
     Q4End* ends = reinterpret_cast<Q4End*>(reinterpret_cast<float*>(a.workspace) + (size_t)gridDim.x * 2 * q4_part_floats<HD>()) + blockIdx.x;
     if (blockIdx.x >= grid) {      // (the whole block)
-        if (tid == 0) ends->ends = 0;
+        if (tid == 0) ends->rows = 0;
         return;
     }
     const long long c0 = total * blockIdx.x / grid, c1 = total * (blockIdx.x + 1) / grid;
@@ -187,7 +187,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
     int s = s_item[0], rb = s_item[1], h = s_item[2], unit = s_item[3];
 
     const uint32_t ring = sm_u32(smem) + warp * STAGES * U * St::BYTES;
-    float* merge = reinterpret_cast<float*>(smem + Sm::RING);             // [W][8][HD + 4]
+    float* merge = reinterpret_cast<float*>(smem);                        // [W][8][HD + 4]
     float* stat = merge + W * QA_ROWS * (HD + 4);                         // [W][8][4]
     // where this lane's words of a stage are: keys of positions g and g + 8; values of positions 2 c + (0, 1, 8, 9), words g and g + 8
     const uint32_t k_at = g * St::ROW + c * (WORDS * 4), v_at = St::V + q4_piece(2 * c, g >> 2) * 16 + (g & 3) * 4;
@@ -221,20 +221,92 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
             continue;
         }
 
+        // ---- the ring.  The page of a step is looked up one step before its rows are asked for.
+        const int32_t* table = a.page_table + (int64_t)s * a.table_stride;
+        const uint8_t* mine_k = reinterpret_cast<const uint8_t*>(a.cache.data) + (int64_t)h * block + lane * 16;
+        int p_look = sp.base + tile * TILE + warp * 16 * U, index = (int)(((uint64_t)(p_look >> 4) * page16) >> 36), row_look = p_look - index * page_size;
+        int p_fetch = p_look, page[U], row[U];
+        const int p_stop = min(sp.hi, sp.base + stop * TILE);
+        bool odd_page = false;      // a page that is none of the cache's came by in this item
+#pragma unroll
+        for (int b = 0; b < U; b++) page[b] = row[b] = 0;
+        auto look = [&]() {
+#pragma unroll
+            for (int b = 0; b < U; b++) {
+                const bool over = row_look + 16 * b >= page_size;
+                row[b] = row_look + 16 * b - (over ? page_size : 0);
+                if (p_look + 16 * b < p_stop) page[b] = table[index + over];
+            }
+            p_look += TILE;
+            index += tile_pages;
+            row_look += tile_rows;
+            if (row_look >= page_size) {
+                row_look -= page_size;
+                index++;
+            }
+        };
+        auto fetch = [&](int stage) {
+#pragma unroll
+            for (int b = 0; b < U; b++)
+                if (p_fetch + 16 * b < p_stop) {
+                    if ((unsigned)page[b] >= n_pages) {      // (masked below)
+                        odd_page = true;
+                        page[b] = 0;
+                        if (a.status && lane == 0) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
+                    }
+                    const uint8_t* k = mine_k + (int64_t)page[b] * page_bytes + row[b] * St::ROW;
+                    const uint32_t at = ring + (stage * U + b) * St::BYTES;
+#pragma unroll
+                    for (int i = 0; i < 16 * P; i += 32) {
+                        cp16(at + lane * 16 + i * 16, k + i * 16);
+                        cp16(at + v_to + q4_piece(i / P, 0) * 16, k + v_off + i * 16);
+                    }
+                    // (lanes 0-3 key scales, 4-7 value scales, which follow page_size floats later: lane * 16 is in k, 64 of it too much for those)
+                    if (lane < 8) cp16(at + St::KS + lane * 16, k - row[b] * (St::ROW - 4) + s_off);
+                }
+            cp_commit();
+            p_fetch += TILE;
+        };
+        // the first steps' pages, the query row, the first steps' rows: each is asked for before the one ahead of it is there
+        int pages[STAGES][U], rows[STAGES][U];
+#pragma unroll
+        for (int i = 0; i < STAGES; i++) {
+            look();
+#pragma unroll
+            for (int b = 0; b < U; b++) {
+                pages[i][b] = page[b];
+                rows[i][b] = row[b];
+            }
+        }
+        const int r = rb * QA_ROWS + g, token = r / G;
+        const bool live = r < q.count * G;
+        const int64_t pos = q.len - q.count + token;
+        // (rows behind the last one compute along with the first: nothing of theirs is written)
+        const int row_hi = live ? (int)max((int64_t)0, pos + 1) : INT32_MAX, row_lo = live && a.window > 0 ? (int)max((int64_t)0, pos + 1 - a.window) : 0;
+        float x[HD / 4];
+        const T* p = reinterpret_cast<const T*>(a.q) + (q.first + (live ? token : 0)) * a.q_token + (h * G + (live ? r - token * G : 0)) * a.q_head + c * (HD / 4);
+        if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) load_n<T, HD / 4, true>(p, x);
+        else load_n<T, HD / 4, false>(p, x);
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; i++) {
+#pragma unroll
+            for (int b = 0; b < U; b++) {
+                page[b] = pages[i][b];
+                row[b] = rows[i][b];
+            }
+            fetch(i);
+        }
+#pragma unroll
+        for (int b = 0; b < U; b++) {
+            page[b] = pages[STAGES - 1][b];
+            row[b] = rows[STAGES - 1][b];
+        }
+
         // ---- query row g as operand; what scores of rows 2 c and 2 c + 1 need
         uint32_t qb[WORDS][2][2], ql[Q2 ? WORDS : 1][2][2];
         float alpha[2], q8[2], m[2], mr[2], l[2], acc[NT][4];
         int hi[2], lo[2], hi_min, lo_max;
         {
-            const int r = rb * QA_ROWS + g, token = r / G;
-            const bool live = r < q.count * G;
-            const int64_t pos = q.len - q.count + token;
-            // (rows behind the last one compute along with the first: nothing of theirs is written)
-            const int row_hi = live ? (int)max((int64_t)0, pos + 1) : INT32_MAX, row_lo = live && a.window > 0 ? (int)max((int64_t)0, pos + 1 - a.window) : 0;
-            float x[HD / 4];
-            const T* p = reinterpret_cast<const T*>(a.q) + (q.first + (live ? token : 0)) * a.q_token + (h * G + (live ? r - token * G : 0)) * a.q_head + c * (HD / 4);
-            if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) load_n<T, HD / 4, true>(p, x);
-            else load_n<T, HD / 4, false>(p, x);
             float top = 0.0f;
 #pragma unroll
             for (int i = 0; i < HD / 4; i++) top = fmaxf(top, fabsf(x[i]));
@@ -285,58 +357,6 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
 #pragma unroll
             for (int k = 0; k < 4; k++) acc[i][k] = 0.0f;
 
-        // ---- the ring.  The page of a step is looked up one step before its rows are asked for.
-        const int32_t* table = a.page_table + (int64_t)s * a.table_stride;
-        const uint8_t* mine_k = reinterpret_cast<const uint8_t*>(a.cache.data) + (int64_t)h * block + lane * 16;
-        int p_look = sp.base + tile * TILE + warp * 16 * U, index = (int)(((uint64_t)(p_look >> 4) * page16) >> 36), row_look = p_look - index * page_size;
-        int p_fetch = p_look, page[U], row[U];
-        const int p_stop = min(sp.hi, sp.base + stop * TILE);
-        bool odd_page = false;      // a page that is none of the cache's came by in this item
-#pragma unroll
-        for (int b = 0; b < U; b++) page[b] = row[b] = 0;
-        auto look = [&]() {
-#pragma unroll
-            for (int b = 0; b < U; b++) {
-                const bool over = row_look + 16 * b >= page_size;
-                row[b] = row_look + 16 * b - (over ? page_size : 0);
-                if (p_look + 16 * b < p_stop) page[b] = table[index + over];
-            }
-            p_look += TILE;
-            index += tile_pages;
-            row_look += tile_rows;
-            if (row_look >= page_size) {
-                row_look -= page_size;
-                index++;
-            }
-        };
-        auto fetch = [&](int stage) {
-#pragma unroll
-            for (int b = 0; b < U; b++)
-                if (p_fetch + 16 * b < p_stop) {
-                    if ((unsigned)page[b] >= n_pages) {      // (masked below)
-                        odd_page = true;
-                        page[b] = 0;
-                        if (a.status && lane == 0) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
-                    }
-                    const uint8_t* k = mine_k + (int64_t)page[b] * page_bytes + row[b] * St::ROW;
-                    const uint32_t at = ring + (stage * U + b) * St::BYTES;
-#pragma unroll
-                    for (int i = 0; i < 16 * P; i += 32) {
-                        cp16(at + lane * 16 + i * 16, k + i * 16);
-                        cp16(at + v_to + q4_piece(i / P, 0) * 16, k + v_off + i * 16);
-                    }
-                    // (lanes 0-3 key scales, 4-7 value scales, which follow page_size floats later: lane * 16 is in k, 64 of it too much for those)
-                    if (lane < 8) cp16(at + St::KS + lane * 16, k - row[b] * (St::ROW - 4) + s_off);
-                }
-            cp_commit();
-            p_fetch += TILE;
-        };
-        look();
-#pragma unroll
-        for (int i = 0; i < STAGES - 1; i++) {
-            fetch(i);
-            look();
-        }
         int stage = 0, stage_to = STAGES - 1;
         uint32_t magic = 0x64006400u;
         asm("" : "+r"(magic));      // (kept in a register: an instruction has room for one constant)
@@ -508,6 +528,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
             }
         }
         cp_wait<0>();
+        __syncthreads();
 
         // ---- the warps' sums into one
 #pragma unroll
@@ -563,10 +584,10 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
             // the block that has the first tile; this item is its first one unless its stretch begins ahead of the item
             end.first_cta = (int)(((start + QA_START + 1) * grid - 1) / total);
             end.first_slot = total * end.first_cta / grid < start;
-            end.seq = s;
+            end.token = q.first;
             end.rb = rb;
             end.head = h;
-            end.ends = 1;
+            end.rows = min((int)QA_ROWS, q.count * G - rb * QA_ROWS);
         }
         first = false;
         __syncthreads();
@@ -583,10 +604,8 @@ template <typename T, int HD> __global__ void __launch_bounds__(256) attention_q
     __shared__ float s_l[GROUPS];
     const float* ws = reinterpret_cast<const float*>(a.workspace);
     const Q4End e = reinterpret_cast<const Q4End*>(ws + (size_t)grid * 2 * PART)[blockIdx.x];
-    if (!e.ends) return;
     const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31, n = (int)blockIdx.x - e.first_cta + 1, G = a.n_heads / a.cache.n_kv_heads, rr = e.rb * QA_ROWS + row;
-    const Q4Seq q = q4_seq(a, e.seq, false);
-    if (rr >= q.count * G) return;
+    if (row >= e.rows) return;
     auto part = [&](int i) { return ws + ((size_t)(e.first_cta + i) * 2 + (i == 0 ? e.first_slot : 0)) * PART; };
     // every group's first parts are asked for before anything waits
     float4 st[AHEAD], v[AHEAD];
@@ -641,7 +660,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(256) attention_q
             l += s_l[k];
         }
         const float r = topr == -INFINITY ? 0.0f : topr;
-        reinterpret_cast<T*>(a.out)[(q.first + rr / G) * a.out_token + (e.head * G + rr % G) * a.out_head + tid] =
+        reinterpret_cast<T*>(a.out)[(int64_t)(e.token + rr / G) * a.out_token + (e.head * G + rr % G) * a.out_head + tid] =
             from_f<T>(l == 0.0f ? 0.0f : ldexpf(x * (1.0f / l), (int)floorf(r)) * ex2(r - floorf(r)));
     }
 }
@@ -652,7 +671,7 @@ constexpr int QA_W = 4, QA_U = 2;      // warps of a block, 16 positions a warp 
 inline int attention_q4_grid(const b200_q4_attention& a) {
     const int64_t G = a.n_heads / a.cache.n_kv_heads, blocks = (a.tokens * G + QA_ROWS - 1) / QA_ROWS + a.seqs;
     const int64_t tiles = blocks * a.cache.n_kv_heads * (((int64_t)a.table_pages * a.cache.page_size + 16 * QA_W * QA_U - 1) / (16 * QA_W * QA_U) + 1 + QA_START);
-    return (int)std::min<int64_t>(148 * (QA_U == 1 ? 16 / QA_W : 12 / QA_W), tiles);
+    return (int)std::min<int64_t>(148 * (QA_WARPS / QA_W), tiles);
 }
 inline size_t attention_q4_workspace(const b200_q4_attention& a) {
     const size_t grid = (size_t)attention_q4_grid(a), part = QA_ROWS * (a.cache.head_dim + 4) * 4;
@@ -669,7 +688,7 @@ template <typename T, int HD> cudaError_t attention_q4_rows(const b200_q4_attent
     const int grid = attention_q4_grid(a);
     e = launch(kernel, dim3(grid), 32 * QA_W, Sm::BYTES, 1, st, a, page16, limit);
     if (e != cudaSuccess) return e;
-    return launch(attention_q4_join_kernel<T, HD>, dim3(grid, QA_ROWS), 256, 0, 1, st, a, grid);
+    return launch(attention_q4_join_kernel<T, HD>, dim3(grid, (unsigned)std::min<int64_t>(QA_ROWS, a.q_starts ? QA_ROWS : a.n_heads / a.cache.n_kv_heads)), 256, 0, 1, st, a, grid);
 }
 
 }  // namespace dev
