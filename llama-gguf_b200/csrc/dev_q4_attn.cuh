@@ -24,7 +24,7 @@
 
 namespace dev {
 
-enum { QA_ROWS = 8, QA_START = 4, QA_WARPS = 12 };      // rows of an item, units of its start, warps of an SM
+enum { QA_ROWS = 8, QA_START = 4, QA_WARPS = 12, QA_STAGES = 3 };      // rows of an item, units of its start, warps of an SM
 
 struct Q4Seq {
     int first, count;      // query tokens
@@ -62,6 +62,12 @@ struct Q4End {
 };
 template <int HD> __host__ __device__ constexpr int q4_part_floats() { return QA_ROWS * (HD + 4); }
 
+// where block i of `grid` begins on a line of `total` units: floor(total i / grid), without a division of 64 bits
+__device__ __forceinline__ long long q4_begin(long long total, int i, int grid) {
+    if (total >> 32) return total * i / grid;
+    const uint32_t each = (uint32_t)total / (uint32_t)grid, over = (uint32_t)total - each * (uint32_t)grid;
+    return (long long)each * i + over * (uint32_t)i / (uint32_t)grid;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -119,7 +125,7 @@ template <int HD> struct Q4Stage {
 __device__ __forceinline__ int q4_piece(int row, int q) { return (((row & 1) | ((row >> 3) & 1) << 1 | (q >> 1) << 2) << 3) | (q & 1) | ((row >> 1) & 3) << 1; }
 
 template <int HD, int W, int U> struct Q4Smem {      // (the warps' sums lie over the drained ring)
-    static constexpr int TILE = 16 * W * U, STAGES = U == 1 ? 4 : 3, RING = W * STAGES * U * Q4Stage<HD>::BYTES, MERGE = W * QA_ROWS * (HD + 4) * 4 + W * QA_ROWS * 16, BYTES = RING > MERGE ? RING : MERGE;
+    static constexpr int TILE = 16 * W * U, STAGES = QA_STAGES, RING = W * STAGES * U * Q4Stage<HD>::BYTES, MERGE = W * QA_ROWS * (HD + 4) * 4 + W * QA_ROWS * 16, BYTES = RING > MERGE ? RING : MERGE;
 };
 
 template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32 * W, QA_WARPS / W) attention_q4_kernel(const b200_q4_attention a, uint64_t page16, int64_t limit) {
@@ -164,7 +170,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
         if (tid == 0) ends->rows = 0;
         return;
     }
-    const long long c0 = total * blockIdx.x / grid, c1 = total * (blockIdx.x + 1) / grid;
+    const long long c0 = q4_begin(total, blockIdx.x, (int)grid), c1 = q4_begin(total, blockIdx.x + 1, (int)grid);
     if (before <= c0 && c0 < before + mine) {
         long long at = c0 - before;
         for (int s = s_beg; s < s_end; s++) {
@@ -176,8 +182,9 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
                 if (at >= (long long)per * nkv) { at -= (long long)per * nkv; continue; }
                 s_item[0] = s;
                 s_item[1] = rb;
-                s_item[2] = (int)(at / per);
-                s_item[3] = (int)(at % per);
+                const int head = (int)(at >> 32 ? at / per : (uint32_t)at / (uint32_t)per);
+                s_item[2] = head;
+                s_item[3] = (int)(at - (long long)head * per);
                 break;
             }
             break;
@@ -233,8 +240,14 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
         auto look = [&]() {
 #pragma unroll
             for (int b = 0; b < U; b++) {
-                const bool over = row_look + 16 * b >= page_size;
-                row[b] = row_look + 16 * b - (over ? page_size : 0);
+                int over = 0;      // pages further on
+                row[b] = row_look + 16 * b;
+#pragma unroll
+                for (int i = 0; i < b; i++)
+                    if (row[b] >= page_size) {
+                        row[b] -= page_size;
+                        over++;
+                    }
                 if (p_look + 16 * b < p_stop) page[b] = table[index + over];
             }
             p_look += TILE;
@@ -583,7 +596,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
         if (first && tile > 0 && stop == sp.tiles) {      // (a part, and the last one)
             // the block that has the first tile; this item is its first one unless its stretch begins ahead of the item
             end.first_cta = (int)(((start + QA_START + 1) * grid - 1) / total);
-            end.first_slot = total * end.first_cta / grid < start;
+            end.first_slot = q4_begin(total, end.first_cta, (int)grid) < start;
             end.token = q.first;
             end.rb = rb;
             end.head = h;
@@ -599,7 +612,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
 // Joins the parts of the items that ended in a block's first stretch: block (x, y) = that block, a row.
 template <typename T, int HD> __global__ void __launch_bounds__(256) attention_q4_join_kernel(const b200_q4_attention a, int grid) {
     before();
-    constexpr int LANES = HD / 4, GROUPS = 256 / LANES, PART = q4_part_floats<HD>(), AHEAD = 5;
+    constexpr int LANES = HD / 4, GROUPS = 256 / LANES, PART = q4_part_floats<HD>(), AHEAD = 8;
     __shared__ __align__(16) float s_o[GROUPS][HD];
     __shared__ float s_l[GROUPS];
     const float* ws = reinterpret_cast<const float*>(a.workspace);
