@@ -23,7 +23,7 @@ enum { QP_ROWS = 128, QP_KEYS = 128, QP_SOFT = 8, QP_MAKE = 8, QP_MMA = 16, QP_T
 template <typename T, int HD> struct Q4PromptSmem {
     static constexpr int NQ = sizeof(T) == 4 ? 2 : 1;
     static constexpr int SLAB = 128 * 128, Q = NQ * (HD / 64) * SLAB, K = (HD / 64) * SLAB, V = 2 * HD * 128;      // rows of 128 bytes, SWIZZLE_128B
-    static constexpr int K_AT = Q, V_AT = K_AT + 2 * K, META_AT = V_AT + 2 * V, META = 128 * 4 * 2 + 16, STAT_AT = META_AT + 4 * META, BAR_AT = STAT_AT + 2 * 128 * 8, BYTES = BAR_AT + 16 * 8;
+    static constexpr int K_AT = Q, V_AT = K_AT + 2 * K, META_AT = V_AT + 2 * V, META = 128 * 4 * 2 + 16, STAT_AT = META_AT + 4 * META, BAR_AT = STAT_AT + 2 * 128 * 8, BARS = 21, BYTES = BAR_AT + 2 * BARS * 8;
 };
 template <bool BF> __device__ __forceinline__ uint32_t sub_2(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -111,7 +111,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
     constexpr int NQ = Sm::NQ, SLABS = HD / 64;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_item[2];
+    __shared__ int s_item[2], s_bad;
     uint8_t* smem = smem_raw + ((1024u - (sm_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t base = sm_u32(smem);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nkv = a.cache.n_kv_heads, G = a.n_heads / nkv, page_size = a.cache.page_size;
@@ -146,19 +146,14 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
             s_item[1] = rb;
         }
     }
-    const uint32_t bars = base + Sm::BAR_AT;
-    const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64, p_full = bars + 80, pv_done = bars + 96;
-    if (tid == 32) {
-        for (int i = 0; i < 2; i++) {
-            bar_init(k_full + 8 * i, QP_MMA - QP_MAKE);
-            bar_init(k_empty + 8 * i, 1);
-            bar_init(v_full + 8 * i, QP_MMA - QP_MAKE);
-            bar_init(v_empty + 8 * i, 1);
-            bar_init(s_full + 8 * i, 1);
-            bar_init(p_full + 8 * i, 4);
-            bar_init(pv_done + 8 * i, 1);
+    // barriers of either pass (see below): keys there, used; values there, used (2 each); scores there (6); weights there, their products done (3 each); all products done
+    if (warp == 1) {
+        for (int i = lane; i < 2 * Sm::BARS; i += 32) {
+            const int b = i % Sm::BARS;
+            bar_init(base + Sm::BAR_AT + 8 * i, b < 2 || b == 4 || b == 5 ? QP_MMA - QP_MAKE : b >= 14 && b < 17 ? 4 : 1);
         }
         bar_init_done();
+        if (lane == 0) s_bad = 0;
     }
     __syncthreads();
     const int s = s_item[0], rb = s_item[1];
@@ -229,347 +224,407 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
     const uint32_t tmem = s_tmem;
     bool alive = true;
 
-    if (warp >= QP_MAKE && warp < QP_MMA) {
-        // ---- operands of keys and values
-        const int pw = warp - QP_MAKE;
-        constexpr int CH = HD / 32, PER = 32 / CH;              // 16-byte words of a row; rows a warp reads at once
-        constexpr int KN = 16 / PER, VW = HD / 32;              // 16-byte words of keys per thread; 32-bit words of each of two values
-        const int block = page_size * (HD + 8), v_off = page_size * (HD / 2);
-        const uint8_t* head = reinterpret_cast<const uint8_t*>(a.cache.data) + (int64_t)h * block;
-        const int64_t page_bytes = (int64_t)nkv * block;
-        const int32_t* table = a.page_table + (int64_t)s * a.table_stride;
-        uint32_t mask = 0x000f000fu;
-        asm("" : "+r"(mask));      // (kept in a register: an instruction has room for one constant)
-        // Lane l looks after the sixteen positions l & 7 of a tile: the page is looked up two tiles ahead, the rows are asked for one tile ahead.
-        int page = 0, row = 0;
-        bool wanted = false;
-        auto look = [&](int t) {
-            const int p = begin + t * QP_KEYS + 16 * (lane & 7);
-            wanted = t < n && p < hi;
-            if (wanted) {
-                const int index = (int)(((uint64_t)(p >> 4) * page16) >> 36);
-                row = p - index * page_size;
-                page = table[index];
-            }
-        };
-        struct Raw {
-            uint4 k[KN];
-            uint32_t v[2][VW];
-            float scale;      // of key 16 pw + lane, or of the value there (lanes from 16 on)
-            bool there;
-        } raw, next;
-        // this warp's keys: the sixteen pw; its values: pairs of half the tile's positions, a quarter of the channels
-        const int v_key = 64 * (pw & 1) + 2 * lane, v_word = (pw >> 1) * VW;
-        auto ask = [&](int t, Raw& w) {
-            const bool good = wanted && (unsigned)page < (uint64_t)a.cache.n_pages;
-            if (wanted && !good && a.status) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
-            const unsigned long long mine = good ? (unsigned long long)(head + page * page_bytes) : 0ull;
-            const int my_row = row;
-            look(t + 1);
-            auto of = [&](int g, int& r) {
-                r = __shfl_sync(0xffffffffu, my_row, g);
-                return reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, mine, g));
+    // One pass over the keys.  steady: references stay where a row's first tiles put them, so that the tiles do not depend on one another: one O, three buffers of scores.  Otherwise they move, with
+    // sums of each group's own.
+    auto pass = [&](auto mode) {
+        constexpr bool steady = decltype(mode)::value;
+        const uint32_t bars = base + Sm::BAR_AT + (steady ? 0 : Sm::BARS * 8);
+        const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64, p_full = bars + 112, pv_done = bars + 136, all_done = bars + 160;
+        if (warp >= QP_MAKE && warp < QP_MMA) {
+            // ---- operands of keys and values
+            const int pw = warp - QP_MAKE;
+            constexpr int CH = HD / 32, PER = 32 / CH;              // 16-byte words of a row; rows a warp reads at once
+            constexpr int KN = 16 / PER, VW = HD / 32;              // 16-byte words of keys per thread; 32-bit words of each of two values
+            const int block = page_size * (HD + 8), v_off = page_size * (HD / 2);
+            const uint8_t* head = reinterpret_cast<const uint8_t*>(a.cache.data) + (int64_t)h * block;
+            const int64_t page_bytes = (int64_t)nkv * block;
+            const int32_t* table = a.page_table + (int64_t)s * a.table_stride;
+            uint32_t mask = 0x000f000fu;
+            asm("" : "+r"(mask));      // (kept in a register: an instruction has room for one constant)
+            // Lane l looks after the sixteen positions l & 7 of a tile: the page is looked up two tiles ahead, the rows are asked for one tile ahead.
+            int page = 0, row = 0;
+            bool wanted = false;
+            auto look = [&](int t) {
+                const int p = begin + t * QP_KEYS + 16 * (lane & 7);
+                wanted = t < n && p < hi;
+                if (wanted) {
+                    const int index = (int)(((uint64_t)(p >> 4) * page16) >> 36);
+                    row = p - index * page_size;
+                    page = table[index];
+                }
             };
-            int rk, rv;
-            const uint8_t *kb = of(pw, rk), *vb = of(v_key >> 4, rv);
-#pragma unroll
-            for (int i = 0; i < KN; i++)
-                w.k[i] = kb ? *reinterpret_cast<const uint4*>(kb + (rk + i * PER + lane / CH) * (HD / 2) + (lane % CH) * 16) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                struct __align__(4 * VW) W { uint32_t x[VW]; };
-                W x{};
-                if (vb) x = *reinterpret_cast<const W*>(vb + v_off + (rv + (v_key & 15) + u) * (HD / 2) + v_word * 4);
-#pragma unroll
-                for (int i = 0; i < VW; i++) w.v[u][i] = x.x[i];
-            }
-            w.there = kb != nullptr && begin + t * QP_KEYS + 16 * pw + (lane & 15) < hi;
-            w.scale = w.there ? reinterpret_cast<const float*>(kb + 2 * v_off)[rk + (lane & 15) + (lane < 16 ? 0 : page_size)] : 0.0f;
-        };
-        auto make_keys = [&](int t, const Raw& w) {
-            const uint32_t kt = base + Sm::K_AT + (t & 1) * Sm::K;
-#pragma unroll
-            for (int i = 0; i < KN; i++) {
-                const int r = pw * 16 + i * PER + lane / CH;
-                const uint32_t x[4] = {w.k[i].x, w.k[i].y, w.k[i].z, w.k[i].w};
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int g = (lane % CH) * 4 + j;          // eight channels
-                    sts128(kt + (g >> 3) * Sm::SLAB + r * 128 + (((g & 7) ^ (r & 7)) << 4), nibbles<BF>(x[j], mask), nibbles<BF>(x[j] >> 4, mask),
-                           nibbles<BF>(x[j] >> 8, mask), nibbles<BF>(x[j] >> 12, mask));
-                }
-            }
-            uint8_t* meta = smem + Sm::META_AT + (t & 3) * Sm::META;
-            reinterpret_cast<float*>(meta)[(lane < 16 ? 0 : 128) + 16 * pw + (lane & 15)] = w.scale;
-            const uint32_t gone = ~__ballot_sync(0xffffffffu, w.there);
-            if (lane == 0) reinterpret_cast<uint16_t*>(meta + 1024)[pw] = (uint16_t)gone;
-        };
-        auto make_values = [&](int t, const Raw& w) {
-            const uint32_t vt = base + Sm::V_AT + (t & 1) * Sm::V + (pw & 1) * (HD * 128) + (lane & 3) * 4;
-            const uint32_t c8 = lane >> 2;
-#pragma unroll
-            for (int j = 0; j < VW; j++) {
-                const uint32_t x[2] = {__byte_perm(w.v[0][j], w.v[1][j], 0x5410), __byte_perm(w.v[0][j], w.v[1][j], 0x7632)};
-#pragma unroll
-                for (int k = 0; k < 8; k++) sts32(vt + ((v_word + j) * 8 + k) * 128 + ((c8 ^ k) << 4), nibbles<true>(x[k >> 2] >> (4 * (k & 3)), mask));
-            }
-        };
-        look(0);
-        if (n > 0) ask(0, raw);
-#pragma unroll 1
-        for (int t = 0; t < n; t++) {
-            if (t + 1 < n) ask(t + 1, next);
-            const int st = t & 1;
-            const uint32_t ph = ((t >> 1) & 1) ^ 1u;
-            bar_wait(k_empty + 8 * st, ph, alive, 11);
-            make_keys(t, raw);
-            async_fence();
-            __syncwarp();
-            if (lane == 0) bar_arrive(k_full + 8 * st);
-            bar_wait(v_empty + 8 * st, ph, alive, 12);
-            make_values(t, raw);
-            async_fence();
-            __syncwarp();
-            if (lane == 0) bar_arrive(v_full + 8 * st);
-            raw = next;
-        }
-    } else if (warp == QP_MMA) {
-        const uint32_t iqk = f16_idesc(BF, 128, QP_KEYS), ipv = f16_idesc(true, 128, HD);
-        auto scores = [&](int t) {
-            const int st = t & 1;
-            bar_wait(k_full + 8 * st, (t >> 1) & 1, alive, 13);
-            alive = __all_sync(0xffffffffu, alive);
-            umma_after_sync();
-            if (elect()) {
-                if (alive) {
-                    const uint64_t dk = umma_desc(base + Sm::K_AT + st * Sm::K);
-#pragma unroll
-                    for (int u = 0; u < NQ; u++)
-#pragma unroll
-                        for (int sl = 0; sl < SLABS; sl++)
-#pragma unroll
-                            for (int kk = 0; kk < 4; kk++)
-                                mma_ss(tmem + st * 128, umma_desc(base + (u * SLABS + sl) * Sm::SLAB) + 2 * kk, dk + (uint64_t)(sl * (Sm::SLAB >> 4) + 2 * kk), iqk, u + sl + kk > 0);
-                }
-                umma_commit<false>(k_empty + 8 * st);
-                umma_commit<false>(s_full + 8 * st);
-            }
-            __syncwarp();
-        };
-        for (int t = 0; t < min(n, 2); t++) scores(t);
-        for (int t = 0; t < n; t++) {
-            const int st = t & 1;
-            const uint32_t ph = (t >> 1) & 1;
-            bar_wait(v_full + 8 * st, ph, alive, 14);
-            bar_wait(p_full + 8 * st, ph, alive, 15);
-            alive = __all_sync(0xffffffffu, alive);
-            umma_after_sync();
-            if (elect()) {
-                if (alive) {
-                    const uint64_t dv = umma_desc(base + Sm::V_AT + st * Sm::V);
-#pragma unroll
-                    for (int kk = 0; kk < 8; kk++)
-#pragma unroll
-                        for (int u = 0; u < 2; u++)
-                            mma_ts(tmem + 256 + st * HD, tmem + st * 128 + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * u, dv + (uint64_t)((kk >> 2) * (HD * 128 >> 4) + 2 * (kk & 3)), ipv,
-                                   t >= 2 || kk + u > 0);
-                }
-                umma_commit<false>(v_empty + 8 * st);
-                umma_commit<false>(pv_done + 8 * st);
-            }
-            __syncwarp();
-            if (t + 2 < n) {
-                // (the scores of t + 2 go where the weights of t are)
-                bar_wait(pv_done + 8 * st, ph, alive, 16);
-                scores(t + 2);
-            }
-        }
-    } else {
-        // ---- rows
-        const int r = tid & 127, grp = warp >> 2, rr = rb * QP_ROWS + r, token = rr / G;
-        const bool live = r < rows;
-        const int row_hi = live ? (int)max((int64_t)0, at0 + token + 1) : INT32_MAX, row_lo = live && a.window > 0 ? (int)max((int64_t)0, at0 + token + 1 - a.window) : 0;
-        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), S = lanes + grp * 128, O = lanes + 256 + grp * HD;
-        float m = -INFINITY, l = 0.0f;
-        for (int t = grp; t < n; t += 2) {
-            const int p0 = begin + t * QP_KEYS;
-            const uint8_t* meta = smem + Sm::META_AT + (t & 3) * Sm::META;
-            bar_wait(s_full + 8 * grp, (t >> 1) & 1, alive, 17);
-            __syncwarp();
-            umma_after_sync();
-            const uint4 gone = *reinterpret_cast<const uint4*>(meta + 1024);
-            const bool all = p0 >= lo_max && p0 + QP_KEYS <= hi_min && !(gone.x | gone.y | gone.z | gone.w);      // (uniform)
-            // a bit per key of a batch of 32 that this row does not see
-            auto hidden = [&](int j) {
-                const int p = p0 + 32 * j, above = row_hi - p, below_ = row_lo - p;
-                uint32_t b = reinterpret_cast<const uint32_t*>(meta + 1024)[j];
-                if (above < 32) b |= above <= 0 ? 0xffffffffu : 0xffffffffu << above;
-                if (below_ > 0) b |= below_ >= 32 ? 0xffffffffu : ~(0xffffffffu << below_);
-                return b;
-            };
-            const float4* k4 = reinterpret_cast<const float4*>(meta);
-            // the largest score
-            auto largest = [&](auto whole) {
-                constexpr bool ALL = decltype(whole)::value;
-                float top[2] = {-INFINITY, -INFINITY};
-                auto take = [&](int j, const uint32_t (&v)[32]) {
-                    const uint32_t hid = ALL ? 0u : hidden(j);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float4 k = k4[8 * j + i];
-                        const float2 x = mul2(make_float2(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1])), make_float2(k.x, k.y)),
-                                     y = mul2(make_float2(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])), make_float2(k.z, k.w));
-                        if (ALL) {
-                            top[0] = fmaxf(fmaxf(x.x, x.y), top[0]);
-                            top[1] = fmaxf(fmaxf(y.x, y.y), top[1]);
-                        } else {
-                            const float z[4] = {x.x, x.y, y.x, y.y};
-#pragma unroll
-                            for (int u = 0; u < 4; u++)
-                                if (!((hid >> (4 * i + u)) & 1u)) top[0] = fmaxf(top[0], z[u]);
-                        }
-                    }
+            struct Raw {
+                uint4 k[KN];
+                uint32_t v[2][VW];
+                float scale;      // of key 16 pw + lane, or of the value there (lanes from 16 on)
+                bool there;
+            } raw, next;
+            // this warp's keys: the sixteen pw; its values: pairs of half the tile's positions, a quarter of the channels
+            const int v_key = 64 * (pw & 1) + 2 * lane, v_word = (pw >> 1) * VW;
+            auto ask = [&](int t, Raw& w) {
+                const bool good = wanted && (unsigned)page < (uint64_t)a.cache.n_pages;
+                if (wanted && !good && a.status) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
+                const unsigned long long mine = good ? (unsigned long long)(head + page * page_bytes) : 0ull;
+                const int my_row = row;
+                look(t + 1);
+                auto of = [&](int g, int& r) {
+                    r = __shfl_sync(0xffffffffu, my_row, g);
+                    return reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, mine, g));
                 };
-                by_32(S, take);
-                return fmaxf(top[0], top[1]);
-            };
-            // the reference goes up by `up` (a whole number, or 0): the sums so far, and the weights of the tile's first `cols` columns, are 2^-up times what they were
-            auto raise = [&](float up, int cols, float2& sum) {
-                const float f = ex2(-up);
-                m += up;
-                l *= f;
-                sum = mul2(sum, make_float2(f, f));
-                uint32_t v[16];
-#pragma unroll 1
-                for (int j = 0; t >= 2 && j < HD; j += 16) {      // (the group's products so far are done: the scores came after them)
-                    tmem_ask16(v, O + j);
-                    tmem_got(v);
+                int rk, rv;
+                const uint8_t *kb = of(pw, rk), *vb = of(v_key >> 4, rv);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                    tmem_st16(O + j, v);
-                }
-                tmem_st_done();
-#pragma unroll 1
-                for (int j = 0; j < cols; j += 16) {
-                    tmem_ask16(v, S + j);
-                    tmem_got(v);
+                for (int i = 0; i < KN; i++)
+                    w.k[i] = kb ? *reinterpret_cast<const uint4*>(kb + (rk + i * PER + lane / CH) * (HD / 2) + (lane % CH) * 16) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) v[i] = pack_bf2(__uint_as_float(v[i] << 16) * f, __uint_as_float(v[i] & 0xffff0000u) * f);
-                    tmem_st16(S + j, v);
+                for (int u = 0; u < 2; u++) {
+                    struct __align__(4 * VW) W { uint32_t x[VW]; };
+                    W x{};
+                    if (vb) x = *reinterpret_cast<const W*>(vb + v_off + (rv + (v_key & 15) + u) * (HD / 2) + v_word * 4);
+#pragma unroll
+                    for (int i = 0; i < VW; i++) w.v[u][i] = x.x[i];
                 }
-                tmem_st_done();
+                w.there = kb != nullptr && begin + t * QP_KEYS + 16 * pw + (lane & 15) < hi;
+                w.scale = w.there ? reinterpret_cast<const float*>(kb + 2 * v_off)[rk + (lane & 15) + (lane < 16 ? 0 : page_size)] : 0.0f;
             };
-            if (__any_sync(0xffffffffu, m == -INFINITY)) {
-                // (alpha = 0: 0, or NaN where nothing is seen, which sets nothing)
-                const float top = (all ? largest(std::true_type{}) : largest(std::false_type{})) * alpha;
-                if (m == -INFINITY) m = fmaxf(m, top);
+            auto make_keys = [&](int t, const Raw& w) {
+                const uint32_t kt = base + Sm::K_AT + (t & 1) * Sm::K;
+#pragma unroll
+                for (int i = 0; i < KN; i++) {
+                    const int r = pw * 16 + i * PER + lane / CH;
+                    const uint32_t x[4] = {w.k[i].x, w.k[i].y, w.k[i].z, w.k[i].w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int g = (lane % CH) * 4 + j;          // eight channels
+                        sts128(kt + (g >> 3) * Sm::SLAB + r * 128 + (((g & 7) ^ (r & 7)) << 4), nibbles<BF>(x[j], mask), nibbles<BF>(x[j] >> 4, mask),
+                               nibbles<BF>(x[j] >> 8, mask), nibbles<BF>(x[j] >> 12, mask));
+                    }
+                }
+                uint8_t* meta = smem + Sm::META_AT + (t & 3) * Sm::META;
+                reinterpret_cast<float*>(meta)[(lane < 16 ? 0 : 128) + 16 * pw + (lane & 15)] = w.scale;
+                const uint32_t gone = ~__ballot_sync(0xffffffffu, w.there);
+                if (lane == 0) reinterpret_cast<uint16_t*>(meta + 1024)[pw] = (uint16_t)gone;
+            };
+            auto make_values = [&](int t, const Raw& w) {
+                const uint32_t vt = base + Sm::V_AT + (t & 1) * Sm::V + (pw & 1) * (HD * 128) + (lane & 3) * 4;
+                const uint32_t c8 = lane >> 2;
+#pragma unroll
+                for (int j = 0; j < VW; j++) {
+                    const uint32_t x[2] = {__byte_perm(w.v[0][j], w.v[1][j], 0x5410), __byte_perm(w.v[0][j], w.v[1][j], 0x7632)};
+#pragma unroll
+                    for (int k = 0; k < 8; k++) sts32(vt + ((v_word + j) * 8 + k) * 128 + ((c8 ^ k) << 4), nibbles<true>(x[k >> 2] >> (4 * (k & 3)), mask));
+                }
+            };
+            look(0);
+            if (n > 0) ask(0, raw);
+#pragma unroll 1
+            for (int t = 0; t < n; t++) {
+                if (t + 1 < n) ask(t + 1, next);
+                const int st = t & 1;
+                const uint32_t ph = ((t >> 1) & 1) ^ 1u;
+                bar_wait(k_empty + 8 * st, ph, alive, 11);
+                make_keys(t, raw);
+                async_fence();
+                __syncwarp();
+                if (lane == 0) bar_arrive(k_full + 8 * st);
+                bar_wait(v_empty + 8 * st, ph, alive, 12);
+                make_values(t, raw);
+                async_fence();
+                __syncwarp();
+                if (lane == 0) bar_arrive(v_full + 8 * st);
+                raw = next;
             }
-            // the weights, in place of the scores: of 32 columns the first sixteen words are theirs, the others what those leave over
-            auto weights = [&](auto whole) {
-                constexpr bool ALL = decltype(whole)::value;
-                const float2 al = make_float2(alpha, alpha);
-                float ref = m == -INFINITY ? 0.0f : m;
-                float2 sum = make_float2(0.0f, 0.0f);
-                auto take = [&](int j, const uint32_t (&v)[32]) {
-                    const uint32_t hid = ALL ? 0u : hidden(j);
-                    float2 x[16];
+        } else if (warp == QP_MMA) {
+            const uint32_t iqk = f16_idesc(BF, 128, QP_KEYS), ipv = f16_idesc(true, 128, HD);
+            constexpr int nb = steady ? 3 : 2, ns = steady ? 6 : 2;      // buffers of scores, barriers of theirs
+            auto scores = [&](int t) {
+                const int st = t & 1;
+                bar_wait(k_full + 8 * st, (t >> 1) & 1, alive, 13);
+                alive = __all_sync(0xffffffffu, alive);
+                umma_after_sync();
+                const uint32_t to = tmem + (t % nb) * 128, done = s_full + 8 * (t % ns);
+                if (elect()) {
+                    if (alive) {
+                        const uint64_t dk = umma_desc(base + Sm::K_AT + st * Sm::K);
+#pragma unroll
+                        for (int u = 0; u < NQ; u++)
+#pragma unroll
+                            for (int sl = 0; sl < SLABS; sl++)
+#pragma unroll
+                                for (int kk = 0; kk < 4; kk++)
+                                    mma_ss(to, umma_desc(base + (u * SLABS + sl) * Sm::SLAB) + 2 * kk, dk + (uint64_t)(sl * (Sm::SLAB >> 4) + 2 * kk), iqk, u + sl + kk > 0);
+                    }
+                    umma_commit<false>(k_empty + 8 * st);
+                    umma_commit<false>(done);
+                }
+                __syncwarp();
+            };
+            for (int t = 0; t < min(n, 2); t++) scores(t);
+            for (int t = 0; t < n; t++) {
+                const int st = t & 1, b = t % nb;
+                bar_wait(v_full + 8 * st, (t >> 1) & 1, alive, 14);
+                bar_wait(p_full + 8 * b, (t / nb) & 1, alive, 15);
+                alive = __all_sync(0xffffffffu, alive);
+                umma_after_sync();
+                const uint32_t to = steady ? tmem + 384 : tmem + 256 + st * HD, from = tmem + b * 128;
+                if (elect()) {
+                    if (alive) {
+                        const uint64_t dv = umma_desc(base + Sm::V_AT + st * Sm::V);
+#pragma unroll
+                        for (int kk = 0; kk < 8; kk++)
+#pragma unroll
+                            for (int u = 0; u < 2; u++)
+                                mma_ts(to, from + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * u, dv + (uint64_t)((kk >> 2) * (HD * 128 >> 4) + 2 * (kk & 3)), ipv, t >= (steady ? 1 : 2) || kk + u > 0);
+                    }
+                    umma_commit<false>(v_empty + 8 * st);
+                    umma_commit<false>(pv_done + 8 * b);
+                    if (t == n - 1) umma_commit<false>(all_done);
+                }
+                __syncwarp();
+                if (t + 2 < n) {
+                    // the scores of t + 2 go where the weights of t (of t - 1, with three buffers) are
+                    const int was = steady ? t - 1 : t;
+                    if (was >= 0) bar_wait(pv_done + 8 * (was % nb), (was / nb) & 1, alive, 16);
+                    scores(t + 2);
+                }
+            }
+        } else {
+            // ---- rows
+            const int r = tid & 127, grp = warp >> 2, rr = rb * QP_ROWS + r, token = rr / G;
+            const bool live = r < rows;
+            const int row_hi = live ? (int)max((int64_t)0, at0 + token + 1) : INT32_MAX, row_lo = live && a.window > 0 ? (int)max((int64_t)0, at0 + token + 1 - a.window) : 0;
+            const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), O = lanes + 256 + grp * HD;
+            float* refs = reinterpret_cast<float*>(smem + Sm::STAT_AT);      // steady: after the first tile, after the second, then the two groups' sums
+            float m = -INFINITY, l = 0.0f;
+            bool bad = false, write = true;
+            for (int t = grp; t < n; t += 2) {
+                const int p0 = begin + t * QP_KEYS;
+                const uint8_t* meta = smem + Sm::META_AT + (t & 3) * Sm::META;
+                const int b = steady ? t % 3 : grp;
+                const uint32_t S = lanes + b * 128;
+                if (steady) bar_wait(s_full + 8 * (t % 6), (t / 6) & 1, alive, 17);
+                else bar_wait(s_full + 8 * grp, (t >> 1) & 1, alive, 17);
+                __syncwarp();
+                umma_after_sync();
+                const uint4 gone = *reinterpret_cast<const uint4*>(meta + 1024);
+                const bool all = p0 >= lo_max && p0 + QP_KEYS <= hi_min && !(gone.x | gone.y | gone.z | gone.w);      // (uniform)
+                // a bit per key of a batch of 32 that this row does not see
+                auto hidden = [&](int j) {
+                    const int p = p0 + 32 * j, above = row_hi - p, below_ = row_lo - p;
+                    uint32_t b = reinterpret_cast<const uint32_t*>(meta + 1024)[j];
+                    if (above < 32) b |= above <= 0 ? 0xffffffffu : 0xffffffffu << above;
+                    if (below_ > 0) b |= below_ >= 32 ? 0xffffffffu : ~(0xffffffffu << below_);
+                    return b;
+                };
+                const float4* k4 = reinterpret_cast<const float4*>(meta);
+                // the largest score
+                auto largest = [&](auto whole) {
+                    constexpr bool ALL = decltype(whole)::value;
                     float top[2] = {-INFINITY, -INFINITY};
+                    auto take = [&](int j, const uint32_t (&v)[32]) {
+                        const uint32_t hid = ALL ? 0u : hidden(j);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float4 k = k4[8 * j + i];
+                        for (int i = 0; i < 8; i++) {
+                            const float4 k = k4[8 * j + i];
+                            const float2 x = mul2(make_float2(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1])), make_float2(k.x, k.y)),
+                                         y = mul2(make_float2(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])), make_float2(k.z, k.w));
+                            if (ALL) {
+                                top[0] = fmaxf(fmaxf(x.x, x.y), top[0]);
+                                top[1] = fmaxf(fmaxf(y.x, y.y), top[1]);
+                            } else {
+                                const float z[4] = {x.x, x.y, y.x, y.y};
 #pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const float2 z = mul2(make_float2(__uint_as_float(v[4 * i + 2 * u]), __uint_as_float(v[4 * i + 2 * u + 1])), u ? make_float2(k.z, k.w) : make_float2(k.x, k.y));
-                            float2 y = fma2(z, al, make_float2(-ref, -ref));
-                            if (!ALL) {
-                                if ((hid >> (4 * i + 2 * u)) & 1u) y.x = -INFINITY;
-                                if ((hid >> (4 * i + 2 * u + 1)) & 1u) y.y = -INFINITY;
+                                for (int u = 0; u < 4; u++)
+                                    if (!((hid >> (4 * i + u)) & 1u)) top[0] = fmaxf(top[0], z[u]);
                             }
-                            x[2 * i + u] = y;
-                            top[u] = fmaxf(fmaxf(y.x, y.y), top[u]);
                         }
-                    }
-                    const float most = fmaxf(top[0], top[1]);
-                    if (__any_sync(0xffffffffu, most > 16.0f)) {
-                        const float up = most > 16.0f ? ceilf(most) : 0.0f;
-                        raise(up, 32 * j, sum);
-                        ref += up;
-#pragma unroll
-                        for (int i = 0; i < 16; i++) x[i] = add2(x[i], make_float2(-up, -up));
-                    }
-                    uint32_t o[32];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float4 d = k4[32 + 8 * j + i];
-#pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const float2 p = make_float2(ex2(x[2 * i + u].x), ex2(x[2 * i + u].y));
-                            float2 w = mul2(p, u ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
-                            if (!ALL) {      // (a scale that other rows see may be NaN)
-                                if ((hid >> (4 * i + 2 * u)) & 1u) w.x = 0.0f;
-                                if ((hid >> (4 * i + 2 * u + 1)) & 1u) w.y = 0.0f;
-                            }
-                            sum = add2(sum, p);
-                            const uint32_t b = pack_bf2(w.x, w.y);
-                            const float2 rest = fma2(make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)), make_float2(-1.0f, -1.0f), w);
-                            o[2 * i + u] = b;
-                            o[16 + 2 * i + u] = pack_bf2(rest.x, rest.y);
-                        }
-                    }
-                    tmem_st32(S + 32 * j, o);
+                    };
+                    by_32(S, take);
+                    return fmaxf(top[0], top[1]);
                 };
-                by_32(S, take);
-                l += sum.x + sum.y;
-            };
-            if (all) weights(std::true_type{});
-            else weights(std::false_type{});
-            tmem_st_done();
-            umma_before_sync();
-            __syncwarp();
-            if (lane == 0) bar_arrive(p_full + 8 * grp);
-        }
-        // ---- the two groups into one: each thread has its row's half of the channels
-        float2* stat = reinterpret_cast<float2*>(smem + Sm::STAT_AT);
-        stat[grp * 128 + r] = make_float2(m, l);
-        const int tiles = grp ? n / 2 : (n + 1) / 2;
-        if (tiles > 0) bar_wait(pv_done + 8 * grp, (tiles - 1) & 1, alive, 18);
-        __syncwarp();
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        __syncwarp();
-        umma_after_sync();
-        const float2 s0 = stat[r], s1 = stat[128 + r];
-        const float t2 = fmaxf(s0.x, s1.x), f0 = ex2(below(s0.x, t2)), f1 = ex2(below(s1.x, t2)), sum = s0.y * f0 + s1.y * f1, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        T* to = reinterpret_cast<T*>(a.out) + (q.first + token) * a.out_token + (h * G + rr - token * G) * a.out_head + grp * (HD / 2);
-        const bool vec = (reinterpret_cast<uintptr_t>(to) & 15) == 0;
+                // the reference goes up by `up` (a whole number, or 0): the sums so far, and the weights of the tile's first `cols` columns, are 2^-up times what they were
+                auto raise = [&](float up, int cols, float2& sum) {
+                    const float f = ex2(-up);
+                    m += up;
+                    l *= f;
+                    sum = mul2(sum, make_float2(f, f));
+                    uint32_t v[16];
 #pragma unroll 1
-        for (int j = 0; j < HD / 64; j++) {
-            float y[32];
+                    for (int j = 0; t >= 2 && j < HD; j += 16) {      // (the group's products so far are done: the scores came after them)
+                        tmem_ask16(v, O + j);
+                        tmem_got(v);
 #pragma unroll
-            for (int i = 0; i < 32; i++) y[i] = 0.0f;
-            if (n > 0) {
-                uint32_t v[32];
-                tmem_ld32(v, lanes + 256 + grp * (HD / 2) + 32 * j);
+                        for (int i = 0; i < 16; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                        tmem_st16(O + j, v);
+                    }
+                    tmem_st_done();
+#pragma unroll 1
+                    for (int j = 0; j < cols; j += 16) {
+                        tmem_ask16(v, S + j);
+                        tmem_got(v);
 #pragma unroll
-                for (int i = 0; i < 32; i++) y[i] = __uint_as_float(v[i]) * f0;
+                        for (int i = 0; i < 16; i++) v[i] = pack_bf2(__uint_as_float(v[i] << 16) * f, __uint_as_float(v[i] & 0xffff0000u) * f);
+                        tmem_st16(S + j, v);
+                    }
+                    tmem_st_done();
+                };
+                if (steady && t == 1) {
+                    asm volatile("bar.sync 2, 256;" ::: "memory");
+                    m = refs[r];
+                } else if (steady && t == 2) {
+                    asm volatile("bar.sync 3, 256;" ::: "memory");
+                    m = refs[128 + r];
+                }
+                if (steady ? t < 2 && __any_sync(0xffffffffu, m == -INFINITY) : __any_sync(0xffffffffu, m == -INFINITY)) {
+                    // (alpha = 0: 0, or NaN where nothing is seen, which sets nothing)
+                    const float top = (all ? largest(std::true_type{}) : largest(std::false_type{})) * alpha;
+                    if (m == -INFINITY) m = fmaxf(m, top);
+                }
+                if (steady && t < 2) {      // for the other group's first tile, or this one's next
+                    refs[128 * t + r] = m;
+                    __threadfence_block();
+                    if (t == 0 && n > 1) asm volatile("bar.arrive 2, 256;" ::: "memory");
+                    if (t == 1 && n > 2) asm volatile("bar.arrive 3, 256;" ::: "memory");
+                }
+                // the weights, in place of the scores: of 32 columns the first sixteen words are theirs, the others what those leave over
+                auto weights = [&](auto whole) {
+                    constexpr bool ALL = decltype(whole)::value;
+                    const float2 al = make_float2(alpha, alpha);
+                    float ref = m == -INFINITY ? 0.0f : m;
+                    float2 sum = make_float2(0.0f, 0.0f);
+                    auto take = [&](int j, const uint32_t (&v)[32]) {
+                        const uint32_t hid = ALL ? 0u : hidden(j);
+                        float2 x[16];
+                        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float4 k = k4[8 * j + i];
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                const float2 z = mul2(make_float2(__uint_as_float(v[4 * i + 2 * u]), __uint_as_float(v[4 * i + 2 * u + 1])), u ? make_float2(k.z, k.w) : make_float2(k.x, k.y));
+                                float2 y = fma2(z, al, make_float2(-ref, -ref));
+                                if (!ALL) {
+                                    if ((hid >> (4 * i + 2 * u)) & 1u) y.x = -INFINITY;
+                                    if ((hid >> (4 * i + 2 * u + 1)) & 1u) y.y = -INFINITY;
+                                }
+                                x[2 * i + u] = y;
+                                top[u] = fmaxf(fmaxf(y.x, y.y), top[u]);
+                            }
+                        }
+                        const float most = fmaxf(top[0], top[1]);
+                        if (steady) {
+                            bad |= most > 64.0f;
+                        } else if (__any_sync(0xffffffffu, most > 16.0f)) {
+                            const float up = most > 16.0f ? ceilf(most) : 0.0f;
+                            raise(up, 32 * j, sum);
+                            ref += up;
+#pragma unroll
+                            for (int i = 0; i < 16; i++) x[i] = add2(x[i], make_float2(-up, -up));
+                        }
+                        uint32_t o[32];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float4 d = k4[32 + 8 * j + i];
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                const float2 p = make_float2(ex2(x[2 * i + u].x), ex2(x[2 * i + u].y));
+                                float2 w = mul2(p, u ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
+                                if (!ALL) {      // (a scale that other rows see may be NaN)
+                                    if ((hid >> (4 * i + 2 * u)) & 1u) w.x = 0.0f;
+                                    if ((hid >> (4 * i + 2 * u + 1)) & 1u) w.y = 0.0f;
+                                }
+                                sum = add2(sum, p);
+                                const uint32_t b = pack_bf2(w.x, w.y);
+                                const float2 rest = fma2(make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)), make_float2(-1.0f, -1.0f), w);
+                                o[2 * i + u] = b;
+                                o[16 + 2 * i + u] = pack_bf2(rest.x, rest.y);
+                            }
+                        }
+                        tmem_st32(S + 32 * j, o);
+                    };
+                    by_32(S, take);
+                    l += sum.x + sum.y;
+                };
+                if (all) weights(std::true_type{});
+                else weights(std::false_type{});
+                tmem_st_done();
+                umma_before_sync();
+                __syncwarp();
+                if (lane == 0) bar_arrive(p_full + 8 * b);
             }
-            if (n > 1) {
-                uint32_t v[32];
-                tmem_ld32(v, lanes + 256 + HD + grp * (HD / 2) + 32 * j);
-#pragma unroll
-                for (int i = 0; i < 32; i++) y[i] = fmaf(__uint_as_float(v[i]), f1, y[i]);
+            // ---- each thread has its row's half of the channels
+            float f0 = 1.0f, f1 = 1.0f, sum;
+            if (steady) {
+                refs[256 + grp * 128 + r] = l;
+                if (n > 0) bar_wait(all_done, 0, alive, 18);
+                __syncwarp();
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                sum = refs[256 + r] + refs[384 + r];
+            } else {
+                float2* stat = reinterpret_cast<float2*>(refs);
+                stat[grp * 128 + r] = make_float2(m, l);
+                if (n > 0) bar_wait(all_done, 0, alive, 18);
+                __syncwarp();
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                const float2 s0 = stat[r], s1 = stat[128 + r];
+                const float top = fmaxf(s0.x, s1.x);
+                f0 = ex2(below(s0.x, top));
+                f1 = ex2(below(s1.x, top));
+                sum = s0.y * f0 + s1.y * f1;
             }
+            __syncwarp();
+            umma_after_sync();
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            T* to = reinterpret_cast<T*>(a.out) + (q.first + token) * a.out_token + (h * G + rr - token * G) * a.out_head + grp * (HD / 2);
+            const bool vec = (reinterpret_cast<uintptr_t>(to) & 15) == 0;
+            auto result = [&](int j, float (&y)[32]) {
 #pragma unroll
-            for (int i = 0; i < 32; i++) y[i] = sum == 0.0f ? 0.0f : y[i] * inv;
-            if (live) {
-                if (vec) store_n<T, 32, true>(to + 32 * j, y);
-                else store_n<T, 32, false>(to + 32 * j, y);
+                for (int i = 0; i < 32; i++) y[i] = 0.0f;
+                if (n > 0) {
+                    uint32_t v[32];
+                    tmem_ld32(v, lanes + (steady ? 384 : 256) + grp * (HD / 2) + 32 * j);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) y[i] = __uint_as_float(v[i]) * f0;
+                }
+                if (n > 1 && !steady) {
+                    uint32_t v[32];
+                    tmem_ld32(v, lanes + 256 + HD + grp * (HD / 2) + 32 * j);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) y[i] = fmaf(__uint_as_float(v[i]), f1, y[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i++) y[i] = sum == 0.0f ? 0.0f : y[i] * inv;
+            };
+            if (steady) {      // what is not finite here may be so under a reference that moves
+                float zero = sum * 0.0f;
+#pragma unroll 1
+                for (int j = 0; j < HD / 64; j++) {
+                    float y[32];
+                    result(j, y);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) zero = fmaf(y[i], 0.0f, zero);
+                }
+                if (__any_sync(0xffffffffu, live && (bad || zero != 0.0f)) && lane == 0) atomicOr(&s_bad, 1);
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (s_bad) write = false;
+            }
+#pragma unroll 1
+            for (int j = 0; write && j < HD / 64; j++) {
+                float y[32];
+                result(j, y);
+                if (live) {
+                    if (vec) store_n<T, 32, true>(to + 32 * j, y);
+                    else store_n<T, 32, false>(to + 32 * j, y);
+                }
             }
         }
-    }
-    __syncwarp();
-    umma_before_sync();
-    __syncthreads();
-    umma_after_sync();
+        __syncwarp();
+        umma_before_sync();
+        __syncthreads();
+        umma_after_sync();
+    };
+    pass(std::true_type{});
+    if (s_bad) pass(std::false_type{});      // a score passed its reference by 2^64, or a result is not finite
     if (warp == QP_MMA) tmem_free<false>(tmem, 512);
 }
 

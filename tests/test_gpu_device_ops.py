@@ -362,6 +362,14 @@ def test_attention_of_prompts(D, dtype, hd):
     check_attention(D, dtype, 2, 2, hd, 64, [40, 70], [90, 70])      # (more tokens than positions: the first ones see nothing)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_of_prompts_with_scores_far_apart(D, dtype):
+    """Scores of thousands, rising from tile to tile: a row's first tile says nothing about the others."""
+    check_attention(D, dtype, 4, 2, 64, 16, [300, 700], [100, 64], gain=1000.0)
+    check_attention(D, dtype, 4, 1, 128, 32, [600], [40], gain=400.0, window=300)
+    check_attention(D, dtype, 4, 1, 64, 32, [600], [40], gain=0.0)
+
+
 @pytest.mark.parametrize("q_len", [9, 50])
 def test_attention_of_several_tokens_with_bad_pages(D, q_len):
     lens = [300, 200]
