@@ -7,7 +7,8 @@
 //   warp 16     issues S = Q K^T (128 x 128, K = hd) and O += P V (N = hd, K = 128).
 //   warps 0-7   one thread per row, two groups of four warps that take every second tile with sums, maximum and statistics of their own, so that one group's exponentials run under the other's
 //               products; the two are joined at the end.  P goes back to tensor memory in place of S.
-// Keys' scales multiply the scores, values' scales the weights.  The weights are bf16 pairs (what the first leaves over is the second: 2^-17), since a weight p_j d_j needs f32's range; f32 queries are
+// Keys' scales multiply the scores, values' scales the weights.  The weights of f32 and f16 results are bf16 pairs (what the first leaves over is the second: 2^-16), since a weight p_j d_j needs f32's range; those of bf16 results are single
+// fp16 numbers (2^-11, an eighth of the result's own step) as long as that type's range holds them, and pairs in the second pass.  f32 queries are
 // pairs of fp16 numbers scaled by a power of two.  bf16 has f32's range, so that the reference of a row's exponentials need only be near: it is the largest score of the first tile
 // that the row sees, and moves (by a whole number, which no bf16 notices) when a score passes it by 2^16.  A tile's scores are so read once.
 // What bounds it: per tile and row 128 x (2 + 2) products of 128 (the values twice for the pairs), and 128 exponentials and their 10 instructions; a tile's MMAs alone are 1536 clocks at hd 128.
@@ -112,6 +113,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_item[2], s_bad;
+    __shared__ float s_above;
     uint8_t* smem = smem_raw + ((1024u - (sm_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t base = sm_u32(smem);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nkv = a.cache.n_kv_heads, G = a.n_heads / nkv, page_size = a.cache.page_size;
@@ -227,7 +229,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
     // One pass over the keys.  steady: references stay where a row's first tiles put them, so that the tiles do not depend on one another: one O, three buffers of scores.  Otherwise they move, with
     // sums of each group's own.
     auto pass = [&](auto mode) {
-        constexpr bool steady = decltype(mode)::value;
+        constexpr bool steady = decltype(mode)::value, ONE = steady && BF;      // ONE: weights of one fp16 number each, values in fp16
         const uint32_t bars = base + Sm::BAR_AT + (steady ? 0 : Sm::BARS * 8);
         const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64, p_full = bars + 112, pv_done = bars + 136, all_done = bars + 160;
         if (warp >= QP_MAKE && warp < QP_MMA) {
@@ -292,10 +294,12 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
 #pragma unroll
                 for (int i = 0; i < KN; i++) {
                     const int r = pw * 16 + i * PER + lane / CH;
-                    const uint32_t x[4] = {w.k[i].x, w.k[i].y, w.k[i].z, w.k[i].w};
+                    // (the second half of a row's lanes take their words in another order: the same chunk of both slabs is in the same banks)
+                    const bool far = HD == 128 && (lane & 2);
+                    const uint32_t x[4] = {far ? w.k[i].z : w.k[i].x, far ? w.k[i].w : w.k[i].y, far ? w.k[i].x : w.k[i].z, far ? w.k[i].y : w.k[i].w};
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const int g = (lane % CH) * 4 + j;          // eight channels
+                        const int g = (lane % CH) * 4 + (far ? j ^ 2 : j);          // eight channels
                         sts128(kt + (g >> 3) * Sm::SLAB + r * 128 + (((g & 7) ^ (r & 7)) << 4), nibbles<BF>(x[j], mask), nibbles<BF>(x[j] >> 4, mask),
                                nibbles<BF>(x[j] >> 8, mask), nibbles<BF>(x[j] >> 12, mask));
                     }
@@ -312,7 +316,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 for (int j = 0; j < VW; j++) {
                     const uint32_t x[2] = {__byte_perm(w.v[0][j], w.v[1][j], 0x5410), __byte_perm(w.v[0][j], w.v[1][j], 0x7632)};
 #pragma unroll
-                    for (int k = 0; k < 8; k++) sts32(vt + ((v_word + j) * 8 + k) * 128 + ((c8 ^ k) << 4), nibbles<true>(x[k >> 2] >> (4 * (k & 3)), mask));
+                    for (int k = 0; k < 8; k++) sts32(vt + ((v_word + j) * 8 + k) * 128 + ((c8 ^ k) << 4), nibbles<!ONE>(x[k >> 2] >> (4 * (k & 3)), mask));
                 }
             };
             look(0);
@@ -335,7 +339,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 raw = next;
             }
         } else if (warp == QP_MMA) {
-            const uint32_t iqk = f16_idesc(BF, 128, QP_KEYS), ipv = f16_idesc(true, 128, HD);
+            const uint32_t iqk = f16_idesc(BF, 128, QP_KEYS), ipv = f16_idesc(!ONE, 128, HD);
             constexpr int nb = steady ? 3 : 2, ns = steady ? 6 : 2;      // buffers of scores, barriers of theirs
             auto scores = [&](int t) {
                 const int st = t & 1;
@@ -373,8 +377,8 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
 #pragma unroll
                         for (int kk = 0; kk < 8; kk++)
 #pragma unroll
-                            for (int u = 0; u < 2; u++)
-                                mma_ts(to, from + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * u, dv + (uint64_t)((kk >> 2) * (HD * 128 >> 4) + 2 * (kk & 3)), ipv, t >= (steady ? 1 : 2) || kk + u > 0);
+                            for (int u = 0; u < (ONE ? 1 : 2); u++)
+                                mma_ts(to, ONE ? from + 8 * kk : from + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * u, dv + (uint64_t)((kk >> 2) * (HD * 128 >> 4) + 2 * (kk & 3)), ipv, t >= (steady ? 1 : 2) || kk + u > 0);
                     }
                     umma_commit<false>(v_empty + 8 * st);
                     umma_commit<false>(pv_done + 8 * b);
@@ -396,7 +400,8 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
             const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), O = lanes + 256 + grp * HD;
             float* refs = reinterpret_cast<float*>(smem + Sm::STAT_AT);      // steady: after the first tile, after the second, then the two groups' sums
             float m = -INFINITY, l = 0.0f;
-            bool bad = false, write = true;
+            float above = 0.0f;
+            bool write = true;
             for (int t = grp; t < n; t += 2) {
                 const int p0 = begin + t * QP_KEYS;
                 const uint8_t* meta = smem + Sm::META_AT + (t & 3) * Sm::META;
@@ -471,6 +476,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 if (steady && t == 1) {
                     asm volatile("bar.sync 2, 256;" ::: "memory");
                     m = refs[r];
+                    if (ONE) above = s_above;
                 } else if (steady && t == 2) {
                     asm volatile("bar.sync 3, 256;" ::: "memory");
                     m = refs[128 + r];
@@ -478,7 +484,16 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 if (steady ? t < 2 && __any_sync(0xffffffffu, m == -INFINITY) : __any_sync(0xffffffffu, m == -INFINITY)) {
                     // (alpha = 0: 0, or NaN where nothing is seen, which sets nothing)
                     const float top = (all ? largest(std::true_type{}) : largest(std::false_type{})) * alpha;
-                    if (m == -INFINITY) m = fmaxf(m, top);
+                    if (ONE && t == 0) {
+                        // the largest value scale of the tile, as a power of two: with the reference that much higher its weights are fp16 numbers of about one
+                        // (of those that are numbers: a row that sees another one makes a second pass necessary anyway)
+                        const float4 d = k4[32 + lane];
+                        auto size = [](float v) { return (__float_as_uint(v) & 0x7fffffffu) < kInfBits ? fabsf(v) : 0.0f; };
+                        const uint32_t big = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(size(d.x), size(d.y)), fmaxf(size(d.z), size(d.w)))));
+                        above = big ? (float)((int)(big >> 23) - 127) : 0.0f;
+                        if (tid == 0) s_above = above;
+                    }
+                    if (m == -INFINITY) m = fmaxf(m, top + above);
                 }
                 if (steady && t < 2) {      // for the other group's first tile, or this one's next
                     refs[128 * t + r] = m;
@@ -508,20 +523,18 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                                     if ((hid >> (4 * i + 2 * u + 1)) & 1u) y.y = -INFINITY;
                                 }
                                 x[2 * i + u] = y;
-                                top[u] = fmaxf(fmaxf(y.x, y.y), top[u]);
+                                if (!steady) top[u] = fmaxf(fmaxf(y.x, y.y), top[u]);
                             }
                         }
                         const float most = fmaxf(top[0], top[1]);
-                        if (steady) {
-                            bad |= most > 64.0f;
-                        } else if (__any_sync(0xffffffffu, most > 16.0f)) {
+                        if (!steady && __any_sync(0xffffffffu, most > 16.0f)) {
                             const float up = most > 16.0f ? ceilf(most) : 0.0f;
                             raise(up, 32 * j, sum);
                             ref += up;
 #pragma unroll
                             for (int i = 0; i < 16; i++) x[i] = add2(x[i], make_float2(-up, -up));
                         }
-                        uint32_t o[32];
+                        uint32_t o[ONE ? 16 : 32];
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             const float4 d = k4[32 + 8 * j + i];
@@ -534,13 +547,18 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                                     if ((hid >> (4 * i + 2 * u + 1)) & 1u) w.y = 0.0f;
                                 }
                                 sum = add2(sum, p);
-                                const uint32_t b = pack_bf2(w.x, w.y);
-                                const float2 rest = fma2(make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)), make_float2(-1.0f, -1.0f), w);
-                                o[2 * i + u] = b;
-                                o[16 + 2 * i + u] = pack_bf2(rest.x, rest.y);
+                                if constexpr (ONE) {
+                                    o[2 * i + u] = pack_h2(w.x, w.y);
+                                } else {
+                                    const uint32_t b = pack_bf2(w.x, w.y);
+                                    const float2 rest = fma2(make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)), make_float2(-1.0f, -1.0f), w);
+                                    o[2 * i + u] = b;
+                                    o[16 + 2 * i + u] = pack_bf2(rest.x, rest.y);
+                                }
                             }
                         }
-                        tmem_st32(S + 32 * j, o);
+                        if constexpr (ONE) tmem_st16(S + 16 * j, o);      // (over columns that have been read)
+                        else tmem_st32(S + 32 * j, o);
                     };
                     by_32(S, take);
                     l += sum.x + sum.y;
@@ -595,16 +613,24 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
 #pragma unroll
                 for (int i = 0; i < 32; i++) y[i] = sum == 0.0f ? 0.0f : y[i] * inv;
             };
-            if (steady) {      // what is not finite here may be so under a reference that moves
-                float zero = sum * 0.0f;
+            if (steady) {
+                // what is not finite may be so under a reference that moves; sums of fp16 weights that are far below one have lost bits
+                float zero = sum * 0.0f, most = 0.0f;
 #pragma unroll 1
                 for (int j = 0; j < HD / 64; j++) {
                     float y[32];
                     result(j, y);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) zero = fmaf(y[i], 0.0f, zero);
+                    for (int i = 0; i < 32; i++) {
+                        zero = fmaf(y[i], 0.0f, zero);
+                        most = fmaxf(most, fabsf(y[i]));
+                    }
                 }
-                if (__any_sync(0xffffffffu, live && (bad || zero != 0.0f)) && lane == 0) atomicOr(&s_bad, 1);
+                if (ONE) refs[grp * 128 + r] = m == -INFINITY ? -1.0f : most;      // (-1: the row has seen nothing, as far as this group knows)
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                const float size = ONE ? fmaxf(refs[r], refs[128 + r]) : 0.0f;
+                const bool small = ONE && size >= 0.0f && !(size * sum >= 0.015625f);
+                if (__any_sync(0xffffffffu, live && (small || zero != 0.0f)) && lane == 0) atomicOr(&s_bad, 1);
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 if (s_bad) write = false;
             }

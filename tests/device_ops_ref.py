@@ -68,9 +68,10 @@ def attention(q, kv, table, lens, starts, page, scale, window, n_pages, dtype=to
     With Z the largest sum of |scale q_c k_c| of a row's scores: an f32 sum of a head's products by tensor-pipe steps of 16 is off by at most hd / 16 * 2^-22 Z (each step
     may cut its products off at the 23rd bit of the largest), the query's two halves add 2^-22 Z, the scale 2^-23 Z; a probability is then off by that times itself (twice: in the
     sum too), by 2^-21 from the exponential's argument and value and 2^-21 from its own two halves (bf16 results: 2^-11 from its one;
-    sequences of more than 32 rows of a kv head: two bf16 numbers, 2^-8 of 2^-8), and the sum over L keys by L / 16 * 2^-22 of sum p |v|.
+    f32 and f16 results of sequences of more than 32 rows of a kv head: two bf16 numbers, 2^-8 of 2^-8), and the sum over L keys by L / 16 * 2^-22 of sum p |v|.
     The two fp16 halves of a weight p d (d a value's scale) end at 2^-24 of a reference that the largest weight reaches: whatever its size, a weight is off by 2^-25 of the largest, and a
-    value is at most 8 d, so that a channel whose large weights meet values of zero keeps L * 2^-25 * 8 max(p d) = L * 2^-25 * max(p max |v|)."""
+    value is at most 8 d, so that a channel whose large weights meet values of zero keeps L * 2^-25 * 8 max(p d) = L * 2^-25 * max(p max |v|).  (bf16 results of many rows: the reference is
+    the largest score of the first tile with the largest scale of a value there, whose own score may be small: L * 2^-25 * max |v| of the sequence.)"""
     k, v = kv
     o = torch.zeros(q.shape, dtype=torch.float64)
     off = torch.zeros(q.shape, dtype=torch.float64)
@@ -78,6 +79,9 @@ def attention(q, kv, table, lens, starts, page, scale, window, n_pages, dtype=to
     g = nh // k.shape[1]
     for s in range(len(lens)):
         n, a, b = lens[s], starts[s], starts[s + 1]
+        many = (b - a) * g > 32
+        held = [table[s][j // page] * page + j % page for j in range(n) if 0 <= table[s][j // page] < n_pages]
+        far = torch.nan_to_num(v[torch.tensor(held)]).abs().max() if held else 0.0
         for i, t in enumerate(range(a, b)):
             pos = n - (b - a) + i
             keys = [j for j in range(max(0, pos - window + 1) if window else 0, pos + 1)]
@@ -92,5 +96,5 @@ def attention(q, kv, table, lens, starts, page, scale, window, n_pages, dtype=to
                 big = float(((kk.abs() @ q[t, h].abs()) * abs(scale)).max())
                 o[t, h] = p @ vv
                 dz = big * (hd / 16 * 2.0**-22 + 2.0**-22 + 2.0**-23 + 2.0**-22)
-                off[t, h] = (p @ vv.abs()) * (2 * dz + (2.0**-16 if (b - a) * g > 32 else 2.0**-11 if dtype == torch.bfloat16 else 0) + 2.0**-20 + len(keys) / 16 * 2.0**-22) + len(keys) * 2.0**-25 * (p * vv.abs().amax(1)).max()
+                off[t, h] = (p @ vv.abs()) * (2 * dz + (2.0**-11 if dtype == torch.bfloat16 else 2.0**-16 if many else 0) + 2.0**-20 + len(keys) / 16 * 2.0**-22) + len(keys) * 2.0**-25 * (far if many and dtype == torch.bfloat16 else (p * vv.abs().amax(1)).max())
     return o, off
