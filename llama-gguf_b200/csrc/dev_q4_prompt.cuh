@@ -655,24 +655,29 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
 }
 
 // ------------------------------------------------------------------------------------------------------------------- host
-// Sequences with more rows than this go to attention_q4_prompt_kernel.
+// Sequences with more rows than this go to attention_q4_prompt_kernel, where a call's rows make it worth while.
 constexpr int64_t kPromptRows = 32;
+// blocks of 128 rows of a kv head, at most: whole ones, and a last one of each sequence that has more rows than kPromptRows
+inline int64_t attention_q4_prompt_blocks(const b200_q4_attention& a) {
+    const int64_t rows = a.tokens * (a.n_heads / a.cache.n_kv_heads);
+    return rows / QP_ROWS + std::min<int64_t>(a.seqs, rows / (kPromptRows + 1));
+}
+// Whether a call's long sequences go there, by what the host knows.  A block of 128 rows takes 2.0 us for 128 keys, whether alone or on every SM; the other kernel 0.68 us of an SM for eight rows, but spreads any
+// number of rows over all SMs.  So: (rows / 8) * 0.68 / 148 against 2.0 for every 148 blocks.  Measured (bf16, 32 heads over 8, hd 128, 4000 keys; rows of a kv head: us there, here): one sequence of 256
+// 61, 70; eight of 32 57, 70, of 64 93, 70; 64 sequences with 1000 keys of 24 84, 97, of 64 185, 104.
+inline bool attention_q4_has_prompts(const b200_q4_attention& a) {
+    const int64_t G = a.n_heads / a.cache.n_kv_heads, nkv = a.cache.n_kv_heads;
+    if (!a.q_starts || (a.max_q ? a.max_q : a.tokens) * G <= kPromptRows) return false;
+    return (a.tokens * G + 7) / 8 * nkv > 435 * ((attention_q4_prompt_blocks(a) * nkv + 147) / 148);
+}
 template <typename T, int HD> cudaError_t attention_q4_prompt(const b200_q4_attention& a, cudaStream_t st) {
     using Sm = Q4PromptSmem<T, HD>;
     static SmemAllowed allowed;
     const auto kernel = attention_q4_prompt_kernel<T, HD>;
     const cudaError_t e = allowed((const void*)kernel, Sm::BYTES + 1024);
     if (e != cudaSuccess) return e;
-    const int64_t G = a.n_heads / a.cache.n_kv_heads, rows = a.tokens * G;
-    // blocks of 128 rows: whole ones, and a last one of each sequence that has more rows than kPromptRows
-    const int64_t blocks = rows / QP_ROWS + std::min<int64_t>(a.seqs, rows / (kPromptRows + 1));
     const uint64_t d = (uint64_t)a.cache.page_size / 16, page16 = (((uint64_t)1 << 36) + d - 1) / d;
-    if (blocks == 0) return cudaSuccess;
-    return launch(kernel, dim3((unsigned)(blocks * a.cache.n_kv_heads)), QP_THREADS, Sm::BYTES + 1024, 1, st, a, page16, kPromptRows);
-}
-// Whether a call may have such sequences, as far as the host can tell.
-inline bool attention_q4_has_prompts(const b200_q4_attention& a) {
-    return a.q_starts && (a.max_q ? a.max_q : a.tokens) * (a.n_heads / a.cache.n_kv_heads) > kPromptRows;
+    return launch(kernel, dim3((unsigned)(attention_q4_prompt_blocks(a) * a.cache.n_kv_heads)), QP_THREADS, Sm::BYTES + 1024, 1, st, a, page16, kPromptRows);
 }
 template <typename T, int HD> cudaError_t attention_q4(const b200_q4_attention& a, cudaStream_t st) {
     const bool prompts = attention_q4_has_prompts(a);

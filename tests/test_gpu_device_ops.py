@@ -291,7 +291,7 @@ def test_attention_of_several_tokens(D, dtype, q_lens, lens):
 def test_attention_window(D, window):
     check_attention(D, torch.float32, 8, 2, 64, 16, [1, 333, 40], [1, 1, 1], window=window)
     check_attention(D, torch.bfloat16, 8, 2, 128, 32, [50, 333, 40], [50, 3, 20], window=window)
-    check_attention(D, torch.float16, 4, 2, 64, 32, [150, 333], [150, 140], window=window, max_q=150)
+    check_attention(D, torch.float16, 32, 16, 64, 32, [150, 333], [150, 140], window=window, max_q=150)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -305,18 +305,20 @@ def test_attention_of_large_scores_and_other_scales(D):
     check_attention(D, torch.float32, 4, 2, 64, 16, [300, 64], [1, 1], gain=60.0)
     check_attention(D, torch.float32, 4, 2, 64, 16, [300, 64], [1, 1], scale=-0.3)
     check_attention(D, torch.float32, 4, 2, 64, 16, [300, 64], [1, 1], scale=0.0)
-    check_attention(D, torch.bfloat16, 4, 2, 128, 16, [300, 164], [100, 64], gain=30.0)
+    check_attention(D, torch.bfloat16, 32, 16, 128, 16, [300, 164], [100, 64], gain=30.0)
+    check_attention(D, torch.bfloat16, 32, 16, 128, 16, [300, 164], [100, 64], scale=-0.3)
+    check_attention(D, torch.float16, 32, 16, 128, 16, [300, 164], [100, 64], scale=0.0)
 
 
 @pytest.mark.parametrize("magnitude", [2.0**-100, 1e-6, 1e6, 2.0**100])
-@pytest.mark.parametrize("q_lens", [[1, 1], [20, 17]])
-def test_attention_of_values_and_queries_of_any_magnitude(D, magnitude, q_lens):
+@pytest.mark.parametrize("q_lens,nkv", [([1, 1], 2), ([20, 17], 2), ([60, 17], 24)])
+def test_attention_of_values_and_queries_of_any_magnitude(D, magnitude, q_lens, nkv):
     """Scales pass through in 32 bits: nothing is rounded to a type of less range."""
-    pages, table = cache(5, [70, 20], 2, 64, 16)
+    pages, table = cache(5, [70, 20], nkv, 64, 16)
     ks, vs = R.sections(pages, 16, 64)[2:]
     vs.mul_(magnitude)
     starts = [0, q_lens[0], sum(q_lens)]
-    q = normal(9, starts[-1], 4, 64)
+    q = normal(9, starts[-1], 2 * nkv, 64)
     lens = torch.tensor([70, 20], dtype=torch.int32).cuda()
     for f in (1.0, magnitude):
         ks.mul_(1 / f)
@@ -327,11 +329,11 @@ def test_attention_of_values_and_queries_of_any_magnitude(D, magnitude, q_lens):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("q_len", [1, 5, 60])
-def test_attention_what_is_masked_is_not_seen(D, dtype, q_len):
+@pytest.mark.parametrize("q_len,nkv", [(1, 2), (5, 2), (60, 2), (60, 40)])
+def test_attention_what_is_masked_is_not_seen(D, dtype, q_len, nkv):
     """NaN and infinite rows behind a sequence's end or ahead of its windows change nothing; inside they make NaN of the rows that see them, and of no others."""
-    pages, table = cache(5, [270], 2, 64, 16)
-    lens, q = torch.tensor([270], dtype=torch.int32).cuda(), normal(9, q_len, 4, 64).to(dtype).cuda()
+    pages, table = cache(5, [270], nkv, 64, 16)
+    lens, q = torch.tensor([270], dtype=torch.int32).cuda(), normal(9, q_len, 2 * nkv, 64).to(dtype).cuda()
     starts, w = torch.tensor([0, q_len], dtype=torch.int32).cuda(), 20
     run = lambda window: D.attention_paged_q4(q, pages.cuda(), table.cuda(), lens, q_starts=starts, window=window)  # noqa: E731
     want = run(w)
@@ -355,27 +357,27 @@ def test_attention_what_is_masked_is_not_seen(D, dtype, q_len):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("hd", [64, 128])
 def test_attention_of_prompts(D, dtype, hd):
-    """More rows than a block has, tiles that end anywhere, groups of heads that do not divide a block's rows."""
-    check_attention(D, dtype, 4, 2, hd, 16, [129, 700], [129, 70])
-    check_attention(D, dtype, 7, 1, hd, 48, [400, 33, 5], [45, 33, 5])
-    check_attention(D, dtype, 5, 5, hd, 32, [257, 1], [200, 1], window=64)
-    check_attention(D, dtype, 2, 2, hd, 64, [40, 70], [90, 70])      # (more tokens than positions: the first ones see nothing)
+    """More rows than a block has, tiles that end anywhere, groups of heads that do not divide a block's rows; enough of them for the kernel of many rows."""
+    check_attention(D, dtype, 36, 12, hd, 16, [129, 700], [129, 70])
+    check_attention(D, dtype, 56, 8, hd, 48, [400, 33, 5], [45, 33, 5])
+    check_attention(D, dtype, 20, 20, hd, 32, [257, 1], [200, 1], window=64)
+    check_attention(D, dtype, 28, 28, hd, 64, [40, 70], [90, 70])      # (more tokens than positions: the first ones see nothing)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
 def test_attention_of_prompts_with_scores_far_apart(D, dtype):
     """Scores of thousands, rising from tile to tile: a row's first tile says nothing about the others."""
-    check_attention(D, dtype, 4, 2, 64, 16, [300, 700], [100, 64], gain=1000.0)
-    check_attention(D, dtype, 4, 1, 128, 32, [600], [40], gain=400.0, window=300)
-    check_attention(D, dtype, 4, 1, 64, 32, [600], [40], gain=0.0)
+    check_attention(D, dtype, 24, 12, 64, 16, [300, 700], [100, 64], gain=1000.0)
+    check_attention(D, dtype, 96, 24, 128, 32, [600], [40], gain=400.0, window=300)
+    check_attention(D, dtype, 96, 24, 64, 32, [600], [40], gain=0.0)
 
 
-@pytest.mark.parametrize("q_len", [9, 50])
-def test_attention_of_several_tokens_with_bad_pages(D, q_len):
+@pytest.mark.parametrize("q_len,nkv", [(9, 2), (50, 2), (50, 20)])
+def test_attention_of_several_tokens_with_bad_pages(D, q_len, nkv):
     lens = [300, 200]
-    pages, table = cache(5, lens, 2, 128, 16)
+    pages, table = cache(5, lens, nkv, 128, 16)
     table[0, 2], table[0, 9], table[1, 12] = -3, pages.shape[0], 2**31 - 1
-    q, status = normal(9, 2 * q_len, 4, 128).to(torch.bfloat16), torch.zeros(1, dtype=torch.int32).cuda()
+    q, status = normal(9, 2 * q_len, 2 * nkv, 128).to(torch.bfloat16), torch.zeros(1, dtype=torch.int32).cuda()
     starts = [0, q_len, 2 * q_len]
     got = D.attention_paged_q4(q.cuda(), pages.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), q_starts=torch.tensor(starts, dtype=torch.int32).cuda(), status=status)
     want, off = R.attention(q.double(), R.values(pages, 16, 128), table.tolist(), lens, starts, 16, 128**-0.5, 0, pages.shape[0], torch.bfloat16)
@@ -501,6 +503,61 @@ def test_a_layer_captured_and_replayed(D, dtype):
     torch.cuda.synchronize()
     for o, w in zip(outs, want):
         assert all(torch.equal(a, b) for a, b in zip(o, w))
+
+
+def test_two_calls_at_once_on_other_streams(D):
+    """Two streams, neither of them the default one, each with its own batch, and a third that reads results after an event."""
+    states = [layer_state(D, torch.bfloat16, [1, 1, 1], [0, 700, 37]), layer_state(D, torch.bfloat16, [30, 1, 9], [0, 640, 5])]
+    want = [[v.clone() for v in layer(D, s)] for s in states]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in states], [[], []]
+    for _ in range(10):
+        for i, (s, st) in enumerate(zip(states, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(layer(D, s))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for r in g:
+            assert all(torch.equal(a, b) for a, b in zip(r, w))
+
+
+def test_calls_from_two_threads(D):
+    import threading
+
+    s = layer_state(D, torch.float16, [30, 1, 9], [0, 640, 5])
+    want = [v.clone() for v in layer(D, s)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                r = layer(D, s)      # (both write the same rows into the cache)
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(r, want)):
+                    wrong.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_a_device_that_is_not_the_current_one(D):
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one GPU")
+    s = {k: v.to("cuda:1") for k, v in layer_state(D, torch.bfloat16, [30, 1, 9], [0, 64, 5]).items()}
+    with torch.cuda.device(1):
+        want = [v.clone() for v in layer(D, s)]
+    assert torch.cuda.current_device() == 0
+    assert all(torch.equal(a, b) for a, b in zip(layer(D, s), want)) and torch.cuda.current_device() == 0
+
+
+def test_what_the_host_says_of_the_longest_changes_no_more_than_rounding(D):
+    for max_q in (0, 1, 100, 10**6):
+        check_attention(D, torch.float16, 36, 12, 64, 16, [129, 300], [129, 70], max_q=max_q)
 
 
 def test_the_same_bits_every_time(D):
