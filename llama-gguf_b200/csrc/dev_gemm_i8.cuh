@@ -245,11 +245,22 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_split_kernel(const __gr
         if (warp < GI_EPI_WARPS) {
             const int c_beg = rank * rows / S, c_end = (rank + 1) * rows / S;
             const float ws = live ? g.ws[n] : 0.0f, bias = live && g.bias ? g.bias[n] : 0.0f;
-            for (int c = c_beg + (int)(threadIdx.x >> 7); c < c_end; c += 2) {
-                int sum = 0;
+            constexpr int AT_ONCE = 4;      // tokens whose sums a thread asks for together
+            for (int c0 = c_beg + (int)(threadIdx.x >> 7); c0 < c_end; c0 += 2 * AT_ONCE) {
+                int v[AT_ONCE][8], sum[AT_ONCE];
 #pragma unroll
-                for (int r = 0; r < 8; r++) sum += r < S ? peer_s32(ring + (uint32_t)(c * GI_M + row) * 4u, (uint32_t)r) : 0;
-                if (live) reinterpret_cast<T*>(g.out)[(int64_t)(t0 + c) * g.ldo + n] = i8_result<T>(sum, g.as[t0 + c], ws, bias);
+                for (int u = 0; u < AT_ONCE; u++)
+#pragma unroll
+                    for (int r = 0; r < 8; r++)
+                        if (r < S) v[u][r] = peer_s32(ring + (uint32_t)(min(c0 + 2 * u, c_end - 1) * GI_M + row) * 4u, (uint32_t)r);
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; u++) {
+                    sum[u] = 0;
+#pragma unroll
+                    for (int r = 0; r < 8; r++) sum[u] += r < S ? v[u][r] : 0;
+                    const int c = c0 + 2 * u;
+                    if (live && c < c_end) reinterpret_cast<T*>(g.out)[(int64_t)(t0 + c) * g.ldo + n] = i8_result<T>(sum[u], g.as[t0 + c], ws, bias);
+                }
             }
         }
         cluster_sync();      // nobody leaves while its sums are read
@@ -265,8 +276,11 @@ struct GemmI8Plan {
     int tn, splits;
     bool wide, pair;
 };
-// The kernel of least estimated clocks on 148 SMs: a step of 128 bytes of K costs the larger of its operand bytes at 64 a clock and its MMAs, a launch what its first bytes and its last epilogue
-// take.  Clusters of 8 do not tile the chip's groups of SMs: 112 of their CTAs run at once.
+// The kernel of least estimated time (ns) on 148 SMs, by what each one measured (bf16 results, weights from DRAM): a step of 128 bytes of K takes 225 + 0.4 TN (wide: 280 with 128 tokens, 361 with 256, 300 for a
+// pair), whatever its MMAs, since it is a step's copies that bound it; a launch 2300 + 20 TN for its first bytes and its last sums, the exchange of a cut 400 and 30 per token and CTA; a wide kernel's start and last tile
+// 5900, 8200 and 9500.  Clusters of 8 do not tile the chip's groups of SMs: 112 of their CTAs run at once.
+// Measured (us; t x n x k): 1 x 4096 x 4096 10.2 in one piece, 7.5 in two, 6.6 in four, 13.7 in eight; 160 x 4096 x 4096 in tiles of 64 tokens 11.9, of 128 13.8; 2048 x 2048 x 2048 wide 13.8, 128 and 14.9 of 128 tokens;
+// 384 x 14336 x 4096 28.6 in pairs, 32.8 and 33.6 without.
 inline GemmI8Plan gemm_i8_plan(int64_t t, int64_t k, int64_t n) {
     const int64_t steps = (k + GI_STEP - 1) / GI_STEP, mt = (n + GI_M - 1) / GI_M;
     GemmI8Plan best{128, 1, false, false};
@@ -275,18 +289,18 @@ inline GemmI8Plan gemm_i8_plan(int64_t t, int64_t k, int64_t n) {
         if (least < 0 || cost < least) { least = cost; best = p; }
     };
     for (int tn : {16, 32, 64, 128}) {
-        if (tn < 128 && t > tn) continue;
+        if (tn < 64 && t > tn) continue;
         for (int s : {1, 2, 4, 8}) {
-            if (s > 1 && steps < 2 * s) break;
+            if (s > steps) break;
             const int64_t fit = s == 8 ? 112 : s == 4 ? 140 : 148, waves = (mt * ((t + tn - 1) / tn) * s + fit - 1) / fit;
-            offer({tn, s, false, false}, waves * ((steps + s - 1) / s * (tn <= 32 ? 300 : tn == 64 ? 375 : 470) + 4500 + 18 * tn + (s > 1 ? 1000 + 24 * tn / s : 0)));
+            offer({tn, s, false, false}, 300 + waves * ((steps + s - 1) / s * (225 + 2 * tn / 5) + 2000 + 20 * tn + (s > 1 ? 400 + 30 * tn / s : 0)));
         }
         if (t <= tn) break;
     }
     if (t > 128) {
-        offer({128, 1, true, false}, 4500 + 17 * 128 + (mt * ((t + 127) / 128) + 147) / 148 * steps * 470);
-        offer({256, 1, true, false}, 4500 + 17 * 256 + (mt * ((t + 255) / 256) + 147) / 148 * steps * 750);
-        offer({256, 1, true, true}, 7500 + 17 * 256 + ((mt + 1) / 2 * ((t + 255) / 256) + 73) / 74 * steps * 680);
+        offer({128, 1, true, false}, 5900 + (mt * ((t + 127) / 128) + 147) / 148 * steps * 280);
+        offer({256, 1, true, false}, 8200 + (mt * ((t + 255) / 256) + 147) / 148 * steps * 361);
+        offer({256, 1, true, true}, 9500 + ((mt + 1) / 2 * ((t + 255) / 256) + 73) / 74 * steps * 300);
     }
     return best;
 }

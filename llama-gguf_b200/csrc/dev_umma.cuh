@@ -56,7 +56,7 @@ __device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
 }
 __device__ __forceinline__ int peer_s32(uint32_t addr, uint32_t rank) {
     int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at_rank(addr, rank)) : "memory");
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at_rank(addr, rank)));      // (behind a barrier: nothing to be ordered with)
     return v;
 }
 template <bool PAIR> __device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t cols) {      // one whole warp
