@@ -289,7 +289,7 @@ inline GemmI8Plan gemm_i8_plan(int64_t t, int64_t k, int64_t n) {
         if (least < 0 || cost < least) { least = cost; best = p; }
     };
     for (int tn : {16, 32, 64, 128}) {
-        if (tn < 64 && t > tn) continue;
+        if ((tn < 64 && t > tn) || (t + tn - 1) / tn > 65535) continue;      // (the grid's second dimension; such a call has enough tiles for the wide kernels)
         for (int s : {1, 2, 4, 8}) {
             if (s > steps) break;
             const int64_t fit = s == 8 ? 112 : s == 4 ? 140 : 148, waves = (mt * ((t + tn - 1) / tn) * s + fit - 1) / fit;
@@ -297,7 +297,7 @@ inline GemmI8Plan gemm_i8_plan(int64_t t, int64_t k, int64_t n) {
         }
         if (t <= tn) break;
     }
-    if (t > 128) {
+    if (t > 128 || least < 0) {
         offer({128, 1, true, false}, 5900 + (mt * ((t + 127) / 128) + 147) / 148 * steps * 280);
         offer({256, 1, true, false}, 8200 + (mt * ((t + 255) / 256) + 147) / 148 * steps * 361);
         offer({256, 1, true, true}, 9500 + ((mt + 1) / 2 * ((t + 255) / 256) + 73) / 74 * steps * 300);

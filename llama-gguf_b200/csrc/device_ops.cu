@@ -24,6 +24,7 @@ int bad_type(const char* op, uint32_t t) {
     return dev_fail(B200_ERR_UNSUPPORTED_DTYPE, (std::string(op) + ": type " + std::to_string(t) + " (F32, F16 and BF16 only)").c_str());
 }
 constexpr int64_t kMost = (int64_t)1 << 31;      // grids and 32-bit counts
+constexpr int64_t kMostTiled = kMost - (1 << 20);      // ... that a last tile may go beyond
 
 // No exception crosses the C boundary.
 template <typename F> int entry(const char* op, F&& body) {
@@ -114,7 +115,7 @@ extern "C" int b200_dev_mat_mat_i8(int device, void* stream, uint32_t out_type, 
     const char* op = "mat_mat_i8";
     return entry(op, [&]() -> int {
         if (!type_bytes(out_type)) return bad_type(op, out_type);
-        if (t_rows < 0 || t_rows >= kMost || n < 1 || n >= kMost || k < 1) return shape(op, "empty or oversized shape");
+        if (t_rows < 0 || t_rows > kMostTiled || n < 1 || n > kMostTiled || k < 1) return shape(op, "empty or oversized shape");
         if (k > 131071) return shape(op, "k must be at most 131071 (32-bit sums)");
         if (lda < k || ldw < k || ldo < n) return shape(op, "rows overlap");
         if (t_rows == 0) return B200_OK;
@@ -178,8 +179,8 @@ static int check_attention(const char* op, const b200_q4_attention* a) {
     int rc = check_pages(op, a->cache);
     if (rc) return rc;
     if (a->n_heads < 1 || a->n_heads > 65536 || a->n_heads % a->cache.n_kv_heads) return shape(op, "the query heads must be a multiple of the kv heads");
-    if (a->seqs < 0 || a->tokens < 0 || a->table_pages < 0 || a->table_stride < a->table_pages || a->max_q < 0) return shape(op, "negative size");
-    if (a->tokens * a->n_heads >= kMost || a->tokens >= kMost || (int64_t)a->table_pages * a->cache.page_size >= kMost) return shape(op, "too many rows or positions for one call");
+    if (a->seqs < 0 || a->tokens < 0 || a->table_pages < 0 || a->table_stride < 0 || a->max_q < 0) return shape(op, "negative size");
+    if (a->tokens * a->n_heads >= kMost || a->tokens >= kMost || (int64_t)a->table_pages * a->cache.page_size > kMostTiled) return shape(op, "too many rows or positions for one call");
     if (!a->q_starts && a->tokens != a->seqs) return shape(op, "without q_starts every sequence has one token");
     if (a->window < 0) return bad(op, "window must not be negative");
     return B200_OK;

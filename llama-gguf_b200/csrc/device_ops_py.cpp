@@ -292,7 +292,9 @@ PyObject* rope_append_q4(PyObject* const* args, Py_ssize_t n) {
     a.slots = (const int64_t*)ptr(slots);
     a.tokens = tokens;
     a.rot_dims = (int32_t)table.size(1);
-    a.use_neox = PyObject_IsTrue(args[7]) == 1;
+    const int neox = PyObject_IsTrue(args[7]);
+    if (neox < 0) throw PythonError{};
+    a.use_neox = neox;
     a.status = c.status(9);
     check(E.rope_append_q4(&a));
     return give(out);

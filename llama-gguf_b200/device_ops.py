@@ -145,5 +145,5 @@ def attention_paged_q4(q, pages, page_table, kv_lens, scale=None, q_starts=None,
     q [tokens, heads, hd]; page_table [sequences, most pages] and kv_lens [sequences] int32: sequence s has kv_lens[s] cached positions, its query tokens (already cached) among
     them.  q_starts int32 [sequences + 1]: its tokens are q_starts[s] .. q_starts[s + 1] - 1 and sit at its last positions, each sees the positions up to its own (the last `window` of
     them, 0: all); None: one token per sequence.  max_q: the most query tokens of a sequence where the host knows it; it only chooses between kernels.  A token that sees nothing
-    gets zeros; tokens of `out` behind the last sequence are left as they were."""
+    gets zeros; tokens of `out` ahead of the first sequence and behind the last are left as they were (without `out`: not set)."""
     return _ops().attention_paged_q4(q, pages, page_table, kv_lens, scale, q_starts, max_q, window, out, status)

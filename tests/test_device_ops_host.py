@@ -49,6 +49,7 @@ def test_product_refusals(b200, D):
     good = dict(device=0, stream=None, type=0, a=AT, lda=64, s=AT, w=AT, ldw=64, ws=AT, bias=None, out=AT, ldo=8, t=2, k=64, n=8)
     for change, exc, words in [
             (dict(type=1000), b200.UnsupportedDType, "type"), (dict(k=0), b200.ShapeMismatch, "shape"), (dict(n=0), b200.ShapeMismatch, "shape"), (dict(t=-3), b200.ShapeMismatch, "shape"),
+            (dict(n=(1 << 31) - 1, ldo=1 << 31), b200.ShapeMismatch, "shape"), (dict(t=(1 << 31) - 1), b200.ShapeMismatch, "shape"),
             (dict(k=131072, lda=131072, ldw=131072), b200.ShapeMismatch, "131071"), (dict(lda=48), b200.ShapeMismatch, "overlap"), (dict(ldo=7), b200.ShapeMismatch, "overlap"),
             (dict(a=AT + 8), b200.InvalidArgument, "16 bytes"), (dict(w=AT + 1), b200.InvalidArgument, "16 bytes"), (dict(lda=65), b200.InvalidArgument, "16 bytes"),
             (dict(ldw=72), b200.InvalidArgument, "16 bytes"), (dict(out=None), b200.InvalidArgument, "null"), (dict(ws=None), b200.InvalidArgument, "null")]:
@@ -112,7 +113,7 @@ def test_attention_refusals(b200, D):
         refused(b200, L.b200_dev_attention_paged_q4(C.byref(struct(pages(D, **change)))), getattr(b200, exc), words)
     for change, exc, words in [
             (dict(type=7), b200.UnsupportedDType, "type 7"), (dict(n_heads=3), b200.ShapeMismatch, "multiple"), (dict(seqs=-1), b200.ShapeMismatch, "negative"),
-            (dict(table_stride=3), b200.ShapeMismatch, "negative"), (dict(tokens=4), b200.ShapeMismatch, "one token"), (dict(window=-1), b200.InvalidArgument, "window"),
+            (dict(table_stride=-1), b200.ShapeMismatch, "negative"), (dict(table_pages=(1 << 31) // 16 - 1, table_stride=1 << 30), b200.ShapeMismatch, "too many"), (dict(tokens=4), b200.ShapeMismatch, "one token"), (dict(window=-1), b200.InvalidArgument, "window"),
             (dict(tokens=1 << 30, seqs=1 << 30), b200.ShapeMismatch, "too many"), (dict(table_pages=1 << 27, table_stride=1 << 27), b200.ShapeMismatch, "too many"),
             (dict(q=None), b200.InvalidArgument, "null"), (dict(kv_lens=None), b200.InvalidArgument, "null"), (dict(page_table=None), b200.InvalidArgument, "null")]:
         refused(b200, L.b200_dev_attention_paged_q4(C.byref(struct(**change))), exc, words)

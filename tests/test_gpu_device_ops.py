@@ -421,6 +421,14 @@ def test_attention_leaves_other_tokens_and_strided_outputs(D):
     assert torch.equal(o[2:9], D.attention_paged_q4(q[2:9].contiguous(), pages.cuda(), table.cuda(), lens, q_starts=starts - 2))
 
 
+def test_attention_of_sequences_that_share_a_table(D):
+    pages, table = cache(5, [100], 2, 64, 16)
+    q, lens = normal(9, 3, 4, 64).cuda(), torch.tensor([100, 60, 7], dtype=torch.int32).cuda()
+    one = table.cuda().expand(3, -1)
+    assert one.stride(0) == 0
+    assert torch.equal(D.attention_paged_q4(q, pages.cuda(), one, lens), D.attention_paged_q4(q, pages.cuda(), one.contiguous(), lens))
+
+
 # ---------------------------------------------------------------------------------------------------------------- together
 def layer(D, s):
     """One attention sublayer as a server runs it: norm, product, rotation and append, attention, norm of the output."""
