@@ -8,6 +8,7 @@
 //                          tile of 256 x 256 (cta_group::2), each with its own weight rows and half of the token rows: 32 KB a step per CTA instead of 48.
 //   gemm_i8_split_kernel   few tiles: S CTAs of a cluster share a tile's steps and add their sums through distributed shared memory.  With one token the weights' bytes are all there is
 //                          to do, and a ring of up to 192 KB per SM keeps enough of them on the way.
+// Measured (tokens x n x k): 2048 x 14336 x 4096 100 us in a loop (2400 TOP/s; 90 us cold and by itself), bound by the steps' copies to shared memory; 4 x 14336 x 4096 13.3 us for 59 MB (4.4 TB/s).
 #pragma once
 #include "dev_umma.cuh"
 

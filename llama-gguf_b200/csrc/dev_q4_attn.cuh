@@ -10,13 +10,16 @@
 // A warp takes 16 positions at a time (never more than one page) through a ring in shared memory (cp.async, 16 bytes per lane) and multiplies with mma.m16n8k16 (fp16, f32 sums), the
 // positions (scores) or channels (values) as its 16 rows and the eight query rows as its columns:
 //   scores  a nibble in the low bits of an fp16 is the number n 2^-24 exactly (four bits further up: 16 n 2^-24, and that channel's query element is divided by 16): one shift
-//           and four ands turn eight nibbles into operands.  - 8 sum q is taken off afterwards in f32.
+//           and four ands turn eight nibbles into operands.  - 8 sum q is taken off afterwards in f32 (not for f32 results, which that would cost three bits: theirs are made as the values').
 //   values  1024 + n is n in the low bits of the fp16 1024; minus 1032 it is n - 8.  (Sums of n alone would grow with the keys while the result does not: f32 sums would lose 1e-4 of it.)
 // Queries are scaled by a power of two into fp16's range.  f32 queries are two fp16 numbers (what the first leaves over is the second), and so are the weights of f32 and f16 results: the
 // second ones go through another mma into the same sums.  bf16 has its queries exactly in one, and its weights are rounded to one (2^-11, an eighth of the result's own step).
 // The weight of a value is p_j d_j.  Its reference is not m but m + r, the largest z_j + log2 |d_j| so far: p_j d_j stays in fp16's range whatever the values' scales are (r is kept by itself: large
 // scores leave no bits of log2 |d_j| in a sum).  Both references move only when something passes them by 2^8, so the usual step has no exchange between lanes but the 8 x 8 transposition that makes operands of the weights.
-// What bounds it: the bytes of the cache, 2 (hd / 2 + 4) per position and kv head.
+// What bounds it: the bytes of the cache, hd + 8 per position and kv head.  Measured (both kernels, cold): one token over 131072 positions, 64 heads over 8 of 128, bf16: 47 us for 143 MB (3.0 TB/s): about 7 us until
+// every block knows its stretch and has its first tiles, 29 of stream at 4.9 TB/s (a kernel of the same copies without the arithmetic: 36 altogether), a spread of the blocks' ends, 4 of the join.  32 sequences of up to
+// 8000: 38.5 us for 96 MB.  A warp takes 32 positions a step (two of the above, so that its chains of mma cover each other).  Warps of an SM and positions of a step (us, the two cases): 12 and 32 46.5, 38.7;
+// 16 and 32 51, 44.6; 16 and 16 52, 43; 8 and 48 43.9 to 45, 39.5 to 43: the first of these is the best of the two together and the steadier.
 #pragma once
 #include <type_traits>
 
@@ -352,7 +355,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             const float row_q8 = sum * (8.0f / 16384.0f);                  // in units of 2^-10: (sums of n 2^-24) * 2^10
-            const float row_alpha = ldexpf(a.scale * 1.4426950408889634f, 14 - e);
+            const float row_alpha = ldexpf(a.scale * 1.4426950408889634f, Q2 ? -e : 14 - e);
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 q8[k] = __shfl_sync(0xffffffffu, row_q8, 4 * (2 * c + k));
@@ -403,14 +406,16 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
 #pragma unroll
                     for (int t = 0; t < 2; t++) {
                         const uint32_t x = t ? w[0][j] >> 8 : w[0][j], y = t ? w[1][j] >> 8 : w[1][j];
-                        if (j + t == 0) mma16_first(d, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qb[j][t][0], qb[j][t][1]);
-                        else mma16(d, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qb[j][t][0], qb[j][t][1]);
-                        if (Q2) mma16(d, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, ql[Q2 ? j : 0][t][0], ql[Q2 ? j : 0][t][1]);
+                        const uint32_t k0 = Q2 ? sub_h2(masked_or(x, 0x000f000fu, magic), 0x64086408u) : x & 0x000f000fu, k1 = Q2 ? sub_h2(masked_or(y, 0x000f000fu, magic), 0x64086408u) : y & 0x000f000fu;
+                        const uint32_t k2 = Q2 ? sub_h2(masked_or(x, 0x00f000f0u, magic), 0x64806480u) : x & 0x00f000f0u, k3 = Q2 ? sub_h2(masked_or(y, 0x00f000f0u, magic), 0x64806480u) : y & 0x00f000f0u;
+                        if (j + t == 0) mma16_first(d, k0, k1, k2, k3, qb[j][t][0], qb[j][t][1]);
+                        else mma16(d, k0, k1, k2, k3, qb[j][t][0], qb[j][t][1]);
+                        if (Q2) mma16(d, k0, k1, k2, k3, ql[Q2 ? j : 0][t][0], ql[Q2 ? j : 0][t][1]);
                     }
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int k = 0; k < 2; k++) z[b][u][k] = (fmaf(d[2 * u + k], 1024.0f, -q8[k]) * alpha[k]) * __uint_as_float(ks[u][0]);
+                    for (int k = 0; k < 2; k++) z[b][u][k] = (Q2 ? d[2 * u + k] * alpha[k] : fmaf(d[2 * u + k], 1024.0f, -q8[k]) * alpha[k]) * __uint_as_float(ks[u][0]);
             }
             const bool all = !odd_page && p0 >= lo_max && p0 + 16 * U <= hi_min;
             uint32_t hidden = 0;      // bit 4 b + 2 u + k

@@ -7,11 +7,15 @@
 //   warp 16     issues S = Q K^T (128 x 128, K = hd) and O += P V (N = hd, K = 128).
 //   warps 0-7   one thread per row, two groups of four warps that take every second tile with sums, maximum and statistics of their own, so that one group's exponentials run under the other's
 //               products; the two are joined at the end.  P goes back to tensor memory in place of S.
-// Keys' scales multiply the scores, values' scales the weights.  The weights of f32 and f16 results are bf16 pairs (what the first leaves over is the second: 2^-16), since a weight p_j d_j needs f32's range; those of bf16 results are single
-// fp16 numbers (2^-11, an eighth of the result's own step) as long as that type's range holds them, and pairs in the second pass.  f32 queries are
-// pairs of fp16 numbers scaled by a power of two.  bf16 has f32's range, so that the reference of a row's exponentials need only be near: it is the largest score of the first tile
-// that the row sees, and moves (by a whole number, which no bf16 notices) when a score passes it by 2^16.  A tile's scores are so read once.
-// What bounds it: per tile and row 128 x (2 + 2) products of 128 (the values twice for the pairs), and 128 exponentials and their 10 instructions; a tile's MMAs alone are 1536 clocks at hd 128.
+// Keys' scales multiply the scores, values' scales the weights.  f32 queries are pairs of fp16 numbers scaled by a power of two.  Passes:
+//   steady  The reference of a row's exponentials need only be near: it is the largest score of the first tile that the row sees, and stays.  So no tile waits for another: one O, three buffers of scores,
+//           each score read once.  A weight p_j d_j is an fp16 number (bf16 results: 2^-11, an eighth of their own step) or two of them (what the first leaves over is the second: 2^-22), near one
+//           where the reference was set.
+//   moving  Where a row passes fp16's range, or the last bits of its weights may have cost too much of its result (Q4Weights), or its result is not finite, the block makes a second pass: weights are
+//           pairs of bf16 (2^-16), which have f32's range, and the reference goes up by a whole number, which no bf16 notices, when a score passes it by 2^16.
+// What bounds it: per row and tile 128 x (hd + hd) products (three times that for f32), 128 exponentials with some ten instructions each, and shared memory: both operands of S and the values of P V are
+// read from it, and 48 KB of them written per tile.  One tile takes 2.0 us at hd 128, on one SM as on all.  Measured: 2048 query tokens after 2048 others, 32 heads over 8 of 128, bf16: 202 us, 512 blocks of
+// 17 to 32 tiles, 510 TFLOP/s of the products that the mask leaves (tensor pipe 27 to 33 %).  With references that move, two buffers of scores and pairs of bf16 for all, the same call took 245 us.
 #pragma once
 #include <type_traits>
 
@@ -20,6 +24,12 @@
 namespace dev {
 
 enum { QP_ROWS = 128, QP_KEYS = 128, QP_SOFT = 8, QP_MAKE = 8, QP_MMA = 16, QP_THREADS = 544 };
+
+// by the result's type: the weights' place (2^-kUp at the reference; above it is room for 2^16 2^kUp), and the part of a row's largest channel that its weights' last bits, 2^-25 of each times a
+// value of up to 8, may have cost: half a step of bf16 and of f16 results; of f32 results what the second pass is off by
+template <typename T> struct Q4Weights { static constexpr float kUp = 0.0f, kOff = 1.0f / (1 << 8); };
+template <> struct Q4Weights<__half> { static constexpr float kUp = 0.0f, kOff = 1.0f / (1 << 11); };
+template <> struct Q4Weights<float> { static constexpr float kUp = -4.0f, kOff = 1.0f / (1 << 16); };
 
 template <typename T, int HD> struct Q4PromptSmem {
     static constexpr int NQ = sizeof(T) == 4 ? 2 : 1;
@@ -110,6 +120,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
     using Sm = Q4PromptSmem<T, HD>;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
     constexpr int NQ = Sm::NQ, SLABS = HD / 64;
+    constexpr float kUp = Q4Weights<T>::kUp, kOff = Q4Weights<T>::kOff;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_item[2], s_bad;
@@ -226,10 +237,9 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
     const uint32_t tmem = s_tmem;
     bool alive = true;
 
-    // One pass over the keys.  steady: references stay where a row's first tiles put them, so that the tiles do not depend on one another: one O, three buffers of scores.  Otherwise they move, with
-    // sums of each group's own.
+    // one pass over the keys (the moving one: two buffers, a group's sums of its own)
     auto pass = [&](auto mode) {
-        constexpr bool steady = decltype(mode)::value, ONE = steady && BF;      // ONE: weights of one fp16 number each, values in fp16
+        constexpr bool steady = decltype(mode)::value, ONE = steady && BF;      // steady: weights and values in fp16; ONE: one number per weight
         const uint32_t bars = base + Sm::BAR_AT + (steady ? 0 : Sm::BARS * 8);
         const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64, p_full = bars + 112, pv_done = bars + 136, all_done = bars + 160;
         if (warp >= QP_MAKE && warp < QP_MMA) {
@@ -316,7 +326,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 for (int j = 0; j < VW; j++) {
                     const uint32_t x[2] = {__byte_perm(w.v[0][j], w.v[1][j], 0x5410), __byte_perm(w.v[0][j], w.v[1][j], 0x7632)};
 #pragma unroll
-                    for (int k = 0; k < 8; k++) sts32(vt + ((v_word + j) * 8 + k) * 128 + ((c8 ^ k) << 4), nibbles<!ONE>(x[k >> 2] >> (4 * (k & 3)), mask));
+                    for (int k = 0; k < 8; k++) sts32(vt + ((v_word + j) * 8 + k) * 128 + ((c8 ^ k) << 4), nibbles<!steady>(x[k >> 2] >> (4 * (k & 3)), mask));
                 }
             };
             look(0);
@@ -339,7 +349,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 raw = next;
             }
         } else if (warp == QP_MMA) {
-            const uint32_t iqk = f16_idesc(BF, 128, QP_KEYS), ipv = f16_idesc(!ONE, 128, HD);
+            const uint32_t iqk = f16_idesc(BF, 128, QP_KEYS), ipv = f16_idesc(!steady, 128, HD);
             constexpr int nb = steady ? 3 : 2, ns = steady ? 6 : 2;      // buffers of scores, barriers of theirs
             auto scores = [&](int t) {
                 const int st = t & 1;
@@ -476,7 +486,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 if (steady && t == 1) {
                     asm volatile("bar.sync 2, 256;" ::: "memory");
                     m = refs[r];
-                    if (ONE) above = s_above;
+                    if (steady) above = s_above;
                 } else if (steady && t == 2) {
                     asm volatile("bar.sync 3, 256;" ::: "memory");
                     m = refs[128 + r];
@@ -484,13 +494,13 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 if (steady ? t < 2 && __any_sync(0xffffffffu, m == -INFINITY) : __any_sync(0xffffffffu, m == -INFINITY)) {
                     // (alpha = 0: 0, or NaN where nothing is seen, which sets nothing)
                     const float top = (all ? largest(std::true_type{}) : largest(std::false_type{})) * alpha;
-                    if (ONE && t == 0) {
-                        // the largest value scale of the tile, as a power of two: with the reference that much higher its weights are fp16 numbers of about one
+                    if (steady && t == 0) {
+                        // the largest value scale of the tile, as a power of two: with the reference that much higher (and kUp more) its weights are fp16 numbers of about 2^-kUp
                         // (of those that are numbers: a row that sees another one makes a second pass necessary anyway)
                         const float4 d = k4[32 + lane];
                         auto size = [](float v) { return (__float_as_uint(v) & 0x7fffffffu) < kInfBits ? fabsf(v) : 0.0f; };
                         const uint32_t big = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(size(d.x), size(d.y)), fmaxf(size(d.z), size(d.w)))));
-                        above = big ? (float)((int)(big >> 23) - 127) : 0.0f;
+                        above = (big ? (float)((int)(big >> 23) - 127) : 0.0f) + kUp;
                         if (tid == 0) s_above = above;
                     }
                     if (m == -INFINITY) m = fmaxf(m, top + above);
@@ -549,6 +559,10 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                                 sum = add2(sum, p);
                                 if constexpr (ONE) {
                                     o[2 * i + u] = pack_h2(w.x, w.y);
+                                } else if constexpr (steady) {
+                                    o[2 * i + u] = pack_h2(w.x, w.y);
+                                    const float2 f = unpack_h2(o[2 * i + u]);
+                                    o[16 + 2 * i + u] = pack_h2(w.x - f.x, w.y - f.y);
                                 } else {
                                     const uint32_t b = pack_bf2(w.x, w.y);
                                     const float2 rest = fma2(make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)), make_float2(-1.0f, -1.0f), w);
@@ -614,7 +628,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 for (int i = 0; i < 32; i++) y[i] = sum == 0.0f ? 0.0f : y[i] * inv;
             };
             if (steady) {
-                // what is not finite may be so under a reference that moves; sums of fp16 weights that are far below one have lost bits
+                // what is not finite may be so under a reference that moves; sums of fp16 weights far below one have lost bits
                 float zero = sum * 0.0f, most = 0.0f;
 #pragma unroll 1
                 for (int j = 0; j < HD / 64; j++) {
@@ -626,10 +640,10 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                         most = fmaxf(most, fabsf(y[i]));
                     }
                 }
-                if (ONE) refs[grp * 128 + r] = m == -INFINITY ? -1.0f : most;      // (-1: the row has seen nothing, as far as this group knows)
+                refs[grp * 128 + r] = m == -INFINITY ? -1.0f : most;      // (-1: the row has seen nothing, as far as this group knows)
                 asm volatile("bar.sync 1, 256;" ::: "memory");
-                const float size = ONE ? fmaxf(refs[r], refs[128 + r]) : 0.0f;
-                const bool small = ONE && size >= 0.0f && !(size * sum >= 0.015625f);
+                const float size = fmaxf(refs[r], refs[128 + r]);
+                const bool small = size >= 0.0f && !(size * sum * kOff >= (float)(n * QP_KEYS) * (1.0f / (1 << 22)));
                 if (__any_sync(0xffffffffu, live && (small || zero != 0.0f)) && lane == 0) atomicOr(&s_bad, 1);
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 if (s_bad) write = false;
@@ -650,7 +664,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
         umma_after_sync();
     };
     pass(std::true_type{});
-    if (s_bad) pass(std::false_type{});      // a score passed its reference by 2^64, or a result is not finite
+    if (s_bad) pass(std::false_type{});      // (uniform: written before the pass's last barrier)
     if (warp == QP_MMA) tmem_free<false>(tmem, 512);
 }
 

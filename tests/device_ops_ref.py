@@ -5,6 +5,8 @@ import torch
 
 TINY = 2.0**-119
 HALF_STEP = {torch.float32: 2.0**-24, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}
+FLOOR = {torch.float32: 2.0**-29, torch.float16: 2.0**-25, torch.bfloat16: 2.0**-25}
+COST = {torch.float32: 2.0**-16, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}
 LEAST = {torch.float32: 0.0, torch.float16: 2.0**-25, torch.bfloat16: 0.0}  # half a step of the subnormals
 
 
@@ -70,8 +72,9 @@ def attention(q, kv, table, lens, starts, page, scale, window, n_pages, dtype=to
     sum too), by 2^-21 from the exponential's argument and value and 2^-21 from its own two halves (bf16 results: 2^-11 from its one;
     f32 and f16 results of sequences of more than 32 rows of a kv head: two bf16 numbers, 2^-8 of 2^-8), and the sum over L keys by L / 16 * 2^-22 of sum p |v|.
     The two fp16 halves of a weight p d (d a value's scale) end at 2^-24 of a reference that the largest weight reaches: whatever its size, a weight is off by 2^-25 of the largest, and a
-    value is at most 8 d, so that a channel whose large weights meet values of zero keeps L * 2^-25 * 8 max(p d) = L * 2^-25 * max(p max |v|).  (bf16 results of many rows: the reference is
-    the largest score of the first tile with the largest scale of a value there, whose own score may be small: L * 2^-25 * max |v| of the sequence.)"""
+    value is at most 8 d, so that a channel whose large weights meet values of zero keeps L * 2^-25 * 8 max(p d) = L * 2^-25 * max(p max |v|).  (Many rows: the
+    reference is the largest score of the first tile with the largest scale of a value there, whose own score may be small, and the weights there are 1, or 2^4 for f32:
+    L * 2^-25 or 2^-29 * max |v| of the sequence; a block where that may be more than 2^-8, 2^-11 or 2^-16 (bf16, f16, f32) of a row's largest channel is done again without it.)"""
     k, v = kv
     o = torch.zeros(q.shape, dtype=torch.float64)
     off = torch.zeros(q.shape, dtype=torch.float64)
@@ -96,5 +99,5 @@ def attention(q, kv, table, lens, starts, page, scale, window, n_pages, dtype=to
                 big = float(((kk.abs() @ q[t, h].abs()) * abs(scale)).max())
                 o[t, h] = p @ vv
                 dz = big * (hd / 16 * 2.0**-22 + 2.0**-22 + 2.0**-23 + 2.0**-22)
-                off[t, h] = (p @ vv.abs()) * (2 * dz + (2.0**-11 if dtype == torch.bfloat16 else 2.0**-16 if many else 0) + 2.0**-20 + len(keys) / 16 * 2.0**-22) + len(keys) * 2.0**-25 * (far if many and dtype == torch.bfloat16 else (p * vv.abs().amax(1)).max())
+                off[t, h] = (p @ vv.abs()) * (2 * dz + (2.0**-11 if dtype == torch.bfloat16 else 2.0**-16 if many else 0) + 2.0**-20 + len(keys) / 16 * 2.0**-22) + max(len(keys) * 2.0**-25 * (p * vv.abs().amax(1)).max(), min(len(keys) * FLOOR[dtype] * far, 1.01 * COST[dtype] * o[t, h].abs().max()) if many else 0.0)
     return o, off

@@ -372,6 +372,24 @@ def test_attention_of_prompts_with_scores_far_apart(D, dtype):
     check_attention(D, dtype, 96, 24, 64, 32, [600], [40], gain=0.0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("first", [2.0**-12, 2.0**-8, 1.0])
+def test_attention_of_prompts_with_one_large_score(D, dtype, first):
+    """The first position's score is 15 to 18 above all others, whose weights, thousands of them, are near the end of fp16; its value is small, so that theirs count."""
+    n, q_len, nh, nkv, hd, page = 6000, 40, 96, 24, 64, 16
+    k, v = normal(3, n, nkv, hd) / 16, 0.5 + normal(4, n, nkv, hd).abs()
+    k[0], v[0] = 1.0, v[0] * first
+    table = torch.randperm(n // page, generator=torch.Generator().manual_seed(5)).int()[None]
+    pages = torch.zeros(n // page, nkv, page * (hd + 8), dtype=torch.uint8)
+    at = torch.arange(n)
+    R.put_rows(pages, page, hd, table[0, at // page].long() * page + at % page, k, v)
+    q = (torch.linspace(15, 18, nh)[None, :, None] * hd**-0.5 + 0.01 * normal(6, q_len, nh, hd)).to(dtype)
+    o = D.attention_paged_q4(q.cuda(), pages.cuda(), table.cuda(), torch.tensor([n], dtype=torch.int32).cuda(), q_starts=torch.tensor([0, q_len], dtype=torch.int32).cuda()).cpu().double()
+    want, off = R.attention(q.double(), R.values(pages, page, hd), table.tolist(), [n], [0, q_len], page, hd**-0.5, 0, n // page, dtype)
+    tol = off + 1.001 * R.HALF_STEP[dtype] * (want.abs() + off) + R.LEAST[dtype]
+    assert ((o - want).abs() <= tol).all(), float(((o - want).abs() - tol).max())
+
+
 @pytest.mark.parametrize("q_len,nkv", [(9, 2), (50, 2), (50, 20)])
 def test_attention_of_several_tokens_with_bad_pages(D, q_len, nkv):
     lens = [300, 200]
