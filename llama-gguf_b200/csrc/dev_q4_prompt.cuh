@@ -104,6 +104,18 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(two(a)), "l"(two(b)), "l"(two(c)));
     return two(r);
 }
+// loads that are made where `there` holds, and zeros elsewhere, without a choice after the load, which would wait for it
+template <int N> __device__ __forceinline__ void load_where(uint32_t (&v)[N], const void* p, bool there) {
+    if constexpr (N == 4)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t@p ld.global.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
+                     : "=&r"(v[0]), "=&r"(v[1]), "=&r"(v[2]), "=&r"(v[3])
+                     : "l"(p), "r"((uint32_t)there)
+                     : "memory");
+    else if constexpr (N == 2)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t@p ld.global.v2.u32 {%0,%1}, [%2];\n\t}" : "=&r"(v[0]), "=&r"(v[1]) : "l"(p), "r"((uint32_t)there) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.u32 %0, [%1];\n\t}" : "=&r"(v[0]) : "l"(p), "r"((uint32_t)there) : "memory");
+}
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // D = f32, A = B = bf16 (1) or fp16 (0), K-major
@@ -114,6 +126,9 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
+
+// the pass that few blocks make, in code and registers of its own (by copy: nothing of the first pass gets an address)
+template <typename F> __device__ __noinline__ void apart(F pass) { pass(std::false_type{}); }
 
 template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) attention_q4_prompt_kernel(const b200_q4_attention a, uint64_t page16, int64_t limit) {
     before();
@@ -238,7 +253,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
     bool alive = true;
 
     // one pass over the keys (the moving one: two buffers, a group's sums of its own)
-    auto pass = [&](auto mode) {
+    auto pass = [=](auto mode) mutable {
         constexpr bool steady = decltype(mode)::value, ONE = steady && BF;      // steady: weights and values in fp16; ONE: one number per weight
         const uint32_t bars = base + Sm::BAR_AT + (steady ? 0 : Sm::BARS * 8);
         const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64, p_full = bars + 112, pv_done = bars + 136, all_done = bars + 160;
@@ -254,59 +269,59 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
             uint32_t mask = 0x000f000fu;
             asm("" : "+r"(mask));      // (kept in a register: an instruction has room for one constant)
             // Lane l looks after the sixteen positions l & 7 of a tile: the page is looked up two tiles ahead, the rows are asked for one tile ahead.
-            int page = 0, row = 0;
+            uint32_t page[1] = {0};
+            int row = 0;
             bool wanted = false;
             auto look = [&](int t) {
                 const int p = begin + t * QP_KEYS + 16 * (lane & 7);
                 wanted = t < n && p < hi;
-                if (wanted) {
-                    const int index = (int)(((uint64_t)(p >> 4) * page16) >> 36);
-                    row = p - index * page_size;
-                    page = table[index];
-                }
+                const int index = (int)(((uint64_t)(p >> 4) * page16) >> 36);
+                row = p - index * page_size;
+                load_where<1>(page, table + index, wanted);
             };
-            struct Raw {
-                uint4 k[KN];
-                uint32_t v[2][VW];
-                float scale;      // of key 16 pw + lane, or of the value there (lanes from 16 on)
+            struct Keys {
+                uint32_t k[KN][4];
+                uint32_t scale[1];      // of key 16 pw + lane, or of the value there (lanes from 16 on)
                 bool there;
-            } raw, next;
+            } keys, next_keys;
+            struct Values {
+                uint32_t v[2][VW];
+            } values, next_values;
             // this warp's keys: the sixteen pw; its values: pairs of half the tile's positions, a quarter of the channels
             const int v_key = 64 * (pw & 1) + 2 * lane, v_word = (pw >> 1) * VW;
-            auto ask = [&](int t, Raw& w) {
-                const bool good = wanted && (unsigned)page < (uint64_t)a.cache.n_pages;
-                if (wanted && !good && a.status) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
-                const unsigned long long mine = good ? (unsigned long long)(head + page * page_bytes) : 0ull;
-                const int my_row = row;
-                look(t + 1);
-                auto of = [&](int g, int& r) {
-                    r = __shfl_sync(0xffffffffu, my_row, g);
-                    return reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, mine, g));
-                };
-                int rk, rv;
-                const uint8_t *kb = of(pw, rk), *vb = of(v_key >> 4, rv);
-#pragma unroll
-                for (int i = 0; i < KN; i++)
-                    w.k[i] = kb ? *reinterpret_cast<const uint4*>(kb + (rk + i * PER + lane / CH) * (HD / 2) + (lane % CH) * 16) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    struct __align__(4 * VW) W { uint32_t x[VW]; };
-                    W x{};
-                    if (vb) x = *reinterpret_cast<const W*>(vb + v_off + (rv + (v_key & 15) + u) * (HD / 2) + v_word * 4);
-#pragma unroll
-                    for (int i = 0; i < VW; i++) w.v[u][i] = x.x[i];
-                }
-                w.there = kb != nullptr && begin + t * QP_KEYS + 16 * pw + (lane & 15) < hi;
-                w.scale = w.there ? reinterpret_cast<const float*>(kb + 2 * v_off)[rk + (lane & 15) + (lane < 16 ? 0 : page_size)] : 0.0f;
+            unsigned long long mine = 0;      // where this lane's sixteen positions are: of the tile whose keys were asked for last
+            int my_row = 0;
+            auto of = [&](int g, int& r) {
+                r = __shfl_sync(0xffffffffu, my_row, g);
+                return reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, mine, g));
             };
-            auto make_keys = [&](int t, const Raw& w) {
+            auto ask_values = [&](Values& w) {      // ... and before ask_keys goes on
+                int r;
+                const uint8_t* vb = of(v_key >> 4, r);
+#pragma unroll
+                for (int u = 0; u < 2; u++) load_where<VW>(w.v[u], vb + v_off + (r + (v_key & 15) + u) * (HD / 2) + v_word * 4, vb != nullptr);
+            };
+            auto ask_keys = [&](int t, Keys& w) {
+                const bool good = wanted && page[0] < (uint64_t)a.cache.n_pages;
+                if (wanted && !good && a.status) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
+                mine = good ? (unsigned long long)(head + (int64_t)page[0] * page_bytes) : 0ull;
+                my_row = row;
+                look(t + 1);
+                int r;
+                const uint8_t* kb = of(pw, r);
+#pragma unroll
+                for (int i = 0; i < KN; i++) load_where<4>(w.k[i], kb + (r + i * PER + lane / CH) * (HD / 2) + (lane % CH) * 16, kb != nullptr);
+                w.there = kb != nullptr && begin + t * QP_KEYS + 16 * pw + (lane & 15) < hi;
+                load_where<1>(w.scale, kb + 2 * v_off + (int64_t)(r + (lane & 15) + (lane < 16 ? 0 : page_size)) * 4, w.there);
+            };
+            auto make_keys = [&](int t, const Keys& w) {
                 const uint32_t kt = base + Sm::K_AT + (t & 1) * Sm::K;
 #pragma unroll
                 for (int i = 0; i < KN; i++) {
                     const int r = pw * 16 + i * PER + lane / CH;
                     // (the second half of a row's lanes take their words in another order: the same chunk of both slabs is in the same banks)
                     const bool far = HD == 128 && (lane & 2);
-                    const uint32_t x[4] = {far ? w.k[i].z : w.k[i].x, far ? w.k[i].w : w.k[i].y, far ? w.k[i].x : w.k[i].z, far ? w.k[i].y : w.k[i].w};
+                    const uint32_t x[4] = {far ? w.k[i][2] : w.k[i][0], far ? w.k[i][3] : w.k[i][1], far ? w.k[i][0] : w.k[i][2], far ? w.k[i][1] : w.k[i][3]};
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const int g = (lane % CH) * 4 + (far ? j ^ 2 : j);          // eight channels
@@ -315,11 +330,11 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                     }
                 }
                 uint8_t* meta = smem + Sm::META_AT + (t & 3) * Sm::META;
-                reinterpret_cast<float*>(meta)[(lane < 16 ? 0 : 128) + 16 * pw + (lane & 15)] = w.scale;
+                reinterpret_cast<uint32_t*>(meta)[(lane < 16 ? 0 : 128) + 16 * pw + (lane & 15)] = w.scale[0];
                 const uint32_t gone = ~__ballot_sync(0xffffffffu, w.there);
                 if (lane == 0) reinterpret_cast<uint16_t*>(meta + 1024)[pw] = (uint16_t)gone;
             };
-            auto make_values = [&](int t, const Raw& w) {
+            auto make_values = [&](int t, const Values& w) {
                 const uint32_t vt = base + Sm::V_AT + (t & 1) * Sm::V + (pw & 1) * (HD * 128) + (lane & 3) * 4;
                 const uint32_t c8 = lane >> 2;
 #pragma unroll
@@ -329,24 +344,31 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                     for (int k = 0; k < 8; k++) sts32(vt + ((v_word + j) * 8 + k) * 128 + ((c8 ^ k) << 4), nibbles<!steady>(x[k >> 2] >> (4 * (k & 3)), mask));
                 }
             };
+            // A tile's keys are made before the values of the one ahead of it: these wait for products that need a row's exponentials, those only for the scores two tiles ago.
             look(0);
-            if (n > 0) ask(0, raw);
+            if (n > 0) ask_keys(0, keys);
 #pragma unroll 1
-            for (int t = 0; t < n; t++) {
-                if (t + 1 < n) ask(t + 1, next);
-                const int st = t & 1;
-                const uint32_t ph = ((t >> 1) & 1) ^ 1u;
-                bar_wait(k_empty + 8 * st, ph, alive, 11);
-                make_keys(t, raw);
-                async_fence();
-                __syncwarp();
-                if (lane == 0) bar_arrive(k_full + 8 * st);
-                bar_wait(v_empty + 8 * st, ph, alive, 12);
-                make_values(t, raw);
-                async_fence();
-                __syncwarp();
-                if (lane == 0) bar_arrive(v_full + 8 * st);
-                raw = next;
+            for (int t = 0; t < n + (n > 0); t++) {
+                if (t < n) ask_values(next_values);
+                if (t + 1 < n) ask_keys(t + 1, next_keys);
+                if (t < n) {
+                    const int st = t & 1;
+                    bar_wait(k_empty + 8 * st, ((t >> 1) & 1) ^ 1u, alive, 11);
+                    make_keys(t, keys);
+                    async_fence();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(k_full + 8 * st);
+                }
+                if (t > 0) {
+                    const int st = (t - 1) & 1;
+                    bar_wait(v_empty + 8 * st, (((t - 1) >> 1) & 1) ^ 1u, alive, 12);
+                    make_values(t - 1, values);
+                    async_fence();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(v_full + 8 * st);
+                }
+                keys = next_keys;
+                values = next_values;
             }
         } else if (warp == QP_MMA) {
             const uint32_t iqk = f16_idesc(BF, 128, QP_KEYS), ipv = f16_idesc(!steady, 128, HD);
@@ -373,7 +395,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 }
                 __syncwarp();
             };
-            for (int t = 0; t < min(n, 2); t++) scores(t);
+            for (int t = 0; t < min(n, nb); t++) scores(t);
             for (int t = 0; t < n; t++) {
                 const int st = t & 1, b = t % nb;
                 bar_wait(v_full + 8 * st, (t >> 1) & 1, alive, 14);
@@ -395,11 +417,9 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                     if (t == n - 1) umma_commit<false>(all_done);
                 }
                 __syncwarp();
-                if (t + 2 < n) {
-                    // the scores of t + 2 go where the weights of t (of t - 1, with three buffers) are
-                    const int was = steady ? t - 1 : t;
-                    if (was >= 0) bar_wait(pv_done + 8 * (was % nb), (was / nb) & 1, alive, 16);
-                    scores(t + 2);
+                if (t + nb < n) {      // whose scores go where the weights of t are
+                    bar_wait(pv_done + 8 * b, (t / nb) & 1, alive, 16);
+                    scores(t + nb);
                 }
             }
         } else {
@@ -664,7 +684,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
         umma_after_sync();
     };
     pass(std::true_type{});
-    if (s_bad) pass(std::false_type{});      // (uniform: written before the pass's last barrier)
+    if (s_bad) apart(pass);      // (uniform: written before the pass's last barrier)
     if (warp == QP_MMA) tmem_free<false>(tmem, 512);
 }
 
