@@ -268,16 +268,24 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
             const int32_t* table = a.page_table + (int64_t)s * a.table_stride;
             uint32_t mask = 0x000f000fu;
             asm("" : "+r"(mask));      // (kept in a register: an instruction has room for one constant)
-            // Lane l looks after the sixteen positions l & 7 of a tile: the page is looked up two tiles ahead, the rows are asked for one tile ahead.
-            uint32_t page[1] = {0};
-            int row = 0;
-            bool wanted = false;
-            auto look = [&](int t) {
-                const int p = begin + t * QP_KEYS + 16 * (lane & 7);
-                wanted = t < n && p < hi;
-                const int index = (int)(((uint64_t)(p >> 4) * page16) >> 36);
-                row = p - index * page_size;
-                load_where<1>(page, table + index, wanted);
+            // this warp's keys: the sixteen pw; its values: pairs of half the tile's positions, a quarter of the channels
+            const int v_key = 64 * (pw & 1) + 2 * lane, v_word = (pw >> 1) * VW;
+            // The pages of both are looked up two tiles ahead, the rows are asked for one tile ahead.
+            struct Place {
+                uint32_t page[1] = {0};
+                int row = 0;
+                bool wanted = false;
+            } of_keys, of_values;
+            auto look = [&](int t, int key, Place& w) {      // (key: the first of sixteen, whole in a page)
+                const int p = begin + t * QP_KEYS + key, index = (int)(((uint64_t)(p >> 4) * page16) >> 36);
+                w.wanted = t < n && p < hi;
+                w.row = p - index * page_size;
+                load_where<1>(w.page, table + index, w.wanted);
+            };
+            auto at = [&](const Place& w) -> const uint8_t* {
+                const bool good = w.wanted && w.page[0] < (uint64_t)a.cache.n_pages;
+                if (w.wanted && !good && a.status) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
+                return good ? head + (int64_t)w.page[0] * page_bytes : nullptr;
             };
             struct Keys {
                 uint32_t k[KN][4];
@@ -287,28 +295,17 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
             struct Values {
                 uint32_t v[2][VW];
             } values, next_values;
-            // this warp's keys: the sixteen pw; its values: pairs of half the tile's positions, a quarter of the channels
-            const int v_key = 64 * (pw & 1) + 2 * lane, v_word = (pw >> 1) * VW;
-            unsigned long long mine = 0;      // where this lane's sixteen positions are: of the tile whose keys were asked for last
-            int my_row = 0;
-            auto of = [&](int g, int& r) {
-                r = __shfl_sync(0xffffffffu, my_row, g);
-                return reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, mine, g));
-            };
-            auto ask_values = [&](Values& w) {      // ... and before ask_keys goes on
-                int r;
-                const uint8_t* vb = of(v_key >> 4, r);
+            const uint8_t* v_at = nullptr;      // this lane's values of the tile whose keys were asked for last
+            auto ask_values = [&](Values& w) {
 #pragma unroll
-                for (int u = 0; u < 2; u++) load_where<VW>(w.v[u], vb + v_off + (r + (v_key & 15) + u) * (HD / 2) + v_word * 4, vb != nullptr);
+                for (int u = 0; u < 2; u++) load_where<VW>(w.v[u], v_at + u * (HD / 2), v_at != nullptr);
             };
             auto ask_keys = [&](int t, Keys& w) {
-                const bool good = wanted && page[0] < (uint64_t)a.cache.n_pages;
-                if (wanted && !good && a.status) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
-                mine = good ? (unsigned long long)(head + (int64_t)page[0] * page_bytes) : 0ull;
-                my_row = row;
-                look(t + 1);
-                int r;
-                const uint8_t* kb = of(pw, r);
+                const uint8_t *kb = at(of_keys), *vb = at(of_values);
+                const int r = of_keys.row;
+                v_at = vb ? vb + v_off + (of_values.row + (v_key & 15)) * (HD / 2) + v_word * 4 : nullptr;
+                look(t + 1, 16 * pw, of_keys);
+                look(t + 1, v_key & ~15, of_values);
 #pragma unroll
                 for (int i = 0; i < KN; i++) load_where<4>(w.k[i], kb + (r + i * PER + lane / CH) * (HD / 2) + (lane % CH) * 16, kb != nullptr);
                 w.there = kb != nullptr && begin + t * QP_KEYS + 16 * pw + (lane & 15) < hi;
@@ -345,7 +342,8 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 }
             };
             // A tile's keys are made before the values of the one ahead of it: these wait for products that need a row's exponentials, those only for the scores two tiles ago.
-            look(0);
+            look(0, 16 * pw, of_keys);
+            look(0, v_key & ~15, of_values);
             if (n > 0) ask_keys(0, keys);
 #pragma unroll 1
             for (int t = 0; t < n + (n > 0); t++) {
