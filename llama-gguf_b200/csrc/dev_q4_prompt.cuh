@@ -14,8 +14,9 @@
 //   moving  Where a row passes fp16's range, or the last bits of its weights may have cost too much of its result (Q4Weights), or its result is not finite, the block makes a second pass: weights are
 //           pairs of bf16 (2^-16), which have f32's range, and the reference goes up by a whole number, which no bf16 notices, when a score passes it by 2^16.
 // What bounds it: per row and tile 128 x (hd + hd) products (three times that for f32), 128 exponentials with some ten instructions each, and shared memory: both operands of S and the values of P V are
-// read from it, and 48 KB of them written per tile.  One tile takes 2.0 us at hd 128, on one SM as on all.  Measured: 2048 query tokens after 2048 others, 32 heads over 8 of 128, bf16: 202 us, 512 blocks of
-// 17 to 32 tiles, 510 TFLOP/s of the products that the mask leaves (tensor pipe 27 to 33 %).  With references that move, two buffers of scores and pairs of bf16 for all, the same call took 245 us.
+// read from it, and 48 KB of them written per tile.  A tile takes 1.7 us at hd 128, on one SM as on all: a tile of a warp of rows some 2900 clocks (two groups share the tiles), of a warp that makes operands 2300, the products
+// 1400 with their starts, each slowing the others at the schedulers.  Measured: 2048 query tokens after 2048 others, 32 heads over 8 of 128, bf16: 182 us, 512 blocks of 17 to 32 tiles, 570 TFLOP/s of the products that
+// the mask leaves.  With keys made behind the values of the tile before, scores two tiles ahead and both passes in one piece of code (spills) 202; with references that move and pairs of bf16 for all 245.
 #pragma once
 #include <type_traits>
 
@@ -270,48 +271,66 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
             asm("" : "+r"(mask));      // (kept in a register: an instruction has room for one constant)
             // this warp's keys: the sixteen pw; its values: pairs of half the tile's positions, a quarter of the channels
             const int v_key = 64 * (pw & 1) + 2 * lane, v_word = (pw >> 1) * VW;
-            // The pages of both are looked up two tiles ahead, the rows are asked for one tile ahead.
+            // The page of the next tile's rows is looked up when this one's are asked for; those are asked for as soon as the registers of the tile before are free.
+            const int tile_pages = QP_KEYS / page_size, tile_rows = QP_KEYS - tile_pages * page_size;
+            const uint32_t n_pages = (uint32_t)min(a.cache.n_pages, (int64_t)INT32_MAX);
             struct Place {
-                uint32_t page[1] = {0};
-                int row = 0;
-                bool wanted = false;
+                uint32_t page[1];
+                int p, index, row;      // the first of sixteen positions, all in a page: its number, its page's place in the table, its row there
+                bool wanted;
             } of_keys, of_values;
-            auto look = [&](int t, int key, Place& w) {      // (key: the first of sixteen, whole in a page)
-                const int p = begin + t * QP_KEYS + key, index = (int)(((uint64_t)(p >> 4) * page16) >> 36);
-                w.wanted = t < n && p < hi;
-                w.row = p - index * page_size;
-                load_where<1>(w.page, table + index, w.wanted);
+            auto look = [&](Place& w) {
+                w.wanted = w.p < hi;
+                load_where<1>(w.page, table + w.index, w.wanted);
+            };
+            auto first_look = [&](Place& w, int key) {
+                w.p = begin + key;
+                w.index = (int)(((uint64_t)(w.p >> 4) * page16) >> 36);
+                w.row = w.p - w.index * page_size;
+                look(w);
+            };
+            auto next_look = [&](Place& w) {
+                w.p += QP_KEYS;      // (a call's positions end 2^20 before 2^31)
+                w.row += tile_rows;
+                w.index += tile_pages;
+                if (w.row >= page_size) {
+                    w.row -= page_size;
+                    w.index++;
+                }
+                look(w);
             };
             auto at = [&](const Place& w) -> const uint8_t* {
-                const bool good = w.wanted && w.page[0] < (uint64_t)a.cache.n_pages;
+                const bool good = w.wanted && w.page[0] < n_pages;
                 if (w.wanted && !good && a.status) atomicOr(a.status, (int)B200_STATUS_BAD_PAGE);
-                return good ? head + (int64_t)w.page[0] * page_bytes : nullptr;
+                return good ? head + (int64_t)w.page[0] * page_bytes + w.row * (HD / 2) : nullptr;
             };
             struct Keys {
                 uint32_t k[KN][4];
                 uint32_t scale[1];      // of key 16 pw + lane, or of the value there (lanes from 16 on)
                 bool there;
-            } keys, next_keys;
+            } keys;
             struct Values {
                 uint32_t v[2][VW];
-            } values, next_values;
-            const uint8_t* v_at = nullptr;      // this lane's values of the tile whose keys were asked for last
-            auto ask_values = [&](Values& w) {
+            } values;
+            auto ask_values = [&]() {
+                const uint8_t* from = at(of_values);
+                const bool there = from != nullptr;
+                next_look(of_values);
 #pragma unroll
-                for (int u = 0; u < 2; u++) load_where<VW>(w.v[u], v_at + u * (HD / 2), v_at != nullptr);
+                for (int u = 0; u < 2; u++) load_where<VW>(values.v[u], from + v_off + ((v_key & 15) + u) * (HD / 2) + v_word * 4, there);
             };
-            auto ask_keys = [&](int t, Keys& w) {
-                const uint8_t *kb = at(of_keys), *vb = at(of_values);
-                const int r = of_keys.row;
-                v_at = vb ? vb + v_off + (of_values.row + (v_key & 15)) * (HD / 2) + v_word * 4 : nullptr;
-                look(t + 1, 16 * pw, of_keys);
-                look(t + 1, v_key & ~15, of_values);
+            auto ask_keys = [&]() {
+                const uint8_t* from = at(of_keys);
+                const bool there = from != nullptr;
+                const uint8_t* scales = from + 2 * v_off - of_keys.row * (HD / 2 - 4) + ((lane & 15) + (lane < 16 ? 0 : page_size)) * 4;
+                keys.there = there && of_keys.p + (lane & 15) < hi;
+                next_look(of_keys);
 #pragma unroll
-                for (int i = 0; i < KN; i++) load_where<4>(w.k[i], kb + (r + i * PER + lane / CH) * (HD / 2) + (lane % CH) * 16, kb != nullptr);
-                w.there = kb != nullptr && begin + t * QP_KEYS + 16 * pw + (lane & 15) < hi;
-                load_where<1>(w.scale, kb + 2 * v_off + (int64_t)(r + (lane & 15) + (lane < 16 ? 0 : page_size)) * 4, w.there);
+                for (int i = 0; i < KN; i++) load_where<4>(keys.k[i], from + (i * PER + lane / CH) * (HD / 2) + (lane % CH) * 16, there);
+                load_where<1>(keys.scale, scales, keys.there);
             };
-            auto make_keys = [&](int t, const Keys& w) {
+            auto make_keys = [&](int t) {
+                const Keys& w = keys;
                 const uint32_t kt = base + Sm::K_AT + (t & 1) * Sm::K;
 #pragma unroll
                 for (int i = 0; i < KN; i++) {
@@ -331,7 +350,8 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 const uint32_t gone = ~__ballot_sync(0xffffffffu, w.there);
                 if (lane == 0) reinterpret_cast<uint16_t*>(meta + 1024)[pw] = (uint16_t)gone;
             };
-            auto make_values = [&](int t, const Values& w) {
+            auto make_values = [&](int t) {
+                const Values& w = values;
                 const uint32_t vt = base + Sm::V_AT + (t & 1) * Sm::V + (pw & 1) * (HD * 128) + (lane & 3) * 4;
                 const uint32_t c8 = lane >> 2;
 #pragma unroll
@@ -341,32 +361,33 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                     for (int k = 0; k < 8; k++) sts32(vt + ((v_word + j) * 8 + k) * 128 + ((c8 ^ k) << 4), nibbles<!steady>(x[k >> 2] >> (4 * (k & 3)), mask));
                 }
             };
-            // A tile's keys are made before the values of the one ahead of it: these wait for products that need a row's exponentials, those only for the scores two tiles ago.
-            look(0, 16 * pw, of_keys);
-            look(0, v_key & ~15, of_values);
-            if (n > 0) ask_keys(0, keys);
+            first_look(of_keys, 16 * pw);
+            first_look(of_values, v_key & ~15);
+            if (n > 0) {
+                ask_keys();
+                ask_values();
+            }
+            // (a tile's keys before the values of the one ahead of it: these wait for products that need a row's exponentials, those only for the scores two tiles ago)
 #pragma unroll 1
             for (int t = 0; t < n + (n > 0); t++) {
-                if (t < n) ask_values(next_values);
-                if (t + 1 < n) ask_keys(t + 1, next_keys);
                 if (t < n) {
                     const int st = t & 1;
                     bar_wait(k_empty + 8 * st, ((t >> 1) & 1) ^ 1u, alive, 11);
-                    make_keys(t, keys);
+                    make_keys(t);
                     async_fence();
                     __syncwarp();
                     if (lane == 0) bar_arrive(k_full + 8 * st);
+                    ask_keys();
                 }
                 if (t > 0) {
                     const int st = (t - 1) & 1;
                     bar_wait(v_empty + 8 * st, (((t - 1) >> 1) & 1) ^ 1u, alive, 12);
-                    make_values(t - 1, values);
+                    make_values(t - 1);
                     async_fence();
                     __syncwarp();
                     if (lane == 0) bar_arrive(v_full + 8 * st);
+                    ask_values();
                 }
-                keys = next_keys;
-                values = next_values;
             }
         } else if (warp == QP_MMA) {
             const uint32_t iqk = f16_idesc(BF, 128, QP_KEYS), ipv = f16_idesc(!steady, 128, HD);
@@ -694,13 +715,14 @@ inline int64_t attention_q4_prompt_blocks(const b200_q4_attention& a) {
     const int64_t rows = a.tokens * (a.n_heads / a.cache.n_kv_heads);
     return rows / QP_ROWS + std::min<int64_t>(a.seqs, rows / (kPromptRows + 1));
 }
-// Whether a call's long sequences go there, by what the host knows.  A block of 128 rows takes 2.0 us for 128 keys, whether alone or on every SM; the other kernel 0.68 us of an SM for eight rows, but spreads any
-// number of rows over all SMs.  So: (rows / 8) * 0.68 / 148 against 2.0 for every 148 blocks.  Measured (bf16, 32 heads over 8, hd 128, 4000 keys; rows of a kv head: us there, here): one sequence of 256
-// 61, 70; eight of 32 57, 70, of 64 93, 70; 64 sequences with 1000 keys of 24 84, 97, of 64 185, 104.
+// Whether a call's long sequences go there, by what the host knows.  A block of 128 rows takes 1.7 us for 128 keys, whether alone or on every SM, and 8 more; the other kernel 0.84 us of an SM for eight rows, but
+// spreads any number of rows over all SMs, and 16 more.  So its (rows / 8) * 0.84 / 148 against 1.7 for every 148 blocks, less what they differ by at 4000 keys.  Measured (bf16, 32 heads over 8, hd 128; us there, here,
+// and what the rule compares with 260): 4000 keys, one sequence of 128 rows of a kv head 39, 62 (128), of 256 62, 63 (256), of 384 85, 63 (384); eight of 32 58, 60 (256), of 48 78, 65 (384); 64 sequences of 36 with
+// 1000 keys 124, 91 (461); one of 256 with 500 keys 33, 25 (256).
 inline bool attention_q4_has_prompts(const b200_q4_attention& a) {
     const int64_t G = a.n_heads / a.cache.n_kv_heads, nkv = a.cache.n_kv_heads;
     if (!a.q_starts || (a.max_q ? a.max_q : a.tokens) * G <= kPromptRows) return false;
-    return (a.tokens * G + 7) / 8 * nkv > 435 * ((attention_q4_prompt_blocks(a) * nkv + 147) / 148);
+    return (a.tokens * G + 7) / 8 * nkv > 260 * ((attention_q4_prompt_blocks(a) * nkv + 147) / 148);
 }
 template <typename T, int HD> cudaError_t attention_q4_prompt(const b200_q4_attention& a, cudaStream_t st) {
     using Sm = Q4PromptSmem<T, HD>;
