@@ -611,7 +611,7 @@ typedef struct b200_q4_pages {
  * (a cos - b sin, b cos + a sin), every product and sum rounded to f32.  q_out receives the queries in the activations' type (it may be q itself; q NULL: no queries); keys and
  * values are quantised from f32 and written to slot slots[t] (page * page_size + offset).  slots[t] < 0: the token is not cached (its query is
  * rotated all the same).  A slot behind the last page: not cached, BAD_SLOT; a position outside the table: query rows of NaN, not cached, BAD_POSITION.
- * With the same slot twice in one call the slot holds either token's parts. */
+ * With the same slot twice in one call the slot holds either token's parts.  Rows of q_out do not overlap: either dimension lies between two steps of the other. */
 typedef struct b200_q4_append {
     int32_t device;
     uint32_t type;
@@ -638,7 +638,8 @@ B200_API int b200_dev_read_q4(int device, void* stream, uint32_t type, const b20
  * positions: token i of m sits at kv_lens[s] - m + i and sees the positions up to its own (window > 0: the last `window` of them).  A token that sees nothing gets zeros;
  * tokens ahead of q_starts[0] or from q_starts[seqs] on are left as they were.  Pages outside the cache count as not seen, BAD_PAGE; lengths beyond table_pages * page_size
  * are cut there, and negative ones taken as zero, BAD_LENGTH; q_starts that do not ascend within 0 .. tokens: BAD_LENGTH, the sequence is left out.  max_q: the most query tokens
- * of a sequence, as far as the host knows (0: not known); it only chooses between kernels.  workspace: b200_dev_attention_paged_q4_workspace bytes on 256 bytes. */
+ * of a sequence, as far as the host knows (0: not known); it only chooses between kernels.  Rows of out do
+ * not overlap (as q_out's).  workspace: b200_dev_attention_paged_q4_workspace bytes on 256 bytes. */
 typedef struct b200_q4_attention {
     int32_t device;
     uint32_t type;

@@ -19,6 +19,12 @@ using namespace dev;
 int bad(const char* op, const char* what) { return dev_fail(B200_ERR_INVALID_ARGUMENT, (std::string(op) + ": " + what).c_str()); }
 int shape(const char* op, const char* what) { return dev_fail(B200_ERR_SHAPE_MISMATCH, (std::string(op) + ": " + what).c_str()); }
 bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+// Whether rows of an output, hd elements each, may lie on one another: they do not where all heads of a token are between one token and the next, or all tokens of a head between one head and the next.
+bool overlap(int64_t tokens, int64_t token, int64_t heads, int64_t head, int64_t hd) {
+    if (tokens <= 1 || heads <= 1) return (tokens > 1 && token < hd) || (heads > 1 && head < hd);
+    const int64_t n = token < head ? tokens : heads, inner = std::min(token, head), outer = std::max(token, head);
+    return inner < hd || (outer - hd) / (n - 1) < inner;
+}
 int type_bytes(uint32_t t) { return t == B200_TYPE_F32 ? 4 : t == B200_TYPE_F16 || t == B200_TYPE_BF16 ? 2 : 0; }
 int bad_type(const char* op, uint32_t t) {
     return dev_fail(B200_ERR_UNSUPPORTED_DTYPE, (std::string(op) + ": type " + std::to_string(t) + " (F32, F16 and BF16 only)").c_str());
@@ -137,6 +143,7 @@ extern "C" int b200_dev_rope_append_q4(const b200_q4_append* a) {
         if (a->tokens < 0 || a->table_rows < 1) return shape(op, "bad number of tokens or table rows");
         if (a->q && (a->n_heads < 1 || a->n_heads > 65536)) return shape(op, "bad number of query heads");
         if (a->tokens * ((a->q ? a->n_heads : 0) + 2LL * a->cache.n_kv_heads) >= kMost || a->tokens >= kMost) return shape(op, "too many rows for one call");
+        if (a->q && overlap(a->tokens, a->q_out_token, a->n_heads, a->q_out_head, a->cache.head_dim)) return shape(op, "rows of q_out overlap");
         if (a->tokens == 0) return B200_OK;
         if (!a->k || !a->v || !a->cos_sin || !a->positions || !a->slots || (a->q && !a->q_out)) return bad(op, "null pointer");
         if (a->q && a->q == a->q_out && (a->q_token != a->q_out_token || a->q_head != a->q_out_head)) return bad(op, "q in place needs the same strides");
@@ -202,6 +209,7 @@ extern "C" int b200_dev_attention_paged_q4(const b200_q4_attention* a) {
     return entry(op, [&]() -> int {
         int rc = check_attention(op, a);
         if (rc) return rc;
+        if (overlap(a->tokens, a->out_token, a->n_heads, a->out_head, a->cache.head_dim)) return shape(op, "rows of out overlap");
         if (a->tokens == 0 || a->seqs == 0) return B200_OK;
         if (!a->q || !a->out || !a->kv_lens || (a->table_pages > 0 && !a->page_table)) return bad(op, "null pointer");
         const size_t need = attention_q4_workspace(*a);

@@ -130,7 +130,8 @@ def rope_append_q4(q, k, v, cos_sin, positions, pages, slots, use_neox=False, q_
     """Rotates q and k, puts k and v into the cache in 4 bits, returns the rotated q (q None: None).
 
     q [tokens, heads, hd], k, v [tokens, kv heads, hd] (any distance between tokens and heads), cos_sin [positions, rot dims] f32 (rotary_table), positions int32 and
-    slots int64 [tokens]: token t goes to page slots[t] // page_size, place slots[t] % page_size; slots[t] < 0: it is not cached.  q_out may be q."""
+    slots int64 [tokens]: token t goes to page slots[t] // page_size, place slots[t] % page_size; slots[t] < 0: it is not cached.  The slots of a call
+    are different ones (one that comes twice holds parts of either token).  q_out may be q."""
     return _ops().rope_append_q4(q, k, v, cos_sin, positions, pages, slots, use_neox, q_out, status)
 
 

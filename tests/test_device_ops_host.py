@@ -127,6 +127,17 @@ def test_attention_refusals(b200, D):
             refused(b200, L.b200_dev_attention_paged_q4(C.byref(struct(**change))), b200.InvalidArgument, "workspace")
 
 
+def test_outputs_whose_rows_overlap_are_refused(b200, D):
+    L = D._lib()
+    for token, head in ((0, 64), (256, 0), (63, 256), (256, 63), (64, 64), (-256, 64), (255, 64), (64, 191), (1 << 62, 1 << 61)):
+        a = D.Q4Append(device=0, type=0, q=AT, k=AT, v=AT, q_out=AT + 4096, q_token=256, q_head=64, k_token=128, k_head=64, v_token=128, v_head=64, q_out_token=token, q_out_head=head, cos_sin=AT,
+                       table_rows=10, positions=AT, slots=AT, tokens=3, n_heads=4, rot_dims=64, use_neox=0, cache=pages(D))
+        refused(b200, L.b200_dev_rope_append_q4(C.byref(a)), b200.ShapeMismatch, "overlap")
+        o = D.Q4Attention(device=0, type=0, q=AT, out=AT, q_token=256, q_head=64, out_token=token, out_head=head, kv_lens=AT, page_table=AT, table_stride=4, tokens=3, table_pages=4, seqs=3,
+                          n_heads=4, scale=0.1, cache=pages(D))
+        refused(b200, L.b200_dev_attention_paged_q4(C.byref(o)), b200.ShapeMismatch, "overlap")
+
+
 def test_python_refusals(b200, D):
     f32, i8 = torch.zeros(4, 64), torch.zeros(4, 64, dtype=torch.int8)
     one = torch.ones(64)
