@@ -16,9 +16,9 @@
 // second ones go through another mma into the same sums.  bf16 has its queries exactly in one, and its weights are rounded to one (2^-11, an eighth of the result's own step).
 // The weight of a value is p_j d_j.  Its reference is not m but m + r, the largest z_j + log2 |d_j| so far: p_j d_j stays in fp16's range whatever the values' scales are (r is kept by itself: large
 // scores leave no bits of log2 |d_j| in a sum).  Both references move only when something passes them by 2^8, so the usual step has no exchange between lanes but the 8 x 8 transposition that makes operands of the weights.
-// What bounds it: the bytes of the cache, hd + 8 per position and kv head.  Measured (both kernels, cold): one token over 131072 positions, 64 heads over 8 of 128, bf16: 47 us for 143 MB (3.0 TB/s): about 7 us until
+// What bounds it: the bytes of the cache, hd + 8 per position and kv head.  Measured (both kernels, cold): one token over 131072 positions, 64 heads over 8 of 128, bf16: 46 us for 143 MB (3.1 TB/s): about 7 us until
 // every block knows its stretch and has its first tiles, 29 of stream at 4.9 TB/s (a kernel of the same copies without the arithmetic: 36 altogether), a spread of the blocks' ends, 4 of the join.  32 sequences of up to
-// 8000: 38.5 us for 96 MB.  A warp takes 32 positions a step (two of the above, so that its chains of mma cover each other).  Warps of an SM and positions of a step (us, the two cases): 12 and 32 46.5, 38.7;
+// 8000: 38 to 41 us for 96 MB.  A warp takes 32 positions a step (two of the above, so that its chains of mma cover each other).  When the last steps were tried, warps of an SM and positions of a step (us, the two cases): 12 and 32 46.5, 38.7;
 // 16 and 32 51, 44.6; 16 and 16 52, 43; 8 and 48 43.9 to 45, 39.5 to 43: the first of these is the best of the two together and the steadier.
 #pragma once
 #include <type_traits>
@@ -110,6 +110,18 @@ __device__ __forceinline__ uint32_t transposed8x8(uint32_t v) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
+}
+// loads that are made where `there` holds, and zeros elsewhere, without a choice after the load, which would wait for it
+template <int N> __device__ __forceinline__ void load_where(uint32_t (&v)[N], const void* p, bool there) {
+    if constexpr (N == 4)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t@p ld.global.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
+                     : "=&r"(v[0]), "=&r"(v[1]), "=&r"(v[2]), "=&r"(v[3])
+                     : "l"(p), "r"((uint32_t)there)
+                     : "memory");
+    else if constexpr (N == 2)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t@p ld.global.v2.u32 {%0,%1}, [%2];\n\t}" : "=&r"(v[0]), "=&r"(v[1]) : "l"(p), "r"((uint32_t)there) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.u32 %0, [%1];\n\t}" : "=&r"(v[0]) : "l"(p), "r"((uint32_t)there) : "memory");
 }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -251,7 +263,9 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
                         row[b] -= page_size;
                         over++;
                     }
-                if (p_look + 16 * b < p_stop) page[b] = table[index + over];
+                uint32_t got[1];
+                load_where<1>(got, table + index + over, p_look + 16 * b < p_stop);
+                page[b] = (int)got[0];
             }
             p_look += TILE;
             index += tile_pages;

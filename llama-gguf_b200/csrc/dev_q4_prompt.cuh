@@ -105,18 +105,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(two(a)), "l"(two(b)), "l"(two(c)));
     return two(r);
 }
-// loads that are made where `there` holds, and zeros elsewhere, without a choice after the load, which would wait for it
-template <int N> __device__ __forceinline__ void load_where(uint32_t (&v)[N], const void* p, bool there) {
-    if constexpr (N == 4)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t@p ld.global.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
-                     : "=&r"(v[0]), "=&r"(v[1]), "=&r"(v[2]), "=&r"(v[3])
-                     : "l"(p), "r"((uint32_t)there)
-                     : "memory");
-    else if constexpr (N == 2)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t@p ld.global.v2.u32 {%0,%1}, [%2];\n\t}" : "=&r"(v[0]), "=&r"(v[1]) : "l"(p), "r"((uint32_t)there) : "memory");
-    else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.u32 %0, [%1];\n\t}" : "=&r"(v[0]) : "l"(p), "r"((uint32_t)there) : "memory");
-}
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // D = f32, A = B = bf16 (1) or fp16 (0), K-major
