@@ -261,7 +261,8 @@ def run(s):
 
     if s["op"] == "norm":
         q, scale, r = D.add_rms_norm_q8(s["x"], s["w"], EPS, residual=s["r"])
-        return [D.read_q8(q, scale, torch.bfloat16), scale] + ([] if r is None else [r])
+        value = torch.mul(q, scale[:, None], out=torch.empty(q.shape, dtype=torch.bfloat16, device=q.device))
+        return [value, scale] + ([] if r is None else [r])
     if s["op"] == "product":
         return D.mat_mat_i8(s["q"], s["s"], s["w"], s["ws"], bias=s["b"], dtype=t)
     if s["op"] == "append":
