@@ -1,6 +1,7 @@
 // dev_norm_q8.cuh — RMS norm of a residual sum with the result in 8 bits and a scale per row (b200_dev_add_rms_norm_q8).
 #pragma once
 #include <algorithm>
+#include <type_traits>
 
 #include "dev_common.cuh"
 
@@ -50,7 +51,8 @@ __device__ __forceinline__ Q8Row q8_row(uint32_t top) {
 }
 
 // Rows of whole 16-byte words on 16 bytes: a block per row, which stays in registers (V words per thread, asked for together) from its only load on.
-// The squares of 16-bit types are exact in f32; each is added in 64 bits, so that the sum, and with it every 8-bit number, does not depend on the order.
+// A square has twice its element's bits and exponent: f16's fits f32, bf16's passes its range both ways, so that one and f32's are made and added in 64 bits.  (A sum of them is rounded, and
+// its order that of the kernel: at 2^-53 of the sum, which only a reciprocal root next to a border of f32 shows.)
 template <typename T, int V> __global__ void __launch_bounds__(1024) add_rms_norm_q8_kernel(const NormQ8Args a) {
     before();
     constexpr int E = 16 / (int)sizeof(T);
@@ -82,7 +84,7 @@ template <typename T, int V> __global__ void __launch_bounds__(1024) add_rms_nor
 #pragma unroll
         for (int e = 0; e < E; e++) {
             r[v][e] = to_f(reinterpret_cast<T*>(&w[v])[e]);
-            ss += sizeof(T) == 2 ? (double)(r[v][e] * r[v][e]) : (double)r[v][e] * r[v][e];
+            ss += std::is_same<T, __half>::value ? (double)(r[v][e] * r[v][e]) : (double)r[v][e] * r[v][e];
         }
     }
     const float rstd = q8_rstd(block_sum(ss, s_sum), a.hidden, a.eps);
