@@ -14,8 +14,8 @@
 //   values  1024 + n is n in the low bits of the fp16 1024; minus 1032 it is n - 8.  (Sums of n alone would grow with the keys while the result does not: f32 sums would lose 1e-4 of it.)
 // Queries are scaled by a power of two into fp16's range.  f32 queries are two fp16 numbers (what the first leaves over is the second), and so are the weights of f32 and f16 results: the
 // second ones go through another mma into the same sums.  bf16 has its queries exactly in one, and its weights are rounded to one (2^-11, an eighth of the result's own step).
-// The weight of a value is p_j d_j.  Its reference is not m but m + r, the largest z_j + log2 |d_j| so far: p_j d_j stays in fp16's range whatever the values' scales are (r is kept by itself: large
-// scores leave no bits of log2 |d_j| in a sum).  Both references move only when something passes them by 2^8, so the usual step has no exchange between lanes but the 8 x 8 transposition that makes operands of the weights.
+// The weight of a value is p_j d_j.  Its reference is not m but m + r, the largest z_j + log2 |d_j| so far less 7: p_j d_j stays in fp16's range whatever the values' scales are, from 2^7 to 2^15 where it is largest,
+// so that fp16's last bit, 2^-25, is 2^-32 of that (r is kept by itself: large scores leave no bits of log2 |d_j| in a sum).  Both references move only when something passes them by 2^8, so the usual step has no exchange between lanes but the 8 x 8 transposition that makes operands of the weights.
 // What bounds it: the bytes of the cache, hd + 8 per position and kv head.  Measured (both kernels, cold): one token over 131072 positions, 64 heads over 8 of 128, bf16: 46 us for 143 MB (3.1 TB/s): about 7 us until
 // every block knows its stretch and has its first tiles, 29 of stream at 4.9 TB/s (a kernel of the same copies without the arithmetic: 36 altogether), a spread of the blocks' ends, 4 of the join.  32 sequences of up to
 // 8000: 38 to 41 us for 96 MB.  A warp takes 32 positions a step (two of the above, so that its chains of mma cover each other).  When the last steps were tried, warps of an SM and positions of a step (us, the two cases): 12 and 32 46.5, 38.7;
@@ -28,6 +28,7 @@
 namespace dev {
 
 enum { QA_ROWS = 8, QA_START = 4, QA_WARPS = 12, QA_STAGES = 3 };      // rows of an item, units of its start, warps of an SM
+constexpr float QA_UP = 7.0f;                                           // log2 of the weight that a reference is set to
 
 struct Q4Seq {
     int first, count;      // query tokens
@@ -464,7 +465,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
                     for (int k = 0; k < 2; k++) {
                         x[b][u][k] = z[b][u][k] - m[k];
                         y[b][u][k] = x[b][u][k] + (ex[b][u] - mr[k]);
-                        past |= x[b][u][k] > 8.0f || y[b][u][k] > 8.0f;
+                        past |= x[b][u][k] > 8.0f || y[b][u][k] > 8.0f + QA_UP;
                     }
                 }
             if (__any_sync(0xffffffffu, past)) {
@@ -482,7 +483,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
                     for (int b = 0; b < U; b++) topr = fmaxf(topr, fmaxf(z[b][0][k] - top + ex[b][0], z[b][1][k] - top + ex[b][1]));
 #pragma unroll
                     for (int o = 4; o <= 16; o <<= 1) topr = fmaxf(topr, __shfl_xor_sync(0xffffffffu, topr, o));
-                    topr = fmaxf(topr, was);
+                    topr = fmaxf(topr - QA_UP, was);
                     l[k] *= ex2(up);
                     const float f = ex2(below(was, topr));
 #pragma unroll

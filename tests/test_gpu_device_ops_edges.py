@@ -2,7 +2,9 @@
 import pytest
 import torch
 
-from test_gpu_device_ops import D, check_norm, normal  # noqa: F401
+import device_ops_exact as X
+import device_ops_ref as R
+from test_gpu_device_ops import TYPES, D, cache, check_norm, normal  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -20,3 +22,45 @@ def test_norm_of_rows_of_any_magnitude(D, dtype, magnitude, rows, hidden):  # no
     odd = torch.empty(rows, hidden + 1, dtype=dtype, device="cuda")[:, 1:]
     odd.copy_(x)
     assert all(torch.equal(a, b) for a, b in zip(D.add_rms_norm_q8(x, w, eps)[:2], D.add_rms_norm_q8(odd, w, eps)[:2]))
+
+
+# -------------------------------------------------------------------------------------------------------------- attention
+def run_attention(D, q, pages, table, lens, starts, **kw):  # noqa: F811
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    return D.attention_paged_q4(q.cuda(), pages.cuda(), table.cuda(), i32(lens), q_starts=None if starts == list(range(len(lens) + 1)) else i32(starts), **kw).double()
+
+
+def within(got, want, off, dtype):
+    low, high = X.rounded(want, off, dtype)
+    wrong = ~((got >= low) & (got <= high))
+    assert not wrong.any(), (int(wrong.sum()), float(((got - want).abs() / (off + 2.0**-149))[wrong].max()))
+
+
+def starts_of(q_lens):
+    s = [0]
+    for m in q_lens:
+        s.append(s[-1] + m)
+    return s
+
+
+def one_large_score(nh, nkv, hd, page, seqs, n, first):
+    """Positions of which the first one's key is far ahead of all others; its value is `first` times as large as theirs, and nothing but in channel 0."""
+    k, v = normal(3, n, nkv, hd) / 16, 0.5 + normal(4, n, nkv, hd).abs()
+    k[0], v[0, :, 0], v[0, :, 1:] = 1.0, v[0, :, 0] * first, 0.0
+    table = torch.randperm(n // page, generator=torch.Generator().manual_seed(5)).int()[None].expand(seqs, -1).contiguous()
+    pages = torch.zeros(n // page, nkv, page * (hd + 8), dtype=torch.uint8)
+    at = torch.arange(n)
+    R.put_rows(pages, page, hd, table[0, at // page].long() * page + at % page, k, v)
+    return pages, table
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("first", [2.0**-6, 1.0, 8.0])
+@pytest.mark.parametrize("high", [14.0, 18.0])
+def test_attention_of_single_tokens_with_one_large_score(D, dtype, first, high):  # noqa: F811
+    """The first position's weight is e^14 to e^18 times any other's, but its value has one channel: the rest of the result is theirs."""
+    n, nh, nkv, hd, page, seqs = 4096, 32, 32, 64, 16, 8
+    pages, table = one_large_score(nh, nkv, hd, page, seqs, n, first)
+    q = (high * hd**-0.5 + 0.01 * normal(6, seqs, nh, hd)).to(dtype)
+    want, off = X.attention(q, pages, table, [n] * seqs, list(range(seqs + 1)), page, hd**-0.5)
+    within(run_attention(D, q, pages, table, [n] * seqs, list(range(seqs + 1))), want, off, dtype)
