@@ -12,8 +12,8 @@
 //   scores  a nibble in the low bits of an fp16 is the number n 2^-24 exactly (four bits further up: 16 n 2^-24, and that channel's query element is divided by 16): one shift
 //           and four ands turn eight nibbles into operands.  - 8 sum q is taken off afterwards in f32 (not for f32 results, which that would cost three bits: theirs are made as the values').
 //   values  1024 + n is n in the low bits of the fp16 1024; minus 1032 it is n - 8.  (Sums of n alone would grow with the keys while the result does not: f32 sums would lose 1e-4 of it.)
-// Queries are scaled by a power of two into fp16's range.  f32 queries are two fp16 numbers (what the first leaves over is the second), and so are the weights of f32 and f16 results: the
-// second ones go through another mma into the same sums.  bf16 has its queries exactly in one, and its weights are rounded to one (2^-11, an eighth of the result's own step).
+// Queries are scaled by a power of two into fp16's range.  Weights are two fp16 numbers (what the first leaves over is the second: 2^-22), and so are f32 queries: the second ones go through another mma into the
+// same sums.  f16 and bf16 queries are one exactly.  (Weights of one number, 2^-11, took a tenth less time for bf16 results, which they moved to the next number now and then.)
 // The weight of a value is p_j d_j.  Its reference is not m but m + r, the largest z_j + log2 |d_j| so far less 7: p_j d_j stays in fp16's range whatever the values' scales are, from 2^7 to 2^15 where it is largest,
 // so that fp16's last bit, 2^-25, is 2^-32 of that (r is kept by itself: large scores leave no bits of log2 |d_j| in a sum).  Both references move only when something passes them by 2^8, so the usual step has no exchange between lanes but the 8 x 8 transposition that makes operands of the weights.
 // What bounds it: the bytes of the cache, hd + 8 per position and kv head.  Measured (both kernels, cold): one token over 131072 positions, 64 heads over 8 of 128, bf16: 46 us for 143 MB (3.1 TB/s): about 7 us until
@@ -148,7 +148,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
     using St = Q4Stage<HD>;
     using Sm = Q4Smem<HD, W, U>;
     constexpr int STAGES = Sm::STAGES, TILE = Sm::TILE, WORDS = HD / 32, NT = HD / 16;      // words of a key row per lane; row tiles of the values
-    constexpr bool Q2 = sizeof(T) == 4, P2 = !std::is_same<T, __nv_bfloat16>::value;
+    constexpr bool Q2 = sizeof(T) == 4;
     before();
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ long long s_sum[W];
@@ -524,10 +524,8 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
                         w[k] = __uint_as_float(__float_as_uint(ex2(y[b][u][k])) ^ (vs[b][u] & 0x80000000u));
                     }
                     pb[u] = pack_h2(w[0], w[1]);
-                    if (P2) {
-                        const float2 f = unpack_h2(pb[u]);
-                        pl[u] = transposed8x8(pack_h2(w[0] - f.x, w[1] - f.y));
-                    }
+                    const float2 f = unpack_h2(pb[u]);
+                    pl[u] = transposed8x8(pack_h2(w[0] - f.x, w[1] - f.y));
                     pb[u] = transposed8x8(pb[u]);
                 }
                 // values: [positions 2 c, 2 c + 1; + 8][word g, word g + 8], channels 0-3 and 4-7 of the word
@@ -556,7 +554,7 @@ template <typename T, int HD, int W, int U> __global__ void __launch_bounds__(32
                         v[2 * u + 1] = HD == 128 ? nibble(HD / 64 - 1, u, i) : nibble(0, u, i + 4);
                     }
                     mma16(acc[i], v[0], v[1], v[2], v[3], pb[0], pb[1]);
-                    if (P2) mma16(acc[i], v[0], v[1], v[2], v[3], pl[0], pl[1]);
+                    mma16(acc[i], v[0], v[1], v[2], v[3], pl[0], pl[1]);
                 }
             }
         }

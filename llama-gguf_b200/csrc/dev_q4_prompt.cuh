@@ -9,8 +9,7 @@
 //               products; the two are joined at the end.  P goes back to tensor memory in place of S.
 // Keys' scales multiply the scores, values' scales the weights.  f32 queries are pairs of fp16 numbers scaled by a power of two.  Passes:
 //   steady  The reference of a row's exponentials need only be near: it is the largest score of the first tile that the row sees, and stays.  So no tile waits for another: one O, three buffers of scores,
-//           each score read once.  A weight p_j d_j is an fp16 number (bf16 results: 2^-11, an eighth of their own step) or two of them (what the first leaves over is the second: 2^-22), near one
-//           where the reference was set.
+//           each score read once.  A weight p_j d_j is two fp16 numbers (what the first leaves over is the second: 2^-22), near one where the reference was set.
 //   moving  Where a row passes fp16's range, or the last bits of its weights may have cost too much of its result (Q4Weights), or its result is not finite, the block makes a second pass: weights are
 //           pairs of bf16 (2^-16), which have f32's range, and the reference goes up by a whole number, which no bf16 notices, when a score passes it by 2^16.
 // What bounds it: per row and tile 128 x (hd + hd) products (three times that for f32), 128 exponentials with some ten instructions each, and shared memory: both operands of S and the values of P V are
@@ -243,7 +242,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
 
     // one pass over the keys (the moving one: two buffers, a group's sums of its own)
     auto pass = [=](auto mode) mutable {
-        constexpr bool steady = decltype(mode)::value, ONE = steady && BF;      // steady: weights and values in fp16; ONE: one number per weight
+        constexpr bool steady = decltype(mode)::value;      // weights and values in fp16
         const uint32_t bars = base + Sm::BAR_AT + (steady ? 0 : Sm::BARS * 8);
         const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64, p_full = bars + 112, pv_done = bars + 136, all_done = bars + 160;
         if (warp >= QP_MAKE && warp < QP_MMA) {
@@ -416,8 +415,8 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
 #pragma unroll
                         for (int kk = 0; kk < 8; kk++)
 #pragma unroll
-                            for (int u = 0; u < (ONE ? 1 : 2); u++)
-                                mma_ts(to, ONE ? from + 8 * kk : from + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * u, dv + (uint64_t)((kk >> 2) * (HD * 128 >> 4) + 2 * (kk & 3)), ipv, t >= (steady ? 1 : 2) || kk + u > 0);
+                            for (int u = 0; u < 2; u++)
+                                mma_ts(to, from + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * u, dv + (uint64_t)((kk >> 2) * (HD * 128 >> 4) + 2 * (kk & 3)), ipv, t >= (steady ? 1 : 2) || kk + u > 0);
                     }
                     umma_commit<false>(v_empty + 8 * st);
                     umma_commit<false>(pv_done + 8 * b);
@@ -571,7 +570,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
 #pragma unroll
                             for (int i = 0; i < 16; i++) x[i] = add2(x[i], make_float2(-up, -up));
                         }
-                        uint32_t o[ONE ? 16 : 32];
+                        uint32_t o[32];
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             const float4 d = k4[32 + 8 * j + i];
@@ -584,9 +583,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                                     if ((hid >> (4 * i + 2 * u + 1)) & 1u) w.y = 0.0f;
                                 }
                                 sum = add2(sum, p);
-                                if constexpr (ONE) {
-                                    o[2 * i + u] = pack_h2(w.x, w.y);
-                                } else if constexpr (steady) {
+                                if constexpr (steady) {
                                     o[2 * i + u] = pack_h2(w.x, w.y);
                                     const float2 f = unpack_h2(o[2 * i + u]);
                                     o[16 + 2 * i + u] = pack_h2(w.x - f.x, w.y - f.y);
@@ -598,8 +595,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                                 }
                             }
                         }
-                        if constexpr (ONE) tmem_st16(S + 16 * j, o);      // (over columns that have been read)
-                        else tmem_st32(S + 32 * j, o);
+                        tmem_st32(S + 32 * j, o);      // (over columns that have been read)
                     };
                     by_32(S, take);
                     l += sum.x + sum.y;

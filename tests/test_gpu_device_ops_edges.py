@@ -43,6 +43,19 @@ def starts_of(q_lens):
     return s
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nh,nkv,hd,lens,q_lens", [(8, 2, 128, [1, 0, 333, 1000], [1] * 4), (16, 1, 64, [40, 2500], [1, 1]), (4, 2, 128, [40, 500], [7, 3]), (96, 24, 128, [300, 90], [70, 33]),
+                                                   (24, 24, 64, [513], [200])])
+@pytest.mark.parametrize("gain", [1.0, 6.0])
+def test_attention_is_rounded_once(D, dtype, nh, nkv, hd, lens, q_lens, gain):  # noqa: F811
+    """A result is what 64 bits give, rounded to its type: nothing on the way is held in fewer bits than f32 has, but for what the bound counts."""
+    pages, table = cache(3, lens, nkv, hd, 16)
+    starts = starts_of(q_lens)
+    q = (gain * normal(8, starts[-1], nh, hd)).to(dtype)
+    want, off = X.attention(q, pages, table, lens, starts, 16, hd**-0.5)
+    within(run_attention(D, q, pages, table, lens, starts), want, off, dtype)
+
+
 def one_large_score(nh, nkv, hd, page, seqs, n, first):
     """Positions of which the first one's key is far ahead of all others; its value is `first` times as large as theirs, and nothing but in channel 0."""
     k, v = normal(3, n, nkv, hd) / 16, 0.5 + normal(4, n, nkv, hd).abs()
