@@ -2,16 +2,18 @@
 //
 // The same function as dev_q4_attn.cuh.  A block has 128 query rows (row = token * G + head) of one sequence and kv head and walks the keys they see in tiles of 128:
 //   warps 8-15  read a tile's nibbles (a page's row is one to four 16-byte words) and write them to shared memory as operands: 128 + n is n in the low bits of the bf16 128, 1024 + n those of the
-//               fp16 1024; minus 136 or 1032 it is n - 8.  Keys as they lie, their channels in groups of eight in the order 0 4 1 5 2 6 3 7 (one shift and one and give two of them), which the
+//               fp16 1024; minus 136 or 1032 it is n - 8 (keys have the queries' type, values are fp16).  Keys as they lie, their channels in groups of eight in the order 0 4 1 5 2 6 3 7 (one shift and one and give two of them), which the
 //               queries have too; values transposed, two positions per 32-bit word.
 //   warp 16     issues S = Q K^T (128 x 128, K = hd) and O += P V (N = hd, K = 128).
 //   warps 0-7   one thread per row, two groups of four warps that take every second tile with sums, maximum and statistics of their own, so that one group's exponentials run under the other's
 //               products; the two are joined at the end.  P goes back to tensor memory in place of S.
 // Keys' scales multiply the scores, values' scales the weights.  f32 queries are pairs of fp16 numbers scaled by a power of two.  Passes:
-//   steady  The reference of a row's exponentials need only be near: it is the largest score of the first tile that the row sees, and stays.  So no tile waits for another: one O, three buffers of scores,
-//           each score read once.  A weight p_j d_j is two fp16 numbers (what the first leaves over is the second: 2^-22), near one where the reference was set.
-//   moving  Where a row passes fp16's range, or the last bits of its weights may have cost too much of its result (Q4Weights), or its result is not finite, the block makes a second pass: weights are
-//           pairs of bf16 (2^-16), which have f32's range, and the reference goes up by a whole number, which no bf16 notices, when a score passes it by 2^16.
+//   first   The reference of a row's exponentials need only be near: it is the largest score of the first tile that the row sees, and stays.  So no tile waits for another: one O, three buffers of scores,
+//           each score read once.  A weight p_j d_j is two fp16 numbers (what the first leaves over is the second: 2^-22), 2^4 or so
+//           where the reference was set.
+//   scan, again   Where a row passes fp16's range, or the last bits of its weights may have cost too much of its result (Q4Weights), or its result is not finite, the block goes over the keys twice more: once for
+//           the scores alone, which gives each row its largest score m and its largest weight, and once as above with these for references: probabilities 2^(z_j - m), weights p_j d_j 2^e of up to 2^14 in pairs of fp16
+//           numbers, whose last bit, 2^-25, is 2^-38 of the largest.
 // What bounds it: per row and tile 128 x (hd + hd) products (three times that for f32), 128 exponentials with some ten instructions each, and shared memory: both operands of S and the values of P V are
 // read from it, and 48 KB of them written per tile.  A tile takes 1.7 us at hd 128, on one SM as on all: a tile of a warp of rows some 2900 clocks (two groups share the tiles), of a warp that makes operands 2300, the products
 // 1400 with their starts, each slowing the others at the schedulers.  Measured: 2048 query tokens after 2048 others, 32 heads over 8 of 128, bf16: 182 us, 512 blocks of 17 to 32 tiles, 570 TFLOP/s of the products that
@@ -25,16 +27,19 @@ namespace dev {
 
 enum { QP_ROWS = 128, QP_KEYS = 128, QP_SOFT = 8, QP_MAKE = 8, QP_MMA = 16, QP_THREADS = 544 };
 
-// by the result's type: the weights' place (2^-kUp at the reference; above it is room for 2^16 2^kUp), and the part of a row's largest channel that its weights' last bits, 2^-25 of each times a
-// value of up to 8, may have cost: half a step of bf16 and of f16 results; of f32 results what the second pass is off by
-template <typename T> struct Q4Weights { static constexpr float kUp = 0.0f, kOff = 1.0f / (1 << 8); };
-template <> struct Q4Weights<__half> { static constexpr float kUp = 0.0f, kOff = 1.0f / (1 << 11); };
-template <> struct Q4Weights<float> { static constexpr float kUp = -4.0f, kOff = 1.0f / (1 << 16); };
+// The weights' place: 2^4 at the reference, so that 2^-29 of it is their last bit, and scores have room for 2^12 above it (8.3 in natural logarithms; of Gaussian scores of standard deviation 2 a few in 1e8 pass
+// 2^10, which cost 2048 tokens behind 2048 a third of their time).
+constexpr float kUp = -4.0f;
+// by the result's type: the part of a row's largest channel that its weights' last bits, 2^-25 of each times a value of up to 8, may have cost at most, had they all one sign: half a step of bf16 and of f16
+// results, 2^-16 of f32 ones
+template <typename T> struct Q4Weights { static constexpr float kOff = 1.0f / (1 << 8); };
+template <> struct Q4Weights<__half> { static constexpr float kOff = 1.0f / (1 << 11); };
+template <> struct Q4Weights<float> { static constexpr float kOff = 1.0f / (1 << 16); };
 
 template <typename T, int HD> struct Q4PromptSmem {
     static constexpr int NQ = sizeof(T) == 4 ? 2 : 1;
     static constexpr int SLAB = 128 * 128, Q = NQ * (HD / 64) * SLAB, K = (HD / 64) * SLAB, V = 2 * HD * 128;      // rows of 128 bytes, SWIZZLE_128B
-    static constexpr int K_AT = Q, V_AT = K_AT + 2 * K, META_AT = V_AT + 2 * V, META = 128 * 4 * 2 + 16, STAT_AT = META_AT + 4 * META, BAR_AT = STAT_AT + 2 * 128 * 8, BARS = 21, BYTES = BAR_AT + 2 * BARS * 8;
+    static constexpr int K_AT = Q, V_AT = K_AT + 2 * K, META_AT = V_AT + 2 * V, META = 128 * 4 * 2 + 16, STAT_AT = META_AT + 4 * META, BAR_AT = STAT_AT + 2 * 128 * 8, BARS = 21, BYTES = BAR_AT + 3 * BARS * 8;
 };
 template <bool BF> __device__ __forceinline__ uint32_t sub_2(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -59,23 +64,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
         "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
         "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
         : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
-                 "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr)
-                 : "memory");
-}
-// sixteen columns of this warp's lanes: asked for, and there (the registers are not to be touched in between)
-__device__ __forceinline__ void tmem_ask16(uint32_t (&v)[16], uint32_t taddr) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-                   "=r"(v[14]), "=r"(v[15])
-                 : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_got(uint32_t (&v)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]),
-                   "+r"(v[14]), "+r"(v[15])::"memory");
 }
 // take(j, columns 32 j .. 32 j + 31) for a tile's 128 (a loop: the code of all of them at once does not stay in the instruction cache)
 template <typename F> __device__ __forceinline__ void by_32(uint32_t taddr, F&& take) {
@@ -115,15 +103,19 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// the pass that few blocks make, in code and registers of its own (by copy: nothing of the first pass gets an address)
-template <typename F> __device__ __noinline__ void apart(F pass) { pass(std::false_type{}); }
+// passes; the two that few blocks make have code and registers of their own (by copy: nothing of the first one gets an address)
+enum { QP_FIRST, QP_SCAN, QP_AGAIN };
+template <typename F> __device__ __noinline__ void once_more(F pass) {
+    pass(std::integral_constant<int, QP_SCAN>{});
+    pass(std::integral_constant<int, QP_AGAIN>{});
+}
 
 template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) attention_q4_prompt_kernel(const b200_q4_attention a, uint64_t page16, int64_t limit) {
     before();
     using Sm = Q4PromptSmem<T, HD>;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
     constexpr int NQ = Sm::NQ, SLABS = HD / 64;
-    constexpr float kUp = Q4Weights<T>::kUp, kOff = Q4Weights<T>::kOff;
+    constexpr float kOff = Q4Weights<T>::kOff;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_item[2], s_bad;
@@ -162,11 +154,11 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
             s_item[1] = rb;
         }
     }
-    // barriers of either pass (see below): keys there, used; values there, used (2 each); scores there (6); weights there, their products done (3 each); all products done
+    // barriers of each pass (see below): keys there, used; values there, used (2 each); scores there (6); weights there, their products done (3 each; the scan: scores read, 6); all products done
     if (warp == 1) {
-        for (int i = lane; i < 2 * Sm::BARS; i += 32) {
+        for (int i = lane; i < 3 * Sm::BARS; i += 32) {
             const int b = i % Sm::BARS;
-            bar_init(base + Sm::BAR_AT + 8 * i, b < 2 || b == 4 || b == 5 ? QP_MMA - QP_MAKE : b >= 14 && b < 17 ? 4 : 1);
+            bar_init(base + Sm::BAR_AT + 8 * i, b < 2 || b == 4 || b == 5 ? QP_MMA - QP_MAKE : b >= 14 && b < (i / Sm::BARS == QP_SCAN ? 20 : 17) ? 4 : 1);
         }
         bar_init_done();
         if (lane == 0) s_bad = 0;
@@ -240,10 +232,10 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
     const uint32_t tmem = s_tmem;
     bool alive = true;
 
-    // one pass over the keys (the moving one: two buffers, a group's sums of its own)
+    // one pass over the keys
     auto pass = [=](auto mode) mutable {
-        constexpr bool steady = decltype(mode)::value;      // weights and values in fp16
-        const uint32_t bars = base + Sm::BAR_AT + (steady ? 0 : Sm::BARS * 8);
+        constexpr int PASS = decltype(mode)::value;
+        const uint32_t bars = base + Sm::BAR_AT + PASS * Sm::BARS * 8;
         const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, s_full = bars + 64, p_full = bars + 112, pv_done = bars + 136, all_done = bars + 160;
         if (warp >= QP_MAKE && warp < QP_MMA) {
             // ---- operands of keys and values
@@ -333,7 +325,8 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                     }
                 }
                 uint8_t* meta = smem + Sm::META_AT + (t & 3) * Sm::META;
-                reinterpret_cast<uint32_t*>(meta)[(lane < 16 ? 0 : 128) + 16 * pw + (lane & 15)] = w.scale[0];
+                // (the scan wants the values' scales as powers of two)
+                reinterpret_cast<uint32_t*>(meta)[(lane < 16 ? 0 : 128) + 16 * pw + (lane & 15)] = PASS == QP_SCAN && lane >= 16 ? __float_as_uint(__log2f(fabsf(__uint_as_float(w.scale[0])))) : w.scale[0];
                 const uint32_t gone = ~__ballot_sync(0xffffffffu, w.there);
                 if (lane == 0) reinterpret_cast<uint16_t*>(meta + 1024)[pw] = (uint16_t)gone;
             };
@@ -345,14 +338,14 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 for (int j = 0; j < VW; j++) {
                     const uint32_t x[2] = {__byte_perm(w.v[0][j], w.v[1][j], 0x5410), __byte_perm(w.v[0][j], w.v[1][j], 0x7632)};
 #pragma unroll
-                    for (int k = 0; k < 8; k++) sts32(vt + ((v_word + j) * 8 + k) * 128 + ((c8 ^ k) << 4), nibbles<!steady>(x[k >> 2] >> (4 * (k & 3)), mask));
+                    for (int k = 0; k < 8; k++) sts32(vt + ((v_word + j) * 8 + k) * 128 + ((c8 ^ k) << 4), nibbles<false>(x[k >> 2] >> (4 * (k & 3)), mask));
                 }
             };
             first_look(of_keys, 16 * pw);
-            first_look(of_values, v_key & ~15);
+            if (PASS != QP_SCAN) first_look(of_values, v_key & ~15);
             if (n > 0) {
                 ask_keys();
-                ask_values();
+                if (PASS != QP_SCAN) ask_values();
             }
             // (a tile's keys before the values of the one ahead of it: these wait for products that need a row's exponentials, those only for the scores two tiles ago)
 #pragma unroll 1
@@ -360,13 +353,15 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 if (t < n) {
                     const int st = t & 1;
                     bar_wait(k_empty + 8 * st, ((t >> 1) & 1) ^ 1u, alive, 11);
+                    // (the scales of the tile four ago have been read: where values are made, those of two tiles ago were behind the products of its weights)
+                    if (PASS == QP_SCAN && t >= 4) bar_wait(p_full + 8 * ((t - 4) % 6), ((t - 4) / 6) & 1, alive, 19);
                     make_keys(t);
                     async_fence();
                     __syncwarp();
                     if (lane == 0) bar_arrive(k_full + 8 * st);
                     ask_keys();
                 }
-                if (t > 0) {
+                if (PASS != QP_SCAN && t > 0) {
                     const int st = (t - 1) & 1;
                     bar_wait(v_empty + 8 * st, (((t - 1) >> 1) & 1) ^ 1u, alive, 12);
                     make_values(t - 1);
@@ -377,8 +372,8 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 }
             }
         } else if (warp == QP_MMA) {
-            const uint32_t iqk = f16_idesc(BF, 128, QP_KEYS), ipv = f16_idesc(!steady, 128, HD);
-            constexpr int nb = steady ? 3 : 2, ns = steady ? 6 : 2;      // buffers of scores, barriers of theirs
+            const uint32_t iqk = f16_idesc(BF, 128, QP_KEYS), ipv = f16_idesc(false, 128, HD);
+            constexpr int nb = 3, ns = 6;      // buffers of scores, barriers of theirs
             auto scores = [&](int t) {
                 const int st = t & 1;
                 bar_wait(k_full + 8 * st, (t >> 1) & 1, alive, 13);
@@ -404,11 +399,19 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
             for (int t = 0; t < min(n, nb); t++) scores(t);
             for (int t = 0; t < n; t++) {
                 const int st = t & 1, b = t % nb;
+                if constexpr (PASS == QP_SCAN) {      // whose scores go where those of t have been read
+                    if (t + nb < n) {
+                        bar_wait(p_full + 8 * (t % 6), (t / 6) & 1, alive, 15);
+                        umma_after_sync();
+                        scores(t + nb);
+                    }
+                    continue;
+                }
                 bar_wait(v_full + 8 * st, (t >> 1) & 1, alive, 14);
                 bar_wait(p_full + 8 * b, (t / nb) & 1, alive, 15);
                 alive = __all_sync(0xffffffffu, alive);
                 umma_after_sync();
-                const uint32_t to = steady ? tmem + 384 : tmem + 256 + st * HD, from = tmem + b * 128;
+                const uint32_t to = tmem + 384, from = tmem + b * 128;
                 if (elect()) {
                     if (alive) {
                         const uint64_t dv = umma_desc(base + Sm::V_AT + st * Sm::V);
@@ -416,7 +419,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                         for (int kk = 0; kk < 8; kk++)
 #pragma unroll
                             for (int u = 0; u < 2; u++)
-                                mma_ts(to, from + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * u, dv + (uint64_t)((kk >> 2) * (HD * 128 >> 4) + 2 * (kk & 3)), ipv, t >= (steady ? 1 : 2) || kk + u > 0);
+                                mma_ts(to, from + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * u, dv + (uint64_t)((kk >> 2) * (HD * 128 >> 4) + 2 * (kk & 3)), ipv, t >= 1 || kk + u > 0);
                     }
                     umma_commit<false>(v_empty + 8 * st);
                     umma_commit<false>(pv_done + 8 * b);
@@ -433,18 +436,23 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
             const int r = tid & 127, grp = warp >> 2, rr = rb * QP_ROWS + r, token = rr / G;
             const bool live = r < rows;
             const int row_hi = live ? (int)max((int64_t)0, at0 + token + 1) : INT32_MAX, row_lo = live && a.window > 0 ? (int)max((int64_t)0, at0 + token + 1 - a.window) : 0;
-            const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), O = lanes + 256 + grp * HD;
-            float* refs = reinterpret_cast<float*>(smem + Sm::STAT_AT);      // steady: after the first tile, after the second, then the two groups' sums
+            const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+            float* refs = reinterpret_cast<float*>(smem + Sm::STAT_AT);      // first: after the first tile, after the second, then the two groups' sums; scan to again: m, e
             float m = -INFINITY, l = 0.0f;
-            float above = 0.0f;
+            float above = 0.0f, heavy = -INFINITY;      // (scan: the largest log2 of a weight)
+            int e = 0;                                  // again: weights are p d 2^e
+            if constexpr (PASS == QP_AGAIN) {
+                m = refs[r];
+                e = (int)refs[128 + r];
+            }
+            const float unit = PASS == QP_AGAIN ? __int_as_float((127 + e) << 23) : 1.0f;
             bool write = true;
             for (int t = grp; t < n; t += 2) {
                 const int p0 = begin + t * QP_KEYS;
                 const uint8_t* meta = smem + Sm::META_AT + (t & 3) * Sm::META;
-                const int b = steady ? t % 3 : grp;
+                const int b = t % 3;
                 const uint32_t S = lanes + b * 128;
-                if (steady) bar_wait(s_full + 8 * (t % 6), (t / 6) & 1, alive, 17);
-                else bar_wait(s_full + 8 * grp, (t >> 1) & 1, alive, 17);
+                bar_wait(s_full + 8 * (t % 6), (t / 6) & 1, alive, 17);
                 __syncwarp();
                 umma_after_sync();
                 const uint4 gone = *reinterpret_cast<const uint4*>(meta + 1024);
@@ -483,46 +491,58 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                     by_32(S, take);
                     return fmaxf(top[0], top[1]);
                 };
-                // the reference goes up by `up` (a whole number, or 0): the sums so far, and the weights of the tile's first `cols` columns, are 2^-up times what they were
-                auto raise = [&](float up, int cols, float2& sum) {
-                    const float f = ex2(-up);
-                    m += up;
-                    l *= f;
-                    sum = mul2(sum, make_float2(f, f));
-                    uint32_t v[16];
-#pragma unroll 1
-                    for (int j = 0; t >= 2 && j < HD; j += 16) {      // (the group's products so far are done: the scores came after them)
-                        tmem_ask16(v, O + j);
-                        tmem_got(v);
+                if constexpr (PASS == QP_SCAN) {
+                    // the largest score so far, and the largest weight, as a power of two and with that score for reference
+                    auto take = [&](int j, const uint32_t (&v)[32]) {
+                        const uint32_t hid = all ? 0u : hidden(j);
+                        const float2 al = make_float2(alpha, alpha);
+                        float2 z[16];
+                        float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                        for (int i = 0; i < 16; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                        tmem_st16(O + j, v);
-                    }
-                    tmem_st_done();
-#pragma unroll 1
-                    for (int j = 0; j < cols; j += 16) {
-                        tmem_ask16(v, S + j);
-                        tmem_got(v);
+                        for (int i = 0; i < 8; i++) {
+                            const float4 k = k4[8 * j + i];
 #pragma unroll
-                        for (int i = 0; i < 16; i++) v[i] = pack_bf2(__uint_as_float(v[i] << 16) * f, __uint_as_float(v[i] & 0xffff0000u) * f);
-                        tmem_st16(S + j, v);
-                    }
-                    tmem_st_done();
-                };
-                if (steady && t == 1) {
+                            for (int u = 0; u < 2; u++) {
+                                float2 y = mul2(make_float2(__uint_as_float(v[4 * i + 2 * u]), __uint_as_float(v[4 * i + 2 * u + 1])), u ? make_float2(k.z, k.w) : make_float2(k.x, k.y));
+                                if ((hid >> (4 * i + 2 * u)) & 1u) y.x = -INFINITY;
+                                if ((hid >> (4 * i + 2 * u + 1)) & 1u) y.y = -INFINITY;
+                                z[2 * i + u] = y;
+                                top[u] = fmaxf(fmaxf(y.x, y.y), top[u]);
+                            }
+                        }
+                        const float was = m;
+                        m = fmaxf(m, fmaxf(top[0], top[1]) * alpha);      // (alpha = 0: 0, or NaN where nothing is seen, which sets nothing)
+                        heavy += below(was, m);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float4 d = k4[32 + 8 * j + i];
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                const float2 w = add2(fma2(z[2 * i + u], al, make_float2(-m, -m)), u ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
+                                heavy = fmaxf(heavy, fmaxf(w.x, w.y));
+                            }
+                        }
+                    };
+                    by_32(S, take);
+                    umma_before_sync();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(p_full + 8 * (t % 6));
+                    continue;
+                }
+                if (PASS == QP_FIRST && t == 1) {
                     asm volatile("bar.sync 2, 256;" ::: "memory");
                     m = refs[r];
-                    if (steady) above = s_above;
-                } else if (steady && t == 2) {
+                    above = s_above;
+                } else if (PASS == QP_FIRST && t == 2) {
                     asm volatile("bar.sync 3, 256;" ::: "memory");
                     m = refs[128 + r];
                 }
-                if (steady ? t < 2 && __any_sync(0xffffffffu, m == -INFINITY) : __any_sync(0xffffffffu, m == -INFINITY)) {
+                if (PASS == QP_FIRST && t < 2 && __any_sync(0xffffffffu, m == -INFINITY)) {
                     // (alpha = 0: 0, or NaN where nothing is seen, which sets nothing)
                     const float top = (all ? largest(std::true_type{}) : largest(std::false_type{})) * alpha;
-                    if (steady && t == 0) {
+                    if (t == 0) {
                         // the largest value scale of the tile, as a power of two: with the reference that much higher (and kUp more) its weights are fp16 numbers of about 2^-kUp
-                        // (of those that are numbers: a row that sees another one makes a second pass necessary anyway)
+                        // (of those that are numbers: a row that sees another one has no other result than NaN)
                         const float4 d = k4[32 + lane];
                         auto size = [](float v) { return (__float_as_uint(v) & 0x7fffffffu) < kInfBits ? fabsf(v) : 0.0f; };
                         const uint32_t big = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(size(d.x), size(d.y)), fmaxf(size(d.z), size(d.w)))));
@@ -531,7 +551,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                     }
                     if (m == -INFINITY) m = fmaxf(m, top + above);
                 }
-                if (steady && t < 2) {      // for the other group's first tile, or this one's next
+                if (PASS == QP_FIRST && t < 2) {      // for the other group's first tile, or this one's next
                     refs[128 * t + r] = m;
                     __threadfence_block();
                     if (t == 0 && n > 1) asm volatile("bar.arrive 2, 256;" ::: "memory");
@@ -541,12 +561,11 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 auto weights = [&](auto whole) {
                     constexpr bool ALL = decltype(whole)::value;
                     const float2 al = make_float2(alpha, alpha);
-                    float ref = m == -INFINITY ? 0.0f : m;
+                    const float ref = m == -INFINITY ? 0.0f : m;
                     float2 sum = make_float2(0.0f, 0.0f);
                     auto take = [&](int j, const uint32_t (&v)[32]) {
                         const uint32_t hid = ALL ? 0u : hidden(j);
                         float2 x[16];
-                        float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             const float4 k = k4[8 * j + i];
@@ -559,16 +578,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                                     if ((hid >> (4 * i + 2 * u + 1)) & 1u) y.y = -INFINITY;
                                 }
                                 x[2 * i + u] = y;
-                                if (!steady) top[u] = fmaxf(fmaxf(y.x, y.y), top[u]);
                             }
-                        }
-                        const float most = fmaxf(top[0], top[1]);
-                        if (!steady && __any_sync(0xffffffffu, most > 16.0f)) {
-                            const float up = most > 16.0f ? ceilf(most) : 0.0f;
-                            raise(up, 32 * j, sum);
-                            ref += up;
-#pragma unroll
-                            for (int i = 0; i < 16; i++) x[i] = add2(x[i], make_float2(-up, -up));
                         }
                         uint32_t o[32];
 #pragma unroll
@@ -578,21 +588,15 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                             for (int u = 0; u < 2; u++) {
                                 const float2 p = make_float2(ex2(x[2 * i + u].x), ex2(x[2 * i + u].y));
                                 float2 w = mul2(p, u ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
+                                if (PASS == QP_AGAIN) w = mul2(w, make_float2(unit, unit));
                                 if (!ALL) {      // (a scale that other rows see may be NaN)
                                     if ((hid >> (4 * i + 2 * u)) & 1u) w.x = 0.0f;
                                     if ((hid >> (4 * i + 2 * u + 1)) & 1u) w.y = 0.0f;
                                 }
                                 sum = add2(sum, p);
-                                if constexpr (steady) {
-                                    o[2 * i + u] = pack_h2(w.x, w.y);
-                                    const float2 f = unpack_h2(o[2 * i + u]);
-                                    o[16 + 2 * i + u] = pack_h2(w.x - f.x, w.y - f.y);
-                                } else {
-                                    const uint32_t b = pack_bf2(w.x, w.y);
-                                    const float2 rest = fma2(make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)), make_float2(-1.0f, -1.0f), w);
-                                    o[2 * i + u] = b;
-                                    o[16 + 2 * i + u] = pack_bf2(rest.x, rest.y);
-                                }
+                                o[2 * i + u] = pack_h2(w.x, w.y);
+                                const float2 f = unpack_h2(o[2 * i + u]);
+                                o[16 + 2 * i + u] = pack_h2(w.x - f.x, w.y - f.y);
                             }
                         }
                         tmem_st32(S + 32 * j, o);      // (over columns that have been read)
@@ -607,77 +611,72 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 __syncwarp();
                 if (lane == 0) bar_arrive(p_full + 8 * b);
             }
-            // ---- each thread has its row's half of the channels
-            float f0 = 1.0f, f1 = 1.0f, sum;
-            if (steady) {
+            if constexpr (PASS == QP_SCAN) {
+                float2* stat = reinterpret_cast<float2*>(refs);
+                stat[grp * 128 + r] = make_float2(m, heavy);
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                const float2 s0 = stat[r], s1 = stat[128 + r];
+                m = fmaxf(s0.x, s1.x);
+                heavy = fmaxf(s0.y + below(s0.x, m), s1.y + below(s1.x, m));
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (grp == 0) {
+                    refs[r] = m;
+                    refs[128 + r] = m > -INFINITY && heavy > -INFINITY ? fminf(fmaxf(14.0f - ceilf(heavy), -126.0f), 126.0f) : 0.0f;
+                }
+            }
+            if constexpr (PASS != QP_SCAN) {
+                // ---- each thread has its row's half of the channels
                 refs[256 + grp * 128 + r] = l;
                 if (n > 0) bar_wait(all_done, 0, alive, 18);
                 __syncwarp();
                 asm volatile("bar.sync 1, 256;" ::: "memory");
-                sum = refs[256 + r] + refs[384 + r];
-            } else {
-                float2* stat = reinterpret_cast<float2*>(refs);
-                stat[grp * 128 + r] = make_float2(m, l);
-                if (n > 0) bar_wait(all_done, 0, alive, 18);
+                const float sum = refs[256 + r] + refs[384 + r];
                 __syncwarp();
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                const float2 s0 = stat[r], s1 = stat[128 + r];
-                const float top = fmaxf(s0.x, s1.x);
-                f0 = ex2(below(s0.x, top));
-                f1 = ex2(below(s1.x, top));
-                sum = s0.y * f0 + s1.y * f1;
-            }
-            __syncwarp();
-            umma_after_sync();
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            T* to = reinterpret_cast<T*>(a.out) + (q.first + token) * a.out_token + (h * G + rr - token * G) * a.out_head + grp * (HD / 2);
-            const bool vec = (reinterpret_cast<uintptr_t>(to) & 15) == 0;
-            auto result = [&](int j, float (&y)[32]) {
+                umma_after_sync();
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                T* to = reinterpret_cast<T*>(a.out) + (q.first + token) * a.out_token + (h * G + rr - token * G) * a.out_head + grp * (HD / 2);
+                const bool vec = (reinterpret_cast<uintptr_t>(to) & 15) == 0;
+                auto result = [&](int j, float (&y)[32]) {
 #pragma unroll
-                for (int i = 0; i < 32; i++) y[i] = 0.0f;
-                if (n > 0) {
-                    uint32_t v[32];
-                    tmem_ld32(v, lanes + (steady ? 384 : 256) + grp * (HD / 2) + 32 * j);
+                    for (int i = 0; i < 32; i++) y[i] = 0.0f;
+                    if (n > 0) {
+                        uint32_t v[32];
+                        tmem_ld32(v, lanes + 384 + grp * (HD / 2) + 32 * j);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) y[i] = __uint_as_float(v[i]) * f0;
-                }
-                if (n > 1 && !steady) {
-                    uint32_t v[32];
-                    tmem_ld32(v, lanes + 256 + HD + grp * (HD / 2) + 32 * j);
+                        for (int i = 0; i < 32; i++) y[i] = __uint_as_float(v[i]);
+                    }
 #pragma unroll
-                    for (int i = 0; i < 32; i++) y[i] = fmaf(__uint_as_float(v[i]), f1, y[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < 32; i++) y[i] = sum == 0.0f ? 0.0f : y[i] * inv;
-            };
-            if (steady) {
-                // what is not finite may be so under a reference that moves; sums of fp16 weights far below one have lost bits
-                float zero = sum * 0.0f, most = 0.0f;
+                    for (int i = 0; i < 32; i++) y[i] = sum == 0.0f ? 0.0f : PASS == QP_AGAIN ? ldexpf(y[i] * inv, -e) : y[i] * inv;
+                };
+                if (PASS == QP_FIRST) {
+                    // what is not finite may be so with another reference; sums of fp16 weights far below one have lost bits
+                    float zero = sum * 0.0f, most = 0.0f;
 #pragma unroll 1
-                for (int j = 0; j < HD / 64; j++) {
+                    for (int j = 0; j < HD / 64; j++) {
+                        float y[32];
+                        result(j, y);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            zero = fmaf(y[i], 0.0f, zero);
+                            most = fmaxf(most, fabsf(y[i]));
+                        }
+                    }
+                    refs[grp * 128 + r] = m == -INFINITY ? -1.0f : most;      // (-1: the row has seen nothing, as far as this group knows)
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    const float size = fmaxf(refs[r], refs[128 + r]);
+                    const bool small = size >= 0.0f && !(size * sum * kOff >= (float)(n * QP_KEYS) * (1.0f / (1 << 22)));
+                    if (__any_sync(0xffffffffu, live && (small || zero != 0.0f)) && lane == 0) atomicOr(&s_bad, 1);
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    if (s_bad) write = false;
+                }
+#pragma unroll 1
+                for (int j = 0; write && j < HD / 64; j++) {
                     float y[32];
                     result(j, y);
-#pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        zero = fmaf(y[i], 0.0f, zero);
-                        most = fmaxf(most, fabsf(y[i]));
+                    if (live) {
+                        if (vec) store_n<T, 32, true>(to + 32 * j, y);
+                        else store_n<T, 32, false>(to + 32 * j, y);
                     }
-                }
-                refs[grp * 128 + r] = m == -INFINITY ? -1.0f : most;      // (-1: the row has seen nothing, as far as this group knows)
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                const float size = fmaxf(refs[r], refs[128 + r]);
-                const bool small = size >= 0.0f && !(size * sum * kOff >= (float)(n * QP_KEYS) * (1.0f / (1 << 22)));
-                if (__any_sync(0xffffffffu, live && (small || zero != 0.0f)) && lane == 0) atomicOr(&s_bad, 1);
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (s_bad) write = false;
-            }
-#pragma unroll 1
-            for (int j = 0; write && j < HD / 64; j++) {
-                float y[32];
-                result(j, y);
-                if (live) {
-                    if (vec) store_n<T, 32, true>(to + 32 * j, y);
-                    else store_n<T, 32, false>(to + 32 * j, y);
                 }
             }
         }
@@ -686,8 +685,8 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
         __syncthreads();
         umma_after_sync();
     };
-    pass(std::true_type{});
-    if (s_bad) apart(pass);      // (uniform: written before the pass's last barrier)
+    pass(std::integral_constant<int, QP_FIRST>{});
+    if (s_bad) once_more(pass);      // (uniform: written before the pass's last barrier)
     if (warp == QP_MMA) tmem_free<false>(tmem, 512);
 }
 

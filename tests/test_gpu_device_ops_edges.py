@@ -77,3 +77,24 @@ def test_attention_of_single_tokens_with_one_large_score(D, dtype, first, high):
     q = (high * hd**-0.5 + 0.01 * normal(6, seqs, nh, hd)).to(dtype)
     want, off = X.attention(q, pages, table, [n] * seqs, list(range(seqs + 1)), page, hd**-0.5)
     within(run_attention(D, q, pages, table, [n] * seqs, list(range(seqs + 1))), want, off, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("far", [1200, 200, 1279])
+def test_attention_of_prompts_whose_references_move(D, dtype, sign, far):  # noqa: F811
+    """One key is e^14 and more ahead of what the first tiles have, further than fp16 goes: its weight, nearly all of the result, has f32's bits.  One channel makes the scores, in numbers that
+    need no rounding."""
+    n, q_len, nh, nkv, hd, page = 1280, 40, 96, 24, 64, 16
+    k, v = torch.zeros(n, nkv, hd), normal(4, n, nkv, hd)
+    k[:, :, 0] = -(32 + torch.randint(0, 32, (n, nkv), generator=torch.Generator().manual_seed(1)).float()) / 64      # (a row's largest value is exact in 4 bits)
+    k[far, :, 0] = 0.375
+    table = torch.randperm(n // page, generator=torch.Generator().manual_seed(5)).int()[None]
+    pages = torch.zeros(n // page, nkv, page * (hd + 8), dtype=torch.uint8)
+    at = torch.arange(n)
+    R.put_rows(pages, page, hd, table[0, at // page].long() * page + at % page, k, v)
+    q = torch.zeros(q_len, nh, hd)
+    q[:, :, 0] = sign * (1024 + torch.randint(0, 128, (q_len, nh), generator=torch.Generator().manual_seed(2)).float()) / 64      # 16 to 18
+    q = q.to(dtype)
+    want, off = X.attention(q, pages, table, [n], [0, q_len], page, sign, again=True, exact_scores=True)
+    within(run_attention(D, q, pages, table, [n], [0, q_len], scale=sign), want, off, dtype)
