@@ -661,10 +661,11 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                             most = fmaxf(most, fabsf(y[i]));
                         }
                     }
-                    refs[grp * 128 + r] = m == -INFINITY ? -1.0f : most;      // (-1: the row has seen nothing, as far as this group knows)
+                    refs[grp * 128 + r] = m == -INFINITY ? -1.0f : most;      // (-1: the row has no reference, as far as this group knows)
                     asm volatile("bar.sync 1, 256;" ::: "memory");
                     const float size = fmaxf(refs[r], refs[128 + r]);
-                    const bool small = size >= 0.0f && !(size * sum * kOff >= (float)(n * QP_KEYS) * (1.0f / (1 << 22)));
+                    // (none at all: its first two tiles lie in pages that are not there, and what follows them, if anything does, went without one)
+                    const bool small = size < 0.0f ? row_hi > begin + 2 * QP_KEYS : !(size * sum * kOff >= (float)(n * QP_KEYS) * (1.0f / (1 << 22)));
                     if (__any_sync(0xffffffffu, live && (small || zero != 0.0f)) && lane == 0) atomicOr(&s_bad, 1);
                     asm volatile("bar.sync 1, 256;" ::: "memory");
                     if (s_bad) write = false;

@@ -98,3 +98,26 @@ def test_attention_of_prompts_whose_references_move(D, dtype, sign, far):  # noq
     q = q.to(dtype)
     want, off = X.attention(q, pages, table, [n], [0, q_len], page, sign, again=True, exact_scores=True)
     within(run_attention(D, q, pages, table, [n], [0, q_len], scale=sign), want, off, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page,gone", [(1024, 1), (256, 1), (16, 17)])
+def test_attention_of_prompts_without_their_first_pages(D, dtype, page, gone):  # noqa: F811
+    """The first tiles have no key that is there: what follows counts as it does for single tokens, with scores far below zero and small values."""
+    n, q_len, nh, nkv, hd = 1500, 40, 96, 24, 64
+    pages, table = cache(5, [n], nkv, hd, page)
+    ks, vs = R.sections(pages, page, hd)[2:]
+    vs.mul_(2.0**-10)
+    kb = R.sections(pages, page, hd)[0]
+    kb[..., 0] = (kb[..., 0] & 0xF0) | 0      # channel 0 of every key is -8 of its scale's, whose sign makes it so
+    ks.copy_(torch.where(torch.isnan(ks), ks, ks.abs()))
+    table[0, :gone] = torch.tensor([-1, pages.shape[0], 2**31 - 1], dtype=torch.int32).repeat(6)[:gone]
+    q = normal(9, q_len, nh, hd)
+    q[:, :, 0] = 24.0      # (scores of some -24 * 8 * 0.3 / 8, give or take)
+    q = q.to(dtype)
+    status = torch.zeros(1, dtype=torch.int32).cuda()
+    want, off = X.attention(q, pages, table, [n], [0, q_len], page, hd**-0.5)
+    within(run_attention(D, q, pages, table, [n], [0, q_len], status=status), want, off, dtype)
+    assert status.item() == D.STATUS_BAD_PAGE
+    # ... and none at all
+    assert (run_attention(D, q, pages, torch.full_like(table, -1), [n], [0, q_len]) == 0).all()
