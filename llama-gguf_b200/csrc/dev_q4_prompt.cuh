@@ -666,7 +666,8 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                     const float size = fmaxf(refs[r], refs[128 + r]);
                     // (none at all: its first two tiles lie in pages that are not there, and what follows them, if anything does, went without one)
                     const bool small = size < 0.0f ? row_hi > begin + 2 * QP_KEYS : !(size * sum * kOff >= (float)(n * QP_KEYS) * (1.0f / (1 << 22)));
-                    if (__any_sync(0xffffffffu, live && (small || zero != 0.0f)) && lane == 0) atomicOr(&s_bad, 1);
+                    // (values from 2^60 on: under their reference probabilities leave f32 below while they count)
+                    if (__any_sync(0xffffffffu, live && (small || zero != 0.0f || above > 60.0f)) && lane == 0) atomicOr(&s_bad, 1);
                     asm volatile("bar.sync 1, 256;" ::: "memory");
                     if (s_bad) write = false;
                 }

@@ -121,3 +121,16 @@ def test_attention_of_prompts_without_their_first_pages(D, dtype, page, gone):  
     assert status.item() == D.STATUS_BAD_PAGE
     # ... and none at all
     assert (run_attention(D, q, pages, torch.full_like(table, -1), [n], [0, q_len]) == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("magnitude", [2.0**-115, 2.0**110, 2.0**120])
+@pytest.mark.parametrize("q_lens,nkv", [([1, 1], 2), ([60, 17], 24)])
+def test_attention_of_values_near_the_ends_of_f32(D, dtype, magnitude, q_lens, nkv):  # noqa: F811
+    lens = [700, 120]
+    pages, table = cache(5, lens, nkv, 64, 16)
+    R.sections(pages, 16, 64)[3].mul_(magnitude)
+    starts = starts_of(q_lens)
+    q = (3.0 * normal(9, starts[-1], 4 * nkv, 64)).to(dtype)
+    want, off = X.attention(q, pages, table, lens, starts, 16, 0.125)
+    within(run_attention(D, q, pages, table, lens, starts), want, off, dtype)
