@@ -151,13 +151,6 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 // distance of rows in elements (torch gives any number where there is one row)
 int64_t ld(const Tensor& t) { return !t.defined() ? 0 : t.size(0) > 1 ? t.stride(0) : t.size(1); }
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
-// A tensor in `all`'s memory from byte `at` on: two results that live about as long share one allocation (0.9 us each).
-Tensor part(const Tensor& all, int64_t at, at::IntArrayRef size, at::ScalarType t) {
-    Tensor r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(t));
-    r.unsafeGetTensorImpl()->set_sizes_contiguous(size);
-    r.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(t));
-    return r;
-}
 PyObject* give(const Tensor& t) {
     if (!t.defined()) Py_RETURN_NONE;
     return THPVariable_Wrap(t);
@@ -188,13 +181,10 @@ PyObject* add_rms_norm_q8(PyObject* const* args, Py_ssize_t n) {
     c.together(x, w, res, sum, q, s);
     int64_t ldq = up16(hidden);
     if (q.defined()) ldq = ld(q);
-    if (!q.defined() && !s.defined()) {
-        const Tensor both = c.empty({rows * (ldq + 4)}, at::kByte);      // (ldq is a multiple of 16)
-        q = part(both, 0, {rows, ldq}, at::kChar);
-        s = part(both, rows * ldq, {rows}, at::kFloat);
+    if (!q.defined()) {
+        q = c.empty({rows, ldq}, at::kChar);
         if (ldq != hidden) q = q.narrow(1, 0, hidden);
     }
-    if (!q.defined()) q = c.empty({rows, ldq}, at::kChar).narrow(1, 0, hidden);
     if (!s.defined()) s = c.empty({rows}, at::kFloat);
     if (res.defined() && !sum.defined()) sum = c.empty({rows, hidden}, x.scalar_type());
     check(E.add_rms_norm_q8(c.device.index(), c.stream(), t, ptr(x), ld(x), ptr(res), ld(res), ptr(sum), ld(sum), w.data_ptr<float>(), (float)eps, (int8_t*)ptr(q), ldq, (float*)ptr(s), rows,
@@ -310,8 +300,7 @@ PyObject* read_q4(PyObject* const* args, Py_ssize_t n) {
     c.vector("slots", slots, slots.numel(), at::kLong);
     c.together(pages, slots);
     const int64_t tokens = slots.numel();
-    const int64_t each = (tokens * p.n_kv_heads * hd * (int64_t)c10::elementSize(dt) + 255) / 256 * 256;
-    const Tensor both = c.empty({2 * each}, at::kByte), k = part(both, 0, {tokens, p.n_kv_heads, hd}, dt), v = part(both, each, {tokens, p.n_kv_heads, hd}, dt);
+    const Tensor k = c.empty({tokens, p.n_kv_heads, hd}, dt), v = c.empty({tokens, p.n_kv_heads, hd}, dt);
     check(E.read_q4(c.device.index(), c.stream(), t, &p, (const int64_t*)ptr(slots), tokens, ptr(k), ptr(v), c.status(4)));
     return give(k, v);
 }

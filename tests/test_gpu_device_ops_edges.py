@@ -134,3 +134,16 @@ def test_attention_of_values_near_the_ends_of_f32(D, dtype, magnitude, q_lens, n
     q = (3.0 * normal(9, starts[-1], 4 * nkv, 64)).to(dtype)
     want, off = X.attention(q, pages, table, lens, starts, 16, 0.125)
     within(run_attention(D, q, pages, table, lens, starts), want, off, dtype)
+
+
+# ---------------------------------------------------------------------------------------------------------------- results
+def test_results_have_memory_of_their_own(D):  # noqa: F811
+    """A result that grows in place does not grow into another one, and one that is kept does not keep the others."""
+    x = normal(1, 3, 256).bfloat16().cuda()
+    pages = D.q4_pages(2, 2, 64, 16)
+    for results in (D.add_rms_norm_q8(x, torch.ones(256).cuda(), 1e-5, residual=x), D.read_q4(pages, torch.arange(5).cuda(), 64, torch.bfloat16)):
+        keep = [r.clone() for r in results]
+        assert len({r.untyped_storage().data_ptr() for r in results}) == len(results)
+        assert all(r.untyped_storage().nbytes() == r.numel() * r.element_size() for r in results)
+        results[0].resize_(4 * results[0].numel()).fill_(77)
+        assert all(torch.equal(a, b) for a, b in zip(results[1:], keep[1:]))
