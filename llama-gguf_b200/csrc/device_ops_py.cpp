@@ -7,6 +7,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -127,10 +128,11 @@ struct Call {
     // all on the first one's device, a CUDA device, and none that a gradient would have to come through
     template <typename... Ts> void together(const Tensor& first, const Ts&... rest) {
         device = first.device();
-        const bool grad = c10::GradMode::is_enabled();
+        const bool grad = c10::GradMode::is_enabled(), tangent = c10::AutogradState::get_tls_state().get_fw_grad_mode();
         auto one = [&](const Tensor& t) {
             if (!t.defined()) return;
             if (grad && t.requires_grad()) refuse(B200_ERR_UNSUPPORTED, op, "an argument requires a gradient, and results carry none (detach it)");
+            if (tangent && t._fw_grad(0).defined()) refuse(B200_ERR_UNSUPPORTED, op, "an argument has a forward-mode tangent, and results carry none");
             if (t.device() != device) refuse(B200_ERR_INVALID_ARGUMENT, op, "an argument is on " + t.device().str() + ", expected " + device.str());
         };
         one(first);
