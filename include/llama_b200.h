@@ -637,7 +637,7 @@ B200_API int b200_dev_read_q4(int device, void* stream, uint32_t type, const b20
  * position p in page page_table[s * table_stride + p / page_size], and the query tokens q_starts[s] .. q_starts[s + 1] - 1 (NULL: token s), which are its last
  * positions: token i of m sits at kv_lens[s] - m + i and sees the positions up to its own (window > 0: the last `window` of them).  A token that sees nothing gets zeros;
  * tokens ahead of q_starts[0] or from q_starts[seqs] on are left as they were.  Pages outside the cache count as not seen, BAD_PAGE; lengths beyond table_pages * page_size
- * are cut there, and negative ones taken as zero, BAD_LENGTH; q_starts that do not ascend within 0 .. tokens: BAD_LENGTH, the sequence is left out.  max_q: the most query tokens
+ * are cut there, and negative ones taken as zero, BAD_LENGTH; q_starts that do not ascend within 0 .. tokens: BAD_LENGTH, the sequence is left out.  scale is finite.  max_q: the most query tokens
  * of a sequence, as far as the host knows (0: not known); it only chooses between kernels.  Rows of out do
  * not overlap (as q_out's).  workspace: b200_dev_attention_paged_q4_workspace bytes on 256 bytes. */
 typedef struct b200_q4_attention {

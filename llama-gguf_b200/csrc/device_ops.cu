@@ -3,6 +3,7 @@
 #include "device_ops.h"
 
 #include <algorithm>
+#include <cmath>
 #include <exception>
 #include <string>
 
@@ -190,6 +191,7 @@ static int check_attention(const char* op, const b200_q4_attention* a) {
     if (a->tokens * a->n_heads >= kMost || a->tokens >= kMost || (int64_t)a->table_pages * a->cache.page_size > kMostTiled) return shape(op, "too many rows or positions for one call");
     if (!a->q_starts && a->tokens != a->seqs) return shape(op, "without q_starts every sequence has one token");
     if (a->window < 0) return bad(op, "window must not be negative");
+    if (!std::isfinite(a->scale)) return bad(op, "scale is not finite");
     return B200_OK;
 }
 

@@ -325,7 +325,7 @@ PyObject* attention_paged_q4(PyObject* const* args, Py_ssize_t n) {
     if (starts.defined()) c.vector("q_starts", starts, seqs + 1, at::kInt);
     if (out.defined()) c.heads("out", out, tokens, nh, hd, dt);
     const double scale = args[4] == Py_None ? 1.0 / std::sqrt((double)hd) : c.number(4);
-    if (!std::isfinite(scale)) refuse(B200_ERR_INVALID_ARGUMENT, c.op, "scale is not finite");
+    if (!std::isfinite((float)scale)) refuse(B200_ERR_INVALID_ARGUMENT, c.op, "scale is not finite");
     const int64_t max_q = c.integer(6), window = c.integer(7);
     if (seqs >= INT32_MAX || width >= INT32_MAX || nh > 65536) refuse(B200_ERR_SHAPE_MISMATCH, c.op, "too many sequences, pages or heads");
     if (max_q < 0 || max_q > INT32_MAX || window < 0 || window > INT32_MAX) refuse(B200_ERR_INVALID_ARGUMENT, c.op, "max_q and window must be from 0 to 2^31 - 1");

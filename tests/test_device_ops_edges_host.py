@@ -1,6 +1,11 @@
 """Calls that the operators on device tensors refuse where a result would be wrong without a word, without a GPU."""
+import ctypes as C
+import math
+
 import pytest
 import torch
+
+from test_device_ops_host import AT, pages, refused
 
 
 @pytest.fixture(scope="module")
@@ -22,3 +27,13 @@ def test_forward_tangents_are_refused(b200, D):
                 D.add_rms_norm_q8(*args, 1e-5)
         with pytest.raises(b200.InvalidArgument, match="CUDA"):
             D.add_rms_norm_q8(fw.unpack_dual(dual).primal, w, 1e-5)
+
+
+def test_scales_that_are_no_f32_numbers_are_refused(b200, D):
+    """The scale is f32: what is a number in 64 bits may be infinite there, and results NaN."""
+    for scale in (math.inf, -math.inf, math.nan, 1e300):
+        a = D.Q4Attention(device=0, type=0, q=AT, out=AT, q_token=256, q_head=64, out_token=256, out_head=64, kv_lens=AT, page_table=AT, table_stride=4, tokens=3, table_pages=4, seqs=3,
+                          n_heads=4, scale=scale, cache=pages(D))
+        refused(b200, D._lib().b200_dev_attention_paged_q4(C.byref(a)), b200.InvalidArgument, "scale")
+        with pytest.raises(b200.InvalidArgument, match="scale"):
+            D.attention_paged_q4(torch.zeros(3, 4, 64), D.q4_pages(4, 2, 64, 16, device="cpu"), torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), scale)
