@@ -514,6 +514,8 @@ B200_API int b200_debug_err(b200_ctx* ctx, int* out8);
 B200_API int b200_debug_plan_split(int n_rows, int K, int T, int n_sm, int persistent, int* k_split_out);
 /* Host logic of the fp16 products' plan (no device needed): out4 = persistent, tokens per tile, cuts of K, pairs of CTAs. */
 B200_API int b200_debug_tc_plan(int rows, int n, int k, int glu, int may_cut, int pairs, int* out4);
+/* Host logic of b200_dev_mat_mat_i8's plan (no device needed): out4 = tokens per tile, CTAs that share a tile's K, kernel of many tokens, pairs of CTAs. */
+B200_API int b200_debug_i8_plan(int64_t t, int64_t k, int64_t n, int* out4);
 /* The RMS norm of a prompt's rows to fp16 [rows][n] (tests): the kernel that rows of n elements take, or the one for any length. */
 B200_API int b200_debug_prompt_norm(const float* x, const float* w, float eps, int rows, int n, int any_length, uint16_t* out);
 /* Lab: take the first `pos` positions of the slot's KV cache as valid as they are (attention at depth without a prompt). */
@@ -658,6 +660,8 @@ typedef struct b200_q4_attention {
 } b200_q4_attention;
 B200_API int b200_dev_attention_paged_q4_workspace(const b200_q4_attention* a, size_t* bytes);
 B200_API int b200_dev_attention_paged_q4(const b200_q4_attention* a);
+/* Host logic of the above (no device needed): the blocks of the kernel of many query tokens (0: the call does not take it). */
+B200_API int b200_debug_q4_prompt_blocks(const b200_q4_attention* a, int64_t* blocks);
 
 #ifdef __cplusplus
 }

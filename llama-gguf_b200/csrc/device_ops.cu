@@ -133,6 +133,19 @@ extern "C" int b200_dev_mat_mat_i8(int device, void* stream, uint32_t out_type, 
     });
 }
 
+extern "C" int b200_debug_i8_plan(int64_t t, int64_t k, int64_t n, int* out4) {
+    const char* op = "b200_debug_i8_plan";
+    return entry(op, [&]() -> int {
+        if (!out4 || t < 1 || t > kMostTiled || n < 1 || n > kMostTiled || k < 1 || k > 131071) return bad(op, "bad argument");
+        const GemmI8Plan p = gemm_i8_plan(t, k, n);
+        out4[0] = p.tn;
+        out4[1] = p.splits;
+        out4[2] = p.wide;
+        out4[3] = p.pair;
+        return B200_OK;
+    });
+}
+
 extern "C" int b200_dev_rope_append_q4(const b200_q4_append* a) {
     const char* op = "rope_append_q4";
     return entry(op, [&]() -> int {
@@ -202,6 +215,17 @@ extern "C" int b200_dev_attention_paged_q4_workspace(const b200_q4_attention* a,
         if (rc) return rc;
         if (!bytes) return bad(op, "null pointer");
         *bytes = attention_q4_workspace(*a);
+        return B200_OK;
+    });
+}
+
+extern "C" int b200_debug_q4_prompt_blocks(const b200_q4_attention* a, int64_t* blocks) {
+    const char* op = "b200_debug_q4_prompt_blocks";
+    return entry(op, [&]() -> int {
+        int rc = check_attention(op, a);
+        if (rc) return rc;
+        if (!blocks) return bad(op, "null pointer");
+        *blocks = attention_q4_has_prompts(*a) ? attention_q4_prompt_blocks(*a) * a->cache.n_kv_heads : 0;
         return B200_OK;
     });
 }

@@ -62,6 +62,8 @@ def _lib():
         L.b200_dev_read_q4.argtypes = [C.c_int, vp, C.c_uint32, C.POINTER(Q4Pages), vp, i64, vp, vp, vp]
         L.b200_dev_attention_paged_q4_workspace.argtypes = [C.POINTER(Q4Attention), sp]
         L.b200_dev_attention_paged_q4.argtypes = [C.POINTER(Q4Attention)]
+        L.b200_debug_i8_plan.argtypes = [i64, i64, i64, C.POINTER(C.c_int)]
+        L.b200_debug_q4_prompt_blocks.argtypes = [C.POINTER(Q4Attention), C.POINTER(i64)]
         _library = L
     return _library
 
@@ -89,6 +91,13 @@ def watchdog(device=0):
     v = C.c_int(0)
     _check(_lib().b200_dev_watchdog(int(device), C.byref(v)))
     return v.value
+
+
+def i8_plan(t, k, n):
+    """(tokens per tile, CTAs that share a tile's K, kernel of many tokens, pairs of CTAs) of mat_mat_i8: host logic, no device needed."""
+    v = (C.c_int * 4)()
+    _check(_lib().b200_debug_i8_plan(int(t), int(k), int(n), v))
+    return tuple(v)
 
 
 def padded_rows(rows, cols, device, dtype=torch.int8):

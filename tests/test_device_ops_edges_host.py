@@ -37,3 +37,16 @@ def test_scales_that_are_no_f32_numbers_are_refused(b200, D):
         refused(b200, D._lib().b200_dev_attention_paged_q4(C.byref(a)), b200.InvalidArgument, "scale")
         with pytest.raises(b200.InvalidArgument, match="scale"):
             D.attention_paged_q4(torch.zeros(3, 4, 64), D.q4_pages(4, 2, 64, 16, device="cpu"), torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), scale)
+
+
+def test_every_plan_of_products_is_tested(D):
+    """The plans that calls of all sizes have are those of the tests' list."""
+    import random
+
+    from test_gpu_device_ops_edges import PLANS
+
+    assert all(D.i8_plan(t, k, n) == plan for plan, t, k, n in PLANS)
+    rng, seen = random.Random(1), set()
+    for _ in range(20000):
+        seen.add(D.i8_plan(*(int(2 ** rng.uniform(0, m)) for m in (13, 14, 15))))
+    assert seen <= {p[0] for p in PLANS}

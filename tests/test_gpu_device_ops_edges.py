@@ -1,10 +1,13 @@
 """Operators on device tensors where magnitudes, masks and sizes are far from ordinary, against plain forms in 64 bits."""
+import ctypes as C
+
 import pytest
 import torch
 
 import device_ops_exact as X
 import device_ops_ref as R
-from test_gpu_device_ops import TYPES, D, cache, check_norm, normal  # noqa: F401
+import test_gpu_device_ops as T
+from test_gpu_device_ops import TYPES, D, bytes_of, cache, check_norm, check_product, layer, layer_state, normal  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -22,6 +25,27 @@ def test_norm_of_rows_of_any_magnitude(D, dtype, magnitude, rows, hidden):  # no
     odd = torch.empty(rows, hidden + 1, dtype=dtype, device="cuda")[:, 1:]
     odd.copy_(x)
     assert all(torch.equal(a, b) for a, b in zip(D.add_rms_norm_q8(x, w, eps)[:2], D.add_rms_norm_q8(odd, w, eps)[:2]))
+
+
+# ---------------------------------------------------------------------------------------------------------------- product
+# every plan that a call can have, at sizes that end inside a tile in t, k and n: (tokens per tile, CTAs of a cluster that share K, kernel of many tokens, pairs of CTAs).  The kernels of many tokens: with an odd and an even
+# number of tiles of weights (pairs: the last one has one row of tiles), once around and with more than two tiles for each CTA, so that both accumulators come again
+PLANS = [((16, 1, 0, 0), 2, 300, 38404), ((16, 2, 0, 0), 3, 643, 4504), ((16, 4, 0, 0), 8, 1063, 2251), ((16, 8, 0, 0), 13, 1905, 130), ((32, 1, 0, 0), 18, 333, 77), ((32, 2, 0, 0), 17, 907, 4713),
+         ((32, 4, 0, 0), 19, 700, 130), ((32, 8, 0, 0), 20, 2047, 300), ((64, 1, 0, 0), 65, 200, 333), ((64, 2, 0, 0), 2249, 1461, 1), ((64, 4, 0, 0), 66, 659, 300), ((64, 8, 0, 0), 65, 1919, 131),
+         ((128, 1, 0, 0), 4752, 1, 135), ((128, 2, 0, 0), 4749, 4258, 1), ((128, 4, 0, 0), 2335, 2855, 1), ((128, 8, 0, 0), 911, 5655, 1), ((128, 1, 1, 0), 130, 4, 9496), ((128, 1, 1, 0), 130, 131, 9899),
+         ((128, 1, 1, 0), 129, 4, 18967), ((128, 1, 1, 0), 130, 2, 19699), ((256, 1, 1, 0), 291, 1476, 6573), ((256, 1, 1, 0), 299, 1463, 6447), ((256, 1, 1, 0), 1312, 388, 8919), ((256, 1, 1, 0), 796, 392, 13688),
+         ((256, 1, 1, 1), 5141, 2781, 387), ((256, 1, 1, 1), 6694, 2865, 263), ((256, 1, 1, 1), 269, 1110, 25328), ((256, 1, 1, 1), 313, 897, 25608)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("plan,t,k,n", PLANS)
+def test_product_of_every_plan(D, dtype, plan, t, k, n):  # noqa: F811
+    assert D.i8_plan(t, k, n) == plan
+    a, w = bytes_of(t, t, k, 16), bytes_of(n, n, k)
+    check_product(D, a, w, dtype, bias=t % 2 == 0)
+    buf = torch.full((t, n + 9), 5.0, dtype=dtype, device="cuda")
+    check_product(D, a, w, dtype, bias=t % 2 == 1, out=buf[:, 4 : n + 4])
+    assert (buf[:, :4] == 5).all() and (buf[:, n + 4 :] == 5).all()
 
 
 # -------------------------------------------------------------------------------------------------------------- attention
@@ -147,3 +171,53 @@ def test_results_have_memory_of_their_own(D):  # noqa: F811
         assert all(r.untyped_storage().nbytes() == r.numel() * r.element_size() for r in results)
         results[0].resize_(4 * results[0].numel()).fill_(77)
         assert all(torch.equal(a, b) for a, b in zip(results[1:], keep[1:]))
+
+
+# ---------------------------------------------------------------------------------------------------------------- together
+PROMPTS = ([300, 1, 9], [64, 640, 5])      # (a layer whose attention takes both kernels: one sequence has many rows)
+
+
+def takes_prompts(D, q_lens, nh, nkv, hd):  # noqa: F811
+    a = D.Q4Attention(type=0, q_starts=1, kv_lens=1, page_table=1, table_stride=9, tokens=sum(q_lens), table_pages=9, seqs=len(q_lens), n_heads=nh, scale=1.0,
+                      cache=D.Q4Pages(data=16, n_pages=4, page_size=16, n_kv_heads=nkv, head_dim=hd))
+    blocks = C.c_int64(-1)
+    assert D._lib().b200_debug_q4_prompt_blocks(C.byref(a), C.byref(blocks)) == 0
+    return blocks.value > 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_layer_with_a_prompt(D, dtype):  # noqa: F811
+    assert takes_prompts(D, PROMPTS[0], 8, 2, 64) and not takes_prompts(D, [30, 1, 9], 8, 2, 64)
+    T.test_a_layer(D, dtype, *PROMPTS)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_layer_with_a_prompt_captured_replayed_and_at_once(D, dtype):  # noqa: F811
+    """Graphs of a batch with a prompt and of a step, replayed in turn on two streams, then both eagerly at once: the same bits as one after the other."""
+    states = [layer_state(D, dtype, *PROMPTS), layer_state(D, dtype, [1, 1, 1], [0, 300, 37])]
+    want = [[v.clone() for v in layer(D, s)] for s in states]
+    for s, w in zip(states, want):
+        assert all(torch.equal(a, b) for a, b in zip(layer(D, s), w))
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in states:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(layer(D, s))
+        graphs.append(g)
+    for _ in range(5):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    got = [list(outs)]
+    for _ in range(5):
+        now = []
+        for s, st in zip(states, streams):
+            with torch.cuda.stream(st):
+                now.append(layer(D, s))
+        got.append(now)
+    torch.cuda.synchronize()
+    for run in got:
+        for r, w in zip(run, want):
+            assert all(torch.equal(a, b) for a, b in zip(r, w))
