@@ -133,6 +133,7 @@ struct Call {
             if (!t.defined()) return;
             if (grad && t.requires_grad()) refuse(B200_ERR_UNSUPPORTED, op, "an argument requires a gradient, and results carry none (detach it)");
             if (tangent && t._fw_grad(0).defined()) refuse(B200_ERR_UNSUPPORTED, op, "an argument has a forward-mode tangent, and results carry none");
+            if (t.is_neg()) refuse(B200_ERR_UNSUPPORTED, op, "an argument is a view that stands for its memory's negative (resolve_neg it)");
             if (t.device() != device) refuse(B200_ERR_INVALID_ARGUMENT, op, "an argument is on " + t.device().str() + ", expected " + device.str());
         };
         one(first);

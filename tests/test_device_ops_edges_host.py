@@ -39,6 +39,17 @@ def test_scales_that_are_no_f32_numbers_are_refused(b200, D):
             D.attention_paged_q4(torch.zeros(3, 4, 64), D.q4_pages(4, 2, 64, 16, device="cpu"), torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), scale)
 
 
+def test_views_of_the_negative_are_refused(b200, D):
+    """A view whose negative bit is set (imag of a conjugate, taken on) has the other sign in memory."""
+    x = torch.randn(4, 64)
+    view = torch._neg_view(x)
+    assert view.is_neg() and torch.equal(view, -x)
+    with pytest.raises(b200.Unsupported, match="negative"):
+        D.add_rms_norm_q8(view, torch.ones(64), 1e-5)
+    with pytest.raises(b200.InvalidArgument, match="CUDA"):
+        D.add_rms_norm_q8(view.resolve_neg(), torch.ones(64), 1e-5)
+
+
 def test_every_plan_of_products_is_tested(D):
     """The plans that calls of all sizes have are those of the tests' list."""
     import random
