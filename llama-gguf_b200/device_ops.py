@@ -74,7 +74,7 @@ def _ops():
     if _calls is None:
         path = os.path.join(_HERE, "_device_ops.so")
         if not os.path.exists(path):
-            raise NotAvailable(f"{path} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+            raise NotAvailable(f"{path} is missing (it needs torch's headers): build it with `python -c 'import __graft_entry__ as g; g.build()'`")
         L = _lib()
         spec = importlib.util.spec_from_file_location("_device_ops", path)
         mod = importlib.util.module_from_spec(spec)

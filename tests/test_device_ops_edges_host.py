@@ -1,6 +1,9 @@
 """Calls that the operators on device tensors refuse where a result would be wrong without a word, without a GPU."""
 import ctypes as C
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -61,3 +64,24 @@ def test_every_plan_of_products_is_tested(D):
     for _ in range(20000):
         seen.add(D.i8_plan(*(int(2 ** rng.uniform(0, m)) for m in (13, 14, 15))))
     assert seen <= {p[0] for p in PLANS}
+
+
+def test_the_library_builds_without_torch_and_the_calls_again_for_another_one(tmp_path):
+    csrc = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "llama-gguf_b200", "csrc")
+
+    def steps(*args):
+        return subprocess.run(["make", "-n", "-C", csrc, "OBJDIR=" + str(tmp_path), *args], capture_output=True, text=True, check=True).stdout
+
+    without = steps(f"PYTHON={sys.executable} -S")      # (no site-packages)
+    assert "device_ops.cu" in without and "device_ops_py.cpp" not in without and "not built" in without
+    built = os.path.join(csrc, "..", "_device_ops.so")
+    known = tmp_path / "torch.txt"
+    assert not known.exists()
+    if "device_ops_py.cpp" not in steps(f"PYTHON={sys.executable}"):
+        pytest.skip("torch without headers")
+    assert torch.__version__ in known.read_text()
+    if os.path.exists(built):
+        os.utime(known, (0, 0))
+        assert "device_ops_py.cpp" not in steps(f"PYTHON={sys.executable}")
+        known.write_text("another one")
+        assert "device_ops_py.cpp" in steps(f"PYTHON={sys.executable}")
