@@ -700,14 +700,17 @@ inline int64_t attention_q4_prompt_blocks(const b200_q4_attention& a) {
     const int64_t rows = a.tokens * (a.n_heads / a.cache.n_kv_heads);
     return rows / QP_ROWS + std::min<int64_t>(a.seqs, rows / (kPromptRows + 1));
 }
-// Whether a call's long sequences go there, by what the host knows.  A block of 128 rows takes 1.7 us for 128 keys, whether alone or on every SM, and 8 more; the other kernel 0.84 us of an SM for eight rows, but
-// spreads any number of rows over all SMs, and 16 more.  So its (rows / 8) * 0.84 / 148 against 1.7 for every 148 blocks, less what they differ by at 4000 keys.  Measured (bf16, 32 heads over 8, hd 128; us there, here,
-// and what the rule compares with 260): 4000 keys, one sequence of 128 rows of a kv head 39, 62 (128), of 256 62, 63 (256), of 384 85, 63 (384); eight of 32 58, 60 (256), of 48 78, 65 (384); 64 sequences of 36 with
-// 1000 keys 124, 91 (461); one of 256 with 500 keys 33, 25 (256).
+// Whether a call's long sequences go there, by what the host knows.  A block of 128 rows takes 1.8 us for 128 keys (f32 2.1), whether alone or on every SM, and some 12 more; the other kernel spreads any number of rows
+// over all SMs, a unit of eight of them some 0.04 us and 0.03 for 1000 keys.  So the units are compared with what a wave of 148 blocks is worth, 170 units where keys are few and up to 310 where they are many.  Of the keys
+// the host knows the page table's width, or the window.  (Wider tables than a call needs: 310 for 190, rows that would take 31 us there take up to 40.)  Measured (32 heads over 8, hd 128, bf16, one sequence; units of the call:
+// us there, here): 256 keys 128: 26, 28, 192: 30, 28; 500 keys 128: 30, 30, 256: 36, 32; 1000 keys 128: 32, 38, 192: 40, 38, 256: 44, 38; 2000 keys 192: 46, 52, 256: 54, 52; 4000 keys 256: 71, 83, 384: 93, 81;
+// 16 000 keys 256: 167, 253, 384: 239, 249, 512: 304, 243.  Eight sequences with 1000 keys 288: 44, 38, with 4000 288: 77, 83, 384: 93, 83.  f32: 500 keys 192: 38, 38; 1000 keys 256: 46, 46; 4000 keys 256: 77, 93,
+// 384: 104, 91.  32 heads over 4, hd 64: 1000 keys 128: 32, 34, 192: 38, 32; 4000 keys 256: 61, 67, 384: 81, 67.
 inline bool attention_q4_has_prompts(const b200_q4_attention& a) {
     const int64_t G = a.n_heads / a.cache.n_kv_heads, nkv = a.cache.n_kv_heads;
     if (!a.q_starts || (a.max_q ? a.max_q : a.tokens) * G <= kPromptRows) return false;
-    return (a.tokens * G + 7) / 8 * nkv > 260 * ((attention_q4_prompt_blocks(a) * nkv + 147) / 148);
+    const int64_t width = (int64_t)a.table_pages * a.cache.page_size, keys = a.window > 0 ? std::min<int64_t>(width, (int64_t)a.window + QP_ROWS) : width;
+    return (a.tokens * G + 7) / 8 * nkv > std::min<int64_t>(310, 170 + keys * 35 / 1000) * ((attention_q4_prompt_blocks(a) * nkv + 147) / 148);
 }
 template <typename T, int HD> cudaError_t attention_q4_prompt(const b200_q4_attention& a, cudaStream_t st) {
     using Sm = Q4PromptSmem<T, HD>;

@@ -85,3 +85,20 @@ def test_the_library_builds_without_torch_and_the_calls_again_for_another_one(tm
         assert "device_ops_py.cpp" not in steps(f"PYTHON={sys.executable}")
         known.write_text("another one")
         assert "device_ops_py.cpp" in steps(f"PYTHON={sys.executable}")
+
+
+def test_which_kernel_attention_takes(D):
+    """By the rows of a call, the keys that its table or its window has room for, and what the host says of the longest sequence."""
+    def blocks(tokens, seqs=1, keys=4096, nh=32, nkv=8, max_q=0, window=0, starts=1):
+        a = D.Q4Attention(type=0, q_starts=starts, kv_lens=1, page_table=1, table_stride=keys // 16, tokens=tokens, table_pages=keys // 16, seqs=seqs, n_heads=nh, scale=1.0, max_q=max_q, window=window,
+                          cache=D.Q4Pages(data=16, n_pages=4, page_size=16, n_kv_heads=nkv, head_dim=64))
+        n = C.c_int64(-1)
+        assert D._lib().b200_debug_q4_prompt_blocks(C.byref(a), C.byref(n)) == 0
+        return n.value
+
+    assert blocks(2048) == (2048 * 4 // 128 + 1) * 8
+    assert not blocks(64) and blocks(96)
+    assert not blocks(48, keys=2048) and blocks(48, keys=512)
+    assert blocks(48, keys=65536, window=100) and not blocks(48, keys=65536)
+    assert not blocks(2048, max_q=8) and not blocks(512, seqs=512, starts=None)
+    assert not blocks(8)
