@@ -9,7 +9,7 @@
 //               products; the two are joined at the end.  P goes back to tensor memory in place of S.
 // Keys' scales multiply the scores, values' scales the weights.  f32 queries are pairs of fp16 numbers scaled by a power of two.  Passes:
 //   first   The reference of a row's exponentials need only be near: it is the largest score of the first tile that the row sees, and stays.  So no tile waits for another: one O, three buffers of scores,
-//           each score read once.  A weight p_j d_j is two fp16 numbers (what the first leaves over is the second: 2^-22), 2^4 or so
+//           each score read once.  A weight p_j d_j is two fp16 numbers (what the first leaves over is the second: 2^-22), 2^3 or 2^4
 //           where the reference was set.
 //   scan, again   Where a row passes fp16's range, or the last bits of its weights may have cost too much of its result (Q4Weights), or its result is not finite, the block goes over the keys twice more: once for
 //           the scores alone, which gives each row its largest score m and its largest weight, and once as above with these for references: probabilities 2^(z_j - m), weights p_j d_j 2^e of up to 2^14 in pairs of fp16
@@ -27,14 +27,13 @@ namespace dev {
 
 enum { QP_ROWS = 128, QP_KEYS = 128, QP_SOFT = 8, QP_MAKE = 8, QP_MMA = 16, QP_THREADS = 544 };
 
-// The weights' place: 2^4 at the reference, so that 2^-29 of it is their last bit, and scores have room for 2^12 above it (8.3 in natural logarithms; of Gaussian scores of standard deviation 2 a few in 1e8 pass
-// 2^10, which cost 2048 tokens behind 2048 a third of their time).
-constexpr float kUp = -4.0f;
-// by the result's type: the part of a row's largest channel that its weights' last bits, 2^-25 of each times a value of up to 8, may have cost at most, had they all one sign: half a step of bf16 and of f16
-// results, 2^-16 of f32 ones
-template <typename T> struct Q4Weights { static constexpr float kOff = 1.0f / (1 << 8); };
-template <> struct Q4Weights<__half> { static constexpr float kOff = 1.0f / (1 << 11); };
-template <> struct Q4Weights<float> { static constexpr float kOff = 1.0f / (1 << 16); };
+// By the result's type: the weights' place, 2^-kUp at the reference, so that scores have room for 2^(16 + kUp) above it (9 and 8.3 in natural logarithms), and the part of a row's largest channel that its weights' last
+// bits, 2^-25 of each times a value of up to 8, may have cost at most, had they all one sign: half a step of bf16 and of f16 results, 2^-16 of f32 ones.
+// (2^6 for Gaussian scores of standard deviation 2: some rows of 2048 tokens behind 2048 pass 2^10, and the call takes a third longer; 2^4: now and then a call has such a row; 1: a first position that draws most of the
+// weight and has a twentieth of the others' values costs too many bits there already.)
+template <typename T> struct Q4Weights { static constexpr float kUp = -3.0f, kOff = 1.0f / (1 << 8); };
+template <> struct Q4Weights<__half> { static constexpr float kUp = -3.0f, kOff = 1.0f / (1 << 11); };
+template <> struct Q4Weights<float> { static constexpr float kUp = -4.0f, kOff = 1.0f / (1 << 16); };
 
 template <typename T, int HD> struct Q4PromptSmem {
     static constexpr int NQ = sizeof(T) == 4 ? 2 : 1;
@@ -115,7 +114,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
     using Sm = Q4PromptSmem<T, HD>;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
     constexpr int NQ = Sm::NQ, SLABS = HD / 64;
-    constexpr float kOff = Q4Weights<T>::kOff;
+    constexpr float kUp = Q4Weights<T>::kUp, kOff = Q4Weights<T>::kOff;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_item[2], s_bad;

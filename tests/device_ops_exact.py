@@ -15,7 +15,7 @@ def attention(q, pages, table, lens, starts, page, scale, window=0, again=False,
     The weights of values alone: 2^-22 from their two fp16 halves, 2^-24 from the product with d, the value's scale, or with 2^(log2 p + log2 d) in its place 2^-24 times these logarithms and the 16 of the
     reference's place.  A sum of products: 2^-22 of what is there, in each step of 16 keys from a key's own to the last, and 4 for what joins parts; the reciprocal and the end 2^-21 of the result.
     The halves end at 2^-25.  A reference that moves keeps the largest weight p d of a row (a value is at most 8 d) at 2^7 or above: L * 2^-32 * max(p max |v|).  A row of a sequence with more than 32 rows of
-    a kv head may have one that stays: a weight of 2^4 stands for the largest scale of a value in the first tile: L * 2^-29 * max |v| of the sequence, or what makes the block go over the keys again,
+    a kv head may have one that stays: a weight of 2^3 (f32: 2^4) stands for the largest scale of a value in the first tile: L * 2^-28 (2^-29) * max |v| of the sequence, or what makes the block go over the keys again,
     2^-8, 2^-11 or 2^-16 (bf16, f16, f32) of the row's largest channel.  again: the inputs make it."""
     dev = torch.device(DEVICE)
     tokens, nh, hd = q.shape
@@ -56,7 +56,7 @@ def attention(q, pages, table, lens, starts, page, scale, window=0, again=False,
             own = p * (2.0**-22 + 2.0**-24 * (1 + 16 + power - p.clamp(min=2.0**-300).log2()) + steps * 2.0**-22)
             low = keys * 2.0**-32 * (p * v.abs().amax(1)).amax(-1)
             if many and not again:
-                low = torch.maximum(low, torch.minimum(keys * 2.0**-29 * v.abs().max(), 1.01 * R.COST[dtype] * r.abs().amax(-1)))
+                low = torch.maximum(low, torch.minimum(keys * (2.0**-29 if dtype == torch.float32 else 2.0**-28) * v.abs().max(), 1.01 * R.COST[dtype] * r.abs().amax(-1)))
             off[a:b, h * g : (h + 1) * g] = spread * (dz + 2.0**-20)[..., None] + own @ v.abs() + 2.0**-21 * r.abs() + low[..., None]
     return o, off
 
