@@ -173,7 +173,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
     const int begin = lo_min & ~15, n = (hi - begin + QP_KEYS - 1) / QP_KEYS;      // tiles (0: nothing is seen)
     if (warp == QP_MMA) tmem_alloc<false>(&s_tmem, 512);
 
-    // ---- queries: thread = row, half the channels each of two; pairs of fp16 for f32, scaled so that the row's elements are below 2^14
+    // ---- queries: thread = row, half the channels each of two; pairs of fp16 for f32; scaled so that the row's elements are below 2^14 (bf16 too: sums of products with 8 stay in f32)
     float alpha = 0.0f;      // what a row's scores are multiplied with (its sign is in the queries)
     if (warp < QP_SOFT) {
         const int r = tid & 127, half = tid >> 7;
@@ -181,34 +181,32 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
         const int rr = rb * QP_ROWS + (live ? r : 0), token = rr / G;
         const T* p = reinterpret_cast<const T*>(a.q) + (q.first + token) * a.q_token + (h * G + rr - token * G) * a.q_head;
         const bool vec = (reinterpret_cast<uintptr_t>(p) & 15) == 0;
-        float f1 = 1.0f, f2 = 1.0f;
-        int e = 0;
-        if (!BF) {
-            float top = 0.0f;
-#pragma unroll 4
-            for (int i = 0; i < HD; i += 8) {
-                float x[8];
-                if (vec) load_n<T, 8, true>(p + i, x);
-                else load_n<T, 8, false>(p + i, x);
+        float* tops = reinterpret_cast<float*>(smem + Sm::STAT_AT);
+        __align__(16) T x[HD / 2];
+        if (vec) {
 #pragma unroll
-                for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(x[k]));
-            }
-            e = top < INFINITY ? 140 - (int)(__float_as_uint(top) >> 23) : 0;
-            f1 = __int_as_float((127 + e / 2) << 23);
-            f2 = __int_as_float((127 + e - e / 2) << 23);
+            for (int i = 0; i < HD / 32 * (int)sizeof(T); i++) reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(p + half * (HD / 2))[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < HD / 2; i++) x[i] = p[half * (HD / 2) + i];
         }
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < HD / 2; i++) top = fmaxf(top, fabsf(to_f(x[i])));
+        tops[tid] = top;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        top = fmaxf(tops[r], tops[128 + r]);
+        const int e = top < INFINITY ? 140 - (int)(__float_as_uint(top) >> 23) : 0;
+        float f1 = __int_as_float((127 + e / 2) << 23);
+        const float f2 = __int_as_float((127 + e - e / 2) << 23);
         alpha = ldexpf(fabsf(a.scale) * 1.4426950408889634f, -e);
         if (a.scale < 0.0f) f1 = -f1;
-        if (!live) f1 = 0.0f;
-#pragma unroll 2
-        for (int i = half * (HD / 16); i < (half + 1) * (HD / 16); i++) {
-            float x[8];
-            if (vec) load_n<T, 8, true>(p + 8 * i, x);
-            else load_n<T, 8, false>(p + 8 * i, x);
+#pragma unroll
+        for (int g = 0; g < HD / 16; g++) {
             uint32_t o[4], ol[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const float u = live ? x[k] * f1 * f2 : 0.0f, v = live ? x[k + 4] * f1 * f2 : 0.0f;
+                const float u = live ? to_f(x[8 * g + k]) * f1 * f2 : 0.0f, v = live ? to_f(x[8 * g + k + 4]) * f1 * f2 : 0.0f;
                 if (BF) {
                     o[k] = pack_bf2(u, v);
                 } else {
@@ -219,6 +217,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                     }
                 }
             }
+            const int i = half * (HD / 16) + g;
             const uint32_t to = base + (i >> 3) * Sm::SLAB + r * 128 + (((i & 7) ^ (r & 7)) << 4);
             sts128(to, o[0], o[1], o[2], o[3]);
             if (NQ == 2) sts128(to + SLABS * Sm::SLAB, ol[0], ol[1], ol[2], ol[3]);
@@ -469,13 +468,14 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 auto largest = [&](auto whole) {
                     constexpr bool ALL = decltype(whole)::value;
                     float top[2] = {-INFINITY, -INFINITY};
+                    const float2 al = make_float2(alpha, alpha);
                     auto take = [&](int j, const uint32_t (&v)[32]) {
                         const uint32_t hid = ALL ? 0u : hidden(j);
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             const float4 k = k4[8 * j + i];
-                            const float2 x = mul2(make_float2(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1])), make_float2(k.x, k.y)),
-                                         y = mul2(make_float2(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])), make_float2(k.z, k.w));
+                            const float2 x = mul2(mul2(make_float2(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1])), al), make_float2(k.x, k.y)),
+                                         y = mul2(mul2(make_float2(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])), al), make_float2(k.z, k.w));
                             if (ALL) {
                                 top[0] = fmaxf(fmaxf(x.x, x.y), top[0]);
                                 top[1] = fmaxf(fmaxf(y.x, y.y), top[1]);
@@ -502,23 +502,24 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                             const float4 k = k4[8 * j + i];
 #pragma unroll
                             for (int u = 0; u < 2; u++) {
-                                float2 y = mul2(make_float2(__uint_as_float(v[4 * i + 2 * u]), __uint_as_float(v[4 * i + 2 * u + 1])), u ? make_float2(k.z, k.w) : make_float2(k.x, k.y));
+                                z[2 * i + u] = mul2(make_float2(__uint_as_float(v[4 * i + 2 * u]), __uint_as_float(v[4 * i + 2 * u + 1])), al);
+                                float2 y = mul2(z[2 * i + u], u ? make_float2(k.z, k.w) : make_float2(k.x, k.y));
                                 if ((hid >> (4 * i + 2 * u)) & 1u) y.x = -INFINITY;
                                 if ((hid >> (4 * i + 2 * u + 1)) & 1u) y.y = -INFINITY;
-                                z[2 * i + u] = y;
                                 top[u] = fmaxf(fmaxf(y.x, y.y), top[u]);
                             }
                         }
                         const float was = m;
-                        m = fmaxf(m, fmaxf(top[0], top[1]) * alpha);      // (alpha = 0: 0, or NaN where nothing is seen, which sets nothing)
+                        m = fmaxf(m, fmaxf(top[0], top[1]));
                         heavy += below(was, m);
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
-                            const float4 d = k4[32 + 8 * j + i];
+                            const float4 k = k4[8 * j + i], d = k4[32 + 8 * j + i];
 #pragma unroll
                             for (int u = 0; u < 2; u++) {
-                                const float2 w = add2(fma2(z[2 * i + u], al, make_float2(-m, -m)), u ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
-                                heavy = fmaxf(heavy, fmaxf(w.x, w.y));
+                                const float2 w = add2(fma2(z[2 * i + u], u ? make_float2(k.z, k.w) : make_float2(k.x, k.y), make_float2(-m, -m)), u ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
+                                if (!((hid >> (4 * i + 2 * u)) & 1u)) heavy = fmaxf(heavy, w.x);
+                                if (!((hid >> (4 * i + 2 * u + 1)) & 1u)) heavy = fmaxf(heavy, w.y);
                             }
                         }
                     };
@@ -537,8 +538,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                     m = refs[128 + r];
                 }
                 if (PASS == QP_FIRST && t < 2 && __any_sync(0xffffffffu, m == -INFINITY)) {
-                    // (alpha = 0: 0, or NaN where nothing is seen, which sets nothing)
-                    const float top = (all ? largest(std::true_type{}) : largest(std::false_type{})) * alpha;
+                    const float top = all ? largest(std::true_type{}) : largest(std::false_type{});
                     if (t == 0) {
                         // the largest value scale of the tile, as a power of two: with the reference that much higher (and kUp more) its weights are fp16 numbers of about 2^-kUp
                         // (of those that are numbers: a row that sees another one has no other result than NaN)
@@ -570,8 +570,9 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                             const float4 k = k4[8 * j + i];
 #pragma unroll
                             for (int u = 0; u < 2; u++) {
-                                const float2 z = mul2(make_float2(__uint_as_float(v[4 * i + 2 * u]), __uint_as_float(v[4 * i + 2 * u + 1])), u ? make_float2(k.z, k.w) : make_float2(k.x, k.y));
-                                float2 y = fma2(z, al, make_float2(-ref, -ref));
+                                // (alpha first: scaled queries times the scale of a large key would leave f32)
+                                const float2 z = mul2(make_float2(__uint_as_float(v[4 * i + 2 * u]), __uint_as_float(v[4 * i + 2 * u + 1])), al);
+                                float2 y = fma2(z, u ? make_float2(k.z, k.w) : make_float2(k.x, k.y), make_float2(-ref, -ref));
                                 if (!ALL) {
                                     if ((hid >> (4 * i + 2 * u)) & 1u) y.x = -INFINITY;
                                     if ((hid >> (4 * i + 2 * u + 1)) & 1u) y.y = -INFINITY;

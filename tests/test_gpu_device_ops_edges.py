@@ -160,6 +160,20 @@ def test_attention_of_values_near_the_ends_of_f32(D, dtype, magnitude, q_lens, n
     within(run_attention(D, q, pages, table, lens, starts), want, off, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("magnitude", [2.0**-115, 2.0**120, 2.0**122])
+@pytest.mark.parametrize("q_lens,nkv", [([1, 1], 2), ([60, 17], 24)])
+def test_attention_of_queries_near_the_ends_of_f32(D, dtype, magnitude, q_lens, nkv):  # noqa: F811
+    """Scores are ordinary: the keys' scales are as small as the queries are large."""
+    lens = [700, 120]
+    pages, table = cache(5, lens, nkv, 64, 16)
+    R.sections(pages, 16, 64)[2].mul_(1 / magnitude)
+    starts = starts_of(q_lens)
+    q = ((2.0 * normal(9, starts[-1], 4 * nkv, 64)).clamp(-7, 7) * magnitude).to(dtype)
+    want, off = X.attention(q, pages, table, lens, starts, 16, 0.125)
+    within(run_attention(D, q, pages, table, lens, starts), want, off, dtype)
+
+
 # ---------------------------------------------------------------------------------------------------------------- results
 def test_results_have_memory_of_their_own(D):  # noqa: F811
     """A result that grows in place does not grow into another one, and one that is kept does not keep the others."""
