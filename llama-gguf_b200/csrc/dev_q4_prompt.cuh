@@ -492,38 +492,52 @@ template <typename T, int HD> __global__ void __launch_bounds__(QP_THREADS, 1) a
                 };
                 if constexpr (PASS == QP_SCAN) {
                     // the largest score so far, and the largest weight, as a power of two and with that score for reference
-                    auto take = [&](int j, const uint32_t (&v)[32]) {
-                        const uint32_t hid = all ? 0u : hidden(j);
+                    auto scan = [&](auto whole) {
+                        constexpr bool ALL = decltype(whole)::value;
                         const float2 al = make_float2(alpha, alpha);
-                        float2 z[16];
-                        float top[2] = {-INFINITY, -INFINITY};
+                        auto take = [&](int j, const uint32_t (&v)[32]) {
+                            const uint32_t hid = ALL ? 0u : hidden(j);
+                            float2 z[16];
+                            float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float4 k = k4[8 * j + i];
+                            for (int i = 0; i < 8; i++) {
+                                const float4 k = k4[8 * j + i];
 #pragma unroll
-                            for (int u = 0; u < 2; u++) {
-                                z[2 * i + u] = mul2(make_float2(__uint_as_float(v[4 * i + 2 * u]), __uint_as_float(v[4 * i + 2 * u + 1])), al);
-                                float2 y = mul2(z[2 * i + u], u ? make_float2(k.z, k.w) : make_float2(k.x, k.y));
-                                if ((hid >> (4 * i + 2 * u)) & 1u) y.x = -INFINITY;
-                                if ((hid >> (4 * i + 2 * u + 1)) & 1u) y.y = -INFINITY;
-                                top[u] = fmaxf(fmaxf(y.x, y.y), top[u]);
+                                for (int u = 0; u < 2; u++) {
+                                    z[2 * i + u] = mul2(make_float2(__uint_as_float(v[4 * i + 2 * u]), __uint_as_float(v[4 * i + 2 * u + 1])), al);
+                                    const float2 y = mul2(z[2 * i + u], u ? make_float2(k.z, k.w) : make_float2(k.x, k.y));
+                                    if (ALL) {
+                                        top[u] = fmaxf(fmaxf(y.x, y.y), top[u]);
+                                    } else {
+                                        if (!((hid >> (4 * i + 2 * u)) & 1u)) top[u] = fmaxf(top[u], y.x);
+                                        if (!((hid >> (4 * i + 2 * u + 1)) & 1u)) top[u] = fmaxf(top[u], y.y);
+                                    }
+                                }
                             }
-                        }
-                        const float was = m;
-                        m = fmaxf(m, fmaxf(top[0], top[1]));
-                        heavy += below(was, m);
+                            const float was = m;
+                            m = fmaxf(m, fmaxf(top[0], top[1]));
+                            heavy += below(was, m);
+                            float most[2] = {heavy, heavy};
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float4 k = k4[8 * j + i], d = k4[32 + 8 * j + i];
+                            for (int i = 0; i < 8; i++) {
+                                const float4 k = k4[8 * j + i], d = k4[32 + 8 * j + i];
 #pragma unroll
-                            for (int u = 0; u < 2; u++) {
-                                const float2 w = add2(fma2(z[2 * i + u], u ? make_float2(k.z, k.w) : make_float2(k.x, k.y), make_float2(-m, -m)), u ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
-                                if (!((hid >> (4 * i + 2 * u)) & 1u)) heavy = fmaxf(heavy, w.x);
-                                if (!((hid >> (4 * i + 2 * u + 1)) & 1u)) heavy = fmaxf(heavy, w.y);
+                                for (int u = 0; u < 2; u++) {
+                                    const float2 w = add2(fma2(z[2 * i + u], u ? make_float2(k.z, k.w) : make_float2(k.x, k.y), make_float2(-m, -m)), u ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
+                                    if (ALL) {
+                                        most[u] = fmaxf(fmaxf(w.x, w.y), most[u]);
+                                    } else {
+                                        if (!((hid >> (4 * i + 2 * u)) & 1u)) most[u] = fmaxf(most[u], w.x);
+                                        if (!((hid >> (4 * i + 2 * u + 1)) & 1u)) most[u] = fmaxf(most[u], w.y);
+                                    }
+                                }
                             }
-                        }
+                            heavy = fmaxf(most[0], most[1]);
+                        };
+                        by_32(S, take);
                     };
-                    by_32(S, take);
+                    if (all) scan(std::true_type{});
+                    else scan(std::false_type{});
                     umma_before_sync();
                     __syncwarp();
                     if (lane == 0) bar_arrive(p_full + 8 * (t % 6));
