@@ -8,7 +8,7 @@
 //                          tile of 256 x 256 (cta_group::2), each with its own weight rows and half of the token rows: 32 KB a step per CTA instead of 48.
 //   gemm_i8_split_kernel   few tiles: S CTAs of a cluster share a tile's steps and add their sums through distributed shared memory.  With one token the weights' bytes are all there is
 //                          to do, and a ring of up to 192 KB per SM keeps enough of them on the way.
-// Measured (tokens x n x k): 2048 x 14336 x 4096 100 us in a loop (2400 TOP/s; 90 us cold and by itself), bound by the steps' copies to shared memory; 4 x 14336 x 4096 13.3 us for 59 MB (4.4 TB/s).
+// Measured (tokens x n x k): 2048 x 14336 x 4096 101 us in a loop (2400 TOP/s; 88 us by itself), bound by the tensor pipe (79 % of cycles, 91 on the SMs with the most tiles) and a last wave; 4 x 14336 x 4096 13.3 us for 59 MB (4.4 TB/s).
 #pragma once
 #include "dev_umma.cuh"
 
@@ -278,7 +278,7 @@ struct GemmI8Plan {
     bool wide, pair;
 };
 // The kernel of least estimated time (ns) on 148 SMs, by what each one measured (bf16 results, weights from DRAM): a step of 128 bytes of K takes 225 + 0.4 TN (wide: 280 with 128 tokens, 361 with 256, 300 for a
-// pair), whatever its MMAs, since it is a step's copies that bound it; a launch 2300 + 20 TN for its first bytes and its last sums, the exchange of a cut 400 and 30 per token and CTA; a wide kernel's start and last tile
+// pair), whatever its MMAs, since it is a step's copies that bound it (a pair's MMAs take 276 of its 300); a launch 2300 + 20 TN for its first bytes and its last sums, the exchange of a cut 400 and 30 per token and CTA; a wide kernel's start and last tile
 // 5900, 8200 and 9500.  Clusters of 8 do not tile the chip's groups of SMs: 112 of their CTAs run at once.
 // Measured (us; t x n x k): 1 x 4096 x 4096 10.2 in one piece, 7.5 in two, 6.6 in four, 13.7 in eight; 160 x 4096 x 4096 in tiles of 64 tokens 11.9, of 128 13.8; 2048 x 2048 x 2048 wide 13.8, 128 and 14.9 of 128 tokens;
 // 384 x 14336 x 4096 28.6 in pairs, 32.8 and 33.6 without.

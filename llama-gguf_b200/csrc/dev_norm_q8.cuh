@@ -155,7 +155,7 @@ template <typename T> __global__ void __launch_bounds__(256) add_rms_norm_q8_any
 template <typename T, int V> cudaError_t add_rms_norm_q8_words(const NormQ8Args& a, int threads, cudaStream_t st) {
     return launch(add_rms_norm_q8_kernel<T, V>, dim3((unsigned)a.rows), threads, 0, 1, st, a);
 }
-// Bound by the rows' bytes where there are many (2048 x 4096 bf16 with a residual: 58.7 MB in 15.5 us, cold and by itself, 3.8 TB/s with the launch), by the launch and two reductions where there are few (one row of 4096: 6.5 us so).
+// Bound by the rows' bytes where there are many (2048 x 4096 bf16 with a residual: 58.7 MB in 15 us by itself, 13 among others), by the launch and two reductions where there are few (one row of 4096: 5 us by itself).
 // A block per row with two reads of it took 42 and 22.
 // Few rows: as many threads as the row has words, up to 1024 (one token of 4096 in bf16: latency).  Many rows: four words per thread, so that a block has fewer warps to wait for and the loads of a
 // thread cover one another.  Rows of more than 4 x 1024 words do not fit the registers.

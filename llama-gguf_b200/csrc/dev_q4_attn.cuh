@@ -16,9 +16,9 @@
 // same sums.  f16 and bf16 queries are one exactly.  (Weights of one number, 2^-11, took a tenth less time for bf16 results, which they moved to the next number now and then.)
 // The weight of a value is p_j d_j.  Its reference is not m but m + r, the largest z_j + log2 |d_j| so far less 7: p_j d_j stays in fp16's range whatever the values' scales are, from 2^7 to 2^15 where it is largest,
 // so that fp16's last bit, 2^-25, is 2^-32 of that (r is kept by itself: large scores leave no bits of log2 |d_j| in a sum).  Both references move only when something passes them by 2^8, so the usual step has no exchange between lanes but the 8 x 8 transposition that makes operands of the weights.
-// What bounds it: the bytes of the cache, hd + 8 per position and kv head.  Measured (both kernels, cold): one token over 131072 positions, 64 heads over 8 of 128, bf16: 46 us for 143 MB (3.1 TB/s): about 7 us until
-// every block knows its stretch and has its first tiles, 29 of stream at 4.9 TB/s (a kernel of the same copies without the arithmetic: 36 altogether), a spread of the blocks' ends, 4 of the join.  32 sequences of up to
-// 8000: 38 to 41 us for 96 MB.  A warp takes 32 positions a step (two of the above, so that its chains of mma cover each other).  When the last steps were tried, warps of an SM and positions of a step (us, the two cases): 12 and 32 46.5, 38.7;
+// What bounds it: the bytes of the cache, hd + 8 per position and kv head.  Measured (both kernels, cold): one token over 131072 positions, 64 heads over 8 of 128, bf16 and f16: 50 us for 143 MB (2.8 TB/s): about 7 us until
+// every block knows its stretch and has its first tiles, some 33 of stream (a kernel of the same copies without the arithmetic: 36 altogether), a spread of the blocks' ends, 4 of the join; f32 56.  Issue slots are 54 % used.  32 sequences of
+// up to 8000: 43 us for 96 MB.  With single weights (bf16) 46 and 39.  A warp takes 32 positions a step (two of the above, so that its chains of mma cover each other).  When single weights were the rule, warps of an SM and positions of a step (us, the two cases): 12 and 32 46.5, 38.7;
 // 16 and 32 51, 44.6; 16 and 16 52, 43; 8 and 48 43.9 to 45, 39.5 to 43: the first of these is the best of the two together and the steadier.
 #pragma once
 #include <type_traits>

@@ -9,15 +9,17 @@
 //               products; the two are joined at the end.  P goes back to tensor memory in place of S.
 // Keys' scales multiply the scores, values' scales the weights.  f32 queries are pairs of fp16 numbers scaled by a power of two.  Passes:
 //   first   The reference of a row's exponentials need only be near: it is the largest score of the first tile that the row sees, and stays.  So no tile waits for another: one O, three buffers of scores,
-//           each score read once.  A weight p_j d_j is two fp16 numbers (what the first leaves over is the second: 2^-22), 2^3 or 2^4
-//           where the reference was set.
+//           each score read once.  A weight p_j d_j is two fp16 numbers (what the first leaves over is the second: 2^-22), 2^3 or 2^4 where the reference was set.
 //   scan, again   Where a row passes fp16's range, or the last bits of its weights may have cost too much of its result (Q4Weights), or its result is not finite, the block goes over the keys twice more: once for
 //           the scores alone, which gives each row its largest score m and its largest weight, and once as above with these for references: probabilities 2^(z_j - m), weights p_j d_j 2^e of up to 2^14 in pairs of fp16
 //           numbers, whose last bit, 2^-25, is 2^-38 of the largest.
 // What bounds it: per row and tile 128 x (hd + hd) products (three times that for f32), 128 exponentials with some ten instructions each, and shared memory: both operands of S and the values of P V are
-// read from it, and 48 KB of them written per tile.  A tile takes 1.7 us at hd 128, on one SM as on all: a tile of a warp of rows some 2900 clocks (two groups share the tiles), of a warp that makes operands 2300, the products
-// 1400 with their starts, each slowing the others at the schedulers.  Measured: 2048 query tokens after 2048 others, 32 heads over 8 of 128, bf16: 182 us, 512 blocks of 17 to 32 tiles, 570 TFLOP/s of the products that
-// the mask leaves.  With keys made behind the values of the tile before, scores two tiles ahead and both passes in one piece of code (spills) 202; with references that move and pairs of bf16 for all 245.
+// read from it, and 48 KB of them written per tile.  A tile takes 1.8 us at hd 128 (f32 2.1), on one SM as on all; issue slots are 59 % used, the tensor pipe 41 %, and the three roles slow one another at the schedulers.
+// Measured: 2048 query tokens after 2048 others, 32 heads over 8 of 128: bf16 and f16 204 us, 512 blocks of 17 to 32 tiles, 505 TFLOP/s of the products that the mask leaves; f32 237.  bf16 results with single fp16 weights
+// (2^-11) took 182, and then 20 more with keys made behind the values of the tile before.  Where every block goes over its keys again 545 (bf16), 556 (f16), 597 (f32): a scan takes 145 over the first pass, the pass behind it
+// as long as the first.  (A second pass whose references moved, with pairs of bf16, took as long, and lost bits; with pairs of fp16 640.)  Blocks that need it: scores that pass a row's first tile by 2^12 or so, and rows whose
+// largest channel is small next to the sum of their weights.  Gaussian scores of up to 4000 keys none; a first position with e^12 of the others' weight each and a twentieth of their values none in bf16, most in f16;
+// f32 rows of Gaussian scores from some 5000 keys on.
 #pragma once
 #include <type_traits>
 
