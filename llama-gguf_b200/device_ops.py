@@ -2,7 +2,8 @@
 
 The peers of CudaB200Backend's rms_norm, mat_mat_q, rope, attention_cached and dequantize for a decoder layer that is served with activations in 8 bits
 and a paged cache in 4 bits.  Tensors are torch CUDA tensors; the work is queued on the current stream of their device, outputs and workspaces come from torch's
-allocator on that stream, so that the calls can be captured into a CUDA graph (a graph has its own workspaces).  Results carry no gradients.
+allocator on that stream, so that the calls can be captured into a CUDA graph (a graph has its own workspaces).  Results carry no gradients (arguments
+that require one, or have a forward-mode tangent, are refused), and have memory of their own.
 
     q, s, r = add_rms_norm_q8(x, weight, eps, residual=r)               # rows in 8 bits with a scale each, and the new residual
     qkv = mat_mat_i8(q, s, w, ws)                                       # 8-bit product

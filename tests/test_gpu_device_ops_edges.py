@@ -174,6 +174,26 @@ def test_attention_of_queries_near_the_ends_of_f32(D, dtype, magnitude, q_lens, 
     within(run_attention(D, q, pages, table, lens, starts), want, off, dtype)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_of_prompts_at_odd_places(D, dtype, hd):  # noqa: F811
+    """Queries and results that no word fits, tokens ahead of the first sequence and behind the last, sequences without tokens: the same bits as from rows side by side, and nothing else written."""
+    lens, q_lens, nh, nkv = [5, 300, 0, 160, 40], [0, 70, 0, 45, 1], 48, 12
+    pages, table = cache(5, lens, nkv, hd, 48)
+    starts = [s + 3 for s in starts_of(q_lens)]
+    n = starts[-1] + 5
+    wide = normal(9, n, nh + 1, hd + 3).to(dtype).cuda()
+    q, buf = wide[:, 1:, 1 : hd + 1], torch.full((n, nh, hd + 5), 7.0, dtype=dtype, device="cuda")
+    got = run_attention(D, q, pages, table, lens, starts, out=buf[:, :, 3 : hd + 3])
+    assert (buf[: starts[0]] == 7).all() and (buf[starts[-1] :] == 7).all() and (buf[:, :, :3] == 7).all() and (buf[:, :, hd + 3 :] == 7).all()
+    side = q[starts[0] : starts[-1]].contiguous()
+    own = [s - starts[0] for s in starts]
+    assert torch.equal(got[starts[0] : starts[-1]], run_attention(D, side, pages, table, lens, own))
+    assert takes_prompts(D, q_lens, nh, nkv, hd)
+    want, off = X.attention(side, pages, table, lens, own, 48, hd**-0.5)
+    within(got[starts[0] : starts[-1]], want, off, dtype)
+
+
 # ---------------------------------------------------------------------------------------------------------------- results
 def test_results_have_memory_of_their_own(D):  # noqa: F811
     """A result that grows in place does not grow into another one, and one that is kept does not keep the others."""
