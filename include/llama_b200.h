@@ -576,7 +576,7 @@ B200_API int b200_op_attention(const float* q, const float* k, const float* v, f
  * until the work is done.  Arguments are checked on the host first (also without a GPU); indices that lie in device memory are checked by the kernels: a bad
  * one is never followed, and sets a bit of *status (int32 on the device, added to with atomicOr, NULL: not wanted).
  * Activations are f32, f16 or bf16 (B200_TYPE_*); distances between rows, tokens and heads are in elements, the last dimension is contiguous. */
-enum { B200_STATUS_BAD_SLOT = 1, B200_STATUS_BAD_POSITION = 2, B200_STATUS_BAD_PAGE = 4, B200_STATUS_BAD_LENGTH = 8 };
+enum { B200_STATUS_BAD_SLOT = 1, B200_STATUS_BAD_POSITION = 2, B200_STATUS_BAD_PAGE = 4, B200_STATUS_BAD_LENGTH = 8, B200_STATUS_BAD_EXPERT = 16 };
 /* 0, or the code of the bounded wait inside one of these operators that gave up last (its results are then not valid); clears it.  Waits for the device's default stream. */
 B200_API int b200_dev_watchdog(int device, int* out);
 /* RMS norm of a residual sum, with the result in 8 bits and one scale per row:
@@ -597,6 +597,79 @@ B200_API int b200_dev_read_q8(int device, void* stream, uint32_t type, const int
 B200_API int b200_dev_mat_mat_i8(int device, void* stream, uint32_t out_type, const int8_t* a, int64_t lda, const float* a_scales,
                                  const int8_t* w, int64_t ldw, const float* w_scales, const float* bias /* may be NULL */, void* out, int64_t ldo,
                                  int64_t t_rows, int64_t k, int64_t n);
+/* Routing: each token's `top` experts by its router logits [tokens][n] of `type`, and their weights.  The scores are p = softmax(z) (over all n) or, with `sigmoid`, 1 / (1 + exp(-z)); the
+ * choice goes by z, or by p + correction ([n] f32) where that is given.  groups > 1: n / groups neighbours are a group, which counts by the sum of its two best p (p + correction), and only the best
+ * top_groups groups' experts are left (the scores are still over all).  Experts come in falling order of what chose them, the lower number first among equals (groups too).  weights = p, with
+ * `renormalise` over the sum of the chosen ones' (a sum of zero stays), times `scale`, rounded to f32 once.  What decides is made in 64 bits.
+ * An expert whose logit or correction is -infinity or NaN is not chosen; where fewer than `top` are left the places behind them are expert -1 with weight 0 (a row of -infinity: a place of a batch that
+ * holds no token).  A row that holds NaN (softmax: or +infinity) has weights NaN, and its choice goes by z alone, a group's by its largest.
+ * 1 <= n <= 1024, groups divides n, 1 <= top <= 32, top <= n / groups * top_groups, groups <= 32.  experts, weights: [tokens][top]. */
+typedef struct b200_route {
+    int32_t device;
+    uint32_t type;
+    void* stream;
+    const void* logits;
+    int64_t ld, tokens;
+    int32_t n, top, groups, top_groups, sigmoid, renormalise;
+    float scale;
+    const float* correction;         /* may be NULL */
+    int32_t* experts;
+    float* weights;
+} b200_route;
+B200_API int b200_dev_route_experts(const b200_route* a);
+/* Product of rows in 8 bits with 4-bit weights that have a scale per group of `group` channels (32, 64 or 128; it divides k):
+ *   out[t][n] = (sum_g ws[n][g] * (sum over group g's k of a[t][k] w[n][k])) * a_scales[t] + bias[n], the inner sums exact, the outer one f32, rounded to out_type.
+ * Weights lie in tiles of 16 rows x 64 channels of 512 bytes, [ceil(n / 16)][ceil(k / 64)][row % 8][4][half][row half][4 bytes]: byte b at (g, t, half, row_half) has channel 32 half + 8t + b
+ * in its low four bits and channel 32 half + 8t + 4 + b in its high four, of row 8 row_half + g of the tile, in two's complement (-8 .. 7).  Channels behind k and rows behind n count for nothing.  Scales:
+ * [ceil(n / 16)][k / group][8][row half] of scale_type (F32, F16 or BF16).
+ * With `experts` ([tokens][top] int32) there are n_experts such matrices one after the other (and [n_experts][n] of bias), out has a row for each pair (token, place) and is
+ * [tokens * top][n]; a has a row per token, or per pair where rows_per_pair is set.  Pairs of expert -1 get zeros; other numbers outside 0 .. n_experts - 1 too, BAD_EXPERT.
+ * a starts on 16 bytes with rows a multiple of 16 bytes apart; what lies between k and the next row is not used.  w starts on 16 bytes, the scales on 8.  Meant for few rows: the weights' bytes
+ * are read once per 64 rows (of an expert). */
+typedef struct b200_i4_product {
+    int32_t device;
+    uint32_t out_type, scale_type;
+    int32_t group;
+    void* stream;
+    const int8_t* a;
+    int64_t lda;
+    const float* a_scales;
+    const void *w, *w_scales;
+    const float* bias;               /* may be NULL */
+    void* out;
+    int64_t ldo, tokens, k, n;
+    const int32_t* experts;          /* may be NULL: one matrix */
+    int32_t top, n_experts, rows_per_pair;
+    int32_t* status;
+} b200_i4_product;
+B200_API int b200_dev_mat_mat_i4(const b200_i4_product* a);
+/* Gated unit with the result in 8 bits and one scale per row: y[i] = act(x[row][i]) * x[row][ff + i], scales[row] = max |y| / 127, q = round(y * (127 / max |y|)), halves to even, decided
+ * as if y were exact.  Rows with max |y| < 2^-119 give zeros with scale 0, rows with max |y| = infinity or NaN give zeros with scale NaN.  GELU is its tanh form.  1 <= ff <= 65536. */
+enum { B200_GLU_SILU = 0, B200_GLU_GELU = 1, B200_GLU_RELU = 2 };
+B200_API int b200_dev_glu_q8(int device, void* stream, uint32_t type, int act, const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scales, int64_t rows, int64_t ff);
+/* A block's output onto the residual stream, and the next norm with its result in 8 bits:
+ *   m = y (mix NULL), or sum over j < top of mix[row][j] * y[row * top + j] (f32, in that order);  p = m / sqrt(mean(m^2) + eps) * post_weight, or m where that is NULL;
+ *   r = residual + (p * gate) * scale, rounded to the type, to `sum`;  q, scales = r / sqrt(mean(r^2) + eps) * weight as b200_dev_add_rms_norm_q8 makes them (weight NULL: neither).
+ * Every product and sum is rounded to f32, means are taken in 64 bits.  gate: element (row, i) at row * gate_row + i * gate_col, so that one per row, one per channel or one for
+ * each may be given (NULL: none).  `sum` may be `residual` with the same row distance; other overlaps are not allowed.  mix: [rows][top], 1 <= top <= 32.  1 <= hidden <= 65536. */
+typedef struct b200_gated_norm {
+    int32_t device;
+    uint32_t type;
+    void* stream;
+    const void* y;
+    const float* mix;
+    const float* post_weight;
+    const void* gate;
+    const void* residual;
+    void* sum;
+    const float* weight;
+    int8_t* q;
+    float* scales;
+    int64_t ldy, gate_row, gate_col, ldr, lds, ldq, rows, hidden;
+    int32_t top;
+    float scale, eps;
+} b200_gated_norm;
+B200_API int b200_dev_add_gated_norm_q8(const b200_gated_norm* a);
 /* Paged cache in 4 bits.  A page holds page_size positions; per kv head one block of page_size * (head_dim + 8) bytes: page_size rows of
  * head_dim / 2 bytes of keys, as many of values, page_size f32 key scales, page_size f32 value scales.  Byte i of a row has channel 2i in
  * its low four bits and channel 2i + 1 in its high four; a value is scale * (n - 8).  Blocks follow one another: [page][kv head].

@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/llama_b200.h"
 
 namespace dev {
@@ -87,5 +89,20 @@ template <typename... P, typename... A> cudaError_t launch(void (*kernel)(P...),
     cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
+
+// A kernel's dynamic shared memory is allowed once per device (64 devices; further ones ask every time).  One per kernel, by its address.
+struct SmemAllowed {
+    std::atomic<uint64_t> done{0};
+    cudaError_t operator()(const void* kernel, size_t bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+        if (bit && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+        return e;
+    }
+};
 
 }  // namespace dev

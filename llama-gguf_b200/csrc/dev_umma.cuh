@@ -3,8 +3,6 @@
 #pragma once
 #include <cuda.h>
 
-#include <atomic>
-
 #include "dev_common.cuh"
 
 namespace dev {
@@ -126,18 +124,4 @@ inline bool byte_map(CUtensorMap* map, const void* p, int64_t cols, int64_t rows
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// A kernel's dynamic shared memory is allowed once per device (64 devices; further ones ask every time).  One per kernel, by its address.
-struct SmemAllowed {
-    std::atomic<uint64_t> done{0};
-    cudaError_t operator()(const void* kernel, size_t bytes) {
-        int dev = 0;
-        cudaError_t e = cudaGetDevice(&dev);
-        if (e != cudaSuccess) return e;
-        const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
-        if (bit && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
-        return e;
-    }
-};
 }  // namespace dev

@@ -26,6 +26,10 @@ struct Entries {
     decltype(&b200_dev_add_rms_norm_q8) add_rms_norm_q8 = nullptr;
     decltype(&b200_dev_read_q8) read_q8 = nullptr;
     decltype(&b200_dev_mat_mat_i8) mat_mat_i8 = nullptr;
+    decltype(&b200_dev_route_experts) route_experts = nullptr;
+    decltype(&b200_dev_mat_mat_i4) mat_mat_i4 = nullptr;
+    decltype(&b200_dev_glu_q8) glu_q8 = nullptr;
+    decltype(&b200_dev_add_gated_norm_q8) add_gated_norm_q8 = nullptr;
     decltype(&b200_dev_rope_append_q4) rope_append_q4 = nullptr;
     decltype(&b200_dev_read_q4) read_q4 = nullptr;
     decltype(&b200_dev_attention_paged_q4_workspace) attention_workspace = nullptr;
@@ -111,11 +115,34 @@ struct Call {
         if (t.dim() != 2 || t.size(0) != rows || t.size(1) != cols || (cols > 1 && t.stride(1) != 1))
             refuse(B200_ERR_SHAPE_MISMATCH, op, std::string(name) + ": expected [" + std::to_string(rows) + ", " + std::to_string(cols) + "] with contiguous rows, got " + sizes(t));
     }
+    void whole(const char* name, const Tensor& t, int64_t rows, int64_t cols, at::ScalarType want) const {
+        typed(name, t, want);
+        if (t.dim() != 2 || t.size(0) != rows || t.size(1) != cols || !t.is_contiguous())
+            refuse(B200_ERR_SHAPE_MISMATCH, op, std::string(name) + ": expected [" + std::to_string(rows) + ", " + std::to_string(cols) + "] contiguous, got " + sizes(t));
+    }
     void heads(const char* name, const Tensor& t, int64_t tokens, int64_t n, int64_t hd, at::ScalarType want) const {      // n < 0: any number of heads
         typed(name, t, want);
         if (t.dim() != 3 || t.size(0) != tokens || (n >= 0 && t.size(1) != n) || t.size(2) != hd || t.stride(2) != 1)
             refuse(B200_ERR_SHAPE_MISMATCH, op,
                    std::string(name) + ": expected [" + std::to_string(tokens) + ", " + (n >= 0 ? std::to_string(n) : "heads") + ", " + std::to_string(hd) + "] with contiguous channels, got " + sizes(t));
+    }
+    bool flag(int i) const {
+        const int v = PyObject_IsTrue(args[i]);
+        if (v < 0) throw PythonError{};
+        return v;
+    }
+    // argument i, one of `names`: its place there
+    template <size_t N> int choice(int i, const char* name, const char* const (&names)[N]) const {
+        if (!PyUnicode_Check(args[i])) {
+            PyErr_Format(PyExc_TypeError, "%s: %s: a text expected", op, name);
+            throw PythonError{};
+        }
+        std::string all;
+        for (size_t k = 0; k < N; k++) {
+            if (!PyUnicode_CompareWithASCIIString(args[i], names[k])) return (int)k;
+            all += std::string(k ? ", " : "") + names[k];
+        }
+        refuse(B200_ERR_INVALID_ARGUMENT, op, std::string(name) + ": one of " + all + " expected");
     }
     b200_q4_pages pages(const Tensor& t, int64_t hd) const {
         typed("pages", t, at::kByte);
@@ -236,6 +263,201 @@ PyObject* mat_mat_i8(PyObject* const* args, Py_ssize_t n_args) {
     return give(out);
 }
 
+PyObject* route_experts(PyObject* const* args, Py_ssize_t n) {
+    Call c("route_experts", args, n, 10);
+    const Tensor z = c.tensor(0, "logits"), corr = c.maybe(3, "correction");
+    Tensor experts = c.maybe(8, "experts"), weights = c.maybe(9, "weights");
+    if (z.dim() != 2) refuse(B200_ERR_SHAPE_MISMATCH, c.op, "logits: expected [tokens, experts], got " + sizes(z));
+    const int64_t tokens = z.size(0), many = z.size(1), top = c.integer(1), groups = c.integer(4), top_groups = c.integer(5);
+    static const char* const scores[] = {"softmax", "sigmoid"};
+    b200_route a{};
+    a.type = c.type(z.scalar_type());
+    a.sigmoid = c.choice(2, "score", scores);
+    a.renormalise = c.flag(6);
+    a.scale = (float)c.number(7);
+    if (many > 1024) refuse(B200_ERR_SHAPE_MISMATCH, c.op, "1 to 1024 experts expected");
+    if (top < 1 || top > 32 || groups < 1 || groups > 32 || top_groups < 1 || top_groups > 32) refuse(B200_ERR_SHAPE_MISMATCH, c.op, "top, groups and top_groups must be from 1 to 32");
+    c.matrix("logits", z, tokens, many, z.scalar_type());
+    if (corr.defined()) c.vector("correction", corr, many, at::kFloat);
+    if (experts.defined()) c.whole("experts", experts, tokens, top, at::kInt);
+    if (weights.defined()) c.whole("weights", weights, tokens, top, at::kFloat);
+    c.together(z, corr, experts, weights);
+    if (!experts.defined()) experts = c.empty({tokens, top}, at::kInt);
+    if (!weights.defined()) weights = c.empty({tokens, top}, at::kFloat);
+    a.device = c.device.index();
+    a.stream = c.stream();
+    a.logits = ptr(z);
+    a.ld = ld(z);
+    a.tokens = tokens;
+    a.n = (int32_t)many;
+    a.top = (int32_t)top;
+    a.groups = (int32_t)groups;
+    a.top_groups = (int32_t)top_groups;
+    a.correction = (const float*)ptr(corr);
+    a.experts = (int32_t*)ptr(experts);
+    a.weights = (float*)ptr(weights);
+    check(E.route_experts(&a));
+    return give(experts, weights);
+}
+
+PyObject* mat_mat_i4(PyObject* const* args, Py_ssize_t n_args) {
+    Call c("mat_mat_i4", args, n_args, 10);
+    const Tensor x = c.tensor(0, "a"), xs = c.tensor(1, "a_scales"), w = c.tensor(2, "w"), ws = c.tensor(3, "w_scales"), experts = c.maybe(5, "experts"), bias = c.maybe(6, "bias");
+    Tensor out = c.maybe(8, "out");
+    if (x.dim() != 2) refuse(B200_ERR_SHAPE_MISMATCH, c.op, "a: expected [rows, k], got " + sizes(x));
+    const int64_t rows = x.size(0), k = x.size(1), lead = experts.defined() ? 1 : 0;
+    b200_i4_product a{};
+    a.scale_type = c.type(ws.scalar_type());
+    const at::ScalarType dt = out.defined() ? out.scalar_type() : c.dtype(7);
+    a.out_type = c.type(dt);
+    c.typed("w", w, at::kByte);
+    if (w.dim() != 3 + lead || !w.is_contiguous() || w.size(lead + 2) != 512 || w.size(lead + 1) != (k + 63) / 64 || w.size(lead) < 1)
+        refuse(B200_ERR_SHAPE_MISMATCH, c.op, std::string("w: expected ") + (lead ? "[experts, " : "[") + "row tiles, " + std::to_string((k + 63) / 64) + ", 512] contiguous, got " + sizes(w));
+    const int64_t tiles = w.size(lead), n = args[4] == Py_None ? tiles * 16 : c.integer(4);
+    if (n < 1 || (n + 15) / 16 != tiles) refuse(B200_ERR_SHAPE_MISMATCH, c.op, "n: " + std::to_string(n) + " rows are not " + std::to_string(tiles) + " tiles of 16");
+    if (ws.dim() != 4 + lead || !ws.is_contiguous() || (lead && ws.size(0) != w.size(0)) || ws.size(lead) != tiles || ws.size(lead + 1) < 1 || ws.size(lead + 2) != 8 || ws.size(lead + 3) != 2 ||
+        k % ws.size(lead + 1))
+        refuse(B200_ERR_SHAPE_MISMATCH, c.op, std::string("w_scales: expected ") + (lead ? "[experts, " : "[") + std::to_string(tiles) + ", groups, 8, 2] contiguous, got " + sizes(ws));
+    const int64_t group = k / ws.size(lead + 1);
+    if (group != 32 && group != 64 && group != 128) refuse(B200_ERR_UNSUPPORTED, c.op, "groups of " + std::to_string(group) + " channels (32, 64 and 128 only)");
+    c.matrix("a", x, rows, k, at::kChar);
+    c.vector("a_scales", xs, rows, at::kFloat);
+    int64_t tokens = rows, many = rows;
+    if (lead) {
+        c.typed("experts", experts, at::kInt);
+        if (experts.dim() != 2 || !experts.is_contiguous() || experts.size(1) < 1) refuse(B200_ERR_SHAPE_MISMATCH, c.op, "experts: expected [tokens, top] contiguous, got " + sizes(experts));
+        tokens = experts.size(0);
+        many = experts.numel();
+        if (rows != tokens && rows != many) refuse(B200_ERR_SHAPE_MISMATCH, c.op, "a has " + std::to_string(rows) + " rows for " + std::to_string(tokens) + " tokens of " + std::to_string(experts.size(1)) + " experts");
+        if (experts.size(1) > 32 || w.size(0) > 1024) refuse(B200_ERR_SHAPE_MISMATCH, c.op, "1 to 32 places of 1 to 1024 experts expected");
+    }
+    if (bias.defined()) {
+        if (lead) c.whole("bias", bias, w.size(0), n, at::kFloat);
+        else c.vector("bias", bias, n, at::kFloat);
+    }
+    if (out.defined()) c.matrix("out", out, many, n, dt);
+    c.together(x, xs, w, ws, experts, bias, out);
+    if (!out.defined()) out = c.empty({many, n}, dt);
+    a.device = c.device.index();
+    a.stream = c.stream();
+    a.group = (int32_t)group;
+    a.a = (const int8_t*)ptr(x);
+    a.lda = rows > 1 ? x.stride(0) : up16(k);      // (one row has no distance)
+    a.a_scales = (const float*)ptr(xs);
+    a.w = ptr(w);
+    a.w_scales = ptr(ws);
+    a.bias = (const float*)ptr(bias);
+    a.out = ptr(out);
+    a.ldo = ld(out);
+    a.tokens = tokens;
+    a.k = k;
+    a.n = n;
+    if (lead) {
+        a.experts = (const int32_t*)ptr(experts);
+        a.top = (int32_t)experts.size(1);
+        a.n_experts = (int32_t)w.size(0);
+        a.rows_per_pair = rows != tokens;
+    }
+    a.status = c.status(9);
+    check(E.mat_mat_i4(&a));
+    return give(out);
+}
+
+PyObject* glu_q8(PyObject* const* args, Py_ssize_t n) {
+    Call c("glu_q8", args, n, 4);
+    const Tensor x = c.tensor(0, "x");
+    Tensor q = c.maybe(2, "out"), s = c.maybe(3, "scales");
+    if (x.dim() != 2 || x.size(1) % 2) refuse(B200_ERR_SHAPE_MISMATCH, c.op, "x: expected [rows, 2 ff], got " + sizes(x));
+    const int64_t rows = x.size(0), ff = x.size(1) / 2;
+    const uint32_t t = c.type(x.scalar_type());
+    static const char* const acts[] = {"silu", "gelu", "relu"};
+    const int act = c.choice(1, "act", acts);
+    c.matrix("x", x, rows, 2 * ff, x.scalar_type());
+    if (q.defined()) c.matrix("out", q, rows, ff, at::kChar);
+    if (s.defined()) c.vector("scales", s, rows, at::kFloat);
+    c.together(x, q, s);
+    int64_t ldq = up16(ff);
+    if (q.defined()) ldq = ld(q);
+    if (!q.defined()) {
+        q = c.empty({rows, ldq}, at::kChar);
+        if (ldq != ff) q = q.narrow(1, 0, ff);
+    }
+    if (!s.defined()) s = c.empty({rows}, at::kFloat);
+    check(E.glu_q8(c.device.index(), c.stream(), t, act, ptr(x), ld(x), (int8_t*)ptr(q), ldq, (float*)ptr(s), rows, ff));
+    return give(q, s);
+}
+
+PyObject* add_gated_norm_q8(PyObject* const* args, Py_ssize_t n) {
+    Call c("add_gated_norm_q8", args, n, 11);
+    const Tensor y = c.tensor(0, "y"), res = c.tensor(1, "residual"), w = c.maybe(2, "weight"), mix = c.maybe(4, "mix"), post = c.maybe(5, "post_weight"), gate = c.maybe(6, "gate");
+    Tensor sum = c.maybe(8, "sum_out"), q = c.maybe(9, "out"), s = c.maybe(10, "scales");
+    const double eps = c.number(3), scale = c.number(7);
+    if (res.dim() != 2) refuse(B200_ERR_SHAPE_MISMATCH, c.op, "residual: expected [rows, hidden], got " + sizes(res));
+    const int64_t rows = res.size(0), hidden = res.size(1);
+    const at::ScalarType dt = res.scalar_type();
+    b200_gated_norm a{};
+    a.type = c.type(dt);
+    int64_t top = 1;
+    if (mix.defined()) {
+        if (mix.dim() != 2 || mix.size(1) < 1 || mix.size(1) > 32) refuse(B200_ERR_SHAPE_MISMATCH, c.op, "mix: expected [rows, 1 to 32], got " + sizes(mix));
+        top = mix.size(1);
+        c.whole("mix", mix, rows, top, at::kFloat);
+    }
+    c.matrix("residual", res, rows, hidden, dt);
+    c.matrix("y", y, rows * top, hidden, dt);
+    if (post.defined()) c.vector("post_weight", post, hidden, at::kFloat);
+    if (w.defined()) c.vector("weight", w, hidden, at::kFloat);
+    else if (q.defined() || s.defined()) refuse(B200_ERR_INVALID_ARGUMENT, c.op, "out or scales without a weight");
+    if (gate.defined()) {
+        c.typed("gate", gate, dt);
+        if (gate.dim() != 2 || (gate.size(0) != rows && gate.size(0) != 1) || (gate.size(1) != hidden && gate.size(1) != 1))
+            refuse(B200_ERR_SHAPE_MISMATCH, c.op, "gate: expected [rows or 1, hidden or 1], got " + sizes(gate));
+    }
+    if (sum.defined()) c.matrix("sum_out", sum, rows, hidden, dt);
+    if (q.defined()) c.matrix("out", q, rows, hidden, at::kChar);
+    if (s.defined()) c.vector("scales", s, rows, at::kFloat);
+    c.together(res, y, w, mix, post, gate, sum, q, s);
+    int64_t ldq = up16(hidden);
+    if (q.defined()) ldq = ld(q);
+    if (w.defined() && !q.defined()) {
+        q = c.empty({rows, ldq}, at::kChar);
+        if (ldq != hidden) q = q.narrow(1, 0, hidden);
+    }
+    if (w.defined() && !s.defined()) s = c.empty({rows}, at::kFloat);
+    if (!sum.defined()) sum = c.empty({rows, hidden}, dt);
+    a.device = c.device.index();
+    a.stream = c.stream();
+    a.y = ptr(y);
+    a.ldy = ld(y);
+    a.mix = (const float*)ptr(mix);
+    a.top = (int32_t)top;
+    a.post_weight = (const float*)ptr(post);
+    if (gate.defined()) {
+        a.gate = ptr(gate);
+        a.gate_row = gate.size(0) > 1 ? gate.stride(0) : 0;
+        a.gate_col = gate.size(1) > 1 ? gate.stride(1) : 0;
+    }
+    a.residual = ptr(res);
+    a.ldr = ld(res);
+    a.sum = ptr(sum);
+    a.lds = ld(sum);
+    a.weight = (const float*)ptr(w);
+    a.q = (int8_t*)ptr(q);
+    a.ldq = ldq;
+    a.scales = (float*)ptr(s);
+    a.rows = rows;
+    a.hidden = hidden;
+    a.scale = (float)scale;
+    a.eps = (float)eps;
+    check(E.add_gated_norm_q8(&a));
+    PyObject* r = PyTuple_New(3);
+    if (!r) throw PythonError{};
+    PyTuple_SET_ITEM(r, 0, give(q));
+    PyTuple_SET_ITEM(r, 1, give(s));
+    PyTuple_SET_ITEM(r, 2, give(sum));
+    return r;
+}
+
 PyObject* rope_append_q4(PyObject* const* args, Py_ssize_t n) {
     Call c("rope_append_q4", args, n, 10);
     const Tensor q = c.maybe(0, "q"), k = c.tensor(1, "k"), v = c.tensor(2, "v"), table = c.tensor(3, "cos_sin"), pos = c.tensor(4, "positions"), pages = c.tensor(5, "pages"), slots = c.tensor(6, "slots");
@@ -285,9 +507,7 @@ PyObject* rope_append_q4(PyObject* const* args, Py_ssize_t n) {
     a.slots = (const int64_t*)ptr(slots);
     a.tokens = tokens;
     a.rot_dims = (int32_t)table.size(1);
-    const int neox = PyObject_IsTrue(args[7]);
-    if (neox < 0) throw PythonError{};
-    a.use_neox = neox;
+    a.use_neox = c.flag(7);
     a.status = c.status(9);
     check(E.rope_append_q4(&a));
     return give(out);
@@ -401,7 +621,8 @@ PyObject* bind(PyObject*, PyObject* args) {
         return to != nullptr;
     };
     if (!take("b200_last_error", E.last_error) || !take("b200_dev_add_rms_norm_q8", E.add_rms_norm_q8) || !take("b200_dev_read_q8", E.read_q8) || !take("b200_dev_mat_mat_i8", E.mat_mat_i8) ||
-        !take("b200_dev_rope_append_q4", E.rope_append_q4) || !take("b200_dev_read_q4", E.read_q4) || !take("b200_dev_attention_paged_q4_workspace", E.attention_workspace) ||
+        !take("b200_dev_route_experts", E.route_experts) || !take("b200_dev_mat_mat_i4", E.mat_mat_i4) || !take("b200_dev_glu_q8", E.glu_q8) ||
+        !take("b200_dev_add_gated_norm_q8", E.add_gated_norm_q8) || !take("b200_dev_rope_append_q4", E.rope_append_q4) || !take("b200_dev_read_q4", E.read_q4) || !take("b200_dev_attention_paged_q4_workspace", E.attention_workspace) ||
         !take("b200_dev_attention_paged_q4", E.attention)) {
         if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: null address");
         return nullptr;
@@ -410,7 +631,8 @@ PyObject* bind(PyObject*, PyObject* args) {
 }
 
 #define FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<f>)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(add_rms_norm_q8), FAST(read_q8), FAST(mat_mat_i8), FAST(rope_append_q4), FAST(read_q4), FAST(attention_paged_q4), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(add_rms_norm_q8), FAST(read_q8), FAST(mat_mat_i8), FAST(route_experts), FAST(mat_mat_i4), FAST(glu_q8), FAST(add_gated_norm_q8),
+                         FAST(rope_append_q4), FAST(read_q4), FAST(attention_paged_q4), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_device_ops", "device_ops.py's calls", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -19,9 +19,9 @@ import os
 
 import torch
 
-from . import _HERE, _STATUS, NotAvailable, _check, lib
+from . import _HERE, _STATUS, DTypeMismatch, NotAvailable, ShapeMismatch, _check, lib
 
-STATUS_BAD_SLOT, STATUS_BAD_POSITION, STATUS_BAD_PAGE, STATUS_BAD_LENGTH = 1, 2, 4, 8
+STATUS_BAD_SLOT, STATUS_BAD_POSITION, STATUS_BAD_PAGE, STATUS_BAD_LENGTH, STATUS_BAD_EXPERT = 1, 2, 4, 8, 16
 
 
 class Q4Pages(C.Structure):
@@ -46,6 +46,26 @@ class Q4Attention(C.Structure):
                    ("cache", Q4Pages), ("status", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)])
 
 
+class Route(C.Structure):
+    """b200_route"""
+    _fields_ = ([("device", C.c_int32), ("type", C.c_uint32), ("stream", C.c_void_p), ("logits", C.c_void_p), ("ld", C.c_int64), ("tokens", C.c_int64)]
+                + [(n, C.c_int32) for n in ("n", "top", "groups", "top_groups", "sigmoid", "renormalise")]
+                + [("scale", C.c_float), ("correction", C.c_void_p), ("experts", C.c_void_p), ("weights", C.c_void_p)])
+
+
+class I4Product(C.Structure):
+    """b200_i4_product"""
+    _fields_ = ([("device", C.c_int32), ("out_type", C.c_uint32), ("scale_type", C.c_uint32), ("group", C.c_int32), ("stream", C.c_void_p), ("a", C.c_void_p), ("lda", C.c_int64)]
+                + [(n, C.c_void_p) for n in ("a_scales", "w", "w_scales", "bias", "out")] + [(n, C.c_int64) for n in ("ldo", "tokens", "k", "n")]
+                + [("experts", C.c_void_p), ("top", C.c_int32), ("n_experts", C.c_int32), ("rows_per_pair", C.c_int32), ("status", C.c_void_p)])
+
+
+class GatedNorm(C.Structure):
+    """b200_gated_norm"""
+    _fields_ = ([("device", C.c_int32), ("type", C.c_uint32)] + [(n, C.c_void_p) for n in ("stream", "y", "mix", "post_weight", "gate", "residual", "sum", "weight", "q", "scales")]
+                + [(n, C.c_int64) for n in ("ldy", "gate_row", "gate_col", "ldr", "lds", "ldq", "rows", "hidden")] + [("top", C.c_int32), ("scale", C.c_float), ("eps", C.c_float)])
+
+
 _library = None
 _calls = None
 
@@ -59,6 +79,10 @@ def _lib():
         L.b200_dev_add_rms_norm_q8.argtypes = [C.c_int, vp, C.c_uint32, vp, i64, vp, i64, vp, i64, vp, C.c_float, vp, i64, vp, i64, i64]
         L.b200_dev_read_q8.argtypes = [C.c_int, vp, C.c_uint32, vp, i64, vp, vp, i64, i64, i64]
         L.b200_dev_mat_mat_i8.argtypes = [C.c_int, vp, C.c_uint32, vp, i64, vp, vp, i64, vp, vp, vp, i64, i64, i64, i64]
+        L.b200_dev_route_experts.argtypes = [C.POINTER(Route)]
+        L.b200_dev_mat_mat_i4.argtypes = [C.POINTER(I4Product)]
+        L.b200_dev_glu_q8.argtypes = [C.c_int, vp, C.c_uint32, C.c_int, vp, i64, vp, i64, vp, i64, i64]
+        L.b200_dev_add_gated_norm_q8.argtypes = [C.POINTER(GatedNorm)]
         L.b200_dev_rope_append_q4.argtypes = [C.POINTER(Q4Append)]
         L.b200_dev_read_q4.argtypes = [C.c_int, vp, C.c_uint32, C.POINTER(Q4Pages), vp, i64, vp, vp, vp]
         L.b200_dev_attention_paged_q4_workspace.argtypes = [C.POINTER(Q4Attention), sp]
@@ -80,7 +104,8 @@ def _ops():
         spec = importlib.util.spec_from_file_location("_device_ops", path)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
-        names = ("b200_last_error", "b200_dev_add_rms_norm_q8", "b200_dev_read_q8", "b200_dev_mat_mat_i8", "b200_dev_rope_append_q4", "b200_dev_read_q4",
+        names = ("b200_last_error", "b200_dev_add_rms_norm_q8", "b200_dev_read_q8", "b200_dev_mat_mat_i8", "b200_dev_route_experts", "b200_dev_mat_mat_i4", "b200_dev_glu_q8",
+                 "b200_dev_add_gated_norm_q8", "b200_dev_rope_append_q4", "b200_dev_read_q4",
                  "b200_dev_attention_paged_q4_workspace", "b200_dev_attention_paged_q4")
         mod.bind(_STATUS, {n: C.cast(getattr(L, n), C.c_void_p).value for n in names})
         _calls = mod
@@ -123,6 +148,84 @@ def mat_mat_i8(a, a_scales, w, w_scales, bias=None, dtype=torch.bfloat16, out=No
 
     The sums are exact (k <= 131071).  a and w start on 16 bytes with rows a multiple of 16 bytes apart (padded_rows)."""
     return _ops().mat_mat_i8(a, a_scales, w, w_scales, bias, dtype, out)
+
+
+def i4_weights(values, scales):
+    """(w, w_scales) of mat_mat_i4: values int8 [.., n, k] from -8 to 7 and scales [.., n, k / group] (f32, f16 or bf16; group 32, 64 or 128) as b200_i4_product lays them out.
+
+    What mat_mat_i4 multiplies with is scale * value.  Leading dimensions (experts) stay; rows behind n and channels behind k become zeros."""
+    if values.dtype != torch.int8:
+        raise DTypeMismatch(f"i4_weights: values: expected torch.int8, got {values.dtype}")
+    if values.dim() < 2 or scales.shape[:-1] != values.shape[:-1] or scales.shape[-1] < 1 or values.shape[-1] % scales.shape[-1]:
+        raise ShapeMismatch(f"i4_weights: expected [.., n, k] and [.., n, k / group], got {list(values.shape)} and {list(scales.shape)}")
+    *lead, n, k = values.shape
+    down, right = -n % 16, -k % 64
+    v = (torch.nn.functional.pad(values, (0, right, 0, down)) & 15).view(torch.uint8).unflatten(-1, (-1, 2, 4, 2, 4)).unflatten(-6, (-1, 2, 8))
+    d = len(lead)
+    v = v.permute(*range(d), *(d + i for i in (0, 3, 2, 5, 4, 1, 6, 7)))      # row tile, step, g, t, half, row half, (low, high), byte
+    s = torch.nn.functional.pad(scales, (0, 0, 0, down)).unflatten(-2, (-1, 2, 8)).movedim(-1, -3).transpose(-1, -2)
+    return (v[..., 0, :] | v[..., 1, :] << 4).flatten(d + 2), s.contiguous()
+
+
+def read_i4(w, w_scales, n, k):
+    """[.., n, k] f32: the values that weights of mat_mat_i4 stand for."""
+    d = w.dim() - 3
+    b = w.unflatten(-1, (8, 4, 2, 2, 4))
+    v = (torch.stack([b << 4, b & 240], -2).view(torch.int8) >> 4).permute(*range(d), *(d + i for i in (0, 5, 2, 1, 4, 3, 6, 7))).flatten(d + 3).flatten(d, d + 2)[..., :n, :k].float()
+    s = w_scales.float().transpose(-1, -2).movedim(-3, -1).flatten(d, d + 2)[..., :n, :]
+    return (v.unflatten(-1, (s.shape[-1], -1)) * s[..., None]).flatten(-2)
+
+
+def quantise_i4(x, group=32, dtype=torch.float16):
+    """(w, w_scales) of mat_mat_i4 for weights x [.., n, k]: a group's scale is its value of the largest magnitude / -8 in `dtype`, as a Q4_0 block's is, and the values round(x / scale)."""
+    if group not in (32, 64, 128) or x.dim() < 2 or x.shape[-1] % group:
+        raise ShapeMismatch(f"quantise_i4: expected [.., n, a multiple of the group], groups of 32, 64 or 128, got {list(x.shape)} and {group}")
+    g = x.float().unflatten(-1, (-1, group))
+    top = g.gather(-1, g.abs().argmax(-1, keepdim=True))
+    d = (top / -8).to(dtype)
+    v = torch.where(d == 0, 0.0, g / torch.where(d == 0, 1.0, d.float())).round_().clamp_(-8, 7)
+    return i4_weights(v.to(torch.int8).flatten(-2), d[..., 0])
+
+
+def i4_from_q4_0(blocks, k):
+    """(w, w_scales) of mat_mat_i4 for rows of GGUF Q4_0 blocks, uint8 [.., n, k / 32 * 18]: the same values, groups of 32 with f16 scales."""
+    if blocks.dtype != torch.uint8 or blocks.dim() < 2 or k % 32 or blocks.shape[-1] != k // 32 * 18:
+        raise ShapeMismatch(f"i4_from_q4_0: expected uint8 [.., n, {k // 32 * 18}], got {blocks.dtype} {list(blocks.shape)}")
+    b = blocks.unflatten(-1, (-1, 18))
+    v = torch.cat([b[..., 2:] & 15, b[..., 2:] >> 4], -1).to(torch.int8) - 8
+    return i4_weights(v.flatten(-2), b[..., :2].contiguous().view(torch.float16)[..., 0])
+
+
+def mat_mat_i4(a, a_scales, w, w_scales, n=None, experts=None, bias=None, dtype=torch.bfloat16, out=None, status=None):
+    """a [t, k] int8 (a scale per row) times 4-bit weights (a scale per row and group of channels) -> [t, n] of `dtype` (of `out` where that is given), plus bias [n] f32.
+
+    w, w_scales: i4_weights, quantise_i4 or i4_from_q4_0 make them; n None: all rows of their tiles.  experts int32 [tokens, top] (route_experts): w, w_scales and bias have a leading dimension of
+    experts, and the result [tokens * top, n] has a row for each of a token's experts; a has a row per token, or [tokens * top] rows, one for each.  Pairs of expert -1 get zeros, other numbers that
+    are no expert too (and set STATUS_BAD_EXPERT).  The sums of a group are exact.  a starts on 16 bytes with rows a multiple of 16 bytes apart (padded_rows).  For few rows: the weights'
+    bytes are what it costs, once for every 64 rows of a matrix."""
+    return _ops().mat_mat_i4(a, a_scales, w, w_scales, n, experts, bias, dtype, out, status)
+
+
+def route_experts(logits, top, score="softmax", correction=None, groups=1, top_groups=1, renormalise=True, scale=1.0, experts=None, weights=None):
+    """(experts int32, weights f32) [tokens, top]: each token's experts by its router logits [tokens, n] (f32, f16 or bf16, contiguous rows), best first, the lower number among equals.
+
+    The scores p are the softmax over all experts or (score="sigmoid") 1 / (1 + exp(-logit)); the choice goes by the logits, or by p + correction [n] f32 (a bias for balance, which the weights do not
+    have).  groups > 1: of that many groups of neighbours only the best top_groups are left, by the sum of their two best scores.  weights: p, with renormalise over the chosen ones' sum, times scale.
+    Logits of -inf (or NaN) are not chosen; places that nothing is left for hold expert -1 with weight 0, so that a row of -inf is a place without a token.  A row with a NaN has weights NaN."""
+    return _ops().route_experts(logits, top, score, correction, groups, top_groups, renormalise, scale, experts, weights)
+
+
+def glu_q8(x, act="silu", out=None, scales=None):
+    """(q, scales): q [rows, ff] int8 and scales [rows] f32 with q * scales = act(x[:, :ff]) * x[:, ff:]; act silu, gelu (tanh form) or relu.  x: [rows, 2 ff] f32, f16 or bf16 with contiguous rows."""
+    return _ops().glu_q8(x, act, out, scales)
+
+
+def add_gated_norm_q8(y, residual, weight, eps, mix=None, post_weight=None, gate=None, scale=1.0, sum_out=None, out=None, scales=None):
+    """(q, scales, r): r = residual + scale * gate * p in their type; q [rows, hidden] int8 and scales [rows] f32 with q * scales = the RMS norm of r times weight (weight None: both None).
+
+    p is the block's output y [rows, hidden], or with mix f32 [rows, top] the sum of each row's `top` rows of y [rows * top, hidden] by those weights (route_experts' and mat_mat_i4's); with
+    post_weight f32 [hidden] its RMS norm times that.  gate: of y's type, [rows, hidden], or 1 in place of either (broadcast).  sum_out may be residual itself."""
+    return _ops().add_gated_norm_q8(y, residual, weight, eps, mix, post_weight, gate, scale, sum_out, out, scales)
 
 
 def q4_pages(n_pages, n_kv_heads, head_dim, page_size, device="cuda"):
