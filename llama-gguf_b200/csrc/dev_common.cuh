@@ -67,6 +67,28 @@ __device__ __forceinline__ Q4Block q4_block(const b200_q4_pages& c, int64_t page
     return Q4Block{p, p + rows, reinterpret_cast<const float*>(p + 2 * rows), reinterpret_cast<const float*>(p + 2 * rows) + c.page_size};
 }
 
+// Clusters: barriers, and what lies in another block's shared memory
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
+    uint32_t p;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
+    return p;
+}
+__device__ __forceinline__ int peer_s32(uint32_t addr, uint32_t rank) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at_rank(addr, rank)));      // (behind a barrier: nothing to be ordered with)
+    return v;
+}
+__device__ __forceinline__ float peer_f32(uint32_t addr, uint32_t rank) { return __int_as_float(peer_s32(addr, rank)); }
+
 // Programmatic launches: a kernel may be scheduled while the one before it on the stream ends.  Every block of every kernel here calls before() first thing, ahead of any access to global memory (it
 // returns when all that came before is done and visible), and so no kernel can end before its predecessors have.
 __device__ __forceinline__ void before() {

@@ -56,6 +56,7 @@ extern "C" int b200_dev_mat_mat_i4(const b200_i4_product* a) {
         m.lda = a->lda;
         m.ldo = a->ldo;
         m.rows = (int)(a->tokens * (a->experts ? a->top : 1));
+        m.tokens = (int)a->tokens;
         m.k = (int)a->k;
         m.n = (int)a->n;
         m.div = a->experts && !a->rows_per_pair ? a->top : 1;

@@ -191,13 +191,16 @@ def test_product_of_rows_apart_and_into_tensors(D):
 
 
 def test_product_of_a_row_is_the_same_among_others(D):
-    """A row's result does not depend on the rows beside it as long as the call takes the same kernel."""
+    """A row's result does not depend on what is in the rows beside it, nor on its place (another number of rows may be another kernel, whose sums have another order)."""
     values, scales = four_bits(1, 70, 1024), (0.01 * normal(2, 70, 32)).half()
     w, ws = (v.cuda() for v in D.i4_weights(values, scales))
-    a = bytes_of(3, 8, 1024)
-    whole = D.mat_mat_i4(a, torch.ones(8).cuda(), w, ws, dtype=torch.float32)
-    for i in range(8):
-        assert torch.equal(D.mat_mat_i4(a[i : i + 1].contiguous(), torch.ones(1).cuda(), w, ws, dtype=torch.float32), whole[i : i + 1])
+    for rows in (2, 4, 8, 16, 32, 64):
+        a = bytes_of(3, rows, 1024)
+        whole = D.mat_mat_i4(a, torch.ones(rows).cuda(), w, ws, dtype=torch.float32)
+        for i in (0, rows // 2, rows - 1):
+            b = bytes_of(4 + i, rows, 1024)
+            b[rows - 1 - i] = a[i]
+            assert torch.equal(D.mat_mat_i4(b, torch.ones(rows).cuda(), w, ws, dtype=torch.float32)[rows - 1 - i], whole[i])
 
 
 def chosen(seed, tokens, top, n, empty=0.0):
