@@ -7,13 +7,12 @@
 // halves of its bytes and the next four in the high halves; (word << 4) & 0xf0f0f0f0 and word & 0xf0f0f0f0 are those values times sixteen as signed bytes, three instructions for eight weights.  Eight rows of a are
 // the columns.  Sums begin at the bits of 1.5 * 2^23, so that read as f32 they are that plus the sum (|16 sum| <= 2^21).
 //
-// Work.  A unit is R tiles of weight rows and up to 8 NT rows of a; its channels go 128 at a time (a step: two tiles, a whole number of groups).  Each lane copies the bytes that it will read itself into a
-// ring of its warp (cp.async), some steps ahead, so that no warp waits for another.  With experts every block lists the pairs (token, expert) by expert first, all in the same order; a chunk of up to
-// 8 NT pairs of an expert is a unit for each R tiles.
-//   few rows (NT 1 or 2, R 1): the weights' bytes.  A block per SM has consecutive units; its warps share their steps evenly, whichever unit they are of, and leave the sums of a unit that two or more warps have a part of in
-//   shared memory for the end.  Rows of a come from L1.
-//   more rows (NT 4 or 8, R 4): rows of a cost as much as weights.  A block's warps share a unit's steps, with clusters the blocks of one too; the rows' bytes go through the ring with the weights', and
-//   serve four tiles.
+// Work.  A unit is one or four tiles of weight rows and as many rows of a as the kernel takes at once.  Each lane copies the bytes that it will read itself into a ring in shared memory (cp.async), some steps ahead, so that no warp waits
+// for another's weights.  With experts every block lists the pairs (token, expert) by expert first, all in the same order; up to that many pairs of an expert are a unit for each tile.
+//   few rows (up to 16): the weights' bytes.  A block per SM has consecutive units of one tile; its warps share their steps of 256 channels evenly, whichever unit they are of, and leave the sums of a unit that two or
+//   more warps have a part of in shared memory for the end.  Rows of a come from L1 and L2.
+//   more rows (up to 64 at a time): rows of a cost as much as weights.  A block's sixteen warps have four tiles and a step of 512 channels, a quarter of it each; the rows' bytes go through the ring with the
+//   weights' and serve the four tiles.  With few units the blocks of a cluster share the channels of one.
 #pragma once
 #include <algorithm>
 #include <cmath>
@@ -158,42 +157,102 @@ template <typename S> __device__ __forceinline__ float2 i4_scales(const uint8_t*
     const W w = *reinterpret_cast<const W*>(p);
     return make_float2(to_f(w.lo), to_f(w.hi));
 }
-// What a ring holds of a step (C tiles' channels of R tiles of rows): the weights of each, then the groups' scales of each.
-template <typename S, int GROUP, int R, int C> __host__ __device__ constexpr int i4_slot() { return R * (C * I4_TILE + 16 * (int)sizeof(S) * (64 * C / GROUP)); }
-// ... copied: step s of R tiles from `tile` on, whose weights and scales are at w and d
-template <typename S, int GROUP, int R, int C> __device__ __forceinline__ void i4_copy(const MatI4Args& a, uint32_t to, const uint8_t* w, const uint8_t* d, int tile, int s, int lane) {
+// What a ring holds of a step of C tiles' channels of one tile of rows: the weights, then the groups' scales.
+template <typename S, int GROUP, int C> __host__ __device__ constexpr int i4_slot() { return C * I4_TILE + 16 * (int)sizeof(S) * (64 * C / GROUP); }
+// ... copied: step s of the tile whose weights and scales are at w and d
+template <typename S, int GROUP, int C> __device__ __forceinline__ void i4_copy(const MatI4Args& a, uint32_t to, const uint8_t* w, const uint8_t* d, int s, int lane) {
     constexpr int GS = 64 * C / GROUP, SB = 16 * (int)sizeof(S), WORDS = GS * SB / 8;
     const uint8_t *p = w + (int64_t)s * (C * I4_TILE) + lane * 16, *q = d + (int64_t)s * (GS * SB) + lane * 8;
-    const int room = a.steps - s * C, scales = (a.groups - s * GS) * (SB / 8);      // tiles of the step, and 8-byte words of its scales
+    to += lane * 16;
+    if ((s + 1) * C <= a.steps && (s + 1) * GS <= a.groups) {
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        const bool in = R == 1 || tile + r < a.tiles;
-#pragma unroll
-        for (int c = 0; c < C; c++) copy_where<16>(to + (r * C + c) * I4_TILE + lane * 16, in && c < room ? p + c * I4_TILE : a.w, in && c < room);
+        for (int c = 0; c < C; c++) copy_where<16>(to + c * I4_TILE, p + c * I4_TILE, true);
 #pragma unroll
         for (int c = 0; c < WORDS; c += 32)
-            if (c + 32 <= WORDS || lane < WORDS - c) {
-                const bool there = in && c + lane < scales;
-                copy_where<8>(to + R * C * I4_TILE + r * GS * SB + c * 8 + lane * 8, there ? q + c * 8 : a.w, there);
-            }
-        p += (int64_t)a.steps * I4_TILE;
-        q += (int64_t)a.groups * SB;
+            if (c + 32 <= WORDS || lane < WORDS - c) copy_where<8>(to - lane * 8 + C * I4_TILE + c * 8, q + c * 8, true);
+    } else {      // (the last step: zeros behind the last channel)
+        const int room = a.steps - s * C, scales = (a.groups - s * GS) * (SB / 8);      // tiles, and 8-byte words of the scales
+#pragma unroll
+        for (int c = 0; c < C; c++) copy_where<16>(to + c * I4_TILE, c < room ? p + c * I4_TILE : a.w, c < room);
+#pragma unroll
+        for (int c = 0; c < WORDS; c += 32)
+            if (c + 32 <= WORDS || lane < WORDS - c) copy_where<8>(to - lane * 8 + C * I4_TILE + c * 8, c + lane < scales ? q + c * 8 : a.w, c + lane < scales);
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------- few rows
-// TC rows of a are TC of the eight columns; with fewer than eight the other columns take the same rows' other groups: column n has row n % TC and group n / TC of the (up to) 8 / TC that one set of sums
-// has, so that what a group's sum costs afterwards (a subtraction and a multiplication in each lane) is paid once for all of them.  (One row in all columns took 240 instructions for 128 channels.)
-// NT > 1: TC = 8, and that many times eight columns.
+// A step's sums of one tile with TC rows of a (1, 2, 4; 8: eight rows each in NT blocks of columns).  TC rows are TC of the eight columns; with fewer than eight the other columns take the same rows' other
+// groups: column n has row n % TC and group n / TC of the (up to) 8 / TC that one set of sums has, so that what a group's sum costs afterwards (a subtraction and a multiplication in each lane) is paid once for all
+// of them.  (One row in one column took 240 instructions for 128 channels.)
+template <typename S, int GROUP, int TC, int NT> struct I4Step {
+    static constexpr int GC = GROUP / 32, GS = 256 / GROUP, SETS = GS * TC > 8 ? GS * TC / 8 : 1, PER = GS / SETS;      // chunks (of 32 channels) of a group, groups of a step, sets of sums, groups of a set
+    static constexpr int SB = 16 * (int)sizeof(S);
+    uint2 b[NT][SETS * GC];
+    // this lane's bytes of the rows; `at`: row g % TC, channel 8 t; columns that no group has, and channels behind the last one, are zeros
+    __device__ __forceinline__ void load(const int8_t* const (&at)[NT], int s, int k, int g) {
+        const int group = g / TC, from = s * 256 + group * GROUP;
+        const bool used = PER * TC == 8 || group < PER;
+        if ((s + 1) * 256 <= k) {
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int i = 0; i < SETS * GC; i++) b[j][i] = used ? *reinterpret_cast<const uint2*>(at[j] + from + i / GC * PER * GROUP + i % GC * 32) : make_uint2(0, 0);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int i = 0; i < SETS * GC; i++) {
+                    const int ch = from + i / GC * PER * GROUP + i % GC * 32;
+                    b[j][i] = used && ch < k ? *reinterpret_cast<const uint2*>(at[j] + ch) : make_uint2(0, 0);
+                }
+        }
+    }
+    __device__ __forceinline__ void add(float (&acc)[NT][4], const uint8_t* in, int lane) const {
+        const int g = lane >> 2, t = lane & 3, group = g / TC;
+        const uint8_t* scales = in + 4 * I4_TILE + g * 2 * sizeof(S);
+#pragma unroll
+        for (int z = 0; z < SETS; z++) {
+            int sum[NT][4];
+#pragma unroll
+            for (int i = 0; i < PER * GC; i++) {
+                const int k = z * PER * GC + i;      // the chunk: half a tile
+                const uint2 v = *reinterpret_cast<const uint2*>(in + (k / 2) * I4_TILE + lane * 16 + (k % 2) * 8);
+                const uint32_t a0 = (v.x << 4) & 0xf0f0f0f0u, a1 = (v.y << 4) & 0xf0f0f0f0u, a2 = v.x & 0xf0f0f0f0u, a3 = v.y & 0xf0f0f0f0u;
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    const uint2 w = b[j][z * GC + i % GC];
+                    const uint32_t b0 = PER == 1 || group == i / GC ? w.x : 0, b1 = PER == 1 || group == i / GC ? w.y : 0;
+                    if (i == 0) mma_s8_first(sum[j], a0, a1, a2, a3, b0, b1);
+                    else mma_s8(sum[j], a0, a1, a2, a3, b0, b1);
+                }
+            }
+            // columns 2t and 2t + 1: one group's, but for TC = 1
+            const int q0 = 2 * t / TC, q1 = (2 * t + 1) / TC;
+            float2 d0 = i4_scales<S>(scales + (z * PER + (PER > 1 ? min(q0, PER - 1) : 0)) * SB), d1 = d0;
+            if constexpr (TC == 1) d1 = i4_scales<S>(scales + (z * PER + (PER > 1 ? min(q1, PER - 1) : 0)) * SB);
+            if constexpr (PER * TC < 8) {      // (columns that no group has)
+                if (q0 >= PER) d0 = make_float2(0, 0);
+                if (q1 >= PER) d1 = make_float2(0, 0);
+            }
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                acc[j][0] = fmaf(d0.x, i4_sum(sum[j][0]), acc[j][0]);
+                acc[j][1] = fmaf(d1.x, i4_sum(sum[j][1]), acc[j][1]);
+                acc[j][2] = fmaf(d0.y, i4_sum(sum[j][2]), acc[j][2]);
+                acc[j][3] = fmaf(d1.y, i4_sum(sum[j][3]), acc[j][3]);
+            }
+        }
+    }
+};
+
 template <int NT> __host__ __device__ constexpr int i4_few_warps() { return NT == 1 ? 24 : 16; }
-template <typename S, int GROUP, int TC, int NT> __global__ void __launch_bounds__(i4_few_warps<NT>() * 32, 1) mat_mat_i4_few_kernel(const MatI4Args a) {
+template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_few_warps<NT>() * 32, 1) mat_mat_i4_few_kernel(const MatI4Args a) {
     before();
-    constexpr int C = 4, SLOT = i4_slot<S, GROUP, 1, C>(), SB = 16 * (int)sizeof(S), CHUNK = TC * NT, WARPS = i4_few_warps<NT>();
-    constexpr int GC = GROUP / 32, GS = 256 / GROUP, SETS = GS * TC > 8 ? GS * TC / 8 : 1, PER = GS / SETS;      // chunks (of 32 channels) of a group, groups of a step, sets of sums, groups of a set
+    constexpr int SLOT = i4_slot<S, GROUP, 4>(), SB = 16 * (int)sizeof(S), CHUNK = 8 * NT, WARPS = i4_few_warps<NT>();
     extern __shared__ __align__(16) uint8_t i4_smem[];
     float4* parts = reinterpret_cast<float4*>(i4_smem + WARPS * I4_RING * SLOT);      // [warps][its first unit, its last][NT][32]
     const I4List l = i4_list(parts + WARPS * 2 * NT * 32, a);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, whole = (a.steps + C - 1) / C;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, whole = (a.steps + 3) / 4;
     const uint8_t* slots = i4_smem + warp * I4_RING * SLOT;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(slots);
     int chunks = (a.rows + CHUNK - 1) / CHUNK;
@@ -208,28 +267,32 @@ template <typename S, int GROUP, int TC, int NT> __global__ void __launch_bounds
     auto begin = [&](int w) { return (int)((int64_t)steps * w / WARPS); };
     // sums over a row's columns, and the results of a unit
     auto finish = [&](float4 (&y)[NT], const I4Chunk& x, int tile) {
+        const int tc = x.many > 4 ? 8 : x.many > 2 ? 4 : x.many;      // (columns of one row are 1, 2, 4 apart)
+        if (tc == 1) y[0].x += y[0].y, y[0].z += y[0].w;
+        if (tc < 4) {
+            y[0].x += __shfl_xor_sync(0xffffffffu, y[0].x, 1);
+            y[0].y += __shfl_xor_sync(0xffffffffu, y[0].y, 1);
+            y[0].z += __shfl_xor_sync(0xffffffffu, y[0].z, 1);
+            y[0].w += __shfl_xor_sync(0xffffffffu, y[0].w, 1);
+        }
+        if (tc < 8) {
+            y[0].x += __shfl_xor_sync(0xffffffffu, y[0].x, 2);
+            y[0].y += __shfl_xor_sync(0xffffffffu, y[0].y, 2);
+            y[0].z += __shfl_xor_sync(0xffffffffu, y[0].z, 2);
+            y[0].w += __shfl_xor_sync(0xffffffffu, y[0].w, 2);
+        }
+        const int n = tile * 16 + g;
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-            if constexpr (TC == 1) y[j].x += y[j].y, y[j].z += y[j].w;
-#pragma unroll
-            for (int o = TC == 4 ? 2 : 1; o < 4 && TC < 8; o <<= 1) {
-                y[j].x += __shfl_xor_sync(0xffffffffu, y[j].x, o);
-                y[j].z += __shfl_xor_sync(0xffffffffu, y[j].z, o);
-                if constexpr (TC > 1) {
-                    y[j].y += __shfl_xor_sync(0xffffffffu, y[j].y, o);
-                    y[j].w += __shfl_xor_sync(0xffffffffu, y[j].w, o);
-                }
-            }
+        for (int j = 0; j < NT; j++)
 #pragma unroll
             for (int q = 0; q < 2; q++) {
-                const int col = 8 * j + 2 * t + q, n = tile * 16 + g;
-                if (col < (TC < 8 ? min(TC, x.many) : x.many)) {
+                const int col = 8 * j + 2 * t + q;
+                if (col < x.many) {
                     const int p = i4_pair(a, l, x.lo + col);
                     if (n < a.n) i4_put(a, x.e, p, n, q ? y[j].y : y[j].x);
                     if (n + 8 < a.n) i4_put(a, x.e, p, n + 8, q ? y[j].w : y[j].z);
                 }
             }
-        }
     };
     const int f0 = begin(warp), f1 = begin(warp + 1);
     if (f0 < f1) {
@@ -247,7 +310,7 @@ template <typename S, int GROUP, int TC, int NT> __global__ void __launch_bounds
         place();
         auto copy = [&]() {
             if (left > 0) {
-                i4_copy<S, GROUP, 1, C>(a, ring + into * SLOT, cw, cd, ct, cs, lane);
+                i4_copy<S, GROUP, 4>(a, ring + into * SLOT, cw, cd, cs, lane);
                 into = into + 1 == I4_RING ? 0 : into + 1;
                 left--;
                 if (++cs == whole && left > 0) {
@@ -263,71 +326,36 @@ template <typename S, int GROUP, int TC, int NT> __global__ void __launch_bounds
         };
 #pragma unroll
         for (int i = 0; i < I4_RING - 1; i++) copy();
-        const int group = g / TC;      // this column's, of a set's
         int slot = 0;
         for (int f = f0; f < f1;) {
             const int sa = s, sb = min(whole, s + f1 - f);
             float acc[NT][4];
-            const int8_t* rows[NT];
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-                acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0;
-                // (columns without a row take another's: nothing reads their sums)
-                const int col = 8 * j + g % TC;
-                rows[j] = a.a + (int64_t)((a.first + i4_pair(a, l, x.lo + (col < x.many ? col : 0))) / a.div) * a.lda + group * GROUP + 8 * t;
-            }
-            for (; s < sb; s++) {
-                uint2 b[NT][SETS * GC];
-                const int room = a.k - s * 256 - group * GROUP;
+            for (int j = 0; j < NT; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0;
+            auto products = [&](auto step, auto& sums) {
+                constexpr int N = sizeof(sums) / sizeof(sums[0]);
+                const int tc = x.many > 4 ? 8 : x.many > 2 ? 4 : x.many;
+                const int8_t* at[N];
 #pragma unroll
-                for (int j = 0; j < NT; j++)
-#pragma unroll
-                    for (int z = 0; z < SETS; z++)
-#pragma unroll
-                        for (int h = 0; h < GC; h++)
-                            b[j][z * GC + h] = z * PER * GROUP + h * 32 < room && (PER * TC == 8 || group < PER) && (j == 0 || 8 * j < x.many)
-                                                   ? *reinterpret_cast<const uint2*>(rows[j] + s * 256 + z * PER * GROUP + h * 32) : make_uint2(0, 0);
-                asm volatile("cp.async.wait_group %0;" ::"n"(I4_RING - 2) : "memory");
-                __syncwarp();
-                const uint8_t *in = slots + slot * SLOT, *scales = in + C * I4_TILE + g * 2 * sizeof(S);
-                copy();
-                slot = slot + 1 == I4_RING ? 0 : slot + 1;
-#pragma unroll
-                for (int z = 0; z < SETS; z++) {
-                    int sum[NT][4];
-#pragma unroll
-                    for (int q = 0; q < PER; q++)
-#pragma unroll
-                        for (int h = 0; h < GC; h++) {
-                            const int k = (z * PER + q) * GC + h;      // the chunk: half a tile
-                            const uint2 v = *reinterpret_cast<const uint2*>(in + (k / 2) * I4_TILE + lane * 16 + (k % 2) * 8);
-                            const uint32_t a0 = (v.x << 4) & 0xf0f0f0f0u, a1 = (v.y << 4) & 0xf0f0f0f0u, a2 = v.x & 0xf0f0f0f0u, a3 = v.y & 0xf0f0f0f0u;
-#pragma unroll
-                            for (int j = 0; j < NT; j++) {
-                                if (j && 8 * j >= x.many) break;
-                                const uint32_t b0 = PER == 1 || group == q ? b[j][z * GC + h].x : 0, b1 = PER == 1 || group == q ? b[j][z * GC + h].y : 0;
-                                if (q == 0 && h == 0) mma_s8_first(sum[j], a0, a1, a2, a3, b0, b1);
-                                else mma_s8(sum[j], a0, a1, a2, a3, b0, b1);
-                            }
-                        }
-                    // columns 2t and 2t + 1: one group's, but for TC = 1
-                    const int q0 = 2 * t / TC, q1 = (2 * t + 1) / TC;
-                    float2 d0 = i4_scales<S>(scales + (z * PER + (PER > 1 ? min(q0, PER - 1) : 0)) * SB), d1 = d0;
-                    if constexpr (TC == 1) d1 = i4_scales<S>(scales + (z * PER + (PER > 1 ? min(q1, PER - 1) : 0)) * SB);
-                    if (PER * TC < 8) {      // (columns that no group has)
-                        if (q0 >= PER) d0 = make_float2(0, 0);
-                        if (q1 >= PER) d1 = make_float2(0, 0);
-                    }
-#pragma unroll
-                    for (int j = 0; j < NT; j++) {
-                        if (j && 8 * j >= x.many) break;
-                        acc[j][0] = fmaf(d0.x, i4_sum(sum[j][0]), acc[j][0]);
-                        acc[j][1] = fmaf(d1.x, i4_sum(sum[j][1]), acc[j][1]);
-                        acc[j][2] = fmaf(d0.y, i4_sum(sum[j][2]), acc[j][2]);
-                        acc[j][3] = fmaf(d1.y, i4_sum(sum[j][3]), acc[j][3]);
-                    }
+                for (int j = 0; j < N; j++) {
+                    const int col = 8 * j + (g & (tc - 1));      // (columns without a row take another's: nothing reads their sums)
+                    at[j] = a.a + (int64_t)((a.first + i4_pair(a, l, x.lo + (col < x.many ? col : 0))) / a.div) * a.lda + 8 * t;
                 }
-            }
+                for (; s < sb; s++) {
+                    step.load(at, s, a.k, g);
+                    asm volatile("cp.async.wait_group %0;" ::"n"(I4_RING - 2) : "memory");
+                    __syncwarp();
+                    copy();
+                    step.add(sums, slots + slot * SLOT, lane);
+                    slot = slot + 1 == I4_RING ? 0 : slot + 1;
+                }
+            };
+            auto& one = reinterpret_cast<float(&)[1][4]>(acc);
+            if (NT > 1 && x.many > 8) products(I4Step<S, GROUP, 8, NT>(), acc);
+            else if (x.many > 4) products(I4Step<S, GROUP, 8, 1>(), one);
+            else if (x.many > 2) products(I4Step<S, GROUP, 4, 1>(), one);
+            else if (x.many > 1) products(I4Step<S, GROUP, 2, 1>(), one);
+            else products(I4Step<S, GROUP, 1, 1>(), one);
             float4 y[NT];
 #pragma unroll
             for (int j = 0; j < NT; j++) y[j] = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
@@ -373,129 +401,107 @@ template <typename S, int GROUP, int TC, int NT> __global__ void __launch_bounds
 }
 
 // ------------------------------------------------------------------------------------------------------------- more rows
-// A block has four tiles of rows and its eight pairs of warps a part of the channels each: a pair's warps have two tiles each, and the same rows of a, which both copy a half of.
-enum { I4_PAIRS_OF_WARPS = 8, I4_R = 2 };
-template <typename S, int GROUP, int NT> __host__ __device__ constexpr int i4_many_slot() { return 2 * i4_slot<S, GROUP, I4_R, 2>() + NT * 8 * 128; }
-template <typename S, int GROUP, int NT> __host__ __device__ constexpr int i4_many_ring() {      // steps of a pair's ring: as many as fit a block's 227 KiB with the longest lists, up to four
-    const int fit = (int)(227 * 1024 - 1024 - i4_list_bytes(1024, I4_PAIRS)) / (I4_PAIRS_OF_WARPS * i4_many_slot<S, GROUP, NT>());
-    return fit < 4 ? fit : 4;
-}
-
-template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(I4_PAIRS_OF_WARPS * 64, 1) mat_mat_i4_many_kernel(const MatI4Args a) {
+enum { I4_MANY_WARPS = 16, I4_MANY_TILES = 4, I4_MANY_NT = 8, I4_MANY_RING = 4 };
+template <typename S, int GROUP> __host__ __device__ constexpr int i4_many_slot() { return I4_MANY_WARPS * i4_slot<S, GROUP, 2>() + I4_MANY_NT * 8 * 512; }
+// Warp w has tile w % 4 of the unit's and quarter w / 4 of a step.
+template <typename S, int GROUP> __global__ void __launch_bounds__(I4_MANY_WARPS * 32, 1) mat_mat_i4_many_kernel(const MatI4Args a) {
     before();
-    constexpr int R = I4_R, P = I4_PAIRS_OF_WARPS, RING = i4_many_ring<S, GROUP, NT>(), WSLOT = i4_slot<S, GROUP, R, 2>(), SLOT = i4_many_slot<S, GROUP, NT>(), GS = 128 / GROUP, SB = 16 * (int)sizeof(S),
-                  GC = GROUP / 32, J = NT < 4 ? NT : 4;
-    static_assert(RING >= 2 && RING * SLOT >= 2 * R * NT * 512, "a pair's sums take its ring's place");
+    constexpr int R = I4_MANY_TILES, NT = I4_MANY_NT, RING = I4_MANY_RING, WARPS = I4_MANY_WARPS, WSLOT = i4_slot<S, GROUP, 2>(), SLOT = i4_many_slot<S, GROUP>(), GS = 128 / GROUP, SB = 16 * (int)sizeof(S),
+                  GC = GROUP / 32;
     extern __shared__ __align__(16) uint8_t i4_smem[];
     __shared__ int64_t s_row[8 * NT];      // where the unit's rows of a begin
-    const I4List l = i4_list(i4_smem + P * RING * SLOT, a);
-    const int tid = threadIdx.x, lane = tid & 31, pair = tid >> 6, half = (tid >> 5) & 1, g = lane >> 2, t = lane & 3;
-    uint8_t* slots = i4_smem + pair * RING * SLOT;
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(slots);
-    const int blocks = (a.tiles + 2 * R - 1) / (2 * R), whole = (a.steps + 1) / 2;
+    const I4List l = i4_list(i4_smem + RING * SLOT, a);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, quarter = warp / R;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(i4_smem);
+    const int blocks = (a.tiles + R - 1) / R, whole = (a.steps + 7) / 8;
     int chunks = (a.rows + 8 * NT - 1) / (8 * NT);
     if (a.experts) {
         i4_lists(a, l, 8 * NT);
         chunks = l.chunk[a.n_experts];
         i4_zeros(a, l);
     }
-    const int rank = blockIdx.x % a.split, parts = P * a.split, part = rank * P + pair, s0 = (int)((int64_t)whole * part / parts), s1 = (int)((int64_t)whole * (part + 1) / parts);
-    auto together = [&] { asm volatile("bar.sync %0, 64;" ::"r"(pair + 1) : "memory"); };
+    const int rank = blockIdx.x % a.split, s0 = (int)((int64_t)whole * rank / a.split), s1 = (int)((int64_t)whole * (rank + 1) / a.split);
     for (int64_t u = blockIdx.x / a.split; u < (int64_t)chunks * blocks; u += gridDim.x / a.split) {
-        const int c = (int)(u / blocks), tile = (int)(u - (int64_t)c * blocks) * 2 * R + half * R;
+        const int c = (int)(u / blocks), tile0 = (int)(u - (int64_t)c * blocks) * R, tile = min(tile0 + warp % R, a.tiles - 1);      // (a warp without a tile takes another's: nothing reads its sums)
         const I4Chunk x = i4_chunk<8 * NT>(a, l, c);
-        if (tid < 8 * NT) s_row[tid] = tid < x.many ? (int64_t)((a.first + i4_pair(a, l, x.lo + tid)) / a.div) * a.lda : 0;
+        const int nt = (x.many + 7) / 8;
+        if (tid < 8 * NT) s_row[tid] = (int64_t)((a.first + i4_pair(a, l, x.lo + (tid < x.many ? tid : 0))) / a.div) * a.lda;
         __syncthreads();
         const int64_t at = (int64_t)x.e * a.tiles + tile;
         const uint8_t *w = a.w + at * a.steps * I4_TILE, *d = reinterpret_cast<const uint8_t*>(a.ws) + at * a.groups * SB;
-        // rows of 128 bytes; 16 bytes u of row i lie at u ^ (2 (i % 4)), so that the eight rows of a column block are read without bank conflicts
+        // rows of 128 bytes per quarter; 16 bytes u of row i lie at u ^ (2 (i % 4)), so that the eight rows of a block of columns are read without bank conflicts
         auto copy = [&](int s, int into) {
             if (s < s1) {
-                const int unit = lane & 7, ch = s * 128 + unit * 16;
-                const uint32_t to = ring + into * SLOT + 2 * WSLOT;
-#pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    const int row = i * 8 + half * 4 + (lane >> 3);
-                    if (i * 8 < x.many) {
-                        const bool there = row < x.many && ch < a.k;
-                        copy_where<16>(to + row * 128 + ((unit ^ ((row & 3) << 1)) << 4), there ? a.a + s_row[row] + ch : a.a, there);
-                    }
-                }
-                i4_copy<S, GROUP, R, 2>(a, ring + into * SLOT + half * WSLOT, w, d, tile, s, lane);
+                const int ch = s * 512 + lane * 16;
+                const uint32_t to = ring + into * SLOT + WARPS * WSLOT + (lane >> 3) * (NT * 8 * 128) + (((lane & 7) ^ ((warp & 3) << 1)) << 4);
+                const int8_t* from = a.a + ch;
+                for (int row = warp; row < nt * 8; row += WARPS) copy_where<16>(to + row * 128, ch < a.k ? from + s_row[row] : a.a, ch < a.k);
+                const int mine = s * 4 + quarter;
+                if (mine * 2 < a.steps) i4_copy<S, GROUP, 2>(a, ring + into * SLOT + warp * WSLOT, w, d, mine, lane);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
         for (int i = 0; i < RING - 1; i++) copy(s0 + i, i);
-        float acc[R][NT][4];
+        float acc[NT][4];
 #pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) acc[r][j][0] = acc[r][j][1] = acc[r][j][2] = acc[r][j][3] = 0;
+        for (int j = 0; j < NT; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0;
         int slot = 0, into = RING - 1;
         for (int s = s0; s < s1; s++) {
             asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
-            together();      // (both warps' copies of this step are there, and both are done with the step before)
+            __syncthreads();      // (all copies of this step are there, and all warps are done with the step before)
             copy(s + RING - 1, into);
-            const uint8_t *in = slots + slot * SLOT, *mine = in + half * WSLOT;
+            const uint8_t *in = i4_smem + slot * SLOT, *mine = in + warp * WSLOT, *rows = in + WARPS * WSLOT + quarter * (NT * 8 * 128) + g * 128;
             into = into + 1 == RING ? 0 : into + 1;
             slot = slot + 1 == RING ? 0 : slot + 1;
+            if ((s * 4 + quarter) * 2 >= a.steps) continue;      // (no channels left: nothing was copied)
+            const uint4 w0 = *reinterpret_cast<const uint4*>(mine + lane * 16), w1 = *reinterpret_cast<const uint4*>(mine + I4_TILE + lane * 16);
+            const uint32_t v[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+            uint32_t lo[8], hi[8];
 #pragma unroll
-            for (int j0 = 0; j0 < NT; j0 += J) {
-                if (j0 * 8 >= x.many) break;
+            for (int i = 0; i < 8; i++) lo[i] = (v[i] << 4) & 0xf0f0f0f0u, hi[i] = v[i] & 0xf0f0f0f0u;
+            float2 e[GS];
+#pragma unroll
+            for (int q = 0; q < GS; q++) e[q] = i4_scales<S>(mine + 2 * I4_TILE + q * SB + g * 2 * sizeof(S));
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                if (j >= nt) break;
+                uint2 b[4];
+#pragma unroll
+                for (int h = 0; h < 4; h++) b[h] = *reinterpret_cast<const uint2*>(rows + j * 1024 + (((h * 2 + (t >> 1)) ^ ((g & 3) << 1)) << 4) + (t & 1) * 8);
 #pragma unroll
                 for (int q = 0; q < GS; q++) {
-                    uint2 b[J][GC];
+                    int sum[4];
 #pragma unroll
-                    for (int j = 0; j < J; j++)
-#pragma unroll
-                        for (int h = 0; h < GC; h++)
-                            b[j][h] = *reinterpret_cast<const uint2*>(in + 2 * WSLOT + ((j0 + j) * 8 + g) * 128 + ((((q * GC + h) * 2 + (t >> 1)) ^ ((g & 3) << 1)) << 4) + (t & 1) * 8);
-#pragma unroll
-                    for (int r = 0; r < R; r++) {
-                        uint2 v[GC];
-#pragma unroll
-                        for (int h = 0; h < GC; h++) v[h] = *reinterpret_cast<const uint2*>(mine + (r * 2 + (q * GC + h) / 2) * I4_TILE + lane * 16 + (q * GC + h) % 2 * 8);
-                        const float2 e = i4_scales<S>(mine + R * 2 * I4_TILE + (r * GS + q) * SB + g * 2 * sizeof(S));
-#pragma unroll
-                        for (int j = 0; j < J; j++) {
-                            if ((j0 + j) * 8 >= x.many) break;
-                            int sum[4];
-#pragma unroll
-                            for (int h = 0; h < GC; h++) {
-                                const uint32_t a0 = (v[h].x << 4) & 0xf0f0f0f0u, a1 = (v[h].y << 4) & 0xf0f0f0f0u, a2 = v[h].x & 0xf0f0f0f0u, a3 = v[h].y & 0xf0f0f0f0u;
-                                if (h == 0) mma_s8_first(sum, a0, a1, a2, a3, b[j][h].x, b[j][h].y);
-                                else mma_s8(sum, a0, a1, a2, a3, b[j][h].x, b[j][h].y);
-                            }
-                            acc[r][j0 + j][0] = fmaf(e.x, i4_sum(sum[0]), acc[r][j0 + j][0]);
-                            acc[r][j0 + j][1] = fmaf(e.x, i4_sum(sum[1]), acc[r][j0 + j][1]);
-                            acc[r][j0 + j][2] = fmaf(e.y, i4_sum(sum[2]), acc[r][j0 + j][2]);
-                            acc[r][j0 + j][3] = fmaf(e.y, i4_sum(sum[3]), acc[r][j0 + j][3]);
-                        }
+                    for (int i = 0; i < GC; i++) {
+                        const int h = q * GC + i;
+                        if (i == 0) mma_s8_first(sum, lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1], b[h].x, b[h].y);
+                        else mma_s8(sum, lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1], b[h].x, b[h].y);
                     }
+                    acc[j][0] = fmaf(e[q].x, i4_sum(sum[0]), acc[j][0]);
+                    acc[j][1] = fmaf(e[q].x, i4_sum(sum[1]), acc[j][1]);
+                    acc[j][2] = fmaf(e[q].y, i4_sum(sum[2]), acc[j][2]);
+                    acc[j][3] = fmaf(e[q].y, i4_sum(sum[3]), acc[j][3]);
                 }
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-        together();
-        // sums to this pair's part of the ring
+        __syncthreads();
+        // sums to the ring's place
 #pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int j = 0; j < NT; j++)
-                reinterpret_cast<float4*>(slots)[((half * R + r) * NT + j) * 32 + lane] = make_float4(acc[r][j][0], acc[r][j][1], acc[r][j][2], acc[r][j][3]);
+        for (int j = 0; j < NT; j++) reinterpret_cast<float4*>(i4_smem)[(warp * NT + j) * 32 + lane] = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
         __syncwarp();
         if (a.split > 1) cluster_sync();
         else __syncthreads();
-        for (int o = tid + rank * P * 64; o < 32 * R * x.many; o += P * 64 * a.split) {      // row i of the unit's, column q
-            const int i = o % (32 * R), q = o / (32 * R), n = (tile - half * R) * 16 + i;
+        for (int o = tid + rank * WARPS * 32; o < 16 * R * x.many; o += WARPS * 32 * a.split) {      // row i of the unit's, column q
+            const int i = o % (16 * R), q = o / (16 * R), n = tile0 * 16 + i;
             if (n >= a.n) continue;
             const uint8_t* from = i4_smem + (((i / 16 * NT + q / 8) * 32 + (i % 8) * 4 + q % 8 / 2) * 4 + (i % 16) / 8 * 2 + q % 2) * 4;
             float y = 0;
             for (int b = 0; b < a.split; b++)
 #pragma unroll
-                for (int w = 0; w < P; w++) {
-                    const uint8_t* f = from + w * RING * SLOT;
+                for (int k = 0; k < WARPS / R; k++) {
+                    const uint8_t* f = from + k * R * NT * 512;
                     y += a.split > 1 ? peer_f32((uint32_t)__cvta_generic_to_shared(f), b) : *reinterpret_cast<const float*>(f);
                 }
             i4_put(a, x.e, i4_pair(a, l, x.lo + q), n, y);
@@ -523,13 +529,13 @@ template <int CHUNK, int R, int WARPS, typename F> cudaError_t mat_mat_i4_launch
     }
     return e;
 }
-template <typename S, int GROUP, int TC, int NT> cudaError_t mat_mat_i4_few(const MatI4Args& a, int sms, cudaStream_t st) {
+template <typename S, int GROUP, int NT> cudaError_t mat_mat_i4_few(const MatI4Args& a, int sms, cudaStream_t st) {
     static SmemAllowed allowed;
-    return mat_mat_i4_launch<TC * NT, 1, i4_few_warps<NT>()>(a, mat_mat_i4_few_kernel<S, GROUP, TC, NT>, allowed, i4_few_warps<NT>() * (I4_RING * i4_slot<S, GROUP, 1, 4>() + 2 * NT * 512), sms, st);
+    return mat_mat_i4_launch<8 * NT, 1, i4_few_warps<NT>()>(a, mat_mat_i4_few_kernel<S, GROUP, NT>, allowed, i4_few_warps<NT>() * (I4_RING * i4_slot<S, GROUP, 4>() + 2 * NT * 512), sms, st);
 }
-template <typename S, int GROUP, int NT> cudaError_t mat_mat_i4_many(const MatI4Args& a, int sms, cudaStream_t st) {
+template <typename S, int GROUP> cudaError_t mat_mat_i4_many(const MatI4Args& a, int sms, cudaStream_t st) {
     static SmemAllowed allowed;
-    return mat_mat_i4_launch<NT * 8, 2 * I4_R, 2 * I4_PAIRS_OF_WARPS>(a, mat_mat_i4_many_kernel<S, GROUP, NT>, allowed, I4_PAIRS_OF_WARPS * i4_many_ring<S, GROUP, NT>() * i4_many_slot<S, GROUP, NT>(), sms, st);
+    return mat_mat_i4_launch<I4_MANY_NT * 8, I4_MANY_TILES, I4_MANY_WARPS>(a, mat_mat_i4_many_kernel<S, GROUP>, allowed, I4_MANY_RING * i4_many_slot<S, GROUP>(), sms, st);
 }
 template <typename S, int GROUP> cudaError_t mat_mat_i4(const MatI4Args& a, cudaStream_t st) {
     int dev = 0, sms = 0;
@@ -542,9 +548,7 @@ template <typename S, int GROUP> cudaError_t mat_mat_i4(const MatI4Args& a, cuda
         const double each = (double)a.rows / a.n_experts;
         rows = std::min<int64_t>(a.tokens, (int64_t)std::ceil(each + 2 * std::sqrt(each)));
     }
-    return rows <= 1 ? mat_mat_i4_few<S, GROUP, 1, 1>(a, sms, st) : rows <= 2 ? mat_mat_i4_few<S, GROUP, 2, 1>(a, sms, st) : rows <= 4 ? mat_mat_i4_few<S, GROUP, 4, 1>(a, sms, st)
-         : rows <= 8 ? mat_mat_i4_few<S, GROUP, 8, 1>(a, sms, st) : rows <= 16 ? mat_mat_i4_few<S, GROUP, 8, 2>(a, sms, st) : rows <= 32 ? mat_mat_i4_many<S, GROUP, 4>(a, sms, st)
-         : mat_mat_i4_many<S, GROUP, 8>(a, sms, st);
+    return rows <= 8 ? mat_mat_i4_few<S, GROUP, 1>(a, sms, st) : rows <= 16 ? mat_mat_i4_few<S, GROUP, 2>(a, sms, st) : mat_mat_i4_many<S, GROUP>(a, sms, st);
 }
 
 }  // namespace dev
