@@ -87,7 +87,11 @@ __device__ __forceinline__ int peer_s32(uint32_t addr, uint32_t rank) {
     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at_rank(addr, rank)));      // (behind a barrier: nothing to be ordered with)
     return v;
 }
-__device__ __forceinline__ float peer_f32(uint32_t addr, uint32_t rank) { return __int_as_float(peer_s32(addr, rank)); }
+__device__ __forceinline__ float4 peer_f32x4(uint32_t addr, uint32_t rank) {      // (a block without a cluster is rank 0 of its own)
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at_rank(addr, rank)) : "memory");
+    return v;
+}
 
 // Programmatic launches: a kernel may be scheduled while the one before it on the stream ends.  Every block of every kernel here calls before() first thing, ahead of any access to global memory (it
 // returns when all that came before is done and visible), and so no kernel can end before its predecessors have.

@@ -5,17 +5,18 @@
 //
 // A tile of weights is 16 rows x 64 channels in 512 bytes, placed so that the 16 bytes of a lane are the operands of two mma.m16n8k32 (s8, s32 sums): a word has four channels in the low
 // halves of its bytes and the next four in the high halves; (word << 4) & 0xf0f0f0f0 and word & 0xf0f0f0f0 are those values times sixteen as signed bytes, three instructions for eight weights.  Eight rows of a are
-// the columns.  Sums begin at the bits of 1.5 * 2^23, so that read as f32 they are that plus the sum (|16 sum| <= 2^21).
+// the columns.
 //
-// Work.  A unit is one or four tiles of weight rows and as many rows of a as the kernel takes at once.  Each lane copies the bytes that it will read itself into a ring in shared memory (cp.async), some steps ahead, so that no warp waits
+// Work.  A unit is one or eight tiles of weight rows and as many rows of a as the kernel takes at once.  Each lane copies the bytes that it will read itself into a ring in shared memory (cp.async), some steps ahead, so that no warp waits
 // for another's weights.  With experts every block lists the pairs (token, expert) by expert first, all in the same order; up to that many pairs of an expert are a unit for each tile.
-//   few rows (up to 16): the weights' bytes.  A block per SM has consecutive units of one tile; its warps share their steps of 256 channels evenly, whichever unit they are of, and leave the sums of a unit that two or
+//   few rows (up to 16): the weights' bytes.  Two blocks per SM have consecutive units of one tile each; its warps share their steps of 256 channels evenly, whichever unit they are of, and leave the sums of a unit that two or
 //   more warps have a part of in shared memory for the end.  Rows of a come from L1 and L2.
-//   more rows (up to 64 at a time): rows of a cost as much as weights.  A block's sixteen warps have four tiles and a step of 512 channels, a quarter of it each; the rows' bytes go through the ring with the
-//   weights' and serve the four tiles.  With few units the blocks of a cluster share the channels of one.
+//   more rows (up to 64 at a time): rows of a cost as much as weights.  A block has eight tiles; its teams of four warps have a part of the channels each, whose rows of a serve all eight.  With few units the
+//   blocks of a cluster share the channels of one.
 #pragma once
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "dev_common.cuh"
 
@@ -45,14 +46,13 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-constexpr int kI4Zero = 0x4B400000;      // the bits of 1.5 * 2^23
-// ... with sums that begin there
+// ... with sums that begin here
 __device__ __forceinline__ void mma_s8_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(kI4Zero));
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
-__device__ __forceinline__ float i4_sum(int bits) { return __int_as_float(bits) - 12582912.0f; }
+__device__ __forceinline__ float i4_sum(int sum) { return (float)sum; }
 // 16 or 8 bytes to shared memory, zeros where `there` is not set (the address is a valid one all the same)
 template <int N> __device__ __forceinline__ void copy_where(uint32_t to, const void* from, bool there) {
     if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
@@ -132,8 +132,9 @@ template <int MOST> __device__ __forceinline__ I4Chunk i4_chunk(const MatI4Args&
     return I4Chunk{e, lo, min(MOST, l.end[e] - lo)};
 }
 __device__ __forceinline__ int i4_pair(const MatI4Args& a, const I4List& l, int i) { return a.experts ? l.list[i] : i; }
-__device__ __forceinline__ void i4_put(const MatI4Args& a, int e, int p, int n, float sum) {
-    float y = sum * 0.0625f * a.a_scales[(a.first + p) / a.div];
+__device__ __forceinline__ float i4_row_scale(const MatI4Args& a, int p) { return 0.0625f * a.a_scales[(a.first + p) / a.div]; }
+__device__ __forceinline__ void i4_put(const MatI4Args& a, int e, int p, int n, float sum, float scale) {
+    float y = sum * scale;
     if (a.bias) y += a.bias[(int64_t)e * a.n + n];
     const int64_t to = (int64_t)(a.first + p) * a.ldo + n;
     if (a.out_type == B200_TYPE_F32) reinterpret_cast<float*>(a.out)[to] = y;
@@ -245,8 +246,8 @@ template <typename S, int GROUP, int TC, int NT> struct I4Step {
     }
 };
 
-template <int NT> __host__ __device__ constexpr int i4_few_warps() { return NT == 1 ? 24 : 16; }
-template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_few_warps<NT>() * 32, 1) mat_mat_i4_few_kernel(const MatI4Args a) {
+template <int NT> __host__ __device__ constexpr int i4_few_warps() { return NT == 1 ? 12 : 8; }
+template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_few_warps<NT>() * 32, 2) mat_mat_i4_few_kernel(const MatI4Args a) {
     before();
     constexpr int SLOT = i4_slot<S, GROUP, 4>(), SB = 16 * (int)sizeof(S), CHUNK = 8 * NT, WARPS = i4_few_warps<NT>();
     extern __shared__ __align__(16) uint8_t i4_smem[];
@@ -266,7 +267,14 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
     const int many = (int)(u1 - u0), steps = many * whole;
     auto begin = [&](int w) { return (int)((int64_t)steps * w / WARPS); };
     // sums over a row's columns, and the results of a unit
-    auto finish = [&](float4 (&y)[NT], const I4Chunk& x, int tile) {
+    auto row_scales = [&](float2 (&d)[NT], const I4Chunk& x) {
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const int col = 8 * j + 2 * t;
+            d[j] = make_float2(col < x.many ? i4_row_scale(a, i4_pair(a, l, x.lo + col)) : 0.0f, col + 1 < x.many ? i4_row_scale(a, i4_pair(a, l, x.lo + col + 1)) : 0.0f);
+        }
+    };
+    auto finish = [&](float4 (&y)[NT], const float2 (&d)[NT], const I4Chunk& x, int tile) {
         const int tc = x.many > 4 ? 8 : x.many > 2 ? 4 : x.many;      // (columns of one row are 1, 2, 4 apart)
         if (tc == 1) y[0].x += y[0].y, y[0].z += y[0].w;
         if (tc < 4) {
@@ -289,8 +297,8 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
                 const int col = 8 * j + 2 * t + q;
                 if (col < x.many) {
                     const int p = i4_pair(a, l, x.lo + col);
-                    if (n < a.n) i4_put(a, x.e, p, n, q ? y[j].y : y[j].x);
-                    if (n + 8 < a.n) i4_put(a, x.e, p, n + 8, q ? y[j].w : y[j].z);
+                    if (n < a.n) i4_put(a, x.e, p, n, q ? y[j].y : y[j].x, q ? d[j].y : d[j].x);
+                    if (n + 8 < a.n) i4_put(a, x.e, p, n + 8, q ? y[j].w : y[j].z, q ? d[j].y : d[j].x);
                 }
             }
     };
@@ -330,6 +338,8 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
         for (int f = f0; f < f1;) {
             const int sa = s, sb = min(whole, s + f1 - f);
             float acc[NT][4];
+            float2 d[NT];
+            row_scales(d, x);
 #pragma unroll
             for (int j = 0; j < NT; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0;
             auto products = [&](auto step, auto& sums) {
@@ -360,7 +370,7 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
 #pragma unroll
             for (int j = 0; j < NT; j++) y[j] = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
             if (sa == 0 && sb == whole) {
-                finish(y, x, tile);
+                finish(y, d, x, tile);
             } else {
 #pragma unroll
                 for (int j = 0; j < NT; j++) parts[((warp * 2 + (f != f0)) * NT + j) * 32 + lane] = y[j];
@@ -396,115 +406,169 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
             }
         }
         const int c = (int)((u0 + v) / a.tiles);
-        finish(y, i4_chunk<CHUNK>(a, l, c), (int)(u0 + v - (int64_t)c * a.tiles));
+        const I4Chunk x = i4_chunk<CHUNK>(a, l, c);
+        float2 d[NT];
+        row_scales(d, x);
+        finish(y, d, x, (int)(u0 + v - (int64_t)c * a.tiles));
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------- more rows
-enum { I4_MANY_WARPS = 16, I4_MANY_TILES = 4, I4_MANY_NT = 8, I4_MANY_RING = 4 };
-template <typename S, int GROUP> __host__ __device__ constexpr int i4_many_slot() { return I4_MANY_WARPS * i4_slot<S, GROUP, 2>() + I4_MANY_NT * 8 * 512; }
-// Warp w has tile w % 4 of the unit's and quarter w / 4 of a step.
-template <typename S, int GROUP> __global__ void __launch_bounds__(I4_MANY_WARPS * 32, 1) mat_mat_i4_many_kernel(const MatI4Args a) {
+// Four teams of four warps; a team has a part of the channels, 128 at a time, and its own ring, so that the teams' copies, products and sums overlap.  A warp has two of the unit's eight tiles; the rows of a are the
+// team's.
+enum { I4_TEAMS = 4, I4_TEAM_TILES = 8, I4_MANY_NT = 8 };
+template <typename S, int GROUP> __host__ __device__ constexpr int i4_many_slot() { return I4_TEAM_TILES * i4_slot<S, GROUP, 2>() + I4_MANY_NT * 8 * 128; }
+template <typename S, int GROUP> __host__ __device__ constexpr int i4_many_ring() {      // steps of a team's ring: three where they fit a block's 227 KiB with the longest lists
+    return 3 * I4_TEAMS * i4_many_slot<S, GROUP>() + (int)i4_list_bytes(1024, I4_PAIRS) + 1024 <= 227 * 1024 ? 3 : 2;
+}
+template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * 128, 1) mat_mat_i4_many_kernel(const MatI4Args a) {
     before();
-    constexpr int R = I4_MANY_TILES, NT = I4_MANY_NT, RING = I4_MANY_RING, WARPS = I4_MANY_WARPS, WSLOT = i4_slot<S, GROUP, 2>(), SLOT = i4_many_slot<S, GROUP>(), GS = 128 / GROUP, SB = 16 * (int)sizeof(S),
-                  GC = GROUP / 32;
+    constexpr int T = I4_TEAM_TILES, NT = I4_MANY_NT, RING = i4_many_ring<S, GROUP>(), WSLOT = i4_slot<S, GROUP, 2>(), SLOT = i4_many_slot<S, GROUP>(), GS = 128 / GROUP, SB = 16 * (int)sizeof(S), GC = GROUP / 32;
+    static_assert(RING * SLOT >= T * NT * 512, "a team's sums take its ring's place");
     extern __shared__ __align__(16) uint8_t i4_smem[];
-    __shared__ int64_t s_row[8 * NT];      // where the unit's rows of a begin
-    const I4List l = i4_list(i4_smem + RING * SLOT, a);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, quarter = warp / R;
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(i4_smem);
-    const int blocks = (a.tiles + R - 1) / R, whole = (a.steps + 7) / 8;
+    const I4List l = i4_list(i4_smem + I4_TEAMS * RING * SLOT, a);
+    const int tid = threadIdx.x, lane = tid & 31, team = tid >> 7, member = (tid >> 5) & 3, g = lane >> 2, t = lane & 3;
+    uint8_t* slots = i4_smem + team * RING * SLOT;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(slots);
+    const int blocks = (a.tiles + T - 1) / T, whole = (a.steps + 1) / 2;
     int chunks = (a.rows + 8 * NT - 1) / (8 * NT);
     if (a.experts) {
         i4_lists(a, l, 8 * NT);
         chunks = l.chunk[a.n_experts];
         i4_zeros(a, l);
     }
-    const int rank = blockIdx.x % a.split, s0 = (int)((int64_t)whole * rank / a.split), s1 = (int)((int64_t)whole * (rank + 1) / a.split);
+    const int rank = blockIdx.x % a.split, parts = I4_TEAMS * a.split, part = rank * I4_TEAMS + team, s0 = (int)((int64_t)whole * part / parts), s1 = (int)((int64_t)whole * (part + 1) / parts);
+    auto together = [&] { asm volatile("bar.sync %0, 128;" ::"r"(team + 1) : "memory"); };
     for (int64_t u = blockIdx.x / a.split; u < (int64_t)chunks * blocks; u += gridDim.x / a.split) {
-        const int c = (int)(u / blocks), tile0 = (int)(u - (int64_t)c * blocks) * R, tile = min(tile0 + warp % R, a.tiles - 1);      // (a warp without a tile takes another's: nothing reads its sums)
+        const int c = (int)(u / blocks), tile0 = (int)(u - (int64_t)c * blocks) * T;
         const I4Chunk x = i4_chunk<8 * NT>(a, l, c);
         const int nt = (x.many + 7) / 8;
-        if (tid < 8 * NT) s_row[tid] = (int64_t)((a.first + i4_pair(a, l, x.lo + (tid < x.many ? tid : 0))) / a.div) * a.lda;
-        __syncthreads();
-        const int64_t at = (int64_t)x.e * a.tiles + tile;
-        const uint8_t *w = a.w + at * a.steps * I4_TILE, *d = reinterpret_cast<const uint8_t*>(a.ws) + at * a.groups * SB;
-        // rows of 128 bytes per quarter; 16 bytes u of row i lie at u ^ (2 (i % 4)), so that the eight rows of a block of columns are read without bank conflicts
+        // this warp's tiles (where there are none others': nothing reads their sums), and the rows of a that this thread copies 16 bytes of
+        const uint8_t *w[2], *d[2];
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const int64_t at = (int64_t)x.e * a.tiles + min(tile0 + member * 2 + r, a.tiles - 1);
+            w[r] = a.w + at * a.steps * I4_TILE;
+            d[r] = reinterpret_cast<const uint8_t*>(a.ws) + at * a.groups * SB;
+        }
+        const int8_t* from[NT / 2];
+#pragma unroll
+        for (int i = 0; i < NT / 2; i++) {
+            const int q = i * 16 + (tid & 127) / 8;
+            from[i] = a.a + (int64_t)((a.first + i4_pair(a, l, x.lo + (q < x.many ? q : 0))) / a.div) * a.lda + (tid & 7) * 16;
+        }
+        // rows of 128 bytes; 16 bytes u of row i lie at u ^ (2 (i % 4)), so that the eight rows of a block of columns are read without bank conflicts
+        const uint32_t to = ring + T * WSLOT + (tid & 127) / 8 * 128 + (((tid & 7) ^ ((tid >> 3 & 3) << 1)) << 4);
         auto copy = [&](int s, int into) {
             if (s < s1) {
-                const int ch = s * 512 + lane * 16;
-                const uint32_t to = ring + into * SLOT + WARPS * WSLOT + (lane >> 3) * (NT * 8 * 128) + (((lane & 7) ^ ((warp & 3) << 1)) << 4);
-                const int8_t* from = a.a + ch;
-                for (int row = warp; row < nt * 8; row += WARPS) copy_where<16>(to + row * 128, ch < a.k ? from + s_row[row] : a.a, ch < a.k);
-                const int mine = s * 4 + quarter;
-                if (mine * 2 < a.steps) i4_copy<S, GROUP, 2>(a, ring + into * SLOT + warp * WSLOT, w, d, mine, lane);
+                const bool there = s * 128 + (tid & 7) * 16 < a.k;
+#pragma unroll
+                for (int i = 0; i < NT / 2; i++)
+                    if (i * 16 < nt * 8) copy_where<16>(to + into * SLOT + i * 2048, there ? from[i] + s * 128 : a.a, there);
+#pragma unroll
+                for (int r = 0; r < 2; r++) i4_copy<S, GROUP, 2>(a, ring + into * SLOT + (member * 2 + r) * WSLOT, w[r], d[r], s, lane);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
         for (int i = 0; i < RING - 1; i++) copy(s0 + i, i);
-        float acc[NT][4];
+        auto products = [&](auto blocks_of_columns) {
+            constexpr int N = decltype(blocks_of_columns)::value, AT_ONCE = N * GC > 12 ? 1 : 2;      // (both tiles at once, or one after the other where registers do not hold both)
+            float acc[2][N][4];
 #pragma unroll
-        for (int j = 0; j < NT; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0;
-        int slot = 0, into = RING - 1;
-        for (int s = s0; s < s1; s++) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
-            __syncthreads();      // (all copies of this step are there, and all warps are done with the step before)
-            copy(s + RING - 1, into);
-            const uint8_t *in = i4_smem + slot * SLOT, *mine = in + warp * WSLOT, *rows = in + WARPS * WSLOT + quarter * (NT * 8 * 128) + g * 128;
-            into = into + 1 == RING ? 0 : into + 1;
-            slot = slot + 1 == RING ? 0 : slot + 1;
-            if ((s * 4 + quarter) * 2 >= a.steps) continue;      // (no channels left: nothing was copied)
-            const uint4 w0 = *reinterpret_cast<const uint4*>(mine + lane * 16), w1 = *reinterpret_cast<const uint4*>(mine + I4_TILE + lane * 16);
-            const uint32_t v[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-            uint32_t lo[8], hi[8];
+            for (int r = 0; r < 2; r++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) lo[i] = (v[i] << 4) & 0xf0f0f0f0u, hi[i] = v[i] & 0xf0f0f0f0u;
-            float2 e[GS];
+                for (int j = 0; j < N; j++) acc[r][j][0] = acc[r][j][1] = acc[r][j][2] = acc[r][j][3] = 0;
+            int slot = 0, into = RING - 1;
+            for (int s = s0; s < s1; s++) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
+                together();      // (all copies of this step are there, and all warps are done with the step before)
+                copy(s + RING - 1, into);
+                const uint8_t *in = slots + slot * SLOT, *mine = in + member * 2 * WSLOT, *rows = in + T * WSLOT + g * 128;
+                into = into + 1 == RING ? 0 : into + 1;
+                slot = slot + 1 == RING ? 0 : slot + 1;
 #pragma unroll
-            for (int q = 0; q < GS; q++) e[q] = i4_scales<S>(mine + 2 * I4_TILE + q * SB + g * 2 * sizeof(S));
+                for (int q = 0; q < GS; q++)
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-                if (j >= nt) break;
-                uint2 b[4];
+                    for (int r0 = 0; r0 < 2; r0 += AT_ONCE) {
+                        uint32_t lo[AT_ONCE][2 * GC], hi[AT_ONCE][2 * GC];
+                        float2 e[AT_ONCE];
 #pragma unroll
-                for (int h = 0; h < 4; h++) b[h] = *reinterpret_cast<const uint2*>(rows + j * 1024 + (((h * 2 + (t >> 1)) ^ ((g & 3) << 1)) << 4) + (t & 1) * 8);
+                        for (int r = 0; r < AT_ONCE; r++) {
+                            const uint8_t* tile = mine + (r0 + r) * WSLOT;
 #pragma unroll
-                for (int q = 0; q < GS; q++) {
-                    int sum[4];
+                            for (int i = 0; i < GC; i++) {
+                                const int h = q * GC + i;
+                                const uint2 v = *reinterpret_cast<const uint2*>(tile + (h / 2) * I4_TILE + lane * 16 + (h % 2) * 8);
+                                lo[r][2 * i] = (v.x << 4) & 0xf0f0f0f0u, lo[r][2 * i + 1] = (v.y << 4) & 0xf0f0f0f0u;
+                                hi[r][2 * i] = v.x & 0xf0f0f0f0u, hi[r][2 * i + 1] = v.y & 0xf0f0f0f0u;
+                            }
+                            e[r] = i4_scales<S>(tile + 2 * I4_TILE + q * SB + g * 2 * sizeof(S));
+                        }
 #pragma unroll
-                    for (int i = 0; i < GC; i++) {
-                        const int h = q * GC + i;
-                        if (i == 0) mma_s8_first(sum, lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1], b[h].x, b[h].y);
-                        else mma_s8(sum, lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1], b[h].x, b[h].y);
+                        for (int j = 0; j < N; j++) {
+                            uint2 b[GC];
+#pragma unroll
+                            for (int i = 0; i < GC; i++) b[i] = *reinterpret_cast<const uint2*>(rows + j * 1024 + ((((q * GC + i) * 2 + (t >> 1)) ^ ((g & 3) << 1)) << 4) + (t & 1) * 8);
+#pragma unroll
+                            for (int r = 0; r < AT_ONCE; r++) {
+                                int sum[4];
+#pragma unroll
+                                for (int i = 0; i < GC; i++) {
+                                    if (i == 0) mma_s8_first(sum, lo[r][0], lo[r][1], hi[r][0], hi[r][1], b[0].x, b[0].y);
+                                    else mma_s8(sum, lo[r][2 * i], lo[r][2 * i + 1], hi[r][2 * i], hi[r][2 * i + 1], b[i].x, b[i].y);
+                                }
+                                float(&y)[4] = acc[r0 + r][j];
+                                y[0] = fmaf(e[r].x, i4_sum(sum[0]), y[0]);
+                                y[1] = fmaf(e[r].x, i4_sum(sum[1]), y[1]);
+                                y[2] = fmaf(e[r].y, i4_sum(sum[2]), y[2]);
+                                y[3] = fmaf(e[r].y, i4_sum(sum[3]), y[3]);
+                            }
+                        }
                     }
-                    acc[j][0] = fmaf(e[q].x, i4_sum(sum[0]), acc[j][0]);
-                    acc[j][1] = fmaf(e[q].x, i4_sum(sum[1]), acc[j][1]);
-                    acc[j][2] = fmaf(e[q].y, i4_sum(sum[2]), acc[j][2]);
-                    acc[j][3] = fmaf(e[q].y, i4_sum(sum[3]), acc[j][3]);
-                }
             }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();
-        // sums to the ring's place
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            together();
+            // sums to the team's ring's place
 #pragma unroll
-        for (int j = 0; j < NT; j++) reinterpret_cast<float4*>(i4_smem)[(warp * NT + j) * 32 + lane] = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+            for (int r = 0; r < 2; r++)
+#pragma unroll
+                for (int j = 0; j < N; j++)
+                    reinterpret_cast<float4*>(slots)[((member * 2 + r) * NT + j) * 32 + lane] = make_float4(acc[r][j][0], acc[r][j][1], acc[r][j][2], acc[r][j][3]);
+        };
+        if (nt <= 2) products(std::integral_constant<int, 2>());
+        else if (nt <= 3) products(std::integral_constant<int, 3>());
+        else if (nt <= 4) products(std::integral_constant<int, 4>());
+        else if (nt <= 5) products(std::integral_constant<int, 5>());
+        else if (nt <= 6) products(std::integral_constant<int, 6>());
+        else products(std::integral_constant<int, 8>());
         __syncwarp();
         if (a.split > 1) cluster_sync();
         else __syncthreads();
-        for (int o = tid + rank * WARPS * 32; o < 16 * R * x.many; o += WARPS * 32 * a.split) {      // row i of the unit's, column q
-            const int i = o % (16 * R), q = o / (16 * R), n = tile0 * 16 + i;
-            if (n >= a.n) continue;
-            const uint8_t* from = i4_smem + (((i / 16 * NT + q / 8) * 32 + (i % 8) * 4 + q % 8 / 2) * 4 + (i % 16) / 8 * 2 + q % 2) * 4;
-            float y = 0;
+        // a warp for every tile and block of columns; the cluster's blocks take turns
+        for (int o = (tid >> 5) * a.split + rank; o < T * nt; o += I4_TEAMS * 4 * a.split) {
+            const int i = o % T, j = o / T, col = 8 * j + 2 * t, n = (tile0 + i) * 16 + g;
+            int p[2];
+            float scale[2];
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                p[q] = col + q < x.many ? i4_pair(a, l, x.lo + col + q) : -1;
+                scale[q] = p[q] >= 0 ? i4_row_scale(a, p[q]) : 0.0f;
+            }
+            const uint32_t at = (uint32_t)__cvta_generic_to_shared(i4_smem) + ((i * NT + j) * 32 + lane) * 16;
+            float4 y = make_float4(0, 0, 0, 0);
             for (int b = 0; b < a.split; b++)
 #pragma unroll
-                for (int k = 0; k < WARPS / R; k++) {
-                    const uint8_t* f = from + k * R * NT * 512;
-                    y += a.split > 1 ? peer_f32((uint32_t)__cvta_generic_to_shared(f), b) : *reinterpret_cast<const float*>(f);
+                for (int k = 0; k < I4_TEAMS; k++) {
+                    const float4 z = peer_f32x4(at + k * RING * SLOT, b);
+                    y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
                 }
-            i4_put(a, x.e, i4_pair(a, l, x.lo + q), n, y);
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+                if (p[q] >= 0) {
+                    if (n < a.n) i4_put(a, x.e, p[q], n, q ? y.y : y.x, scale[q]);
+                    if (n + 8 < a.n) i4_put(a, x.e, p[q], n + 8, q ? y.w : y.z, scale[q]);
+                }
         }
         __syncwarp();
         if (a.split > 1) cluster_sync();
@@ -514,7 +578,7 @@ template <typename S, int GROUP> __global__ void __launch_bounds__(I4_MANY_WARPS
 
 // ----------------------------------------------------------------------------------------------------------------- host
 // (a launch's list of pairs is bounded: more pairs are more launches)
-template <int CHUNK, int R, int WARPS, typename F> cudaError_t mat_mat_i4_launch(MatI4Args a, F kernel, SmemAllowed& allowed, size_t base, int sms, cudaStream_t st) {
+template <int CHUNK, int R, int WARPS, int PER_SM, typename F> cudaError_t mat_mat_i4_launch(MatI4Args a, F kernel, SmemAllowed& allowed, size_t base, int sms, cudaStream_t st) {
     cudaError_t e = allowed(reinterpret_cast<const void*>(kernel), base + i4_list_bytes(1024, I4_PAIRS));
     const int rows = a.rows, per = a.experts ? I4_PAIRS / a.div * a.div : rows;
     const int64_t blocks = (a.tiles + R - 1) / R;
@@ -525,17 +589,17 @@ template <int CHUNK, int R, int WARPS, typename F> cudaError_t mat_mat_i4_launch
         a.split = 1;
         if (R > 1)
             while (a.split < 8 && units * a.split * 2 <= sms && a.steps >= 32 * a.split) a.split *= 2;
-        e = launch(kernel, dim3((unsigned)(std::min<int64_t>(units, sms / a.split) * a.split)), WARPS * 32, base + (a.experts ? i4_list_bytes(a.n_experts, a.rows) : 0), a.split, st, a);
+        e = launch(kernel, dim3((unsigned)(std::min<int64_t>(units, PER_SM * sms / a.split) * a.split)), WARPS * 32, base + (a.experts ? i4_list_bytes(a.n_experts, a.rows) : 0), a.split, st, a);
     }
     return e;
 }
 template <typename S, int GROUP, int NT> cudaError_t mat_mat_i4_few(const MatI4Args& a, int sms, cudaStream_t st) {
     static SmemAllowed allowed;
-    return mat_mat_i4_launch<8 * NT, 1, i4_few_warps<NT>()>(a, mat_mat_i4_few_kernel<S, GROUP, NT>, allowed, i4_few_warps<NT>() * (I4_RING * i4_slot<S, GROUP, 4>() + 2 * NT * 512), sms, st);
+    return mat_mat_i4_launch<8 * NT, 1, i4_few_warps<NT>(), 2>(a, mat_mat_i4_few_kernel<S, GROUP, NT>, allowed, i4_few_warps<NT>() * (I4_RING * i4_slot<S, GROUP, 4>() + 2 * NT * 512), sms, st);
 }
 template <typename S, int GROUP> cudaError_t mat_mat_i4_many(const MatI4Args& a, int sms, cudaStream_t st) {
     static SmemAllowed allowed;
-    return mat_mat_i4_launch<I4_MANY_NT * 8, I4_MANY_TILES, I4_MANY_WARPS>(a, mat_mat_i4_many_kernel<S, GROUP>, allowed, I4_MANY_RING * i4_many_slot<S, GROUP>(), sms, st);
+    return mat_mat_i4_launch<I4_MANY_NT * 8, I4_TEAM_TILES, I4_TEAMS * 4, 1>(a, mat_mat_i4_many_kernel<S, GROUP>, allowed, I4_TEAMS * i4_many_ring<S, GROUP>() * i4_many_slot<S, GROUP>(), sms, st);
 }
 template <typename S, int GROUP> cudaError_t mat_mat_i4(const MatI4Args& a, cudaStream_t st) {
     int dev = 0, sms = 0;
