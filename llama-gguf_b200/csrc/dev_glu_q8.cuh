@@ -39,7 +39,17 @@ __device__ __forceinline__ double block_max_double(double v, double* s) {
     return v;
 }
 
-// A block per row, read twice, everything in 64 bits.
+// largest magnitude whose f32 is finite
+constexpr double kGluMost = 3.4028235677973366e38;      // 2^128 - 2^103
+struct GluRow {
+    float scale;
+    double inv;      // 127 / maximum (0: the row is zeros)
+};
+__device__ __forceinline__ GluRow glu_row(double top) {
+    const bool live = top >= (double)kTiny && top < kGluMost;
+    return GluRow{top < kGluMost ? live ? (float)(top / 127.0) : 0.0f : NAN, live ? 127.0 / top : 0.0};
+}
+// Rows of any length and alignment: a block per row, read twice, everything in 64 bits.
 template <typename T> __global__ void __launch_bounds__(256) glu_q8_any_kernel(const GluQ8Args a) {
     before();
     __shared__ double s_max[32];
@@ -52,14 +62,103 @@ template <typename T> __global__ void __launch_bounds__(256) glu_q8_any_kernel(c
         bad |= !isfinite(y);
         top = fmax(top, fabs(y));
     }
-    if (bad) top = INFINITY;
-    top = block_max_double(top, s_max);
-    const bool live = top >= (double)kTiny && top < INFINITY;
-    const double inv = live ? 127.0 / top : 0.0;
-    for (int i = threadIdx.x; i < a.ff; i += blockDim.x) a.q[row * a.ldq + i] = live ? (int8_t)__double2int_rn(glu_exact(to_f(g[i]), to_f(u[i]), a.act) * inv) : (int8_t)0;
-    if (threadIdx.x == 0) a.scales[row] = top == INFINITY ? NAN : live ? (float)(top / 127.0) : 0.0f;
+    const GluRow r = glu_row(block_max_double(bad ? INFINITY : top, s_max));
+    for (int i = threadIdx.x; i < a.ff; i += blockDim.x) a.q[row * a.ldq + i] = r.inv != 0 ? (int8_t)__double2int_rn(glu_exact(to_f(g[i]), to_f(u[i]), a.act) * r.inv) : (int8_t)0;
+    if (threadIdx.x == 0) a.scales[row] = r.scale;
 }
 
-template <typename T> cudaError_t glu_q8(const GluQ8Args& a, cudaStream_t st) { return launch(glu_q8_any_kernel<T>, dim3((unsigned)a.rows), 256, 0, 1, st, a); }
+// y in f32, off by less than 2^-17 of itself (2^-16: a product with 127 / maximum and what is compared with it too).  With z = g (SiLU) or its tanh form's argument (GELU), 1 / (1 + exp(-z)) by ex2.approx (2^-22) and
+// rcp.approx (2^-23): the exponential's argument is off by |z| 2^-21.5 at most, which counts while z > -16; further down the result is made in 64 bits.
+constexpr float kGluOff = 1.52587890625e-5f;      // 2^-16
+template <int ACT> __device__ __forceinline__ float glu_near(float g, float u) {
+    if constexpr (ACT == GLU_RELU) return (g > 0 ? g : g == g ? 0.0f : g) * u;
+    const float z = ACT == GLU_GELU ? 1.5957691216057308f * fmaf(0.044715f * g * g, g, g) : g;
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    float y = g * r * u;
+    if (z <= -16.0f) y = (float)glu_exact(g, u, ACT);
+    return y;
+}
+// Rows of whole 16-byte words on 16 bytes: a block per row, which stays in registers as y (V words of each half per thread, asked for together).  The largest value is found among the f32 ones and those that may
+// be it are made again in 64 bits; a number next to the border between two 8-bit ones is made again too (some three of ten thousand).
+template <typename T, int V, int ACT> __global__ void __launch_bounds__(1024) glu_q8_kernel(const GluQ8Args a) {
+    before();
+    constexpr int E = 16 / (int)sizeof(T);
+    __shared__ uint32_t s_max[32];
+    __shared__ unsigned long long s_top;
+    const int64_t row = blockIdx.x;
+    const int words = a.ff / E;
+    const T *gate = reinterpret_cast<const T*>(a.x) + row * a.ldx, *up = gate + a.ff;
+    uint4 g[V], u[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const int i = v * blockDim.x + threadIdx.x;
+        g[v] = i < words ? reinterpret_cast<const uint4*>(gate)[i] : make_uint4(0, 0, 0, 0);
+        u[v] = i < words ? reinterpret_cast<const uint4*>(up)[i] : make_uint4(0, 0, 0, 0);
+    }
+    if (threadIdx.x == 0) s_top = 0;
+    float y[V][E];
+    uint32_t top = 0;
+#pragma unroll
+    for (int v = 0; v < V; v++)
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            y[v][e] = glu_near<ACT>(to_f(reinterpret_cast<const T*>(&g[v])[e]), to_f(reinterpret_cast<const T*>(&u[v])[e]));
+            top = max(top, __float_as_uint(fabsf(y[v][e])));
+        }
+    if (blockDim.x == 32) __syncwarp();
+    top = block_max(top, s_max);
+    if (top < kInfBits) {
+        const float least = __uint_as_float(top) * (1.0f - 2 * kGluOff);
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const int i = v * blockDim.x + threadIdx.x;
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (fabsf(y[v][e]) >= least && i < words) atomicMax(&s_top, (unsigned long long)__double_as_longlong(fabs(glu_exact(to_f(gate[i * E + e]), to_f(up[i * E + e]), ACT))));
+        }
+    }
+    __syncthreads();
+    const GluRow r = glu_row(top < kInfBits ? __longlong_as_double((long long)s_top) : INFINITY);
+    const float inv = (float)r.inv;
+    int8_t* out = a.q + row * a.ldq;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const int i = v * blockDim.x + threadIdx.x;
+        if (i < words) {
+            uint32_t o[E / 4];
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+                int n[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float t = y[v][e + k] * inv;
+                    n[k] = __float2int_rn(t);
+                    if (0.5f - fabsf(t - (float)n[k]) <= fabsf(t) * kGluOff && inv != 0.0f)
+                        n[k] = __double2int_rn(glu_exact(to_f(gate[i * E + e + k]), to_f(up[i * E + e + k]), ACT) * r.inv);
+                }
+                o[e / 4] = r.inv != 0 ? __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410) : 0;
+            }
+            if constexpr (E == 8) reinterpret_cast<uint2*>(out)[i] = make_uint2(o[0], o[1]);
+            else reinterpret_cast<uint32_t*>(out)[i] = o[0];
+        }
+    }
+    if (threadIdx.x == 0) a.scales[row] = r.scale;
+}
+
+template <typename T, int V> cudaError_t glu_q8_words(const GluQ8Args& a, int threads, cudaStream_t st) {
+    auto go = [&](auto kernel) { return launch(kernel, dim3((unsigned)a.rows), threads, 0, 1, st, a); };
+    return a.act == GLU_SILU ? go(glu_q8_kernel<T, V, GLU_SILU>) : a.act == GLU_GELU ? go(glu_q8_kernel<T, V, GLU_GELU>) : go(glu_q8_kernel<T, V, GLU_RELU>);
+}
+// Few rows: as many threads as a half has words, up to 1024 (latency).  Many rows: two or four words per thread, whose loads cover one another.
+template <typename T> cudaError_t glu_q8(const GluQ8Args& a, cudaStream_t st) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const bool words = a.ff % E == 0 && a.ff / E <= 4096 && !(reinterpret_cast<uintptr_t>(a.x) & 15) && a.ldx % E == 0 && !(reinterpret_cast<uintptr_t>(a.q) % E) && a.ldq % E == 0;
+    if (!words) return launch(glu_q8_any_kernel<T>, dim3((unsigned)a.rows), 256, 0, 1, st, a);
+    const int n = a.ff / E, few = a.rows <= 296;
+    const int v = n > 2048 || (!few && n >= 1024) ? 4 : n > 1024 || (!few && n >= 128) ? 2 : 1, threads = ((n + v - 1) / v + 31) / 32 * 32;
+    return v == 4 ? glu_q8_words<T, 4>(a, threads, st) : v == 2 ? glu_q8_words<T, 2>(a, threads, st) : glu_q8_words<T, 1>(a, threads, st);
+}
 
 }  // namespace dev

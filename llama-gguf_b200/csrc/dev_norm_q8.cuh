@@ -50,6 +50,20 @@ __device__ __forceinline__ Q8Row q8_row(uint32_t top) {
     return Q8Row{top >= kInfBits ? __uint_as_float(0x7fffffffu) : live ? __fdiv_rn(m, 127.0f) : 0.0f, live ? __fdiv_rn(127.0f, m) : 0.0f};
 }
 
+// E values times `inv` as 8-bit numbers at `out`, a word of them (inv 0: zeros)
+template <int E> __device__ __forceinline__ void store_q8(int8_t* out, const float (&y)[E], float inv) {
+    uint32_t o[E / 4];
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+        uint32_t n[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) n[k] = inv == 0.0f ? 0u : (uint32_t)__float2int_rn(__fmul_rn(y[e + k], inv));
+        o[e / 4] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+    }
+    if constexpr (E == 8) *reinterpret_cast<uint2*>(out) = make_uint2(o[0], o[1]);
+    else *reinterpret_cast<uint32_t*>(out) = o[0];
+}
+
 // Rows of whole 16-byte words on 16 bytes: a block per row, which stays in registers (V words per thread, asked for together) from its only load on.
 // A square has twice its element's bits and exponent: f16's fits f32, bf16's passes its range both ways, so that one and f32's are made and added in 64 bits.  (A sum of them is rounded, and
 // its order that of the kernel: at 2^-53 of the sum, which only a reciprocal root next to a border of f32 shows.)
@@ -107,18 +121,7 @@ template <typename T, int V> __global__ void __launch_bounds__(1024) add_rms_nor
 #pragma unroll
     for (int v = 0; v < V; v++) {
         const int i = v * blockDim.x + threadIdx.x;
-        if (i < words) {
-            uint32_t o[E / 4];
-#pragma unroll
-            for (int e = 0; e < E; e += 4) {
-                uint32_t n[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) n[k] = q.inv == 0.0f ? 0u : (uint32_t)__float2int_rn(__fmul_rn(r[v][e + k], q.inv));
-                o[e / 4] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
-            }
-            if constexpr (E == 8) reinterpret_cast<uint2*>(out)[i] = make_uint2(o[0], o[1]);
-            else reinterpret_cast<uint32_t*>(out)[i] = o[0];
-        }
+        if (i < words) store_q8<E>(out + i * E, r[v], q.inv);
     }
     if (threadIdx.x == 0) a.scales[row] = q.scale;
 }
