@@ -116,6 +116,12 @@ template <typename... P, typename... A> cudaError_t launch(void (*kernel)(P...),
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
+// SMs of the current device
+inline cudaError_t sm_count(int* sms) {
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    return e == cudaSuccess ? cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) : e;
+}
 // A kernel's dynamic shared memory is allowed once per device (64 devices; further ones ask every time).  One per kernel, by its address.
 struct SmemAllowed {
     std::atomic<uint64_t> done{0};

@@ -63,115 +63,129 @@ template <typename T> __global__ void __launch_bounds__(256) add_gated_norm_any_
     if (threadIdx.x == 0) a.scales[row] = q.scale;
 }
 
-// Rows of whole 16-byte words on 16 bytes: a block per row, which stays in registers (V words per thread) from its loads on.  GATE: 0 none, 1 one number per row, 2 words (of this row, or of all rows).
+// Rows of whole 16-byte words on 16 bytes: blocks stride over the rows; a row stays in registers (V words per thread) from its loads on, the next one's words are asked for before this one's sums, and with one word per
+// thread both weights are kept.  GATE: 0 none, 1 one number per row, 2 words (of this row, or of all rows).
 template <typename T, int V, int GATE, bool POST> __global__ void __launch_bounds__(1024) add_gated_norm_kernel(const GatedNormArgs a) {
     before();
     constexpr int E = 16 / (int)sizeof(T);
-    __shared__ double s_sum[32], s_sum2[32];
+    constexpr bool AHEAD = V < 4, KEPT = V == 1;
+    __shared__ double s_sum[2][32];
     __shared__ uint32_t s_max[32];
-    const int64_t row = blockIdx.x;
-    const int words = a.hidden / E;
-    const uint4* res = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.residual) + row * a.ldr);
-    const T *y = reinterpret_cast<const T*>(a.y) + row * a.top * a.ldy, *gate = reinterpret_cast<const T*>(a.gate) + row * a.gate_row;
+    const int words = a.hidden / E, tid = threadIdx.x;
     uint4 d[V], w[V], h[V];
-#pragma unroll
-    for (int v = 0; v < V; v++) {
-        const int i = v * blockDim.x + threadIdx.x;
-        w[v] = i < words ? reinterpret_cast<const uint4*>(y)[i] : make_uint4(0, 0, 0, 0);
-        d[v] = i < words ? res[i] : make_uint4(0, 0, 0, 0);
-        if (GATE == 2) h[v] = i < words ? reinterpret_cast<const uint4*>(gate)[i] : make_uint4(0, 0, 0, 0);
-    }
-    const float one = GATE == 1 ? to_f(gate[0]) : 1.0f;
-    float r[V][E];
-    const float* mix = a.mix ? a.mix + row * a.top : nullptr;
-    const float m0 = mix ? mix[0] : 1.0f;
-#pragma unroll
-    for (int v = 0; v < V; v++)
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            r[v][e] = to_f(reinterpret_cast<const T*>(&w[v])[e]);
-            if (mix) r[v][e] = __fmul_rn(m0, r[v][e]);
-        }
-    for (int j = 1; j < a.top; j++) {
-        const float m = mix[j];
-        const uint4* p = reinterpret_cast<const uint4*>(y + j * a.ldy);
+    auto load = [&](int64_t row) {
+        const uint4 *res = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.residual) + row * a.ldr), *y = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.y) + row * a.top * a.ldy),
+                    *gate = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.gate) + row * a.gate_row);
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const int i = v * blockDim.x + threadIdx.x;
-            w[v] = i < words ? p[i] : make_uint4(0, 0, 0, 0);
+            const int i = v * blockDim.x + tid;
+            w[v] = i < words ? y[i] : make_uint4(0, 0, 0, 0);
+            d[v] = i < words ? res[i] : make_uint4(0, 0, 0, 0);
+            if (GATE == 2) h[v] = i < words ? gate[i] : make_uint4(0, 0, 0, 0);
         }
+    };
+    float pw[KEPT ? E : 1], nw[KEPT ? E : 1];
+    if constexpr (KEPT)
+        if (tid < words) {
+            if constexpr (POST) load_n<float, E, true>(a.post_weight + tid * E, pw);
+            if (a.weight) load_n<float, E, true>(a.weight + tid * E, nw);
+        }
+    if (AHEAD) load(blockIdx.x);
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        if (!AHEAD) load(row);
+        const float one = GATE == 1 ? to_f(reinterpret_cast<const T*>(a.gate)[row * a.gate_row]) : 1.0f;
+        float r[V][E];
+        const float* mix = a.mix ? a.mix + row * a.top : nullptr;
+        const float m0 = mix ? mix[0] : 1.0f;
 #pragma unroll
         for (int v = 0; v < V; v++)
 #pragma unroll
-            for (int e = 0; e < E; e++) r[v][e] = __fadd_rn(r[v][e], __fmul_rn(m, to_f(reinterpret_cast<const T*>(&w[v])[e])));
-    }
-    if constexpr (POST) {
+            for (int e = 0; e < E; e++) r[v][e] = __fmul_rn(m0, to_f(reinterpret_cast<const T*>(&w[v])[e]));      // (by one: nothing changes)
+        for (int j = 1; j < a.top; j++) {
+            const float m = mix[j];
+            const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.y) + (row * a.top + j) * a.ldy);
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const int i = v * blockDim.x + tid;
+                w[v] = i < words ? p[i] : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int v = 0; v < V; v++)
+#pragma unroll
+                for (int e = 0; e < E; e++) r[v][e] = __fadd_rn(r[v][e], __fmul_rn(m, to_f(reinterpret_cast<const T*>(&w[v])[e])));
+        }
+        if constexpr (POST) {
+            double ss = 0;
+#pragma unroll
+            for (int v = 0; v < V; v++)
+#pragma unroll
+                for (int e = 0; e < E; e++) ss += (double)r[v][e] * r[v][e];
+            const float post = q8_rstd(block_sum(ss, s_sum[0]), a.hidden, a.eps);
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const int i = v * blockDim.x + tid;
+                if (i < words) {
+                    float g[E];
+                    if constexpr (!KEPT) load_n<float, E, true>(a.post_weight + i * E, g);
+#pragma unroll
+                    for (int e = 0; e < E; e++) r[v][e] = __fmul_rn(__fmul_rn(r[v][e], post), KEPT ? pw[KEPT ? e : 0] : g[e]);
+                }
+            }
+        }
+        uint4* sum = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.sum) + row * a.lds);
         double ss = 0;
 #pragma unroll
-        for (int v = 0; v < V; v++)
-#pragma unroll
-            for (int e = 0; e < E; e++) ss += (double)r[v][e] * r[v][e];
-        const float post = q8_rstd(block_sum(ss, s_sum), a.hidden, a.eps);
-#pragma unroll
         for (int v = 0; v < V; v++) {
-            const int i = v * blockDim.x + threadIdx.x;
-            if (i < words) {
-                float g[E];
-                load_n<float, E, true>(a.post_weight + i * E, g);
-#pragma unroll
-                for (int e = 0; e < E; e++) r[v][e] = __fmul_rn(__fmul_rn(r[v][e], post), g[e]);
-            }
-        }
-    }
-    uint4* sum = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.sum) + row * a.lds);
-    double ss = 0;
-#pragma unroll
-    for (int v = 0; v < V; v++) {
-        const int i = v * blockDim.x + threadIdx.x;
-        T* p = reinterpret_cast<T*>(&d[v]);
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            if (GATE == 1) r[v][e] = __fmul_rn(r[v][e], one);
-            if (GATE == 2) r[v][e] = __fmul_rn(r[v][e], to_f(reinterpret_cast<const T*>(&h[v])[e]));
-            p[e] = from_f<T>(__fadd_rn(to_f(p[e]), __fmul_rn(r[v][e], a.scale)));
-            r[v][e] = to_f(p[e]);
-            ss += std::is_same<T, __half>::value ? (double)(r[v][e] * r[v][e]) : (double)r[v][e] * r[v][e];      // (squares of f16 are exact in f32)
-        }
-        if (i < words) sum[i] = d[v];
-    }
-    if (!a.weight) return;
-    const float rstd = q8_rstd(block_sum(ss, s_sum2), a.hidden, a.eps);
-    uint32_t top = 0;
-#pragma unroll
-    for (int v = 0; v < V; v++) {
-        const int i = v * blockDim.x + threadIdx.x;
-        if (i < words) {
-            float g[E];
-            load_n<float, E, true>(a.weight + i * E, g);
+            const int i = v * blockDim.x + tid;
+            T* p = reinterpret_cast<T*>(&d[v]);
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                r[v][e] = __fmul_rn(__fmul_rn(r[v][e], rstd), g[e]);
-                top = max(top, __float_as_uint(fabsf(r[v][e])));
+                if (GATE == 1) r[v][e] = __fmul_rn(r[v][e], one);
+                if (GATE == 2) r[v][e] = __fmul_rn(r[v][e], to_f(reinterpret_cast<const T*>(&h[v])[e]));
+                p[e] = from_f<T>(__fadd_rn(to_f(p[e]), __fmul_rn(r[v][e], a.scale)));
+                r[v][e] = to_f(p[e]);
+                ss += std::is_same<T, __half>::value ? (double)(r[v][e] * r[v][e]) : (double)r[v][e] * r[v][e];      // (squares of f16 are exact in f32)
+            }
+            if (i < words) sum[i] = d[v];
+        }
+        if (AHEAD && row + gridDim.x < a.rows) load(row + gridDim.x);      // (sum may be residual: other rows)
+        if (!a.weight) {
+            if (POST) __syncthreads();      // (the next row writes what this one's sums are read from)
+            continue;
+        }
+        const float rstd = q8_rstd(block_sum(ss, s_sum[1]), a.hidden, a.eps);
+        uint32_t top = 0;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const int i = v * blockDim.x + tid;
+            if (i < words) {
+                float g[E];
+                if constexpr (!KEPT) load_n<float, E, true>(a.weight + i * E, g);
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    r[v][e] = __fmul_rn(__fmul_rn(r[v][e], rstd), KEPT ? nw[KEPT ? e : 0] : g[e]);
+                    top = max(top, __float_as_uint(fabsf(r[v][e])));
+                }
             }
         }
-    }
-    const Q8Row q = q8_row(block_max(top, s_max));
-    int8_t* out = a.q + row * a.ldq;
+        const Q8Row q = q8_row(block_max(top, s_max));
+        int8_t* out = a.q + row * a.ldq;
 #pragma unroll
-    for (int v = 0; v < V; v++) {
-        const int i = v * blockDim.x + threadIdx.x;
-        if (i < words) store_q8<E>(out + i * E, r[v], q.inv);
+        for (int v = 0; v < V; v++) {
+            const int i = v * blockDim.x + tid;
+            if (i < words) store_q8<E>(out + i * E, r[v], q.inv);
+        }
+        if (tid == 0) a.scales[row] = q.scale;
     }
-    if (threadIdx.x == 0) a.scales[row] = q.scale;
 }
 
-template <typename T, int V> cudaError_t add_gated_norm_words(const GatedNormArgs& a, int threads, cudaStream_t st) {
-    auto go = [&](auto kernel) { return launch(kernel, dim3((unsigned)a.rows), threads, 0, 1, st, a); };
+template <typename T, int V> cudaError_t add_gated_norm_words(const GatedNormArgs& a, int threads, int blocks, cudaStream_t st) {
+    auto go = [&](auto kernel) { return launch(kernel, dim3((unsigned)std::min<int64_t>(a.rows, blocks)), threads, 0, 1, st, a); };
     const int gate = !a.gate ? 0 : a.gate_col == 0 ? 1 : 2;
     if (a.post_weight) return gate == 0 ? go(add_gated_norm_kernel<T, V, 0, true>) : gate == 1 ? go(add_gated_norm_kernel<T, V, 1, true>) : go(add_gated_norm_kernel<T, V, 2, true>);
     return gate == 0 ? go(add_gated_norm_kernel<T, V, 0, false>) : gate == 1 ? go(add_gated_norm_kernel<T, V, 1, false>) : go(add_gated_norm_kernel<T, V, 2, false>);
 }
-// (threads and words per thread as in add_rms_norm_q8)
+// As many threads as a row has words, up to 1024; the SMs' 65 536 registers hold 1024 threads.
 template <typename T> cudaError_t add_gated_norm(const GatedNormArgs& a, cudaStream_t st) {
     constexpr int E = 16 / (int)sizeof(T);
     auto off = [](const void* p, int64_t ld, int bytes, int size) { return reinterpret_cast<uintptr_t>(p) % bytes || ld * size % bytes; };
@@ -179,9 +193,11 @@ template <typename T> cudaError_t add_gated_norm(const GatedNormArgs& a, cudaStr
                        (!a.post_weight || !off(a.post_weight, 0, 16, 4)) && (!a.weight || (!off(a.weight, 0, 16, 4) && !off(a.q, a.ldq, E, 1))) &&
                        (!a.gate || a.gate_col == 0 || (a.gate_col == 1 && !off(a.gate, a.gate_row, 16, sizeof(T))));
     if (!words) return launch(add_gated_norm_any_kernel<T>, dim3((unsigned)a.rows), 256, 0, 1, st, a);
-    const int n = a.hidden / E, few = a.rows <= 296;
-    const int v = n > 2048 || (!few && n >= 256) ? 4 : n > 1024 || (!few && n >= 128) ? 2 : 1, threads = ((n + v - 1) / v + 31) / 32 * 32;
-    return v == 4 ? add_gated_norm_words<T, 4>(a, threads, st) : v == 2 ? add_gated_norm_words<T, 2>(a, threads, st) : add_gated_norm_words<T, 1>(a, threads, st);
+    int sms = 0;
+    const cudaError_t e = sm_count(&sms);
+    if (e != cudaSuccess) return e;
+    const int n = a.hidden / E, v = n > 2048 ? 4 : n > 1024 ? 2 : 1, threads = ((n + v - 1) / v + 31) / 32 * 32, blocks = sms * std::max(1, 1024 / threads);
+    return v == 4 ? add_gated_norm_words<T, 4>(a, threads, blocks, st) : v == 2 ? add_gated_norm_words<T, 2>(a, threads, blocks, st) : add_gated_norm_words<T, 1>(a, threads, blocks, st);
 }
 
 }  // namespace dev

@@ -70,95 +70,127 @@ template <typename T> __global__ void __launch_bounds__(256) glu_q8_any_kernel(c
 // y in f32, off by less than 2^-17 of itself (2^-16: a product with 127 / maximum and what is compared with it too).  With z = g (SiLU) or its tanh form's argument (GELU), 1 / (1 + exp(-z)) by ex2.approx (2^-22) and
 // rcp.approx (2^-23): the exponential's argument is off by |z| 2^-21.5 at most, which counts while z > -16; further down the result is made in 64 bits.
 constexpr float kGluOff = 1.52587890625e-5f;      // 2^-16
+template <int ACT> __device__ __forceinline__ float glu_z(float g) { return ACT == GLU_GELU ? 1.5957691216057308f * fmaf(0.044715f * g * g, g, g) : g; }
 template <int ACT> __device__ __forceinline__ float glu_near(float g, float u) {
     if constexpr (ACT == GLU_RELU) return (g > 0 ? g : g == g ? 0.0f : g) * u;
-    const float z = ACT == GLU_GELU ? 1.5957691216057308f * fmaf(0.044715f * g * g, g, g) : g;
     float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(glu_z<ACT>(g) * -1.4426950408889634f));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-    float y = g * r * u;
-    if (z <= -16.0f) y = (float)glu_exact(g, u, ACT);
-    return y;
+    return g * r * u;
 }
-// Rows of whole 16-byte words on 16 bytes: a block per row, which stays in registers as y (V words of each half per thread, asked for together).  The largest value is found among the f32 ones and those that may
-// be it are made again in 64 bits; a number next to the border between two 8-bit ones is made again too (some three of ten thousand).
+__device__ __forceinline__ float max_nan(float a, float b) {      // NaN where either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+template <typename T, int ACT> __device__ __noinline__ double glu_again(const T* gate, const T* up, int i) { return glu_exact(to_f(gate[i]), to_f(up[i]), ACT); }
+// Rows of whole 16-byte words on 16 bytes: blocks stride over the rows; a row stays in registers as y (V words of each half per thread), the next one's words are asked for before this one's sums (V < 4).  The largest
+// value is found among the f32 ones and those that may be it are made again in 64 bits; a number next to the border between two 8-bit ones is made again too (some three of ten thousand).
 template <typename T, int V, int ACT> __global__ void __launch_bounds__(1024) glu_q8_kernel(const GluQ8Args a) {
     before();
     constexpr int E = 16 / (int)sizeof(T);
-    __shared__ uint32_t s_max[32];
-    __shared__ unsigned long long s_top;
-    const int64_t row = blockIdx.x;
-    const int words = a.ff / E;
-    const T *gate = reinterpret_cast<const T*>(a.x) + row * a.ldx, *up = gate + a.ff;
+    constexpr bool AHEAD = V < 4;
+    __shared__ uint32_t s_max[2][32];
+    __shared__ unsigned long long s_top[2];
+    const int words = a.ff / E, tid = threadIdx.x, lane = tid & 31, warps = blockDim.x >> 5;
+    if (tid < 2) s_top[tid] = 0;
     uint4 g[V], u[V];
-#pragma unroll
-    for (int v = 0; v < V; v++) {
-        const int i = v * blockDim.x + threadIdx.x;
-        g[v] = i < words ? reinterpret_cast<const uint4*>(gate)[i] : make_uint4(0, 0, 0, 0);
-        u[v] = i < words ? reinterpret_cast<const uint4*>(up)[i] : make_uint4(0, 0, 0, 0);
-    }
-    if (threadIdx.x == 0) s_top = 0;
-    float y[V][E];
-    uint32_t top = 0;
-#pragma unroll
-    for (int v = 0; v < V; v++)
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            y[v][e] = glu_near<ACT>(to_f(reinterpret_cast<const T*>(&g[v])[e]), to_f(reinterpret_cast<const T*>(&u[v])[e]));
-            top = max(top, __float_as_uint(fabsf(y[v][e])));
-        }
-    if (blockDim.x == 32) __syncwarp();
-    top = block_max(top, s_max);
-    if (top < kInfBits) {
-        const float least = __uint_as_float(top) * (1.0f - 2 * kGluOff);
+    auto load = [&](int64_t row) {
+        const uint4 *p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.x) + row * a.ldx), *q = p + words;
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const int i = v * blockDim.x + threadIdx.x;
-#pragma unroll
-            for (int e = 0; e < E; e++)
-                if (fabsf(y[v][e]) >= least && i < words) atomicMax(&s_top, (unsigned long long)__double_as_longlong(fabs(glu_exact(to_f(gate[i * E + e]), to_f(up[i * E + e]), ACT))));
+            const int i = v * blockDim.x + tid;
+            g[v] = i < words ? p[i] : make_uint4(0, 0, 0, 0);
+            u[v] = i < words ? q[i] : make_uint4(0, 0, 0, 0);
         }
-    }
-    __syncthreads();
-    const GluRow r = glu_row(top < kInfBits ? __longlong_as_double((long long)s_top) : INFINITY);
-    const float inv = (float)r.inv;
-    int8_t* out = a.q + row * a.ldq;
+    };
+    if (AHEAD) load(blockIdx.x);
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const T *gate = reinterpret_cast<const T*>(a.x) + row * a.ldx, *up = gate + a.ff;
+        if (!AHEAD) load(row);
+        float y[V][E], top = 0;
 #pragma unroll
-    for (int v = 0; v < V; v++) {
-        const int i = v * blockDim.x + threadIdx.x;
-        if (i < words) {
-            uint32_t o[E / 4];
+        for (int v = 0; v < V; v++) {
+            const int i = v * blockDim.x + tid;
+            float least = 0;
 #pragma unroll
-            for (int e = 0; e < E; e += 4) {
-                int n[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const float t = y[v][e + k] * inv;
-                    n[k] = __float2int_rn(t);
-                    if (0.5f - fabsf(t - (float)n[k]) <= fabsf(t) * kGluOff && inv != 0.0f)
-                        n[k] = __double2int_rn(glu_exact(to_f(gate[i * E + e + k]), to_f(up[i * E + e + k]), ACT) * r.inv);
-                }
-                o[e / 4] = r.inv != 0 ? __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410) : 0;
+            for (int e = 0; e < E; e++) {
+                const float x = to_f(reinterpret_cast<const T*>(&g[v])[e]);
+                y[v][e] = glu_near<ACT>(x, to_f(reinterpret_cast<const T*>(&u[v])[e]));
+                if (ACT != GLU_RELU) least = fminf(least, glu_z<ACT>(x));
             }
-            if constexpr (E == 8) reinterpret_cast<uint2*>(out)[i] = make_uint2(o[0], o[1]);
-            else reinterpret_cast<uint32_t*>(out)[i] = o[0];
+            if (least <= -16.0f)
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (glu_z<ACT>(to_f(reinterpret_cast<const T*>(&g[v])[e])) <= -16.0f) y[v][e] = (float)glu_again<T, ACT>(gate, up, i * E + e);
+#pragma unroll
+            for (int e = 0; e < E; e++) top = max_nan(top, fabsf(y[v][e]));
         }
+        if (AHEAD && row + gridDim.x < a.rows) load(row + gridDim.x);
+        const uint32_t mine = __float_as_uint(top);
+        uint32_t most = __reduce_max_sync(0xffffffffu, mine);
+        if (lane == 0) s_max[turn][tid >> 5] = most;
+        __syncthreads();
+        most = __reduce_max_sync(0xffffffffu, lane < warps ? s_max[turn][lane] : 0u);
+        const float least = __uint_as_float(most) * (1.0f - 2 * kGluOff);
+        if (most < kInfBits && top >= least) {
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const int i = v * blockDim.x + tid;
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (fabsf(y[v][e]) >= least && i < words) atomicMax(&s_top[turn], (unsigned long long)__double_as_longlong(fabs(glu_again<T, ACT>(gate, up, i * E + e))));
+            }
+        }
+        __syncthreads();
+        const GluRow r = glu_row(most < kInfBits ? __longlong_as_double((long long)s_top[turn]) : INFINITY);
+        if (tid == 0) s_top[turn ^ 1] = 0;      // (the next row's: it was read before this row's first barrier)
+        const float inv = (float)r.inv;
+        int8_t* out = a.q + row * a.ldq;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const int i = v * blockDim.x + tid;
+            if (i < words) {
+                uint32_t n[E];
+                float near = 0;
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const float t = y[v][e] * inv, m = t + 12582912.0f;      // (1.5 * 2^23: the sum's low bits are t rounded, halves to even)
+                    n[e] = __float_as_uint(m);
+                    near = fmaxf(near, fmaf(fabsf(t), kGluOff, fabsf(t - (m - 12582912.0f))));
+                }
+                if (near >= 0.5f && r.inv != 0)
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        const float t = y[v][e] * inv, m = t + 12582912.0f;
+                        if (fmaf(fabsf(t), kGluOff, fabsf(t - (m - 12582912.0f))) >= 0.5f) n[e] = (uint32_t)__double2int_rn(glu_again<T, ACT>(gate, up, i * E + e) * r.inv);
+                    }
+                uint32_t o[E / 4];
+#pragma unroll
+                for (int e = 0; e < E; e += 4) o[e / 4] = r.inv != 0 ? __byte_perm(__byte_perm(n[e], n[e + 1], 0x0040), __byte_perm(n[e + 2], n[e + 3], 0x0040), 0x5410) : 0;
+                if constexpr (E == 8) reinterpret_cast<uint2*>(out)[i] = make_uint2(o[0], o[1]);
+                else reinterpret_cast<uint32_t*>(out)[i] = o[0];
+            }
+        }
+        if (tid == 0) a.scales[row] = r.scale;
     }
-    if (threadIdx.x == 0) a.scales[row] = r.scale;
 }
 
-template <typename T, int V> cudaError_t glu_q8_words(const GluQ8Args& a, int threads, cudaStream_t st) {
-    auto go = [&](auto kernel) { return launch(kernel, dim3((unsigned)a.rows), threads, 0, 1, st, a); };
+template <typename T, int V> cudaError_t glu_q8_words(const GluQ8Args& a, int threads, int blocks, cudaStream_t st) {
+    auto go = [&](auto kernel) { return launch(kernel, dim3((unsigned)std::min<int64_t>(a.rows, blocks)), threads, 0, 1, st, a); };
     return a.act == GLU_SILU ? go(glu_q8_kernel<T, V, GLU_SILU>) : a.act == GLU_GELU ? go(glu_q8_kernel<T, V, GLU_GELU>) : go(glu_q8_kernel<T, V, GLU_RELU>);
 }
-// Few rows: as many threads as a half has words, up to 1024 (latency).  Many rows: two or four words per thread, whose loads cover one another.
+// As many threads as a half has words, up to 1024, or half as many; the SMs' 65 536 registers hold 1024 threads.
 template <typename T> cudaError_t glu_q8(const GluQ8Args& a, cudaStream_t st) {
     constexpr int E = 16 / (int)sizeof(T);
     const bool words = a.ff % E == 0 && a.ff / E <= 4096 && !(reinterpret_cast<uintptr_t>(a.x) & 15) && a.ldx % E == 0 && !(reinterpret_cast<uintptr_t>(a.q) % E) && a.ldq % E == 0;
     if (!words) return launch(glu_q8_any_kernel<T>, dim3((unsigned)a.rows), 256, 0, 1, st, a);
-    const int n = a.ff / E, few = a.rows <= 296;
-    const int v = n > 2048 || (!few && n >= 1024) ? 4 : n > 1024 || (!few && n >= 128) ? 2 : 1, threads = ((n + v - 1) / v + 31) / 32 * 32;
-    return v == 4 ? glu_q8_words<T, 4>(a, threads, st) : v == 2 ? glu_q8_words<T, 2>(a, threads, st) : glu_q8_words<T, 1>(a, threads, st);
+    int sms = 0;
+    const cudaError_t e = sm_count(&sms);
+    if (e != cudaSuccess) return e;
+    const int n = a.ff / E, v = n > 2048 ? 4 : n > 1024 || (a.rows > 2 * sms && n >= 128) ? 2 : 1, threads = ((n + v - 1) / v + 31) / 32 * 32, blocks = sms * std::max(1, 1024 / threads);
+    return v == 4 ? glu_q8_words<T, 4>(a, threads, blocks, st) : v == 2 ? glu_q8_words<T, 2>(a, threads, blocks, st) : glu_q8_words<T, 1>(a, threads, blocks, st);
 }
 
 }  // namespace dev

@@ -602,9 +602,8 @@ template <typename S, int GROUP> cudaError_t mat_mat_i4_many(const MatI4Args& a,
     return mat_mat_i4_launch<I4_MANY_NT * 8, I4_TEAM_TILES, I4_TEAMS * 4, 1>(a, mat_mat_i4_many_kernel<S, GROUP>, allowed, I4_TEAMS * i4_many_ring<S, GROUP>() * i4_many_slot<S, GROUP>(), sms, st);
 }
 template <typename S, int GROUP> cudaError_t mat_mat_i4(const MatI4Args& a, cudaStream_t st) {
-    int dev = 0, sms = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    int sms = 0;
+    const cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) return e;
     // rows of a that meet the same weights: all of them, or with experts no more than there are tokens, and seldom more than two standard deviations above the average
     int64_t rows = a.rows;
