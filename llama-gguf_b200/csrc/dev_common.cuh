@@ -52,6 +52,11 @@ template <typename T, int N, bool VEC> __device__ __forceinline__ void store_n(T
     }
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {      // NaN where either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 // magnitudes below this count as zero, so that 1 / scale and 127 / magnitude stay finite
 constexpr float kTiny = 1.504632769052528e-36f;      // 2^-119
 constexpr uint32_t kInfBits = 0x7f800000u;
@@ -65,6 +70,12 @@ __device__ __forceinline__ Q4Block q4_block(const b200_q4_pages& c, int64_t page
     const uint8_t* p = reinterpret_cast<const uint8_t*>(c.data) + (page * c.n_kv_heads + head) * ((int64_t)c.page_size * (c.head_dim + 8));
     const int rows = c.page_size * c.head_dim / 2;
     return Q4Block{p, p + rows, reinterpret_cast<const float*>(p + 2 * rows), reinterpret_cast<const float*>(p + 2 * rows) + c.page_size};
+}
+
+// 16 or 8 bytes to shared memory, zeros where `there` is not set (the address is a valid one all the same)
+template <int N> __device__ __forceinline__ void copy_where(uint32_t to, const void* from, bool there) {
+    if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(N), "r"(there ? N : 0) : "memory");
 }
 
 // Clusters: barriers, and what lies in another block's shared memory
@@ -116,11 +127,17 @@ template <typename... P, typename... A> cudaError_t launch(void (*kernel)(P...),
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
-// SMs of the current device
+// SMs of the current device (asked for once per device, of 64 devices)
 inline cudaError_t sm_count(int* sms) {
+    static std::atomic<int> known[64];
     int dev = 0;
-    const cudaError_t e = cudaGetDevice(&dev);
-    return e == cudaSuccess ? cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) : e;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    *sms = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (*sms) return cudaSuccess;
+    e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess && dev < 64) known[dev].store(*sms, std::memory_order_relaxed);
+    return e;
 }
 // A kernel's dynamic shared memory is allowed once per device (64 devices; further ones ask every time).  One per kernel, by its address.
 struct SmemAllowed {
@@ -136,5 +153,11 @@ struct SmemAllowed {
         return e;
     }
 };
+// a launch of KERNEL, which is allowed up to `most` bytes of dynamic shared memory
+template <auto KERNEL, typename A> cudaError_t launch_with(size_t most, dim3 grid, unsigned threads, size_t smem, cudaStream_t st, const A& a) {
+    static SmemAllowed allowed;
+    const cudaError_t e = allowed(reinterpret_cast<const void*>(KERNEL), most);
+    return e != cudaSuccess ? e : launch(KERNEL, grid, threads, smem, 1, st, a);
+}
 
 }  // namespace dev

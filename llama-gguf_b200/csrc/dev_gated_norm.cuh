@@ -18,8 +18,21 @@ struct GatedNormArgs {
     int64_t ldy, ldr, lds, ldq, gate_row, gate_col, rows;
     int hidden, top;      // rows of y per row (mix)
     float scale, eps;
+    double per;      // 1 / hidden
 };
 
+// 1 / sqrt(sum / hidden + eps), rounded to f32 once: the root's first bits from rsqrt.approx, then two steps of Newton's method in 64 bits (2^-50 off).  (A division and a root in 64 bits took a third of the kernel's
+// instructions.)
+__device__ __forceinline__ float gated_rstd(double sum, double per, float eps) {
+    const double x = fma(sum, per, (double)eps);
+    double r;
+    asm("rsqrt.approx.ftz.f64 %0, %1;" : "=d"(r) : "d"(x));
+    if (!(x > 1e-300 && x < 1e300)) return (float)(1.0 / sqrt(x));
+    const double h = 0.5 * x;
+    r = r * fma(-h * r, r, 1.5);
+    r = r * fma(-h * r, r, 1.5);
+    return (float)r;
+}
 // Rows of any length and alignment: a block per row; what it makes of a row is kept in the sum's place.
 template <typename T> __global__ void __launch_bounds__(256) add_gated_norm_any_kernel(const GatedNormArgs a) {
     before();
@@ -42,7 +55,7 @@ template <typename T> __global__ void __launch_bounds__(256) add_gated_norm_any_
             const double m = mixed(i);
             ss += m * m;
         }
-        post = q8_rstd(block_sum(ss, s_sum), a.hidden, a.eps);
+        post = gated_rstd(block_sum(ss, s_sum), a.per, a.eps);
     }
     double ss = 0;
     for (int i = threadIdx.x; i < a.hidden; i += blockDim.x) {
@@ -54,7 +67,7 @@ template <typename T> __global__ void __launch_bounds__(256) add_gated_norm_any_
         ss += (double)to_f(r) * to_f(r);
     }
     if (!a.weight) return;
-    const float rstd = q8_rstd(block_sum(ss, s_sum2), a.hidden, a.eps);
+    const float rstd = gated_rstd(block_sum(ss, s_sum2), a.per, a.eps);
     uint32_t top = 0;
     for (int i = threadIdx.x; i < a.hidden; i += blockDim.x) top = max(top, __float_as_uint(fabsf(__fmul_rn(__fmul_rn(to_f(sum[i]), rstd), a.weight[i]))));
     const Q8Row q = q8_row(block_max(top, s_max));
@@ -63,26 +76,31 @@ template <typename T> __global__ void __launch_bounds__(256) add_gated_norm_any_
     if (threadIdx.x == 0) a.scales[row] = q.scale;
 }
 
-// Rows of whole 16-byte words on 16 bytes: blocks stride over the rows; a row stays in registers (V words per thread) from its loads on, the next one's words are asked for before this one's sums, and with one word per
-// thread both weights are kept.  GATE: 0 none, 1 one number per row, 2 words (of this row, or of all rows).
+// Rows of whole 16-byte words on 16 bytes: blocks stride over the rows; a row stays in registers (V words per thread), the next one's words are on their way to shared memory meanwhile, where each thread reads what it has
+// copied itself.  With one word per thread both weights are kept.  GATE: 0 none, 1 one number per row, 2 words (of this row, or of all rows).
 template <typename T, int V, int GATE, bool POST> __global__ void __launch_bounds__(1024) add_gated_norm_kernel(const GatedNormArgs a) {
     before();
     constexpr int E = 16 / (int)sizeof(T);
-    constexpr bool AHEAD = V < 4, KEPT = V == 1;
+    constexpr bool KEPT = V == 1;
+    extern __shared__ uint4 gated_words[];      // [y, residual, gate][V][threads]
     __shared__ double s_sum[2][32];
     __shared__ uint32_t s_max[32];
-    const int words = a.hidden / E, tid = threadIdx.x;
-    uint4 d[V], w[V], h[V];
-    auto load = [&](int64_t row) {
-        const uint4 *res = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.residual) + row * a.ldr), *y = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.y) + row * a.top * a.ldy),
-                    *gate = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.gate) + row * a.gate_row);
+    const int words = a.hidden / E, tid = threadIdx.x, step = blockDim.x;
+    const uint4* mine = gated_words + tid;
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(mine);
+    auto copy = [&](int64_t row) {
+        if (row < a.rows) {
+            const uint4 *res = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.residual) + row * a.ldr) + tid, *y = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.y) + row * a.top * a.ldy) + tid,
+                        *gate = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.gate) + row * a.gate_row) + tid;
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-            const int i = v * blockDim.x + tid;
-            w[v] = i < words ? y[i] : make_uint4(0, 0, 0, 0);
-            d[v] = i < words ? res[i] : make_uint4(0, 0, 0, 0);
-            if (GATE == 2) h[v] = i < words ? gate[i] : make_uint4(0, 0, 0, 0);
+            for (int v = 0; v < V; v++) {
+                const bool there = v * step + tid < words;
+                copy_where<16>(to + v * step * 16, there ? y + v * step : a.y, there);
+                copy_where<16>(to + (V + v) * step * 16, there ? res + v * step : a.y, there);
+                if (GATE == 2) copy_where<16>(to + (2 * V + v) * step * 16, there ? gate + v * step : a.y, there);
+            }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     float pw[KEPT ? E : 1], nw[KEPT ? E : 1];
     if constexpr (KEPT)
@@ -90,23 +108,26 @@ template <typename T, int V, int GATE, bool POST> __global__ void __launch_bound
             if constexpr (POST) load_n<float, E, true>(a.post_weight + tid * E, pw);
             if (a.weight) load_n<float, E, true>(a.weight + tid * E, nw);
         }
-    if (AHEAD) load(blockIdx.x);
+    copy(blockIdx.x);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        if (!AHEAD) load(row);
         const float one = GATE == 1 ? to_f(reinterpret_cast<const T*>(a.gate)[row * a.gate_row]) : 1.0f;
         float r[V][E];
         const float* mix = a.mix ? a.mix + row * a.top : nullptr;
         const float m0 = mix ? mix[0] : 1.0f;
+        asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
-        for (int v = 0; v < V; v++)
+        for (int v = 0; v < V; v++) {
+            const uint4 w = mine[v * step];
 #pragma unroll
-            for (int e = 0; e < E; e++) r[v][e] = __fmul_rn(m0, to_f(reinterpret_cast<const T*>(&w[v])[e]));      // (by one: nothing changes)
+            for (int e = 0; e < E; e++) r[v][e] = __fmul_rn(m0, to_f(reinterpret_cast<const T*>(&w)[e]));      // (by one: nothing changes)
+        }
         for (int j = 1; j < a.top; j++) {
             const float m = mix[j];
             const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.y) + (row * a.top + j) * a.ldy);
+            uint4 w[V];
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                const int i = v * blockDim.x + tid;
+                const int i = v * step + tid;
                 w[v] = i < words ? p[i] : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
@@ -120,10 +141,10 @@ template <typename T, int V, int GATE, bool POST> __global__ void __launch_bound
             for (int v = 0; v < V; v++)
 #pragma unroll
                 for (int e = 0; e < E; e++) ss += (double)r[v][e] * r[v][e];
-            const float post = q8_rstd(block_sum(ss, s_sum[0]), a.hidden, a.eps);
+            const float post = gated_rstd(block_sum(ss, s_sum[0]), a.per, a.eps);
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                const int i = v * blockDim.x + tid;
+                const int i = v * step + tid;
                 if (i < words) {
                     float g[E];
                     if constexpr (!KEPT) load_n<float, E, true>(a.post_weight + i * E, g);
@@ -136,43 +157,45 @@ template <typename T, int V, int GATE, bool POST> __global__ void __launch_bound
         double ss = 0;
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const int i = v * blockDim.x + tid;
-            T* p = reinterpret_cast<T*>(&d[v]);
+            const int i = v * step + tid;
+            uint4 d = mine[(V + v) * step];
+            const uint4 h = GATE == 2 ? mine[(2 * V + v) * step] : make_uint4(0, 0, 0, 0);
+            T* p = reinterpret_cast<T*>(&d);
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 if (GATE == 1) r[v][e] = __fmul_rn(r[v][e], one);
-                if (GATE == 2) r[v][e] = __fmul_rn(r[v][e], to_f(reinterpret_cast<const T*>(&h[v])[e]));
+                if (GATE == 2) r[v][e] = __fmul_rn(r[v][e], to_f(reinterpret_cast<const T*>(&h)[e]));
                 p[e] = from_f<T>(__fadd_rn(to_f(p[e]), __fmul_rn(r[v][e], a.scale)));
                 r[v][e] = to_f(p[e]);
                 ss += std::is_same<T, __half>::value ? (double)(r[v][e] * r[v][e]) : (double)r[v][e] * r[v][e];      // (squares of f16 are exact in f32)
             }
-            if (i < words) sum[i] = d[v];
+            if (i < words) sum[i] = d;
         }
-        if (AHEAD && row + gridDim.x < a.rows) load(row + gridDim.x);      // (sum may be residual: other rows)
+        copy(row + gridDim.x);      // (sum may be residual: other rows)
         if (!a.weight) {
             if (POST) __syncthreads();      // (the next row writes what this one's sums are read from)
             continue;
         }
-        const float rstd = q8_rstd(block_sum(ss, s_sum[1]), a.hidden, a.eps);
-        uint32_t top = 0;
+        const float rstd = gated_rstd(block_sum(ss, s_sum[1]), a.per, a.eps);
+        float top = 0;
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const int i = v * blockDim.x + tid;
+            const int i = v * step + tid;
             if (i < words) {
                 float g[E];
                 if constexpr (!KEPT) load_n<float, E, true>(a.weight + i * E, g);
 #pragma unroll
                 for (int e = 0; e < E; e++) {
                     r[v][e] = __fmul_rn(__fmul_rn(r[v][e], rstd), KEPT ? nw[KEPT ? e : 0] : g[e]);
-                    top = max(top, __float_as_uint(fabsf(r[v][e])));
+                    top = max_nan(top, fabsf(r[v][e]));
                 }
             }
         }
-        const Q8Row q = q8_row(block_max(top, s_max));
+        const Q8Row q = q8_row(block_max(__float_as_uint(top), s_max));
         int8_t* out = a.q + row * a.ldq;
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const int i = v * blockDim.x + tid;
+            const int i = v * step + tid;
             if (i < words) store_q8<E>(out + i * E, r[v], q.inv);
         }
         if (tid == 0) a.scales[row] = q.scale;
@@ -180,12 +203,19 @@ template <typename T, int V, int GATE, bool POST> __global__ void __launch_bound
 }
 
 template <typename T, int V> cudaError_t add_gated_norm_words(const GatedNormArgs& a, int threads, int blocks, cudaStream_t st) {
-    auto go = [&](auto kernel) { return launch(kernel, dim3((unsigned)std::min<int64_t>(a.rows, blocks)), threads, 0, 1, st, a); };
     const int gate = !a.gate ? 0 : a.gate_col == 0 ? 1 : 2;
-    if (a.post_weight) return gate == 0 ? go(add_gated_norm_kernel<T, V, 0, true>) : gate == 1 ? go(add_gated_norm_kernel<T, V, 1, true>) : go(add_gated_norm_kernel<T, V, 2, true>);
-    return gate == 0 ? go(add_gated_norm_kernel<T, V, 0, false>) : gate == 1 ? go(add_gated_norm_kernel<T, V, 1, false>) : go(add_gated_norm_kernel<T, V, 2, false>);
+    const dim3 grid((unsigned)std::min<int64_t>(a.rows, blocks));
+    const size_t most = V * 1024 * 48, smem = V * threads * (gate == 2 ? 48 : 32);
+    if (a.post_weight)
+        return gate == 0   ? launch_with<add_gated_norm_kernel<T, V, 0, true>>(most, grid, threads, smem, st, a)
+               : gate == 1 ? launch_with<add_gated_norm_kernel<T, V, 1, true>>(most, grid, threads, smem, st, a)
+                           : launch_with<add_gated_norm_kernel<T, V, 2, true>>(most, grid, threads, smem, st, a);
+    return gate == 0   ? launch_with<add_gated_norm_kernel<T, V, 0, false>>(most, grid, threads, smem, st, a)
+           : gate == 1 ? launch_with<add_gated_norm_kernel<T, V, 1, false>>(most, grid, threads, smem, st, a)
+                       : launch_with<add_gated_norm_kernel<T, V, 2, false>>(most, grid, threads, smem, st, a);
 }
-// As many threads as a row has words, up to 1024; the SMs' 65 536 registers hold 1024 threads.
+// Few rows: as many threads as a row has words, up to 1024 (latency).  Many rows: four words per thread, so that several blocks of an SM (its 65 536 registers hold 1024 threads) cover one another's barriers, and the sums over
+// a block take fewer instructions.
 template <typename T> cudaError_t add_gated_norm(const GatedNormArgs& a, cudaStream_t st) {
     constexpr int E = 16 / (int)sizeof(T);
     auto off = [](const void* p, int64_t ld, int bytes, int size) { return reinterpret_cast<uintptr_t>(p) % bytes || ld * size % bytes; };
@@ -196,7 +226,7 @@ template <typename T> cudaError_t add_gated_norm(const GatedNormArgs& a, cudaStr
     int sms = 0;
     const cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) return e;
-    const int n = a.hidden / E, v = n > 2048 ? 4 : n > 1024 ? 2 : 1, threads = ((n + v - 1) / v + 31) / 32 * 32, blocks = sms * std::max(1, 1024 / threads);
+    const int n = a.hidden / E, v = n > 2048 || (a.rows > 2 * sms && n >= 256) ? 4 : n > 1024 || (a.rows > 2 * sms && n >= 64) ? 2 : 1, threads = ((n + v - 1) / v + 31) / 32 * 32, blocks = sms * std::max(1, 1024 / threads);
     return v == 4 ? add_gated_norm_words<T, 4>(a, threads, blocks, st) : v == 2 ? add_gated_norm_words<T, 2>(a, threads, blocks, st) : add_gated_norm_words<T, 1>(a, threads, blocks, st);
 }
 

@@ -41,14 +41,8 @@ __device__ __forceinline__ double block_max_double(double v, double* s) {
 
 // largest magnitude whose f32 is finite
 constexpr double kGluMost = 3.4028235677973366e38;      // 2^128 - 2^103
-struct GluRow {
-    float scale;
-    double inv;      // 127 / maximum (0: the row is zeros)
-};
-__device__ __forceinline__ GluRow glu_row(double top) {
-    const bool live = top >= (double)kTiny && top < kGluMost;
-    return GluRow{top < kGluMost ? live ? (float)(top / 127.0) : 0.0f : NAN, live ? 127.0 / top : 0.0};
-}
+__device__ __forceinline__ bool glu_live(double top) { return top >= (double)kTiny && top < kGluMost; }
+__device__ __forceinline__ float glu_scale(double top) { return !(top < kGluMost) ? NAN : glu_live(top) ? (float)(top / 127.0) : 0.0f; }
 // Rows of any length and alignment: a block per row, read twice, everything in 64 bits.
 template <typename T> __global__ void __launch_bounds__(256) glu_q8_any_kernel(const GluQ8Args a) {
     before();
@@ -62,14 +56,15 @@ template <typename T> __global__ void __launch_bounds__(256) glu_q8_any_kernel(c
         bad |= !isfinite(y);
         top = fmax(top, fabs(y));
     }
-    const GluRow r = glu_row(block_max_double(bad ? INFINITY : top, s_max));
-    for (int i = threadIdx.x; i < a.ff; i += blockDim.x) a.q[row * a.ldq + i] = r.inv != 0 ? (int8_t)__double2int_rn(glu_exact(to_f(g[i]), to_f(u[i]), a.act) * r.inv) : (int8_t)0;
-    if (threadIdx.x == 0) a.scales[row] = r.scale;
+    top = block_max_double(bad ? INFINITY : top, s_max);
+    const double inv = glu_live(top) ? 127.0 / top : 0.0;
+    for (int i = threadIdx.x; i < a.ff; i += blockDim.x) a.q[row * a.ldq + i] = inv != 0 ? (int8_t)__double2int_rn(glu_exact(to_f(g[i]), to_f(u[i]), a.act) * inv) : (int8_t)0;
+    if (threadIdx.x == 0) a.scales[row] = glu_scale(top);
 }
 
-// y in f32, off by less than 2^-17 of itself (2^-16: a product with 127 / maximum and what is compared with it too).  With z = g (SiLU) or its tanh form's argument (GELU), 1 / (1 + exp(-z)) by ex2.approx (2^-22) and
-// rcp.approx (2^-23): the exponential's argument is off by |z| 2^-21.5 at most, which counts while z > -16; further down the result is made in 64 bits.
-constexpr float kGluOff = 1.52587890625e-5f;      // 2^-16
+// y in f32.  With z = g (SiLU) or its tanh form's argument (GELU), 1 / (1 + exp(-z)) by ex2.approx (2^-22 off) and rcp.approx (2^-23); the exponential's argument is off by up to 1.5 2^-24 of itself (GELU: 2^-21.7), which counts
+// where z is negative.  With the products' roundings, y and y times rcp.approx of (maximum / 127) are off by less than 2^-19 + |z| 2^-21 of themselves.  Where z <= -16 y is made in 64 bits.
+constexpr float kGluOff = 1.9073486328125e-6f, kGluOffZ = 4.76837158203125e-7f, kGluOffMost = 1.1444091796875e-5f;      // 2^-19, 2^-21, both for z = -16 and a half more
 template <int ACT> __device__ __forceinline__ float glu_z(float g) { return ACT == GLU_GELU ? 1.5957691216057308f * fmaf(0.044715f * g * g, g, g) : g; }
 template <int ACT> __device__ __forceinline__ float glu_near(float g, float u) {
     if constexpr (ACT == GLU_RELU) return (g > 0 ? g : g == g ? 0.0f : g) * u;
@@ -78,62 +73,63 @@ template <int ACT> __device__ __forceinline__ float glu_near(float g, float u) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
     return g * r * u;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {      // NaN where either is
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 template <typename T, int ACT> __device__ __noinline__ double glu_again(const T* gate, const T* up, int i) { return glu_exact(to_f(gate[i]), to_f(up[i]), ACT); }
-// Rows of whole 16-byte words on 16 bytes: blocks stride over the rows; a row stays in registers as y (V words of each half per thread), the next one's words are asked for before this one's sums (V < 4).  The largest
-// value is found among the f32 ones and those that may be it are made again in 64 bits; a number next to the border between two 8-bit ones is made again too (some three of ten thousand).
+// Rows of whole 16-byte words on 16 bytes: blocks stride over the rows; a row stays in registers as y (V words of each half per thread), the next one's words are on their way to shared memory meanwhile, where each thread
+// reads what it has copied itself.  The largest value is found among the f32 ones and those that may be it are made again in 64 bits; a number next to the border between two 8-bit ones is made again too (some
+// of a hundred thousand).
 template <typename T, int V, int ACT> __global__ void __launch_bounds__(1024) glu_q8_kernel(const GluQ8Args a) {
     before();
     constexpr int E = 16 / (int)sizeof(T);
-    constexpr bool AHEAD = V < 4;
+    extern __shared__ uint4 glu_words[];      // [gate, up][V][threads]
     __shared__ uint32_t s_max[2][32];
     __shared__ unsigned long long s_top[2];
     const int words = a.ff / E, tid = threadIdx.x, lane = tid & 31, warps = blockDim.x >> 5;
     if (tid < 2) s_top[tid] = 0;
-    uint4 g[V], u[V];
-    auto load = [&](int64_t row) {
-        const uint4 *p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.x) + row * a.ldx), *q = p + words;
+    uint4 *g = glu_words + tid, *u = g + V * blockDim.x;
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(g);
+    auto copy = [&](int64_t row) {
+        if (row < a.rows) {
+            const uint4 *p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.x) + row * a.ldx) + tid, *q = p + words;
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-            const int i = v * blockDim.x + tid;
-            g[v] = i < words ? p[i] : make_uint4(0, 0, 0, 0);
-            u[v] = i < words ? q[i] : make_uint4(0, 0, 0, 0);
+            for (int v = 0; v < V; v++) {
+                const bool there = v * (int)blockDim.x + tid < words;
+                copy_where<16>(to + v * blockDim.x * 16, there ? p + v * blockDim.x : a.x, there);
+                copy_where<16>(to + (V + v) * blockDim.x * 16, there ? q + v * blockDim.x : a.x, there);
+            }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (AHEAD) load(blockIdx.x);
+    copy(blockIdx.x);
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
         const T *gate = reinterpret_cast<const T*>(a.x) + row * a.ldx, *up = gate + a.ff;
-        if (!AHEAD) load(row);
-        float y[V][E], top = 0;
+        float y[V][E], top = 0, low = 0;
+        asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const int i = v * blockDim.x + tid;
+            const uint4 gw = g[v * blockDim.x], uw = u[v * blockDim.x];
             float least = 0;
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                const float x = to_f(reinterpret_cast<const T*>(&g[v])[e]);
-                y[v][e] = glu_near<ACT>(x, to_f(reinterpret_cast<const T*>(&u[v])[e]));
+                const float x = to_f(reinterpret_cast<const T*>(&gw)[e]);
+                y[v][e] = glu_near<ACT>(x, to_f(reinterpret_cast<const T*>(&uw)[e]));
                 if (ACT != GLU_RELU) least = fminf(least, glu_z<ACT>(x));
             }
-            if (least <= -16.0f)
+            if (least <= -16.0f) {
 #pragma unroll
                 for (int e = 0; e < E; e++)
-                    if (glu_z<ACT>(to_f(reinterpret_cast<const T*>(&g[v])[e])) <= -16.0f) y[v][e] = (float)glu_again<T, ACT>(gate, up, i * E + e);
+                    if (glu_z<ACT>(to_f(reinterpret_cast<const T*>(&gw)[e])) <= -16.0f) y[v][e] = (float)glu_exact(to_f(reinterpret_cast<const T*>(&gw)[e]), to_f(reinterpret_cast<const T*>(&uw)[e]), ACT);
+            }
 #pragma unroll
             for (int e = 0; e < E; e++) top = max_nan(top, fabsf(y[v][e]));
+            low = fminf(low, least);
         }
-        if (AHEAD && row + gridDim.x < a.rows) load(row + gridDim.x);
-        const uint32_t mine = __float_as_uint(top);
-        uint32_t most = __reduce_max_sync(0xffffffffu, mine);
+        copy(row + gridDim.x);
+        uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
         if (lane == 0) s_max[turn][tid >> 5] = most;
         __syncthreads();
         most = __reduce_max_sync(0xffffffffu, lane < warps ? s_max[turn][lane] : 0u);
-        const float least = __uint_as_float(most) * (1.0f - 2 * kGluOff);
+        const float least = __uint_as_float(most) * (1.0f - 2 * kGluOffMost);
         if (most < kInfBits && top >= least) {
 #pragma unroll
             for (int v = 0; v < V; v++) {
@@ -144,9 +140,16 @@ template <typename T, int V, int ACT> __global__ void __launch_bounds__(1024) gl
             }
         }
         __syncthreads();
-        const GluRow r = glu_row(most < kInfBits ? __longlong_as_double((long long)s_top[turn]) : INFINITY);
-        if (tid == 0) s_top[turn ^ 1] = 0;      // (the next row's: it was read before this row's first barrier)
-        const float inv = (float)r.inv;
+        const double exact = most < kInfBits ? __longlong_as_double((long long)s_top[turn]) : INFINITY;
+        if (tid == 0) {
+            s_top[turn ^ 1] = 0;      // (the next row's: it was read before this row's first barrier)
+            a.scales[row] = glu_scale(exact);
+        }
+        const bool live = glu_live(exact);
+        float inv;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"((float)exact * (1.0f / 127.0f)));      // (from 2^-126 to 2^121: neither side leaves the range)
+        inv = live ? inv : 0.0f;
+        const float off = kGluOff - fmaxf(low, -16.0f) * kGluOffZ;
         int8_t* out = a.q + row * a.ldq;
 #pragma unroll
         for (int v = 0; v < V; v++) {
@@ -156,32 +159,31 @@ template <typename T, int V, int ACT> __global__ void __launch_bounds__(1024) gl
                 float near = 0;
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    const float t = y[v][e] * inv, m = t + 12582912.0f;      // (1.5 * 2^23: the sum's low bits are t rounded, halves to even)
+                    const float t = live ? y[v][e] * inv : 0.0f, m = t + kRoundHere;
                     n[e] = __float_as_uint(m);
-                    near = fmaxf(near, fmaf(fabsf(t), kGluOff, fabsf(t - (m - 12582912.0f))));
+                    near = fmaxf(near, fmaf(fabsf(t), off, fabsf(t - (m - kRoundHere))));
                 }
-                if (near >= 0.5f && r.inv != 0)
+                if (near >= 0.5f) {
 #pragma unroll
                     for (int e = 0; e < E; e++) {
-                        const float t = y[v][e] * inv, m = t + 12582912.0f;
-                        if (fmaf(fabsf(t), kGluOff, fabsf(t - (m - 12582912.0f))) >= 0.5f) n[e] = (uint32_t)__double2int_rn(glu_again<T, ACT>(gate, up, i * E + e) * r.inv);
+                        const float t = y[v][e] * inv, m = t + kRoundHere;
+                        if (fmaf(fabsf(t), off, fabsf(t - (m - kRoundHere))) >= 0.5f) n[e] = (uint32_t)__double2int_rn(glu_again<T, ACT>(gate, up, i * E + e) * (127.0 / exact));
                     }
-                uint32_t o[E / 4];
-#pragma unroll
-                for (int e = 0; e < E; e += 4) o[e / 4] = r.inv != 0 ? __byte_perm(__byte_perm(n[e], n[e + 1], 0x0040), __byte_perm(n[e + 2], n[e + 3], 0x0040), 0x5410) : 0;
-                if constexpr (E == 8) reinterpret_cast<uint2*>(out)[i] = make_uint2(o[0], o[1]);
-                else reinterpret_cast<uint32_t*>(out)[i] = o[0];
+                }
+                store_bytes<E>(out + i * E, n);
             }
         }
-        if (tid == 0) a.scales[row] = r.scale;
     }
 }
 
 template <typename T, int V> cudaError_t glu_q8_words(const GluQ8Args& a, int threads, int blocks, cudaStream_t st) {
-    auto go = [&](auto kernel) { return launch(kernel, dim3((unsigned)std::min<int64_t>(a.rows, blocks)), threads, 0, 1, st, a); };
-    return a.act == GLU_SILU ? go(glu_q8_kernel<T, V, GLU_SILU>) : a.act == GLU_GELU ? go(glu_q8_kernel<T, V, GLU_GELU>) : go(glu_q8_kernel<T, V, GLU_RELU>);
+    const dim3 grid((unsigned)std::min<int64_t>(a.rows, blocks));
+    const size_t most = V * 1024 * 32, smem = V * threads * 32;
+    return a.act == GLU_SILU   ? launch_with<glu_q8_kernel<T, V, GLU_SILU>>(most, grid, threads, smem, st, a)
+           : a.act == GLU_GELU ? launch_with<glu_q8_kernel<T, V, GLU_GELU>>(most, grid, threads, smem, st, a)
+                               : launch_with<glu_q8_kernel<T, V, GLU_RELU>>(most, grid, threads, smem, st, a);
 }
-// As many threads as a half has words, up to 1024, or half as many; the SMs' 65 536 registers hold 1024 threads.
+// Few rows: as many threads as a half has words, up to 1024 (latency).  Many rows: four words per thread, so that two and more blocks of an SM (its 65 536 registers hold 1024 threads) cover one another's barriers.
 template <typename T> cudaError_t glu_q8(const GluQ8Args& a, cudaStream_t st) {
     constexpr int E = 16 / (int)sizeof(T);
     const bool words = a.ff % E == 0 && a.ff / E <= 4096 && !(reinterpret_cast<uintptr_t>(a.x) & 15) && a.ldx % E == 0 && !(reinterpret_cast<uintptr_t>(a.q) % E) && a.ldq % E == 0;
@@ -189,7 +191,7 @@ template <typename T> cudaError_t glu_q8(const GluQ8Args& a, cudaStream_t st) {
     int sms = 0;
     const cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) return e;
-    const int n = a.ff / E, v = n > 2048 ? 4 : n > 1024 || (a.rows > 2 * sms && n >= 128) ? 2 : 1, threads = ((n + v - 1) / v + 31) / 32 * 32, blocks = sms * std::max(1, 1024 / threads);
+    const int n = a.ff / E, v = n > 2048 || (a.rows > 2 * sms && n >= 256) ? 4 : n > 1024 || (a.rows > 2 * sms && n >= 64) ? 2 : 1, threads = ((n + v - 1) / v + 31) / 32 * 32, blocks = sms * std::max(1, 1024 / threads);
     return v == 4 ? glu_q8_words<T, 4>(a, threads, blocks, st) : v == 2 ? glu_q8_words<T, 2>(a, threads, blocks, st) : glu_q8_words<T, 1>(a, threads, blocks, st);
 }
 

@@ -53,12 +53,6 @@ __device__ __forceinline__ void mma_s8_first(int (&d)[4], uint32_t a0, uint32_t 
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 __device__ __forceinline__ float i4_sum(int sum) { return (float)sum; }
-// 16 or 8 bytes to shared memory, zeros where `there` is not set (the address is a valid one all the same)
-template <int N> __device__ __forceinline__ void copy_where(uint32_t to, const void* from, bool there) {
-    if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(N), "r"(there ? N : 0) : "memory");
-}
-
 // Pairs by expert, in shared memory: expert e's pairs are list[end[e - 1]] .. list[end[e] - 1] (those without an expert come last), its first chunk is chunk[e].
 struct I4List {
     int *end, *chunk;

@@ -50,18 +50,21 @@ __device__ __forceinline__ Q8Row q8_row(uint32_t top) {
     return Q8Row{top >= kInfBits ? __uint_as_float(0x7fffffffu) : live ? __fdiv_rn(m, 127.0f) : 0.0f, live ? __fdiv_rn(127.0f, m) : 0.0f};
 }
 
-// E values times `inv` as 8-bit numbers at `out`, a word of them (inv 0: zeros)
-template <int E> __device__ __forceinline__ void store_q8(int8_t* out, const float (&y)[E], float inv) {
+constexpr float kRoundHere = 12582912.0f;      // 1.5 * 2^23: the low bits of a sum with it are the other number (up to 2^22) rounded to an integer, halves to even
+// the low bytes of E words at `out`, as a word of them
+template <int E> __device__ __forceinline__ void store_bytes(int8_t* out, const uint32_t (&n)[E]) {
     uint32_t o[E / 4];
 #pragma unroll
-    for (int e = 0; e < E; e += 4) {
-        uint32_t n[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) n[k] = inv == 0.0f ? 0u : (uint32_t)__float2int_rn(__fmul_rn(y[e + k], inv));
-        o[e / 4] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
-    }
+    for (int e = 0; e < E; e += 4) o[e / 4] = __byte_perm(__byte_perm(n[e], n[e + 1], 0x0040), __byte_perm(n[e + 2], n[e + 3], 0x0040), 0x5410);
     if constexpr (E == 8) *reinterpret_cast<uint2*>(out) = make_uint2(o[0], o[1]);
     else *reinterpret_cast<uint32_t*>(out) = o[0];
+}
+// E values times `inv` (at most 127 and its roundings) as 8-bit numbers (inv 0: zeros)
+template <int E> __device__ __forceinline__ void store_q8(int8_t* out, const float (&y)[E], float inv) {
+    uint32_t n[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) n[e] = inv == 0.0f ? 0u : __float_as_uint(__fadd_rn(__fmul_rn(y[e], inv), kRoundHere));
+    store_bytes<E>(out, n);
 }
 
 // Rows of whole 16-byte words on 16 bytes: a block per row, which stays in registers (V words per thread, asked for together) from its only load on.

@@ -104,7 +104,7 @@ extern "C" int b200_dev_add_gated_norm_q8(const b200_gated_norm* a) {
         if (a->sum == a->residual && a->lds != a->ldr) return bad(op, "sum in place needs the same row distance");
         if (a->sum == a->y || (a->gate && a->sum == a->gate)) return bad(op, "sum must not be y or gate");
         const GatedNormArgs g{a->y, a->residual, a->gate, a->sum, a->mix, a->post_weight, a->weight, a->q, a->scales, a->ldy, a->ldr, a->lds, a->ldq, a->gate_row, a->gate_col, a->rows,
-                              (int)a->hidden, a->mix ? a->top : 1, a->scale, a->eps};
+                              (int)a->hidden, a->mix ? a->top : 1, a->scale, a->eps, 1.0 / (double)a->hidden};
         return on_device(op, a->device, [&] { return by_type(a->type, [&](auto t) { return add_gated_norm<decltype(t)>(g, (cudaStream_t)a->stream); }); });
     });
 }
