@@ -78,10 +78,10 @@ template <typename T> __global__ void __launch_bounds__(256) add_gated_norm_any_
 
 // Rows of whole 16-byte words on 16 bytes: blocks stride over the rows; a row stays in registers (V words per thread), the next one's words are on their way to shared memory meanwhile, where each thread reads what it has
 // copied itself.  With one word per thread both weights are kept.  GATE: 0 none, 1 one number per row, 2 words (of this row, or of all rows).
-template <typename T, int V, int GATE, bool POST> __global__ void __launch_bounds__(1024) add_gated_norm_kernel(const GatedNormArgs a) {
+template <typename T, int V, int GATE, bool POST, int MOST> __global__ void __launch_bounds__(MOST) add_gated_norm_kernel(const GatedNormArgs a) {
     before();
     constexpr int E = 16 / (int)sizeof(T);
-    constexpr bool KEPT = V == 1;
+    constexpr bool KEPT = V == 1, EARLY = MOST < 1024 && !KEPT;      // weights in registers; asked for ahead of the sum that they wait for
     extern __shared__ uint4 gated_words[];      // [y, residual, gate][V][threads]
     __shared__ double s_sum[2][32];
     __shared__ uint32_t s_max[32];
@@ -108,6 +108,19 @@ template <typename T, int V, int GATE, bool POST> __global__ void __launch_bound
             if constexpr (POST) load_n<float, E, true>(a.post_weight + tid * E, pw);
             if (a.weight) load_n<float, E, true>(a.weight + tid * E, nw);
         }
+    constexpr int W = EARLY ? V * E : 1;
+    float ew[W];
+    auto ask = [&](const float* from) {
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                float g[E] = {};
+                if (v * step + tid < words) load_n<float, E, true>(from + (v * step + tid) * E, g);
+#pragma unroll
+                for (int e = 0; e < E; e++) ew[v * E + e] = g[e];
+            }
+        }
+    };
     copy(blockIdx.x);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const float one = GATE == 1 ? to_f(reinterpret_cast<const T*>(a.gate)[row * a.gate_row]) : 1.0f;
@@ -119,7 +132,13 @@ template <typename T, int V, int GATE, bool POST> __global__ void __launch_bound
         for (int v = 0; v < V; v++) {
             const uint4 w = mine[v * step];
 #pragma unroll
-            for (int e = 0; e < E; e++) r[v][e] = __fmul_rn(m0, to_f(reinterpret_cast<const T*>(&w)[e]));      // (by one: nothing changes)
+            for (int e = 0; e < E; e++) r[v][e] = to_f(reinterpret_cast<const T*>(&w)[e]);
+        }
+        if (mix) {
+#pragma unroll
+            for (int v = 0; v < V; v++)
+#pragma unroll
+                for (int e = 0; e < E; e++) r[v][e] = __fmul_rn(m0, r[v][e]);
         }
         for (int j = 1; j < a.top; j++) {
             const float m = mix[j];
@@ -141,15 +160,16 @@ template <typename T, int V, int GATE, bool POST> __global__ void __launch_bound
             for (int v = 0; v < V; v++)
 #pragma unroll
                 for (int e = 0; e < E; e++) ss += (double)r[v][e] * r[v][e];
+            ask(a.post_weight);
             const float post = gated_rstd(block_sum(ss, s_sum[0]), a.per, a.eps);
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 const int i = v * step + tid;
                 if (i < words) {
                     float g[E];
-                    if constexpr (!KEPT) load_n<float, E, true>(a.post_weight + i * E, g);
+                    if constexpr (!KEPT && !EARLY) load_n<float, E, true>(a.post_weight + i * E, g);
 #pragma unroll
-                    for (int e = 0; e < E; e++) r[v][e] = __fmul_rn(__fmul_rn(r[v][e], post), KEPT ? pw[KEPT ? e : 0] : g[e]);
+                    for (int e = 0; e < E; e++) r[v][e] = __fmul_rn(__fmul_rn(r[v][e], post), KEPT ? pw[KEPT ? e : 0] : EARLY ? ew[EARLY ? v * E + e : 0] : g[e]);
                 }
             }
         }
@@ -176,6 +196,7 @@ template <typename T, int V, int GATE, bool POST> __global__ void __launch_bound
             if (POST) __syncthreads();      // (the next row writes what this one's sums are read from)
             continue;
         }
+        ask(a.weight);
         const float rstd = gated_rstd(block_sum(ss, s_sum[1]), a.per, a.eps);
         float top = 0;
 #pragma unroll
@@ -183,10 +204,10 @@ template <typename T, int V, int GATE, bool POST> __global__ void __launch_bound
             const int i = v * step + tid;
             if (i < words) {
                 float g[E];
-                if constexpr (!KEPT) load_n<float, E, true>(a.weight + i * E, g);
+                if constexpr (!KEPT && !EARLY) load_n<float, E, true>(a.weight + i * E, g);
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    r[v][e] = __fmul_rn(__fmul_rn(r[v][e], rstd), KEPT ? nw[KEPT ? e : 0] : g[e]);
+                    r[v][e] = __fmul_rn(__fmul_rn(r[v][e], rstd), KEPT ? nw[KEPT ? e : 0] : EARLY ? ew[EARLY ? v * E + e : 0] : g[e]);
                     top = max_nan(top, fabsf(r[v][e]));
                 }
             }
@@ -202,17 +223,17 @@ template <typename T, int V, int GATE, bool POST> __global__ void __launch_bound
     }
 }
 
-template <typename T, int V> cudaError_t add_gated_norm_words(const GatedNormArgs& a, int threads, int blocks, cudaStream_t st) {
+template <typename T, int V, int MOST> cudaError_t add_gated_norm_words(const GatedNormArgs& a, int threads, int blocks, cudaStream_t st) {
     const int gate = !a.gate ? 0 : a.gate_col == 0 ? 1 : 2;
     const dim3 grid((unsigned)std::min<int64_t>(a.rows, blocks));
-    const size_t most = V * 1024 * 48, smem = V * threads * (gate == 2 ? 48 : 32);
+    const size_t most = V * MOST * 48, smem = V * threads * (gate == 2 ? 48 : 32);
     if (a.post_weight)
-        return gate == 0   ? launch_with<add_gated_norm_kernel<T, V, 0, true>>(most, grid, threads, smem, st, a)
-               : gate == 1 ? launch_with<add_gated_norm_kernel<T, V, 1, true>>(most, grid, threads, smem, st, a)
-                           : launch_with<add_gated_norm_kernel<T, V, 2, true>>(most, grid, threads, smem, st, a);
-    return gate == 0   ? launch_with<add_gated_norm_kernel<T, V, 0, false>>(most, grid, threads, smem, st, a)
-           : gate == 1 ? launch_with<add_gated_norm_kernel<T, V, 1, false>>(most, grid, threads, smem, st, a)
-                       : launch_with<add_gated_norm_kernel<T, V, 2, false>>(most, grid, threads, smem, st, a);
+        return gate == 0   ? launch_with<add_gated_norm_kernel<T, V, 0, true, MOST>>(most, grid, threads, smem, st, a)
+               : gate == 1 ? launch_with<add_gated_norm_kernel<T, V, 1, true, MOST>>(most, grid, threads, smem, st, a)
+                           : launch_with<add_gated_norm_kernel<T, V, 2, true, MOST>>(most, grid, threads, smem, st, a);
+    return gate == 0   ? launch_with<add_gated_norm_kernel<T, V, 0, false, MOST>>(most, grid, threads, smem, st, a)
+           : gate == 1 ? launch_with<add_gated_norm_kernel<T, V, 1, false, MOST>>(most, grid, threads, smem, st, a)
+                       : launch_with<add_gated_norm_kernel<T, V, 2, false, MOST>>(most, grid, threads, smem, st, a);
 }
 // Few rows: as many threads as a row has words, up to 1024 (latency).  Many rows: four words per thread, so that several blocks of an SM (its 65 536 registers hold 1024 threads) cover one another's barriers, and the sums over
 // a block take fewer instructions.
@@ -226,8 +247,10 @@ template <typename T> cudaError_t add_gated_norm(const GatedNormArgs& a, cudaStr
     int sms = 0;
     const cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) return e;
-    const int n = a.hidden / E, v = n > 2048 || (a.rows > 2 * sms && n >= 256) ? 4 : n > 1024 || (a.rows > 2 * sms && n >= 64) ? 2 : 1, threads = ((n + v - 1) / v + 31) / 32 * 32, blocks = sms * std::max(1, 1024 / threads);
-    return v == 4 ? add_gated_norm_words<T, 4>(a, threads, blocks, st) : v == 2 ? add_gated_norm_words<T, 2>(a, threads, blocks, st) : add_gated_norm_words<T, 1>(a, threads, blocks, st);
+    const int n = a.hidden / E, many = a.rows > 2 * sms, v = n > 2048 || (many && n >= 256) ? 4 : n > 1024 || (many && n >= 64) ? 2 : 1, threads = ((n + v - 1) / v + 31) / 32 * 32;
+    if (v == 4 && threads <= 256) return add_gated_norm_words<T, 4, 256>(a, threads, sms * std::max(1, 512 / threads), st);
+    const int blocks = sms * std::max(1, 1024 / threads);
+    return v == 4 ? add_gated_norm_words<T, 4, 1024>(a, threads, blocks, st) : v == 2 ? add_gated_norm_words<T, 2, 1024>(a, threads, blocks, st) : add_gated_norm_words<T, 1, 1024>(a, threads, blocks, st);
 }
 
 }  // namespace dev

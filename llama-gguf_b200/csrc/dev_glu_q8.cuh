@@ -4,6 +4,7 @@
 // largest value of the row, and what lies next to the border between two numbers).
 #pragma once
 #include <algorithm>
+#include <type_traits>
 
 #include "dev_norm_q8.cuh"
 
@@ -22,7 +23,14 @@ struct GluQ8Args {
 __device__ __noinline__ double glu_exact(float gate, float up, int act) {
     const double g = gate;
     const double z = act == GLU_GELU ? 1.5957691216057308 * (g + 0.044715 * g * g * g) : g;      // 0.5 (1 + tanh(z)) is 1 / (1 + exp(-2 z))
-    return (act == GLU_RELU ? (isnan(g) ? g : fmax(g, 0.0)) : g / (1.0 + exp(-z))) * up;
+    if (act == GLU_RELU) return (isnan(g) ? g : fmax(g, 0.0)) * up;
+    const double d = 1.0 + exp(-z);
+    if (!(d < 1e300)) return g / d * up;
+    double r;      // 1 / d: its first bits, then two steps of Newton's method
+    asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(r) : "d"(d));
+    r = fma(r, fma(-d, r, 1.0), r);
+    r = fma(r, fma(-d, r, 1.0), r);
+    return g * r * up;
 }
 
 // largest of the block of values that are not negative
@@ -73,28 +81,39 @@ template <int ACT> __device__ __forceinline__ float glu_near(float g, float u) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
     return g * r * u;
 }
-template <typename T, int ACT> __device__ __noinline__ double glu_again(const T* gate, const T* up, int i) { return glu_exact(to_f(gate[i]), to_f(up[i]), ACT); }
+// the gate down to which y is made in f32 (z = -16, and -15.6)
+template <int ACT> __device__ __forceinline__ constexpr float glu_least() { return ACT == GLU_GELU ? -4.8f : -16.0f; }
+template <int ACT> __device__ __forceinline__ float glu_y(float g, float u) { return ACT != GLU_RELU && g <= glu_least<ACT>() ? (float)glu_exact(g, u, ACT) : glu_near<ACT>(g, u); }
+// the smallest of `least` and a word's elements (NaN does not count)
+template <typename T> __device__ __forceinline__ float word_min(const uint4& w, float least) {
+    if constexpr (sizeof(T) == 4) {
+        return fminf(fminf(least, fminf(__uint_as_float(w.x), __uint_as_float(w.y))), fminf(__uint_as_float(w.z), __uint_as_float(w.w)));
+    } else {
+        using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+        const T2* p = reinterpret_cast<const T2*>(&w);
+        const T2 m = __hmin2(__hmin2(p[0], p[1]), __hmin2(p[2], p[3]));
+        return fminf(least, fminf(to_f(m.x), to_f(m.y)));
+    }
+}
 // Rows of whole 16-byte words on 16 bytes: blocks stride over the rows; a row stays in registers as y (V words of each half per thread), the next one's words are on their way to shared memory meanwhile, where each thread
-// reads what it has copied itself.  The largest value is found among the f32 ones and those that may be it are made again in 64 bits; a number next to the border between two 8-bit ones is made again too (some
-// of a hundred thousand).
+// reads what it has copied itself.  A warp finds its largest value among the f32 ones and makes those that may be it again in 64 bits, so that the block needs one barrier a row; a number next to the border between
+// two 8-bit ones is made again too (some of a hundred thousand).
 template <typename T, int V, int ACT> __global__ void __launch_bounds__(1024) glu_q8_kernel(const GluQ8Args a) {
     before();
     constexpr int E = 16 / (int)sizeof(T);
     extern __shared__ uint4 glu_words[];      // [gate, up][V][threads]
-    __shared__ uint32_t s_max[2][32];
-    __shared__ unsigned long long s_top[2];
-    const int words = a.ff / E, tid = threadIdx.x, lane = tid & 31, warps = blockDim.x >> 5;
-    if (tid < 2) s_top[tid] = 0;
-    uint4 *g = glu_words + tid, *u = g + V * blockDim.x;
+    __shared__ double s_top[2][32];
+    const int words = a.ff / E, tid = threadIdx.x, lane = tid & 31, warps = blockDim.x >> 5, step = blockDim.x;
+    const uint4 *g = glu_words + tid, *u = g + V * step;
     const uint32_t to = (uint32_t)__cvta_generic_to_shared(g);
     auto copy = [&](int64_t row) {
         if (row < a.rows) {
             const uint4 *p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.x) + row * a.ldx) + tid, *q = p + words;
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                const bool there = v * (int)blockDim.x + tid < words;
-                copy_where<16>(to + v * blockDim.x * 16, there ? p + v * blockDim.x : a.x, there);
-                copy_where<16>(to + (V + v) * blockDim.x * 16, there ? q + v * blockDim.x : a.x, there);
+                const bool there = v * step + tid < words;
+                copy_where<16>(to + v * step * 16, there ? p + v * step : a.x, there);
+                copy_where<16>(to + (V + v) * step * 16, there ? q + v * step : a.x, there);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -102,75 +121,82 @@ template <typename T, int V, int ACT> __global__ void __launch_bounds__(1024) gl
     copy(blockIdx.x);
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-        const T *gate = reinterpret_cast<const T*>(a.x) + row * a.ldx, *up = gate + a.ff;
-        float y[V][E], top = 0, low = 0;
+        float y[V][E], most_of[V], top = 0, low = 0;
         asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const uint4 gw = g[v * blockDim.x], uw = u[v * blockDim.x];
-            float least = 0;
+            const uint4 gw = g[v * step], uw = u[v * step];
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                const float x = to_f(reinterpret_cast<const T*>(&gw)[e]);
-                y[v][e] = glu_near<ACT>(x, to_f(reinterpret_cast<const T*>(&uw)[e]));
-                if (ACT != GLU_RELU) least = fminf(least, glu_z<ACT>(x));
+            for (int e = 0; e < E; e++) y[v][e] = glu_near<ACT>(to_f(reinterpret_cast<const T*>(&gw)[e]), to_f(reinterpret_cast<const T*>(&uw)[e]));
+            if constexpr (ACT != GLU_RELU) {
+                const float least = word_min<T>(gw, 0.0f);
+                low = fminf(low, least);
+                if (least <= glu_least<ACT>()) {
+#pragma unroll
+                    for (int e = 0; e < E; e++) y[v][e] = glu_y<ACT>(to_f(reinterpret_cast<const T*>(&gw)[e]), to_f(reinterpret_cast<const T*>(&uw)[e]));
+                }
             }
-            if (least <= -16.0f) {
+            most_of[v] = 0;
 #pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (glu_z<ACT>(to_f(reinterpret_cast<const T*>(&gw)[e])) <= -16.0f) y[v][e] = (float)glu_exact(to_f(reinterpret_cast<const T*>(&gw)[e]), to_f(reinterpret_cast<const T*>(&uw)[e]), ACT);
-            }
-#pragma unroll
-            for (int e = 0; e < E; e++) top = max_nan(top, fabsf(y[v][e]));
-            low = fminf(low, least);
+            for (int e = 0; e < E; e++) most_of[v] = max_nan(most_of[v], fabsf(y[v][e]));
+            top = max_nan(top, most_of[v]);
         }
-        copy(row + gridDim.x);
-        uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-        if (lane == 0) s_max[turn][tid >> 5] = most;
-        __syncthreads();
-        most = __reduce_max_sync(0xffffffffu, lane < warps ? s_max[turn][lane] : 0u);
+        const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
         const float least = __uint_as_float(most) * (1.0f - 2 * kGluOffMost);
+        double mine = most < kInfBits ? 0.0 : INFINITY;
         if (most < kInfBits && top >= least) {
+            uint32_t which = 0;
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                const int i = v * blockDim.x + tid;
+            for (int v = 0; v < V; v++)
+                if (most_of[v] >= least) {
 #pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (fabsf(y[v][e]) >= least && i < words) atomicMax(&s_top[turn], (unsigned long long)__double_as_longlong(fabs(glu_again<T, ACT>(gate, up, i * E + e))));
+                    for (int e = 0; e < E; e++) which |= fabsf(y[v][e]) >= least ? 1u << (v * E + e) : 0u;
+                }
+            for (; which; which &= which - 1) {
+                const int o = __ffs(which) - 1;
+                mine = fmax(mine, fabs(glu_exact(to_f(reinterpret_cast<const T*>(g + o / E * step)[o % E]), to_f(reinterpret_cast<const T*>(u + o / E * step)[o % E]), ACT)));
             }
         }
+        // (largest of the warp: the lanes' doubles are not negative, so that their bits ascend as they do)
+        const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)__double2hiint(mine)), lo = __reduce_max_sync(0xffffffffu, (uint32_t)__double2hiint(mine) == hi ? (uint32_t)__double2loint(mine) : 0u);
+        if (lane == 0) s_top[turn][tid >> 5] = __hiloint2double((int)hi, (int)lo);
+        copy(row + gridDim.x);
         __syncthreads();
-        const double exact = most < kInfBits ? __longlong_as_double((long long)s_top[turn]) : INFINITY;
-        if (tid == 0) {
-            s_top[turn ^ 1] = 0;      // (the next row's: it was read before this row's first barrier)
-            a.scales[row] = glu_scale(exact);
+        const double other = lane < warps ? s_top[turn][lane] : 0.0;
+        const uint32_t bh = __reduce_max_sync(0xffffffffu, (uint32_t)__double2hiint(other)), bl = __reduce_max_sync(0xffffffffu, (uint32_t)__double2hiint(other) == bh ? (uint32_t)__double2loint(other) : 0u);
+        const double exact = __hiloint2double((int)bh, (int)bl);
+        if (tid == 0) a.scales[row] = glu_scale(exact);
+        int8_t* out = a.q + row * a.ldq;
+        if (!glu_live(exact)) {
+            const uint32_t none[E] = {};
+#pragma unroll
+            for (int v = 0; v < V; v++)
+                if (v * step + tid < words) store_bytes<E>(out + (v * step + tid) * E, none);
+            continue;
         }
-        const bool live = glu_live(exact);
         float inv;
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"((float)exact * (1.0f / 127.0f)));      // (from 2^-126 to 2^121: neither side leaves the range)
-        inv = live ? inv : 0.0f;
-        const float off = kGluOff - fmaxf(low, -16.0f) * kGluOffZ;
-        int8_t* out = a.q + row * a.ldq;
+        // rounded from both ends of what y may be: where the two are one number it is that
+        const float off = kGluOff - fmaxf(glu_z<ACT>(fmaxf(low, glu_least<ACT>())), -16.0f) * kGluOffZ, up = inv + inv * off, down = inv - inv * off;
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const int i = v * blockDim.x + tid;
+            const int i = v * step + tid;
             if (i < words) {
-                uint32_t n[E];
-                float near = 0;
+                uint32_t n[E], differ = 0;
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    const float t = live ? y[v][e] * inv : 0.0f, m = t + kRoundHere;
-                    n[e] = __float_as_uint(m);
-                    near = fmaxf(near, fmaf(fabsf(t), off, fabsf(t - (m - kRoundHere))));
-                }
-                if (near >= 0.5f) {
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        const float t = y[v][e] * inv, m = t + kRoundHere;
-                        if (fmaf(fabsf(t), off, fabsf(t - (m - kRoundHere))) >= 0.5f) n[e] = (uint32_t)__double2int_rn(glu_again<T, ACT>(gate, up, i * E + e) * (127.0 / exact));
-                    }
+                    n[e] = __float_as_uint(fmaf(y[v][e], up, kRoundHere));
+                    differ |= n[e] ^ __float_as_uint(fmaf(y[v][e], down, kRoundHere));
                 }
                 store_bytes<E>(out + i * E, n);
+                if (differ) {      // (the row's words are from memory again: the next one's have their place)
+                    const T *p = reinterpret_cast<const T*>(a.x) + row * a.ldx + i * E, *q = p + a.ff;
+#pragma unroll 1
+                    for (int e = 0; e < E; e++) {
+                        const float x = to_f(p[e]), z = to_f(q[e]), f = glu_y<ACT>(x, z);
+                        if (fmaf(f, up, kRoundHere) != fmaf(f, down, kRoundHere)) out[i * E + e] = (int8_t)__double2int_rn(glu_exact(x, z, ACT) * (127.0 / exact));
+                    }
+                }
             }
         }
     }

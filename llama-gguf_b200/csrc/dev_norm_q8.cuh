@@ -61,9 +61,11 @@ template <int E> __device__ __forceinline__ void store_bytes(int8_t* out, const 
 }
 // E values times `inv` (at most 127 and its roundings) as 8-bit numbers (inv 0: zeros)
 template <int E> __device__ __forceinline__ void store_q8(int8_t* out, const float (&y)[E], float inv) {
-    uint32_t n[E];
+    uint32_t n[E] = {};
+    if (inv != 0.0f) {
 #pragma unroll
-    for (int e = 0; e < E; e++) n[e] = inv == 0.0f ? 0u : __float_as_uint(__fadd_rn(__fmul_rn(y[e], inv), kRoundHere));
+        for (int e = 0; e < E; e++) n[e] = __float_as_uint(__fadd_rn(__fmul_rn(y[e], inv), kRoundHere));
+    }
     store_bytes<E>(out, n);
 }
 

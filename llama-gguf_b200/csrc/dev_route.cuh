@@ -3,8 +3,9 @@
 // p = softmax(z) or 1 / (1 + exp(-z)); c = z, or p + correction; experts by c, the lower number first among equals; weights p, or p over the sum of the chosen ones', times a factor.
 // What decides is made in 64 bits: scores of 32 bits next to one another would be chosen by their rounding.
 //
-// A warp per token; expert e is lane e % 32's value e / 32.  A choice is the largest key of all lanes (keys are the values' bits, so that they ascend as unsigned numbers) by redux.sync, its
-// high word, then its low word among those that have it, then the lowest expert.
+// A warp per token; expert e is lane e % 32's value e / 32.  A choice is the largest key of all lanes (keys are the values' bits, so that they ascend as unsigned numbers) by redux.sync, then the lowest expert that
+// has it.  Logits choose as they are.  Scores are made in f32 first (off by less than 2^-21) and choose where everything chosen is further from what follows it than that may be off; the other tokens (some of a
+// thousand) go through the same in 64 bits, which took 34 us for 8192 tokens of 256 experts in 8 groups where all did.
 #pragma once
 #include <algorithm>
 
@@ -38,51 +39,52 @@ __device__ __forceinline__ uint64_t route_max(uint64_t k) {
     return (uint64_t)hi << 32 | lo;
 }
 
-template <typename T, int V> __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_experts_kernel(const RouteArgs a) {
-    before();
-    __shared__ uint64_t s_key[ROUTE_WARPS][V * 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t token = (int64_t)blockIdx.x * ROUTE_WARPS + warp;
-    if (token >= a.tokens) return;
-    const T* z = reinterpret_cast<const T*>(a.logits) + token * a.ld;
-    float x[V];
-    bool nan = false;
-#pragma unroll
-    for (int v = 0; v < V; v++) {
-        x[v] = v * 32 + lane < a.n ? to_f(z[v * 32 + lane]) : -INFINITY;
-        nan |= isnan(x[v]) || (!a.sigmoid && x[v] == INFINITY);
+// Group `lane`'s two best keys (of `each` neighbours in s_key; `of` lanes share a group's): read in turns, so that lanes of different groups meet different banks.
+template <typename K> __device__ __forceinline__ void route_two(const K* s_key, int lane, int groups, int each, K& first, K& second) {
+    int of = 1;
+    while (of * 2 * groups <= 32) of *= 2;
+    const int mine = lane / of, part = lane % of;
+    first = second = 0;
+    if (mine < groups)
+        for (int i = part; i < each; i += of) {
+            int at = i + mine * of;
+            at = at < each ? at : at % each;
+            // (the turn keeps each lane's set of places: those of `part` modulo `of` where `of` divides each, any fair split otherwise)
+            const K k = s_key[mine * each + (each % of == 0 ? at : i)];
+            second = max(second, min(first, k));
+            first = max(first, k);
+        }
+    for (int o = 1; o < of; o <<= 1) {
+        const K f = __shfl_xor_sync(0xffffffffu, first, o), s = __shfl_xor_sync(0xffffffffu, second, o);
+        second = max(min(first, f), max(second, s));
+        first = max(first, f);
     }
-    nan = __any_sync(0xffffffffu, nan);      // (no weights then; the choice goes by the logits)
-    float most = -INFINITY;
-#pragma unroll
-    for (int v = 0; v < V; v++) most = fmaxf(most, x[v]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    // lane g: group g's
+    const int from = lane * of & 31;
+    const K f = __shfl_sync(0xffffffffu, first, from), s = __shfl_sync(0xffffffffu, second, from);
+    first = lane < groups ? f : 0;
+    second = lane < groups ? s : 0;
+}
+
+// One token in 64 bits.  x: its logits, most: their largest; returns this lane's (place's) expert, and its logit in `at`.
+template <int V> __device__ __noinline__ int route_exactly(const RouteArgs& a, const float* x, float most, bool by_score, bool nan, uint64_t* s_key, int lane, float* at) {
     double total = 0;
     if (!a.sigmoid) {
-#pragma unroll
         for (int v = 0; v < V; v++) total += x[v] > -INFINITY ? exp((double)x[v] - most) : 0.0;
 #pragma unroll
         for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     }
-    auto score = [&](float v) { return !(v > -INFINITY) ? 0.0 : a.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : exp((double)v - most) / total; };
-    const bool by_score = a.correction && !nan;
+    auto score = [&](float v) { return a.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : exp((double)v - most) / total; };
     uint64_t key[V];
 #pragma unroll
     for (int v = 0; v < V; v++) key[v] = !(x[v] > -INFINITY) ? 0 : route_key(by_score ? score(x[v]) + a.correction[v * 32 + lane] : (double)x[v]);
     if (a.groups > 1) {
-        // a lane per group: its two best
         const int each = a.n / a.groups;
 #pragma unroll
-        for (int v = 0; v < V; v++) s_key[warp][v * 32 + lane] = by_score || nan ? key[v] : key[v] ? route_key(score(x[v])) : 0;
+        for (int v = 0; v < V; v++) s_key[v * 32 + lane] = by_score || nan ? key[v] : key[v] ? route_key(score(x[v])) : 0;
         __syncwarp();
-        uint64_t first = 0, second = 0;
-        if (lane < a.groups)
-            for (int i = 0; i < each; i++) {
-                const uint64_t k = s_key[warp][lane * each + i];
-                second = max(second, min(first, k));
-                first = max(first, k);
-            }
+        uint64_t first, second;
+        route_two<uint64_t>(s_key, lane, a.groups, each, first, second);
         uint64_t value = second && !nan ? route_key(route_value(first) + route_value(second)) : first;
         uint32_t kept = 0;
         for (int i = 0; i < a.top_groups; i++) {
@@ -95,8 +97,8 @@ template <typename T, int V> __global__ void __launch_bounds__(ROUTE_WARPS * 32)
         for (int v = 0; v < V; v++)
             if (v * 32 + lane < a.n && !(kept >> ((v * 32 + lane) / each) & 1)) key[v] = 0;
     }
-    int mine = -1;      // lane j: the token's expert j
-    float at = -INFINITY;
+    int mine = -1;
+    *at = -INFINITY;
     for (int j = 0; j < a.top; j++) {
         uint64_t k = 0;
         int e = 0;
@@ -107,17 +109,140 @@ template <typename T, int V> __global__ void __launch_bounds__(ROUTE_WARPS * 32)
         const uint64_t best = route_max(k);
         const int who = best ? (int)__reduce_min_sync(0xffffffffu, k == best ? (uint32_t)e : 0xffffffffu) : -1;
         const float value = __shfl_sync(0xffffffffu, l, who & 31);
-        if (lane == j) mine = who, at = best ? value : -INFINITY;
+        if (lane == j) mine = who, *at = best ? value : -INFINITY;
 #pragma unroll
         for (int v = 0; v < V; v++)
             if (v * 32 + lane == who) key[v] = 0;
     }
-    double p = score(at);
-    if (a.renormalise) {
-        double sum = p;
+    return mine;
+}
+
+__device__ __forceinline__ uint32_t route_key32(float c) {
+    if (!(c > -INFINITY)) return 0;
+    const uint32_t b = __float_as_uint(c + 0.0f);
+    return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float route_value32(uint32_t key) { return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key); }
+
+template <typename T, int V> __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_experts_kernel(const RouteArgs a) {
+    before();
+    __shared__ uint64_t s_key[ROUTE_WARPS][V * 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t token = (int64_t)blockIdx.x * ROUTE_WARPS + warp;
+    if (token >= a.tokens) return;
+    const T* z = reinterpret_cast<const T*>(a.logits) + token * a.ld;
+    float x[V];
 #pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        p = sum > 0 ? p / sum : p;
+    for (int v = 0; v < V; v++) x[v] = v * 32 + lane < a.n ? to_f(z[v * 32 + lane]) : -INFINITY;
+    float most = -INFINITY;
+    bool nan = false;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        nan |= isnan(x[v]) || (!a.sigmoid && x[v] == INFINITY);
+        most = fmaxf(most, x[v]);
+    }
+    nan = __any_sync(0xffffffffu, nan);      // (no weights then; the choice goes by the logits)
+    {
+        const uint32_t k = __reduce_max_sync(0xffffffffu, route_key32(most));
+        most = k ? route_value32(k) : -INFINITY;
+    }
+    const bool by_score = a.correction && !nan, scores = by_score || (a.groups > 1 && !nan);
+    // the choice in f32; `close`: it may be another one in 64 bits
+    float c[V];
+    bool close = false;
+    if (scores) {
+        float per = 1.0f;
+        if (!a.sigmoid) {
+            double total = 0;
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                c[v] = expf(x[v] - most);
+                total += x[v] > -INFINITY ? c[v] : 0.0f;
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+            per = (float)(1.0 / total);
+        }
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const float p = a.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-x[v])) : c[v] * per;
+            c[v] = !(x[v] > -INFINITY) ? -INFINITY : by_score ? p + a.correction[v * 32 + lane] : p;
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; v++) c[v] = x[v];
+    }
+    uint32_t key[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) key[v] = route_key32(c[v]);
+    if (a.groups > 1) {
+        const int each = a.n / a.groups;
+        uint32_t* s_key32 = reinterpret_cast<uint32_t*>(s_key[warp]);
+#pragma unroll
+        for (int v = 0; v < V; v++) s_key32[v * 32 + lane] = key[v];
+        __syncwarp();
+        uint32_t first, second;
+        route_two<uint32_t>(s_key32, lane, a.groups, each, first, second);
+        uint32_t value = second && !nan ? route_key32(route_value32(first) + route_value32(second)) : first, kept = 0, least = 0;
+        for (int i = 0; i < a.top_groups; i++) {
+            least = __reduce_max_sync(0xffffffffu, value);
+            const int who = __reduce_min_sync(0xffffffffu, value == least ? lane : 32);
+            if (least) kept |= 1u << who;
+            if (lane == who) value = 0;
+        }
+        const uint32_t next = __reduce_max_sync(0xffffffffu, value);
+        if (scores && next && least) {      // (a sum of two: 2^-20, and a rounding)
+            const float lo = route_value32(next), hi = route_value32(least);
+            close = !(hi - lo > 0x1p-18f + 0x1p-21f * fabsf(hi));
+        }
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            if (scores && !by_score) key[v] = route_key32(x[v]);      // (chosen by logits)
+            if (v * 32 + lane < a.n && !(kept >> ((v * 32 + lane) / each) & 1)) key[v] = 0;
+        }
+    }
+    int mine = -1;      // lane j: the token's expert j
+    float at = -INFINITY, before_it = INFINITY;
+    for (int j = 0; j < a.top + (by_score ? 1 : 0); j++) {
+        uint32_t k = 0;
+        int e = 0;
+        float l = 0;
+#pragma unroll
+        for (int v = V - 1; v >= 0; v--)
+            if (key[v] >= k) k = key[v], e = v * 32 + lane, l = x[v];
+        const uint32_t best = __reduce_max_sync(0xffffffffu, k);
+        if (by_score) {
+            const float value = route_value32(best);
+            if (best && !(before_it - value > 0x1p-19f + 0x1p-22f * fabsf(value))) close = true;
+            before_it = value;
+            if (j == a.top) break;
+        }
+        const int who = best ? (int)__reduce_min_sync(0xffffffffu, k == best ? (uint32_t)e : 0xffffffffu) : -1;
+        const float logit = __shfl_sync(0xffffffffu, l, who & 31);
+        if (lane == j) mine = who, at = best ? logit : -INFINITY;
+#pragma unroll
+        for (int v = 0; v < V; v++)
+            if (v * 32 + lane == who) key[v] = 0;
+    }
+    if (close) mine = route_exactly<V>(a, x, most, by_score, nan, s_key[warp], lane, &at);
+    // weights: in 64 bits
+    double p = 0;
+    if (a.sigmoid) {
+        if (at > -INFINITY) p = 1.0 / (1.0 + exp(-(double)at));
+    } else if (at > -INFINITY) {
+        p = exp((double)at - most);
+    }
+    double total = 0;
+    if (a.renormalise) {
+        total = p;
+    } else if (!a.sigmoid) {
+#pragma unroll
+        for (int v = 0; v < V; v++) total += x[v] > -INFINITY ? exp((double)x[v] - most) : 0.0;
+    }
+    if (a.renormalise || !a.sigmoid) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        p = total > 0 ? p / total : p;
     }
     if (lane < a.top) {
         a.experts[token * a.top + lane] = mine;
