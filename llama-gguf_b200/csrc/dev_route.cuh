@@ -3,9 +3,10 @@
 // p = softmax(z) or 1 / (1 + exp(-z)); c = z, or p + correction; experts by c, the lower number first among equals; weights p, or p over the sum of the chosen ones', times a factor.
 // What decides is made in 64 bits: scores of 32 bits next to one another would be chosen by their rounding.
 //
-// A warp per token; expert e is lane e % 32's value e / 32.  A choice is the largest key of all lanes (keys are the values' bits, so that they ascend as unsigned numbers) by redux.sync, then the lowest expert that
-// has it.  Logits choose as they are.  Scores are made in f32 first (off by less than 2^-21) and choose where everything chosen is further from what follows it than that may be off; the other tokens (some of a
-// thousand) go through the same in 64 bits, which took 34 us for 8192 tokens of 256 experts in 8 groups where all did.
+// A warp per token; expert e is lane e % 32's value e / 32.  Keys ascend as unsigned numbers: 22 bits of the value (16-bit logits whole, f32 logits' first bits, scores in fixed point between the token's least and
+// largest), then 1023 - e, so that one redux.sync gives a choice and its expert, the lower one among equals; each lane's keys are sorted once and the chosen one's lane moves up.  Scores are made in f32 (off by less
+// than 2^-21).  Where two that follow one another are closer than all that may be off, the token (some of a hundred) is chosen for again with 64-bit scores and keys, which took 34 us for 8192 tokens of 256
+// experts in 8 groups where all did.
 #pragma once
 #include <algorithm>
 
@@ -23,6 +24,7 @@ struct RouteArgs {
     int64_t ld, tokens;
     int n, top, groups, top_groups, sigmoid, renormalise;
     float scale;
+    uint32_t per_group;      // 2^20 / experts of a group, rounded up: e * per_group >> 20 is expert e's group
 };
 
 // ascending as unsigned; 0: not to be chosen
@@ -43,14 +45,12 @@ __device__ __forceinline__ uint64_t route_max(uint64_t k) {
 template <typename K> __device__ __forceinline__ void route_two(const K* s_key, int lane, int groups, int each, K& first, K& second) {
     int of = 1;
     while (of * 2 * groups <= 32) of *= 2;
-    const int mine = lane / of, part = lane % of;
+    const int mine = lane / of, part = lane % of, turn = each % of == 0 ? mine * of % each : 0;
     first = second = 0;
     if (mine < groups)
         for (int i = part; i < each; i += of) {
-            int at = i + mine * of;
-            at = at < each ? at : at % each;
-            // (the turn keeps each lane's set of places: those of `part` modulo `of` where `of` divides each, any fair split otherwise)
-            const K k = s_key[mine * each + (each % of == 0 ? at : i)];
+            const int at = i + turn;      // (the places of a lane are those of its part, whichever it begins at)
+            const K k = s_key[mine * each + (at < each ? at : at - each)];
             second = max(second, min(first, k));
             first = max(first, k);
         }
@@ -124,32 +124,47 @@ __device__ __forceinline__ uint32_t route_key32(float c) {
 }
 __device__ __forceinline__ float route_value32(uint32_t key) { return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key); }
 
-template <typename T, int V> __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_experts_kernel(const RouteArgs a) {
+// descending
+template <int V> __device__ __forceinline__ void route_sort(uint32_t (&k)[V]) {
+#pragma unroll
+    for (int size = 2; size <= V; size *= 2)
+#pragma unroll
+        for (int apart = size / 2; apart; apart /= 2)
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const int o = i ^ apart;
+                if (o > i) {
+                    const uint32_t hi = max(k[i], k[o]), lo = min(k[i], k[o]);
+                    k[i] = i & size ? lo : hi;
+                    k[o] = i & size ? hi : lo;
+                }
+            }
+}
+
+template <typename T, int V> __global__ void __launch_bounds__(ROUTE_WARPS * 32, V <= 4 ? 12 : V == 8 ? 8 : 4) route_experts_kernel(const RouteArgs a) {
     before();
     __shared__ uint64_t s_key[ROUTE_WARPS][V * 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t token = (int64_t)blockIdx.x * ROUTE_WARPS + warp;
     if (token >= a.tokens) return;
     const T* z = reinterpret_cast<const T*>(a.logits) + token * a.ld;
-    float x[V];
+    float x[V], most = -INFINITY;
+    bool nan = false;
 #pragma unroll
     for (int v = 0; v < V; v++) x[v] = v * 32 + lane < a.n ? to_f(z[v * 32 + lane]) : -INFINITY;
-    float most = -INFINITY;
-    bool nan = false;
 #pragma unroll
     for (int v = 0; v < V; v++) {
         nan |= isnan(x[v]) || (!a.sigmoid && x[v] == INFINITY);
         most = fmaxf(most, x[v]);
     }
     nan = __any_sync(0xffffffffu, nan);      // (no weights then; the choice goes by the logits)
-    {
+    if (!a.sigmoid || nan) {
         const uint32_t k = __reduce_max_sync(0xffffffffu, route_key32(most));
         most = k ? route_value32(k) : -INFINITY;
     }
     const bool by_score = a.correction && !nan, scores = by_score || (a.groups > 1 && !nan);
-    // the choice in f32; `close`: it may be another one in 64 bits
-    float c[V];
-    bool close = false;
+    bool close = false;      // the choice may be another one in 64 bits
+    float c[V];              // scores (with the correction)
     if (scores) {
         float per = 1.0f;
         if (!a.sigmoid) {
@@ -165,25 +180,21 @@ template <typename T, int V> __global__ void __launch_bounds__(ROUTE_WARPS * 32)
         }
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const float p = a.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-x[v])) : c[v] * per;
+            float p = c[v] * per;
+            if (a.sigmoid) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(1.0f + __expf(-x[v])));
             c[v] = !(x[v] > -INFINITY) ? -INFINITY : by_score ? p + a.correction[v * 32 + lane] : p;
         }
-    } else {
-#pragma unroll
-        for (int v = 0; v < V; v++) c[v] = x[v];
     }
-    uint32_t key[V];
-#pragma unroll
-    for (int v = 0; v < V; v++) key[v] = route_key32(c[v]);
+    uint32_t kept = 0xffffffffu;
     if (a.groups > 1) {
-        const int each = a.n / a.groups;
         uint32_t* s_key32 = reinterpret_cast<uint32_t*>(s_key[warp]);
 #pragma unroll
-        for (int v = 0; v < V; v++) s_key32[v * 32 + lane] = key[v];
+        for (int v = 0; v < V; v++) s_key32[v * 32 + lane] = route_key32(scores ? c[v] : x[v]);
         __syncwarp();
-        uint32_t first, second;
-        route_two<uint32_t>(s_key32, lane, a.groups, each, first, second);
-        uint32_t value = second && !nan ? route_key32(route_value32(first) + route_value32(second)) : first, kept = 0, least = 0;
+        uint32_t first, second, least = 0;
+        route_two<uint32_t>(s_key32, lane, a.groups, a.n / a.groups, first, second);
+        uint32_t value = second && !nan ? route_key32(route_value32(first) + route_value32(second)) : first;
+        kept = 0;
         for (int i = 0; i < a.top_groups; i++) {
             least = __reduce_max_sync(0xffffffffu, value);
             const int who = __reduce_min_sync(0xffffffffu, value == least ? lane : 32);
@@ -195,43 +206,56 @@ template <typename T, int V> __global__ void __launch_bounds__(ROUTE_WARPS * 32)
             const float lo = route_value32(next), hi = route_value32(least);
             close = !(hi - lo > 0x1p-18f + 0x1p-21f * fabsf(hi));
         }
+    }
+    // keys, and by how much (in their 22 bits) a choice must be ahead of what follows it
+    uint32_t key[V], ahead = sizeof(T) == 2 ? 0 : 1;
+    if (by_score) {
+        float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            if (scores && !by_score) key[v] = route_key32(x[v]);      // (chosen by logits)
-            if (v * 32 + lane < a.n && !(kept >> ((v * 32 + lane) / each) & 1)) key[v] = 0;
+            hi = fmaxf(hi, c[v]);
+            if (c[v] > -INFINITY) lo = fminf(lo, c[v]);
+        }
+        const uint32_t top = __reduce_max_sync(0xffffffffu, route_key32(hi)), bottom = __reduce_min_sync(0xffffffffu, lo < INFINITY ? route_key32(lo) : 0xffffffffu);
+        hi = route_value32(top);
+        lo = route_value32(bottom);
+        const float range = fmaxf(hi - lo, 0x1p-10f), per = 4194000.0f / range;      // (below 2^22 - 2 for any rounding)
+        close |= !(range < 1e30f) && top;
+        ahead = (uint32_t)fminf((0x1p-19f + 0x1p-22f * fmaxf(fabsf(lo), fabsf(hi))) * per + 3.0f, 4e6f);
+#pragma unroll
+        for (int v = 0; v < V; v++) key[v] = c[v] > -INFINITY ? ((uint32_t)fminf((c[v] - lo) * per, 4194000.0f) + 1) << 10 : 0;
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const uint32_t k = route_key32(x[v]);      // (16-bit numbers: the last 13 or 16 bits are all zeros or all ones)
+            key[v] = k ? (k >> 10 ? k & ~1023u : 1024u) : 0;
         }
     }
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const int e = v * 32 + lane;
+        key[v] = key[v] && kept >> ((uint32_t)e * a.per_group >> 20 & 31) & 1 ? key[v] | (uint32_t)(1023 - e) : 0;
+    }
+    route_sort<V>(key);
     int mine = -1;      // lane j: the token's expert j
-    float at = -INFINITY, before_it = INFINITY;
-    for (int j = 0; j < a.top + (by_score ? 1 : 0); j++) {
-        uint32_t k = 0;
-        int e = 0;
-        float l = 0;
+    uint32_t last = 0xffffffffu;
+    for (int j = 0; j <= a.top; j++) {
+        const uint32_t best = __reduce_max_sync(0xffffffffu, key[0]);
+        if (!best) break;
+        close |= (last >> 10) - (best >> 10) < ahead;
+        last = best;
+        if (lane == j && j < a.top) mine = 1023 - (int)(best & 1023u);
+        if (key[0] == best) {
 #pragma unroll
-        for (int v = V - 1; v >= 0; v--)
-            if (key[v] >= k) k = key[v], e = v * 32 + lane, l = x[v];
-        const uint32_t best = __reduce_max_sync(0xffffffffu, k);
-        if (by_score) {
-            const float value = route_value32(best);
-            if (best && !(before_it - value > 0x1p-19f + 0x1p-22f * fabsf(value))) close = true;
-            before_it = value;
-            if (j == a.top) break;
+            for (int v = 0; v + 1 < V; v++) key[v] = key[v + 1];
+            key[V - 1] = 0;
         }
-        const int who = best ? (int)__reduce_min_sync(0xffffffffu, k == best ? (uint32_t)e : 0xffffffffu) : -1;
-        const float logit = __shfl_sync(0xffffffffu, l, who & 31);
-        if (lane == j) mine = who, at = best ? logit : -INFINITY;
-#pragma unroll
-        for (int v = 0; v < V; v++)
-            if (v * 32 + lane == who) key[v] = 0;
     }
+    float at = mine >= 0 ? to_f(z[mine]) : -INFINITY;
     if (close) mine = route_exactly<V>(a, x, most, by_score, nan, s_key[warp], lane, &at);
     // weights: in 64 bits
     double p = 0;
-    if (a.sigmoid) {
-        if (at > -INFINITY) p = 1.0 / (1.0 + exp(-(double)at));
-    } else if (at > -INFINITY) {
-        p = exp((double)at - most);
-    }
+    if (at > -INFINITY) p = a.sigmoid ? 1.0 / (1.0 + exp(-(double)at)) : exp((double)at - most);
     double total = 0;
     if (a.renormalise) {
         total = p;

@@ -22,7 +22,8 @@ extern "C" int b200_dev_route_experts(const b200_route* a) {
         if (!std::isfinite(a->scale)) return bad(op, "scale is not finite");
         if (a->tokens == 0) return B200_OK;
         if (!a->logits || !a->experts || !a->weights) return bad(op, "null pointer");
-        const RouteArgs r{a->logits, a->correction, a->experts, a->weights, a->ld, a->tokens, a->n, a->top, a->groups, a->top_groups, a->sigmoid != 0, a->renormalise != 0, a->scale};
+        const RouteArgs r{a->logits, a->correction, a->experts, a->weights, a->ld, a->tokens, a->n, a->top, a->groups, a->top_groups, a->sigmoid != 0, a->renormalise != 0, a->scale,
+                          ((1u << 20) + a->n / a->groups - 1) / (a->n / a->groups)};
         return on_device(op, a->device, [&] { return by_type(a->type, [&](auto t) { return route_experts<decltype(t)>(r, (cudaStream_t)a->stream); }); });
     });
 }
