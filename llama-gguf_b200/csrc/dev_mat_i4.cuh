@@ -11,7 +11,7 @@
 // for another's weights.  With experts every block lists the pairs (token, expert) by expert first, all in the same order; up to that many pairs of an expert are a unit for each tile.
 //   few rows (up to 16): the weights' bytes.  Two blocks per SM have consecutive units of one tile each; its warps share their steps of 256 channels evenly, whichever unit they are of, and leave the sums of a unit that two or
 //   more warps have a part of in shared memory for the end.  Rows of a come from L1 and L2.
-//   more rows (up to 64 at a time): rows of a cost as much as weights.  A block has eight tiles; its teams of four warps have a part of the channels each, whose rows of a serve all eight.  With few units the
+//   more rows (up to 64 at a time): rows of a cost as much as weights.  A block has eight tiles; its teams of eight warps have a part of the channels each, whose rows of a serve all eight.  With few units the
 //   blocks of a cluster share the channels of one.
 #pragma once
 #include <algorithm>
@@ -39,6 +39,7 @@ struct MatI4Args {
     int tokens;     // rows of `experts`
     int first;      // the first row of out that this launch makes; `rows` counts from there
     int split;      // blocks of a cluster, which share a unit's channels
+    int most, ring;      // more rows: rows that a step has room for (a multiple of eight), steps of a team's ring
 };
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -154,25 +155,20 @@ template <typename S> __device__ __forceinline__ float2 i4_scales(const uint8_t*
 }
 // What a ring holds of a step of C tiles' channels of one tile of rows: the weights, then the groups' scales.
 template <typename S, int GROUP, int C> __host__ __device__ constexpr int i4_slot() { return C * I4_TILE + 16 * (int)sizeof(S) * (64 * C / GROUP); }
-// ... copied: step s of the tile whose weights and scales are at w and d
-template <typename S, int GROUP, int C> __device__ __forceinline__ void i4_copy(const MatI4Args& a, uint32_t to, const uint8_t* w, const uint8_t* d, int s, int lane) {
-    constexpr int GS = 64 * C / GROUP, SB = 16 * (int)sizeof(S), WORDS = GS * SB / 8;
-    const uint8_t *p = w + (int64_t)s * (C * I4_TILE) + lane * 16, *q = d + (int64_t)s * (GS * SB) + lane * 8;
-    to += lane * 16;
-    if ((s + 1) * C <= a.steps && (s + 1) * GS <= a.groups) {
+// ... copied, from w (this lane's 16 bytes of the step's first tile) and d (its 8 bytes of the scales).  A whole step, with nothing to be asked; and the last one of a tile, with zeros behind the last channel.
+template <typename S, int GROUP, int C> __device__ __forceinline__ void i4_copy(uint32_t to, const uint8_t* w, const uint8_t* d, int lane) {
+    constexpr int WORDS = 64 * C / GROUP * 2 * (int)sizeof(S);      // 8-byte words of the scales
 #pragma unroll
-        for (int c = 0; c < C; c++) copy_where<16>(to + c * I4_TILE, p + c * I4_TILE, true);
+    for (int c = 0; c < C; c++) copy_all<16>(to + c * I4_TILE + lane * 16, w + c * I4_TILE);
 #pragma unroll
-        for (int c = 0; c < WORDS; c += 32)
-            if (c + 32 <= WORDS || lane < WORDS - c) copy_where<8>(to - lane * 8 + C * I4_TILE + c * 8, q + c * 8, true);
-    } else {      // (the last step: zeros behind the last channel)
-        const int room = a.steps - s * C, scales = (a.groups - s * GS) * (SB / 8);      // tiles, and 8-byte words of the scales
-#pragma unroll
-        for (int c = 0; c < C; c++) copy_where<16>(to + c * I4_TILE, c < room ? p + c * I4_TILE : a.w, c < room);
-#pragma unroll
-        for (int c = 0; c < WORDS; c += 32)
-            if (c + 32 <= WORDS || lane < WORDS - c) copy_where<8>(to - lane * 8 + C * I4_TILE + c * 8, c + lane < scales ? q + c * 8 : a.w, c + lane < scales);
-    }
+    for (int c = 0; c < WORDS; c += 32)
+        if (c + 32 <= WORDS || lane < WORDS - c) copy_all<8>(to + C * I4_TILE + c * 8 + lane * 8, d + c * 8);
+}
+template <typename S, int GROUP, int C> __device__ __noinline__ void i4_copy_last(uint32_t to, const uint8_t* w, const uint8_t* d, int tiles, int groups, int lane) {      // how many there are left
+    constexpr int WORDS = 64 * C / GROUP * 2 * (int)sizeof(S);
+    const uint8_t* any = w - lane * 16;
+    for (int c = 0; c < C; c++) copy_where<16>(to + c * I4_TILE + lane * 16, c < tiles ? w + c * I4_TILE : any, c < tiles);
+    for (int c = lane; c < WORDS; c += 32) copy_where<8>(to + C * I4_TILE + c * 8, c < groups * 2 * (int)sizeof(S) ? d + (c - lane) * 8 : any, c < groups * 2 * (int)sizeof(S));
 }
 
 // ------------------------------------------------------------------------------------------------------------- few rows
@@ -205,13 +201,15 @@ template <typename S, int GROUP, int TC, int NT> struct I4Step {
     __device__ __forceinline__ void add(float (&acc)[NT][4], const uint8_t* in, int lane) const {
         const int g = lane >> 2, t = lane & 3, group = g / TC;
         const uint8_t* scales = in + 4 * I4_TILE + g * 2 * sizeof(S);
+        uint4 tile;
 #pragma unroll
         for (int z = 0; z < SETS; z++) {
             int sum[NT][4];
 #pragma unroll
             for (int i = 0; i < PER * GC; i++) {
                 const int k = z * PER * GC + i;      // the chunk: half a tile
-                const uint2 v = *reinterpret_cast<const uint2*>(in + (k / 2) * I4_TILE + lane * 16 + (k % 2) * 8);
+                if (k % 2 == 0) tile = *reinterpret_cast<const uint4*>(in + (k / 2) * I4_TILE + lane * 16);
+                const uint2 v = k % 2 ? make_uint2(tile.z, tile.w) : make_uint2(tile.x, tile.y);
                 const uint32_t a0 = (v.x << 4) & 0xf0f0f0f0u, a1 = (v.y << 4) & 0xf0f0f0f0u, a2 = v.x & 0xf0f0f0f0u, a3 = v.y & 0xf0f0f0f0u;
 #pragma unroll
                 for (int j = 0; j < NT; j++) {
@@ -302,18 +300,23 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
         int c = (int)((u0 + v0) / a.tiles), tile = (int)(u0 + v0 - (int64_t)c * a.tiles), s = f0 - v0 * whole;
         I4Chunk x = i4_chunk<CHUNK>(a, l, c);
         // copies, I4_RING - 1 steps ahead of the products
-        int cc = c, ct = tile, ce = x.e, cs = s, left = f1 - f0, into = 0;
+        int cc = c, ct = tile, ce = x.e, cs = s, left = f1 - f0;
+        const int full = a.steps / 4;      // (whole steps of a tile: of its scales too, whose groups are whole)
+        uint32_t into = ring;
         const uint8_t *cw = nullptr, *cd = nullptr;
         auto place = [&]() {
             const int64_t at = (int64_t)ce * a.tiles + ct;
-            cw = a.w + at * a.steps * I4_TILE;
-            cd = reinterpret_cast<const uint8_t*>(a.ws) + at * a.groups * SB;
+            cw = a.w + (at * a.steps + cs * 4) * I4_TILE + lane * 16;
+            cd = reinterpret_cast<const uint8_t*>(a.ws) + (at * a.groups + cs * (256 / GROUP)) * SB + lane * 8;
         };
         place();
         auto copy = [&]() {
             if (left > 0) {
-                i4_copy<S, GROUP, 4>(a, ring + into * SLOT, cw, cd, cs, lane);
-                into = into + 1 == I4_RING ? 0 : into + 1;
+                if (cs < full) i4_copy<S, GROUP, 4>(into, cw, cd, lane);
+                else i4_copy_last<S, GROUP, 4>(into, cw, cd, a.steps - cs * 4, a.groups - cs * (256 / GROUP), lane);
+                cw += 4 * I4_TILE;
+                cd += 256 / GROUP * SB;
+                into = into + SLOT == ring + I4_RING * SLOT ? ring : into + SLOT;
                 left--;
                 if (++cs == whole && left > 0) {
                     cs = 0;
@@ -328,7 +331,7 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
         };
 #pragma unroll
         for (int i = 0; i < I4_RING - 1; i++) copy();
-        int slot = 0;
+        const uint8_t* slot = slots;
         for (int f = f0; f < f1;) {
             const int sa = s, sb = min(whole, s + f1 - f);
             float acc[NT][4];
@@ -350,8 +353,8 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
                     asm volatile("cp.async.wait_group %0;" ::"n"(I4_RING - 2) : "memory");
                     __syncwarp();
                     copy();
-                    step.add(sums, slots + slot * SLOT, lane);
-                    slot = slot + 1 == I4_RING ? 0 : slot + 1;
+                    step.add(sums, slot, lane);
+                    slot = slot + SLOT == slots + I4_RING * SLOT ? slots : slot + SLOT;
                 }
             };
             auto& one = reinterpret_cast<float(&)[1][4]>(acc);
@@ -408,127 +411,117 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
 }
 
 // ------------------------------------------------------------------------------------------------------------- more rows
-// Four teams of four warps; a team has a part of the channels, 128 at a time, and its own ring, so that the teams' copies, products and sums overlap.  A warp has two of the unit's eight tiles; the rows of a are the
+// Four teams of eight warps; a team has a part of the channels, 128 at a time, and its own ring, so that the teams' copies, products and sums overlap.  A warp has one of the unit's eight tiles; the rows of a are the
 // team's.
-enum { I4_TEAMS = 4, I4_TEAM_TILES = 8, I4_MANY_NT = 8 };
-template <typename S, int GROUP> __host__ __device__ constexpr int i4_many_slot() { return I4_TEAM_TILES * i4_slot<S, GROUP, 2>() + I4_MANY_NT * 8 * 128; }
-template <typename S, int GROUP> __host__ __device__ constexpr int i4_many_ring() {      // steps of a team's ring: three where they fit a block's 227 KiB with the longest lists
-    return 3 * I4_TEAMS * i4_many_slot<S, GROUP>() + (int)i4_list_bytes(1024, I4_PAIRS) + 1024 <= 227 * 1024 ? 3 : 2;
-}
-template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * 128, 1) mat_mat_i4_many_kernel(const MatI4Args a) {
+enum { I4_TEAMS = 4, I4_TEAM_WARPS = 8, I4_MANY_ROWS = 64, I4_MANY_RING = 4 };
+template <typename S, int GROUP> __host__ __device__ constexpr int i4_many_slot(int rows) { return I4_TEAM_WARPS * i4_slot<S, GROUP, 2>() + rows * 128; }
+
+template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * I4_TEAM_WARPS * 32, 1) mat_mat_i4_many_kernel(const MatI4Args a) {
     before();
-    constexpr int T = I4_TEAM_TILES, NT = I4_MANY_NT, RING = i4_many_ring<S, GROUP>(), WSLOT = i4_slot<S, GROUP, 2>(), SLOT = i4_many_slot<S, GROUP>(), GS = 128 / GROUP, SB = 16 * (int)sizeof(S), GC = GROUP / 32;
-    static_assert(RING * SLOT >= T * NT * 512, "a team's sums take its ring's place");
+    constexpr int T = I4_TEAM_WARPS, WSLOT = i4_slot<S, GROUP, 2>(), GS = 128 / GROUP, SB = 16 * (int)sizeof(S), GC = GROUP / 32;
     extern __shared__ __align__(16) uint8_t i4_smem[];
+    const int RING = a.ring, SLOT = i4_many_slot<S, GROUP>(a.most), most_nt = a.most / 8;
     const I4List l = i4_list(i4_smem + I4_TEAMS * RING * SLOT, a);
-    const int tid = threadIdx.x, lane = tid & 31, team = tid >> 7, member = (tid >> 5) & 3, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp / T, member = warp % T, g = lane >> 2, t = lane & 3;
     uint8_t* slots = i4_smem + team * RING * SLOT;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(slots);
     const int blocks = (a.tiles + T - 1) / T, whole = (a.steps + 1) / 2;
-    int chunks = (a.rows + 8 * NT - 1) / (8 * NT);
+    int chunks = (a.rows + I4_MANY_ROWS - 1) / I4_MANY_ROWS;
     if (a.experts) {
-        i4_lists(a, l, 8 * NT);
+        i4_lists(a, l, I4_MANY_ROWS);
         chunks = l.chunk[a.n_experts];
         i4_zeros(a, l);
     }
     const int rank = blockIdx.x % a.split, parts = I4_TEAMS * a.split, part = rank * I4_TEAMS + team, s0 = (int)((int64_t)whole * part / parts), s1 = (int)((int64_t)whole * (part + 1) / parts);
-    auto together = [&] { asm volatile("bar.sync %0, 128;" ::"r"(team + 1) : "memory"); };
+    auto together = [&] { asm volatile("bar.sync %0, 256;" ::"r"(team + 1) : "memory"); };
     for (int64_t u = blockIdx.x / a.split; u < (int64_t)chunks * blocks; u += gridDim.x / a.split) {
         const int c = (int)(u / blocks), tile0 = (int)(u - (int64_t)c * blocks) * T;
-        const I4Chunk x = i4_chunk<8 * NT>(a, l, c);
+        const I4Chunk x = i4_chunk<I4_MANY_ROWS>(a, l, c);
         const int nt = (x.many + 7) / 8;
-        // this warp's tiles (where there are none others': nothing reads their sums), and the rows of a that this thread copies 16 bytes of
-        const uint8_t *w[2], *d[2];
+        // this warp's tile (where there is none another: nothing reads its sums), and the rows of a that this thread copies 16 bytes of: at the next step to be copied
+        const int64_t mine_at = (int64_t)x.e * a.tiles + min(tile0 + member, a.tiles - 1);
+        const uint8_t *w = a.w + (mine_at * a.steps + 2 * s0) * I4_TILE + lane * 16, *d = reinterpret_cast<const uint8_t*>(a.ws) + (mine_at * a.groups + s0 * GS) * SB + lane * 8;
+        const int unit = tid & 7, row0 = (tid & 255) >> 3, full = a.k / 128;
+        const int8_t* from[2];
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            const int64_t at = (int64_t)x.e * a.tiles + min(tile0 + member * 2 + r, a.tiles - 1);
-            w[r] = a.w + at * a.steps * I4_TILE;
-            d[r] = reinterpret_cast<const uint8_t*>(a.ws) + at * a.groups * SB;
-        }
-        const int8_t* from[NT / 2];
-#pragma unroll
-        for (int i = 0; i < NT / 2; i++) {
-            const int q = i * 16 + (tid & 127) / 8;
-            from[i] = a.a + (int64_t)((a.first + i4_pair(a, l, x.lo + (q < x.many ? q : 0))) / a.div) * a.lda + (tid & 7) * 16;
-        }
+        for (int i = 0; i < 2; i++)
+            from[i] = a.a + (int64_t)((a.first + i4_pair(a, l, x.lo + (i * 32 + row0 < x.many ? i * 32 + row0 : 0))) / a.div) * a.lda + s0 * 128 + unit * 16;
         // rows of 128 bytes; 16 bytes u of row i lie at u ^ (2 (i % 4)), so that the eight rows of a block of columns are read without bank conflicts
-        const uint32_t to = ring + T * WSLOT + (tid & 127) / 8 * 128 + (((tid & 7) ^ ((tid >> 3 & 3) << 1)) << 4);
-        auto copy = [&](int s, int into) {
-            if (s < s1) {
-                const bool there = s * 128 + (tid & 7) * 16 < a.k;
-#pragma unroll
-                for (int i = 0; i < NT / 2; i++)
-                    if (i * 16 < nt * 8) copy_where<16>(to + into * SLOT + i * 2048, there ? from[i] + s * 128 : a.a, there);
-#pragma unroll
-                for (int r = 0; r < 2; r++) i4_copy<S, GROUP, 2>(a, ring + into * SLOT + (member * 2 + r) * WSLOT, w[r], d[r], s, lane);
+        const uint32_t row_to = T * WSLOT + row0 * 128 + ((unit ^ ((row0 & 3) << 1)) << 4), wrap = ring + RING * SLOT;
+        const bool low = row0 < nt * 8, high = 32 + row0 < nt * 8;
+        int cs = s0;
+        uint32_t into = ring;
+        auto copy = [&]() {
+            if (cs < s1) {
+                if (cs < full) {
+                    if (low) copy_all<16>(into + row_to, from[0]);
+                    if (high) copy_all<16>(into + row_to + 4096, from[1]);
+                    i4_copy<S, GROUP, 2>(into + member * WSLOT, w, d, lane);
+                } else {
+                    const bool there = cs * 128 + unit * 16 < a.k;
+                    if (low) copy_where<16>(into + row_to, there ? from[0] : a.a, there);
+                    if (high) copy_where<16>(into + row_to + 4096, there ? from[1] : a.a, there);
+                    i4_copy_last<S, GROUP, 2>(into + member * WSLOT, w, d, a.steps - cs * 2, a.groups - cs * GS, lane);
+                }
+                w += 2 * I4_TILE;
+                d += GS * SB;
+                from[0] += 128;
+                from[1] += 128;
+                cs++;
+                into = into + SLOT == wrap ? ring : into + SLOT;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-#pragma unroll
-        for (int i = 0; i < RING - 1; i++) copy(s0 + i, i);
+        for (int i = 0; i < RING - 1; i++) copy();
         auto products = [&](auto blocks_of_columns) {
-            constexpr int N = decltype(blocks_of_columns)::value, AT_ONCE = N * GC > 12 ? 1 : 2;      // (both tiles at once, or one after the other where registers do not hold both)
-            float acc[2][N][4];
+            constexpr int N = decltype(blocks_of_columns)::value;
+            float acc[N][4];
 #pragma unroll
-            for (int r = 0; r < 2; r++)
-#pragma unroll
-                for (int j = 0; j < N; j++) acc[r][j][0] = acc[r][j][1] = acc[r][j][2] = acc[r][j][3] = 0;
-            int slot = 0, into = RING - 1;
+            for (int j = 0; j < N; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0;
+            const uint8_t* in = slots;
             for (int s = s0; s < s1; s++) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
+                if (RING == 4) asm volatile("cp.async.wait_group 2;" ::: "memory");
+                else if (RING == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
+                else asm volatile("cp.async.wait_group 0;" ::: "memory");
                 together();      // (all copies of this step are there, and all warps are done with the step before)
-                copy(s + RING - 1, into);
-                const uint8_t *in = slots + slot * SLOT, *mine = in + member * 2 * WSLOT, *rows = in + T * WSLOT + g * 128;
-                into = into + 1 == RING ? 0 : into + 1;
-                slot = slot + 1 == RING ? 0 : slot + 1;
+                copy();
+                const uint8_t *mine = in + member * WSLOT + lane * 16, *rows = in + T * WSLOT + g * 128, *scales = in + member * WSLOT + 2 * I4_TILE + g * 2 * sizeof(S);
+                in = in + SLOT == slots + RING * SLOT ? slots : in + SLOT;
+                uint4 tile;
 #pragma unroll
-                for (int q = 0; q < GS; q++)
+                for (int q = 0; q < GS; q++) {
+                    uint32_t lo[2 * GC], hi[2 * GC];
 #pragma unroll
-                    for (int r0 = 0; r0 < 2; r0 += AT_ONCE) {
-                        uint32_t lo[AT_ONCE][2 * GC], hi[AT_ONCE][2 * GC];
-                        float2 e[AT_ONCE];
-#pragma unroll
-                        for (int r = 0; r < AT_ONCE; r++) {
-                            const uint8_t* tile = mine + (r0 + r) * WSLOT;
-#pragma unroll
-                            for (int i = 0; i < GC; i++) {
-                                const int h = q * GC + i;
-                                const uint2 v = *reinterpret_cast<const uint2*>(tile + (h / 2) * I4_TILE + lane * 16 + (h % 2) * 8);
-                                lo[r][2 * i] = (v.x << 4) & 0xf0f0f0f0u, lo[r][2 * i + 1] = (v.y << 4) & 0xf0f0f0f0u;
-                                hi[r][2 * i] = v.x & 0xf0f0f0f0u, hi[r][2 * i + 1] = v.y & 0xf0f0f0f0u;
-                            }
-                            e[r] = i4_scales<S>(tile + 2 * I4_TILE + q * SB + g * 2 * sizeof(S));
-                        }
-#pragma unroll
-                        for (int j = 0; j < N; j++) {
-                            uint2 b[GC];
-#pragma unroll
-                            for (int i = 0; i < GC; i++) b[i] = *reinterpret_cast<const uint2*>(rows + j * 1024 + ((((q * GC + i) * 2 + (t >> 1)) ^ ((g & 3) << 1)) << 4) + (t & 1) * 8);
-#pragma unroll
-                            for (int r = 0; r < AT_ONCE; r++) {
-                                int sum[4];
-#pragma unroll
-                                for (int i = 0; i < GC; i++) {
-                                    if (i == 0) mma_s8_first(sum, lo[r][0], lo[r][1], hi[r][0], hi[r][1], b[0].x, b[0].y);
-                                    else mma_s8(sum, lo[r][2 * i], lo[r][2 * i + 1], hi[r][2 * i], hi[r][2 * i + 1], b[i].x, b[i].y);
-                                }
-                                float(&y)[4] = acc[r0 + r][j];
-                                y[0] = fmaf(e[r].x, i4_sum(sum[0]), y[0]);
-                                y[1] = fmaf(e[r].x, i4_sum(sum[1]), y[1]);
-                                y[2] = fmaf(e[r].y, i4_sum(sum[2]), y[2]);
-                                y[3] = fmaf(e[r].y, i4_sum(sum[3]), y[3]);
-                            }
-                        }
+                    for (int i = 0; i < GC; i++) {
+                        const int h = q * GC + i;
+                        if (h % 2 == 0) tile = *reinterpret_cast<const uint4*>(mine + (h / 2) * I4_TILE);
+                        const uint2 v = h % 2 ? make_uint2(tile.z, tile.w) : make_uint2(tile.x, tile.y);
+                        lo[2 * i] = (v.x << 4) & 0xf0f0f0f0u, lo[2 * i + 1] = (v.y << 4) & 0xf0f0f0f0u;
+                        hi[2 * i] = v.x & 0xf0f0f0f0u, hi[2 * i + 1] = v.y & 0xf0f0f0f0u;
                     }
+                    const float2 e = i4_scales<S>(scales + q * SB);
+#pragma unroll
+                    for (int j = 0; j < N; j++) {
+                        int sum[4];
+#pragma unroll
+                        for (int i = 0; i < GC; i++) {
+                            const uint2 b = *reinterpret_cast<const uint2*>(rows + j * 1024 + ((((q * GC + i) * 2 + (t >> 1)) ^ ((g & 3) << 1)) << 4) + (t & 1) * 8);
+                            if (i == 0) mma_s8_first(sum, lo[0], lo[1], hi[0], hi[1], b.x, b.y);
+                            else mma_s8(sum, lo[2 * i], lo[2 * i + 1], hi[2 * i], hi[2 * i + 1], b.x, b.y);
+                        }
+                        acc[j][0] = fmaf(e.x, i4_sum(sum[0]), acc[j][0]);
+                        acc[j][1] = fmaf(e.x, i4_sum(sum[1]), acc[j][1]);
+                        acc[j][2] = fmaf(e.y, i4_sum(sum[2]), acc[j][2]);
+                        acc[j][3] = fmaf(e.y, i4_sum(sum[3]), acc[j][3]);
+                    }
+                }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             together();
             // sums to the team's ring's place
 #pragma unroll
-            for (int r = 0; r < 2; r++)
-#pragma unroll
-                for (int j = 0; j < N; j++)
-                    reinterpret_cast<float4*>(slots)[((member * 2 + r) * NT + j) * 32 + lane] = make_float4(acc[r][j][0], acc[r][j][1], acc[r][j][2], acc[r][j][3]);
+            for (int j = 0; j < N; j++)
+                if (j < nt) reinterpret_cast<float4*>(slots)[(member * most_nt + j) * 32 + lane] = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
         };
         if (nt <= 2) products(std::integral_constant<int, 2>());
         else if (nt <= 3) products(std::integral_constant<int, 3>());
@@ -540,7 +533,7 @@ template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * 12
         if (a.split > 1) cluster_sync();
         else __syncthreads();
         // a warp for every tile and block of columns; the cluster's blocks take turns
-        for (int o = (tid >> 5) * a.split + rank; o < T * nt; o += I4_TEAMS * 4 * a.split) {
+        for (int o = warp * a.split + rank; o < T * nt; o += I4_TEAMS * T * a.split) {
             const int i = o % T, j = o / T, col = 8 * j + 2 * t, n = (tile0 + i) * 16 + g;
             int p[2];
             float scale[2];
@@ -549,7 +542,7 @@ template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * 12
                 p[q] = col + q < x.many ? i4_pair(a, l, x.lo + col + q) : -1;
                 scale[q] = p[q] >= 0 ? i4_row_scale(a, p[q]) : 0.0f;
             }
-            const uint32_t at = (uint32_t)__cvta_generic_to_shared(i4_smem) + ((i * NT + j) * 32 + lane) * 16;
+            const uint32_t at = (uint32_t)__cvta_generic_to_shared(i4_smem) + ((i * most_nt + j) * 32 + lane) * 16;
             float4 y = make_float4(0, 0, 0, 0);
             for (int b = 0; b < a.split; b++)
 #pragma unroll
@@ -572,8 +565,8 @@ template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * 12
 
 // ----------------------------------------------------------------------------------------------------------------- host
 // (a launch's list of pairs is bounded: more pairs are more launches)
-template <int CHUNK, int R, int WARPS, int PER_SM, typename F> cudaError_t mat_mat_i4_launch(MatI4Args a, F kernel, SmemAllowed& allowed, size_t base, int sms, cudaStream_t st) {
-    cudaError_t e = allowed(reinterpret_cast<const void*>(kernel), base + i4_list_bytes(1024, I4_PAIRS));
+template <int CHUNK, int R, int WARPS, int PER_SM, typename F> cudaError_t mat_mat_i4_launch(MatI4Args a, F kernel, SmemAllowed& allowed, size_t base, size_t most, int sms, cudaStream_t st) {
+    cudaError_t e = allowed(reinterpret_cast<const void*>(kernel), most);
     const int rows = a.rows, per = a.experts ? I4_PAIRS / a.div * a.div : rows;
     const int64_t blocks = (a.tiles + R - 1) / R;
     for (int first = 0; e == cudaSuccess && first < rows; first += per) {
@@ -589,11 +582,17 @@ template <int CHUNK, int R, int WARPS, int PER_SM, typename F> cudaError_t mat_m
 }
 template <typename S, int GROUP, int NT> cudaError_t mat_mat_i4_few(const MatI4Args& a, int sms, cudaStream_t st) {
     static SmemAllowed allowed;
-    return mat_mat_i4_launch<8 * NT, 1, i4_few_warps<NT>(), 2>(a, mat_mat_i4_few_kernel<S, GROUP, NT>, allowed, i4_few_warps<NT>() * (I4_RING * i4_slot<S, GROUP, 4>() + 2 * NT * 512), sms, st);
+    constexpr size_t base = i4_few_warps<NT>() * (I4_RING * i4_slot<S, GROUP, 4>() + 2 * NT * 512);
+    return mat_mat_i4_launch<8 * NT, 1, i4_few_warps<NT>(), 2>(a, mat_mat_i4_few_kernel<S, GROUP, NT>, allowed, base, base + i4_list_bytes(1024, I4_PAIRS), sms, st);
 }
-template <typename S, int GROUP> cudaError_t mat_mat_i4_many(const MatI4Args& a, int sms, cudaStream_t st) {
+template <typename S, int GROUP> cudaError_t mat_mat_i4_many(MatI4Args a, int sms, cudaStream_t st) {
     static SmemAllowed allowed;
-    return mat_mat_i4_launch<I4_MANY_NT * 8, I4_TEAM_TILES, I4_TEAMS * 4, 1>(a, mat_mat_i4_many_kernel<S, GROUP>, allowed, I4_TEAMS * i4_many_ring<S, GROUP>() * i4_many_slot<S, GROUP>(), sms, st);
+    constexpr int most = 227 * 1024;
+    const int lists = a.experts ? (int)i4_list_bytes(a.n_experts, std::min<int>(a.rows, I4_PAIRS)) : 0;
+    a.most = std::min((a.rows + 7) / 8 * 8, (int)I4_MANY_ROWS);
+    const int ring = I4_TEAMS * i4_many_slot<S, GROUP>(a.most);
+    a.ring = std::min((int)I4_MANY_RING, (most - lists) / ring);      // (two at least: 144 KiB and the longest lists' 16)
+    return mat_mat_i4_launch<I4_MANY_ROWS, I4_TEAM_WARPS, I4_TEAMS * I4_TEAM_WARPS, 1>(a, mat_mat_i4_many_kernel<S, GROUP>, allowed, a.ring * ring, most, sms, st);
 }
 template <typename S, int GROUP> cudaError_t mat_mat_i4(const MatI4Args& a, cudaStream_t st) {
     int sms = 0;

@@ -9,6 +9,13 @@
 
 using namespace dev;
 
+int dev_experts_watchdog(int* code) {
+    const int zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(code, dev_watchdog, sizeof(int));
+    if (e == cudaSuccess && *code) e = cudaMemcpyToSymbol(dev_watchdog, &zero, sizeof(int));
+    return (int)e;
+}
+
 extern "C" int b200_dev_route_experts(const b200_route* a) {
     const char* op = "route_experts";
     return entry(op, [&]() -> int {
@@ -44,7 +51,7 @@ extern "C" int b200_dev_mat_mat_i4(const b200_i4_product* a) {
         if (a->tokens == 0) return B200_OK;
         if (!a->a || !a->a_scales || !a->w || !a->w_scales || !a->out) return bad(op, "null pointer");
         if (off16(a->a) || off16(a->w) || a->lda % 16) return bad(op, "a and w must start on 16 bytes, with rows of a a multiple of 16 bytes apart");
-        if (reinterpret_cast<uintptr_t>(a->w_scales) & 7) return bad(op, "the scales must start on 8 bytes");
+        if (off16(a->w_scales)) return bad(op, "the scales must start on 16 bytes");
         MatI4Args m{};
         m.a = a->a;
         m.a_scales = a->a_scales;

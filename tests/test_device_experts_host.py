@@ -107,7 +107,7 @@ def test_product_refusals(b200, D):
             (dict(group=128), b200.ShapeMismatch, "multiple"), (dict(k=0), b200.ShapeMismatch, "shape"), (dict(n=0), b200.ShapeMismatch, "shape"), (dict(tokens=-1), b200.ShapeMismatch, "shape"),
             (dict(n=(1 << 31) - 1, ldo=1 << 31), b200.ShapeMismatch, "shape"), (dict(tokens=(1 << 31) - 1), b200.ShapeMismatch, "rows"), (dict(lda=48), b200.ShapeMismatch, "overlap"),
             (dict(ldo=7), b200.ShapeMismatch, "overlap"), (dict(a=AT + 8), b200.InvalidArgument, "16 bytes"), (dict(w=AT + 1), b200.InvalidArgument, "16 bytes"), (dict(lda=72), b200.InvalidArgument, "16 bytes"),
-            (dict(w_scales=AT + 4), b200.InvalidArgument, "8 bytes"), (dict(out=None), b200.InvalidArgument, "null"), (dict(w=None), b200.InvalidArgument, "null"), (dict(a_scales=None), b200.InvalidArgument, "null"),
+            (dict(w_scales=AT + 8), b200.InvalidArgument, "16 bytes"), (dict(out=None), b200.InvalidArgument, "null"), (dict(w=None), b200.InvalidArgument, "null"), (dict(a_scales=None), b200.InvalidArgument, "null"),
             (dict(top=2), b200.InvalidArgument, "without experts"), (dict(rows_per_pair=1), b200.InvalidArgument, "without experts"), ({**experts, "top": 0}, b200.ShapeMismatch, "places"),
             ({**experts, "top": 33}, b200.ShapeMismatch, "places"), ({**experts, "n_experts": 0}, b200.ShapeMismatch, "places"), ({**experts, "n_experts": 1025}, b200.ShapeMismatch, "places"),
             ({**experts, "tokens": 1 << 30}, b200.ShapeMismatch, "rows")]:
