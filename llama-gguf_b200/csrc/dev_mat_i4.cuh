@@ -11,7 +11,7 @@
 // for another's weights.  With experts every block lists the pairs (token, expert) by expert first, all in the same order; up to that many pairs of an expert are a unit for each tile.
 //   few rows (up to 16): the weights' bytes.  Two blocks per SM have consecutive units of one tile each; its warps share their steps of 256 channels evenly, whichever unit they are of, and leave the sums of a unit that two or
 //   more warps have a part of in shared memory for the end.  Rows of a come from L1 and L2.
-//   more rows (up to 64 at a time): rows of a cost as much as weights.  A block has eight tiles; its teams of eight warps have a part of the channels each, whose rows of a serve all eight.  With few units the
+//   more rows (up to 64 at a time): rows of a cost as much as weights.  A block has eight tiles; its teams of four warps have a part of the channels each, whose rows of a serve all eight.  With few units the
 //   blocks of a cluster share the channels of one.
 #pragma once
 #include <algorithm>
@@ -411,21 +411,23 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
 }
 
 // ------------------------------------------------------------------------------------------------------------- more rows
-// Four teams of eight warps; a team has a part of the channels, 128 at a time, and its own ring, so that the teams' copies, products and sums overlap.  A warp has one of the unit's eight tiles; the rows of a are the
+// Four teams of four warps; a team has a part of the channels, 128 at a time, and its own ring, so that the teams' copies, products and sums overlap.  A warp has two of the unit's eight tiles; the rows of a are the
 // team's.
-enum { I4_TEAMS = 4, I4_TEAM_WARPS = 8, I4_MANY_ROWS = 64, I4_MANY_RING = 4 };
-template <typename S, int GROUP> __host__ __device__ constexpr int i4_many_slot(int rows) { return I4_TEAM_WARPS * i4_slot<S, GROUP, 2>() + rows * 128; }
+enum { I4_TEAMS = 4, I4_TEAM_WARPS = 4, I4_TEAM_TILES = 8, I4_MANY_ROWS = 64, I4_MANY_RING = 4 };
+template <typename S, int GROUP> __host__ __device__ constexpr int i4_many_slot(int rows) { return I4_TEAM_TILES * i4_slot<S, GROUP, 2>() + rows * 128; }
 
 template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * I4_TEAM_WARPS * 32, 1) mat_mat_i4_many_kernel(const MatI4Args a) {
     before();
-    constexpr int T = I4_TEAM_WARPS, WSLOT = i4_slot<S, GROUP, 2>(), GS = 128 / GROUP, SB = 16 * (int)sizeof(S), GC = GROUP / 32;
+    constexpr int T = I4_TEAM_TILES, WSLOT = i4_slot<S, GROUP, 2>(), GS = 128 / GROUP, SB = 16 * (int)sizeof(S), GC = GROUP / 32;
     extern __shared__ __align__(16) uint8_t i4_smem[];
+    __shared__ float s_scale[I4_MANY_ROWS];
+    __shared__ int s_pair[I4_MANY_ROWS];      // the unit's rows of out, and their scales
     const int RING = a.ring, SLOT = i4_many_slot<S, GROUP>(a.most), most_nt = a.most / 8;
     const I4List l = i4_list(i4_smem + I4_TEAMS * RING * SLOT, a);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp / T, member = warp % T, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp / I4_TEAM_WARPS, member = warp % I4_TEAM_WARPS, g = lane >> 2, t = lane & 3;
     uint8_t* slots = i4_smem + team * RING * SLOT;
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(slots);
-    const int blocks = (a.tiles + T - 1) / T, whole = (a.steps + 1) / 2;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(slots), wrap = ring + RING * SLOT;
+    const int blocks = (a.tiles + T - 1) / T, whole = (a.steps + 1) / 2, full = a.k / 128;
     int chunks = (a.rows + I4_MANY_ROWS - 1) / I4_MANY_ROWS;
     if (a.experts) {
         i4_lists(a, l, I4_MANY_ROWS);
@@ -433,95 +435,114 @@ template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * I4
         i4_zeros(a, l);
     }
     const int rank = blockIdx.x % a.split, parts = I4_TEAMS * a.split, part = rank * I4_TEAMS + team, s0 = (int)((int64_t)whole * part / parts), s1 = (int)((int64_t)whole * (part + 1) / parts);
-    auto together = [&] { asm volatile("bar.sync %0, 256;" ::"r"(team + 1) : "memory"); };
+    auto together = [&] { asm volatile("bar.sync %0, 128;" ::"r"(team + 1) : "memory"); };
     for (int64_t u = blockIdx.x / a.split; u < (int64_t)chunks * blocks; u += gridDim.x / a.split) {
         const int c = (int)(u / blocks), tile0 = (int)(u - (int64_t)c * blocks) * T;
         const I4Chunk x = i4_chunk<I4_MANY_ROWS>(a, l, c);
         const int nt = (x.many + 7) / 8;
-        // this warp's tile (where there is none another: nothing reads its sums), and the rows of a that this thread copies 16 bytes of: at the next step to be copied
-        const int64_t mine_at = (int64_t)x.e * a.tiles + min(tile0 + member, a.tiles - 1);
-        const uint8_t *w = a.w + (mine_at * a.steps + 2 * s0) * I4_TILE + lane * 16, *d = reinterpret_cast<const uint8_t*>(a.ws) + (mine_at * a.groups + s0 * GS) * SB + lane * 8;
-        const int unit = tid & 7, row0 = (tid & 255) >> 3, full = a.k / 128;
-        const int8_t* from[2];
+        // this warp's tiles (where there are none others': nothing reads their sums), and the rows of a that this thread copies 16 bytes of: at the next step to be copied
+        const int first = min(tile0 + member * 2, a.tiles - 1);
+        const int64_t at = (int64_t)x.e * a.tiles + first, tile_w = first + 1 < a.tiles ? (int64_t)a.steps * I4_TILE : 0, tile_d = first + 1 < a.tiles ? (int64_t)a.groups * SB : 0;
+        const uint8_t *w = a.w + (at * a.steps + 2 * s0) * I4_TILE + lane * 16, *d = reinterpret_cast<const uint8_t*>(a.ws) + (at * a.groups + s0 * GS) * SB + lane * 8;
+        const int unit = tid & 7, row0 = (tid & 127) >> 3;
+        const int8_t* from[4];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-            from[i] = a.a + (int64_t)((a.first + i4_pair(a, l, x.lo + (i * 32 + row0 < x.many ? i * 32 + row0 : 0))) / a.div) * a.lda + s0 * 128 + unit * 16;
+        for (int i = 0; i < 4; i++)
+            from[i] = a.a + (int64_t)((a.first + i4_pair(a, l, x.lo + (i * 16 + row0 < x.many ? i * 16 + row0 : 0))) / a.div) * a.lda + s0 * 128 + unit * 16;
         // rows of 128 bytes; 16 bytes u of row i lie at u ^ (2 (i % 4)), so that the eight rows of a block of columns are read without bank conflicts
-        const uint32_t row_to = T * WSLOT + row0 * 128 + ((unit ^ ((row0 & 3) << 1)) << 4), wrap = ring + RING * SLOT;
-        const bool low = row0 < nt * 8, high = 32 + row0 < nt * 8;
+        const uint32_t row_to = T * WSLOT + row0 * 128 + ((unit ^ ((row0 & 3) << 1)) << 4), tile_to = member * 2 * WSLOT;
         int cs = s0;
         uint32_t into = ring;
         auto copy = [&]() {
             if (cs < s1) {
-                if (cs < full) {
-                    if (low) copy_all<16>(into + row_to, from[0]);
-                    if (high) copy_all<16>(into + row_to + 4096, from[1]);
-                    i4_copy<S, GROUP, 2>(into + member * WSLOT, w, d, lane);
-                } else {
-                    const bool there = cs * 128 + unit * 16 < a.k;
-                    if (low) copy_where<16>(into + row_to, there ? from[0] : a.a, there);
-                    if (high) copy_where<16>(into + row_to + 4096, there ? from[1] : a.a, there);
-                    i4_copy_last<S, GROUP, 2>(into + member * WSLOT, w, d, a.steps - cs * 2, a.groups - cs * GS, lane);
+                const bool there = cs < full || cs * 128 + unit * 16 < a.k;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (i * 16 + row0 < nt * 8) copy_where<16>(into + row_to + i * 2048, there ? from[i] : a.a, there);
+                    from[i] += 128;
+                }
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    if (cs < full) i4_copy<S, GROUP, 2>(into + tile_to + r * WSLOT, w + r * tile_w, d + r * tile_d, lane);
+                    else i4_copy_last<S, GROUP, 2>(into + tile_to + r * WSLOT, w + r * tile_w, d + r * tile_d, a.steps - cs * 2, a.groups - cs * GS, lane);
                 }
                 w += 2 * I4_TILE;
                 d += GS * SB;
-                from[0] += 128;
-                from[1] += 128;
                 cs++;
                 into = into + SLOT == wrap ? ring : into + SLOT;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         for (int i = 0; i < RING - 1; i++) copy();
+        if (tid < x.many) {
+            const int p = i4_pair(a, l, x.lo + tid);
+            s_pair[tid] = p;
+            s_scale[tid] = i4_row_scale(a, p);
+        }
         auto products = [&](auto blocks_of_columns) {
-            constexpr int N = decltype(blocks_of_columns)::value;
-            float acc[N][4];
+            constexpr int N = decltype(blocks_of_columns)::value, AT_ONCE = N * GC > 12 ? 1 : 2;      // (both tiles at once, or one after the other where registers do not hold both)
+            float acc[2][N][4];
 #pragma unroll
-            for (int j = 0; j < N; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0;
-            const uint8_t* in = slots;
+            for (int r = 0; r < 2; r++)
+#pragma unroll
+                for (int j = 0; j < N; j++) acc[r][j][0] = acc[r][j][1] = acc[r][j][2] = acc[r][j][3] = 0;
+            uint32_t slot = 0;
             for (int s = s0; s < s1; s++) {
                 if (RING == 4) asm volatile("cp.async.wait_group 2;" ::: "memory");
                 else if (RING == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
                 else asm volatile("cp.async.wait_group 0;" ::: "memory");
                 together();      // (all copies of this step are there, and all warps are done with the step before)
                 copy();
-                const uint8_t *mine = in + member * WSLOT + lane * 16, *rows = in + T * WSLOT + g * 128, *scales = in + member * WSLOT + 2 * I4_TILE + g * 2 * sizeof(S);
-                in = in + SLOT == slots + RING * SLOT ? slots : in + SLOT;
-                uint4 tile;
+                const uint8_t *in = slots + slot, *mine = in + tile_to, *rows = in + T * WSLOT + g * 128;
+                slot = slot + SLOT == RING * SLOT ? 0 : slot + SLOT;
 #pragma unroll
-                for (int q = 0; q < GS; q++) {
-                    uint32_t lo[2 * GC], hi[2 * GC];
+                for (int q = 0; q < GS; q++)
 #pragma unroll
-                    for (int i = 0; i < GC; i++) {
-                        const int h = q * GC + i;
-                        if (h % 2 == 0) tile = *reinterpret_cast<const uint4*>(mine + (h / 2) * I4_TILE);
-                        const uint2 v = h % 2 ? make_uint2(tile.z, tile.w) : make_uint2(tile.x, tile.y);
-                        lo[2 * i] = (v.x << 4) & 0xf0f0f0f0u, lo[2 * i + 1] = (v.y << 4) & 0xf0f0f0f0u;
-                        hi[2 * i] = v.x & 0xf0f0f0f0u, hi[2 * i + 1] = v.y & 0xf0f0f0f0u;
-                    }
-                    const float2 e = i4_scales<S>(scales + q * SB);
+                    for (int r0 = 0; r0 < 2; r0 += AT_ONCE) {
+                        uint32_t lo[AT_ONCE][2 * GC], hi[AT_ONCE][2 * GC];
+                        float2 e[AT_ONCE];
 #pragma unroll
-                    for (int j = 0; j < N; j++) {
-                        int sum[4];
+                        for (int r = 0; r < AT_ONCE; r++) {
+                            const uint8_t* tile = mine + (r0 + r) * WSLOT;
 #pragma unroll
-                        for (int i = 0; i < GC; i++) {
-                            const uint2 b = *reinterpret_cast<const uint2*>(rows + j * 1024 + ((((q * GC + i) * 2 + (t >> 1)) ^ ((g & 3) << 1)) << 4) + (t & 1) * 8);
-                            if (i == 0) mma_s8_first(sum, lo[0], lo[1], hi[0], hi[1], b.x, b.y);
-                            else mma_s8(sum, lo[2 * i], lo[2 * i + 1], hi[2 * i], hi[2 * i + 1], b.x, b.y);
+                            for (int i = 0; i < GC; i++) {
+                                const int h = q * GC + i;
+                                const uint2 v = *reinterpret_cast<const uint2*>(tile + (h / 2) * I4_TILE + lane * 16 + (h % 2) * 8);
+                                lo[r][2 * i] = (v.x << 4) & 0xf0f0f0f0u, lo[r][2 * i + 1] = (v.y << 4) & 0xf0f0f0f0u;
+                                hi[r][2 * i] = v.x & 0xf0f0f0f0u, hi[r][2 * i + 1] = v.y & 0xf0f0f0f0u;
+                            }
+                            e[r] = i4_scales<S>(tile + 2 * I4_TILE + q * SB + g * 2 * sizeof(S));
                         }
-                        acc[j][0] = fmaf(e.x, i4_sum(sum[0]), acc[j][0]);
-                        acc[j][1] = fmaf(e.x, i4_sum(sum[1]), acc[j][1]);
-                        acc[j][2] = fmaf(e.y, i4_sum(sum[2]), acc[j][2]);
-                        acc[j][3] = fmaf(e.y, i4_sum(sum[3]), acc[j][3]);
+#pragma unroll
+                        for (int j = 0; j < N; j++) {
+                            uint2 b[GC];
+#pragma unroll
+                            for (int i = 0; i < GC; i++) b[i] = *reinterpret_cast<const uint2*>(rows + j * 1024 + ((((q * GC + i) * 2 + (t >> 1)) ^ ((g & 3) << 1)) << 4) + (t & 1) * 8);
+#pragma unroll
+                            for (int r = 0; r < AT_ONCE; r++) {
+                                int sum[4];
+#pragma unroll
+                                for (int i = 0; i < GC; i++) {
+                                    if (i == 0) mma_s8_first(sum, lo[r][0], lo[r][1], hi[r][0], hi[r][1], b[0].x, b[0].y);
+                                    else mma_s8(sum, lo[r][2 * i], lo[r][2 * i + 1], hi[r][2 * i], hi[r][2 * i + 1], b[i].x, b[i].y);
+                                }
+                                float(&y)[4] = acc[r0 + r][j];
+                                y[0] = fmaf(e[r].x, i4_sum(sum[0]), y[0]);
+                                y[1] = fmaf(e[r].x, i4_sum(sum[1]), y[1]);
+                                y[2] = fmaf(e[r].y, i4_sum(sum[2]), y[2]);
+                                y[3] = fmaf(e[r].y, i4_sum(sum[3]), y[3]);
+                            }
+                        }
                     }
-                }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             together();
             // sums to the team's ring's place
 #pragma unroll
-            for (int j = 0; j < N; j++)
-                if (j < nt) reinterpret_cast<float4*>(slots)[(member * most_nt + j) * 32 + lane] = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+            for (int r = 0; r < 2; r++)
+#pragma unroll
+                for (int j = 0; j < N; j++)
+                    if (j < nt) reinterpret_cast<float4*>(slots)[((member * 2 + r) * most_nt + j) * 32 + lane] = make_float4(acc[r][j][0], acc[r][j][1], acc[r][j][2], acc[r][j][3]);
         };
         if (nt <= 2) products(std::integral_constant<int, 2>());
         else if (nt <= 3) products(std::integral_constant<int, 3>());
@@ -533,15 +554,8 @@ template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * I4
         if (a.split > 1) cluster_sync();
         else __syncthreads();
         // a warp for every tile and block of columns; the cluster's blocks take turns
-        for (int o = warp * a.split + rank; o < T * nt; o += I4_TEAMS * T * a.split) {
+        for (int o = warp * a.split + rank; o < T * nt; o += I4_TEAMS * I4_TEAM_WARPS * a.split) {
             const int i = o % T, j = o / T, col = 8 * j + 2 * t, n = (tile0 + i) * 16 + g;
-            int p[2];
-            float scale[2];
-#pragma unroll
-            for (int q = 0; q < 2; q++) {
-                p[q] = col + q < x.many ? i4_pair(a, l, x.lo + col + q) : -1;
-                scale[q] = p[q] >= 0 ? i4_row_scale(a, p[q]) : 0.0f;
-            }
             const uint32_t at = (uint32_t)__cvta_generic_to_shared(i4_smem) + ((i * most_nt + j) * 32 + lane) * 16;
             float4 y = make_float4(0, 0, 0, 0);
             for (int b = 0; b < a.split; b++)
@@ -552,9 +566,9 @@ template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * I4
                 }
 #pragma unroll
             for (int q = 0; q < 2; q++)
-                if (p[q] >= 0) {
-                    if (n < a.n) i4_put(a, x.e, p[q], n, q ? y.y : y.x, scale[q]);
-                    if (n + 8 < a.n) i4_put(a, x.e, p[q], n + 8, q ? y.w : y.z, scale[q]);
+                if (col + q < x.many) {
+                    if (n < a.n) i4_put(a, x.e, s_pair[col + q], n, q ? y.y : y.x, s_scale[col + q]);
+                    if (n + 8 < a.n) i4_put(a, x.e, s_pair[col + q], n + 8, q ? y.w : y.z, s_scale[col + q]);
                 }
         }
         __syncwarp();
@@ -587,12 +601,12 @@ template <typename S, int GROUP, int NT> cudaError_t mat_mat_i4_few(const MatI4A
 }
 template <typename S, int GROUP> cudaError_t mat_mat_i4_many(MatI4Args a, int sms, cudaStream_t st) {
     static SmemAllowed allowed;
-    constexpr int most = 227 * 1024;
+    constexpr int most = 226 * 1024;      // (and half a kilobyte of the kernel's own)
     const int lists = a.experts ? (int)i4_list_bytes(a.n_experts, std::min<int>(a.rows, I4_PAIRS)) : 0;
     a.most = std::min((a.rows + 7) / 8 * 8, (int)I4_MANY_ROWS);
     const int ring = I4_TEAMS * i4_many_slot<S, GROUP>(a.most);
     a.ring = std::min((int)I4_MANY_RING, (most - lists) / ring);      // (two at least: 144 KiB and the longest lists' 16)
-    return mat_mat_i4_launch<I4_MANY_ROWS, I4_TEAM_WARPS, I4_TEAMS * I4_TEAM_WARPS, 1>(a, mat_mat_i4_many_kernel<S, GROUP>, allowed, a.ring * ring, most, sms, st);
+    return mat_mat_i4_launch<I4_MANY_ROWS, I4_TEAM_TILES, I4_TEAMS * I4_TEAM_WARPS, 1>(a, mat_mat_i4_many_kernel<S, GROUP>, allowed, a.ring * ring, most, sms, st);
 }
 template <typename S, int GROUP> cudaError_t mat_mat_i4(const MatI4Args& a, cudaStream_t st) {
     int sms = 0;
