@@ -421,7 +421,8 @@ template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * I4
     constexpr int T = I4_TEAM_TILES, WSLOT = i4_slot<S, GROUP, 2>(), GS = 128 / GROUP, SB = 16 * (int)sizeof(S), GC = GROUP / 32;
     extern __shared__ __align__(16) uint8_t i4_smem[];
     __shared__ float s_scale[I4_MANY_ROWS];
-    __shared__ int s_pair[I4_MANY_ROWS];      // the unit's rows of out, and their scales
+    __shared__ int s_pair[I4_MANY_ROWS];      // the unit's rows of out, their scales, where their rows of a begin
+    __shared__ int64_t s_from[I4_MANY_ROWS];
     const int RING = a.ring, SLOT = i4_many_slot<S, GROUP>(a.most), most_nt = a.most / 8;
     const I4List l = i4_list(i4_smem + I4_TEAMS * RING * SLOT, a);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp / I4_TEAM_WARPS, member = warp % I4_TEAM_WARPS, g = lane >> 2, t = lane & 3;
@@ -445,10 +446,14 @@ template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * I4
         const int64_t at = (int64_t)x.e * a.tiles + first, tile_w = first + 1 < a.tiles ? (int64_t)a.steps * I4_TILE : 0, tile_d = first + 1 < a.tiles ? (int64_t)a.groups * SB : 0;
         const uint8_t *w = a.w + (at * a.steps + 2 * s0) * I4_TILE + lane * 16, *d = reinterpret_cast<const uint8_t*>(a.ws) + (at * a.groups + s0 * GS) * SB + lane * 8;
         const int unit = tid & 7, row0 = (tid & 127) >> 3;
-        const int8_t* from[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            from[i] = a.a + (int64_t)((a.first + i4_pair(a, l, x.lo + (i * 16 + row0 < x.many ? i * 16 + row0 : 0))) / a.div) * a.lda + s0 * 128 + unit * 16;
+        const int8_t* from = a.a + s0 * 128 + unit * 16;
+        if (tid < I4_MANY_ROWS) {
+            const int p = i4_pair(a, l, x.lo + (tid < x.many ? tid : 0));
+            s_pair[tid] = p;
+            s_from[tid] = (int64_t)((a.first + p) / a.div) * a.lda;
+            s_scale[tid] = i4_row_scale(a, p);
+        }
+        __syncthreads();
         // rows of 128 bytes; 16 bytes u of row i lie at u ^ (2 (i % 4)), so that the eight rows of a block of columns are read without bank conflicts
         const uint32_t row_to = T * WSLOT + row0 * 128 + ((unit ^ ((row0 & 3) << 1)) << 4), tile_to = member * 2 * WSLOT;
         int cs = s0;
@@ -457,10 +462,9 @@ template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * I4
             if (cs < s1) {
                 const bool there = cs < full || cs * 128 + unit * 16 < a.k;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    if (i * 16 + row0 < nt * 8) copy_where<16>(into + row_to + i * 2048, there ? from[i] : a.a, there);
-                    from[i] += 128;
-                }
+                for (int i = 0; i < 4; i++)
+                    if (i * 16 + row0 < nt * 8) copy_where<16>(into + row_to + i * 2048, there ? from + s_from[i * 16 + row0] : a.a, there);
+                from += 128;
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
                     if (cs < full) i4_copy<S, GROUP, 2>(into + tile_to + r * WSLOT, w + r * tile_w, d + r * tile_d, lane);
@@ -474,11 +478,6 @@ template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * I4
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         for (int i = 0; i < RING - 1; i++) copy();
-        if (tid < x.many) {
-            const int p = i4_pair(a, l, x.lo + tid);
-            s_pair[tid] = p;
-            s_scale[tid] = i4_row_scale(a, p);
-        }
         auto products = [&](auto blocks_of_columns) {
             constexpr int N = decltype(blocks_of_columns)::value, AT_ONCE = N * GC > 12 ? 1 : 2;      // (both tiles at once, or one after the other where registers do not hold both)
             float acc[2][N][4];
@@ -589,7 +588,7 @@ template <int CHUNK, int R, int WARPS, int PER_SM, typename F> cudaError_t mat_m
         const int64_t units = (a.experts ? std::min<int64_t>(a.rows, a.n_experts + a.rows / CHUNK) : (a.rows + CHUNK - 1) / CHUNK) * blocks;
         a.split = 1;
         if (R > 1)
-            while (a.split < 8 && units * a.split * 2 <= sms && a.steps >= 32 * a.split) a.split *= 2;
+            while (a.split < 8 && units * a.split * 2 <= sms && a.steps >= 16 * a.split) a.split *= 2;      // (a step for each team)
         e = launch(kernel, dim3((unsigned)(std::min<int64_t>(units, PER_SM * sms / a.split) * a.split)), WARPS * 32, base + (a.experts ? i4_list_bytes(a.n_experts, a.rows) : 0), a.split, st, a);
     }
     return e;
