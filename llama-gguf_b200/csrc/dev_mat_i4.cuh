@@ -254,10 +254,10 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
         chunks = l.chunk[a.n_experts];
         i4_zeros(a, l);
     }
-    // this block's units, their steps one after the other, and this warp's of those
-    const int64_t units = (int64_t)chunks * a.tiles, u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
-    const int many = (int)(u1 - u0), steps = many * whole;
-    auto begin = [&](int w) { return (int)((int64_t)steps * w / WARPS); };
+    // this block's units (of fewer than 2^31, see mat_mat_i4), their steps one after the other, and this warp's of those
+    const uint32_t units = (uint32_t)chunks * (uint32_t)a.tiles, each = units / gridDim.x, over = units - each * gridDim.x, u0 = each * blockIdx.x + min(over, blockIdx.x);
+    const int many = (int)(each + (blockIdx.x < over)), steps = many * whole, part = steps / WARPS, rest = steps - part * WARPS;
+    auto begin = [&](int w) { return part * w + min(rest, w); };
     // sums over a row's columns, and the results of a unit
     auto row_scales = [&](float2 (&d)[NT], const I4Chunk& x) {
 #pragma unroll
@@ -297,7 +297,7 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
     const int f0 = begin(warp), f1 = begin(warp + 1);
     if (f0 < f1) {
         const int v0 = f0 / whole;
-        int c = (int)((u0 + v0) / a.tiles), tile = (int)(u0 + v0 - (int64_t)c * a.tiles), s = f0 - v0 * whole;
+        int c = (int)((u0 + v0) / (uint32_t)a.tiles), tile = (int)(u0 + v0 - (uint32_t)c * a.tiles), s = f0 - v0 * whole;
         I4Chunk x = i4_chunk<CHUNK>(a, l, c);
         // copies, I4_RING - 1 steps ahead of the products
         int cc = c, ct = tile, ce = x.e, cs = s, left = f1 - f0;
@@ -385,9 +385,8 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
     __syncthreads();
     // units that several warps have a part of, a warp for each; the parts are added in the order of the channels
     for (int v = warp; v < many; v += WARPS) {
-        int w = (int)((int64_t)v * whole * WARPS / steps);      // the warp that has the unit's first step
-        while (begin(w + 1) <= v * whole) w++;
-        while (begin(w) > v * whole) w--;
+        const int f = v * whole;
+        int w = f < rest * (part + 1) ? f / (part + 1) : rest + (f - rest * (part + 1)) / part;      // the warp that has the unit's first step
         if (begin(w + 1) >= (v + 1) * whole) continue;      // one warp's: written
         float4 y[NT];
 #pragma unroll
@@ -402,11 +401,11 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
                 y[j].x += z.x, y[j].y += z.y, y[j].z += z.z, y[j].w += z.w;
             }
         }
-        const int c = (int)((u0 + v) / a.tiles);
+        const int c = (int)((u0 + v) / (uint32_t)a.tiles);
         const I4Chunk x = i4_chunk<CHUNK>(a, l, c);
         float2 d[NT];
         row_scales(d, x);
-        finish(y, d, x, (int)(u0 + v - (int64_t)c * a.tiles));
+        finish(y, d, x, (int)(u0 + v - (uint32_t)c * a.tiles));
     }
 }
 

@@ -47,6 +47,7 @@ extern "C" int b200_dev_mat_mat_i4(const b200_i4_product* a) {
         if (a->experts && (a->top < 1 || a->top > 32 || a->n_experts < 1 || a->n_experts > ROUTE_MOST)) return shape(op, "1 to 32 places of 1 to 1024 experts expected");
         if (!a->experts && a->tokens && (a->top || a->n_experts || a->rows_per_pair)) return bad(op, "top, n_experts or rows_per_pair without experts");
         if (a->tokens > kMostTiled / (a->experts ? a->top : 1)) return shape(op, "too many rows for one call");
+        if (a->experts && a->n > (1 << 23)) return shape(op, "too many rows of weights for one call");      // (chunks times tiles are a 32-bit number)
         if (a->lda < a->k || a->ldo < a->n) return shape(op, "rows overlap");
         if (a->tokens == 0) return B200_OK;
         if (!a->a || !a->a_scales || !a->w || !a->w_scales || !a->out) return bad(op, "null pointer");
