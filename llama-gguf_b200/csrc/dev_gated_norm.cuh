@@ -33,15 +33,27 @@ __device__ __forceinline__ float gated_rstd(double sum, double per, float eps) {
     r = r * fma(-h * r, r, 1.5);
     return (float)r;
 }
-// Rows of any length and alignment: a block per row; what it makes of a row is kept in the sum's place.
-template <typename T> __global__ void __launch_bounds__(256) add_gated_norm_any_kernel(const GatedNormArgs a) {
+// Rows of any alignment: a block per row, which stays in registers where V blocks have its length (V > 0), element by element; longer ones (V = 0) in the sum's place, each element by the thread that wrote it.
+template <typename T, int V> __global__ void __launch_bounds__(1024) add_gated_norm_row_kernel(const GatedNormArgs a) {
     before();
     __shared__ double s_sum[32], s_sum2[32];
     __shared__ uint32_t s_max[32];
     const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, step = blockDim.x;
     const T *y = reinterpret_cast<const T*>(a.y) + row * a.top * a.ldy, *res = reinterpret_cast<const T*>(a.residual) + row * a.ldr;
     const T* gate = a.gate ? reinterpret_cast<const T*>(a.gate) + row * a.gate_row : nullptr;
     T* sum = reinterpret_cast<T*>(a.sum) + row * a.lds;
+    constexpr int N = V > 0 ? V : 1;
+    float r[N];
+    // every element of this thread, with its place in r and whether it is one (a place behind the last is read as the last, so that loads need no branch)
+    auto each = [&](auto&& f) {
+        if constexpr (V > 0) {
+#pragma unroll
+            for (int v = 0; v < V; v++) f(min(v * step + tid, a.hidden - 1), r[v], v * step + tid < a.hidden);
+        } else {
+            for (int i = tid; i < a.hidden; i += step) f(i, r[0], true);
+        }
+    };
     auto mixed = [&](int i) {
         if (!a.mix) return to_f(y[i]);
         float m = __fmul_rn(a.mix[row * a.top], to_f(y[i]));
@@ -51,29 +63,38 @@ template <typename T> __global__ void __launch_bounds__(256) add_gated_norm_any_
     float post = 1;
     if (a.post_weight) {
         double ss = 0;
-        for (int i = threadIdx.x; i < a.hidden; i += blockDim.x) {
-            const double m = mixed(i);
-            ss += m * m;
-        }
+        each([&](int i, float& x, bool) { x = mixed(i); });
+        each([&](int i, float& x, bool there) {
+            if (V == 0) x = mixed(i);
+            ss += there ? (double)x * x : 0.0;
+        });
         post = gated_rstd(block_sum(ss, s_sum), a.per, a.eps);
     }
     double ss = 0;
-    for (int i = threadIdx.x; i < a.hidden; i += blockDim.x) {
-        float p = mixed(i);
-        if (a.post_weight) p = __fmul_rn(__fmul_rn(p, post), a.post_weight[i]);
-        if (gate) p = __fmul_rn(p, to_f(gate[i * a.gate_col]));
-        const T r = from_f<T>(__fadd_rn(to_f(res[i]), __fmul_rn(p, a.scale)));
-        sum[i] = r;
-        ss += (double)to_f(r) * to_f(r);
-    }
+    if (V > 0 && !a.post_weight) each([&](int i, float& x, bool) { x = mixed(i); });
+    each([&](int i, float& x, bool there) {
+        if (V == 0) x = mixed(i);
+        if (a.post_weight) x = __fmul_rn(__fmul_rn(x, post), a.post_weight[i]);
+        if (gate) x = __fmul_rn(x, to_f(gate[i * a.gate_col]));
+        const T t = from_f<T>(__fadd_rn(there ? to_f(res[i]) : 0.0f, __fmul_rn(x, a.scale)));      // (sum may be residual: no thread reads another's element)
+        if (there) sum[i] = t;
+        x = to_f(t);
+        ss += there ? (double)x * x : 0.0;
+    });
     if (!a.weight) return;
     const float rstd = gated_rstd(block_sum(ss, s_sum2), a.per, a.eps);
-    uint32_t top = 0;
-    for (int i = threadIdx.x; i < a.hidden; i += blockDim.x) top = max(top, __float_as_uint(fabsf(__fmul_rn(__fmul_rn(to_f(sum[i]), rstd), a.weight[i]))));
-    const Q8Row q = q8_row(block_max(top, s_max));
-    for (int i = threadIdx.x; i < a.hidden; i += blockDim.x)
-        a.q[row * a.ldq + i] = q.inv == 0.0f ? (int8_t)0 : (int8_t)__float2int_rn(__fmul_rn(__fmul_rn(__fmul_rn(to_f(sum[i]), rstd), a.weight[i]), q.inv));
-    if (threadIdx.x == 0) a.scales[row] = q.scale;
+    float top = 0;
+    each([&](int i, float& x, bool there) {
+        if (V == 0) x = to_f(sum[i]);
+        x = __fmul_rn(__fmul_rn(x, rstd), a.weight[i]);
+        if (there) top = max_nan(top, fabsf(x));
+    });
+    const Q8Row q = q8_row(block_max(__float_as_uint(top), s_max));
+    each([&](int i, float& x, bool there) {
+        if (V == 0) x = __fmul_rn(__fmul_rn(to_f(sum[i]), rstd), a.weight[i]);
+        if (there) a.q[row * a.ldq + i] = q.inv == 0.0f ? (int8_t)0 : (int8_t)(__float_as_uint(__fadd_rn(__fmul_rn(x, q.inv), kRoundHere)) & 0xff);
+    });
+    if (tid == 0) a.scales[row] = q.scale;
 }
 
 // Rows of whole 16-byte words on 16 bytes: blocks stride over the rows; a row stays in registers (V words per thread), the next one's words are on their way to shared memory meanwhile, where each thread reads what it has
@@ -243,7 +264,10 @@ template <typename T> cudaError_t add_gated_norm(const GatedNormArgs& a, cudaStr
     const bool words = a.hidden % E == 0 && a.hidden / E <= 4096 && !off(a.y, a.ldy, 16, sizeof(T)) && !off(a.residual, a.ldr, 16, sizeof(T)) && !off(a.sum, a.lds, 16, sizeof(T)) &&
                        (!a.post_weight || !off(a.post_weight, 0, 16, 4)) && (!a.weight || (!off(a.weight, 0, 16, 4) && !off(a.q, a.ldq, E, 1))) &&
                        (!a.gate || a.gate_col == 0 || (a.gate_col == 1 && !off(a.gate, a.gate_row, 16, sizeof(T))));
-    if (!words) return launch(add_gated_norm_any_kernel<T>, dim3((unsigned)a.rows), 256, 0, 1, st, a);
+    if (!words) {
+        auto go = [&](auto kernel, int v) { return launch(kernel, dim3((unsigned)a.rows), ((a.hidden + v - 1) / v + 31) / 32 * 32, 0, 1, st, a); };
+        return a.hidden <= 1024 ? go(add_gated_norm_row_kernel<T, 4>, 4) : a.hidden <= 16384 ? go(add_gated_norm_row_kernel<T, 16>, 16) : launch(add_gated_norm_row_kernel<T, 0>, dim3((unsigned)a.rows), 1024, 0, 1, st, a);
+    }
     int sms = 0;
     const cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) return e;

@@ -51,8 +51,8 @@ __device__ __forceinline__ double block_max_double(double v, double* s) {
 constexpr double kGluMost = 3.4028235677973366e38;      // 2^128 - 2^103
 __device__ __forceinline__ bool glu_live(double top) { return top >= (double)kTiny && top < kGluMost; }
 __device__ __forceinline__ float glu_scale(double top) { return !(top < kGluMost) ? NAN : glu_live(top) ? (float)(top / 127.0) : 0.0f; }
-// Rows of any length and alignment: a block per row, read twice, everything in 64 bits.
-template <typename T> __global__ void __launch_bounds__(256) glu_q8_any_kernel(const GluQ8Args a) {
+// Rows that no registers hold: a block per row, read twice, everything in 64 bits.
+template <typename T> __global__ void __launch_bounds__(1024) glu_q8_any_kernel(const GluQ8Args a) {
     before();
     __shared__ double s_max[32];
     const int64_t row = blockIdx.x;
@@ -202,6 +202,86 @@ template <typename T, int V, int ACT> __global__ void __launch_bounds__(1024) gl
     }
 }
 
+// The same for rows of any length up to V blocks and any alignment: element by element, from memory again where something is made again.
+template <typename T, int V, int ACT> __global__ void __launch_bounds__(1024) glu_q8_row_kernel(const GluQ8Args a) {
+    before();
+    __shared__ double s_top[32];
+    const int64_t row = blockIdx.x;
+    const T *gate = reinterpret_cast<const T*>(a.x) + row * a.ldx, *up_ = gate + a.ff;
+    const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x >> 5;
+    float y[V], top = 0, low = 0;
+    uint32_t far = 0;      // where the gate is too far down for f32
+    {
+        T g[V], u[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const int i = min(v * (int)blockDim.x + tid, a.ff - 1);
+            g[v] = gate[i];
+            u[v] = up_[i];
+        }
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const bool there = v * (int)blockDim.x + tid < a.ff;
+            const float x = to_f(g[v]);
+            y[v] = there ? glu_near<ACT>(x, to_f(u[v])) : 0.0f;
+            low = fminf(low, x);
+            if (ACT != GLU_RELU && there && x <= glu_least<ACT>()) far |= 1u << v;
+        }
+    }
+    for (; far; far &= far - 1) {
+        const int k = __ffs(far) - 1, i = k * blockDim.x + tid;
+        const float x = (float)glu_exact(to_f(gate[i]), to_f(up_[i]), ACT);
+#pragma unroll
+        for (int v = 0; v < V; v++) y[v] = v == k ? x : y[v];
+    }
+#pragma unroll
+    for (int v = 0; v < V; v++) top = max_nan(top, fabsf(y[v]));
+    const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    const float least = __uint_as_float(most) * (1.0f - 2 * kGluOffMost);
+    double mine = most < kInfBits ? 0.0 : INFINITY;
+    if (most < kInfBits && top >= least) {
+        uint32_t which = 0;
+#pragma unroll
+        for (int v = 0; v < V; v++) which |= fabsf(y[v]) >= least ? 1u << v : 0u;
+        for (; which; which &= which - 1) {
+            const int i = (__ffs(which) - 1) * blockDim.x + tid;
+            if (i < a.ff) mine = fmax(mine, fabs(glu_exact(to_f(gate[i]), to_f(up_[i]), ACT)));
+        }
+    }
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)__double2hiint(mine)), lo = __reduce_max_sync(0xffffffffu, (uint32_t)__double2hiint(mine) == hi ? (uint32_t)__double2loint(mine) : 0u);
+    if (lane == 0) s_top[tid >> 5] = __hiloint2double((int)hi, (int)lo);
+    __syncthreads();
+    const double other = lane < warps ? s_top[lane] : 0.0;
+    const uint32_t bh = __reduce_max_sync(0xffffffffu, (uint32_t)__double2hiint(other)), bl = __reduce_max_sync(0xffffffffu, (uint32_t)__double2hiint(other) == bh ? (uint32_t)__double2loint(other) : 0u);
+    const double exact = __hiloint2double((int)bh, (int)bl);
+    if (tid == 0) a.scales[row] = glu_scale(exact);
+    const bool live = glu_live(exact);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"((float)exact * (1.0f / 127.0f)));
+    const float off = kGluOff - fmaxf(glu_z<ACT>(fmaxf(low, glu_least<ACT>())), -16.0f) * kGluOffZ, up = inv + inv * off, down = inv - inv * off;
+    int8_t* out = a.q + row * a.ldq;
+    uint32_t close = 0;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const int i = v * blockDim.x + tid;
+        const uint32_t n = __float_as_uint(fmaf(y[v], up, kRoundHere));
+        if (i < a.ff) {
+            if (n != __float_as_uint(fmaf(y[v], down, kRoundHere))) close |= 1u << v;
+            out[i] = live ? (int8_t)(n & 0xff) : (int8_t)0;
+        }
+    }
+    if (live)
+        for (; close; close &= close - 1) {
+            const int i = (__ffs(close) - 1) * blockDim.x + tid;
+            out[i] = (int8_t)__double2int_rn(glu_exact(to_f(gate[i]), to_f(up_[i]), ACT) * (127.0 / exact));
+        }
+}
+template <typename T, int V> cudaError_t glu_q8_row(const GluQ8Args& a, cudaStream_t st) {
+    const unsigned threads = ((a.ff + V - 1) / V + 31) / 32 * 32;
+    auto go = [&](auto kernel) { return launch(kernel, dim3((unsigned)a.rows), threads, 0, 1, st, a); };
+    return a.act == GLU_SILU ? go(glu_q8_row_kernel<T, V, GLU_SILU>) : a.act == GLU_GELU ? go(glu_q8_row_kernel<T, V, GLU_GELU>) : go(glu_q8_row_kernel<T, V, GLU_RELU>);
+}
+
 template <typename T, int V> cudaError_t glu_q8_words(const GluQ8Args& a, int threads, int blocks, cudaStream_t st) {
     const dim3 grid((unsigned)std::min<int64_t>(a.rows, blocks));
     const size_t most = V * 1024 * 32, smem = V * threads * 32;
@@ -213,7 +293,7 @@ template <typename T, int V> cudaError_t glu_q8_words(const GluQ8Args& a, int th
 template <typename T> cudaError_t glu_q8(const GluQ8Args& a, cudaStream_t st) {
     constexpr int E = 16 / (int)sizeof(T);
     const bool words = a.ff % E == 0 && a.ff / E <= 4096 && !(reinterpret_cast<uintptr_t>(a.x) & 15) && a.ldx % E == 0 && !(reinterpret_cast<uintptr_t>(a.q) % E) && a.ldq % E == 0;
-    if (!words) return launch(glu_q8_any_kernel<T>, dim3((unsigned)a.rows), 256, 0, 1, st, a);
+    if (!words) return a.ff <= 1024 ? glu_q8_row<T, 4>(a, st) : a.ff <= 16384 ? glu_q8_row<T, 16>(a, st) : launch(glu_q8_any_kernel<T>, dim3((unsigned)a.rows), 1024, 0, 1, st, a);
     int sms = 0;
     const cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) return e;
