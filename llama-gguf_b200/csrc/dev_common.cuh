@@ -83,43 +83,6 @@ template <int N> __device__ __forceinline__ void copy_where(uint32_t to, const v
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(N), "r"(there ? N : 0) : "memory");
 }
 
-// mbarriers.  Every wait is bounded (one second and more at any clock): a wait that gives up leaves a code in dev_watchdog, and its block goes to its end without further waits.
-static __device__ int dev_watchdog;      // 0, or the code of the wait that gave up last (one of each translation unit)
-
-__device__ __forceinline__ uint32_t sm_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
-__device__ __forceinline__ void bar_init_done() {
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, bool& alive, int code) {
-    if (!alive || bar_try(bar, parity)) return;
-    const long long t0 = clock64();
-    while (!bar_try(bar, parity))
-        if (clock64() - t0 > 2000000000LL) {
-            alive = false;
-            if (code) atomicExch(&dev_watchdog, code);
-            return;
-        }
-}
-__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
-// one lane of a converged warp, in a form that keeps the operands of what it issues in uniform registers
-__device__ __forceinline__ bool elect() {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
-    return ok != 0;
-}
-// `bytes` (a multiple of 16) from global to this block's shared memory, both on 16 bytes, counted by `bar`
-__device__ __forceinline__ void bulk_copy(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
-}
-
 // Clusters: barriers, and what lies in another block's shared memory
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;

@@ -301,7 +301,7 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
         I4Chunk x = i4_chunk<CHUNK>(a, l, c);
         // copies, I4_RING - 1 steps ahead of the products
         int cc = c, ct = tile, ce = x.e, cs = s, left = f1 - f0;
-        const int full = a.steps / 4;      // (whole steps of a tile: of its scales too, whose groups are whole)
+        const int full = a.k / 256;      // whole steps of a tile
         uint32_t into = ring;
         const uint8_t *cw = nullptr, *cd = nullptr;
         auto place = [&]() {

@@ -1,4 +1,5 @@
 // dev_umma.cuh — tensor-memory, mbarrier and TMA pieces of the operators on device tensors (tcgen05, sm_100a).
+// Every wait is bounded (one second and more at any clock): a wait that gives up leaves a code in dev_watchdog, and its block goes to its end without further waits.
 #pragma once
 #include <cuda.h>
 
@@ -6,6 +7,37 @@
 
 namespace dev {
 
+__device__ int dev_watchdog;      // 0, or the code of the wait that gave up last
+
+__device__ __forceinline__ uint32_t sm_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void bar_init_done() {
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, bool& alive, int code) {
+    if (!alive || bar_try(bar, parity)) return;
+    const long long t0 = clock64();
+    while (!bar_try(bar, parity))
+        if (clock64() - t0 > 2000000000LL) {
+            alive = false;
+            if (code) atomicExch(&dev_watchdog, code);
+            return;
+        }
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+// one lane of a converged warp, in a form that keeps the operands of what it issues in uniform registers
+__device__ __forceinline__ bool elect() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
+}
 template <bool PAIR> __device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t cols) {      // one whole warp
     if constexpr (PAIR) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm_u32(where)), "r"(cols) : "memory");

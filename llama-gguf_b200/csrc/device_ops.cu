@@ -32,9 +32,6 @@ extern "C" int b200_dev_watchdog(int device, int* out) {
             const int zero = 0;
             cudaError_t e = cudaMemcpyFromSymbol(out, dev_watchdog, sizeof(int));
             if (e == cudaSuccess && *out) e = cudaMemcpyToSymbol(dev_watchdog, &zero, sizeof(int));
-            int more = 0;
-            if (e == cudaSuccess) e = (cudaError_t)dev_experts_watchdog(&more);
-            if (e == cudaSuccess && !*out) *out = more;
             return e;
         });
     });

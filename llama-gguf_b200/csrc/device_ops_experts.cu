@@ -9,13 +9,6 @@
 
 using namespace dev;
 
-int dev_experts_watchdog(int* code) {
-    const int zero = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(code, dev_watchdog, sizeof(int));
-    if (e == cudaSuccess && *code) e = cudaMemcpyToSymbol(dev_watchdog, &zero, sizeof(int));
-    return (int)e;
-}
-
 extern "C" int b200_dev_route_experts(const b200_route* a) {
     const char* op = "route_experts";
     return entry(op, [&]() -> int {

@@ -157,6 +157,27 @@ def test_product(D, dtype, rows, k, n, group):
     check_product(D, bytes_of(rows, rows, k), four_bits(k, n, k), scales, dtype, bias=normal(3, n) if n % 2 else None)
 
 
+@pytest.mark.parametrize("k,group", [(224, 32), (32, 32), (96, 32), (160, 32), (192, 64), (64, 64), (384, 128), (480, 32), (1248, 32)])
+@pytest.mark.parametrize("rows", [1, 2, 4, 8, 16, 20, 64])
+@pytest.mark.parametrize("experts", [0, 3])
+def test_product_reads_nothing_behind_its_operands(D, k, group, rows, experts):
+    """NaN scales behind the last tile's, numbers behind the rows' channels and in a last tile's unused channels: none of them counts."""
+    n, E = 21, max(1, experts)
+    values, scales = four_bits(k, E, n, k), 0.01 * normal(2, E, n, k // group).abs() + 0.001
+    w, ws = D.i4_weights(values, scales)
+    if k % 64:
+        w = w.unflatten(-1, (8, 4, 2, 2, 4)).clone()
+        w[:, :, -1, :, :, 1] = 0x5A      # (channels 32 to 63 of the last tile)
+        w = w.flatten(3)
+    behind = lambda t, v: torch.cat([t.flatten(), torch.full((4096,), v, dtype=t.dtype)]).cuda()[: t.numel()].view(t.shape)  # noqa: E731
+    w, ws = behind(w, 0x77), behind(ws, math.nan)
+    a = bytes_of(3, rows, k, extra=16)
+    s, e = torch.ones(rows), chosen(4, rows, 1, E) if experts else None
+    y = D.mat_mat_i4(a, s.cuda(), w if experts else w[0], ws if experts else ws[0], n=n, experts=None if e is None else e.cuda(), dtype=torch.float32)
+    want, off = R.product(a.cpu(), s, values if experts else values[0], scales if experts else scales[0], e)
+    assert ((y.cpu().double() - want).abs() <= off + 2.0**-24 * want.abs()).all()
+
+
 @pytest.mark.parametrize("scale", TYPES)
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("rows", [1, 12, 33, 70])
