@@ -97,164 +97,140 @@ template <typename T, int V> __global__ void __launch_bounds__(1024) add_gated_n
     if (tid == 0) a.scales[row] = q.scale;
 }
 
-// Rows of whole 16-byte words on 16 bytes: blocks stride over the rows; a row stays in registers (V words per thread), the next one's words are on their way to shared memory meanwhile, where each thread reads what it has
-// copied itself.  With one word per thread both weights are kept.  GATE: 0 none, 1 one number per row, 2 words (of this row, or of all rows).
-template <typename T, int V, int GATE, bool POST, int MOST> __global__ void __launch_bounds__(MOST) add_gated_norm_kernel(const GatedNormArgs a) {
+// Rows of whole 16-byte words on 16 bytes: a block per row, which stays in registers (V words per thread) from its copy to shared memory on (cp.async: each thread reads what it has copied itself, when it needs it).  With one word per thread
+// both weights are asked for at once and kept.  GATE: 0 none, 1 one number per row, 2 words (of this row, or of all rows).
+// What bounds it: 64-bit sums (a conversion of each element for each norm), reductions, and the weights' bytes from L2 behind a sum that they do not need (2048 x 4096 bf16 with both norms and a gate per channel: 16.5 us by itself, 67 MB: 10.2
+// at the measured rate; without the first norm 10.8).  Blocks that strode over the rows with the next row's words on their way took 18.4 and 12.5, with the weights asked for ahead of the sums (128 registers, half the blocks) 18.8.
+template <typename T, int V, int GATE, bool POST> __global__ void __launch_bounds__(1024) add_gated_norm_kernel(const GatedNormArgs a) {
     before();
     constexpr int E = 16 / (int)sizeof(T);
-    constexpr bool KEPT = V == 1, EARLY = MOST < 1024 && !KEPT;      // weights in registers; asked for ahead of the sum that they wait for
+    constexpr bool KEPT = V == 1;
     extern __shared__ uint4 gated_words[];      // [y, residual, gate][V][threads]
     __shared__ double s_sum[2][32];
     __shared__ uint32_t s_max[32];
     const int words = a.hidden / E, tid = threadIdx.x, step = blockDim.x;
     const uint4* mine = gated_words + tid;
     const uint32_t to = (uint32_t)__cvta_generic_to_shared(mine);
-    auto copy = [&](int64_t row) {
-        if (row < a.rows) {
-            const uint4 *res = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.residual) + row * a.ldr) + tid, *y = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.y) + row * a.top * a.ldy) + tid,
-                        *gate = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.gate) + row * a.gate_row) + tid;
+    const int64_t row = blockIdx.x;
+    const uint4 *res = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.residual) + row * a.ldr) + tid, *y = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.y) + row * a.top * a.ldy) + tid,
+                *gate = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.gate) + row * a.gate_row) + tid;
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                const bool there = v * step + tid < words;
-                copy_where<16>(to + v * step * 16, there ? y + v * step : a.y, there);
-                copy_where<16>(to + (V + v) * step * 16, there ? res + v * step : a.y, there);
-                if (GATE == 2) copy_where<16>(to + (2 * V + v) * step * 16, there ? gate + v * step : a.y, there);
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
+    for (int v = 0; v < V; v++) {
+        const bool there = v * step + tid < words;
+        copy_where<16>(to + v * step * 16, there ? y + v * step : a.y, there);
+        copy_where<16>(to + (V + v) * step * 16, there ? res + v * step : a.y, there);
+        if (GATE == 2) copy_where<16>(to + (2 * V + v) * step * 16, there ? gate + v * step : a.y, there);
+    }
     float pw[KEPT ? E : 1], nw[KEPT ? E : 1];
     if constexpr (KEPT)
         if (tid < words) {
             if constexpr (POST) load_n<float, E, true>(a.post_weight + tid * E, pw);
             if (a.weight) load_n<float, E, true>(a.weight + tid * E, nw);
         }
-    constexpr int W = EARLY ? V * E : 1;
-    float ew[W];
-    auto ask = [&](const float* from) {
-        if constexpr (EARLY) {
+    const float one = GATE == 1 ? to_f(reinterpret_cast<const T*>(a.gate)[row * a.gate_row]) : 1.0f;
+    float r[V][E];
+    const float* mix = a.mix ? a.mix + row * a.top : nullptr;
+    const float m0 = mix ? mix[0] : 1.0f;
+    asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                float g[E] = {};
-                if (v * step + tid < words) load_n<float, E, true>(from + (v * step + tid) * E, g);
+    for (int v = 0; v < V; v++) {
+        const uint4 w = mine[v * step];
 #pragma unroll
-                for (int e = 0; e < E; e++) ew[v * E + e] = g[e];
-            }
-        }
-    };
-    copy(blockIdx.x);
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const float one = GATE == 1 ? to_f(reinterpret_cast<const T*>(a.gate)[row * a.gate_row]) : 1.0f;
-        float r[V][E];
-        const float* mix = a.mix ? a.mix + row * a.top : nullptr;
-        const float m0 = mix ? mix[0] : 1.0f;
-        asm volatile("cp.async.wait_all;" ::: "memory");
+        for (int e = 0; e < E; e++) r[v][e] = to_f(reinterpret_cast<const T*>(&w)[e]);
+    }
+    if (mix) {
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-            const uint4 w = mine[v * step];
+        for (int v = 0; v < V; v++)
 #pragma unroll
-            for (int e = 0; e < E; e++) r[v][e] = to_f(reinterpret_cast<const T*>(&w)[e]);
-        }
-        if (mix) {
-#pragma unroll
-            for (int v = 0; v < V; v++)
-#pragma unroll
-                for (int e = 0; e < E; e++) r[v][e] = __fmul_rn(m0, r[v][e]);
-        }
-        for (int j = 1; j < a.top; j++) {
-            const float m = mix[j];
-            const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.y) + (row * a.top + j) * a.ldy);
-            uint4 w[V];
-#pragma unroll
-            for (int v = 0; v < V; v++) {
-                const int i = v * step + tid;
-                w[v] = i < words ? p[i] : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int v = 0; v < V; v++)
-#pragma unroll
-                for (int e = 0; e < E; e++) r[v][e] = __fadd_rn(r[v][e], __fmul_rn(m, to_f(reinterpret_cast<const T*>(&w[v])[e])));
-        }
-        if constexpr (POST) {
-            double ss = 0;
-#pragma unroll
-            for (int v = 0; v < V; v++)
-#pragma unroll
-                for (int e = 0; e < E; e++) ss += (double)r[v][e] * r[v][e];
-            ask(a.post_weight);
-            const float post = gated_rstd(block_sum(ss, s_sum[0]), a.per, a.eps);
-#pragma unroll
-            for (int v = 0; v < V; v++) {
-                const int i = v * step + tid;
-                if (i < words) {
-                    float g[E];
-                    if constexpr (!KEPT && !EARLY) load_n<float, E, true>(a.post_weight + i * E, g);
-#pragma unroll
-                    for (int e = 0; e < E; e++) r[v][e] = __fmul_rn(__fmul_rn(r[v][e], post), KEPT ? pw[KEPT ? e : 0] : EARLY ? ew[EARLY ? v * E + e : 0] : g[e]);
-                }
-            }
-        }
-        uint4* sum = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.sum) + row * a.lds);
-        double ss = 0;
+            for (int e = 0; e < E; e++) r[v][e] = __fmul_rn(m0, r[v][e]);
+    }
+    for (int j = 1; j < a.top; j++) {
+        const float m = mix[j];
+        const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.y) + (row * a.top + j) * a.ldy);
+        uint4 w[V];
 #pragma unroll
         for (int v = 0; v < V; v++) {
             const int i = v * step + tid;
-            uint4 d = mine[(V + v) * step];
-            const uint4 h = GATE == 2 ? mine[(2 * V + v) * step] : make_uint4(0, 0, 0, 0);
-            T* p = reinterpret_cast<T*>(&d);
+            w[v] = i < words ? p[i] : make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                if (GATE == 1) r[v][e] = __fmul_rn(r[v][e], one);
-                if (GATE == 2) r[v][e] = __fmul_rn(r[v][e], to_f(reinterpret_cast<const T*>(&h)[e]));
-                p[e] = from_f<T>(__fadd_rn(to_f(p[e]), __fmul_rn(r[v][e], a.scale)));
-                r[v][e] = to_f(p[e]);
-                ss += std::is_same<T, __half>::value ? (double)(r[v][e] * r[v][e]) : (double)r[v][e] * r[v][e];      // (squares of f16 are exact in f32)
-            }
-            if (i < words) sum[i] = d;
-        }
-        copy(row + gridDim.x);      // (sum may be residual: other rows)
-        if (!a.weight) {
-            if (POST) __syncthreads();      // (the next row writes what this one's sums are read from)
-            continue;
-        }
-        ask(a.weight);
-        const float rstd = gated_rstd(block_sum(ss, s_sum[1]), a.per, a.eps);
-        float top = 0;
+        for (int v = 0; v < V; v++)
+#pragma unroll
+            for (int e = 0; e < E; e++) r[v][e] = __fadd_rn(r[v][e], __fmul_rn(m, to_f(reinterpret_cast<const T*>(&w[v])[e])));
+    }
+    if constexpr (POST) {
+        double ss = 0;
+#pragma unroll
+        for (int v = 0; v < V; v++)
+#pragma unroll
+            for (int e = 0; e < E; e++) ss += (double)r[v][e] * r[v][e];
+        const float post = gated_rstd(block_sum(ss, s_sum[0]), a.per, a.eps);
 #pragma unroll
         for (int v = 0; v < V; v++) {
             const int i = v * step + tid;
             if (i < words) {
                 float g[E];
-                if constexpr (!KEPT && !EARLY) load_n<float, E, true>(a.weight + i * E, g);
+                if constexpr (!KEPT) load_n<float, E, true>(a.post_weight + i * E, g);
 #pragma unroll
-                for (int e = 0; e < E; e++) {
-                    r[v][e] = __fmul_rn(__fmul_rn(r[v][e], rstd), KEPT ? nw[KEPT ? e : 0] : EARLY ? ew[EARLY ? v * E + e : 0] : g[e]);
-                    top = max_nan(top, fabsf(r[v][e]));
-                }
+                for (int e = 0; e < E; e++) r[v][e] = __fmul_rn(__fmul_rn(r[v][e], post), KEPT ? pw[KEPT ? e : 0] : g[e]);
             }
         }
-        const Q8Row q = q8_row(block_max(__float_as_uint(top), s_max));
-        int8_t* out = a.q + row * a.ldq;
-#pragma unroll
-        for (int v = 0; v < V; v++) {
-            const int i = v * step + tid;
-            if (i < words) store_q8<E>(out + i * E, r[v], q.inv);
-        }
-        if (tid == 0) a.scales[row] = q.scale;
     }
+    uint4* sum = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.sum) + row * a.lds);
+    double ss = 0;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const int i = v * step + tid;
+        uint4 d = mine[(V + v) * step];
+        const uint4 h = GATE == 2 ? mine[(2 * V + v) * step] : make_uint4(0, 0, 0, 0);
+        T* p = reinterpret_cast<T*>(&d);
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            if (GATE == 1) r[v][e] = __fmul_rn(r[v][e], one);
+            if (GATE == 2) r[v][e] = __fmul_rn(r[v][e], to_f(reinterpret_cast<const T*>(&h)[e]));
+            p[e] = from_f<T>(__fadd_rn(to_f(p[e]), __fmul_rn(r[v][e], a.scale)));
+            r[v][e] = to_f(p[e]);
+            ss += std::is_same<T, __half>::value ? (double)(r[v][e] * r[v][e]) : (double)r[v][e] * r[v][e];      // (squares of f16 are exact in f32)
+        }
+        if (i < words) sum[i] = d;
+    }
+    if (!a.weight) return;
+    const float rstd = gated_rstd(block_sum(ss, s_sum[1]), a.per, a.eps);
+    float top = 0;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const int i = v * step + tid;
+        if (i < words) {
+            float g[E];
+            if constexpr (!KEPT) load_n<float, E, true>(a.weight + i * E, g);
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                r[v][e] = __fmul_rn(__fmul_rn(r[v][e], rstd), KEPT ? nw[KEPT ? e : 0] : g[e]);
+                top = max_nan(top, fabsf(r[v][e]));
+            }
+        }
+    }
+    const Q8Row q = q8_row(block_max(__float_as_uint(top), s_max));
+    int8_t* out = a.q + row * a.ldq;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const int i = v * step + tid;
+        if (i < words) store_q8<E>(out + i * E, r[v], q.inv);
+    }
+    if (tid == 0) a.scales[row] = q.scale;
 }
 
-template <typename T, int V, int MOST> cudaError_t add_gated_norm_words(const GatedNormArgs& a, int threads, int blocks, cudaStream_t st) {
+template <typename T, int V> cudaError_t add_gated_norm_words(const GatedNormArgs& a, int threads, cudaStream_t st) {
     const int gate = !a.gate ? 0 : a.gate_col == 0 ? 1 : 2;
-    const dim3 grid((unsigned)std::min<int64_t>(a.rows, blocks));
-    const size_t most = V * MOST * 48, smem = V * threads * (gate == 2 ? 48 : 32);
+    const dim3 grid((unsigned)a.rows);
+    const size_t most = V * 1024 * 48, smem = V * threads * (gate == 2 ? 48 : 32);
     if (a.post_weight)
-        return gate == 0   ? launch_with<add_gated_norm_kernel<T, V, 0, true, MOST>>(most, grid, threads, smem, st, a)
-               : gate == 1 ? launch_with<add_gated_norm_kernel<T, V, 1, true, MOST>>(most, grid, threads, smem, st, a)
-                           : launch_with<add_gated_norm_kernel<T, V, 2, true, MOST>>(most, grid, threads, smem, st, a);
-    return gate == 0   ? launch_with<add_gated_norm_kernel<T, V, 0, false, MOST>>(most, grid, threads, smem, st, a)
-           : gate == 1 ? launch_with<add_gated_norm_kernel<T, V, 1, false, MOST>>(most, grid, threads, smem, st, a)
-                       : launch_with<add_gated_norm_kernel<T, V, 2, false, MOST>>(most, grid, threads, smem, st, a);
+        return gate == 0   ? launch_with<add_gated_norm_kernel<T, V, 0, true>>(most, grid, threads, smem, st, a)
+               : gate == 1 ? launch_with<add_gated_norm_kernel<T, V, 1, true>>(most, grid, threads, smem, st, a)
+                           : launch_with<add_gated_norm_kernel<T, V, 2, true>>(most, grid, threads, smem, st, a);
+    return gate == 0   ? launch_with<add_gated_norm_kernel<T, V, 0, false>>(most, grid, threads, smem, st, a)
+           : gate == 1 ? launch_with<add_gated_norm_kernel<T, V, 1, false>>(most, grid, threads, smem, st, a)
+                       : launch_with<add_gated_norm_kernel<T, V, 2, false>>(most, grid, threads, smem, st, a);
 }
 // Few rows: as many threads as a row has words, up to 1024 (latency).  Many rows: four words per thread, so that several blocks of an SM (its 65 536 registers hold 1024 threads) cover one another's barriers, and the sums over
 // a block take fewer instructions.
@@ -272,9 +248,7 @@ template <typename T> cudaError_t add_gated_norm(const GatedNormArgs& a, cudaStr
     const cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) return e;
     const int n = a.hidden / E, many = a.rows > 2 * sms, v = n > 2048 || (many && n >= 256) ? 4 : n > 1024 || (many && n >= 64) ? 2 : 1, threads = ((n + v - 1) / v + 31) / 32 * 32;
-    if (v == 4 && threads <= 256) return add_gated_norm_words<T, 4, 256>(a, threads, sms * std::max(1, 512 / threads), st);
-    const int blocks = sms * std::max(1, 1024 / threads);
-    return v == 4 ? add_gated_norm_words<T, 4, 1024>(a, threads, blocks, st) : v == 2 ? add_gated_norm_words<T, 2, 1024>(a, threads, blocks, st) : add_gated_norm_words<T, 1, 1024>(a, threads, blocks, st);
+    return v == 4 ? add_gated_norm_words<T, 4>(a, threads, st) : v == 2 ? add_gated_norm_words<T, 2>(a, threads, st) : add_gated_norm_words<T, 1>(a, threads, st);
 }
 
 }  // namespace dev
