@@ -624,7 +624,8 @@ B200_API int b200_dev_route_experts(const b200_route* a);
  * [ceil(n / 16)][k / group][8][row half] of scale_type (F32, F16 or BF16).
  * With `experts` ([tokens][top] int32) there are n_experts such matrices one after the other (and [n_experts][n] of bias), out has a row for each pair (token, place) and is
  * [tokens * top][n]; a has a row per token, or per pair where rows_per_pair is set.  Pairs of expert -1 get zeros; other numbers outside 0 .. n_experts - 1 too, BAD_EXPERT.
- * a starts on 16 bytes with rows a multiple of 16 bytes apart; what lies between k and the next row is not used.  w and the scales start on 16 bytes.  Meant for few rows: the weights' bytes
+ * a starts on 16 bytes with rows a multiple of 16 bytes apart; what lies between k and the next row is not used.  w and the scales start on 16 bytes.  With experts n <= 2^23,
+ * n_experts <= 1024, top <= 32.  The same call gives the same bits; another number of rows may add the groups up in another order.  Meant for few rows: the weights' bytes
  * are read once per 64 rows (of an expert). */
 typedef struct b200_i4_product {
     int32_t device;

@@ -13,6 +13,11 @@
 //   more warps have a part of in shared memory for the end.  Rows of a come from L1 and L2.
 //   more rows (up to 64 at a time): rows of a cost as much as weights.  A block has eight tiles; its teams of four warps have a part of the channels each, whose rows of a serve all eight.  With few units the
 //   blocks of a cluster share the channels of one.
+// What bounds it.  Few rows: the weights' bytes from some 30 MB on (one token through two of eight experts, 28672 x 4096 in groups of 32 with f16 scales: 25.2 us for 132 MB, 5.2 TB/s, of which 6.5 us are launch, list, first bytes and the last
+// sums; 4096 to 8192 channels of one matrix add 66 MB in 10 us), below that the launch and a chain of loads (6144 x 4096: 7.3 us; a call of nothing 3.4).  Sixteen tokens' units of up to eight rows: issue slots, 50 us for 263 MB.  More rows: issue
+// slots and the latency of a team's step (33 rows of 4096 x 14336 20.3 us, of 8192 x 28672 56, 2.2 TB/s; the integer pipe is active 24 %).  Measured on the way: loads to registers, two steps ahead, 55 us (token, two experts);
+// the ring, 64-bit arithmetic in every unit, 47; shared steps 38; several groups in the columns 26.  More rows: rows of a from L1 51 us (33 rows); a ring of four tiles a warp 33; sixteen warps on one step 25; teams of eight
+// warps with one tile 24, of four with two 20; a warp that copies for all by bulk copies (of 128 bytes for a row) 73.  Copies with nothing computed per step but an addition took 100 instructions a step off.
 #pragma once
 #include <algorithm>
 #include <cmath>
@@ -173,7 +178,7 @@ template <typename S, int GROUP, int C> __device__ __noinline__ void i4_copy_las
 
 // ------------------------------------------------------------------------------------------------------------- few rows
 // A step's sums of one tile with TC rows of a (1, 2, 4; 8: eight rows each in NT blocks of columns).  TC rows are TC of the eight columns; with fewer than eight the other columns take the same rows' other
-// groups: column n has row n % TC and group n / TC of the (up to) 8 / TC that one set of sums has, so that what a group's sum costs afterwards (a subtraction and a multiplication in each lane) is paid once for all
+// groups: column n has row n % TC and group n / TC of the (up to) 8 / TC that one set of sums has, so that what a group's sum costs afterwards (a conversion and a product in each lane) is paid once for all
 // of them.  (One row in one column took 240 instructions for 128 channels.)
 template <typename S, int GROUP, int TC, int NT> struct I4Step {
     static constexpr int GC = GROUP / 32, GS = 256 / GROUP, SETS = GS * TC > 8 ? GS * TC / 8 : 1, PER = GS / SETS;      // chunks (of 32 channels) of a group, groups of a step, sets of sums, groups of a set

@@ -10,7 +10,15 @@ that require one, or have a forward-mode tangent, are refused), and have memory 
     q = rope_append_q4(q, k, v, table, positions, pages, slots)         # rotation; keys and values into the cache
     o = attention_paged_q4(q, pages, page_table, kv_lens, scale)
 
-Errors are those of the backend (ShapeMismatch, InvalidArgument, ...).  What lies in device memory (slots, positions, pages, lengths) is checked by the kernels:
+and its feed-forward with weights in 4 bits, here of routed experts:
+
+    experts, weights = route_experts(logits, 2)                         # each token's experts
+    h = mat_mat_i4(q, s, up, up_scales, experts=experts)                # 4-bit weights: [tokens * 2, 2 ff], gate and up
+    q, s = glu_q8(h)                                                    # rows in 8 bits again
+    y = mat_mat_i4(q, s, down, down_scales, experts=experts)
+    q, s, r = add_gated_norm_q8(y, r, weight, eps, mix=weights)         # their weighted sum onto the stream, the next norm's rows
+
+Errors are those of the backend (ShapeMismatch, InvalidArgument, ...).  What lies in device memory (slots, positions, pages, lengths, experts) is checked by the kernels:
 a bad entry is never followed, and sets a bit of `status` (an int32 tensor of one element) where one is given: STATUS_*.
 """
 import ctypes as C
@@ -201,8 +209,8 @@ def mat_mat_i4(a, a_scales, w, w_scales, n=None, experts=None, bias=None, dtype=
 
     w, w_scales: i4_weights, quantise_i4 or i4_from_q4_0 make them; n None: all rows of their tiles.  experts int32 [tokens, top] (route_experts): w, w_scales and bias have a leading dimension of
     experts, and the result [tokens * top, n] has a row for each of a token's experts; a has a row per token, or [tokens * top] rows, one for each.  Pairs of expert -1 get zeros, other numbers that
-    are no expert too (and set STATUS_BAD_EXPERT).  The sums of a group are exact.  a starts on 16 bytes with rows a multiple of 16 bytes apart (padded_rows).  For few rows: the weights'
-    bytes are what it costs, once for every 64 rows of a matrix."""
+    are no expert too (and set STATUS_BAD_EXPERT).  The sums of a group are exact; those over the groups are f32, in an order that the number of rows may change.  a starts on 16 bytes with rows a multiple of 16
+    bytes apart (padded_rows).  For few rows: the weights' bytes are what it costs, once for every 64 rows of a matrix."""
     return _ops().mat_mat_i4(a, a_scales, w, w_scales, n, experts, bias, dtype, out, status)
 
 
