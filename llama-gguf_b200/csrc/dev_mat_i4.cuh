@@ -132,9 +132,9 @@ template <int MOST> __device__ __forceinline__ I4Chunk i4_chunk(const MatI4Args&
     return I4Chunk{e, lo, min(MOST, l.end[e] - lo)};
 }
 __device__ __forceinline__ int i4_pair(const MatI4Args& a, const I4List& l, int i) { return a.experts ? l.list[i] : i; }
-__device__ __forceinline__ float i4_row_scale(const MatI4Args& a, int p) { return 0.0625f * a.a_scales[(a.first + p) / a.div]; }
+__device__ __forceinline__ float i4_row_scale(const MatI4Args& a, int p) { return a.a_scales[(a.first + p) / a.div]; }
 __device__ __forceinline__ void i4_put(const MatI4Args& a, int e, int p, int n, float sum, float scale) {
-    float y = sum * scale;
+    float y = (sum * 0.0625f) * scale;      // (the products are sixteen times the values; a scale may be as small as 2^-126, and a sixteenth of that has fewer bits)
     if (a.bias) y += a.bias[(int64_t)e * a.n + n];
     const int64_t to = (int64_t)(a.first + p) * a.ldo + n;
     if (a.out_type == B200_TYPE_F32) reinterpret_cast<float*>(a.out)[to] = y;

@@ -197,6 +197,21 @@ def test_product_of_the_largest_numbers(D, rows):
     check_product(D, a, four_bits(1, 20, 512), torch.ones(20, 4).half(), torch.float32)
 
 
+@pytest.mark.parametrize("rows", [1, 8, 40])
+def test_product_of_rows_with_the_smallest_scales(D, rows):
+    """A row's scale of 2^-126 and a little more has all its bits; the weights' large ones bring the result back."""
+    values, scales = four_bits(1, 20, 256), 2.0**100 * (1 + torch.rand(20, 8, generator=torch.Generator().manual_seed(2)))
+    a, s = bytes_of(2, rows, 256), 2.0**-126 * (1 + torch.rand(rows, generator=torch.Generator().manual_seed(3)))
+    w, ws = (v.cuda() for v in D.i4_weights(values, scales))
+    y = D.mat_mat_i4(a, s.cuda(), w, ws, n=20, dtype=torch.float32)
+    want, off = R.product(a.cpu(), s, values, scales)
+    assert ((y.cpu().double() - want).abs() <= off + 2.0**-24 * want.abs()).all()
+
+
+def test_product_of_many_rows(D):
+    check_product(D, bytes_of(1, 1001, 160), four_bits(2, 200, 160), 0.01 * normal(3, 200, 5), torch.float32, bias=normal(4, 200))
+
+
 def test_product_of_rows_apart_and_into_tensors(D):
     values, scales = four_bits(1, 50, 320), 0.01 * normal(2, 50, 10)
     a = bytes_of(3, 11, 320, extra=48)
