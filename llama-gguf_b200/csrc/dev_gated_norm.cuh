@@ -63,7 +63,7 @@ template <typename T, int V> __global__ void __launch_bounds__(1024) add_gated_n
     float post = 1;
     if (a.post_weight) {
         double ss = 0;
-        each([&](int i, float& x, bool) { x = mixed(i); });
+        if (V > 0) each([&](int i, float& x, bool) { x = mixed(i); });
         each([&](int i, float& x, bool there) {
             if (V == 0) x = mixed(i);
             ss += there ? (double)x * x : 0.0;
@@ -99,8 +99,8 @@ template <typename T, int V> __global__ void __launch_bounds__(1024) add_gated_n
 
 // Rows of whole 16-byte words on 16 bytes: a block per row, which stays in registers (V words per thread) from its copy to shared memory on (cp.async: each thread reads what it has copied itself, when it needs it).  With one word per thread
 // both weights are asked for at once and kept.  GATE: 0 none, 1 one number per row, 2 words (of this row, or of all rows).
-// What bounds it: 64-bit sums (a conversion of each element for each norm), reductions, and the weights' bytes from L2 behind a sum that they do not need (2048 x 4096 bf16 with both norms and a gate per channel: 16.5 us by itself, 67 MB: 10.2
-// at the measured rate; without the first norm 10.8).  Blocks that strode over the rows with the next row's words on their way took 18.4 and 12.5, with the weights asked for ahead of the sums (128 registers, half the blocks) 18.8.
+// What bounds it: 64-bit sums (a conversion of each element for each norm), reductions, and the weights' bytes from L2 behind a sum that they do not need (2048 x 4096 bf16 with both norms and a gate per channel: 15.9 us by itself, 67 MB: 10.2
+// at the measured rate; without the first norm 10.3).  Blocks that strode over the rows with the next row's words on their way took 18.4 and 12.5, with the weights asked for ahead of the sums (128 registers, half the blocks) 18.8.
 template <typename T, int V, int GATE, bool POST> __global__ void __launch_bounds__(1024) add_gated_norm_kernel(const GatedNormArgs a) {
     before();
     constexpr int E = 16 / (int)sizeof(T);
