@@ -24,10 +24,9 @@
 #include <type_traits>
 
 #include "dev_common.cuh"
+#include "dev_mat_i4_plan.cuh"
 
 namespace dev {
-
-enum { I4_TILE = 512, I4_PAIRS = 2048, I4_RING = 3 };      // bytes of a tile, pairs of a launch, steps of a warp's ring (few rows)
 
 struct MatI4Args {
     const int8_t* a;
@@ -64,7 +63,6 @@ struct I4List {
     int *end, *chunk;
     uint16_t *list, *of;
 };
-__host__ __device__ constexpr size_t i4_list_bytes(int experts, int pairs) { return (size_t)(2 * (experts + 2)) * 4 + (size_t)pairs * 4; }
 __device__ __forceinline__ I4List i4_list(void* smem, const MatI4Args& a) {
     int* p = reinterpret_cast<int*>(smem);
     uint16_t* q = reinterpret_cast<uint16_t*>(p + 2 * (a.n_experts + 2));
@@ -158,9 +156,7 @@ template <typename S> __device__ __forceinline__ float2 i4_scales(const uint8_t*
     const W w = *reinterpret_cast<const W*>(p);
     return make_float2(to_f(w.lo), to_f(w.hi));
 }
-// What a ring holds of a step of C tiles' channels of one tile of rows: the weights, then the groups' scales.
-template <typename S, int GROUP, int C> __host__ __device__ constexpr int i4_slot() { return C * I4_TILE + 16 * (int)sizeof(S) * (64 * C / GROUP); }
-// ... copied, from w (this lane's 16 bytes of the step's first tile) and d (its 8 bytes of the scales).  A whole step, with nothing to be asked; and the last one of a tile, with zeros behind the last channel.
+// A step of C tiles' channels of one tile of rows (i4_slot) copied to a ring, from w (this lane's 16 bytes of the step's first tile) and d (its 8 bytes of the scales).  A whole step, with nothing to be asked; and the last one of a tile, with zeros behind the last channel.
 template <typename S, int GROUP, int C> __device__ __forceinline__ void i4_copy(uint32_t to, const uint8_t* w, const uint8_t* d, int lane) {
     constexpr int WORDS = 64 * C / GROUP * 2 * (int)sizeof(S);      // 8-byte words of the scales
 #pragma unroll
@@ -246,7 +242,7 @@ template <typename S, int GROUP, int TC, int NT> struct I4Step {
 template <int NT> __host__ __device__ constexpr int i4_few_warps() { return NT == 1 ? 12 : 8; }
 template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_few_warps<NT>() * 32, 2) mat_mat_i4_few_kernel(const MatI4Args a) {
     before();
-    constexpr int SLOT = i4_slot<S, GROUP, 4>(), SB = 16 * (int)sizeof(S), CHUNK = 8 * NT, WARPS = i4_few_warps<NT>();
+    constexpr int SLOT = i4_slot(sizeof(S), GROUP, 4), SB = 16 * (int)sizeof(S), CHUNK = 8 * NT, WARPS = i4_few_warps<NT>();
     extern __shared__ __align__(16) uint8_t i4_smem[];
     float4* parts = reinterpret_cast<float4*>(i4_smem + WARPS * I4_RING * SLOT);      // [warps][its first unit, its last][NT][32]
     const I4List l = i4_list(parts + WARPS * 2 * NT * 32, a);
@@ -416,18 +412,16 @@ template <typename S, int GROUP, int NT> __global__ void __launch_bounds__(i4_fe
 
 // ------------------------------------------------------------------------------------------------------------- more rows
 // Four teams of four warps; a team has a part of the channels, 128 at a time, and its own ring, so that the teams' copies, products and sums overlap.  A warp has two of the unit's eight tiles; the rows of a are the
-// team's.
-enum { I4_TEAMS = 4, I4_TEAM_WARPS = 4, I4_TEAM_TILES = 8, I4_MANY_ROWS = 64, I4_MANY_RING = 4 };
-template <typename S, int GROUP> __host__ __device__ constexpr int i4_many_slot(int rows) { return I4_TEAM_TILES * i4_slot<S, GROUP, 2>() + rows * 128; }
+// team's.  As many blocks of columns are computed as i4_many_blocks says, and a step has room for the rows of all of them (i4_many_plan).
 
 template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * I4_TEAM_WARPS * 32, 1) mat_mat_i4_many_kernel(const MatI4Args a) {
     before();
-    constexpr int T = I4_TEAM_TILES, WSLOT = i4_slot<S, GROUP, 2>(), GS = 128 / GROUP, SB = 16 * (int)sizeof(S), GC = GROUP / 32;
+    constexpr int T = I4_TEAM_TILES, WSLOT = i4_slot(sizeof(S), GROUP, 2), GS = 128 / GROUP, SB = 16 * (int)sizeof(S), GC = GROUP / 32;
     extern __shared__ __align__(16) uint8_t i4_smem[];
     __shared__ float s_scale[I4_MANY_ROWS];
     __shared__ int s_pair[I4_MANY_ROWS];      // the unit's rows of out, their scales, where their rows of a begin
     __shared__ int64_t s_from[I4_MANY_ROWS];
-    const int RING = a.ring, SLOT = i4_many_slot<S, GROUP>(a.most), most_nt = a.most / 8;
+    const int RING = a.ring, SLOT = i4_many_slot(sizeof(S), GROUP, a.most), most_nt = a.most / 8;
     const I4List l = i4_list(i4_smem + I4_TEAMS * RING * SLOT, a);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp / I4_TEAM_WARPS, member = warp % I4_TEAM_WARPS, g = lane >> 2, t = lane & 3;
     uint8_t* slots = i4_smem + team * RING * SLOT;
@@ -547,12 +541,14 @@ template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * I4
                 for (int j = 0; j < N; j++)
                     if (j < nt) reinterpret_cast<float4*>(slots)[((member * 2 + r) * most_nt + j) * 32 + lane] = make_float4(acc[r][j][0], acc[r][j][1], acc[r][j][2], acc[r][j][3]);
         };
-        if (nt <= 2) products(std::integral_constant<int, 2>());
-        else if (nt <= 3) products(std::integral_constant<int, 3>());
-        else if (nt <= 4) products(std::integral_constant<int, 4>());
-        else if (nt <= 5) products(std::integral_constant<int, 5>());
-        else if (nt <= 6) products(std::integral_constant<int, 6>());
-        else products(std::integral_constant<int, 8>());
+        switch (i4_many_blocks(nt)) {
+            case 2: products(std::integral_constant<int, 2>()); break;
+            case 3: products(std::integral_constant<int, 3>()); break;
+            case 4: products(std::integral_constant<int, 4>()); break;
+            case 5: products(std::integral_constant<int, 5>()); break;
+            case 6: products(std::integral_constant<int, 6>()); break;
+            default: products(std::integral_constant<int, 8>());
+        }
         __syncwarp();
         if (a.split > 1) cluster_sync();
         else __syncthreads();
@@ -600,17 +596,15 @@ template <int CHUNK, int R, int WARPS, int PER_SM, typename F> cudaError_t mat_m
 }
 template <typename S, int GROUP, int NT> cudaError_t mat_mat_i4_few(const MatI4Args& a, int sms, cudaStream_t st) {
     static SmemAllowed allowed;
-    constexpr size_t base = i4_few_warps<NT>() * (I4_RING * i4_slot<S, GROUP, 4>() + 2 * NT * 512);
+    constexpr size_t base = i4_few_warps<NT>() * (I4_RING * i4_slot(sizeof(S), GROUP, 4) + 2 * NT * 512);
     return mat_mat_i4_launch<8 * NT, 1, i4_few_warps<NT>(), 2>(a, mat_mat_i4_few_kernel<S, GROUP, NT>, allowed, base, base + i4_list_bytes(1024, I4_PAIRS), sms, st);
 }
 template <typename S, int GROUP> cudaError_t mat_mat_i4_many(MatI4Args a, int sms, cudaStream_t st) {
     static SmemAllowed allowed;
-    constexpr int most = 226 * 1024;      // (and half a kilobyte of the kernel's own)
-    const int lists = a.experts ? (int)i4_list_bytes(a.n_experts, std::min<int>(a.rows, I4_PAIRS)) : 0;
-    a.most = std::min((a.rows + 7) / 8 * 8, (int)I4_MANY_ROWS);
-    const int ring = I4_TEAMS * i4_many_slot<S, GROUP>(a.most);
-    a.ring = std::min((int)I4_MANY_RING, (most - lists) / ring);      // (two at least: 144 KiB and the longest lists' 16)
-    return mat_mat_i4_launch<I4_MANY_ROWS, I4_TEAM_TILES, I4_TEAMS * I4_TEAM_WARPS, 1>(a, mat_mat_i4_many_kernel<S, GROUP>, allowed, a.ring * ring, most, sms, st);
+    const I4ManyPlan p = i4_many_plan(sizeof(S), GROUP, a.rows, a.n_experts);
+    a.most = p.most;
+    a.ring = p.ring;
+    return mat_mat_i4_launch<I4_MANY_ROWS, I4_TEAM_TILES, I4_TEAMS * I4_TEAM_WARPS, 1>(a, mat_mat_i4_many_kernel<S, GROUP>, allowed, p.smem, I4_MANY_MOST, sms, st);
 }
 template <typename S, int GROUP> cudaError_t mat_mat_i4(const MatI4Args& a, cudaStream_t st) {
     int sms = 0;

@@ -1,0 +1,57 @@
+"""Operators on device tensors for feed-forwards with routed experts and 4-bit weights where their kernels' places end: rings that go round, rows that fill no block of columns, magnitudes at the ends of f32."""
+import pytest
+import torch
+
+import device_experts_ref as R
+from test_gpu_device_experts import bytes_of, four_bits, normal
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def D(b200):
+    from llama_gguf_b200 import device_ops
+
+    return device_ops
+
+
+def product64(a, s, values, scales, experts=None):
+    """device_experts_ref.product's result and bound, in matrix products of 64 bits on the device (values [experts, n, k], a row of a for each pair)."""
+    groups = scales.shape[-1]
+    flat = torch.zeros(len(a), dtype=torch.int64) if experts is None else experts.flatten().long()
+    y, off = (torch.zeros(len(flat), values.shape[1], dtype=torch.float64, device="cuda") for _ in range(2))
+    for e in flat.unique().tolist():
+        rows = (flat == e).nonzero()[:, 0].cuda()
+        w, d = values[e].cuda().unflatten(1, (groups, -1)).double(), scales[e].cuda().double()
+        x = a[rows].unflatten(1, (groups, -1)).double()
+        for g in range(groups):
+            term = (x[:, g] @ w[:, g].T) * d[:, g] * s[rows].double()[:, None]      # (the product: integers below 2^24, exact)
+            y[rows] += term
+            off[rows] += term.abs() * (groups + 10) * 2.0**-24
+    return y, off
+
+
+def check_product(D, rows, k, n, group, scale=torch.float16, experts=None, n_experts=1):
+    values = four_bits(k + n, n_experts, n, k)
+    scales = (0.01 * normal(2, n_experts, n, k // group)).to(scale)
+    w, ws = (v.cuda() for v in D.i4_weights(values.cuda(), scales.cuda()))
+    a, s = bytes_of(rows, rows, k), (0.01 + torch.rand(rows, generator=torch.Generator().manual_seed(1))).cuda()
+    y = D.mat_mat_i4(a, s, w if experts is not None else w[0], ws if experts is not None else ws[0], n=n, experts=None if experts is None else experts.cuda(), dtype=torch.float32)
+    want, off = product64(a, s, values, scales, experts)
+    assert y.shape == want.shape and ((y.double() - want).abs() <= off + 2.0**-24 * (want.abs() + off)).all()
+
+
+@pytest.mark.parametrize("scale", TYPES)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows", [49, 50, 55, 56, 57])
+def test_product_of_rows_that_fill_seven_blocks_of_columns(D, scale, group, rows):
+    """Eight blocks are computed for them, over more steps than a ring has."""
+    check_product(D, rows, 14336, 200, group, scale)
+
+
+@pytest.mark.parametrize("rows,one", [(50, 50), (56, 56), (60, 52), (114, 114)])
+def test_product_of_an_expert_that_has_seven_blocks_of_rows(D, rows, one):
+    experts = torch.zeros(rows, 1, dtype=torch.int32)
+    experts[one:] = 1
+    check_product(D, rows, 14336, 300, 64, experts=experts, n_experts=2)
