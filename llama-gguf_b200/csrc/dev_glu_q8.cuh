@@ -75,19 +75,26 @@ template <typename T> __global__ void __launch_bounds__(1024) glu_q8_any_kernel(
 }
 
 // y in f32.  With z = g (SiLU) or its tanh form's argument (GELU), 1 / (1 + exp(-z)) by ex2.approx (2^-22 off) and rcp.approx (2^-23); the exponential's argument is off by up to 1.5 2^-24 of itself (GELU: 2^-21.7), which counts
-// where z is negative.  With the products' roundings, y and y times rcp.approx of (maximum / 127) are off by less than 2^-19 + |z| 2^-21 of themselves.  Where z <= -16 y is made in 64 bits.
+// where z is negative.  With the products' roundings, y and y times rcp.approx of (maximum / 127) are off by less than 2^-19 + |z| 2^-21 of themselves (the roundings alone by half of that).  Where z <= -16 y is made
+// in 64 bits.  The gate is multiplied with last: it may be as small as 2^-149, where half of it has too few bits and a large up brings it back.  An up is that small in rows that count (from 2^-119 on) too, but then what
+// r * up loses, 2^-150, is small beside y: for r < 1 the gate is below 17, and a number that is not 0 is of a y from 2^-119 / 254 on, so that 17 * 2^-150 is less than 2^-18 of it; in rows from 2^-112 on less than 2^-25.
 constexpr float kGluOff = 1.9073486328125e-6f, kGluOffZ = 4.76837158203125e-7f, kGluOffMost = 1.1444091796875e-5f;      // 2^-19, 2^-21, both for z = -16 and a half more
+constexpr float kGluOffSmall = 3.814697265625e-6f;      // 2^-18
 template <int ACT> __device__ __forceinline__ float glu_z(float g) { return ACT == GLU_GELU ? 1.5957691216057308f * fmaf(0.044715f * g * g, g, g) : g; }
 template <int ACT> __device__ __forceinline__ float glu_near(float g, float u) {
     if constexpr (ACT == GLU_RELU) return (g > 0 ? g : g == g ? 0.0f : g) * u;
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(glu_z<ACT>(g) * -1.4426950408889634f));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-    return g * r * u;
+    return g * (r * u);
 }
 // the gate down to which y is made in f32 (z = -16, and -15.6)
 template <int ACT> __device__ __forceinline__ constexpr float glu_least() { return ACT == GLU_GELU ? -4.8f : -16.0f; }
 template <int ACT> __device__ __forceinline__ float glu_y(float g, float u) { return ACT != GLU_RELU && g <= glu_least<ACT>() ? (float)glu_exact(g, u, ACT) : glu_near<ACT>(g, u); }
+// what a number of a row may be off by, of itself: `low` the least of its gates, `exact` the row's largest value
+template <int ACT> __device__ __forceinline__ float glu_off(float low, double exact) {
+    return kGluOff - fmaxf(glu_z<ACT>(fmaxf(low, glu_least<ACT>())), -16.0f) * kGluOffZ + (exact < 0x1p-112 ? kGluOffSmall : 0.0f);
+}
 // the smallest of `least` and a word's elements (NaN does not count)
 template <typename T> __device__ __forceinline__ float word_min(const uint4& w, float least) {
     if constexpr (sizeof(T) == 4) {
@@ -181,7 +188,7 @@ template <typename T, int V, int ACT> __global__ void __launch_bounds__(1024) gl
         float inv;
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"((float)exact * (1.0f / 127.0f)));      // (from 2^-126 to 2^121: neither side leaves the range)
         // rounded from both ends of what y may be: where the two are one number it is that
-        const float off = kGluOff - fmaxf(glu_z<ACT>(fmaxf(low, glu_least<ACT>())), -16.0f) * kGluOffZ, up = inv + inv * off, down = inv - inv * off;
+        const float off = glu_off<ACT>(low, exact), up = inv + inv * off, down = inv - inv * off;
 #pragma unroll
         for (int v = 0; v < V; v++) {
             const int i = v * step + tid;
@@ -262,7 +269,7 @@ template <typename T, int V, int ACT> __global__ void __launch_bounds__(1024) gl
     const bool live = glu_live(exact);
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"((float)exact * (1.0f / 127.0f)));
-    const float off = kGluOff - fmaxf(glu_z<ACT>(fmaxf(low, glu_least<ACT>())), -16.0f) * kGluOffZ, up = inv + inv * off, down = inv - inv * off;
+    const float off = glu_off<ACT>(low, exact), up = inv + inv * off, down = inv - inv * off;
     int8_t* out = a.q + row * a.ldq;
     uint32_t close = 0;
 #pragma unroll

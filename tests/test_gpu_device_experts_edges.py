@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import device_experts_ref as R
-from test_gpu_device_experts import bytes_of, four_bits, normal
+from test_gpu_device_experts import bytes_of, check_glu, four_bits, normal
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -55,3 +55,28 @@ def test_product_of_an_expert_that_has_seven_blocks_of_rows(D, rows, one):
     experts = torch.zeros(rows, 1, dtype=torch.int32)
     experts[one:] = 1
     check_product(D, rows, 14336, 300, 64, experts=experts, n_experts=2)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("ff", [1024, 1023, 8200, 8199])
+def test_gated_unit_of_gates_below_the_normal_numbers(D, dtype, act, ff):
+    """Gates of some 2^-149 (bf16: 2^-133), whose halves have few bits, and ups that bring them back."""
+    g = torch.Generator().manual_seed(ff)
+    least = 2.0**-149 if dtype == torch.float32 else 2.0**-133
+    for most, up in ((1023, 2.0**60), (31, 2.0**100), (3, 2.0**40), (2**20 - 1, 2.0**50)):
+        most = most if dtype == torch.float32 else min(most, 127)
+        gate = torch.randint(1, most + 1, (16, ff), generator=g).float() * (torch.randint(0, 2, (16, ff), generator=g) * 2 - 1) * least
+        x = torch.cat([gate, up * torch.randn(16, ff, generator=g)], 1).to(dtype)
+        assert (x[:, :ff] != 0).all()
+        check_glu(D, x.cuda(), act)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("ff", [4096, 4095])
+def test_gated_unit_of_ups_below_the_normal_numbers(D, act, ff):
+    """Rows next to the least ones that count: ups of up to 2^-123 and gates up to 16, which make the ups' products' roundings larger."""
+    g = torch.Generator().manual_seed(ff)
+    for place, up in enumerate((2.0**-128, 2.0**-126, 2.0**-124, 2.0**-122)):
+        x = torch.cat([16 * (2 * torch.rand(64, ff, generator=g) - 0.5), up * torch.randn(64, ff, generator=g)], 1)
+        check_glu(D, x.cuda(), act)
