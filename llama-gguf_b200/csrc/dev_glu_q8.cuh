@@ -90,7 +90,11 @@ template <int ACT> __device__ __forceinline__ float glu_near(float g, float u) {
 }
 // the gate down to which y is made in f32 (z = -16, and -15.6)
 template <int ACT> __device__ __forceinline__ constexpr float glu_least() { return ACT == GLU_GELU ? -4.8f : -16.0f; }
-template <int ACT> __device__ __forceinline__ float glu_y(float g, float u) { return ACT != GLU_RELU && g <= glu_least<ACT>() ? (float)glu_exact(g, u, ACT) : glu_near<ACT>(g, u); }
+// ... and y made there may come out infinite where the exact one, next to the largest f32, does not: then it is made in 64 bits too.  (RELU's product is rounded once, as the exact one's.)
+template <int ACT> __device__ __forceinline__ float glu_y(float g, float u) {
+    const float y = glu_near<ACT>(g, u);
+    return ACT != GLU_RELU && (g <= glu_least<ACT>() || !(fabsf(y) < INFINITY)) ? (float)glu_exact(g, u, ACT) : y;
+}
 // what a number of a row may be off by, of itself: `low` the least of its gates, `exact` the row's largest value
 template <int ACT> __device__ __forceinline__ float glu_off(float low, double exact) {
     return kGluOff - fmaxf(glu_z<ACT>(fmaxf(low, glu_least<ACT>())), -16.0f) * kGluOffZ + (exact < 0x1p-112 ? kGluOffSmall : 0.0f);
@@ -152,7 +156,31 @@ template <typename T, int V, int ACT> __global__ void __launch_bounds__(1024) gl
             for (int e = 0; e < E; e++) most_of[v] = max_nan(most_of[v], fabsf(y[v][e]));
             top = max_nan(top, most_of[v]);
         }
-        const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+        uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+        if (ACT != GLU_RELU && most >= kInfBits) {
+            uint32_t far = 0;
+#pragma unroll
+            for (int v = 0; v < V; v++)
+#pragma unroll
+                for (int e = 0; e < E; e++) far |= fabsf(y[v][e]) < INFINITY ? 0u : 1u << (v * E + e);
+            for (; far; far &= far - 1) {
+                const int o = __ffs(far) - 1;
+                const float x = (float)glu_exact(to_f(reinterpret_cast<const T*>(g + o / E * step)[o % E]), to_f(reinterpret_cast<const T*>(u + o / E * step)[o % E]), ACT);
+#pragma unroll
+                for (int v = 0; v < V; v++)
+#pragma unroll
+                    for (int e = 0; e < E; e++) y[v][e] = v * E + e == o ? x : y[v][e];
+            }
+            top = 0;
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                most_of[v] = 0;
+#pragma unroll
+                for (int e = 0; e < E; e++) most_of[v] = max_nan(most_of[v], fabsf(y[v][e]));
+                top = max_nan(top, most_of[v]);
+            }
+            most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+        }
         const float least = __uint_as_float(most) * (1.0f - 2 * kGluOffMost);
         double mine = most < kInfBits ? 0.0 : INFINITY;
         if (most < kInfBits && top >= least) {
@@ -221,7 +249,7 @@ template <typename T, int V, int ACT> __global__ void __launch_bounds__(1024) gl
     const T *gate = reinterpret_cast<const T*>(a.x) + row * a.ldx, *up_ = gate + a.ff;
     const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x >> 5;
     float y[V], top = 0, low = 0;
-    uint32_t far = 0;      // where the gate is too far down for f32
+    uint32_t far = 0;      // where the gate is too far down for f32 (and then what came out infinite)
     {
         T g[V], u[V];
 #pragma unroll
@@ -239,15 +267,22 @@ template <typename T, int V, int ACT> __global__ void __launch_bounds__(1024) gl
             if (ACT != GLU_RELU && there && x <= glu_least<ACT>()) far |= 1u << v;
         }
     }
-    for (; far; far &= far - 1) {
-        const int k = __ffs(far) - 1, i = k * blockDim.x + tid;
-        const float x = (float)glu_exact(to_f(gate[i]), to_f(up_[i]), ACT);
+    uint32_t most;
+    for (bool again = ACT != GLU_RELU;; again = false) {
+        for (; far; far &= far - 1) {
+            const int k = __ffs(far) - 1, i = k * blockDim.x + tid;
+            const float x = (float)glu_exact(to_f(gate[i]), to_f(up_[i]), ACT);
 #pragma unroll
-        for (int v = 0; v < V; v++) y[v] = v == k ? x : y[v];
+            for (int v = 0; v < V; v++) y[v] = v == k ? x : y[v];
+        }
+        top = 0;
+#pragma unroll
+        for (int v = 0; v < V; v++) top = max_nan(top, fabsf(y[v]));
+        most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+        if (!again || most < kInfBits) break;
+#pragma unroll
+        for (int v = 0; v < V; v++) far |= fabsf(y[v]) < INFINITY ? 0u : 1u << v;      // (behind the row's last element y is 0)
     }
-#pragma unroll
-    for (int v = 0; v < V; v++) top = max_nan(top, fabsf(y[v]));
-    const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
     const float least = __uint_as_float(most) * (1.0f - 2 * kGluOffMost);
     double mine = most < kInfBits ? 0.0 : INFINITY;
     if (most < kInfBits && top >= least) {

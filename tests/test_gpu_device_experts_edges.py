@@ -80,3 +80,33 @@ def test_gated_unit_of_ups_below_the_normal_numbers(D, act, ff):
     for place, up in enumerate((2.0**-128, 2.0**-126, 2.0**-124, 2.0**-122)):
         x = torch.cat([16 * (2 * torch.rand(64, ff, generator=g) - 0.5), up * torch.randn(64, ff, generator=g)], 1)
         check_glu(D, x.cuda(), act)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("ff", [256, 257, 20000])
+def test_gated_unit_next_to_the_largest_numbers(D, act, ff):
+    """Largest values a step below 2^128 - 2^103, where f32 becomes infinite, and a step above: the exact one decides."""
+    rows = 300
+    g = torch.Generator().manual_seed(ff)
+    x = torch.randn(rows, 2 * ff, generator=g)
+    at = torch.randint(0, ff, (rows,), generator=g)
+    every = torch.arange(rows)
+    x[every, at] = 2 + 18 * torch.rand(rows, generator=g)
+    x[every, ff + at] = 1.0
+    per = R.glu(x, act)[every, at]      # act(gate)
+    border = 2.0**128 - 2.0**103
+    up = (border / per).float()
+    y = per * up.double()
+    assert torch.isfinite(up).all()
+    above = torch.where(y >= border, up, torch.nextafter(up, torch.tensor(torch.inf)))
+    below = torch.nextafter(above, torch.tensor(0.0))
+    for u, live in ((below, True), (above, False)):
+        x[every, ff + at] = u
+        away = ((per * u.double() / border - 1).abs() > 2.0**-40) & torch.isfinite(u)      # (exact ones that 64 bits tell from the border)
+        assert away.sum() > 250
+        part = x[away].cuda()
+        if live:
+            check_glu(D, part, act)
+        else:
+            q, s = D.glu_q8(part, act)
+            assert (q == 0).all() and torch.isnan(s).all()
