@@ -203,9 +203,10 @@ template <typename T, int V> __global__ void __launch_bounds__(ROUTE_WARPS * 32,
             if (lane == who) value = 0;
         }
         const uint32_t next = __reduce_max_sync(0xffffffffu, value);
-        if (scores && next && least) {      // (a sum of two: 2^-20, and a rounding)
-            const float lo = route_value32(next), hi = route_value32(least);
-            close = !(hi - lo > 0x1p-18f + 0x1p-21f * fabsf(hi));
+        if (scores) {      // (a sum of two: 2^-20, and its rounding and theirs, which are those of the largest where they cancel)
+            const float most_of = fmaxf(first ? fabsf(route_value32(first)) : 0.0f, second ? fabsf(route_value32(second)) : 0.0f), largest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_of)));
+            if (next && least) close = !(route_value32(least) - route_value32(next) > 0x1p-18f + 0x1p-21f * largest);
+            close |= largest > 1e38f;      // (a sum may leave the range)
         }
     }
     // keys, and by how much (in their 22 bits) a choice must be ahead of what follows it

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import device_experts_ref as R
-from test_gpu_device_experts import bytes_of, check_glu, four_bits, normal
+from test_gpu_device_experts import bytes_of, check_glu, check_route, four_bits, normal
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -110,3 +110,16 @@ def test_gated_unit_next_to_the_largest_numbers(D, act, ff):
         else:
             q, s = D.glu_q8(part, act)
             assert (q == 0).all() and torch.isnan(s).all()
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("size", [64.0, 1000.0, 8000.0, 3e38])
+@pytest.mark.parametrize("n,groups,top_groups", [(8, 4, 2), (64, 32, 8), (64, 16, 4), (256, 8, 4)])
+def test_routing_by_groups_with_corrections_that_cancel(D, score, size, n, groups, top_groups):
+    """A group's two best scores of opposite signs: their sum is small, the roundings of f32 are those of the scores."""
+    rows = 400 if size < 1e30 else 20
+    z = normal(n, rows, n) * (min(size, 1e4) * 2.0**-23 * 2.0 ** (torch.arange(rows) % 8))[:, None]      # (scores some of the corrections' roundings apart)
+    place = torch.arange(n) % (n // groups)
+    for first, second in ((size, -size), (-size, -size), (size, size)):
+        c = torch.where(place == 0, first, torch.where(place == 1, second, -size))
+        check_route(D, z, min(6, n // groups * top_groups), score=score, correction=c, groups=groups, top_groups=top_groups)
