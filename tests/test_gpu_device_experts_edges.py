@@ -21,7 +21,7 @@ def product64(a, s, values, scales, experts=None):
     groups = scales.shape[-1]
     flat = torch.zeros(len(a), dtype=torch.int64) if experts is None else experts.flatten().long()
     y, off = (torch.zeros(len(flat), values.shape[1], dtype=torch.float64, device="cuda") for _ in range(2))
-    for e in flat.unique().tolist():
+    for e in flat[flat >= 0].unique().tolist():      # (expert -1: zeros)
         rows = (flat == e).nonzero()[:, 0].cuda()
         w, d = values[e].cuda().unflatten(1, (groups, -1)).double(), scales[e].cuda().double()
         x = a[rows].unflatten(1, (groups, -1)).double()
@@ -123,3 +123,39 @@ def test_routing_by_groups_with_corrections_that_cancel(D, score, size, n, group
     for first, second in ((size, -size), (-size, -size), (size, size)):
         c = torch.where(place == 0, first, torch.where(place == 1, second, -size))
         check_route(D, z, min(6, n // groups * top_groups), score=score, correction=c, groups=groups, top_groups=top_groups)
+
+
+# (rows, k, n, group): by the kernels' own arithmetic on 148 SMs
+@pytest.mark.parametrize("rows,k,n,group,scale", [
+    (40, 28672, 200, 64, torch.float16),       # clusters of eight, seven steps a team, rings of four
+    (64, 28672, 140, 32, torch.float32),       # ... rings of three, two units
+    (20, 28672, 100, 128, torch.bfloat16),
+    (33, 14336, 4096, 64, torch.bfloat16),     # clusters of four, seven steps
+    (24, 8192, 8192, 32, torch.float16),       # clusters of two, eight steps
+    (33, 4096, 9700, 128, torch.float32),      # no clusters, eight steps a team
+    (56, 6144, 9600, 64, torch.float16),       # twelve steps
+    (40, 2048, 20000, 32, torch.float16),      # two units a block, one after the other
+    (130, 2048, 9700, 64, torch.bfloat16),     # ... of three chunks of rows, the last of two
+    (185, 1056, 9608, 32, torch.float32),      # ... the last of 57
+])
+def test_product_of_more_rows_whose_rings_go_round(D, rows, k, n, group, scale):
+    check_product(D, rows, k, n, group, scale)
+
+
+@pytest.mark.parametrize("rows,k,n,group,scale", [
+    (1, 4096, 12000, 128, torch.float16), (1, 14336, 4800, 32, torch.float32), (2, 14336, 4801, 32, torch.float16), (4, 8192, 9000, 64, torch.bfloat16),      # units that begin within a warp's steps
+    (9, 14336, 4800, 32, torch.float16), (16, 14336, 4752, 64, torch.float32), (13, 4096, 12000, 128, torch.bfloat16), (6, 8192, 5000, 32, torch.float32)])
+def test_product_of_few_rows_whose_rings_go_round(D, rows, k, n, group, scale):
+    check_product(D, rows, k, n, group, scale)
+
+
+@pytest.mark.parametrize("tokens,top,experts,k,n,group", [(100, 2, 4, 1056, 6000, 32), (300, 1, 5, 2048, 3000, 128), (64, 1, 2, 14336, 500, 64), (16, 2, 8, 4096, 2000, 32), (1, 2, 8, 4096, 6000, 32), (40, 4, 16, 2048, 1500, 64)])
+@pytest.mark.parametrize("even", [True, False])
+def test_product_of_experts_whose_rings_go_round(D, tokens, top, experts, k, n, group, even):
+    """Units of several experts one after the other; with most tokens at one expert, units of other sizes than the average's."""
+    g = torch.Generator().manual_seed(tokens)
+    e = torch.stack([torch.randperm(experts, generator=g)[:top] for _ in range(tokens)]).int()
+    if not even:
+        e[torch.rand(tokens, top, generator=g) < 0.8] = experts - 1
+        e[torch.rand(tokens, top, generator=g) < 0.1] = -1
+    check_product(D, tokens * top, k, n, group, experts=e, n_experts=experts)
