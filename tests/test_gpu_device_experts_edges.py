@@ -159,3 +159,31 @@ def test_product_of_experts_whose_rings_go_round(D, tokens, top, experts, k, n, 
         e[torch.rand(tokens, top, generator=g) < 0.8] = experts - 1
         e[torch.rand(tokens, top, generator=g) < 0.1] = -1
     check_product(D, tokens * top, k, n, group, experts=e, n_experts=experts)
+
+
+def test_products_in_clusters_captured_and_replayed_on_two_streams(D):
+    """Clusters of eight and of four, and a product of few rows: graphs replayed at once on two streams with new inputs, each as by itself."""
+    jobs = []
+    for rows, k, n, group in ((50, 14336, 300, 64), (33, 14336, 4096, 32), (7, 4096, 5000, 128)):
+        w, ws = D.quantise_i4(normal(rows, n, k).cuda(), group)
+        a, s, out = bytes_of(rows, rows, k), torch.ones(rows).cuda(), torch.empty(rows, n).cuda()
+        D.mat_mat_i4(a, s, w, ws, n=n, out=out)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(4):
+                D.mat_mat_i4(a, s, w, ws, n=n, out=out)
+        jobs.append((a, s, w, ws, n, out, g))
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for turn in range(3):
+        want = []
+        for a, s, w, ws, n, out, _ in jobs:
+            a.copy_(bytes_of(100 + turn, *a.shape))
+            want.append(D.mat_mat_i4(a, s, w, ws, n=n, dtype=torch.float32))
+            out.fill_(0)
+        torch.cuda.synchronize()
+        for job, st in zip(jobs, streams):
+            with torch.cuda.stream(st):
+                job[-1].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(job[5], v) for job, v in zip(jobs, want))
