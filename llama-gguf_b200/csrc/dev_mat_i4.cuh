@@ -541,14 +541,14 @@ template <typename S, int GROUP> __global__ void __launch_bounds__(I4_TEAMS * I4
                 for (int j = 0; j < N; j++)
                     if (j < nt) reinterpret_cast<float4*>(slots)[((member * 2 + r) * most_nt + j) * 32 + lane] = make_float4(acc[r][j][0], acc[r][j][1], acc[r][j][2], acc[r][j][3]);
         };
-        switch (i4_many_blocks(nt)) {
-            case 2: products(std::integral_constant<int, 2>()); break;
-            case 3: products(std::integral_constant<int, 3>()); break;
-            case 4: products(std::integral_constant<int, 4>()); break;
-            case 5: products(std::integral_constant<int, 5>()); break;
-            case 6: products(std::integral_constant<int, 6>()); break;
-            default: products(std::integral_constant<int, 8>());
-        }
+        auto columns = [](auto blocks) { return std::integral_constant<int, i4_many_blocks(decltype(blocks)::value)>(); };
+        static_assert(i4_many_blocks(1) == i4_many_blocks(2) && i4_many_blocks(7) == i4_many_blocks(8), "one case each below");
+        if (nt <= 2) products(columns(std::integral_constant<int, 2>()));
+        else if (nt <= 3) products(columns(std::integral_constant<int, 3>()));
+        else if (nt <= 4) products(columns(std::integral_constant<int, 4>()));
+        else if (nt <= 5) products(columns(std::integral_constant<int, 5>()));
+        else if (nt <= 6) products(columns(std::integral_constant<int, 6>()));
+        else products(columns(std::integral_constant<int, 8>()));
         __syncwarp();
         if (a.split > 1) cluster_sync();
         else __syncthreads();
