@@ -187,3 +187,13 @@ def test_products_in_clusters_captured_and_replayed_on_two_streams(D):
                 job[-1].replay()
         torch.cuda.synchronize()
         assert all(torch.equal(job[5], v) for job, v in zip(jobs, want))
+
+
+@pytest.mark.parametrize("rows", [1, 8, 40])
+def test_product_of_the_largest_scales(D, rows):
+    """Sums over the groups up to 2^124 (they are kept at sixteen times their value)."""
+    a, values, scales = torch.full((rows, 256), 127, dtype=torch.int8).cuda(), torch.full((1, 20, 256), 7, dtype=torch.int8), torch.full((1, 20, 8), 2.0**106)      # 8 * 32 * 127 * 7 * 2^106: 2^123.8
+    w, ws = (v.cuda() for v in D.i4_weights(values[0], scales[0]))
+    s = torch.full((rows,), 2.0**-100).cuda()
+    y = D.mat_mat_i4(a, s, w, ws, n=20, dtype=torch.float32)
+    assert torch.equal(y.double(), torch.full((rows, 20), 8 * 32 * 127 * 7 * 2.0**6, dtype=torch.float64).cuda())      # (few bits: exact in any order)
