@@ -625,8 +625,9 @@ B200_API int b200_dev_route_experts(const b200_route* a);
  * With `experts` ([tokens][top] int32) there are n_experts such matrices one after the other (and [n_experts][n] of bias), out has a row for each pair (token, place) and is
  * [tokens * top][n]; a has a row per token, or per pair where rows_per_pair is set.  Pairs of expert -1 get zeros; other numbers outside 0 .. n_experts - 1 too, BAD_EXPERT.
  * a starts on 16 bytes with rows a multiple of 16 bytes apart; what lies between k and the next row is not used.  w and the scales start on 16 bytes.  With experts n <= 2^23,
- * n_experts <= 1024, top <= 32.  The same call gives the same bits; another number of rows may add the groups up in another order.  Meant for few rows: the weights' bytes
- * are read once per 64 rows (of an expert). */
+ * n_experts <= 1024, top <= 32.  The same call gives the same bits.  The order in which the groups are added up goes by the sizes and, with experts, by how many pairs each of them has: another
+ * number of rows, or another token's choice, may change a result's last bits.  The sum over the groups is kept at sixteen times its value: from 2^124 on it may come out infinite.  Meant for few
+ * rows: weights are read once for up to 16 rows, else once per 64 of them; with experts once per 8, 16 or 64 pairs of an expert (by the average expert's number), and anew for every 2048 pairs. */
 typedef struct b200_i4_product {
     int32_t device;
     uint32_t out_type, scale_type;
@@ -651,7 +652,7 @@ B200_API int b200_dev_glu_q8(int device, void* stream, uint32_t type, int act, c
 /* A block's output onto the residual stream, and the next norm with its result in 8 bits:
  *   m = y (mix NULL), or sum over j < top of mix[row][j] * y[row * top + j] (f32, in that order);  p = m / sqrt(mean(m^2) + eps) * post_weight, or m where that is NULL;
  *   r = residual + (p * gate) * scale, rounded to the type, to `sum`;  q, scales = r / sqrt(mean(r^2) + eps) * weight as b200_dev_add_rms_norm_q8 makes them (weight NULL: neither).
- * Every product and sum is rounded to f32, means are taken in 64 bits.  gate: element (row, i) at row * gate_row + i * gate_col, so that one per row, one per channel or one for
+ * Every product and sum is rounded to f32; means, roots and reciprocals are taken in 64 bits and rounded to f32 once.  gate: element (row, i) at row * gate_row + i * gate_col, so that one per row, one per channel or one for
  * each may be given (NULL: none).  `sum` may be `residual` with the same row distance; other overlaps are not allowed.  mix: [rows][top], 1 <= top <= 32.  1 <= hidden <= 65536. */
 typedef struct b200_gated_norm {
     int32_t device;

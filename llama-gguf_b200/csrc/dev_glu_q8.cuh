@@ -3,7 +3,7 @@
 // y = act(g) * u; scale = max |y| / 127; q = round(y * 127 / max |y|), halves to even, all of it as if y were exact: it is made in f32, and again in 64 bits where that could decide otherwise (the
 // largest value of the row, and what lies next to the border between two numbers).  In 64 bits throughout 4096 x 14336 bf16 took 495 us.
 //
-// What bounds it: instructions and their latency (4096 x 14336 bf16 76 us by itself, 294 MB: 45 at the measured rate; relu, without the exponentials, 51; f32 rows of half as many, 264 MB, 49).  Steps: one block a row and a barrier on either side of
+// What bounds it: instructions and their latency (4096 x 14336 bf16 77 us by itself, 294 MB: 45 at the measured rate; relu, without the exponentials, 51, gelu 146; f32 rows of half as many, 264 MB, 50; rows of zeros 295, each of whose values may be the largest).  Steps: one block a row and a barrier on either side of
 // the largest value's 64 bits 99 us; every warp making its own largest one in 64 bits, which leaves one barrier, and rounding from both ends of what y may be (two FMA and an exclusive or for a product, two sums, a difference and
 // a comparison) 76.
 #pragma once
@@ -339,7 +339,7 @@ template <typename T, int V> cudaError_t glu_q8_words(const GluQ8Args& a, int th
 template <typename T> cudaError_t glu_q8(const GluQ8Args& a, cudaStream_t st) {
     constexpr int E = 16 / (int)sizeof(T);
     const bool words = a.ff % E == 0 && a.ff / E <= 4096 && !(reinterpret_cast<uintptr_t>(a.x) & 15) && a.ldx % E == 0 && !(reinterpret_cast<uintptr_t>(a.q) % E) && a.ldq % E == 0;
-    // (2000 x 16383 bf16: 102 us, 215 in 64 bits throughout; 16384 wide rows, as words, 41 for as many)
+    // (2000 x 16383 bf16: 104 us, 215 in 64 bits throughout; 16384 wide rows, as words, 41 for as many)
     if (!words) return a.ff <= 1024 ? glu_q8_row<T, 4>(a, st) : a.ff <= 16384 ? glu_q8_row<T, 16>(a, st) : launch(glu_q8_any_kernel<T>, dim3((unsigned)a.rows), 1024, 0, 1, st, a);
     int sms = 0;
     const cudaError_t e = sm_count(&sms);

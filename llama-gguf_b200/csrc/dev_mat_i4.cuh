@@ -1,7 +1,7 @@
 // dev_mat_i4.cuh — product of rows in 8 bits with 4-bit weights that have a scale per group of channels, of one matrix or of each token's experts (b200_dev_mat_mat_i4).
 //
 // out[p][n] = a_scales[r] * sum_g ws[e][n][g] * (sum over the channels k of group g of a[r][k] * w[e][n][k]) + bias[e][n], r the row of a and e the expert of output row p.
-// The inner sums are integers and exact; the outer one is f32, in an order that only the sizes decide.
+// The inner sums are integers and exact; the outer one is f32, in an order that the sizes decide and, with experts, how many pairs each expert has (columns of a unit, and where warps and blocks cut a unit's channels).
 //
 // A tile of weights is 16 rows x 64 channels in 512 bytes, placed so that the 16 bytes of a lane are the operands of two mma.m16n8k32 (s8, s32 sums): a word has four channels in the low
 // halves of its bytes and the next four in the high halves; (word << 4) & 0xf0f0f0f0 and word & 0xf0f0f0f0 are those values times sixteen as signed bytes, three instructions for eight weights.  Eight rows of a are
@@ -14,8 +14,8 @@
 //   more rows (up to 64 at a time): rows of a cost as much as weights.  A block has eight tiles; its teams of four warps have a part of the channels each, whose rows of a serve all eight.  With few units the
 //   blocks of a cluster share the channels of one.
 // What bounds it.  Few rows: the weights' bytes from some 30 MB on (one token through two of eight experts, 28672 x 4096 in groups of 32 with f16 scales: 25.2 us for 132 MB, 5.2 TB/s, of which 6.5 us are launch, list, first bytes and the last
-// sums; 4096 to 8192 channels of one matrix add 66 MB in 10 us), below that the launch and a chain of loads (6144 x 4096: 7.3 us; a call of nothing 3.4).  Sixteen tokens' units of up to eight rows: issue slots, 50 us for 263 MB.  More rows: issue
-// slots and the latency of a team's step (33 rows of 4096 x 14336 20.3 us, of 8192 x 28672 56, 2.2 TB/s; the integer pipe is active 24 %).  Measured on the way: loads to registers, two steps ahead, 55 us (token, two experts);
+// sums; 4096 to 8192 channels of one matrix add 66 MB in 10 us), below that the launch and a chain of loads (6144 x 4096: 7.0 us; a call of nothing 3.4).  Sixteen tokens' units of up to eight rows: waits for rows of a
+// and issue slots (55 %), 50 to 58 us for 263 MB, by what the tokens choose.  More rows: the latency of a team's step, with issue slots at 44 % (33 rows of 4096 x 14336 20.4 us, of 8192 x 28672 56, 2.2 TB/s; the integer pipe is active 24 %).  Measured on the way: loads to registers, two steps ahead, 55 us (token, two experts);
 // the ring, 64-bit arithmetic in every unit, 47; shared steps 38; several groups in the columns 26.  More rows: rows of a from L1 51 us (33 rows); a ring of four tiles a warp 33; sixteen warps on one step 25; teams of eight
 // warps with one tile 24, of four with two 20; a warp that copies for all by bulk copies (of 128 bytes for a row) 73.  Copies with nothing computed per step but an addition took 100 instructions a step off.
 #pragma once

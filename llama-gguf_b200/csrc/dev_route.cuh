@@ -7,7 +7,7 @@
 // largest), then 1023 - e, so that one redux.sync gives a choice and its expert, the lower one among equals; each lane's keys are sorted once and the chosen one's lane moves up.  Scores are made in f32 (off by less
 // than 2^-21).  Where two that follow one another are closer than all that may be off, the token (some of a hundred) is chosen for again with 64-bit scores and keys, which took 34 us for 8192 tokens of 256
 // experts in 8 groups where all did.
-// What bounds it: instructions, some 1500 a token with groups (8192 tokens of 256 experts, sigmoid with a correction, 8 of them in 4 of 8 groups: 21.8 us; without groups 15.3, softmax by logits 9.9; the logits' bytes 0.6).  One token: 2 us by itself.
+// What bounds it: instructions, some 1560 a token with groups (8192 tokens of 256 experts, sigmoid with a correction, 8 of them in 4 of 8 groups: 22.6 us; without groups 15.3, softmax by logits 9.9; the logits' bytes 0.6).  One token: 2 us by itself.
 #pragma once
 #include <algorithm>
 

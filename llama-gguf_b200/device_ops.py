@@ -209,8 +209,9 @@ def mat_mat_i4(a, a_scales, w, w_scales, n=None, experts=None, bias=None, dtype=
 
     w, w_scales: i4_weights, quantise_i4 or i4_from_q4_0 make them; n None: all rows of their tiles.  experts int32 [tokens, top] (route_experts): w, w_scales and bias have a leading dimension of
     experts, and the result [tokens * top, n] has a row for each of a token's experts; a has a row per token, or [tokens * top] rows, one for each.  Pairs of expert -1 get zeros, other numbers that
-    are no expert too (and set STATUS_BAD_EXPERT).  The sums of a group are exact; those over the groups are f32, in an order that the number of rows may change.  a starts on 16 bytes with rows a multiple of 16
-    bytes apart (padded_rows).  For few rows: the weights' bytes are what it costs, once for every 64 rows of a matrix."""
+    are no expert too (and set STATUS_BAD_EXPERT).  The sums of a group are exact; those over the groups are f32 (below 2^124), in an order that the number of rows may change and, with experts, what other
+    tokens choose.  a starts on 16 bytes with rows a multiple of 16 bytes apart (padded_rows).  For few rows: the weights' bytes are what it costs, once for up to 16 rows, else for every 64 (of an expert: for
+    every 8, 16 or 64 pairs, by the average expert's number, and anew for every 2048 pairs of the call)."""
     return _ops().mat_mat_i4(a, a_scales, w, w_scales, n, experts, bias, dtype, out, status)
 
 
